@@ -698,6 +698,131 @@ int rhip_bn_backward(const void *grad_y, const void *y, const void *x, int64_t n
                      float *grad_beta, int32_t dtype, void *workspace,
                      size_t workspace_bytes, hipStream_t stream);
 
+/* ------------------------------------------------------------- attention
+ *
+ * Attention over packed sequences, for transformer stages over the rows of
+ * several scenes (or texts): query rows [n_q, heads, dim], key and value rows
+ * [n_k, kv_heads, dim], sequence s = query rows q_offsets[s] .. q_offsets[s+1]
+ * against key rows k_offsets[s] .. k_offsets[s+1], of which the first
+ * k_lengths[s] are in use (all, when k_lengths is null: a cache passes its
+ * regions as offsets and its fill as lengths). Head h attends to key head
+ * h / (heads / kv_heads).
+ *
+ *   out_i = sum_j softmax_j(scale * q_i . k_j) v_j  over the keys j row i sees:
+ *   all keys in use, or with causal != 0 those with j <= i + (Lk - Lq), Lq and
+ *   Lk the sequence's rows and keys in use (the last row sees every key).
+ *
+ * A row that sees no key, and query rows behind the last sequence, get zeros.
+ * What lies in rows that a row does not see never reaches it, infinities and
+ * NaN included (forward; in the backward pass under a causal mask, a row of
+ * grad_out or q that is not finite may also reach the gradients of up to 31
+ * later keys).
+ *
+ * Offsets are int32 [n_seq + 1] on the device, the first 0 and none smaller
+ * than the one before, at most n_q (n_k); sums, maxima and the softmax's
+ * statistics are fp32. bf16: probabilities and score gradients are rounded
+ * to bf16 as operands of the second products. Results do not change from run
+ * to run. dim <= 128.
+ */
+typedef struct rhip_attn {
+  int64_t n_q, n_k;         /* query rows; key rows */
+  int64_t q_row, q_head;    /* strides in elements; the last axis is dense */
+  int64_t k_row, k_head;
+  int64_t v_row, v_head;
+  const int32_t *q_offsets; /* device */
+  const int32_t *k_offsets; /* device */
+  const int32_t *k_lengths; /* device [n_seq], or null */
+  int32_t n_seq;
+  int32_t heads, kv_heads, dim;
+  int32_t causal;
+  int32_t dtype; /* of q, k, v, out and the gradients */
+  float scale;
+} rhip_attn;
+
+/* Workspace bytes of rhip_attn_forward (backward = 0) or rhip_attn_backward. */
+int rhip_attn_workspace_bytes(const rhip_attn *attn, int32_t backward,
+                              size_t *bytes);
+
+/*
+ * out [n_q, heads, dim] (dense). lse [heads, n_q], the natural logarithm of
+ * each row's softmax denominator (-inf for a row that sees no key), is
+ * written when not null; the backward pass needs it.
+ */
+int rhip_attn_forward(const rhip_attn *attn, const void *q, const void *k,
+                      const void *v, void *out, float *lse, void *workspace,
+                      size_t workspace_bytes, hipStream_t stream);
+
+/*
+ * grad_q [n_q, heads, dim], grad_k and grad_v [n_k, kv_heads, dim] (dense,
+ * overwritten; key rows not in use get zeros) from out and lse of the
+ * forward pass; grad_out has its own strides. Gradients of a key head are
+ * summed over its query heads. grad_q may be null, and grad_k and grad_v both.
+ */
+int rhip_attn_backward(const rhip_attn *attn, const void *grad_out,
+                       int64_t grad_out_row, int64_t grad_out_head,
+                       const void *q, const void *k, const void *v,
+                       const void *out, const float *lse, void *grad_q,
+                       void *grad_k, void *grad_v, void *workspace,
+                       size_t workspace_bytes, hipStream_t stream);
+
+/* ------------------------------------------------------------ layer norm
+ *
+ * Layer normalisation of the rows of x [n, C] (row stride x_row elements):
+ * y = (x - mean) * rstd * weight + bias over each row's C channels, rstd =
+ * 1 / sqrt(biased variance + eps); weight and bias fp32 [C] or null. The
+ * variance is summed around the mean, in fp32.
+ */
+
+/* Workspace bytes for rhip_ln_backward. */
+int rhip_ln_workspace_bytes(int64_t n, int32_t C, size_t *bytes);
+
+/* y [n, C] dense; mean and rstd (fp32 [n], both or neither) for the backward. */
+int rhip_ln_forward(const void *x, int64_t x_row, int64_t n, int32_t C,
+                    const float *weight, const float *bias, double eps, void *y,
+                    float *mean, float *rstd, int32_t dtype, hipStream_t stream);
+
+/*
+ * With xhat = (x - mean) * rstd and g = grad_y * weight:
+ * grad_x = rstd * (g - mean(g) - xhat * mean(g * xhat)) (means over the row),
+ * grad_weight = sum over rows of grad_y * xhat, grad_bias = sum of grad_y.
+ * One pass over x and grad_y; the sums over rows are added in a fixed order.
+ * Any of grad_x, grad_weight, grad_bias may be null.
+ */
+int rhip_ln_backward(const void *grad_y, int64_t grad_y_row, const void *x,
+                     int64_t x_row, int64_t n, int32_t C, const float *mean,
+                     const float *rstd, const float *weight, void *grad_x,
+                     float *grad_weight, float *grad_bias, int32_t dtype,
+                     void *workspace, size_t workspace_bytes,
+                     hipStream_t stream);
+
+/* ------------------------------------------------------------- embedding
+ *
+ * y[i] = scale * weight[ids[i]] for a table weight [vocabulary, C] (row stride
+ * weight_row elements); ids outside [0, vocabulary) (voxels without a class)
+ * give a zero row and take no part in the gradient. ids are int64, or int32
+ * with ids_int32 != 0.
+ */
+int rhip_embed_forward(const void *ids, int32_t ids_int32, int64_t n,
+                       const void *weight, int64_t weight_row,
+                       int64_t vocabulary, int32_t C, float scale, void *y,
+                       int32_t dtype, hipStream_t stream);
+
+/* Workspace bytes for rhip_embed_backward. */
+int rhip_embed_workspace_bytes(int64_t n, int64_t vocabulary, int32_t C,
+                               size_t *bytes);
+
+/*
+ * grad_weight [vocabulary, C] (dense, overwritten; rows no id names get
+ * zeros) = scale * the sum of grad_y's rows over each id's positions, fp32
+ * sums in an order that depends on the ids alone (the positions are sorted by
+ * id; no float atomics).
+ */
+int rhip_embed_backward(const void *grad_y, int64_t grad_y_row, const void *ids,
+                        int32_t ids_int32, int64_t n, int64_t vocabulary,
+                        int32_t C, float scale, void *grad_weight,
+                        int32_t dtype, void *workspace, size_t workspace_bytes,
+                        hipStream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

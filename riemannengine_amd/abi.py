@@ -49,6 +49,9 @@ EXPORTS = (
     "rhip_global_pool_forward", "rhip_global_pool_backward",
     "rhip_bn_workspace_bytes", "rhip_bn_stats", "rhip_bn_invstd", "rhip_bn_forward",
     "rhip_bn_backward",
+    "rhip_attn_workspace_bytes", "rhip_attn_forward", "rhip_attn_backward",
+    "rhip_ln_workspace_bytes", "rhip_ln_forward", "rhip_ln_backward",
+    "rhip_embed_forward", "rhip_embed_workspace_bytes", "rhip_embed_backward",
 )
 
 
@@ -63,6 +66,20 @@ class RhipTable(ctypes.Structure):
         ("order", ctypes.c_void_p), ("bricks", ctypes.c_void_p),
         ("morton_bits", ctypes.c_int32), ("brick_levels", ctypes.c_int32),
         ("brick_dims", ctypes.c_int32 * MAX_COLS),
+    ]
+
+
+class RhipAttn(ctypes.Structure):
+    _fields_ = [
+        ("n_q", ctypes.c_int64), ("n_k", ctypes.c_int64),
+        ("q_row", ctypes.c_int64), ("q_head", ctypes.c_int64),
+        ("k_row", ctypes.c_int64), ("k_head", ctypes.c_int64),
+        ("v_row", ctypes.c_int64), ("v_head", ctypes.c_int64),
+        ("q_offsets", ctypes.c_void_p), ("k_offsets", ctypes.c_void_p),
+        ("k_lengths", ctypes.c_void_p),
+        ("n_seq", ctypes.c_int32), ("heads", ctypes.c_int32), ("kv_heads", ctypes.c_int32),
+        ("dim", ctypes.c_int32), ("causal", ctypes.c_int32), ("dtype", ctypes.c_int32),
+        ("scale", ctypes.c_float),
     ]
 
 
@@ -151,6 +168,21 @@ def _declare(lib):
                                            _i32, _vp]),
         "rhip_bn_backward": (ctypes.c_int, [_vp, _vp, _vp, _i64, _i32, _vp, _vp, _vp, _i32,
                                             _i32, _vp, _vp, _vp, _vp, _i32, _vp, _sz, _vp]),
+        "rhip_attn_workspace_bytes": (ctypes.c_int, [_P(RhipAttn), _i32, _P(_sz)]),
+        "rhip_attn_forward": (ctypes.c_int, [_P(RhipAttn), _vp, _vp, _vp, _vp, _vp, _vp, _sz,
+                                             _vp]),
+        "rhip_attn_backward": (ctypes.c_int, [_P(RhipAttn), _vp, _i64, _i64, _vp, _vp, _vp, _vp,
+                                              _vp, _vp, _vp, _vp, _vp, _sz, _vp]),
+        "rhip_ln_workspace_bytes": (ctypes.c_int, [_i64, _i32, _P(_sz)]),
+        "rhip_ln_forward": (ctypes.c_int, [_vp, _i64, _i64, _i32, _vp, _vp, ctypes.c_double, _vp,
+                                           _vp, _vp, _i32, _vp]),
+        "rhip_ln_backward": (ctypes.c_int, [_vp, _i64, _vp, _i64, _i64, _i32, _vp, _vp, _vp, _vp,
+                                            _vp, _vp, _i32, _vp, _sz, _vp]),
+        "rhip_embed_forward": (ctypes.c_int, [_vp, _i32, _i64, _vp, _i64, _i64, _i32,
+                                              ctypes.c_float, _vp, _i32, _vp]),
+        "rhip_embed_workspace_bytes": (ctypes.c_int, [_i64, _i64, _i32, _P(_sz)]),
+        "rhip_embed_backward": (ctypes.c_int, [_vp, _i64, _vp, _i32, _i64, _i64, _i32,
+                                               ctypes.c_float, _vp, _i32, _vp, _sz, _vp]),
     }
     for name, (res, args) in sig.items():
         fn = getattr(lib, name)
@@ -946,3 +978,142 @@ def bn_backward(grad_y: torch.Tensor, y: Optional[torch.Tensor], x: torch.Tensor
                                   _ptr(gx), _ptr(gr), _ptr(gg), _ptr(gb), dt, _ptr(ws),
                                   ws.numel(), _stream(x.device)), "rhip_bn_backward")
     return gx, gr, gg, gb
+
+
+def _dense_last(t: torch.Tensor) -> torch.Tensor:
+    """t itself where its last axis is dense, else a dense copy."""
+    return t if t.shape[-1] <= 1 or t.stride(-1) == 1 else t.contiguous()
+
+
+def _attn_desc(q, k, v, q_offsets, k_offsets, k_lengths, causal, scale) -> RhipAttn:
+    for t, name in ((q, "q"), (k, "k"), (v, "v"), (q_offsets, "q_offsets"),
+                    (k_offsets, "k_offsets")):
+        _require_cuda(t, name)
+    if q.dim() != 3 or k.dim() != 3 or v.shape != k.shape or q.shape[2] != k.shape[2]:
+        raise RuntimeError("q must be [n_q, heads, dim], k and v [n_k, kv_heads, dim]")
+    if k.dtype != q.dtype or v.dtype != q.dtype:
+        raise RuntimeError("q, k and v must share their dtype")
+    for t, name in ((q_offsets, "q_offsets"), (k_offsets, "k_offsets"), (k_lengths, "k_lengths")):
+        if t is not None and (t.dtype != torch.int32 or t.dim() != 1 or not t.is_contiguous()):
+            raise RuntimeError(f"{name} must be a dense int32 vector")
+    n_seq = q_offsets.numel() - 1
+    if n_seq < 0 or k_offsets.numel() != n_seq + 1:
+        raise RuntimeError("q_offsets and k_offsets must hold n_seq + 1 values each")
+    if k_lengths is not None and k_lengths.numel() != n_seq:
+        raise RuntimeError("k_lengths must hold one value per sequence")
+    return RhipAttn(q.shape[0], k.shape[0], q.stride(0), q.stride(1), k.stride(0), k.stride(1),
+                    v.stride(0), v.stride(1), q_offsets.data_ptr(), k_offsets.data_ptr(),
+                    None if k_lengths is None else k_lengths.data_ptr(), n_seq, q.shape[1],
+                    k.shape[1], q.shape[2], int(causal), _dtype_code(q.dtype),
+                    q.shape[2] ** -0.5 if scale is None else scale)
+
+
+def _attn_ws(desc: RhipAttn, backward: bool, device) -> torch.Tensor:
+    return torch.empty(_sizeq(lib().rhip_attn_workspace_bytes, ctypes.byref(desc),
+                              int(backward)), dtype=torch.uint8, device=device)
+
+
+def attn_forward(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, q_offsets: torch.Tensor,
+                 k_offsets: torch.Tensor, k_lengths: Optional[torch.Tensor] = None,
+                 causal: bool = False, scale: Optional[float] = None):
+    """(out [n_q, heads, dim], lse [heads, n_q]) of attention over packed
+    sequences; offsets and lengths int32 on the device."""
+    q, k, v = _dense_last(q), _dense_last(k), _dense_last(v)
+    desc = _attn_desc(q, k, v, q_offsets, k_offsets, k_lengths, causal, scale)
+    out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    lse = torch.empty((q.shape[1], q.shape[0]), dtype=torch.float32, device=q.device)
+    ws = _attn_ws(desc, False, q.device)
+    _check(lib().rhip_attn_forward(ctypes.byref(desc), _ptr(q), _ptr(k), _ptr(v), _ptr(out),
+                                   _ptr(lse), _ptr(ws), ws.numel(), _stream(q.device)),
+           "rhip_attn_forward")
+    return out, lse
+
+
+def attn_backward(grad_out: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
+                  out: torch.Tensor, lse: torch.Tensor, q_offsets: torch.Tensor,
+                  k_offsets: torch.Tensor, k_lengths: Optional[torch.Tensor] = None,
+                  causal: bool = False, scale: Optional[float] = None):
+    """(grad_q, grad_k, grad_v) from the forward's out and lse."""
+    q, k, v = _dense_last(q), _dense_last(k), _dense_last(v)
+    grad_out = _dense_last(grad_out.to(q.dtype))
+    desc = _attn_desc(q, k, v, q_offsets, k_offsets, k_lengths, causal, scale)
+    gq = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    gk = torch.empty(k.shape, dtype=q.dtype, device=q.device)
+    gv = torch.empty(k.shape, dtype=q.dtype, device=q.device)
+    ws = _attn_ws(desc, True, q.device)
+    _check(lib().rhip_attn_backward(ctypes.byref(desc), _ptr(grad_out), grad_out.stride(0),
+                                    grad_out.stride(1), _ptr(q), _ptr(k), _ptr(v), _ptr(out),
+                                    _ptr(lse), _ptr(gq), _ptr(gk), _ptr(gv), _ptr(ws),
+                                    ws.numel(), _stream(q.device)), "rhip_attn_backward")
+    return gq, gk, gv
+
+
+def ln_forward(x: torch.Tensor, weight: Optional[torch.Tensor] = None,
+               bias: Optional[torch.Tensor] = None, eps: float = 1e-5):
+    """(y, mean, rstd) of the rows of x [n, C]; weight and bias fp32 [C]."""
+    _require_cuda(x, "x")
+    dt = _dtype_code(x.dtype)
+    x = _dense_last(x)
+    n, C = x.shape
+    y = torch.empty((n, C), dtype=x.dtype, device=x.device)
+    f32 = dict(dtype=torch.float32, device=x.device)
+    mean, rstd = torch.empty(n, **f32), torch.empty(n, **f32)
+    _check(lib().rhip_ln_forward(_ptr(x), x.stride(0), n, C, _ptr(weight), _ptr(bias), eps,
+                                 _ptr(y), _ptr(mean), _ptr(rstd), dt, _stream(x.device)),
+           "rhip_ln_forward")
+    return y, mean, rstd
+
+
+def ln_backward(grad_y: torch.Tensor, x: torch.Tensor, mean: torch.Tensor, rstd: torch.Tensor,
+                weight: Optional[torch.Tensor] = None):
+    """(grad_x, grad_weight, grad_bias)."""
+    _require_cuda(x, "x")
+    dt = _dtype_code(x.dtype)
+    x, grad_y = _dense_last(x), _dense_last(grad_y.to(x.dtype))
+    n, C = x.shape
+    gx = torch.empty((n, C), dtype=x.dtype, device=x.device)
+    f32 = dict(dtype=torch.float32, device=x.device)
+    gw, gb = torch.empty(C, **f32), torch.empty(C, **f32)
+    ws = torch.empty(_sizeq(lib().rhip_ln_workspace_bytes, n, C), dtype=torch.uint8,
+                     device=x.device)
+    _check(lib().rhip_ln_backward(_ptr(grad_y), grad_y.stride(0), _ptr(x), x.stride(0), n, C,
+                                  _ptr(mean), _ptr(rstd), _ptr(weight), _ptr(gx), _ptr(gw),
+                                  _ptr(gb), dt, _ptr(ws), ws.numel(), _stream(x.device)),
+           "rhip_ln_backward")
+    return gx, gw, gb
+
+
+def _ids(ids: torch.Tensor) -> torch.Tensor:
+    _require_cuda(ids, "ids")
+    if ids.dtype not in (torch.int32, torch.int64) or ids.dim() != 1:
+        raise RuntimeError("ids must be an int32 or int64 vector")
+    return ids.contiguous()
+
+
+def embed_forward(ids: torch.Tensor, weight: torch.Tensor, scale: float = 1.0) -> torch.Tensor:
+    """scale * weight[ids], zero rows for ids outside the table."""
+    ids, weight = _ids(ids), _dense_last(weight)
+    _require_cuda(weight, "weight")
+    V, C = weight.shape
+    y = torch.empty((ids.numel(), C), dtype=weight.dtype, device=weight.device)
+    _check(lib().rhip_embed_forward(_ptr(ids), int(ids.dtype == torch.int32), ids.numel(),
+                                    _ptr(weight), weight.stride(0), V, C, scale, _ptr(y),
+                                    _dtype_code(weight.dtype), _stream(weight.device)),
+           "rhip_embed_forward")
+    return y
+
+
+def embed_backward(grad_y: torch.Tensor, ids: torch.Tensor, vocabulary: int,
+                   scale: float = 1.0) -> torch.Tensor:
+    """grad_weight [vocabulary, C] of embed_forward."""
+    ids, grad_y = _ids(ids), _dense_last(grad_y)
+    _require_cuda(grad_y, "grad_y")
+    n, C = grad_y.shape
+    gw = torch.empty((vocabulary, C), dtype=grad_y.dtype, device=grad_y.device)
+    ws = torch.empty(_sizeq(lib().rhip_embed_workspace_bytes, n, vocabulary, C),
+                     dtype=torch.uint8, device=grad_y.device)
+    _check(lib().rhip_embed_backward(_ptr(grad_y), grad_y.stride(0), _ptr(ids),
+                                     int(ids.dtype == torch.int32), n, vocabulary, C, scale,
+                                     _ptr(gw), _dtype_code(grad_y.dtype), _ptr(ws), ws.numel(),
+                                     _stream(grad_y.device)), "rhip_embed_backward")
+    return gw

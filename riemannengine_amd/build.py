@@ -29,7 +29,8 @@ HIPCC = os.path.join(ROCM, "bin", "hipcc")
 
 HIP_SOURCES = ["abi.hip", "sort.hip", "hash.hip", "kmap.hip", "conv.hip", "conv_thin.hip",
                "conv_x3.hip", "conv_pad.hip", "conv_small.hip",
-               "pool.hip", "norm.hip"]
+               "pool.hip", "norm.hip", "layer_norm.hip", "embed.hip",
+               "attn.hip", "attn_fwd.hip", "attn_bwd.hip"]
 # gfx950 only. Packed-FP32 instructions are disabled: the compiler would
 # otherwise form v_pk_* FP32 ops from plain float code.
 HIP_FLAGS = [

@@ -1,0 +1,34 @@
+// The attention passes behind rhip_attn_* (attn.hip), one translation unit
+// each, and the choice of their kernel variants.
+#pragma once
+
+#include <type_traits>
+
+#include "attn_device.hpp"
+
+namespace rhip {
+
+void attn_forward_run(const AttnArgs &a, int32_t dtype, bool vec, hipStream_t stream);
+void attn_backward_run(const AttnArgs &a, int32_t dtype, bool vec, hipStream_t stream);
+
+// f(T{}, head width of the variant, whether rows load in 16-byte chunks).
+// Rows that do not (a width or a stride that is no multiple of 16 bytes, an
+// unaligned view) load element by element into the widest tile of the type.
+template <typename F> void with_attn(int32_t dtype, int32_t dim, bool vec, F &&f) {
+  auto typed = [&](auto t) {
+    if (!vec)
+      f(t, std::integral_constant<int, kAttnMaxDim>{}, std::false_type{});
+    else if (dim <= 32)
+      f(t, std::integral_constant<int, 32>{}, std::true_type{});
+    else if (dim <= 64)
+      f(t, std::integral_constant<int, 64>{}, std::true_type{});
+    else
+      f(t, std::integral_constant<int, 128>{}, std::true_type{});
+  };
+  if (dtype == RHIP_F32)
+    typed(float{});
+  else
+    typed(__bf16{});
+}
+
+} // namespace rhip

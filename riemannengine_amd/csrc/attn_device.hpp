@@ -1,0 +1,272 @@
+// Device helpers shared by the attention kernels: sequences and tiles of
+// packed rows, 32-row LDS tiles and the two matrix products over them.
+//
+// Every kernel works on 32x32 score blocks with the 32x32 matrix
+// instructions (bf16 32x32x16, fp32 32x32x2): lane l holds, of a block's
+// column l % 32, the 16 rows 8 (r / 4) + 4 (l / 32) + r % 4, r = 0 .. 15.
+// Scores are computed transposed to the product that follows, so a lane
+// holds 16 entries of one softmax row (or of one key) and the block goes into
+// the next product as it lies: the sum over its rows may run in any order, so
+// the other operand is read in the order the lanes hold (no exchange between
+// lanes, no trip through LDS).
+#pragma once
+
+#include "conv_device.hpp"
+
+namespace rhip {
+
+typedef float v16f __attribute__((ext_vector_type(16)));
+
+constexpr int kAttnMaxDim = 128;
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLn2 = 0.6931471805599453f;
+
+// The kernels' arguments: rhip_attn's fields (strides in elements), scale
+// times log2(e) and the buffers.
+struct AttnArgs {
+  const void *q, *k, *v, *go;
+  const int32_t *q_off, *k_off, *k_len;
+  int64_t q_row, q_head, k_row, k_head, v_row, v_head, go_row, go_head;
+  int32_t n_q, n_k, n_seq, heads, kv_heads, group, dim, causal, tiles;
+  float scale, c; // c = scale * log2(e)
+  void *o;
+  float *lse;   // [heads, n_q], natural logarithm
+  float *delta; // [heads, n_q], rowsum(grad_out * out)
+  void *gq, *gk, *gv;
+};
+
+// One sequence of the packed rows, clamped to the buffers whatever the
+// offsets hold.
+struct AttnSeq {
+  int32_t s, tile; // sequence, tile within it
+  int32_t q0, lq, k0, lk;
+};
+
+__device__ __forceinline__ int32_t clamp_off(int32_t v, int32_t lo, int32_t hi) {
+  return v < lo ? lo : (v > hi ? hi : v);
+}
+
+// Tile t of packed rows cut into tiles of `bm` rows at every sequence.
+// Sequence s starts at tile floor(off[s] * mul / bm) + s: no two sequences
+// share a tile, the tiles between one's last and the next's first are empty,
+// and n * mul / bm + n_seq + 1 tiles cover them all, so neither the host nor
+// another kernel has to count tiles. Rows behind the last sequence count as
+// one more, without keys. mul: rows of a tile per packed row (grouped heads).
+__device__ __forceinline__ void find_tile(const int32_t *off, int32_t n_seq, int32_t n, int bm,
+                                          int mul, int32_t t, int32_t &seq, int32_t &tile,
+                                          int32_t &r0, int32_t &len) {
+  int lo = 0, hi = n_seq; // largest s with base(s) <= t
+  while (lo < hi) {
+    const int mid = (lo + hi + 1) >> 1;
+    const int64_t b =
+        static_cast<int64_t>(clamp_off(off[mid], 0, n)) * mul / bm + mid;
+    if (b <= t)
+      lo = mid;
+    else
+      hi = mid - 1;
+  }
+  seq = lo;
+  r0 = lo == 0 ? 0 : clamp_off(off[lo], 0, n);
+  const int32_t r1 = lo == n_seq ? n : clamp_off(off[lo + 1], r0, n);
+  len = r1 - r0;
+  tile = t - static_cast<int32_t>(static_cast<int64_t>(r0) * mul / bm + lo);
+}
+
+__device__ __forceinline__ AttnSeq query_tile(const AttnArgs &a, int bm, int mul, int32_t t) {
+  AttnSeq q;
+  find_tile(a.q_off, a.n_seq, a.n_q, bm, mul, t, q.s, q.tile, q.q0, q.lq);
+  q.k0 = q.lk = 0;
+  if (q.s < a.n_seq) {
+    q.k0 = q.s == 0 ? 0 : clamp_off(a.k_off[q.s], 0, a.n_k);
+    q.lk = clamp_off(a.k_off[q.s + 1], q.k0, a.n_k) - q.k0;
+    if (a.k_len)
+      q.lk = clamp_off(a.k_len[q.s], 0, q.lk);
+  }
+  return q;
+}
+
+// The same over the key rows (backward of k and v): lk counts the rows in
+// use, `room` all rows of the region.
+__device__ __forceinline__ AttnSeq key_tile(const AttnArgs &a, int bm, int32_t t, int32_t &room) {
+  AttnSeq q;
+  find_tile(a.k_off, a.n_seq, a.n_k, bm, 1, t, q.s, q.tile, q.k0, room);
+  q.q0 = q.lq = q.lk = 0;
+  if (q.s < a.n_seq) {
+    q.lk = a.k_len ? clamp_off(a.k_len[q.s], 0, room) : room;
+    q.q0 = q.s == 0 ? 0 : clamp_off(a.q_off[q.s], 0, a.n_q);
+    q.lq = clamp_off(a.q_off[q.s + 1], q.q0, a.n_q) - q.q0;
+  }
+  return q;
+}
+
+// Rows of `DP` elements (the head width padded to 32, 64 or 128) as 16-byte
+// chunks in LDS. Chunk c of row r lies at c ^ swz(r): 16 consecutive rows
+// then hold one chunk column in 16 different bank groups (row reads), and so
+// do 4 consecutive chunks of 4 consecutive rows (transpose reads).
+template <typename T, int DP> struct AttnTile {
+  static constexpr int E = 16 / sizeof(T);  // elements per chunk
+  static constexpr int C = DP / E;          // chunks per row
+  static constexpr int kDBlocks = DP / 32;  // 32-wide blocks of the head width
+  static constexpr int kSteps = C / 2;      // row_product steps (two chunks each)
+  using Frag = typename Mfma<T>::Frag;      // one chunk
+
+  __device__ static __forceinline__ int swz(int row) {
+    if constexpr (C >= 16)
+      return ((row & 3) << 2) | ((row >> 2) & 3);
+    else if constexpr (C == 8)
+      return (((row >> 1) & 1) << 2) | ((row >> 2) & 3);
+    else
+      return (row >> 2) & 3;
+  }
+  // byte address of chunk c of row
+  __device__ static __forceinline__ char *at(char *lds, int row, int c) {
+    return lds + (row * C + (c ^ swz(row))) * 16;
+  }
+  __device__ static __forceinline__ const char *at(const char *lds, int row, int c) {
+    return lds + (row * C + (c ^ swz(row))) * 16;
+  }
+
+  // Chunk c of a global row (E elements from p + c * E), zero past dim.
+  template <bool VEC>
+  __device__ static __forceinline__ uint4 chunk(const T *p, int c, int dim, bool row_ok) {
+    if constexpr (VEC) { // dim is a multiple of E and rows are 16-byte aligned
+      if (row_ok && c * E < dim)
+        return *reinterpret_cast<const uint4 *>(p + c * E);
+      return uint4{0u, 0u, 0u, 0u};
+    } else {
+      T e[E];
+#pragma unroll
+      for (int i = 0; i < E; ++i)
+        e[i] = row_ok && c * E + i < dim ? p[c * E + i] : static_cast<T>(0.f);
+      return __builtin_bit_cast(uint4, e);
+    }
+  }
+
+  // acc += A[32 rows x dim] B[dim x 32 columns]: A's rows row0 .. row0 + 31
+  // from the LDS tile, B the chunks a lane holds of its column.
+  __device__ static __forceinline__ void row_product(const char *lds, int row0,
+                                                     const Frag (&b)[kSteps], v16f &acc) {
+    const int lane = lane_id(), row = row0 + (lane & 31), half = lane >> 5;
+#pragma unroll
+    for (int s = 0; s < kSteps; ++s)
+      mma(*reinterpret_cast<const Frag *>(at(lds, row, 2 * s + half)), b[s], acc);
+  }
+
+  // The product of one chunk pair: lane half h holds elements (2 s + h) E ..
+  __device__ static __forceinline__ void mma(const Frag &a, const Frag &b, v16f &acc) {
+    if constexpr (sizeof(T) == 2) {
+      acc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, acc, 0, 0, 0);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        acc = __builtin_amdgcn_mfma_f32_32x32x2f32(a[i], b[i], acc, 0, 0, 0);
+    }
+  }
+
+  // A 32x32 block as the right operand of col_product: bf16 rounds here (the
+  // products' operands are 16 bits wide; their sums stay fp32).
+  struct Block {
+    v8bf lo, hi;
+    v16f f;
+  };
+  __device__ static __forceinline__ void pack(const v16f &p, Block &b) {
+    if constexpr (sizeof(T) == 2) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        b.lo[i] = static_cast<__bf16>(p[i]);
+        b.hi[i] = static_cast<__bf16>(p[8 + i]);
+      }
+    } else {
+      b.f = p;
+    }
+  }
+
+  // acc[db] += X^T[dim x 32 rows] B[32 rows x 32 columns]: X's rows row0 ..
+  // row0 + 31 from the LDS tile, B the block the lanes hold. Slot j of half h
+  // in step s stands for row 16 s + 8 (j / 4) + 4 h + j % 4, B's own order;
+  // a transpose read gives four consecutive rows of a lane's element column.
+  __device__ static __forceinline__ void col_product(const char *lds, int row0, const Block &b,
+                                                     v16f (&acc)[kDBlocks]) {
+    const int lane = lane_id(), half = lane >> 5;
+    if constexpr (sizeof(T) == 2) {
+      const int i = lane & 15, g = (lane >> 4) & 1;
+      const int r = row0 + 4 * half + (i >> 2);
+      const int c = 2 * g + ((i & 3) >> 1), sub = (i & 1) * 8;
+#pragma unroll
+      for (int s = 0; s < 2; ++s)
+#pragma unroll
+        for (int db = 0; db < kDBlocks; ++db) {
+          const v4s lo = ds_read_tr16(at(lds, r + 16 * s, 4 * db + c) + sub);
+          const v4s hi = ds_read_tr16(at(lds, r + 16 * s + 8, 4 * db + c) + sub);
+          const v8bf a = __builtin_bit_cast(
+              v8bf, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+          acc[db] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, s ? b.hi : b.lo, acc[db], 0, 0, 0);
+        }
+    } else {
+      const int col = lane & 31;
+#pragma unroll
+      for (int e = 0; e < 16; ++e) {
+        const int r = row0 + 8 * (e >> 2) + 4 * half + (e & 3);
+#pragma unroll
+        for (int db = 0; db < kDBlocks; ++db) {
+          const int d = 32 * db + col;
+          const float a =
+              reinterpret_cast<const float *>(at(lds, r, d / E))[d % E];
+          acc[db] = __builtin_amdgcn_mfma_f32_32x32x2f32(a, b.f[e], acc[db], 0, 0, 0);
+        }
+      }
+    }
+  }
+
+  // One lane's column of a [32 DB x 32] result, scaled, as a row of dim
+  // elements at p.
+  template <bool VEC>
+  __device__ static __forceinline__ void store_column(T *p, int dim, float mul,
+                                                      const v16f (&acc)[kDBlocks]) {
+    const int half = lane_id() >> 5;
+#pragma unroll
+    for (int db = 0; db < kDBlocks; ++db)
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        const int d = 32 * db + 8 * g + 4 * half;
+        T e[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          e[i] = from_f32<T>(acc[db][4 * g + i] * mul);
+        if constexpr (VEC) { // dim is a multiple of E, so of 4
+          if (d < dim) {
+            if constexpr (sizeof(T) == 2)
+              *reinterpret_cast<uint2 *>(p + d) = __builtin_bit_cast(uint2, e);
+            else
+              *reinterpret_cast<uint4 *>(p + d) = __builtin_bit_cast(uint4, e);
+          }
+        } else {
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            if (d + i < dim)
+              p[d + i] = e[i];
+        }
+      }
+  }
+};
+
+// Row r of a lane's 16 entries of a 32x32 block.
+__device__ __forceinline__ int block_row(int r) {
+  return 8 * (r >> 2) + 4 * (lane_id() >> 5) + (r & 3);
+}
+
+// Maximum and sum over the lane pair l, l ^ 32 (a column's two halves).
+__device__ __forceinline__ float pair_max(float v) {
+  const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false,
+                                                  false);
+  return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+__device__ __forceinline__ float pair_sum(float v) {
+  const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false,
+                                                  false);
+  return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+
+__device__ __forceinline__ float exp2_fast(float v) { return __builtin_amdgcn_exp2f(v); }
+
+} // namespace rhip

@@ -422,4 +422,80 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
            py::arg("inplanes"), py::arg("planes"), py::arg("stride") = 1,
            py::arg("dilation") = 1, py::arg("downsample") = py::none(), py::arg("bn_momentum") = 0.1,
            py::arg("dimension") = 3);
+
+  // transformer stages over packed rows; the calls release the interpreter
+  // lock while they queue their kernels
+  using OptTensor = c10::optional<at::Tensor>;
+  nn.def(
+      "packed_attention",
+      [](const at::Tensor &query, const at::Tensor &key, const at::Tensor &value,
+         const at::Tensor &query_offsets, OptTensor key_offsets, OptTensor key_lengths,
+         bool causal, c10::optional<double> scale) {
+        py::gil_scoped_release release;
+        return hip_packed_attention(query, key, value, query_offsets,
+                                    key_offsets.value_or(at::Tensor()),
+                                    key_lengths.value_or(at::Tensor()), causal, scale);
+      },
+      "softmax(scale * query key^T) value inside every packed sequence; query [rows, heads, "
+      "width], key and value [rows, key heads, width], offsets [sequences + 1].",
+      py::arg("query"), py::arg("key"), py::arg("value"), py::arg("query_offsets"),
+      py::arg("key_offsets") = py::none(), py::arg("key_lengths") = py::none(),
+      py::arg("causal") = false, py::arg("scale") = py::none());
+  nn.def(
+      "layer_norm",
+      [](const at::Tensor &input, OptTensor weight, OptTensor bias, double eps) {
+        py::gil_scoped_release release;
+        return hip_layer_norm(input, weight.value_or(at::Tensor()), bias.value_or(at::Tensor()),
+                              eps);
+      },
+      "Layer norm over the last axis; weight and bias fp32.", py::arg("input"),
+      py::arg("weight") = py::none(), py::arg("bias") = py::none(), py::arg("eps") = 1e-5);
+  nn.def(
+      "embedding",
+      [](const at::Tensor &ids, const at::Tensor &weight, double scale) {
+        py::gil_scoped_release release;
+        return hip_embedding(ids, weight, scale);
+      },
+      "scale * weight[ids]; zero rows, without a gradient, for ids outside the table.",
+      py::arg("ids"), py::arg("weight"), py::arg("scale") = 1.0);
+  auto layer_norm = bind_unary<RiemannLayerNormImpl>(nn, "RiemannLayerNorm");
+  layer_norm.def(py::init([](int64_t num_features, double eps, bool affine) {
+                   return std::make_shared<RiemannLayerNormImpl>(num_features, eps, affine);
+                 }),
+                 py::arg("num_features"), py::arg("eps") = 1e-5, py::arg("affine") = true);
+  auto embedding = bind_module<RiemannEmbeddingImpl>(nn, "RiemannEmbedding");
+  embedding.def(py::init([](int64_t num_embeddings, int64_t channels, double scale) {
+                  return std::make_shared<RiemannEmbeddingImpl>(num_embeddings, channels, scale);
+                }),
+                py::arg("num_embeddings"), py::arg("channels"), py::arg("scale") = 1.0);
+  for (const char *name : {"forward", "__call__"})
+    embedding
+        .def(
+            name,
+            [](RiemannEmbeddingImpl &self, const at::Tensor &ids) { return self.forward(ids); },
+            py::arg("ids"))
+        .def(
+            name,
+            [](RiemannEmbeddingImpl &self, const at::Tensor &ids, const SparseTensor &rows) {
+              return self.forward(ids, rows);
+            },
+            py::arg("ids"), py::arg("rows"));
+  embedding.def_property_readonly("weight",
+                                  [](RiemannEmbeddingImpl &self) { return self.weight_; });
+  bind_unary<RiemannAttentionImpl>(nn, "RiemannAttention")
+      .def(py::init([](int64_t channels, int64_t heads, int64_t kv_heads, bool causal,
+                       bool bias) {
+             return std::make_shared<RiemannAttentionImpl>(channels, heads, kv_heads, causal,
+                                                           bias);
+           }),
+           py::arg("channels"), py::arg("heads"), py::arg("kv_heads") = 0,
+           py::arg("causal") = false, py::arg("bias") = true);
+  bind_unary<AttentionBlockImpl>(nn, "AttentionBlock")
+      .def(py::init([](int64_t channels, int64_t heads, int64_t kv_heads, int64_t expansion,
+                       bool causal) {
+             return std::make_shared<AttentionBlockImpl>(channels, heads, kv_heads, expansion,
+                                                         causal);
+           }),
+           py::arg("channels"), py::arg("heads"), py::arg("kv_heads") = 0,
+           py::arg("expansion") = 4, py::arg("causal") = false);
 }

@@ -621,4 +621,96 @@ public:
 };
 TORCH_MODULE(BasicBlock);
 
+// ------------------------------------------------------------ transformer
+
+// Attention over packed sequences through the HIP kernels (autograd-aware):
+// query [n_q, heads, width], key and value [n_k, key heads, width], offsets
+// int32 or int64 [sequences + 1] (key_offsets undefined: the query's),
+// key_lengths (keys in use per sequence) may be undefined. causal: the last
+// query row of a sequence sees every key, each earlier one a key less. scale
+// defaults to 1 / sqrt(width). fp32 or bf16, width <= 128.
+at::Tensor hip_packed_attention(const at::Tensor &query, const at::Tensor &key,
+                                const at::Tensor &value, const at::Tensor &query_offsets,
+                                const at::Tensor &key_offsets = at::Tensor(),
+                                const at::Tensor &key_lengths = at::Tensor(),
+                                bool causal = false, c10::optional<double> scale = c10::nullopt);
+
+// Layer norm over the last axis (autograd-aware); weight and bias fp32 or
+// undefined.
+at::Tensor hip_layer_norm(const at::Tensor &input, const at::Tensor &weight = at::Tensor(),
+                          const at::Tensor &bias = at::Tensor(), double eps = 1e-5);
+
+// scale * weight[ids] (autograd-aware); ids outside the table give zero rows
+// without a gradient.
+at::Tensor hip_embedding(const at::Tensor &ids, const at::Tensor &weight, double scale = 1.0);
+
+class RiemannLayerNormImpl : public torch::nn::Cloneable<RiemannLayerNormImpl> {
+public:
+  explicit RiemannLayerNormImpl(int64_t num_features, double eps = 1e-5, bool affine = true);
+  void reset() override;
+  SparseTensor forward(const SparseTensor &input);
+  // The affine parameters stay fp32 under a dtype cast, as RiemannBatchNorm's.
+  using torch::nn::Module::to;
+  void to(torch::Dtype dtype, bool non_blocking = false) override;
+  void to(torch::Device device, torch::Dtype dtype, bool non_blocking = false) override;
+
+  torch::Tensor weight_, bias_;
+
+private:
+  int64_t num_features_;
+  double eps_;
+  bool affine_;
+};
+TORCH_MODULE(RiemannLayerNorm);
+
+// Feature rows of class or token ids.
+class RiemannEmbeddingImpl : public torch::nn::Cloneable<RiemannEmbeddingImpl> {
+public:
+  RiemannEmbeddingImpl(int64_t num_embeddings, int64_t channels, double scale = 1.0);
+  void reset() override;
+  at::Tensor forward(const at::Tensor &ids);
+  // One id per row of `rows`: the features on its map.
+  SparseTensor forward(const at::Tensor &ids, const SparseTensor &rows);
+
+  torch::Tensor weight_;
+
+private:
+  int64_t num_embeddings_, channels_;
+  double scale_;
+};
+TORCH_MODULE(RiemannEmbedding);
+
+// Multi-head attention among the rows of each batch, in their row order;
+// kv_heads 0: as many as heads.
+class RiemannAttentionImpl : public torch::nn::Cloneable<RiemannAttentionImpl> {
+public:
+  RiemannAttentionImpl(int64_t channels, int64_t heads, int64_t kv_heads = 0,
+                       bool causal = false, bool bias = true);
+  void reset() override;
+  SparseTensor forward(const SparseTensor &input);
+
+private:
+  int64_t channels_, heads_, kv_heads_;
+  bool causal_, has_bias_;
+  torch::nn::Linear projection_{nullptr}, output_{nullptr};
+};
+TORCH_MODULE(RiemannAttention);
+
+// x + attention(norm1(x)), then x + down(gelu(up(norm2(x)))).
+class AttentionBlockImpl : public torch::nn::Cloneable<AttentionBlockImpl> {
+public:
+  AttentionBlockImpl(int64_t channels, int64_t heads, int64_t kv_heads = 0,
+                     int64_t expansion = 4, bool causal = false);
+  void reset() override;
+  SparseTensor forward(const SparseTensor &input);
+
+private:
+  int64_t channels_, heads_, kv_heads_, expansion_;
+  bool causal_;
+  RiemannLayerNorm norm1_{nullptr}, norm2_{nullptr};
+  RiemannAttention attention_{nullptr};
+  torch::nn::Linear up_{nullptr}, down_{nullptr};
+};
+TORCH_MODULE(AttentionBlock);
+
 } // namespace riemann

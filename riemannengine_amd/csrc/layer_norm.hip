@@ -1,0 +1,500 @@
+// Layer normalisation of feature rows on gfx950, forward and backward with
+// the parameters' gradients.
+//
+// A row belongs to G lanes (8 .. 64 of a wave, or the workgroup's 256), which
+// keep it in registers between its statistics and its output: x is read once
+// in the forward, x and grad_y once in the backward. The variance is summed
+// around the mean from the registers, so no cancellation: fp32 is enough.
+// Rows too wide for the registers are streamed again from the caches.
+//
+// The parameters' gradients are sums over rows. A backward workgroup walks
+// many rows and keeps its sums in registers next to the rows' own, writes
+// them once, and a second kernel adds the workgroups' sums (fp64, fixed
+// order). Both directions are bounded by memory.
+#include <climits>
+#include <type_traits>
+
+#include "row_chunk.hpp"
+
+namespace rhip {
+namespace {
+
+constexpr int kLnThreads = 256;
+// Backward workgroups to aim for: each writes 2 C fp32 sums.
+constexpr int kLnBlocks = 1024;
+constexpr int kSumCols = 16, kSumRows = 64; // ln_sums_kernel's columns and row lanes
+
+// Sum over a row's G lanes, in every lane; G = 256: the workgroup, through
+// LDS (buf holds 4 floats and is free again after the next barrier).
+template <int G> __device__ __forceinline__ float row_sum(float v, float *buf) {
+#pragma unroll
+  for (int off = 1; off < (G < kWave ? G : kWave); off <<= 1)
+    v += __shfl_xor(v, off, kWave);
+  if constexpr (G > kWave) {
+    if (lane_id() == 0)
+      buf[threadIdx.x / kWave] = v;
+    __syncthreads();
+    v = (buf[0] + buf[1]) + (buf[2] + buf[3]);
+  }
+  return v;
+}
+
+// y = (x - mean) rstd w + b, NC chunks of a row per lane.
+template <typename T, int G, int NC>
+__global__ __launch_bounds__(kLnThreads) void ln_forward_kernel(
+    const T *__restrict__ x, int64_t x_row, int64_t n, int C, const float *__restrict__ weight,
+    const float *__restrict__ bias, float eps, T *__restrict__ y, float *__restrict__ mean_out,
+    float *__restrict__ rstd_out) {
+  using R = RowChunk<T>;
+  __shared__ float buf[2][4];
+  const int lane = threadIdx.x % G;
+  const int64_t row = static_cast<int64_t>(blockIdx.x) * (kLnThreads / G) + threadIdx.x / G;
+  if (row >= n) // whole groups of lanes: the row sums stay within them
+    return;
+  float v[NC][R::V];
+  float s = 0.f;
+#pragma unroll
+  for (int i = 0; i < NC; ++i) {
+    const int c = (lane + i * G) * R::V;
+    R::load(x + row * x_row + c, C - c, v[i]);
+  }
+#pragma unroll
+  for (int i = 0; i < NC; ++i)
+#pragma unroll
+    for (int e = 0; e < R::V; ++e)
+      s += v[i][e];
+  const float mean = row_sum<G>(s, buf[0]) / static_cast<float>(C);
+  s = 0.f;
+#pragma unroll
+  for (int i = 0; i < NC; ++i) {
+    const int c = (lane + i * G) * R::V;
+#pragma unroll
+    for (int e = 0; e < R::V; ++e) {
+      v[i][e] = c + e < C ? v[i][e] - mean : 0.f;
+      s = fmaf(v[i][e], v[i][e], s);
+    }
+  }
+  const float var = row_sum<G>(s, buf[1]) / static_cast<float>(C);
+  const float rstd = 1.f / sqrtf(var + eps);
+#pragma unroll
+  for (int i = 0; i < NC; ++i) {
+    const int c = (lane + i * G) * R::V;
+    if (c < C) {
+      float w[R::V], b[R::V];
+      load_params<R::V>(weight, c, C, 1.f, w);
+      load_params<R::V>(bias, c, C, 0.f, b);
+#pragma unroll
+      for (int e = 0; e < R::V; ++e)
+        v[i][e] = fmaf(v[i][e] * rstd, w[e], b[e]);
+      R::store(y + row * C + c, C - c, v[i]);
+    }
+  }
+  if (mean_out && lane == 0) {
+    mean_out[row] = mean;
+    rstd_out[row] = rstd;
+  }
+}
+
+// Rows wider than the registers: three passes over the row, the later two
+// from the caches. One workgroup per row.
+template <typename T>
+__global__ __launch_bounds__(kLnThreads) void ln_forward_wide_kernel(
+    const T *__restrict__ x, int64_t x_row, int64_t n, int C, const float *__restrict__ weight,
+    const float *__restrict__ bias, float eps, T *__restrict__ y, float *__restrict__ mean_out,
+    float *__restrict__ rstd_out) {
+  using R = RowChunk<T>;
+  __shared__ float buf[2][4];
+  const int64_t row = blockIdx.x;
+  const T *xr = x + row * x_row;
+  const int c0 = threadIdx.x * R::V, step = kLnThreads * R::V;
+  float v[R::V], s = 0.f;
+  for (int c = c0; c < C; c += step) {
+    R::load(xr + c, C - c, v);
+#pragma unroll
+    for (int e = 0; e < R::V; ++e)
+      s += v[e];
+  }
+  const float mean = row_sum<kLnThreads>(s, buf[0]) / static_cast<float>(C);
+  s = 0.f;
+  for (int c = c0; c < C; c += step) {
+    R::load(xr + c, C - c, v);
+#pragma unroll
+    for (int e = 0; e < R::V; ++e) {
+      const float d = c + e < C ? v[e] - mean : 0.f;
+      s = fmaf(d, d, s);
+    }
+  }
+  const float var = row_sum<kLnThreads>(s, buf[1]) / static_cast<float>(C);
+  const float rstd = 1.f / sqrtf(var + eps);
+  for (int c = c0; c < C; c += step) {
+    float w[R::V], b[R::V];
+    R::load(xr + c, C - c, v);
+    load_params<R::V>(weight, c, C, 1.f, w);
+    load_params<R::V>(bias, c, C, 0.f, b);
+#pragma unroll
+    for (int e = 0; e < R::V; ++e)
+      v[e] = fmaf((v[e] - mean) * rstd, w[e], b[e]);
+    R::store(y + row * C + c, C - c, v);
+  }
+  if (mean_out && threadIdx.x == 0) {
+    mean_out[row] = mean;
+    rstd_out[row] = rstd;
+  }
+}
+
+// grad_x of the rows b, b + blocks, .. (in groups of 256 / G rows) and the
+// workgroup's sums of grad_y and grad_y xhat into part[b] = [2][C].
+template <typename T, int G, int NC>
+__global__ __launch_bounds__(kLnThreads) void ln_backward_kernel(
+    const T *__restrict__ gy, int64_t gy_row, const T *__restrict__ x, int64_t x_row, int64_t n,
+    int C, const float *__restrict__ mean, const float *__restrict__ rstd,
+    const float *__restrict__ weight, T *__restrict__ gx, float *__restrict__ part) {
+  using R = RowChunk<T>;
+  constexpr int kGroups = kLnThreads / G;
+  __shared__ float buf[2][2][4];
+  const int lane = threadIdx.x % G, group = threadIdx.x / G;
+  float w[NC][R::V], sb[NC][R::V], sw[NC][R::V];
+#pragma unroll
+  for (int i = 0; i < NC; ++i) {
+    load_params<R::V>(weight, (lane + i * G) * R::V, C, 1.f, w[i]);
+#pragma unroll
+    for (int e = 0; e < R::V; ++e)
+      sb[i][e] = sw[i][e] = 0.f;
+  }
+  const float inv_c = 1.f / static_cast<float>(C);
+  int turn = 0;
+  // the workgroup's groups go through the loop together (its barriers)
+  for (int64_t r0 = static_cast<int64_t>(blockIdx.x) * kGroups; r0 < n;
+       r0 += static_cast<int64_t>(gridDim.x) * kGroups) {
+    const int64_t row = r0 + group;
+    const bool ok = row < n;
+    const float mu = ok ? mean[row] : 0.f, rs = ok ? rstd[row] : 0.f;
+    float g[NC][R::V], h[NC][R::V]; // grad_y, xhat
+    float s1 = 0.f, s2 = 0.f;
+#pragma unroll
+    for (int i = 0; i < NC; ++i) {
+      const int c = (lane + i * G) * R::V;
+      R::load(gy + row * gy_row + c, ok ? C - c : 0, g[i]);
+      R::load(x + row * x_row + c, ok ? C - c : 0, h[i]);
+    }
+#pragma unroll
+    for (int i = 0; i < NC; ++i) {
+      const int c = (lane + i * G) * R::V;
+#pragma unroll
+      for (int e = 0; e < R::V; ++e) {
+        h[i][e] = c + e < C ? (h[i][e] - mu) * rs : 0.f;
+        const float gw = g[i][e] * w[i][e];
+        s1 += gw;
+        s2 = fmaf(gw, h[i][e], s2);
+        sb[i][e] += g[i][e];
+        sw[i][e] = fmaf(g[i][e], h[i][e], sw[i][e]);
+      }
+    }
+    if (gx) {
+      s1 = row_sum<G>(s1, buf[turn][0]) * inv_c;
+      s2 = row_sum<G>(s2, buf[turn][1]) * inv_c;
+      turn ^= 1;
+      if (ok) {
+#pragma unroll
+        for (int i = 0; i < NC; ++i) {
+          const int c = (lane + i * G) * R::V;
+          if (c < C) {
+            float o[R::V];
+#pragma unroll
+            for (int e = 0; e < R::V; ++e)
+              o[e] = rs * (g[i][e] * w[i][e] - s1 - h[i][e] * s2);
+            R::store(gx + row * C + c, C - c, o);
+          }
+        }
+      }
+    }
+  }
+  if (!part)
+    return;
+  float *dst = part + static_cast<int64_t>(blockIdx.x) * 2 * C;
+  auto put = [&](int i, const float (&b)[R::V], const float (&s)[R::V]) {
+    const int c = (lane + i * G) * R::V;
+#pragma unroll
+    for (int e = 0; e < R::V; ++e)
+      if (c + e < C) {
+        dst[c + e] = b[e];
+        dst[C + c + e] = s[e];
+      }
+  };
+  if constexpr (kGroups == 1) {
+#pragma unroll
+    for (int i = 0; i < NC; ++i)
+      put(i, sb[i], sw[i]);
+  } else {
+    // the groups' sums, added in group order
+    __shared__ float lds[kLnThreads][2 * R::V + 1];
+#pragma unroll
+    for (int i = 0; i < NC; ++i) {
+      __syncthreads();
+#pragma unroll
+      for (int e = 0; e < R::V; ++e) {
+        lds[threadIdx.x][e] = sb[i][e];
+        lds[threadIdx.x][R::V + e] = sw[i][e];
+      }
+      __syncthreads();
+      if (group == 0) {
+#pragma unroll 1
+        for (int k = 1; k < kGroups; ++k)
+#pragma unroll
+          for (int e = 0; e < R::V; ++e) {
+            sb[i][e] += lds[k * G + lane][e];
+            sw[i][e] += lds[k * G + lane][R::V + e];
+          }
+        put(i, sb[i], sw[i]);
+      }
+    }
+  }
+}
+
+// Wide rows: grad_x alone, a workgroup per row, reading the row twice.
+template <typename T>
+__global__ __launch_bounds__(kLnThreads) void ln_backward_wide_kernel(
+    const T *__restrict__ gy, int64_t gy_row, const T *__restrict__ x, int64_t x_row, int C,
+    const float *__restrict__ mean, const float *__restrict__ rstd,
+    const float *__restrict__ weight, T *__restrict__ gx) {
+  using R = RowChunk<T>;
+  __shared__ float buf[2][4];
+  const int64_t row = blockIdx.x;
+  const T *xr = x + row * x_row, *gr = gy + row * gy_row;
+  const float mu = mean[row], rs = rstd[row], inv_c = 1.f / static_cast<float>(C);
+  const int c0 = threadIdx.x * R::V, step = kLnThreads * R::V;
+  float g[R::V], h[R::V], w[R::V], s1 = 0.f, s2 = 0.f;
+  auto load = [&](int c) {
+    R::load(gr + c, C - c, g);
+    R::load(xr + c, C - c, h);
+    load_params<R::V>(weight, c, C, 1.f, w);
+#pragma unroll
+    for (int e = 0; e < R::V; ++e) {
+      h[e] = c + e < C ? (h[e] - mu) * rs : 0.f;
+      g[e] *= w[e];
+    }
+  };
+  for (int c = c0; c < C; c += step) {
+    load(c);
+#pragma unroll
+    for (int e = 0; e < R::V; ++e) {
+      s1 += g[e];
+      s2 = fmaf(g[e], h[e], s2);
+    }
+  }
+  s1 = row_sum<kLnThreads>(s1, buf[0]) * inv_c;
+  s2 = row_sum<kLnThreads>(s2, buf[1]) * inv_c;
+  for (int c = c0; c < C; c += step) {
+    load(c);
+#pragma unroll
+    for (int e = 0; e < R::V; ++e)
+      g[e] = rs * (g[e] - s1 - h[e] * s2);
+    R::store(gx + row * C + c, C - c, g);
+  }
+}
+
+// Wide rows: the parameters' sums of the rows b, b + blocks, .. over one tile
+// of 256 chunks (blockIdx.y).
+template <typename T>
+__global__ __launch_bounds__(kLnThreads) void ln_param_wide_kernel(
+    const T *__restrict__ gy, int64_t gy_row, const T *__restrict__ x, int64_t x_row, int64_t n,
+    int C, const float *__restrict__ mean, const float *__restrict__ rstd,
+    float *__restrict__ part) {
+  using R = RowChunk<T>;
+  const int c = (blockIdx.y * kLnThreads + threadIdx.x) * R::V;
+  if (c >= C)
+    return;
+  float sb[R::V], sw[R::V];
+#pragma unroll
+  for (int e = 0; e < R::V; ++e)
+    sb[e] = sw[e] = 0.f;
+  for (int64_t row = blockIdx.x; row < n; row += gridDim.x) {
+    const float mu = mean[row], rs = rstd[row];
+    float g[R::V], h[R::V];
+    R::load(gy + row * gy_row + c, C - c, g);
+    R::load(x + row * x_row + c, C - c, h);
+#pragma unroll
+    for (int e = 0; e < R::V; ++e) {
+      sb[e] += g[e];
+      sw[e] = fmaf(g[e], (h[e] - mu) * rs, sw[e]);
+    }
+  }
+  float *dst = part + static_cast<int64_t>(blockIdx.x) * 2 * C;
+#pragma unroll
+  for (int e = 0; e < R::V; ++e)
+    if (c + e < C) {
+      dst[c + e] = sb[e];
+      dst[C + c + e] = sw[e];
+    }
+}
+
+// grad_bias = sum over b of part[b][0], grad_weight of part[b][1]: 16 columns
+// by 64 row lanes per workgroup, then a tree in LDS.
+__global__ __launch_bounds__(kSumCols *kSumRows) void ln_sums_kernel(
+    const float *__restrict__ part, int blocks, int C, float *__restrict__ gw,
+    float *__restrict__ gb) {
+  __shared__ double lds[kSumRows][kSumCols];
+  const int col = threadIdx.x % kSumCols, r = threadIdx.x / kSumCols;
+  const int c = blockIdx.x * kSumCols + col;
+  double s = 0.0;
+  if (c < 2 * C)
+    for (int b = r; b < blocks; b += kSumRows)
+      s += part[static_cast<int64_t>(b) * 2 * C + c];
+  lds[r][col] = s;
+#pragma unroll
+  for (int off = kSumRows / 2; off; off >>= 1) {
+    __syncthreads();
+    if (r < off)
+      lds[r][col] += lds[r + off][col];
+  }
+  if (r == 0 && c < 2 * C) {
+    float *dst = c < C ? gb : gw;
+    if (dst)
+      dst[c < C ? c : c - C] = static_cast<float>(lds[0][col]);
+  }
+}
+
+// ------------------------------------------------------------------ host
+
+// f(T{}, lanes per row, chunks per lane); lanes 0: wider than the registers.
+// Two chunks per lane until a wave is full, then up to four, then the
+// workgroup shares the row.
+template <typename F> void with_row(int32_t dtype, int C, F &&f) {
+  auto typed = [&](auto t) {
+    const int chunks = static_cast<int>(ceil_div(C, RowChunk<decltype(t)>::V));
+    auto go = [&](auto g, auto nc) { f(t, g, nc); };
+    using std::integral_constant;
+    if (chunks <= 16)
+      go(integral_constant<int, 8>{}, integral_constant<int, 2>{});
+    else if (chunks <= 32)
+      go(integral_constant<int, 16>{}, integral_constant<int, 2>{});
+    else if (chunks <= 64)
+      go(integral_constant<int, 32>{}, integral_constant<int, 2>{});
+    else if (chunks <= 128)
+      go(integral_constant<int, 64>{}, integral_constant<int, 2>{});
+    else if (chunks <= 256)
+      go(integral_constant<int, 64>{}, integral_constant<int, 4>{});
+    else if (chunks <= 512)
+      go(integral_constant<int, 256>{}, integral_constant<int, 2>{});
+    else if (chunks <= 1024)
+      go(integral_constant<int, 256>{}, integral_constant<int, 4>{});
+    else
+      go(integral_constant<int, 0>{}, integral_constant<int, 0>{});
+  };
+  if (dtype == RHIP_F32)
+    typed(float{});
+  else
+    typed(__bf16{});
+}
+
+void check_rows(int32_t dtype, int64_t n, int32_t C) {
+  if (dtype != RHIP_F32 && dtype != RHIP_BF16)
+    throw Error(RHIP_ERR_UNSUPPORTED, "dtype must be RHIP_F32 or RHIP_BF16");
+  RHIP_CHECK_ARG(n >= 0 && C >= 1, "bad sizes");
+  if (n > INT32_MAX)
+    throw Error(RHIP_ERR_UNSUPPORTED, "too many rows");
+}
+
+// Workgroups of the backward: no more than row groups, at most kLnBlocks.
+int64_t ln_blocks(int64_t n) { return std::max<int64_t>(1, std::min<int64_t>(n, kLnBlocks)); }
+
+} // namespace
+} // namespace rhip
+
+using namespace rhip;
+
+extern "C" int rhip_ln_workspace_bytes(int64_t n, int32_t C, size_t *bytes) {
+  return guarded([&] {
+    RHIP_CHECK_ARG(bytes != nullptr, "bytes is null");
+    RHIP_CHECK_ARG(n >= 0 && C >= 1, "bad sizes");
+    Carve cv(nullptr, 0);
+    cv.take<float>(ln_blocks(n) * 2 * static_cast<size_t>(C));
+    *bytes = cv.used + 256;
+  });
+}
+
+extern "C" int rhip_ln_forward(const void *x, int64_t x_row, int64_t n, int32_t C,
+                               const float *weight, const float *bias, double eps, void *y,
+                               float *mean, float *rstd, int32_t dtype, hipStream_t stream) {
+  return guarded([&] {
+    check_rows(dtype, n, C);
+    RHIP_CHECK_ARG(eps > 0, "eps must be positive");
+    RHIP_CHECK_ARG((mean == nullptr) == (rstd == nullptr), "mean and rstd go together");
+    if (n == 0)
+      return;
+    RHIP_CHECK_ARG(x && y, "x and y are required");
+    with_row(dtype, C, [&](auto t, auto g, auto nc) {
+      using T = decltype(t);
+      constexpr int G = decltype(g)::value, NC = decltype(nc)::value;
+      const T *xp = static_cast<const T *>(x);
+      T *yp = static_cast<T *>(y);
+      const float e = static_cast<float>(eps);
+      if constexpr (G == 0)
+        hipLaunchKernelGGL((ln_forward_wide_kernel<T>), dim3(static_cast<unsigned>(n)),
+                           dim3(kLnThreads), 0, stream, xp, x_row, n, C, weight, bias, e, yp,
+                           mean, rstd);
+      else
+        hipLaunchKernelGGL((ln_forward_kernel<T, G, NC>),
+                           dim3(static_cast<unsigned>(ceil_div(n, kLnThreads / G))),
+                           dim3(kLnThreads), 0, stream, xp, x_row, n, C, weight, bias, e, yp,
+                           mean, rstd);
+      RHIP_LAUNCH_CHECK();
+    });
+  });
+}
+
+extern "C" int rhip_ln_backward(const void *grad_y, int64_t grad_y_row, const void *x,
+                                int64_t x_row, int64_t n, int32_t C, const float *mean,
+                                const float *rstd, const float *weight, void *grad_x,
+                                float *grad_weight, float *grad_bias, int32_t dtype,
+                                void *workspace, size_t ws_bytes, hipStream_t stream) {
+  return guarded([&] {
+    check_rows(dtype, n, C);
+    RHIP_CHECK_ARG(n == 0 || (grad_y && x && mean && rstd),
+                   "grad_y, x, mean and rstd are required");
+    const bool params = grad_weight || grad_bias;
+    RHIP_CHECK_ARG(!params || workspace, "workspace is required");
+    int64_t blocks = ln_blocks(n);
+    float *part = nullptr;
+    if (params) {
+      Carve cv(workspace, ws_bytes);
+      part = cv.take<float>(blocks * 2 * static_cast<size_t>(C));
+    }
+    if (!params && (!grad_x || n == 0))
+      return;
+    with_row(dtype, C, [&](auto t, auto g, auto nc) {
+      using T = decltype(t);
+      constexpr int G = decltype(g)::value, NC = decltype(nc)::value;
+      const T *gp = static_cast<const T *>(grad_y), *xp = static_cast<const T *>(x);
+      T *gxp = static_cast<T *>(grad_x);
+      if constexpr (G == 0) {
+        if (gxp && n > 0) {
+          hipLaunchKernelGGL((ln_backward_wide_kernel<T>), dim3(static_cast<unsigned>(n)),
+                             dim3(kLnThreads), 0, stream, gp, grad_y_row, xp, x_row, C, mean,
+                             rstd, weight, gxp);
+          RHIP_LAUNCH_CHECK();
+        }
+        if (part) {
+          const unsigned tiles =
+              static_cast<unsigned>(ceil_div(C, kLnThreads * RowChunk<T>::V));
+          hipLaunchKernelGGL((ln_param_wide_kernel<T>), dim3(static_cast<unsigned>(blocks), tiles),
+                             dim3(kLnThreads), 0, stream, gp, grad_y_row, xp, x_row, n, C, mean,
+                             rstd, part);
+          RHIP_LAUNCH_CHECK();
+        }
+      } else {
+        blocks = std::max<int64_t>(1, std::min(blocks, ceil_div(n, kLnThreads / G)));
+        hipLaunchKernelGGL((ln_backward_kernel<T, G, NC>), dim3(static_cast<unsigned>(blocks)),
+                           dim3(kLnThreads), 0, stream, gp, grad_y_row, xp, x_row, n, C, mean,
+                           rstd, weight, n > 0 ? gxp : nullptr, part);
+        RHIP_LAUNCH_CHECK();
+      }
+    });
+    if (part) {
+      hipLaunchKernelGGL(ln_sums_kernel, dim3(static_cast<unsigned>(ceil_div(2 * C, kSumCols))),
+                         dim3(kSumCols * kSumRows), 0, stream, part, static_cast<int>(blocks), C,
+                         grad_weight, grad_bias);
+      RHIP_LAUNCH_CHECK();
+    }
+  });
+}
