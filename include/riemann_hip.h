@@ -714,9 +714,7 @@ int rhip_bn_backward(const void *grad_y, const void *y, const void *x, int64_t n
  *
  * A row that sees no key, and query rows behind the last sequence, get zeros.
  * What lies in rows that a row does not see never reaches it, infinities and
- * NaN included (forward; in the backward pass under a causal mask, a row of
- * grad_out or q that is not finite may also reach the gradients of up to 31
- * later keys).
+ * NaN included.
  *
  * Offsets are int32 [n_seq + 1] on the device, the first 0 and none smaller
  * than the one before, at most n_q (n_k); sums, maxima and the softmax's
@@ -746,24 +744,30 @@ int rhip_attn_workspace_bytes(const rhip_attn *attn, int32_t backward,
 /*
  * out [n_q, heads, dim] (dense). lse [heads, n_q], the natural logarithm of
  * each row's softmax denominator (-inf for a row that sees no key), is
- * written when not null; the backward pass needs it.
+ * written when not null; the backward pass needs it. out_rest (bf16 only,
+ * like out, may be null): what rounding took off out. With it the backward
+ * pass has rowsum(grad_out * out) as exact as fp32 keeps it: the gradients of
+ * scores are differences from that sum, and small ones (rows that see few
+ * keys) would carry out's whole rounding error.
  */
 int rhip_attn_forward(const rhip_attn *attn, const void *q, const void *k,
-                      const void *v, void *out, float *lse, void *workspace,
-                      size_t workspace_bytes, hipStream_t stream);
+                      const void *v, void *out, void *out_rest, float *lse,
+                      void *workspace, size_t workspace_bytes,
+                      hipStream_t stream);
 
 /*
  * grad_q [n_q, heads, dim], grad_k and grad_v [n_k, kv_heads, dim] (dense,
- * overwritten; key rows not in use get zeros) from out and lse of the
- * forward pass; grad_out has its own strides. Gradients of a key head are
+ * overwritten; key rows not in use get zeros) from out, out_rest (may be null)
+ * and lse of the forward pass; grad_out has its own strides. Gradients of a key head are
  * summed over its query heads. grad_q may be null, and grad_k and grad_v both.
  */
 int rhip_attn_backward(const rhip_attn *attn, const void *grad_out,
                        int64_t grad_out_row, int64_t grad_out_head,
                        const void *q, const void *k, const void *v,
-                       const void *out, const float *lse, void *grad_q,
-                       void *grad_k, void *grad_v, void *workspace,
-                       size_t workspace_bytes, hipStream_t stream);
+                       const void *out, const void *out_rest, const float *lse,
+                       void *grad_q, void *grad_k, void *grad_v,
+                       void *workspace, size_t workspace_bytes,
+                       hipStream_t stream);
 
 /* ------------------------------------------------------------ layer norm
  *

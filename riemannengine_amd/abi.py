@@ -169,10 +169,10 @@ def _declare(lib):
         "rhip_bn_backward": (ctypes.c_int, [_vp, _vp, _vp, _i64, _i32, _vp, _vp, _vp, _i32,
                                             _i32, _vp, _vp, _vp, _vp, _i32, _vp, _sz, _vp]),
         "rhip_attn_workspace_bytes": (ctypes.c_int, [_P(RhipAttn), _i32, _P(_sz)]),
-        "rhip_attn_forward": (ctypes.c_int, [_P(RhipAttn), _vp, _vp, _vp, _vp, _vp, _vp, _sz,
-                                             _vp]),
+        "rhip_attn_forward": (ctypes.c_int, [_P(RhipAttn), _vp, _vp, _vp, _vp, _vp, _vp, _vp,
+                                             _sz, _vp]),
         "rhip_attn_backward": (ctypes.c_int, [_P(RhipAttn), _vp, _i64, _i64, _vp, _vp, _vp, _vp,
-                                              _vp, _vp, _vp, _vp, _vp, _sz, _vp]),
+                                              _vp, _vp, _vp, _vp, _vp, _vp, _sz, _vp]),
         "rhip_ln_workspace_bytes": (ctypes.c_int, [_i64, _i32, _P(_sz)]),
         "rhip_ln_forward": (ctypes.c_int, [_vp, _i64, _i64, _i32, _vp, _vp, ctypes.c_double, _vp,
                                            _vp, _vp, _i32, _vp]),
@@ -1015,25 +1015,28 @@ def _attn_ws(desc: RhipAttn, backward: bool, device) -> torch.Tensor:
 
 def attn_forward(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, q_offsets: torch.Tensor,
                  k_offsets: torch.Tensor, k_lengths: Optional[torch.Tensor] = None,
-                 causal: bool = False, scale: Optional[float] = None):
+                 causal: bool = False, scale: Optional[float] = None,
+                 rest: Optional[torch.Tensor] = None):
     """(out [n_q, heads, dim], lse [heads, n_q]) of attention over packed
-    sequences; offsets and lengths int32 on the device."""
+    sequences; offsets and lengths int32 on the device; rest (bf16, like out)
+    receives out's rounding error."""
     q, k, v = _dense_last(q), _dense_last(k), _dense_last(v)
     desc = _attn_desc(q, k, v, q_offsets, k_offsets, k_lengths, causal, scale)
     out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
     lse = torch.empty((q.shape[1], q.shape[0]), dtype=torch.float32, device=q.device)
     ws = _attn_ws(desc, False, q.device)
     _check(lib().rhip_attn_forward(ctypes.byref(desc), _ptr(q), _ptr(k), _ptr(v), _ptr(out),
-                                   _ptr(lse), _ptr(ws), ws.numel(), _stream(q.device)),
-           "rhip_attn_forward")
+                                   _ptr(rest), _ptr(lse), _ptr(ws), ws.numel(),
+                                   _stream(q.device)), "rhip_attn_forward")
     return out, lse
 
 
 def attn_backward(grad_out: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
                   out: torch.Tensor, lse: torch.Tensor, q_offsets: torch.Tensor,
                   k_offsets: torch.Tensor, k_lengths: Optional[torch.Tensor] = None,
-                  causal: bool = False, scale: Optional[float] = None):
-    """(grad_q, grad_k, grad_v) from the forward's out and lse."""
+                  causal: bool = False, scale: Optional[float] = None,
+                  rest: Optional[torch.Tensor] = None):
+    """(grad_q, grad_k, grad_v) from the forward's out, lse and rest."""
     q, k, v = _dense_last(q), _dense_last(k), _dense_last(v)
     grad_out = _dense_last(grad_out.to(q.dtype))
     desc = _attn_desc(q, k, v, q_offsets, k_offsets, k_lengths, causal, scale)
@@ -1043,8 +1046,9 @@ def attn_backward(grad_out: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: t
     ws = _attn_ws(desc, True, q.device)
     _check(lib().rhip_attn_backward(ctypes.byref(desc), _ptr(grad_out), grad_out.stride(0),
                                     grad_out.stride(1), _ptr(q), _ptr(k), _ptr(v), _ptr(out),
-                                    _ptr(lse), _ptr(gq), _ptr(gk), _ptr(gv), _ptr(ws),
-                                    ws.numel(), _stream(q.device)), "rhip_attn_backward")
+                                    _ptr(rest), _ptr(lse), _ptr(gq), _ptr(gk), _ptr(gv),
+                                    _ptr(ws), ws.numel(), _stream(q.device)),
+           "rhip_attn_backward")
     return gq, gk, gv
 
 

@@ -19,6 +19,8 @@ void check_attn(const rhip_attn *a) {
     throw Error(RHIP_ERR_UNSUPPORTED, "row counts must stay below 2^31 - 256");
   RHIP_CHECK_ARG(a->heads >= 1 && a->kv_heads >= 1 && a->heads % a->kv_heads == 0,
                  "heads must be a positive multiple of kv_heads");
+  if (a->n_q * (a->heads / a->kv_heads) > INT32_MAX - 256)
+    throw Error(RHIP_ERR_UNSUPPORTED, "query rows of a group must stay below 2^31 - 256");
   RHIP_CHECK_ARG(a->dim >= 1, "head width must be positive");
   if (a->dim > kAttnMaxDim)
     throw Error(RHIP_ERR_UNSUPPORTED, "head width must not exceed 128");
@@ -40,27 +42,51 @@ AttnArgs make_args(const rhip_attn *a) {
   return r;
 }
 
-// Whether every row starts 16-byte aligned and holds whole 16-byte chunks.
+// Whether every row starts 16-byte aligned and holds whole 16-byte chunks,
+// and a tile's offsets fit the buffer loads.
 bool vector_rows(const rhip_attn *a, std::initializer_list<const void *> ptrs,
                  std::initializer_list<int64_t> strides) {
   const int64_t e = a->dtype == RHIP_F32 ? 4 : 8;
   if (a->dim % e != 0)
     return false;
   for (const void *p : ptrs)
-    if (!aligned16(p))
+    if (p && !aligned16(p))
       return false;
   for (int64_t s : strides)
-    if (s % e != 0)
+    if (s % e != 0 || s < 0 || s > (int64_t(1) << 22))
       return false;
   return true;
 }
 
+struct FwdWs {
+  float *part_o, *part_ml;
+};
+FwdWs carve_forward(Carve &cv, const rhip_attn *a) {
+  FwdWs w{};
+  const int32_t splits =
+      attn_forward_splits(a->n_q, a->n_k, a->n_seq, a->heads, a->kv_heads);
+  if (splits > 1) {
+    const size_t rows = static_cast<size_t>(splits) * a->n_q * a->heads;
+    w.part_o = cv.take<float>(rows * a->dim);
+    w.part_ml = cv.take<float>(rows * 2);
+  }
+  return w;
+}
+
 struct BwdWs {
-  float *delta;
+  float2 *stat;
+  float *part_k, *part_v;
 };
 BwdWs carve_backward(Carve &cv, const rhip_attn *a) {
   BwdWs w{};
-  w.delta = cv.take<float>(static_cast<size_t>(std::max<int64_t>(1, a->n_q)) * a->heads);
+  w.stat = cv.take<float2>(static_cast<size_t>(std::max<int64_t>(1, a->n_q)) * a->heads);
+  const int32_t splits =
+      attn_backward_splits(a->n_q, a->n_k, a->n_seq, a->heads, a->kv_heads);
+  if (splits > 1) {
+    const size_t n = static_cast<size_t>(splits) * a->n_k * a->kv_heads * a->dim;
+    w.part_k = cv.take<float>(n);
+    w.part_v = cv.take<float>(n);
+  }
   return w;
 }
 
@@ -74,23 +100,28 @@ extern "C" int rhip_attn_workspace_bytes(const rhip_attn *attn, int32_t backward
     Carve cv(nullptr, 0);
     if (backward)
       carve_backward(cv, attn);
+    else
+      carve_forward(cv, attn);
     *bytes = cv.used + 256;
   });
 }
 
 extern "C" int rhip_attn_forward(const rhip_attn *attn, const void *q, const void *k,
-                                 const void *v, void *out, float *lse, void *workspace,
-                                 size_t ws_bytes, hipStream_t stream) {
+                                 const void *v, void *out, void *out_rest, float *lse,
+                                 void *workspace, size_t ws_bytes, hipStream_t stream) {
   return guarded([&] {
     check_attn(attn);
     if (attn->n_q == 0)
       return;
     RHIP_CHECK_ARG(q && out, "q and out are required");
     RHIP_CHECK_ARG(attn->n_k == 0 || (k && v), "k and v are required");
-    RHIP_CHECK_ARG(workspace != nullptr || ws_bytes == 0, "workspace is null");
+    RHIP_CHECK_ARG(workspace != nullptr, "workspace is required");
     AttnArgs a = make_args(attn);
-    a.q = q, a.k = k, a.v = v, a.o = out, a.lse = lse;
-    const bool vec = vector_rows(attn, {q, k, v, out},
+    Carve cv(workspace, ws_bytes);
+    const FwdWs w = carve_forward(cv, attn);
+    a.q = q, a.k = k, a.v = v, a.o = out, a.rest = out_rest, a.lse = lse;
+    a.part_o = w.part_o, a.part_ml = w.part_ml;
+    const bool vec = vector_rows(attn, {q, k, v, out, out_rest},
                                  {attn->q_row, attn->q_head, attn->k_row, attn->k_head,
                                   attn->v_row, attn->v_head});
     attn_forward_run(a, attn->dtype, vec, stream);
@@ -100,7 +131,7 @@ extern "C" int rhip_attn_forward(const rhip_attn *attn, const void *q, const voi
 extern "C" int rhip_attn_backward(const rhip_attn *attn, const void *grad_out,
                                   int64_t grad_out_row, int64_t grad_out_head, const void *q,
                                   const void *k, const void *v, const void *out,
-                                  const float *lse, void *grad_q, void *grad_k, void *grad_v,
+                                  const void *out_rest, const float *lse, void *grad_q, void *grad_k, void *grad_v,
                                   void *workspace, size_t ws_bytes, hipStream_t stream) {
   return guarded([&] {
     check_attn(attn);
@@ -118,9 +149,11 @@ extern "C" int rhip_attn_backward(const rhip_attn *attn, const void *grad_out,
     const BwdWs w = carve_backward(cv, attn);
     a.q = q, a.k = k, a.v = v, a.o = const_cast<void *>(out), a.lse = const_cast<float *>(lse);
     a.go = grad_out, a.go_row = grad_out_row, a.go_head = grad_out_head;
-    a.gq = grad_q, a.gk = grad_k, a.gv = grad_v, a.delta = w.delta;
+    a.rest = const_cast<void *>(out_rest);
+    a.gq = grad_q, a.gk = grad_k, a.gv = grad_v;
+    a.stat = w.stat, a.part_k = w.part_k, a.part_v = w.part_v;
     const bool vec = vector_rows(
-        attn, {q, k, v, out, grad_out, grad_q, grad_k, grad_v},
+        attn, {q, k, v, out, out_rest, grad_out, grad_q, grad_k, grad_v},
         {attn->q_row, attn->q_head, attn->k_row, attn->k_head, attn->v_row, attn->v_head,
          grad_out_row, grad_out_head});
     attn_backward_run(a, attn->dtype, vec, stream);

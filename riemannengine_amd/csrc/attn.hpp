@@ -10,6 +10,12 @@ namespace rhip {
 
 void attn_forward_run(const AttnArgs &a, int32_t dtype, bool vec, hipStream_t stream);
 void attn_backward_run(const AttnArgs &a, int32_t dtype, bool vec, hipStream_t stream);
+// Workgroups that share one tile of query rows (forward) or of keys
+// (backward): their partial sums are the workspace.
+int32_t attn_forward_splits(int64_t n_q, int64_t n_k, int32_t n_seq, int32_t heads,
+                            int32_t kv_heads);
+int32_t attn_backward_splits(int64_t n_q, int64_t n_k, int32_t n_seq, int32_t heads,
+                             int32_t kv_heads);
 
 // f(T{}, head width of the variant, whether rows load in 16-byte chunks).
 // Rows that do not (a width or a stride that is no multiple of 16 bytes, an

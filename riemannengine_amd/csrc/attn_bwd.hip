@@ -1,80 +1,272 @@
 // Attention over packed sequences on gfx950, backward. With p = softmax rows
 // (recomputed from lse), dp = do v^T and delta = rowsum(do o):
 //   ds = p (dp - delta),  dq = scale ds k,  dk = scale ds^T q,  dv = p^T do.
-// Two kernels: one over query rows (dq, and delta for the other), one over
-// keys (dk and dv, summed over the query heads of a group inside the
-// workgroup). Each gradient row is summed by one wave in a fixed order, so
-// results do not change from run to run; the price is that scores and dp are
-// computed twice (7 products instead of 5).
+// Two kernels: one over query rows (dq, and each row's statistics for the
+// other), one over keys (dk and dv, summed over the query heads of a group
+// inside the workgroup). Each gradient row is summed by one workgroup in a
+// fixed order, so results do not change from run to run; the price is that
+// scores and dp are computed twice (7 products instead of 5).
+//
+// Both have the forward's two shapes: `shared`, 128 rows (keys) per
+// workgroup, whose four waves read the same tiles of the other side, and
+// `split`, 32 rows (keys), whose waves each take every fourth 32-row tile and
+// add their sums at the end; the keys' kernel may also be split over
+// workgroups, whose partial sums a last kernel adds.
 #include "attn.hpp"
 
 namespace rhip {
 namespace {
 
 constexpr int kBwdThreads = 256;
-constexpr int kBwdRows = 128; // query rows (dq) or keys (dk, dv) per workgroup
+constexpr int kBwdWaves = kBwdThreads / kWave;
+constexpr int kSharedRows = 128, kSplitRows = 32;
+// Workgroups below which the split shape is taken, and how many it aims for.
+constexpr int64_t kFewWorkgroups = 256, kSplitTarget = 1024;
+constexpr int kMaxSplits = 32;
 
-// Tile size over the other axis. fp32 at full width holds 32-row tiles.
-template <typename T> constexpr int kBwdTile = sizeof(T) == 2 ? 64 : 32;
+template <typename T, int DP, bool SPLIT, int SUMS> struct BwdShape {
+  static constexpr int kRows = SPLIT ? kSplitRows : kSharedRows;
+  static constexpr int kBN = SPLIT || (sizeof(T) == 4 && DP == 128) ? 32 : 64;
+  static constexpr int kStreams = SPLIT ? kBwdWaves : 1;
+  static constexpr int kTileBytes = kBN * DP * sizeof(T);
+  static constexpr int kStatBytes = kBN * 8; // (lse2, -delta) of a tile's rows
+  static constexpr int kBufBytes = 2 * kTileBytes + kStatBytes;
+  static constexpr int kBuffers = kStreams * 2 * kBufBytes <= 160 * 1024 ? 2 : 1;
+  static constexpr int kJoinRow = DP + 4; // floats per row of the joined sums
+  static constexpr int kJoinBytes =
+      SPLIT ? kBwdWaves * 32 * kJoinRow * static_cast<int>(sizeof(float)) : 0;
+  static constexpr int kStageBytes = kStreams * kBuffers * kBufBytes;
+  static constexpr int kLds = kStageBytes > kJoinBytes ? kStageBytes : kJoinBytes;
+};
 
-// Workgroup -> (tile, head) as in the forward: head-major runs per XCD.
+// Workgroup -> (tile, head, split) as in the forward: head-major runs per XCD.
 // `last_first`: the tiles with the most work come first under a causal mask.
-__device__ __forceinline__ bool bwd_item(int32_t tiles, int32_t heads, bool last_first,
-                                         int32_t &tile, int32_t &head) {
-  const uint32_t total = static_cast<uint32_t>(tiles) * heads;
+__device__ __forceinline__ bool bwd_item(const AttnArgs &a, bool last_first, int32_t &tile,
+                                         int32_t &kv, int32_t &split) {
+  const uint32_t total = static_cast<uint32_t>(a.tiles) * a.kv_heads * a.splits;
   const uint32_t per = (total + kXcds - 1) / kXcds;
   const uint32_t i = (blockIdx.x % kXcds) * per + blockIdx.x / kXcds;
-  if (i >= total || blockIdx.x / kXcds >= per)
+  if (i >= total)
     return false;
-  head = i / tiles;
-  tile = i % tiles;
+  split = i % a.splits;
+  const uint32_t j = i / a.splits;
+  kv = j / a.tiles;
+  tile = j % a.tiles;
   if (last_first)
-    tile = tiles - 1 - tile;
+    tile = a.tiles - 1 - tile;
   return true;
 }
 
-// dq of 128 query rows of one head, 32 per wave, over the keys; also delta.
-// Blocks are transposed as in the forward (S^T = K Q^T, dP^T = V dO^T), so
-// dS^T is the right operand of dQ^T = K^T dS^T as it lies.
-template <typename T, int DP, bool VEC>
+// The first query row that sees key j, and the keys that row i sees.
+__device__ __forceinline__ int32_t first_row(const AttnArgs &a, const AttnSeq &sq, int64_t j) {
+  const int64_t i = a.causal ? j - (static_cast<int64_t>(sq.lk) - sq.lq) : 0;
+  return static_cast<int32_t>(i < 0 ? 0 : (i > sq.lq ? sq.lq : i));
+}
+__device__ __forceinline__ int32_t keys_seen(const AttnArgs &a, const AttnSeq &sq, int64_t i) {
+  const int64_t n =
+      a.causal ? min<int64_t>(sq.lk, i + static_cast<int64_t>(sq.lk) - sq.lq + 1) : sq.lk;
+  return static_cast<int32_t>(n < 0 ? 0 : n);
+}
+
+template <typename T> __device__ __forceinline__ float dot(const T *x, const T *y, int32_t dim) {
+  float s = 0.f;
+  for (int d = 0; d < dim; ++d)
+    s = fmaf(to_f32(x[d]), to_f32(y[d]), s);
+  return s;
+}
+
+// The places a gradient row is read and computed from.
+template <typename T> struct Rows {
+  const T *q, *go, *k, *v;
+};
+template <typename T>
+__device__ __forceinline__ Rows<T> rows_of(const AttnArgs &a, const AttnSeq &sq, int head) {
+  const int kv = head / a.group;
+  return {static_cast<const T *>(a.q) + sq.q0 * a.q_row + head * a.q_head,
+          static_cast<const T *>(a.go) + sq.q0 * a.go_row + head * a.go_head,
+          static_cast<const T *>(a.k) + sq.k0 * a.k_row + kv * a.k_head,
+          static_cast<const T *>(a.v) + sq.k0 * a.v_row + kv * a.v_head};
+}
+
+// A gradient row by its definition, reading only what it depends on, where
+// the tiles' sums came out not finite under a causal mask (a masked entry's
+// zero times a value that is not finite). One wave; lane l returns elements l
+// and l + 64 of dq (without scale).
+template <typename T>
+__device__ void exact_dq(const AttnArgs &a, const AttnSeq &sq, int32_t i, int head, float &g0,
+                         float &g1) {
+  const Rows<T> p = rows_of<T>(a, sq, head);
+  const int lane = lane_id();
+  const float2 st = a.stat[static_cast<int64_t>(head) * a.n_q + sq.q0 + i];
+  const int32_t lim = keys_seen(a, sq, i);
+  g0 = g1 = 0.f;
+  for (int32_t j0 = 0; j0 < lim; j0 += kWave) {
+    float ds = 0.f;
+    if (j0 + lane < lim) {
+      const T *kj = p.k + static_cast<int64_t>(j0 + lane) * a.k_row;
+      const T *vj = p.v + static_cast<int64_t>(j0 + lane) * a.v_row;
+      const float s = dot(p.q + i * a.q_row, kj, a.dim);
+      ds = exp2_fast(fmaf(s, a.c, -st.x)) * (dot(p.go + i * a.go_row, vj, a.dim) + st.y);
+    }
+    for (int e = 0; e < min(kWave, lim - j0); ++e) {
+      const float de = __shfl(ds, e, kWave);
+      const T *kj = p.k + static_cast<int64_t>(j0 + e) * a.k_row;
+      if (lane < a.dim)
+        g0 = fmaf(de, to_f32(kj[lane]), g0);
+      if (lane + kWave < a.dim)
+        g1 = fmaf(de, to_f32(kj[lane + kWave]), g1);
+    }
+  }
+}
+// The same for dk (without scale) and dv of key j.
+template <typename T>
+__device__ void exact_dkv(const AttnArgs &a, const AttnSeq &sq, int32_t j, int kv, float (&gk)[2],
+                          float (&gv)[2]) {
+  const int lane = lane_id();
+  gk[0] = gk[1] = gv[0] = gv[1] = 0.f;
+  for (int head = kv * a.group; head < (kv + 1) * a.group; ++head) {
+    const Rows<T> p = rows_of<T>(a, sq, head);
+    const T *kj = p.k + static_cast<int64_t>(j) * a.k_row;
+    const T *vj = p.v + static_cast<int64_t>(j) * a.v_row;
+    for (int32_t i0 = first_row(a, sq, j); i0 < sq.lq; i0 += kWave) {
+      float pe = 0.f, ds = 0.f;
+      const int64_t i = i0 + lane;
+      if (i < sq.lq) {
+        const float2 st = a.stat[static_cast<int64_t>(head) * a.n_q + sq.q0 + i];
+        pe = exp2_fast(fmaf(dot(p.q + i * a.q_row, kj, a.dim), a.c, -st.x));
+        ds = pe * (dot(p.go + i * a.go_row, vj, a.dim) + st.y);
+      }
+      for (int e = 0; e < min(kWave, sq.lq - i0); ++e) {
+        const float p1 = __shfl(pe, e, kWave), d1 = __shfl(ds, e, kWave);
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          const int d = lane + u * kWave;
+          if (d < a.dim) {
+            gv[u] = fmaf(p1, to_f32(p.go[static_cast<int64_t>(i0 + e) * a.go_row + d]), gv[u]);
+            gk[u] = fmaf(d1, to_f32(p.q[static_cast<int64_t>(i0 + e) * a.q_row + d]), gk[u]);
+          }
+        }
+      }
+    }
+  }
+}
+
+template <typename T>
+__device__ __forceinline__ void put2(T *p, int dim, float v0, float v1, float mul) {
+  const int lane = lane_id();
+  if (lane < dim)
+    p[lane] = from_f32<T>(v0 * mul);
+  if (lane + kWave < dim)
+    p[lane + kWave] = from_f32<T>(v1 * mul);
+}
+
+// One wave writes a dq row; lane l holds elements l and l + 64 of its sum.
+template <typename T>
+__device__ void finish_dq(const AttnArgs &a, const AttnSeq &sq, int32_t i, int head, float g0,
+                          float g1) {
+  if (a.causal && __any(!isfinite(g0) || !isfinite(g1)))
+    exact_dq<T>(a, sq, i, head, g0, g1);
+  put2(static_cast<T *>(a.gq) +
+           ((sq.q0 + static_cast<int64_t>(i)) * a.heads + head) * a.dim,
+       a.dim, g0, g1, a.scale);
+}
+template <typename T>
+__device__ void finish_dkv(const AttnArgs &a, const AttnSeq &sq, int32_t j, int kv,
+                           float (&gk)[2], float (&gv)[2]) {
+  if (a.causal && j < sq.lk &&
+      __any(!isfinite(gk[0]) || !isfinite(gk[1]) || !isfinite(gv[0]) || !isfinite(gv[1])))
+    exact_dkv<T>(a, sq, j, kv, gk, gv);
+  const int64_t at = ((sq.k0 + static_cast<int64_t>(j)) * a.kv_heads + kv) * a.dim;
+  put2(static_cast<T *>(a.gk) + at, a.dim, gk[0], gk[1], a.scale);
+  put2(static_cast<T *>(a.gv) + at, a.dim, gv[0], gv[1], 1.f);
+}
+
+// The columns a wave's lanes hold, as 32 rows of floats in LDS.
+template <int DB>
+__device__ __forceinline__ void spill_columns(float *rows, int row_floats, const v16f (&acc)[DB]) {
+  const int lane = lane_id(), half = lane >> 5;
+  float *mine = rows + (lane & 31) * row_floats;
+#pragma unroll
+  for (int db = 0; db < DB; ++db)
+#pragma unroll
+    for (int g = 0; g < 4; ++g)
+      *reinterpret_cast<v4f *>(mine + 32 * db + 8 * g + 4 * half) =
+          v4f{acc[db][4 * g], acc[db][4 * g + 1], acc[db][4 * g + 2], acc[db][4 * g + 3]};
+}
+// Elements lane and lane + 64 of row r, summed over the waves in order.
+template <int DP>
+__device__ __forceinline__ void join_row(const float *rows, int row_floats, int r, float &v0,
+                                         float &v1) {
+  const int lane = lane_id();
+  v0 = v1 = 0.f;
+#pragma unroll
+  for (int i = 0; i < kBwdWaves; ++i) {
+    const float *src = rows + (i * 32 + r) * row_floats;
+    if (lane < DP)
+      v0 += src[lane];
+    if (DP > kWave)
+      v1 += src[lane + kWave];
+  }
+}
+
+// dq of 128 (32) packed query rows of one key head's group over the keys;
+// also the rows' statistics. Blocks are transposed as in the forward (S^T = K
+// Q^T, dP^T = V dO^T), so dS^T is the right operand of dQ^T = K^T dS^T as it
+// lies. dP's sums start at -delta.
+template <typename T, int DP, bool VEC, bool SPLIT>
 __global__ __launch_bounds__(kBwdThreads, sizeof(T) == 4 && DP == 128 ? 1 : 2) void
 attn_dq_kernel(AttnArgs a) {
+  using Shape = BwdShape<T, DP, SPLIT, 1>;
   using Tile = AttnTile<T, DP>;
   using Frag = typename Tile::Frag;
-  constexpr int kBN = kBwdTile<T>, kB = kBN / 32;
-  constexpr int kBytes = kBN * Tile::C * 16;
-  constexpr int kPer = kBN * Tile::C / kBwdThreads;
-  __shared__ alignas(16) char lds[2][2][kBytes];
+  constexpr int kBN = Shape::kBN, kB = kBN / 32;
+  using Stream = TileStream<T, DP, kBN, SPLIT ? kWave : kBwdThreads, VEC>;
+  __shared__ alignas(16) char lds[Shape::kLds];
 
-  int32_t t, head;
-  if (!bwd_item(a.tiles, a.heads, true, t, head))
+  int32_t t, kv, split;
+  if (!bwd_item(a, true, t, kv, split))
     return;
-  const AttnSeq sq = query_tile(a, kBwdRows, 1, t);
-  const int32_t row0 = sq.tile * kBwdRows;
-  if (row0 >= sq.lq)
+  const AttnSeq sq = query_tile(a, Shape::kRows, a.group, t);
+  const int32_t n_rows = sq.lq * a.group, row0 = sq.tile * Shape::kRows;
+  if (row0 >= n_rows)
     return;
-  const int lane = lane_id(), w = threadIdx.x / kWave, half = lane >> 5;
-  const int32_t row = row0 + w * 32 + (lane & 31);
-  const bool row_ok = row < sq.lq;
-  const int64_t shift = sq.lk - sq.lq;
-  auto sees = [&](int64_t r) {
-    const int64_t n = a.causal ? min<int64_t>(sq.lk, r + shift + 1) : sq.lk;
-    return static_cast<int32_t>(n < 0 ? 0 : n);
-  };
+  const int lane = lane_id(), half = lane >> 5;
+  const int w = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+  const int32_t wave0 = row0 + (SPLIT ? 0 : w * 32);
+  const int32_t row = wave0 + (lane & 31);
+  const bool row_ok = row < n_rows;
+  const int32_t rc = min(row, n_rows - 1);
+  const int32_t qi = rc / a.group;
+  const int head = kv * a.group + rc % a.group;
+  auto sees = [&](int32_t r) { return keys_seen(a, sq, r / a.group); };
   const int32_t lim = row_ok ? sees(row) : 0;
-  const int32_t wg_lim = sees(min(row0 + kBwdRows, sq.lq) - 1);
-  const int32_t wave_lim = row0 + w * 32 < sq.lq ? sees(min(row0 + w * 32 + 32, sq.lq) - 1) : 0;
-  const int32_t wave_full = row0 + w * 32 < sq.lq ? sees(row0 + w * 32) : 0;
-  const int32_t n_tiles = a.gq ? (wg_lim + kBN - 1) / kBN : 0; // else delta alone
+  const int32_t wg_lim = sees(min(row0 + Shape::kRows, n_rows) - 1);
+  const int32_t wave_lim = wave0 < n_rows ? sees(min(wave0 + 32, n_rows) - 1) : 0;
+  const int32_t wave_full = wave0 < n_rows ? sees(wave0) : 0;
+  const int32_t kt1 = a.gq ? (wg_lim + kBN - 1) / kBN : 0; // else statistics alone
+  const int32_t first = SPLIT ? w : 0, step = SPLIT ? kBwdWaves : 1;
 
-  const int kv = head / a.group;
   const T *kp = static_cast<const T *>(a.k) + sq.k0 * a.k_row + kv * a.k_head;
   const T *vp = static_cast<const T *>(a.v) + sq.k0 * a.v_row + kv * a.v_head;
-  const int64_t gr = sq.q0 + static_cast<int64_t>(row);
+  Stream ks, vs;
+  ks.init(a.k_row, a.dim);
+  vs.init(a.v_row, a.dim);
+  char *stage = lds + (SPLIT ? w : 0) * Shape::kBuffers * Shape::kBufBytes;
+  auto issue = [&](int32_t kt, int buf) {
+    char *to = stage + buf * Shape::kBufBytes;
+    ks.issue(to, kp + static_cast<int64_t>(kt) * kBN * a.k_row, a.k_row, sq.lk - kt * kBN,
+             a.dim);
+    vs.issue(to + Shape::kTileBytes, vp + static_cast<int64_t>(kt) * kBN * a.v_row, a.v_row,
+             sq.lk - kt * kBN, a.dim);
+  };
+  if (first < kt1)
+    issue(first, 0);
+
+  const int64_t gr = sq.q0 + static_cast<int64_t>(qi);
   const T *qp = static_cast<const T *>(a.q) + gr * a.q_row + head * a.q_head;
   const T *gp = static_cast<const T *>(a.go) + gr * a.go_row + head * a.go_head;
   const T *op = static_cast<const T *>(a.o) + (gr * a.heads + head) * a.dim;
-
+  const T *rp = static_cast<const T *>(a.rest) + (gr * a.heads + head) * a.dim;
   Frag qf[Tile::kSteps], gf[Tile::kSteps];
   float delta = 0.f;
 #pragma unroll
@@ -86,111 +278,169 @@ attn_dq_kernel(AttnArgs a) {
 #pragma unroll
     for (int e = 0; e < Tile::E; ++e)
       delta = fmaf(static_cast<float>(gf[s][e]), static_cast<float>(of[e]), delta);
+    if (sizeof(T) == 2 && a.rest) {
+      const Frag rf = __builtin_bit_cast(Frag, Tile::template chunk<VEC>(rp, c, a.dim, row_ok));
+#pragma unroll
+      for (int e = 0; e < Tile::E; ++e)
+        delta = fmaf(static_cast<float>(gf[s][e]), static_cast<float>(rf[e]), delta);
+    }
   }
   delta = pair_sum(delta);
-  const int64_t li = static_cast<int64_t>(head) * a.n_q + gr;
   float lse2 = 0.f; // log2 of the softmax's denominator
   if (row_ok) {
+    const int64_t li = static_cast<int64_t>(head) * a.n_q + gr;
     lse2 = a.lse[li] * kLog2e;
-    if (half == 0)
-      a.delta[li] = delta;
+    if (half == 0 && (!SPLIT || w == 0))
+      a.stat[li] = make_float2(lse2, -delta);
   }
 
-  uint4 rk[kPer], rv[kPer];
-  auto load_tile = [&](int32_t kt) {
-#pragma unroll
-    for (int i = 0; i < kPer; ++i) {
-      const int idx = threadIdx.x + i * kBwdThreads, r = idx / Tile::C, c = idx % Tile::C;
-      const int32_t j = kt * kBN + r;
-      const bool ok = j < sq.lk;
-      rk[i] = Tile::template chunk<VEC>(kp + j * a.k_row, c, a.dim, ok);
-      rv[i] = Tile::template chunk<VEC>(vp + j * a.v_row, c, a.dim, ok);
-    }
-  };
-  v16f dq[Tile::kDBlocks];
+  v16f dq[Tile::kDBlocks], dp0;
 #pragma unroll
   for (int db = 0; db < Tile::kDBlocks; ++db)
     dq[db] = v16f{};
+#pragma unroll
+  for (int r = 0; r < 16; ++r)
+    dp0[r] = -delta;
 
-  if (n_tiles > 0)
-    load_tile(0);
-  for (int32_t kt = 0; kt < n_tiles; ++kt) {
-    char *lk = lds[kt & 1][0], *lv = lds[kt & 1][1];
-#pragma unroll
-    for (int i = 0; i < kPer; ++i) {
-      const int idx = threadIdx.x + i * kBwdThreads, r = idx / Tile::C, c = idx % Tile::C;
-      *reinterpret_cast<uint4 *>(Tile::at(lk, r, c)) = rk[i];
-      *reinterpret_cast<uint4 *>(Tile::at(lv, r, c)) = rv[i];
-    }
-    if (kt + 1 < n_tiles)
-      load_tile(kt + 1);
-    __syncthreads(); // one per tile, as in the forward
+  int buf = 0;
+  for (int32_t kt = first; kt < kt1; kt += step) {
+    wait_stream(); // as in the forward
+    if constexpr (!SPLIT)
+      __syncthreads();
+    char *lk = stage + buf * Shape::kBufBytes, *lv = lk + Shape::kTileBytes;
+    if (Shape::kBuffers == 2 && kt + step < kt1)
+      issue(kt + step, buf ^ 1);
     const int32_t j0 = kt * kBN;
-    if (j0 >= wave_lim)
-      continue;
-    const bool masked = j0 + kBN > wave_full;
+    if (SPLIT || j0 < wave_lim) {
+      const bool masked = j0 + kBN > wave_full;
 #pragma unroll
-    for (int b = 0; b < kB; ++b) {
-      v16f s{}, dp{};
-      Tile::row_product(lk, 32 * b, qf, s);
-      Tile::row_product(lv, 32 * b, gf, dp);
-#pragma unroll
-      for (int r = 0; r < 16; ++r)
-        s[r] = exp2_fast(fmaf(s[r], a.c, -lse2)) * (dp[r] - delta);
-      if (masked) {
+      for (int b = 0; b < kB; ++b) {
+        v16f s{}, dp = dp0;
+        Tile::row_product(lk, 32 * b, qf, s);
+        Tile::row_product(lv, 32 * b, gf, dp);
 #pragma unroll
         for (int r = 0; r < 16; ++r)
-          s[r] = j0 + 32 * b + block_row(r) < lim ? s[r] : 0.f;
+          s[r] = exp2_fast(fmaf(s[r], a.c, -lse2)) * dp[r];
+        if (masked) {
+#pragma unroll
+          for (int r = 0; r < 16; ++r)
+            s[r] = j0 + 32 * b + block_row(r) < lim ? s[r] : 0.f;
+        }
+        typename Tile::Block ds;
+        Tile::pack(s, ds);
+        Tile::col_product(lk, 32 * b, ds, dq);
       }
-      typename Tile::Block ds;
-      Tile::pack(s, ds);
-      Tile::col_product(lk, 32 * b, ds, dq);
+    }
+    if (Shape::kBuffers == 2) {
+      buf ^= 1;
+    } else if (kt + step < kt1) {
+      wait_stream();
+      if constexpr (!SPLIT)
+        __syncthreads();
+      issue(kt + step, 0);
     }
   }
-  if (row_ok && a.gq)
-    Tile::template store_column<VEC>(
-        static_cast<T *>(a.gq) + (gr * a.heads + head) * a.dim, a.dim, a.scale, dq);
+  if (!a.gq)
+    return;
+  if constexpr (!SPLIT) {
+    bool bad = false;
+    if (a.causal && row_ok) {
+#pragma unroll
+      for (int db = 0; db < Tile::kDBlocks; ++db)
+#pragma unroll
+        for (int r = 0; r < 16; ++r)
+          bad |= !isfinite(dq[db][r]);
+    }
+    uint64_t redo = __ballot(bad);
+    redo = (redo | redo >> 32) & 0xffffffffull;
+    if (row_ok && !((redo >> (lane & 31)) & 1))
+      Tile::template store_column<VEC>(
+          static_cast<T *>(a.gq) + (gr * a.heads + head) * a.dim, a.dim, a.scale, dq);
+    while (redo) {
+      const int i = __ffsll(static_cast<unsigned long long>(redo)) - 1;
+      redo &= redo - 1;
+      finish_dq<T>(a, sq, __shfl(qi, i, kWave), __shfl(head, i, kWave), NAN, NAN);
+    }
+  } else {
+    __syncthreads(); // every wave is past its tiles
+    float *join = reinterpret_cast<float *>(lds);
+    spill_columns(join + w * 32 * Shape::kJoinRow, Shape::kJoinRow, dq);
+    __syncthreads();
+    for (int r = w; r < 32 && row0 + r < n_rows; r += kBwdWaves) {
+      float g0, g1;
+      join_row<DP>(join, Shape::kJoinRow, r, g0, g1);
+      finish_dq<T>(a, sq, (row0 + r) / a.group, kv * a.group + (row0 + r) % a.group, g0, g1);
+    }
+  }
 }
 
-// dk and dv of 128 keys of one key head, 32 per wave, over the query rows of
-// every head of its group. A lane holds one key's column (S = Q K^T, dP = dO
-// V^T), so P and dS are the right operands of dV^T = dO^T P and dK^T = Q^T dS
-// as they lie.
-template <typename T, int DP, bool VEC>
-__global__ __launch_bounds__(kBwdThreads, DP == 128 ? 1 : 2) void
+// dk and dv of 128 (32) keys of one key head over the query rows of every
+// head of its group. A lane holds one key's column (S = Q K^T, dP = dO V^T),
+// so P and dS are the right operands of dV^T = dO^T P and dK^T = Q^T dS as
+// they lie.
+template <typename T, int DP, bool VEC, bool SPLIT>
+__global__ __launch_bounds__(kBwdThreads, (sizeof(T) == 4 ? DP >= 64 : DP == 128) ? 1 : 2) void
 attn_dkv_kernel(AttnArgs a) {
+  using Shape = BwdShape<T, DP, SPLIT, 2>;
   using Tile = AttnTile<T, DP>;
   using Frag = typename Tile::Frag;
-  constexpr int kBM = kBwdTile<T>, kB = kBM / 32;
-  constexpr int kBytes = kBM * Tile::C * 16;
-  constexpr int kPer = kBM * Tile::C / kBwdThreads;
-  __shared__ alignas(16) char lds[2][2][kBytes];
-  __shared__ alignas(16) float rows[2][2][kBM]; // lse2 and delta of the tile's rows
+  constexpr int kBM = Shape::kBN, kB = kBM / 32;
+  using Stream = TileStream<T, DP, kBM, SPLIT ? kWave : kBwdThreads, VEC>;
+  __shared__ alignas(16) char lds[Shape::kLds];
 
-  int32_t t, kv;
-  if (!bwd_item(a.tiles, a.kv_heads, false, t, kv))
+  int32_t t, kv, split;
+  if (!bwd_item(a, false, t, kv, split))
     return;
   int32_t room;
-  const AttnSeq sq = key_tile(a, kBwdRows, t, room);
-  const int32_t key0 = sq.tile * kBwdRows;
+  const AttnSeq sq = key_tile(a, Shape::kRows, t, room);
+  const int32_t key0 = sq.tile * Shape::kRows;
   if (key0 >= room)
     return;
-  const int lane = lane_id(), w = threadIdx.x / kWave, half = lane >> 5;
-  const int32_t key = key0 + w * 32 + (lane & 31);
+  const int lane = lane_id(), half = lane >> 5;
+  const int w = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+  const int32_t wave0 = key0 + (SPLIT ? 0 : w * 32);
+  const int32_t key = wave0 + (lane & 31);
   const bool key_ok = key < sq.lk;
-  const int64_t shift = sq.lk - sq.lq;
-  // the first row that sees a key
-  auto first_row = [&](int64_t j) {
-    const int64_t i = a.causal ? j - shift : 0;
-    return static_cast<int32_t>(i < 0 ? 0 : (i > sq.lq ? sq.lq : i));
-  };
-  const int32_t lo = first_row(key);
-  const int32_t wave_lo = first_row(key0 + w * 32);         // no earlier row sees any
-  const int32_t wave_full = first_row(key0 + w * 32 + 31);  // every later row sees all
-  const int32_t it0 = first_row(key0) / kBM;
-  // tiles of query rows from the first that sees a key, for each head
+  const int32_t lo = first_row(a, sq, key);
+  const int32_t wave_lo = first_row(a, sq, wave0);         // no earlier row sees any
+  const int32_t wave_full = first_row(a, sq, wave0 + 31);  // every later row sees all
+  const int32_t it0 = first_row(a, sq, key0) / kBM;
+  // tiles of query rows from the first that sees a key, for each head; this
+  // workgroup's part of them
   const int32_t per_head = key0 < sq.lk ? max((sq.lq + kBM - 1) / kBM - it0, 0) : 0;
-  const int32_t n_tiles = per_head * a.group;
+  int32_t n0 = 0, n1 = per_head * a.group;
+  if (SPLIT && a.splits > 1) {
+    const int32_t per = (n1 + a.splits - 1) / a.splits;
+    n0 = min(split * per, n1);
+    n1 = min(n0 + per, n1);
+  }
+  const int32_t first = n0 + (SPLIT ? w : 0), step = SPLIT ? kBwdWaves : 1;
+
+  Stream qs, gs;
+  qs.init(a.q_row, a.dim);
+  gs.init(a.go_row, a.dim);
+  char *stage = lds + (SPLIT ? w : 0) * Shape::kBuffers * Shape::kBufBytes;
+  auto issue = [&](int32_t n, int buf) {
+    const int h = n / per_head, head = kv * a.group + h;
+    const int32_t i0 = (it0 + n - h * per_head) * kBM;
+    const int64_t r0 = sq.q0 + static_cast<int64_t>(i0);
+    char *to = stage + buf * Shape::kBufBytes;
+    qs.issue(to, static_cast<const T *>(a.q) + r0 * a.q_row + head * a.q_head, a.q_row,
+             sq.lq - i0, a.dim);
+    gs.issue(to + Shape::kTileBytes,
+             static_cast<const T *>(a.go) + r0 * a.go_row + head * a.go_head, a.go_row,
+             sq.lq - i0, a.dim);
+    // (lse2, -delta) of the tile's rows: 64 floats per wave
+    const __amdgpu_buffer_rsrc_t rsrc =
+        buf_rsrc(a.stat + static_cast<int64_t>(head) * a.n_q + r0,
+                 static_cast<int64_t>(min(sq.lq - i0, kBM)) * 8);
+    if (SPLIT)
+      dma4(rsrc, lds_address(to + 2 * Shape::kTileBytes), lane * 4);
+    else if (w * 32 < kBM)
+      dma4(rsrc, lds_address(to + 2 * Shape::kTileBytes + w * 256), threadIdx.x * 4);
+  };
+  if (first < n1)
+    issue(first, 0);
 
   const int64_t gk = sq.k0 + static_cast<int64_t>(key);
   const T *kp = static_cast<const T *>(a.k) + gk * a.k_row + kv * a.k_head;
@@ -202,113 +452,224 @@ attn_dkv_kernel(AttnArgs a) {
     kf[s] = __builtin_bit_cast(Frag, Tile::template chunk<VEC>(kp, c, a.dim, key_ok));
     vf[s] = __builtin_bit_cast(Frag, Tile::template chunk<VEC>(vp, c, a.dim, key_ok));
   }
-
-  uint4 rq[kPer], rg[kPer];
-  float rs = 0.f;
-  auto load_tile = [&](int32_t n) {
-    const int head = kv * a.group + n / per_head;
-    const int32_t i0 = (it0 + n % per_head) * kBM;
-    const T *qp = static_cast<const T *>(a.q) + sq.q0 * a.q_row + head * a.q_head;
-    const T *gp = static_cast<const T *>(a.go) + sq.q0 * a.go_row + head * a.go_head;
-#pragma unroll
-    for (int i = 0; i < kPer; ++i) {
-      const int idx = threadIdx.x + i * kBwdThreads, r = idx / Tile::C, c = idx % Tile::C;
-      const int32_t qi = i0 + r;
-      rq[i] = Tile::template chunk<VEC>(qp + qi * a.q_row, c, a.dim, qi < sq.lq);
-      rg[i] = Tile::template chunk<VEC>(gp + qi * a.go_row, c, a.dim, qi < sq.lq);
-    }
-    if (threadIdx.x < 2 * kBM) {
-      const int r = threadIdx.x % kBM;
-      const float *src = threadIdx.x < kBM ? a.lse : a.delta;
-      rs = i0 + r < sq.lq ? src[static_cast<int64_t>(head) * a.n_q + sq.q0 + i0 + r] : 0.f;
-      if (threadIdx.x < kBM)
-        rs *= kLog2e;
-    }
-  };
-
   v16f dk[Tile::kDBlocks], dv[Tile::kDBlocks];
 #pragma unroll
   for (int db = 0; db < Tile::kDBlocks; ++db)
     dk[db] = dv[db] = v16f{};
 
-  if (n_tiles > 0)
-    load_tile(0);
-  for (int32_t n = 0; n < n_tiles; ++n) {
-    char *lq = lds[n & 1][0], *lg = lds[n & 1][1];
-#pragma unroll
-    for (int i = 0; i < kPer; ++i) {
-      const int idx = threadIdx.x + i * kBwdThreads, r = idx / Tile::C, c = idx % Tile::C;
-      *reinterpret_cast<uint4 *>(Tile::at(lq, r, c)) = rq[i];
-      *reinterpret_cast<uint4 *>(Tile::at(lg, r, c)) = rg[i];
-    }
-    if (threadIdx.x < 2 * kBM)
-      rows[n & 1][threadIdx.x / kBM][threadIdx.x % kBM] = rs;
-    if (n + 1 < n_tiles)
-      load_tile(n + 1);
-    __syncthreads();
+  int buf = 0;
+  for (int32_t n = first; n < n1; n += step) {
+    wait_stream();
+    if constexpr (!SPLIT)
+      __syncthreads();
+    char *lq = stage + buf * Shape::kBufBytes, *lg = lq + Shape::kTileBytes;
+    const char *stat = lg + Shape::kTileBytes;
+    if (Shape::kBuffers == 2 && n + step < n1)
+      issue(n + step, buf ^ 1);
     const int32_t i0 = (it0 + n % per_head) * kBM;
-    if (i0 + kBM <= wave_lo)
-      continue;
-    const bool masked = i0 < wave_full || i0 + kBM > sq.lq;
+    if (i0 + kBM > wave_lo) {
+      const bool masked = i0 < wave_full || i0 + kBM > sq.lq;
 #pragma unroll
-    for (int b = 0; b < kB; ++b) {
-      v16f s{}, dp{};
-      Tile::row_product(lq, 32 * b, kf, s);
-      Tile::row_product(lg, 32 * b, vf, dp);
+      for (int b = 0; b < kB; ++b) {
+        v16f s{}, dp;
+        float l[16];
 #pragma unroll
-      for (int g = 0; g < 4; ++g) {
-        const int r = 32 * b + 8 * g + 4 * half;
-        const v4f l = *reinterpret_cast<const v4f *>(&rows[n & 1][0][r]);
-        const v4f d = *reinterpret_cast<const v4f *>(&rows[n & 1][1][r]);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          s[4 * g + e] = exp2_fast(fmaf(s[4 * g + e], a.c, -l[e]));
-          if (masked) {
-            const int32_t i = i0 + r + e;
-            s[4 * g + e] = i >= lo && i < sq.lq ? s[4 * g + e] : 0.f;
-            dp[4 * g + e] = i >= lo && i < sq.lq ? dp[4 * g + e] : d[e];
-          }
-          dp[4 * g + e] = s[4 * g + e] * (dp[4 * g + e] - d[e]);
+        for (int g = 0; g < 4; ++g) {
+          // rows 8 g + 4 half .. + 3: two (lse2, -delta) pairs per 16 bytes
+          const v4f *p = reinterpret_cast<const v4f *>(stat + (32 * b + 8 * g + 4 * half) * 8);
+          const v4f x = p[0], y = p[1];
+          l[4 * g] = x[0], l[4 * g + 1] = x[2], l[4 * g + 2] = y[0], l[4 * g + 3] = y[2];
+          dp[4 * g] = x[1], dp[4 * g + 1] = x[3], dp[4 * g + 2] = y[1], dp[4 * g + 3] = y[3];
         }
+        Tile::row_product(lq, 32 * b, kf, s);
+        Tile::row_product(lg, 32 * b, vf, dp);
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          s[r] = exp2_fast(fmaf(s[r], a.c, -l[r]));
+          dp[r] *= s[r];
+        }
+        if (masked) {
+#pragma unroll
+          for (int r = 0; r < 16; ++r) {
+            const int32_t i = i0 + 32 * b + block_row(r);
+            const bool sees = i >= lo && i < sq.lq;
+            s[r] = sees ? s[r] : 0.f;
+            dp[r] = sees ? dp[r] : 0.f;
+          }
+        }
+        typename Tile::Block p, ds;
+        Tile::pack(s, p);
+        Tile::col_product(lg, 32 * b, p, dv);
+        Tile::pack(dp, ds);
+        Tile::col_product(lq, 32 * b, ds, dk);
       }
-      typename Tile::Block p, ds;
-      Tile::pack(s, p);
-      Tile::col_product(lg, 32 * b, p, dv);
-      Tile::pack(dp, ds);
-      Tile::col_product(lq, 32 * b, ds, dk);
+    }
+    if (Shape::kBuffers == 2) {
+      buf ^= 1;
+    } else if (n + step < n1) {
+      wait_stream();
+      if constexpr (!SPLIT)
+        __syncthreads();
+      issue(n + step, 0);
     }
   }
-  if (key < room) { // rows behind the keys in use get zeros
-    const int64_t at = (gk * a.kv_heads + kv) * a.dim;
-    Tile::template store_column<VEC>(static_cast<T *>(a.gk) + at, a.dim, a.scale, dk);
-    Tile::template store_column<VEC>(static_cast<T *>(a.gv) + at, a.dim, 1.f, dv);
+
+  // rows behind the keys in use get zeros (no tile was added to them)
+  if constexpr (!SPLIT) {
+    bool bad = false;
+    if (a.causal && key_ok) {
+#pragma unroll
+      for (int db = 0; db < Tile::kDBlocks; ++db)
+#pragma unroll
+        for (int r = 0; r < 16; ++r)
+          bad |= !isfinite(dk[db][r]) || !isfinite(dv[db][r]);
+    }
+    uint64_t redo = __ballot(bad);
+    redo = (redo | redo >> 32) & 0xffffffffull;
+    if (key < room && !((redo >> (lane & 31)) & 1)) {
+      const int64_t at = (gk * a.kv_heads + kv) * a.dim;
+      Tile::template store_column<VEC>(static_cast<T *>(a.gk) + at, a.dim, a.scale, dk);
+      Tile::template store_column<VEC>(static_cast<T *>(a.gv) + at, a.dim, 1.f, dv);
+    }
+    while (redo) {
+      const int i = __ffsll(static_cast<unsigned long long>(redo)) - 1;
+      redo &= redo - 1;
+      float nk[2] = {NAN, NAN}, nv[2] = {NAN, NAN};
+      finish_dkv<T>(a, sq, wave0 + i, kv, nk, nv);
+    }
+  } else {
+    // add the waves' sums, dk then dv through the same LDS; a wave ends with
+    // rows w, w + 4, .. of both
+    float *join = reinterpret_cast<float *>(lds);
+    float rk[32 / kBwdWaves][2], rv[32 / kBwdWaves][2];
+    __syncthreads();
+    spill_columns(join + w * 32 * Shape::kJoinRow, Shape::kJoinRow, dk);
+    __syncthreads();
+#pragma unroll
+    for (int u = 0; u < 32 / kBwdWaves; ++u)
+      join_row<DP>(join, Shape::kJoinRow, w + u * kBwdWaves, rk[u][0], rk[u][1]);
+    __syncthreads();
+    spill_columns(join + w * 32 * Shape::kJoinRow, Shape::kJoinRow, dv);
+    __syncthreads();
+#pragma unroll
+    for (int u = 0; u < 32 / kBwdWaves; ++u)
+      join_row<DP>(join, Shape::kJoinRow, w + u * kBwdWaves, rv[u][0], rv[u][1]);
+#pragma unroll
+    for (int u = 0; u < 32 / kBwdWaves; ++u) {
+      const int32_t j = key0 + w + u * kBwdWaves;
+      if (j >= room)
+        break;
+      if (a.splits == 1) {
+        finish_dkv<T>(a, sq, j, kv, rk[u], rv[u]);
+      } else {
+        const int64_t at =
+            ((split * static_cast<int64_t>(a.n_k) + sq.k0 + j) * a.kv_heads + kv) * a.dim;
+        put2(a.part_k + at, a.dim, rk[u][0], rk[u][1], 1.f);
+        put2(a.part_v + at, a.dim, rv[u][0], rv[u][1], 1.f);
+      }
+    }
   }
 }
 
-unsigned bwd_grid(int64_t tiles, int64_t heads) {
-  const int64_t grid = ceil_div(tiles * heads, kXcds) * kXcds;
+// Adds the splits' partial sums of dk and dv: one wave per key and key head.
+template <typename T>
+__global__ __launch_bounds__(kBwdThreads) void attn_dkv_join_kernel(AttnArgs a) {
+  const int64_t rows = static_cast<int64_t>(a.n_k) * a.kv_heads;
+  const int64_t at = static_cast<int64_t>(blockIdx.x) * kBwdWaves + threadIdx.x / kWave;
+  if (at >= rows)
+    return;
+  const int lane = lane_id();
+  const int32_t key = static_cast<int32_t>(at / a.kv_heads);
+  float gk[2] = {0.f, 0.f}, gv[2] = {0.f, 0.f};
+  for (int s = 0; s < a.splits; ++s) {
+    const int64_t p = (s * rows + at) * a.dim;
+#pragma unroll
+    for (int u = 0; u < 2; ++u)
+      if (lane + u * kWave < a.dim) {
+        gk[u] += a.part_k[p + lane + u * kWave];
+        gv[u] += a.part_v[p + lane + u * kWave];
+      }
+  }
+  const AttnSeq sq = key_row(a, key);
+  finish_dkv<T>(a, sq, key - sq.k0, static_cast<int>(at % a.kv_heads), gk, gv);
+}
+
+struct BwdPlan {
+  bool split;
+  int64_t tiles;
+  int32_t splits;
+};
+// Over n rows (packed query rows or keys) for each key head; `others`: rows of
+// the other side, all sequences and heads of a group counted.
+BwdPlan plan_backward(int64_t n, int32_t n_seq, int32_t kv_heads, int64_t others, bool splits) {
+  BwdPlan p{false, n / kSharedRows + n_seq + 1, 1};
+  if (n / kSharedRows * kv_heads >= kFewWorkgroups)
+    return p;
+  p.split = true;
+  p.tiles = n / kSplitRows + n_seq + 1;
+  if (!splits)
+    return p;
+  const int64_t busy =
+      std::max<int64_t>(1, (n / kSplitRows + std::min<int64_t>(n_seq, n)) * kv_heads);
+  // a split gets four 32-row tiles for each wave, at least
+  const int64_t rows = n_seq > 0 ? others / n_seq : 0;
+  p.splits = static_cast<int32_t>(std::max<int64_t>(
+      1, std::min<int64_t>({kSplitTarget / busy, rows / (16 * kSplitRows), kMaxSplits})));
+  return p;
+}
+
+unsigned bwd_grid(int64_t items) {
+  const int64_t grid = ceil_div(items, kXcds) * kXcds;
   if (grid > INT32_MAX)
     throw Error(RHIP_ERR_UNSUPPORTED, "too many tiles for one launch");
   return static_cast<unsigned>(grid);
 }
 
+BwdPlan plan_keys(int64_t n_q, int64_t n_k, int32_t n_seq, int32_t heads, int32_t kv_heads) {
+  return plan_backward(n_k, n_seq, kv_heads, n_q * (heads / kv_heads), true);
+}
+
 } // namespace
 
+int32_t attn_backward_splits(int64_t n_q, int64_t n_k, int32_t n_seq, int32_t heads,
+                             int32_t kv_heads) {
+  return plan_keys(n_q, n_k, n_seq, heads, kv_heads).splits;
+}
+
 void attn_backward_run(const AttnArgs &args, int32_t dtype, bool vec, hipStream_t stream) {
+  const BwdPlan pq = plan_backward(static_cast<int64_t>(args.n_q) * args.group, args.n_seq,
+                                   args.kv_heads, args.n_k, false);
+  const BwdPlan pk = plan_keys(args.n_q, args.n_k, args.n_seq, args.heads, args.kv_heads);
+  const unsigned gq = bwd_grid(pq.tiles * args.kv_heads);
+  const unsigned gk = bwd_grid(pk.tiles * args.kv_heads * pk.splits);
   AttnArgs aq = args, ak = args;
-  aq.tiles = args.n_q / kBwdRows + args.n_seq + 1;
-  ak.tiles = args.n_k / kBwdRows + args.n_seq + 1;
-  const unsigned gq = bwd_grid(aq.tiles, args.heads), gk = bwd_grid(ak.tiles, args.kv_heads);
+  aq.tiles = static_cast<int32_t>(pq.tiles), aq.splits = 1;
+  ak.tiles = static_cast<int32_t>(pk.tiles), ak.splits = pk.splits;
   with_attn(dtype, args.dim, vec, [&](auto t, auto dp, auto v) {
     using T = decltype(t);
     constexpr int DP = decltype(dp)::value;
     constexpr bool VEC = decltype(v)::value;
-    hipLaunchKernelGGL((attn_dq_kernel<T, DP, VEC>), dim3(gq), dim3(kBwdThreads), 0, stream, aq);
-    RHIP_LAUNCH_CHECK();
-    if (!args.gk)
+    const dim3 b(kBwdThreads);
+    if (args.n_q > 0) {
+      if (pq.split)
+        hipLaunchKernelGGL((attn_dq_kernel<T, DP, VEC, true>), dim3(gq), b, 0, stream, aq);
+      else
+        hipLaunchKernelGGL((attn_dq_kernel<T, DP, VEC, false>), dim3(gq), b, 0, stream, aq);
+      RHIP_LAUNCH_CHECK();
+    }
+    if (!args.gk || args.n_k == 0)
       return;
-    hipLaunchKernelGGL((attn_dkv_kernel<T, DP, VEC>), dim3(gk), dim3(kBwdThreads), 0, stream, ak);
+    if (pk.split)
+      hipLaunchKernelGGL((attn_dkv_kernel<T, DP, VEC, true>), dim3(gk), b, 0, stream, ak);
+    else
+      hipLaunchKernelGGL((attn_dkv_kernel<T, DP, VEC, false>), dim3(gk), b, 0, stream, ak);
     RHIP_LAUNCH_CHECK();
+    if (pk.splits > 1) {
+      const int64_t rows = static_cast<int64_t>(args.n_k) * args.kv_heads;
+      hipLaunchKernelGGL((attn_dkv_join_kernel<T>),
+                         dim3(static_cast<unsigned>(ceil_div(rows, kBwdWaves))), b, 0, stream, ak);
+      RHIP_LAUNCH_CHECK();
+    }
   });
 }
 

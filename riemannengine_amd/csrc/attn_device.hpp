@@ -27,11 +27,14 @@ struct AttnArgs {
   const void *q, *k, *v, *go;
   const int32_t *q_off, *k_off, *k_len;
   int64_t q_row, q_head, k_row, k_head, v_row, v_head, go_row, go_head;
-  int32_t n_q, n_k, n_seq, heads, kv_heads, group, dim, causal, tiles;
-  float scale, c; // c = scale * log2(e)
-  void *o;
-  float *lse;   // [heads, n_q], natural logarithm
-  float *delta; // [heads, n_q], rowsum(grad_out * out)
+  int32_t n_q, n_k, n_seq, heads, kv_heads, group, dim, causal;
+  int32_t tiles, splits; // of the launch
+  float scale, c;        // c = scale * log2(e)
+  void *o, *rest;        // out, and bf16 out's rounding error (training)
+  float *lse;            // [heads, n_q], natural logarithm
+  float *part_o, *part_ml; // [splits, n_q * heads, dim], [splits, n_q * heads, 2]
+  float2 *stat;          // [heads, n_q]: log2 of the denominator, -rowsum(grad_out * out)
+  float *part_k, *part_v; // [splits, n_k * kv_heads, dim]
   void *gq, *gk, *gv;
 };
 
@@ -72,9 +75,8 @@ __device__ __forceinline__ void find_tile(const int32_t *off, int32_t n_seq, int
   tile = t - static_cast<int32_t>(static_cast<int64_t>(r0) * mul / bm + lo);
 }
 
-__device__ __forceinline__ AttnSeq query_tile(const AttnArgs &a, int bm, int mul, int32_t t) {
-  AttnSeq q;
-  find_tile(a.q_off, a.n_seq, a.n_q, bm, mul, t, q.s, q.tile, q.q0, q.lq);
+// The keys of q.s in use.
+__device__ __forceinline__ void key_range(const AttnArgs &a, AttnSeq &q) {
   q.k0 = q.lk = 0;
   if (q.s < a.n_seq) {
     q.k0 = q.s == 0 ? 0 : clamp_off(a.k_off[q.s], 0, a.n_k);
@@ -82,7 +84,41 @@ __device__ __forceinline__ AttnSeq query_tile(const AttnArgs &a, int bm, int mul
     if (a.k_len)
       q.lk = clamp_off(a.k_len[q.s], 0, q.lk);
   }
+}
+
+__device__ __forceinline__ AttnSeq query_tile(const AttnArgs &a, int bm, int mul, int32_t t) {
+  AttnSeq q;
+  find_tile(a.q_off, a.n_seq, a.n_q, bm, mul, t, q.s, q.tile, q.q0, q.lq);
+  key_range(a, q);
   return q;
+}
+
+// The sequence of one query row.
+__device__ __forceinline__ AttnSeq query_row(const AttnArgs &a, int32_t row) {
+  AttnSeq q;
+  int lo = 0, hi = a.n_seq; // largest s with off[s] <= row (empty ones before it)
+  while (lo < hi) {
+    const int mid = (lo + hi + 1) >> 1;
+    if (clamp_off(a.q_off[mid], 0, a.n_q) <= row)
+      lo = mid;
+    else
+      hi = mid - 1;
+  }
+  q.s = lo, q.tile = 0;
+  q.q0 = lo == 0 ? 0 : clamp_off(a.q_off[lo], 0, a.n_q);
+  q.lq = (lo == a.n_seq ? a.n_q : clamp_off(a.q_off[lo + 1], q.q0, a.n_q)) - q.q0;
+  key_range(a, q);
+  return q;
+}
+
+// The keys in use and the query rows of q.s, whose region holds `room` keys.
+__device__ __forceinline__ void query_range(const AttnArgs &a, AttnSeq &q, int32_t room) {
+  q.q0 = q.lq = q.lk = 0;
+  if (q.s < a.n_seq) {
+    q.lk = a.k_len ? clamp_off(a.k_len[q.s], 0, room) : room;
+    q.q0 = q.s == 0 ? 0 : clamp_off(a.q_off[q.s], 0, a.n_q);
+    q.lq = clamp_off(a.q_off[q.s + 1], q.q0, a.n_q) - q.q0;
+  }
 }
 
 // The same over the key rows (backward of k and v): lk counts the rows in
@@ -90,12 +126,25 @@ __device__ __forceinline__ AttnSeq query_tile(const AttnArgs &a, int bm, int mul
 __device__ __forceinline__ AttnSeq key_tile(const AttnArgs &a, int bm, int32_t t, int32_t &room) {
   AttnSeq q;
   find_tile(a.k_off, a.n_seq, a.n_k, bm, 1, t, q.s, q.tile, q.k0, room);
-  q.q0 = q.lq = q.lk = 0;
-  if (q.s < a.n_seq) {
-    q.lk = a.k_len ? clamp_off(a.k_len[q.s], 0, room) : room;
-    q.q0 = q.s == 0 ? 0 : clamp_off(a.q_off[q.s], 0, a.n_q);
-    q.lq = clamp_off(a.q_off[q.s + 1], q.q0, a.n_q) - q.q0;
+  query_range(a, q, room);
+  return q;
+}
+
+// The sequence of one key row; lk as in key_tile.
+__device__ __forceinline__ AttnSeq key_row(const AttnArgs &a, int32_t row) {
+  int lo = 0, hi = a.n_seq;
+  while (lo < hi) {
+    const int mid = (lo + hi + 1) >> 1;
+    if (clamp_off(a.k_off[mid], 0, a.n_k) <= row)
+      lo = mid;
+    else
+      hi = mid - 1;
   }
+  AttnSeq q;
+  q.s = lo, q.tile = 0;
+  q.k0 = lo == 0 ? 0 : clamp_off(a.k_off[lo], 0, a.n_k);
+  const int32_t room = (lo == a.n_seq ? a.n_k : clamp_off(a.k_off[lo + 1], q.k0, a.n_k)) - q.k0;
+  query_range(a, q, room);
   return q;
 }
 
@@ -219,10 +268,22 @@ template <typename T, int DP> struct AttnTile {
   }
 
   // One lane's column of a [32 DB x 32] result, scaled, as a row of dim
-  // elements at p.
+  // elements at p; store_rest: what its rounding left over.
   template <bool VEC>
   __device__ static __forceinline__ void store_column(T *p, int dim, float mul,
                                                       const v16f (&acc)[kDBlocks]) {
+    store<VEC>(p, dim, [&](float v) { return from_f32<T>(v * mul); }, acc);
+  }
+  template <bool VEC>
+  __device__ static __forceinline__ void store_rest(T *p, int dim, float mul,
+                                                    const v16f (&acc)[kDBlocks]) {
+    store<VEC>(p, dim,
+               [&](float v) { return from_f32<T>(v * mul - to_f32(from_f32<T>(v * mul))); }, acc);
+  }
+
+  template <bool VEC, typename F>
+  __device__ static __forceinline__ void store(T *p, int dim, F &&f,
+                                               const v16f (&acc)[kDBlocks]) {
     const int half = lane_id() >> 5;
 #pragma unroll
     for (int db = 0; db < kDBlocks; ++db)
@@ -232,7 +293,7 @@ template <typename T, int DP> struct AttnTile {
         T e[4];
 #pragma unroll
         for (int i = 0; i < 4; ++i)
-          e[i] = from_f32<T>(acc[db][4 * g + i] * mul);
+          e[i] = f(acc[db][4 * g + i]);
         if constexpr (VEC) { // dim is a multiple of E, so of 4
           if (d < dim) {
             if constexpr (sizeof(T) == 2)
@@ -247,6 +308,82 @@ template <typename T, int DP> struct AttnTile {
               p[d + i] = e[i];
         }
       }
+  }
+};
+
+// 16 (or 4) bytes per lane from a buffer straight into LDS, lane l's at lds +
+// l * 16 (* 4); offsets outside the buffer write zeros. The caller waits
+// (wait_stream) and keeps LDS reads of the target behind it.
+__device__ __forceinline__ void dma16(const __amdgpu_buffer_rsrc_t &rsrc, uint32_t lds,
+                                      uint32_t off) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds"
+               :
+               : "s"(lds), "v"(off), "s"(rsrc)
+               : "memory", "m0");
+}
+__device__ __forceinline__ void dma4(const __amdgpu_buffer_rsrc_t &rsrc, uint32_t lds,
+                                     uint32_t off) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dword %1, %2, 0 offen lds"
+               :
+               : "s"(lds), "v"(off), "s"(rsrc)
+               : "memory", "m0");
+}
+// This wave's loads into LDS have landed, and its LDS reads have returned.
+__device__ __forceinline__ void wait_stream() {
+  asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+}
+__device__ __forceinline__ uint32_t lds_address(const void *p) { // wave-uniform
+  return __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(reinterpret_cast<uintptr_t>(p)));
+}
+
+// Tiles of ROWS rows streamed from global memory into swizzled LDS tiles by
+// THREADS threads (a workgroup, or a wave on its own). With VEC the loads go
+// straight to LDS and stay in flight until wait_stream: no registers, no LDS
+// writes. A row's chunk c lands at position c ^ swz(r), so the lane for that
+// position fetches chunk c; rows past `valid` and chunks past dim become zeros.
+template <typename T, int DP, int ROWS, int THREADS, bool VEC> struct TileStream {
+  using Tile = AttnTile<T, DP>;
+  static constexpr int kBytes = ROWS * Tile::C * 16;
+  static constexpr int kPer = ROWS * Tile::C / THREADS;
+  uint32_t off[kPer];
+
+  __device__ __forceinline__ void init(int64_t row_stride, int dim) {
+    const int t = threadIdx.x % THREADS;
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+      const int idx = t + i * THREADS, r = idx / Tile::C;
+      const int c = (idx % Tile::C) ^ Tile::swz(r);
+      off[i] = c * Tile::E < dim ? static_cast<uint32_t>(r * row_stride * sizeof(T) + c * 16)
+                                 : kBufOob;
+    }
+  }
+  // base: the tile's first row; valid: rows from there on (may be 0 or less)
+  __device__ __forceinline__ void issue(char *lds, const T *base, int64_t row_stride,
+                                        int32_t valid, int dim) const {
+    const int t = threadIdx.x % THREADS;
+    const int32_t rows = min(valid, ROWS);
+    if constexpr (VEC) {
+      const int64_t bytes =
+          rows > 0 ? ((rows - 1) * row_stride + dim) * static_cast<int64_t>(sizeof(T)) : 0;
+      const __amdgpu_buffer_rsrc_t rsrc = buf_rsrc(base, bytes);
+      const uint32_t to = lds_address(lds) + lds_address_of_wave(t);
+#pragma unroll
+      for (int i = 0; i < kPer; ++i)
+        dma16(rsrc, to + i * THREADS * 16, off[i]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < kPer; ++i) {
+        const int idx = t + i * THREADS, r = idx / Tile::C;
+        const int c = (idx % Tile::C) ^ Tile::swz(r);
+        *reinterpret_cast<uint4 *>(lds + idx * 16) =
+            Tile::template chunk<false>(base + r * row_stride, c, dim, r < rows);
+      }
+    }
+  }
+
+private:
+  __device__ static __forceinline__ uint32_t lds_address_of_wave(int t) {
+    return __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(t / kWave * kWave * 16));
   }
 };
 

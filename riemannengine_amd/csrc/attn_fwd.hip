@@ -1,28 +1,59 @@
 // Attention over packed sequences on gfx950, forward: softmax(scale q k^T) v
 // for every sequence and head by itself, in one pass over the keys with the
 // running maximum and sum of the softmax.
-#include "attn_device.hpp"
+//
+// The heads of a group are packed: row r of a key head's sequence is query
+// row r / group, head r % group, so all rows that read the same keys stand in
+// the same tiles. Two launch shapes share one kernel:
+//   shared  128 rows per workgroup, 32 per wave; the four waves read the same
+//           LDS tiles of keys;
+//   split   32 rows per workgroup; each wave takes every fourth 32-key tile
+//           through LDS tiles of its own (no barrier until the end) and the
+//           waves' results are joined in LDS. The keys may further be split
+//           over workgroups, joined by a second kernel. For single tokens and
+//           wherever 128-row tiles leave the chip empty.
 #include "attn.hpp"
 
 namespace rhip {
 namespace {
 
 constexpr int kFwdThreads = 256;
-constexpr int kFwdRows = 128; // query rows per workgroup, 32 per wave
-template <typename T> constexpr int kFwdKeys = sizeof(T) == 2 ? 64 : 32; // keys per LDS tile
+constexpr int kFwdWaves = kFwdThreads / kWave;
+constexpr int kSharedRows = 128, kSplitRows = 32;
+// Workgroups below which the split shape is taken, and how many it aims for.
+constexpr int64_t kFewWorkgroups = 256, kSplitTarget = 1024;
+constexpr int kMaxSplits = 64, kMinSplitKeys = 256;
 
-// Workgroup -> (tile, head). Workgroups go to the XCDs round-robin; each XCD
-// takes a contiguous run of the head-major list, so the tiles that read one
-// head's keys share an L2. Within a head the last tiles come first: under a
-// causal mask those have the most keys.
-__device__ __forceinline__ bool fwd_item(const AttnArgs &a, int32_t &tile, int32_t &head) {
-  const uint32_t total = static_cast<uint32_t>(a.tiles) * a.heads;
+template <typename T, int DP, bool SPLIT> struct FwdShape {
+  static constexpr int kRows = SPLIT ? kSplitRows : kSharedRows;
+  // keys per LDS tile: two 32-key blocks where they fit
+  static constexpr int kBN = SPLIT || (sizeof(T) == 4 && DP == 128) ? 32 : 64;
+  static constexpr int kStreams = SPLIT ? kFwdWaves : 1;
+  static constexpr int kTileBytes = kBN * DP * sizeof(T);
+  // two buffers, but for fp32 at full width where four waves' would not fit
+  static constexpr int kBuffers = kStreams * 4 * kTileBytes <= 160 * 1024 ? 2 : 1;
+  static constexpr int kJoinRow = DP + 4; // floats per row of the joined results
+  static constexpr int kJoinBytes =
+      SPLIT ? kFwdWaves * 32 * (kJoinRow + 2) * static_cast<int>(sizeof(float)) : 0;
+  static constexpr int kStageBytes = kStreams * kBuffers * 2 * kTileBytes;
+  static constexpr int kLds = kStageBytes > kJoinBytes ? kStageBytes : kJoinBytes;
+};
+
+// Workgroup -> (tile, key head, split). Workgroups go to the XCDs round-robin;
+// each XCD takes a contiguous run of the head-major list, so the tiles that
+// read one head's keys share an L2. Within a head the last tiles come first:
+// under a causal mask those have the most keys.
+__device__ __forceinline__ bool fwd_item(const AttnArgs &a, int32_t &tile, int32_t &kv,
+                                         int32_t &split) {
+  const uint32_t total = static_cast<uint32_t>(a.tiles) * a.kv_heads * a.splits;
   const uint32_t per = (total + kXcds - 1) / kXcds;
   const uint32_t i = (blockIdx.x % kXcds) * per + blockIdx.x / kXcds;
-  if (i >= total || blockIdx.x / kXcds >= per)
+  if (i >= total)
     return false;
-  head = i / a.tiles;
-  tile = a.tiles - 1 - i % a.tiles;
+  split = i % a.splits;
+  const uint32_t j = i / a.splits;
+  kv = j / a.tiles;
+  tile = a.tiles - 1 - j % a.tiles;
   return true;
 }
 
@@ -65,65 +96,109 @@ __device__ void exact_row(const T *q, const T *k, int64_t k_row, const T *v, int
     sum += __shfl_xor(sum, off, kWave);
 }
 
-// o = softmax(scale q k^T) v and lse for 128 query rows of one head, 32 per
-// wave. Scores are S^T = K Q^T (a lane holds 16 keys of one query row's block,
-// the other half of the pair l, l + 32 the other 16), so maximum and sum are
+// A row's result from one wave: lane l holds elements l and l + 64 of the
+// unnormalised sum. `at`: the row's place in out, [n_q, heads].
+template <typename T>
+__device__ void finish_row(const AttnArgs &a, const AttnSeq &sq, int32_t i, int32_t head,
+                           float o0, float o1, float m, float sum) {
+  const int lane = lane_id();
+  const int64_t row = sq.q0 + static_cast<int64_t>(i);
+  if (a.causal && __any(!isfinite(o0) || !isfinite(o1) || !isfinite(sum))) {
+    const int kv = head / a.group;
+    const int64_t lim = min<int64_t>(sq.lk, i + static_cast<int64_t>(sq.lk) - sq.lq + 1);
+    exact_row<T>(static_cast<const T *>(a.q) + row * a.q_row + head * a.q_head,
+                 static_cast<const T *>(a.k) + sq.k0 * a.k_row + kv * a.k_head, a.k_row,
+                 static_cast<const T *>(a.v) + sq.k0 * a.v_row + kv * a.v_head, a.v_row,
+                 static_cast<int32_t>(max<int64_t>(lim, 0)), a.dim, a.c, o0, o1, m, sum);
+  }
+  const float inv = sum == 0.f ? 0.f : 1.f / sum;
+  const int64_t at = (row * a.heads + head) * a.dim;
+  auto put = [&](int d, float v) {
+    if (d < a.dim) {
+      const T t = from_f32<T>(v * inv);
+      static_cast<T *>(a.o)[at + d] = t;
+      if (sizeof(T) == 2 && a.rest)
+        static_cast<T *>(a.rest)[at + d] = from_f32<T>(v * inv - to_f32(t));
+    }
+  };
+  put(lane, o0);
+  put(lane + kWave, o1);
+  if (a.lse && lane == 0)
+    a.lse[static_cast<int64_t>(head) * a.n_q + row] =
+        sum == 0.f ? -INFINITY : m * a.scale + logf(sum);
+}
+
+// Scores are S^T = K Q^T (a lane holds 16 keys of one query row's block, the
+// other half of the pair l, l + 32 the other 16), so maximum and sum are
 // in-lane but for one exchange, and P^T is the right operand of O^T = V^T P^T
-// as it lies. K and V tiles go through LDS, double-buffered: the next tile's
-// loads are in flight while this one is multiplied.
-template <typename T, int DP, bool VEC>
-__global__ __launch_bounds__(kFwdThreads, 2) void attn_fwd_kernel(AttnArgs a) {
+// as it lies. The next tile's loads are in flight while this one is
+// multiplied.
+template <typename T, int DP, bool VEC, bool SPLIT>
+__global__ __launch_bounds__(kFwdThreads, sizeof(T) == 4 && DP == 128 ? 1 : 2) void
+attn_fwd_kernel(AttnArgs a) {
+  using Shape = FwdShape<T, DP, SPLIT>;
   using Tile = AttnTile<T, DP>;
   using Frag = typename Tile::Frag;
-  constexpr int kBN = kFwdKeys<T>, kB = kBN / 32;
-  constexpr int kBytes = kBN * Tile::C * 16;
-  constexpr int kPer = kBN * Tile::C / kFwdThreads; // chunks per thread of a tile
-  __shared__ alignas(16) char lds[2][2][kBytes];
+  constexpr int kBN = Shape::kBN, kB = kBN / 32;
+  using Stream = TileStream<T, DP, kBN, SPLIT ? kWave : kFwdThreads, VEC>;
+  __shared__ alignas(16) char lds[Shape::kLds];
 
-  int32_t t, head;
-  if (!fwd_item(a, t, head))
+  int32_t t, kv, split;
+  if (!fwd_item(a, t, kv, split))
     return;
-  const AttnSeq sq = query_tile(a, kFwdRows, 1, t);
-  const int32_t row0 = sq.tile * kFwdRows;
-  if (row0 >= sq.lq)
+  const AttnSeq sq = query_tile(a, Shape::kRows, a.group, t);
+  const int32_t n_rows = sq.lq * a.group, row0 = sq.tile * Shape::kRows;
+  if (row0 >= n_rows)
     return;
-  const int lane = lane_id(), w = threadIdx.x / kWave, half = lane >> 5;
-  const int32_t row = row0 + w * 32 + (lane & 31); // this lane's query row
-  const bool row_ok = row < sq.lq;
-  const int64_t shift = sq.lk - sq.lq; // causal: row i sees keys j <= i + shift
-  // keys this lane's row sees, and how far the workgroup's and this wave's go
-  auto sees = [&](int64_t r) {
-    const int64_t n = a.causal ? min<int64_t>(sq.lk, r + shift + 1) : sq.lk;
+  const int lane = lane_id(), half = lane >> 5;
+  const int w = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+  const int32_t wave0 = row0 + (SPLIT ? 0 : w * 32);
+  const int32_t row = wave0 + (lane & 31); // this lane's packed row
+  const bool row_ok = row < n_rows;
+  const int32_t rc = min(row, n_rows - 1);
+  const int32_t qi = rc / a.group;
+  const int head = kv * a.group + rc % a.group;
+  const int64_t shift = static_cast<int64_t>(sq.lk) - sq.lq;
+  // keys a packed row sees (causal: query row i sees keys j <= i + shift)
+  auto sees = [&](int32_t r) {
+    const int64_t n = a.causal ? min<int64_t>(sq.lk, r / a.group + shift + 1) : sq.lk;
     return static_cast<int32_t>(n < 0 ? 0 : n);
   };
   const int32_t lim = row_ok ? sees(row) : 0;
-  const int32_t wg_lim = sees(min(row0 + kFwdRows, sq.lq) - 1);
-  const int32_t wave_lim = row0 + w * 32 < sq.lq ? sees(min(row0 + w * 32 + 32, sq.lq) - 1) : 0;
-  const int32_t wave_full = row0 + w * 32 < sq.lq ? sees(row0 + w * 32) : 0; // seen by all rows
-  const int32_t n_tiles = (wg_lim + kBN - 1) / kBN;
+  const int32_t wg_lim = sees(min(row0 + Shape::kRows, n_rows) - 1);
+  const int32_t wave_lim = wave0 < n_rows ? sees(min(wave0 + 32, n_rows) - 1) : 0;
+  const int32_t wave_full = wave0 < n_rows ? sees(wave0) : 0; // seen by all its rows
+  // this workgroup's tiles [kt0, kt1) of keys; a wave's first and step
+  int32_t kt0 = 0, kt1 = (wg_lim + kBN - 1) / kBN;
+  if (SPLIT && a.splits > 1) {
+    const int32_t per = (kt1 + a.splits - 1) / a.splits;
+    kt0 = min(split * per, kt1);
+    kt1 = min(kt0 + per, kt1);
+  }
+  const int32_t first = kt0 + (SPLIT ? w : 0), step = SPLIT ? kFwdWaves : 1;
 
-  const int kv = head / a.group;
   const T *kp = static_cast<const T *>(a.k) + sq.k0 * a.k_row + kv * a.k_head;
   const T *vp = static_cast<const T *>(a.v) + sq.k0 * a.v_row + kv * a.v_head;
+  Stream ks, vs;
+  ks.init(a.k_row, a.dim);
+  vs.init(a.v_row, a.dim);
+  char *stage = lds + (SPLIT ? w : 0) * Shape::kBuffers * 2 * Shape::kTileBytes;
+  auto issue = [&](int32_t kt, int buf) {
+    char *to = stage + buf * 2 * Shape::kTileBytes;
+    ks.issue(to, kp + static_cast<int64_t>(kt) * kBN * a.k_row, a.k_row, sq.lk - kt * kBN,
+             a.dim);
+    vs.issue(to + Shape::kTileBytes, vp + static_cast<int64_t>(kt) * kBN * a.v_row, a.v_row,
+             sq.lk - kt * kBN, a.dim);
+  };
+  if (first < kt1)
+    issue(first, 0);
 
-  const T *qp = static_cast<const T *>(a.q) + (sq.q0 + static_cast<int64_t>(row)) * a.q_row +
+  const T *qp = static_cast<const T *>(a.q) + (sq.q0 + static_cast<int64_t>(qi)) * a.q_row +
                 head * a.q_head;
   Frag qf[Tile::kSteps];
 #pragma unroll
   for (int s = 0; s < Tile::kSteps; ++s)
     qf[s] = __builtin_bit_cast(Frag, Tile::template chunk<VEC>(qp, 2 * s + half, a.dim, row_ok));
-
-  uint4 rk[kPer], rv[kPer];
-  auto load_tile = [&](int32_t kt) {
-#pragma unroll
-    for (int i = 0; i < kPer; ++i) {
-      const int idx = threadIdx.x + i * kFwdThreads, r = idx / Tile::C, c = idx % Tile::C;
-      const int32_t j = kt * kBN + r;
-      const bool ok = j < sq.lk;
-      rk[i] = Tile::template chunk<VEC>(kp + j * a.k_row, c, a.dim, ok);
-      rv[i] = Tile::template chunk<VEC>(vp + j * a.v_row, c, a.dim, ok);
-    }
-  };
 
   v16f o[Tile::kDBlocks];
 #pragma unroll
@@ -131,118 +206,230 @@ __global__ __launch_bounds__(kFwdThreads, 2) void attn_fwd_kernel(AttnArgs a) {
     o[db] = v16f{};
   float m = -INFINITY, sum = 0.f; // of this lane's row; sum over its half of the keys
 
-  if (n_tiles > 0)
-    load_tile(0);
-  for (int32_t kt = 0; kt < n_tiles; ++kt) {
-    char *lk = lds[kt & 1][0], *lv = lds[kt & 1][1];
-#pragma unroll
-    for (int i = 0; i < kPer; ++i) {
-      const int idx = threadIdx.x + i * kFwdThreads, r = idx / Tile::C, c = idx % Tile::C;
-      *reinterpret_cast<uint4 *>(Tile::at(lk, r, c)) = rk[i];
-      *reinterpret_cast<uint4 *>(Tile::at(lv, r, c)) = rv[i];
-    }
-    if (kt + 1 < n_tiles)
-      load_tile(kt + 1);
-    // one barrier per tile: the buffer written next was last read before the
-    // barrier of the tile between
-    __syncthreads();
+  int buf = 0;
+  for (int32_t kt = first; kt < kt1; kt += step) {
+    // this tile has landed; then every wave is past its reads of the other
+    // buffer, which the next tile's loads overwrite
+    wait_stream();
+    if constexpr (!SPLIT)
+      __syncthreads();
+    char *lk = stage + buf * 2 * Shape::kTileBytes, *lv = lk + Shape::kTileBytes;
+    if (Shape::kBuffers == 2 && kt + step < kt1)
+      issue(kt + step, buf ^ 1);
     const int32_t j0 = kt * kBN;
-    if (j0 >= wave_lim)
-      continue;
-    v16f s[kB];
+    if (SPLIT || j0 < wave_lim) {
+      v16f s[kB];
 #pragma unroll
-    for (int b = 0; b < kB; ++b) {
-      s[b] = v16f{};
-      Tile::row_product(lk, 32 * b, qf, s[b]);
-    }
-    if (j0 + kBN > wave_full) {
+      for (int b = 0; b < kB; ++b) {
+        s[b] = v16f{};
+        Tile::row_product(lk, 32 * b, qf, s[b]);
+      }
+      if (j0 + kBN > wave_full) {
+#pragma unroll
+        for (int b = 0; b < kB; ++b)
+#pragma unroll
+          for (int r = 0; r < 16; ++r)
+            s[b][r] = j0 + 32 * b + block_row(r) < lim ? s[b][r] : -INFINITY;
+      }
+      float top = m;
 #pragma unroll
       for (int b = 0; b < kB; ++b)
 #pragma unroll
         for (int r = 0; r < 16; ++r)
-          s[b][r] = j0 + 32 * b + block_row(r) < lim ? s[b][r] : -INFINITY;
-    }
-    float top = m;
+          top = fmaxf(top, s[b][r]);
+      top = pair_max(top);
+      const float base = (top == -INFINITY ? 0.f : top) * a.c;
+      if (__any(top > m)) { // otherwise every factor is 1
+        const float f = exp2_fast(m * a.c - base);
+        sum *= f;
 #pragma unroll
-    for (int b = 0; b < kB; ++b)
-#pragma unroll
-      for (int r = 0; r < 16; ++r)
-        top = fmaxf(top, s[b][r]);
-    top = pair_max(top);
-    const float base = (top == -INFINITY ? 0.f : top) * a.c;
-    if (__any(top > m)) { // otherwise every factor is 1
-      const float f = exp2_fast(m * a.c - base);
-      sum *= f;
-#pragma unroll
-      for (int db = 0; db < Tile::kDBlocks; ++db)
-        o[db] *= f;
-      m = top;
-    }
-#pragma unroll
-    for (int b = 0; b < kB; ++b) {
-#pragma unroll
-      for (int r = 0; r < 16; ++r) {
-        s[b][r] = exp2_fast(fmaf(s[b][r], a.c, -base));
-        sum += s[b][r];
+        for (int db = 0; db < Tile::kDBlocks; ++db)
+          o[db] *= f;
+        m = top;
       }
-      typename Tile::Block p;
-      Tile::pack(s[b], p);
-      Tile::col_product(lv, 32 * b, p, o);
+#pragma unroll
+      for (int b = 0; b < kB; ++b) {
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          s[b][r] = exp2_fast(fmaf(s[b][r], a.c, -base));
+          sum += s[b][r];
+        }
+        typename Tile::Block p;
+        Tile::pack(s[b], p);
+        Tile::col_product(lv, 32 * b, p, o);
+      }
+    }
+    if (Shape::kBuffers == 2) {
+      buf ^= 1;
+    } else if (kt + step < kt1) {
+      wait_stream();
+      if constexpr (!SPLIT)
+        __syncthreads();
+      issue(kt + step, 0);
     }
   }
-
   sum = pair_sum(sum);
-  float lse = sum == 0.f ? -INFINITY : m * a.scale + logf(sum);
-  float inv = sum == 0.f ? 0.f : 1.f / sum;
-  T *op = static_cast<T *>(a.o) +
-          ((sq.q0 + static_cast<int64_t>(row)) * a.heads + head) * a.dim;
-  bool bad = false;
-  if (a.causal) {
+
+  if constexpr (!SPLIT) {
+    const float inv = sum == 0.f ? 0.f : 1.f / sum;
+    bool bad = false;
+    if (a.causal) {
+#pragma unroll
+      for (int db = 0; db < Tile::kDBlocks; ++db)
+#pragma unroll
+        for (int r = 0; r < 16; ++r)
+          bad |= !isfinite(o[db][r]);
+      bad = (bad || !isfinite(sum)) && row_ok;
+    }
+    uint64_t redo = __ballot(bad);
+    redo = (redo | redo >> 32) & 0xffffffffull;
+    const int64_t at = (sq.q0 + static_cast<int64_t>(qi)) * a.heads + head;
+    if (row_ok && !((redo >> (lane & 31)) & 1)) {
+      Tile::template store_column<VEC>(static_cast<T *>(a.o) + at * a.dim, a.dim, inv, o);
+      if (sizeof(T) == 2 && a.rest)
+        Tile::template store_rest<VEC>(static_cast<T *>(a.rest) + at * a.dim, a.dim, inv, o);
+      if (a.lse && half == 0)
+        a.lse[static_cast<int64_t>(head) * a.n_q + sq.q0 + qi] =
+            sum == 0.f ? -INFINITY : m * a.scale + logf(sum);
+    }
+    while (redo) {
+      const int i = __ffsll(static_cast<unsigned long long>(redo)) - 1;
+      redo &= redo - 1;
+      finish_row<T>(a, sq, __shfl(qi, i, kWave), __shfl(head, i, kWave), NAN, NAN, 0.f, 0.f);
+    }
+  } else {
+    // join the waves: [wave][row][DP] sums, then each row's maximum and sum
+    __syncthreads(); // every wave is past its tiles
+    float *jo = reinterpret_cast<float *>(lds);
+    float *jm = jo + kFwdWaves * 32 * Shape::kJoinRow;
+    float *mine = jo + (w * 32 + (lane & 31)) * Shape::kJoinRow;
 #pragma unroll
     for (int db = 0; db < Tile::kDBlocks; ++db)
 #pragma unroll
-      for (int r = 0; r < 16; ++r)
-        bad |= !isfinite(o[db][r]);
-    bad = (bad || !isfinite(sum)) && row_ok;
+      for (int g = 0; g < 4; ++g)
+        *reinterpret_cast<v4f *>(mine + 32 * db + 8 * g + 4 * half) =
+            v4f{o[db][4 * g], o[db][4 * g + 1], o[db][4 * g + 2], o[db][4 * g + 3]};
+    if (half == 0) {
+      jm[(w * 32 + lane) * 2] = m;
+      jm[(w * 32 + lane) * 2 + 1] = sum;
+    }
+    __syncthreads();
+    for (int r = w; r < 32 && row0 + r < n_rows; r += kFwdWaves) {
+      float mr = -INFINITY;
+#pragma unroll
+      for (int i = 0; i < kFwdWaves; ++i)
+        mr = fmaxf(mr, jm[(i * 32 + r) * 2]);
+      const float base = (mr == -INFINITY ? 0.f : mr) * a.c;
+      float o0 = 0.f, o1 = 0.f, sr = 0.f;
+#pragma unroll
+      for (int i = 0; i < kFwdWaves; ++i) {
+        const float f = exp2_fast(jm[(i * 32 + r) * 2] * a.c - base);
+        sr = fmaf(jm[(i * 32 + r) * 2 + 1], f, sr);
+        const float *src = jo + (i * 32 + r) * Shape::kJoinRow;
+        if (lane < DP)
+          o0 = fmaf(src[lane], f, o0);
+        if (DP > kWave)
+          o1 = fmaf(src[lane + kWave], f, o1);
+      }
+      const int32_t i = (row0 + r) / a.group;
+      const int h = kv * a.group + (row0 + r) % a.group;
+      if (a.splits == 1) {
+        finish_row<T>(a, sq, i, h, o0, o1, mr, sr);
+      } else {
+        const int64_t at = split * static_cast<int64_t>(a.n_q) * a.heads +
+                           (sq.q0 + static_cast<int64_t>(i)) * a.heads + h;
+        if (lane < a.dim)
+          a.part_o[at * a.dim + lane] = o0;
+        if (lane + kWave < a.dim)
+          a.part_o[at * a.dim + lane + kWave] = o1;
+        if (lane == 0) {
+          a.part_ml[2 * at] = mr;
+          a.part_ml[2 * at + 1] = sr;
+        }
+      }
+    }
   }
-  uint64_t redo = __ballot(bad);
-  redo = (redo | redo >> 32) & 0xffffffffull;
-  if (row_ok && !((redo >> (lane & 31)) & 1)) {
-    Tile::template store_column<VEC>(op, a.dim, inv, o);
-    if (a.lse && half == 0)
-      a.lse[static_cast<int64_t>(head) * a.n_q + sq.q0 + row] = lse;
-  }
-  while (redo) {
-    const int i = __ffsll(static_cast<unsigned long long>(redo)) - 1;
-    redo &= redo - 1;
-    const int64_t r = sq.q0 + static_cast<int64_t>(row0) + w * 32 + i;
-    float o0, o1, mr, sr;
-    exact_row<T>(static_cast<const T *>(a.q) + r * a.q_row + head * a.q_head, kp, a.k_row, vp,
-                 a.v_row, sees(row0 + w * 32 + i), a.dim, a.c, o0, o1, mr, sr);
-    T *p = static_cast<T *>(a.o) + (r * a.heads + head) * a.dim;
-    const float iv = sr == 0.f ? 0.f : 1.f / sr;
+}
+
+// Joins the splits' partial sums: one wave per row and head, in split order.
+template <typename T>
+__global__ __launch_bounds__(kFwdThreads) void attn_join_kernel(AttnArgs a) {
+  const int64_t rows = static_cast<int64_t>(a.n_q) * a.heads;
+  const int64_t at = static_cast<int64_t>(blockIdx.x) * kFwdWaves + threadIdx.x / kWave;
+  if (at >= rows)
+    return;
+  const int lane = lane_id();
+  const int32_t row = static_cast<int32_t>(at / a.heads), head = static_cast<int32_t>(at % a.heads);
+  float mr = -INFINITY;
+  for (int s = 0; s < a.splits; ++s)
+    mr = fmaxf(mr, a.part_ml[2 * (s * rows + at)]);
+  const float base = (mr == -INFINITY ? 0.f : mr) * a.c;
+  float o0 = 0.f, o1 = 0.f, sr = 0.f;
+  for (int s = 0; s < a.splits; ++s) {
+    const float f = exp2_fast(a.part_ml[2 * (s * rows + at)] * a.c - base);
+    sr = fmaf(a.part_ml[2 * (s * rows + at) + 1], f, sr);
+    const float *src = a.part_o + (s * rows + at) * a.dim;
     if (lane < a.dim)
-      p[lane] = from_f32<T>(o0 * iv);
+      o0 = fmaf(src[lane], f, o0);
     if (lane + kWave < a.dim)
-      p[lane + kWave] = from_f32<T>(o1 * iv);
-    if (a.lse && lane == 0)
-      a.lse[static_cast<int64_t>(head) * a.n_q + r] = mr * a.scale + logf(sr);
+      o1 = fmaf(src[lane + kWave], f, o1);
   }
+  // the row's sequence, for rows that have to be computed again
+  AttnSeq sq = query_row(a, row);
+  finish_row<T>(a, sq, row - sq.q0, head, o0, o1, mr, sr);
+}
+
+struct FwdPlan {
+  bool split;
+  int64_t tiles;
+  int32_t splits;
+};
+FwdPlan plan_forward(int64_t n_q, int64_t n_k, int32_t n_seq, int32_t heads, int32_t kv_heads) {
+  const int64_t rows = n_q * (heads / kv_heads);
+  FwdPlan p{false, rows / kSharedRows + n_seq + 1, 1};
+  if (rows / kSharedRows * kv_heads >= kFewWorkgroups)
+    return p;
+  p.split = true;
+  p.tiles = rows / kSplitRows + n_seq + 1;
+  // workgroups with rows: a tile of every 32 rows, and one per sequence
+  const int64_t busy = std::max<int64_t>(1, (rows / kSplitRows + std::min<int64_t>(n_seq, rows)) *
+                                                kv_heads);
+  const int64_t keys = n_seq > 0 ? n_k / n_seq : 0;
+  p.splits = static_cast<int32_t>(std::max<int64_t>(
+      1, std::min<int64_t>({kSplitTarget / busy, keys / kMinSplitKeys, kMaxSplits})));
+  return p;
 }
 
 } // namespace
 
+int32_t attn_forward_splits(int64_t n_q, int64_t n_k, int32_t n_seq, int32_t heads,
+                            int32_t kv_heads) {
+  return plan_forward(n_q, n_k, n_seq, heads, kv_heads).splits;
+}
+
 void attn_forward_run(const AttnArgs &args, int32_t dtype, bool vec, hipStream_t stream) {
   AttnArgs a = args;
-  a.tiles = a.n_q / kFwdRows + a.n_seq + 1;
-  const int64_t grid = ceil_div(static_cast<int64_t>(a.tiles) * a.heads, kXcds) * kXcds;
+  const FwdPlan plan = plan_forward(a.n_q, a.n_k, a.n_seq, a.heads, a.kv_heads);
+  const int64_t grid = ceil_div(plan.tiles * a.kv_heads * plan.splits, kXcds) * kXcds;
   if (grid > INT32_MAX)
     throw Error(RHIP_ERR_UNSUPPORTED, "too many query tiles for one launch");
+  a.tiles = static_cast<int32_t>(plan.tiles), a.splits = plan.splits;
   with_attn(dtype, a.dim, vec, [&](auto t, auto dp, auto v) {
     using T = decltype(t);
-    hipLaunchKernelGGL((attn_fwd_kernel<T, decltype(dp)::value, decltype(v)::value>),
-                       dim3(static_cast<unsigned>(grid)), dim3(kFwdThreads), 0, stream, a);
+    constexpr int DP = decltype(dp)::value;
+    constexpr bool VEC = decltype(v)::value;
+    const dim3 g(static_cast<unsigned>(grid)), b(kFwdThreads);
+    if (plan.split)
+      hipLaunchKernelGGL((attn_fwd_kernel<T, DP, VEC, true>), g, b, 0, stream, a);
+    else
+      hipLaunchKernelGGL((attn_fwd_kernel<T, DP, VEC, false>), g, b, 0, stream, a);
     RHIP_LAUNCH_CHECK();
+    if (a.splits > 1) {
+      const int64_t rows = static_cast<int64_t>(a.n_q) * a.heads;
+      hipLaunchKernelGGL((attn_join_kernel<T>),
+                         dim3(static_cast<unsigned>(ceil_div(rows, kFwdWaves))), b, 0, stream, a);
+      RHIP_LAUNCH_CHECK();
+    }
   });
 }
 

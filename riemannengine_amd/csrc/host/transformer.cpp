@@ -88,17 +88,25 @@ struct Attention {
     return d;
   }
 
-  at::Tensor forward(at::Tensor *lse) const {
+  // With lse, also what the backward pass needs of bf16 results: out's
+  // rounding error.
+  at::Tensor forward(at::Tensor *lse, at::Tensor *rest) const {
     const auto dev = q.device();
     at::DeviceGuard guard(dev);
     const rhip_attn d = desc();
     auto out = torch::empty(q.sizes(), q.options());
-    if (lse)
+    if (lse) {
       *lse = torch::empty({q.size(1), q.size(0)}, q.options().dtype(torch::kFloat));
+      if (d.dtype == RHIP_BF16)
+        *rest = torch::empty(q.sizes(), q.options());
+      else
+        *rest = torch::empty({0}, q.options());
+    }
     size_t bytes = 0;
     check_rhip(rhip_attn_workspace_bytes(&d, 0, &bytes), "rhip_attn_workspace_bytes");
     auto ws = byte_buffer(bytes, dev);
     check_rhip(rhip_attn_forward(&d, q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(),
+                                 lse && present(*rest) ? rest->data_ptr() : nullptr,
                                  lse ? lse->data_ptr<float>() : nullptr, ws.data_ptr(),
                                  ws.numel(), stream_of(dev)),
                "rhip_attn_forward");
@@ -111,9 +119,9 @@ struct HipAttentionFunction : public torch::autograd::Function<HipAttentionFunct
                             at::Tensor q_offsets, at::Tensor k_offsets, at::Tensor k_lengths,
                             bool causal, double scale) {
     const Attention a{q, k, v, q_offsets, k_offsets, k_lengths, causal, scale};
-    at::Tensor lse;
-    auto out = a.forward(&lse);
-    ctx->save_for_backward({q, k, v, out, lse, q_offsets, k_offsets, k_lengths});
+    at::Tensor lse, rest;
+    auto out = a.forward(&lse, &rest);
+    ctx->save_for_backward({q, k, v, out, lse, q_offsets, k_offsets, k_lengths, rest});
     ctx->saved_data["causal"] = causal;
     ctx->saved_data["scale"] = scale;
     return out;
@@ -139,6 +147,7 @@ struct HipAttentionFunction : public torch::autograd::Function<HipAttentionFunct
     auto ws = byte_buffer(bytes, dev);
     check_rhip(rhip_attn_backward(&d, go.data_ptr(), go.stride(0), go.stride(1), a.q.data_ptr(),
                                   a.k.data_ptr(), a.v.data_ptr(), s[3].data_ptr(),
+                                  present(s[8]) ? s[8].data_ptr() : nullptr,
                                   s[4].data_ptr<float>(), vptr_mut(gq), vptr_mut(gk),
                                   vptr_mut(gv), ws.data_ptr(), ws.numel(), stream_of(dev)),
                "rhip_attn_backward");
@@ -325,7 +334,7 @@ at::Tensor hip_packed_attention(const at::Tensor &query, const at::Tensor &key,
   auto q = dense_last(query), k = dense_last(key), v = dense_last(value);
   if (wants_grad({query, key, value}))
     return HipAttentionFunction::apply(q, k, v, qo, ko, or_empty(kl, qo), causal, s);
-  return Attention{q, k, v, qo, ko, kl, causal, s}.forward(nullptr);
+  return Attention{q, k, v, qo, ko, kl, causal, s}.forward(nullptr, nullptr);
 }
 
 at::Tensor hip_layer_norm(const at::Tensor &input, const at::Tensor &weight,

@@ -178,6 +178,120 @@ def test_masked_places_do_not_reach_a_row(dtype, bad):
 
 
 @pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("rows", [170, 9000])
+def test_masked_places_do_not_reach_a_gradient(dtype, dim, rows):
+    """Causal: a grad_out row that is not finite reaches the gradients of the
+    keys it sees (and its own), keys and values that are not finite those of
+    the rows that see them; the others keep their values. Both launch shapes
+    (9000 rows on 4 heads fill the chip with whole tiles)."""
+    lens = [40, rows, 90]
+    n = sum(lens)
+    q, k, v, g = inputs(11, n, n, 4, 4 if rows > 1000 else 2, dim, dtype)
+    o = offsets(lens)
+    at = 40 + 77
+    print("masked gradients", dtype, dim, rows, flush=True)
+    out, lse = abi.attn_forward(q, k, v, o, o, causal=True)
+    clean = abi.attn_backward(g, q, k, v, out, lse, o, o, causal=True)
+    tol = [16 * torch.finfo(dtype).eps * c.abs().max() for c in clean]
+    g2 = g.clone()
+    g2[at] = math.nan
+    gq, gk, gv = abi.attn_backward(g2, q, k, v, out, lse, o, o, causal=True)
+    others = torch.arange(n, device=DEV) != at
+    assert (gq[others] - clean[0][others]).abs().max() <= tol[0]
+    unseen = torch.ones(n, dtype=torch.bool, device=DEV)
+    unseen[40:at + 1] = False
+    assert (gk[unseen] - clean[1][unseen]).abs().max() <= tol[1]
+    assert (gv[unseen] - clean[2][unseen]).abs().max() <= tol[2]
+    assert not torch.isfinite(gv[40:at + 1]).any() and not torch.isfinite(gq[at]).any()
+    k2, v2 = k.clone(), v.clone()
+    k2[at], v2[at] = math.inf, math.nan
+    out, lse = abi.attn_forward(q, k2, v2, o, o, causal=True)
+    gq, gk, gv = abi.attn_backward(g, q, k2, v2, out, lse, o, o, causal=True)
+    rows_ok = torch.ones(n, dtype=torch.bool, device=DEV)
+    rows_ok[at:40 + rows] = False
+    assert (gq[rows_ok] - clean[0][rows_ok]).abs().max() <= tol[0]
+    assert (gk[:40] - clean[1][:40]).abs().max() <= tol[1]
+
+
+def test_rounding_error_of_out():
+    """bf16: out + rest is the fp32 result to about twice 8 bits, and with it
+    rows that see one key have no query gradient but fp32 noise."""
+    lens = [1, 60, 1, 2000]
+    n = sum(lens)
+    q, k, v, g = inputs(12, n, n, 8, 2, 64, BF16)
+    o = offsets(lens)
+    print("rest", flush=True)
+    rest = torch.full_like(q, math.nan)
+    out, lse = abi.attn_forward(q, k, v, o, o, causal=True, rest=rest)
+    want = attention(q, k, v, o, o, causal=True)["out"]
+    u = torch.finfo(BF16).eps / 2
+    # P is rounded; the result is not: the bound's other half is u^2 |out|
+    assert_within(out.double() + rest.double(), (want[0], want[1] / 2 + u * u * abs(want[0])),
+                  "out + rest")
+    gq, _, _ = abi.attn_backward(g, q, k, v, out, lse, o, o, causal=True, rest=rest)
+    want = attention(q, k, v, o, o, None, True, None, g)["dq"]
+    assert_within(gq, want, "dq")
+    size = (g.double().abs() * v.double().abs().amax()).sum(-1).amax().item()
+    first = gq[[0, 1, 61, 62]].double().abs().max().item()
+    assert first <= 64 * 2.0 ** -24 * 8 * size, first
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("heads,kv_heads,dim", [(8, 8, 32), (4, 4, 64), (8, 4, 128), (9, 3, 40)])
+def test_shared_tiles(dtype, heads, kv_heads, dim):
+    """Enough rows for whole 128-row tiles on every CU (both sides)."""
+    lens = [40000 // kv_heads // 3 + 77, 1, 0, 130, 3000]
+    n = sum(lens)
+    if heads == 9 and dtype == BF16:
+        lens = [n, 0, 63]
+        n = sum(lens)
+    q, k, v, g = inputs(13, n, n, heads, kv_heads, dim, dtype)
+    o = offsets(lens)
+    print("shared tiles", n, heads, kv_heads, dim, dtype, flush=True)
+    out, lse = abi.attn_forward(q, k, v, o, o, causal=True)
+    grads = abi.attn_backward(g, q, k, v, out, lse, o, o, causal=True)
+    for s in range(len(lens)):  # fp64 by the sequence, on the device
+        sl = slice(int(o[s]), int(o[s + 1]))
+        if lens[s] == 0:
+            continue
+        for h in range(0, heads, max(1, heads // 2)):
+            b = h // (heads // kv_heads)
+            Q, K, V, G = (t.double() for t in (q[sl, h], k[sl, b], v[sl, b], g[sl, h]))
+            S = (Q @ K.t()) * dim ** -0.5
+            S.masked_fill_(torch.ones_like(S, dtype=torch.bool).triu(1), -math.inf)
+            P = S.softmax(-1)
+            del S
+            O = P @ V
+            u = torch.finfo(BF16).eps / 2 if dtype == BF16 else 0.0
+            e = 2.0 ** -24 * (dim + lens[s] + 16) * 8
+            err = (out[sl, h].double() - O).abs() - 1.01 * (2 * u + e) * (P @ V.abs())
+            assert err.max() <= 0, (s, h, "out")
+            big = (G.abs() * O.abs()).sum(1, keepdim=True)
+            dS = P * (G @ V.t() - (G * O).sum(1, keepdim=True))
+            bound = u * (dS.abs() + P * big) + 3 * e * P * (G.abs() @ V.abs().t() + big)
+            want = dim ** -0.5 * (dS @ K)
+            err = ((grads[0][sl, h].double() - want).abs()
+                   - 1.01 * (dim ** -0.5 * (bound @ K.abs()) + u * want.abs()))
+            assert err.max() <= 0, (s, h, "dq")
+    # the keys' gradients against the same in smaller pieces: each head of a
+    # group by itself, added in fp64
+    h0 = heads // kv_heads
+    parts = []
+    for h in range(h0):
+        o1, l1 = abi.attn_forward(q[:, h:h + 1], k[:, :1], v[:, :1], o, o, causal=True)
+        parts.append(abi.attn_backward(g[:, h:h + 1], q[:, h:h + 1], k[:, :1], v[:, :1], o1, l1,
+                                       o, o, causal=True))
+    for i, name in ((1, "dk"), (2, "dv")):
+        want = sum(p[i][:, 0].double() for p in parts)
+        # each side rounds its results and the operands of its sums
+        tol = (h0 + 1) * 4 * torch.finfo(dtype).eps * want.abs().max()
+        if dtype == F32:
+            tol = 1e-4 * want.abs().max()
+        assert (grads[i][:, 0].double() - want).abs().max() <= tol, name
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
 def test_large_scores(dtype):
     """Scores of a few thousand: the maximum is taken off before the exponential."""
     q, k, v, g = inputs(7, 200, 200, 2, 2, 64, F32)
@@ -235,8 +349,9 @@ def test_autograd_and_streams(dtype):
     n = sum(lens)
     q, k, v, g = inputs(9, n, n, h, 1, dim, dtype)
     o = offsets(lens)
-    ref, lse = abi.attn_forward(q, k, v, o, o, causal=True)
-    refs = abi.attn_backward(g, q, k, v, ref, lse, o, o, causal=True)
+    rest = torch.empty_like(q) if dtype == BF16 else None  # as the layer keeps it
+    ref, lse = abi.attn_forward(q, k, v, o, o, causal=True, rest=rest)
+    refs = abi.attn_backward(g, q, k, v, ref, lse, o, o, causal=True, rest=rest)
     leaves = [t.clone().requires_grad_() for t in (q, k, v)]
     torch.cuda.synchronize()
     stream = torch.cuda.Stream()
