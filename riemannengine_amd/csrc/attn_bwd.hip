@@ -302,12 +302,14 @@ attn_dq_kernel(AttnArgs a) {
   for (int r = 0; r < 16; ++r)
     dp0[r] = -delta;
 
+  const typename Tile::Lane lane_at = Tile::lane_addresses();
+  const uint32_t stage_at = lds_address(stage);
   int buf = 0;
   for (int32_t kt = first; kt < kt1; kt += step) {
     wait_stream(); // as in the forward
     if constexpr (!SPLIT)
       __syncthreads();
-    char *lk = stage + buf * Shape::kBufBytes, *lv = lk + Shape::kTileBytes;
+    const typename Tile::Lane at = lane_at.in(stage_at + buf * Shape::kBufBytes);
     if (Shape::kBuffers == 2 && kt + step < kt1)
       issue(kt + step, buf ^ 1);
     const int32_t j0 = kt * kBN;
@@ -316,19 +318,20 @@ attn_dq_kernel(AttnArgs a) {
 #pragma unroll
       for (int b = 0; b < kB; ++b) {
         v16f s{}, dp = dp0;
-        Tile::row_product(lk, 32 * b, qf, s);
-        Tile::row_product(lv, 32 * b, gf, dp);
+        Tile::row_product(at, 0, 32 * b, qf, s);
+        Tile::row_product(at, Shape::kTileBytes, 32 * b, gf, dp);
 #pragma unroll
         for (int r = 0; r < 16; ++r)
           s[r] = exp2_fast(fmaf(s[r], a.c, -lse2)) * dp[r];
         if (masked) {
+          rare_path();
 #pragma unroll
           for (int r = 0; r < 16; ++r)
             s[r] = j0 + 32 * b + block_row(r) < lim ? s[r] : 0.f;
         }
         typename Tile::Block ds;
         Tile::pack(s, ds);
-        Tile::col_product(lk, 32 * b, ds, dq);
+        Tile::col_product(at, 0, 32 * b, ds, dq);
       }
     }
     if (Shape::kBuffers == 2) {
@@ -379,7 +382,7 @@ attn_dq_kernel(AttnArgs a) {
 // so P and dS are the right operands of dV^T = dO^T P and dK^T = Q^T dS as
 // they lie.
 template <typename T, int DP, bool VEC, bool SPLIT>
-__global__ __launch_bounds__(kBwdThreads, (sizeof(T) == 4 ? DP >= 64 : DP == 128) ? 1 : 2) void
+__global__ __launch_bounds__(kBwdThreads, sizeof(T) == 4 && DP >= 64 ? 1 : 2) void
 attn_dkv_kernel(AttnArgs a) {
   using Shape = BwdShape<T, DP, SPLIT, 2>;
   using Tile = AttnTile<T, DP>;
@@ -430,14 +433,14 @@ attn_dkv_kernel(AttnArgs a) {
     gs.issue(to + Shape::kTileBytes,
              static_cast<const T *>(a.go) + r0 * a.go_row + head * a.go_head, a.go_row,
              sq.lq - i0, a.dim);
-    // (lse2, -delta) of the tile's rows: 64 floats per wave
+    // (lse2, -delta) of the tile's rows, parted: for every 32 rows 32 of each
     const __amdgpu_buffer_rsrc_t rsrc =
         buf_rsrc(a.stat + static_cast<int64_t>(head) * a.n_q + r0,
                  static_cast<int64_t>(min(sq.lq - i0, kBM)) * 8);
-    if (SPLIT)
-      dma4(rsrc, lds_address(to + 2 * Shape::kTileBytes), lane * 4);
-    else if (w * 32 < kBM)
-      dma4(rsrc, lds_address(to + 2 * Shape::kTileBytes + w * 256), threadIdx.x * 4);
+    const int block = SPLIT ? 0 : w;
+    if (block * 32 < kBM)
+      dma4(rsrc, lds_address(to + 2 * Shape::kTileBytes + block * 256),
+           (block * 32 + (lane & 31)) * 8 + half * 4);
   };
   if (first < n1)
     issue(first, 0);
@@ -457,13 +460,16 @@ attn_dkv_kernel(AttnArgs a) {
   for (int db = 0; db < Tile::kDBlocks; ++db)
     dk[db] = dv[db] = v16f{};
 
+  const typename Tile::Lane lane_at = Tile::lane_addresses();
+  const uint32_t stage_at = lds_address(stage);
   int buf = 0;
   for (int32_t n = first; n < n1; n += step) {
     wait_stream();
     if constexpr (!SPLIT)
       __syncthreads();
-    char *lq = stage + buf * Shape::kBufBytes, *lg = lq + Shape::kTileBytes;
-    const char *stat = lg + Shape::kTileBytes;
+    const typename Tile::Lane at = lane_at.in(stage_at + buf * Shape::kBufBytes);
+    const uint32_t stat =
+        opaque(stage_at + buf * Shape::kBufBytes + 2 * Shape::kTileBytes + half * 16);
     if (Shape::kBuffers == 2 && n + step < n1)
       issue(n + step, buf ^ 1);
     const int32_t i0 = (it0 + n % per_head) * kBM;
@@ -472,23 +478,27 @@ attn_dkv_kernel(AttnArgs a) {
 #pragma unroll
       for (int b = 0; b < kB; ++b) {
         v16f s{}, dp;
-        float l[16];
+        // this lane's rows: 8 g + 4 half + e
 #pragma unroll
         for (int g = 0; g < 4; ++g) {
-          // rows 8 g + 4 half .. + 3: two (lse2, -delta) pairs per 16 bytes
-          const v4f *p = reinterpret_cast<const v4f *>(stat + (32 * b + 8 * g + 4 * half) * 8);
-          const v4f x = p[0], y = p[1];
-          l[4 * g] = x[0], l[4 * g + 1] = x[2], l[4 * g + 2] = y[0], l[4 * g + 3] = y[2];
-          dp[4 * g] = x[1], dp[4 * g + 1] = x[3], dp[4 * g + 2] = y[1], dp[4 * g + 3] = y[3];
-        }
-        Tile::row_product(lq, 32 * b, kf, s);
-        Tile::row_product(lg, 32 * b, vf, dp);
+          const v4f d = lds_read<v4f>(stat + b * 256 + 128 + g * 32);
 #pragma unroll
-        for (int r = 0; r < 16; ++r) {
-          s[r] = exp2_fast(fmaf(s[r], a.c, -l[r]));
-          dp[r] *= s[r];
+          for (int e = 0; e < 4; ++e)
+            dp[4 * g + e] = d[e];
+        }
+        Tile::row_product(at, Shape::kTileBytes, 32 * b, vf, dp);
+        Tile::row_product(at, 0, 32 * b, kf, s);
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+          const v4f l = lds_read<v4f>(stat + b * 256 + g * 32);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            s[4 * g + e] = exp2_fast(fmaf(s[4 * g + e], a.c, -l[e]));
+            dp[4 * g + e] *= s[4 * g + e];
+          }
         }
         if (masked) {
+          rare_path();
 #pragma unroll
           for (int r = 0; r < 16; ++r) {
             const int32_t i = i0 + 32 * b + block_row(r);
@@ -499,9 +509,9 @@ attn_dkv_kernel(AttnArgs a) {
         }
         typename Tile::Block p, ds;
         Tile::pack(s, p);
-        Tile::col_product(lg, 32 * b, p, dv);
+        Tile::col_product(at, Shape::kTileBytes, 32 * b, p, dv);
         Tile::pack(dp, ds);
-        Tile::col_product(lq, 32 * b, ds, dk);
+        Tile::col_product(at, 0, 32 * b, ds, dk);
       }
     }
     if (Shape::kBuffers == 2) {
@@ -527,9 +537,9 @@ attn_dkv_kernel(AttnArgs a) {
     uint64_t redo = __ballot(bad);
     redo = (redo | redo >> 32) & 0xffffffffull;
     if (key < room && !((redo >> (lane & 31)) & 1)) {
-      const int64_t at = (gk * a.kv_heads + kv) * a.dim;
-      Tile::template store_column<VEC>(static_cast<T *>(a.gk) + at, a.dim, a.scale, dk);
-      Tile::template store_column<VEC>(static_cast<T *>(a.gv) + at, a.dim, 1.f, dv);
+      const int64_t place = (gk * a.kv_heads + kv) * a.dim;
+      Tile::template store_column<VEC>(static_cast<T *>(a.gk) + place, a.dim, a.scale, dk);
+      Tile::template store_column<VEC>(static_cast<T *>(a.gv) + place, a.dim, 1.f, dv);
     }
     while (redo) {
       const int i = __ffsll(static_cast<unsigned long long>(redo)) - 1;
@@ -562,10 +572,10 @@ attn_dkv_kernel(AttnArgs a) {
       if (a.splits == 1) {
         finish_dkv<T>(a, sq, j, kv, rk[u], rv[u]);
       } else {
-        const int64_t at =
+        const int64_t place =
             ((split * static_cast<int64_t>(a.n_k) + sq.k0 + j) * a.kv_heads + kv) * a.dim;
-        put2(a.part_k + at, a.dim, rk[u][0], rk[u][1], 1.f);
-        put2(a.part_v + at, a.dim, rv[u][0], rv[u][1], 1.f);
+        put2(a.part_k + place, a.dim, rk[u][0], rk[u][1], 1.f);
+        put2(a.part_v + place, a.dim, rv[u][0], rv[u][1], 1.f);
       }
     }
   }

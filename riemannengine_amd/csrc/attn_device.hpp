@@ -148,31 +148,78 @@ __device__ __forceinline__ AttnSeq key_row(const AttnArgs &a, int32_t row) {
   return q;
 }
 
+// LDS reads by byte address (wave instructions' immediate offsets hold what is
+// constant, so a kernel keeps a handful of addresses per lane).
+template <typename V> __device__ __forceinline__ V lds_read(uint32_t addr) {
+  return *reinterpret_cast<const __attribute__((address_space(3))) V *>(addr);
+}
+__device__ __forceinline__ v4s lds_read_tr16(uint32_t addr) {
+  return __builtin_amdgcn_ds_read_tr16_b64_v4i16(reinterpret_cast<lds_v4s *>(addr));
+}
+
+// Keeps a branch a branch: what it guards is rare, and as selects it would
+// cost every pass.
+__device__ __forceinline__ void rare_path() { asm volatile(""); }
+
 // Rows of `DP` elements (the head width padded to 32, 64 or 128) as 16-byte
-// chunks in LDS. Chunk c of row r lies at c ^ swz(r): 16 consecutive rows
-// then hold one chunk column in 16 different bank groups (row reads), and so
-// do 4 consecutive chunks of 4 consecutive rows (transpose reads).
+// chunks in LDS, in groups of four rows: chunk c of row r lies at
+//   (r / 4) * 64 C + (c / 4) * 256 + (r % 4) * 64 + ((c % 4) ^ (r / 4 % 4)) * 16.
+// Then 16 consecutive rows hold one chunk column in 16 different bank groups
+// (row reads), so do 4 consecutive chunks of 4 consecutive rows (transpose
+// reads), and a quad of lanes that loads four chunks fetches 64 consecutive
+// bytes. Both kinds of read step by constants but for one bit, so each needs
+// two addresses per lane.
 template <typename T, int DP> struct AttnTile {
   static constexpr int E = 16 / sizeof(T);  // elements per chunk
   static constexpr int C = DP / E;          // chunks per row
   static constexpr int kDBlocks = DP / 32;  // 32-wide blocks of the head width
   static constexpr int kSteps = C / 2;      // row_product steps (two chunks each)
+  static constexpr int kGroup = 64 * C;     // bytes of four rows
   using Frag = typename Mfma<T>::Frag;      // one chunk
 
-  __device__ static __forceinline__ int swz(int row) {
-    if constexpr (C >= 16)
-      return ((row & 3) << 2) | ((row >> 2) & 3);
-    else if constexpr (C == 8)
-      return (((row >> 1) & 1) << 2) | ((row >> 2) & 3);
-    else
-      return (row >> 2) & 3;
+  // Row and chunk of the 16 bytes at position `pos` (in 16-byte units).
+  __device__ static __forceinline__ void place(int pos, int &row, int &c) {
+    const int group = pos / (4 * C), rem = pos % (4 * C);
+    row = 4 * group + (rem >> 2) % 4;
+    c = (rem >> 4) * 4 + ((rem & 3) ^ (group & 3));
   }
-  // byte address of chunk c of row
-  __device__ static __forceinline__ char *at(char *lds, int row, int c) {
-    return lds + (row * C + (c ^ swz(row))) * 16;
-  }
-  __device__ static __forceinline__ const char *at(const char *lds, int row, int c) {
-    return lds + (row * C + (c ^ swz(row))) * 16;
+
+  // A lane's addresses within a tile: of its row (l % 32) for the even and odd
+  // steps of row_product, and for the two reads of a col_product step.
+  struct Lane {
+    uint32_t row[2], col[2];
+    // the same in the tile at `lds`; opaque, so that what is constant stays an
+    // immediate offset of the reads instead of an addition for each
+    __device__ __forceinline__ Lane in(uint32_t lds) const {
+      Lane a;
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        a.row[u] = opaque(row[u] + lds);
+        a.col[u] = opaque(col[u] + lds);
+      }
+      return a;
+    }
+  };
+  __device__ static __forceinline__ Lane lane_addresses() {
+    const int lane = lane_id(), half = lane >> 5, r = lane & 31;
+    Lane a;
+    const uint32_t row = (r >> 2) * kGroup + (r & 3) * 64;
+#pragma unroll
+    for (int u = 0; u < 2; ++u)
+      a.row[u] = row + (((2 * u + half) ^ ((r >> 2) & 3)) * 16);
+    if constexpr (sizeof(T) == 2) {
+      const int i = lane & 15, g = (lane >> 4) & 1;
+#pragma unroll
+      for (int u = 0; u < 2; ++u)
+        a.col[u] = (half + 2 * u) * kGroup + (i >> 2) * 64 +
+                   ((2 * g + ((i & 3) >> 1)) ^ (half + 2 * u)) * 16 + (i & 1) * 8;
+    } else { // element l % 32 of a block: chunk l % 32 / 4; row parity in u
+      const int q = r >> 2;
+#pragma unroll
+      for (int u = 0; u < 2; ++u)
+        a.col[u] = half * kGroup + (q >> 2) * 256 + ((q & 3) ^ (half + 2 * u)) * 16 + (r & 3) * 4;
+    }
+    return a;
   }
 
   // Chunk c of a global row (E elements from p + c * E), zero past dim.
@@ -192,13 +239,14 @@ template <typename T, int DP> struct AttnTile {
   }
 
   // acc += A[32 rows x dim] B[dim x 32 columns]: A's rows row0 .. row0 + 31
-  // from the LDS tile, B the chunks a lane holds of its column.
-  __device__ static __forceinline__ void row_product(const char *lds, int row0,
+  // of the LDS tile (plus `bytes`: of one a constant further on), B the chunks
+  // a lane holds of its column.
+  __device__ static __forceinline__ void row_product(const Lane &at, int bytes, int row0,
                                                      const Frag (&b)[kSteps], v16f &acc) {
-    const int lane = lane_id(), row = row0 + (lane & 31), half = lane >> 5;
 #pragma unroll
     for (int s = 0; s < kSteps; ++s)
-      mma(*reinterpret_cast<const Frag *>(at(lds, row, 2 * s + half)), b[s], acc);
+      mma(lds_read<Frag>(at.row[s & 1] + (bytes + row0 / 4 * kGroup + (s >> 1) * 256)), b[s],
+          acc);
   }
 
   // The product of one chunk pair: lane half h holds elements (2 s + h) E ..
@@ -231,39 +279,32 @@ template <typename T, int DP> struct AttnTile {
   }
 
   // acc[db] += X^T[dim x 32 rows] B[32 rows x 32 columns]: X's rows row0 ..
-  // row0 + 31 from the LDS tile, B the block the lanes hold. Slot j of half h
+  // row0 + 31 of the LDS tile, B the block the lanes hold. Slot j of half h
   // in step s stands for row 16 s + 8 (j / 4) + 4 h + j % 4, B's own order;
   // a transpose read gives four consecutive rows of a lane's element column.
-  __device__ static __forceinline__ void col_product(const char *lds, int row0, const Block &b,
-                                                     v16f (&acc)[kDBlocks]) {
-    const int lane = lane_id(), half = lane >> 5;
+  __device__ static __forceinline__ void col_product(const Lane &at, int bytes, int row0,
+                                                     const Block &b, v16f (&acc)[kDBlocks]) {
     if constexpr (sizeof(T) == 2) {
-      const int i = lane & 15, g = (lane >> 4) & 1;
-      const int r = row0 + 4 * half + (i >> 2);
-      const int c = 2 * g + ((i & 3) >> 1), sub = (i & 1) * 8;
 #pragma unroll
       for (int s = 0; s < 2; ++s)
 #pragma unroll
         for (int db = 0; db < kDBlocks; ++db) {
-          const v4s lo = ds_read_tr16(at(lds, r + 16 * s, 4 * db + c) + sub);
-          const v4s hi = ds_read_tr16(at(lds, r + 16 * s + 8, 4 * db + c) + sub);
+          const int off = bytes + (row0 + 16 * s) / 4 * kGroup + db * 256;
+          const v4s lo = lds_read_tr16(at.col[0] + off), hi = lds_read_tr16(at.col[1] + off);
           const v8bf a = __builtin_bit_cast(
               v8bf, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
           acc[db] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, s ? b.hi : b.lo, acc[db], 0, 0, 0);
         }
     } else {
-      const int col = lane & 31;
 #pragma unroll
-      for (int e = 0; e < 16; ++e) {
-        const int r = row0 + 8 * (e >> 2) + 4 * half + (e & 3);
+      for (int e = 0; e < 16; ++e)
 #pragma unroll
         for (int db = 0; db < kDBlocks; ++db) {
-          const int d = 32 * db + col;
-          const float a =
-              reinterpret_cast<const float *>(at(lds, r, d / E))[d % E];
-          acc[db] = __builtin_amdgcn_mfma_f32_32x32x2f32(a, b.f[e], acc[db], 0, 0, 0);
+          const int off =
+              bytes + (row0 + 8 * (e >> 2)) / 4 * kGroup + db * 512 + (e & 3) * 64;
+          acc[db] = __builtin_amdgcn_mfma_f32_32x32x2f32(
+              lds_read<float>(at.col[(e >> 2) & 1] + off), b.f[e], acc[db], 0, 0, 0);
         }
-      }
     }
   }
 
@@ -339,8 +380,8 @@ __device__ __forceinline__ uint32_t lds_address(const void *p) { // wave-uniform
 // Tiles of ROWS rows streamed from global memory into swizzled LDS tiles by
 // THREADS threads (a workgroup, or a wave on its own). With VEC the loads go
 // straight to LDS and stay in flight until wait_stream: no registers, no LDS
-// writes. A row's chunk c lands at position c ^ swz(r), so the lane for that
-// position fetches chunk c; rows past `valid` and chunks past dim become zeros.
+// writes. Lanes fill LDS in order, so each fetches what belongs at its place;
+// rows past `valid` and chunks past dim become zeros.
 template <typename T, int DP, int ROWS, int THREADS, bool VEC> struct TileStream {
   using Tile = AttnTile<T, DP>;
   static constexpr int kBytes = ROWS * Tile::C * 16;
@@ -351,8 +392,8 @@ template <typename T, int DP, int ROWS, int THREADS, bool VEC> struct TileStream
     const int t = threadIdx.x % THREADS;
 #pragma unroll
     for (int i = 0; i < kPer; ++i) {
-      const int idx = t + i * THREADS, r = idx / Tile::C;
-      const int c = (idx % Tile::C) ^ Tile::swz(r);
+      int r, c;
+      Tile::place(t + i * THREADS, r, c);
       off[i] = c * Tile::E < dim ? static_cast<uint32_t>(r * row_stride * sizeof(T) + c * 16)
                                  : kBufOob;
     }
@@ -373,9 +414,9 @@ template <typename T, int DP, int ROWS, int THREADS, bool VEC> struct TileStream
     } else {
 #pragma unroll
       for (int i = 0; i < kPer; ++i) {
-        const int idx = t + i * THREADS, r = idx / Tile::C;
-        const int c = (idx % Tile::C) ^ Tile::swz(r);
-        *reinterpret_cast<uint4 *>(lds + idx * 16) =
+        int r, c;
+        Tile::place(t + i * THREADS, r, c);
+        *reinterpret_cast<uint4 *>(lds + (t + i * THREADS) * 16) =
             Tile::template chunk<false>(base + r * row_stride, c, dim, r < rows);
       }
     }

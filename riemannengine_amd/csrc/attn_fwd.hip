@@ -206,6 +206,8 @@ attn_fwd_kernel(AttnArgs a) {
     o[db] = v16f{};
   float m = -INFINITY, sum = 0.f; // of this lane's row; sum over its half of the keys
 
+  const typename Tile::Lane lane_at = Tile::lane_addresses();
+  const uint32_t stage_at = lds_address(stage);
   int buf = 0;
   for (int32_t kt = first; kt < kt1; kt += step) {
     // this tile has landed; then every wave is past its reads of the other
@@ -213,7 +215,7 @@ attn_fwd_kernel(AttnArgs a) {
     wait_stream();
     if constexpr (!SPLIT)
       __syncthreads();
-    char *lk = stage + buf * 2 * Shape::kTileBytes, *lv = lk + Shape::kTileBytes;
+    const typename Tile::Lane at = lane_at.in(stage_at + buf * 2 * Shape::kTileBytes);
     if (Shape::kBuffers == 2 && kt + step < kt1)
       issue(kt + step, buf ^ 1);
     const int32_t j0 = kt * kBN;
@@ -222,9 +224,10 @@ attn_fwd_kernel(AttnArgs a) {
 #pragma unroll
       for (int b = 0; b < kB; ++b) {
         s[b] = v16f{};
-        Tile::row_product(lk, 32 * b, qf, s[b]);
+        Tile::row_product(at, 0, 32 * b, qf, s[b]);
       }
       if (j0 + kBN > wave_full) {
+        rare_path();
 #pragma unroll
         for (int b = 0; b < kB; ++b)
 #pragma unroll
@@ -256,7 +259,7 @@ attn_fwd_kernel(AttnArgs a) {
         }
         typename Tile::Block p;
         Tile::pack(s[b], p);
-        Tile::col_product(lv, 32 * b, p, o);
+        Tile::col_product(at, Shape::kTileBytes, 32 * b, p, o);
       }
     }
     if (Shape::kBuffers == 2) {
@@ -283,11 +286,11 @@ attn_fwd_kernel(AttnArgs a) {
     }
     uint64_t redo = __ballot(bad);
     redo = (redo | redo >> 32) & 0xffffffffull;
-    const int64_t at = (sq.q0 + static_cast<int64_t>(qi)) * a.heads + head;
+    const int64_t place = (sq.q0 + static_cast<int64_t>(qi)) * a.heads + head;
     if (row_ok && !((redo >> (lane & 31)) & 1)) {
-      Tile::template store_column<VEC>(static_cast<T *>(a.o) + at * a.dim, a.dim, inv, o);
+      Tile::template store_column<VEC>(static_cast<T *>(a.o) + place * a.dim, a.dim, inv, o);
       if (sizeof(T) == 2 && a.rest)
-        Tile::template store_rest<VEC>(static_cast<T *>(a.rest) + at * a.dim, a.dim, inv, o);
+        Tile::template store_rest<VEC>(static_cast<T *>(a.rest) + place * a.dim, a.dim, inv, o);
       if (a.lse && half == 0)
         a.lse[static_cast<int64_t>(head) * a.n_q + sq.q0 + qi] =
             sum == 0.f ? -INFINITY : m * a.scale + logf(sum);
@@ -336,15 +339,15 @@ attn_fwd_kernel(AttnArgs a) {
       if (a.splits == 1) {
         finish_row<T>(a, sq, i, h, o0, o1, mr, sr);
       } else {
-        const int64_t at = split * static_cast<int64_t>(a.n_q) * a.heads +
+        const int64_t place = split * static_cast<int64_t>(a.n_q) * a.heads +
                            (sq.q0 + static_cast<int64_t>(i)) * a.heads + h;
         if (lane < a.dim)
-          a.part_o[at * a.dim + lane] = o0;
+          a.part_o[place * a.dim + lane] = o0;
         if (lane + kWave < a.dim)
-          a.part_o[at * a.dim + lane + kWave] = o1;
+          a.part_o[place * a.dim + lane + kWave] = o1;
         if (lane == 0) {
-          a.part_ml[2 * at] = mr;
-          a.part_ml[2 * at + 1] = sr;
+          a.part_ml[2 * place] = mr;
+          a.part_ml[2 * place + 1] = sr;
         }
       }
     }
