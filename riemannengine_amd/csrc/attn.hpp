@@ -37,4 +37,14 @@ template <typename F> void with_attn(int32_t dtype, int32_t dim, bool vec, F &&f
     typed(__bf16{});
 }
 
+// f(W): 32-row blocks per workgroup, 4, 2 or 1.
+template <typename F> void with_waves(int32_t waves, F &&f) {
+  if (waves == 4)
+    f(std::integral_constant<int, 4>{});
+  else if (waves == 2)
+    f(std::integral_constant<int, 2>{});
+  else
+    f(std::integral_constant<int, 1>{});
+}
+
 } // namespace rhip

@@ -7,11 +7,11 @@
 // fixed order, so results do not change from run to run; the price is that
 // scores and dp are computed twice (7 products instead of 5).
 //
-// Both have the forward's two shapes: `shared`, 128 rows (keys) per
-// workgroup, whose four waves read the same tiles of the other side, and
-// `split`, 32 rows (keys), whose waves each take every fourth 32-row tile and
-// add their sums at the end; the keys' kernel may also be split over
-// workgroups, whose partial sums a last kernel adds.
+// Both have the forward's shapes: W blocks of 32 rows (keys) per workgroup,
+// whose four waves read the same tiles of the other side (W = 4; 2: two waves
+// share a block, each with half of every tile) or tiles of their own (W = 1),
+// and add what they share at the end. With W = 1 the keys' kernel may also be
+// split over workgroups, whose partial sums a last kernel adds.
 #include "attn.hpp"
 
 namespace rhip {
@@ -19,22 +19,22 @@ namespace {
 
 constexpr int kBwdThreads = 256;
 constexpr int kBwdWaves = kBwdThreads / kWave;
-constexpr int kSharedRows = 128, kSplitRows = 32;
-// Workgroups below which the split shape is taken, and how many it aims for.
+// Workgroups below which W is halved, and how many the splits aim for.
 constexpr int64_t kFewWorkgroups = 256, kSplitTarget = 1024;
 constexpr int kMaxSplits = 32;
 
-template <typename T, int DP, bool SPLIT, int SUMS> struct BwdShape {
-  static constexpr int kRows = SPLIT ? kSplitRows : kSharedRows;
-  static constexpr int kBN = SPLIT || (sizeof(T) == 4 && DP == 128) ? 32 : 64;
-  static constexpr int kStreams = SPLIT ? kBwdWaves : 1;
+template <typename T, int DP, int W> struct BwdShape {
+  static constexpr int kRows = 32 * W;
+  static constexpr int kParts = kBwdWaves / W; // waves that share a block of rows
+  static constexpr int kBN = W == 1 || (W == 4 && sizeof(T) == 4 && DP == 128) ? 32 : 64;
+  static constexpr int kStreams = W == 1 ? kBwdWaves : 1;
   static constexpr int kTileBytes = kBN * DP * sizeof(T);
   static constexpr int kStatBytes = kBN * 8; // (lse2, -delta) of a tile's rows
   static constexpr int kBufBytes = 2 * kTileBytes + kStatBytes;
   static constexpr int kBuffers = kStreams * 2 * kBufBytes <= 160 * 1024 ? 2 : 1;
   static constexpr int kJoinRow = DP + 4; // floats per row of the joined sums
   static constexpr int kJoinBytes =
-      SPLIT ? kBwdWaves * 32 * kJoinRow * static_cast<int>(sizeof(float)) : 0;
+      W < 4 ? kBwdWaves * 32 * kJoinRow * static_cast<int>(sizeof(float)) : 0;
   static constexpr int kStageBytes = kStreams * kBuffers * kBufBytes;
   static constexpr int kLds = kStageBytes > kJoinBytes ? kStageBytes : kJoinBytes;
 };
@@ -193,15 +193,16 @@ __device__ __forceinline__ void spill_columns(float *rows, int row_floats, const
       *reinterpret_cast<v4f *>(mine + 32 * db + 8 * g + 4 * half) =
           v4f{acc[db][4 * g], acc[db][4 * g + 1], acc[db][4 * g + 2], acc[db][4 * g + 3]};
 }
-// Elements lane and lane + 64 of row r, summed over the waves in order.
-template <int DP>
+// Elements lane and lane + 64 of row r of the workgroup's, summed over the
+// PARTS waves that share it in order.
+template <int DP, int PARTS>
 __device__ __forceinline__ void join_row(const float *rows, int row_floats, int r, float &v0,
                                          float &v1) {
   const int lane = lane_id();
   v0 = v1 = 0.f;
 #pragma unroll
-  for (int i = 0; i < kBwdWaves; ++i) {
-    const float *src = rows + (i * 32 + r) * row_floats;
+  for (int i = 0; i < PARTS; ++i) {
+    const float *src = rows + ((r / 32 * PARTS + i) * 32 + r % 32) * row_floats;
     if (lane < DP)
       v0 += src[lane];
     if (DP > kWave)
@@ -213,14 +214,15 @@ __device__ __forceinline__ void join_row(const float *rows, int row_floats, int 
 // also the rows' statistics. Blocks are transposed as in the forward (S^T = K
 // Q^T, dP^T = V dO^T), so dS^T is the right operand of dQ^T = K^T dS^T as it
 // lies. dP's sums start at -delta.
-template <typename T, int DP, bool VEC, bool SPLIT>
+template <typename T, int DP, bool VEC, int W>
 __global__ __launch_bounds__(kBwdThreads, sizeof(T) == 4 && DP == 128 ? 1 : 2) void
 attn_dq_kernel(AttnArgs a) {
-  using Shape = BwdShape<T, DP, SPLIT, 1>;
+  using Shape = BwdShape<T, DP, W>;
   using Tile = AttnTile<T, DP>;
   using Frag = typename Tile::Frag;
-  constexpr int kBN = Shape::kBN, kB = kBN / 32;
-  using Stream = TileStream<T, DP, kBN, SPLIT ? kWave : kBwdThreads, VEC>;
+  constexpr int kBN = Shape::kBN;
+  constexpr int kB = W == 2 ? 1 : kBN / 32; // blocks of a tile that are a wave's
+  using Stream = TileStream<T, DP, kBN, W == 1 ? kWave : kBwdThreads, VEC>;
   __shared__ alignas(16) char lds[Shape::kLds];
 
   int32_t t, kv, split;
@@ -232,7 +234,8 @@ attn_dq_kernel(AttnArgs a) {
     return;
   const int lane = lane_id(), half = lane >> 5;
   const int w = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
-  const int32_t wave0 = row0 + (SPLIT ? 0 : w * 32);
+  const int32_t wave0 = row0 + w / Shape::kParts * 32;
+  const int b0 = W == 2 ? w % 2 : 0; // the wave's first block of a tile
   const int32_t row = wave0 + (lane & 31);
   const bool row_ok = row < n_rows;
   const int32_t rc = min(row, n_rows - 1);
@@ -244,14 +247,14 @@ attn_dq_kernel(AttnArgs a) {
   const int32_t wave_lim = wave0 < n_rows ? sees(min(wave0 + 32, n_rows) - 1) : 0;
   const int32_t wave_full = wave0 < n_rows ? sees(wave0) : 0;
   const int32_t kt1 = a.gq ? (wg_lim + kBN - 1) / kBN : 0; // else statistics alone
-  const int32_t first = SPLIT ? w : 0, step = SPLIT ? kBwdWaves : 1;
+  const int32_t first = W == 1 ? w : 0, step = W == 1 ? kBwdWaves : 1;
 
   const T *kp = static_cast<const T *>(a.k) + sq.k0 * a.k_row + kv * a.k_head;
   const T *vp = static_cast<const T *>(a.v) + sq.k0 * a.v_row + kv * a.v_head;
   Stream ks, vs;
   ks.init(a.k_row, a.dim);
   vs.init(a.v_row, a.dim);
-  char *stage = lds + (SPLIT ? w : 0) * Shape::kBuffers * Shape::kBufBytes;
+  char *stage = lds + (W == 1 ? w : 0) * Shape::kBuffers * Shape::kBufBytes;
   auto issue = [&](int32_t kt, int buf) {
     char *to = stage + buf * Shape::kBufBytes;
     ks.issue(to, kp + static_cast<int64_t>(kt) * kBN * a.k_row, a.k_row, sq.lk - kt * kBN,
@@ -290,7 +293,7 @@ attn_dq_kernel(AttnArgs a) {
   if (row_ok) {
     const int64_t li = static_cast<int64_t>(head) * a.n_q + gr;
     lse2 = a.lse[li] * kLog2e;
-    if (half == 0 && (!SPLIT || w == 0))
+    if (half == 0 && w % Shape::kParts == 0)
       a.stat[li] = make_float2(lse2, -delta);
   }
 
@@ -307,14 +310,15 @@ attn_dq_kernel(AttnArgs a) {
   int buf = 0;
   for (int32_t kt = first; kt < kt1; kt += step) {
     wait_stream(); // as in the forward
-    if constexpr (!SPLIT)
+    if constexpr (W > 1)
       __syncthreads();
-    const typename Tile::Lane at = lane_at.in(stage_at + buf * Shape::kBufBytes);
+    const typename Tile::Lane at =
+        lane_at.in(stage_at + buf * Shape::kBufBytes + b0 * (32 / 4) * Tile::kGroup);
     if (Shape::kBuffers == 2 && kt + step < kt1)
       issue(kt + step, buf ^ 1);
-    const int32_t j0 = kt * kBN;
-    if (SPLIT || j0 < wave_lim) {
-      const bool masked = j0 + kBN > wave_full;
+    const int32_t j0 = kt * kBN + 32 * b0;
+    if (W == 1 || j0 < wave_lim) {
+      const bool masked = j0 + 32 * kB > wave_full;
 #pragma unroll
       for (int b = 0; b < kB; ++b) {
         v16f s{}, dp = dp0;
@@ -338,14 +342,14 @@ attn_dq_kernel(AttnArgs a) {
       buf ^= 1;
     } else if (kt + step < kt1) {
       wait_stream();
-      if constexpr (!SPLIT)
+      if constexpr (W > 1)
         __syncthreads();
       issue(kt + step, 0);
     }
   }
   if (!a.gq)
     return;
-  if constexpr (!SPLIT) {
+  if constexpr (W == 4) {
     bool bad = false;
     if (a.causal && row_ok) {
 #pragma unroll
@@ -369,9 +373,9 @@ attn_dq_kernel(AttnArgs a) {
     float *join = reinterpret_cast<float *>(lds);
     spill_columns(join + w * 32 * Shape::kJoinRow, Shape::kJoinRow, dq);
     __syncthreads();
-    for (int r = w; r < 32 && row0 + r < n_rows; r += kBwdWaves) {
+    for (int r = w; r < Shape::kRows && row0 + r < n_rows; r += kBwdWaves) {
       float g0, g1;
-      join_row<DP>(join, Shape::kJoinRow, r, g0, g1);
+      join_row<DP, Shape::kParts>(join, Shape::kJoinRow, r, g0, g1);
       finish_dq<T>(a, sq, (row0 + r) / a.group, kv * a.group + (row0 + r) % a.group, g0, g1);
     }
   }
@@ -381,14 +385,15 @@ attn_dq_kernel(AttnArgs a) {
 // head of its group. A lane holds one key's column (S = Q K^T, dP = dO V^T),
 // so P and dS are the right operands of dV^T = dO^T P and dK^T = Q^T dS as
 // they lie.
-template <typename T, int DP, bool VEC, bool SPLIT>
+template <typename T, int DP, bool VEC, int W>
 __global__ __launch_bounds__(kBwdThreads, sizeof(T) == 4 && DP >= 64 ? 1 : 2) void
 attn_dkv_kernel(AttnArgs a) {
-  using Shape = BwdShape<T, DP, SPLIT, 2>;
+  using Shape = BwdShape<T, DP, W>;
   using Tile = AttnTile<T, DP>;
   using Frag = typename Tile::Frag;
-  constexpr int kBM = Shape::kBN, kB = kBM / 32;
-  using Stream = TileStream<T, DP, kBM, SPLIT ? kWave : kBwdThreads, VEC>;
+  constexpr int kBM = Shape::kBN;
+  constexpr int kB = W == 2 ? 1 : kBM / 32;
+  using Stream = TileStream<T, DP, kBM, W == 1 ? kWave : kBwdThreads, VEC>;
   __shared__ alignas(16) char lds[Shape::kLds];
 
   int32_t t, kv, split;
@@ -401,7 +406,8 @@ attn_dkv_kernel(AttnArgs a) {
     return;
   const int lane = lane_id(), half = lane >> 5;
   const int w = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
-  const int32_t wave0 = key0 + (SPLIT ? 0 : w * 32);
+  const int32_t wave0 = key0 + w / Shape::kParts * 32;
+  const int b0 = W == 2 ? w % 2 : 0;
   const int32_t key = wave0 + (lane & 31);
   const bool key_ok = key < sq.lk;
   const int32_t lo = first_row(a, sq, key);
@@ -412,17 +418,17 @@ attn_dkv_kernel(AttnArgs a) {
   // workgroup's part of them
   const int32_t per_head = key0 < sq.lk ? max((sq.lq + kBM - 1) / kBM - it0, 0) : 0;
   int32_t n0 = 0, n1 = per_head * a.group;
-  if (SPLIT && a.splits > 1) {
+  if (W == 1 && a.splits > 1) {
     const int32_t per = (n1 + a.splits - 1) / a.splits;
     n0 = min(split * per, n1);
     n1 = min(n0 + per, n1);
   }
-  const int32_t first = n0 + (SPLIT ? w : 0), step = SPLIT ? kBwdWaves : 1;
+  const int32_t first = n0 + (W == 1 ? w : 0), step = W == 1 ? kBwdWaves : 1;
 
   Stream qs, gs;
   qs.init(a.q_row, a.dim);
   gs.init(a.go_row, a.dim);
-  char *stage = lds + (SPLIT ? w : 0) * Shape::kBuffers * Shape::kBufBytes;
+  char *stage = lds + (W == 1 ? w : 0) * Shape::kBuffers * Shape::kBufBytes;
   auto issue = [&](int32_t n, int buf) {
     const int h = n / per_head, head = kv * a.group + h;
     const int32_t i0 = (it0 + n - h * per_head) * kBM;
@@ -437,7 +443,7 @@ attn_dkv_kernel(AttnArgs a) {
     const __amdgpu_buffer_rsrc_t rsrc =
         buf_rsrc(a.stat + static_cast<int64_t>(head) * a.n_q + r0,
                  static_cast<int64_t>(min(sq.lq - i0, kBM)) * 8);
-    const int block = SPLIT ? 0 : w;
+    const int block = W == 1 ? 0 : w;
     if (block * 32 < kBM)
       dma4(rsrc, lds_address(to + 2 * Shape::kTileBytes + block * 256),
            (block * 32 + (lane & 31)) * 8 + half * 4);
@@ -465,16 +471,17 @@ attn_dkv_kernel(AttnArgs a) {
   int buf = 0;
   for (int32_t n = first; n < n1; n += step) {
     wait_stream();
-    if constexpr (!SPLIT)
+    if constexpr (W > 1)
       __syncthreads();
-    const typename Tile::Lane at = lane_at.in(stage_at + buf * Shape::kBufBytes);
-    const uint32_t stat =
-        opaque(stage_at + buf * Shape::kBufBytes + 2 * Shape::kTileBytes + half * 16);
+    const typename Tile::Lane at =
+        lane_at.in(stage_at + buf * Shape::kBufBytes + b0 * (32 / 4) * Tile::kGroup);
+    const uint32_t stat = opaque(stage_at + buf * Shape::kBufBytes + 2 * Shape::kTileBytes +
+                                 b0 * 256 + half * 16);
     if (Shape::kBuffers == 2 && n + step < n1)
       issue(n + step, buf ^ 1);
-    const int32_t i0 = (it0 + n % per_head) * kBM;
-    if (i0 + kBM > wave_lo) {
-      const bool masked = i0 < wave_full || i0 + kBM > sq.lq;
+    const int32_t i0 = (it0 + n % per_head) * kBM + 32 * b0;
+    if (i0 + 32 * kB > wave_lo) {
+      const bool masked = i0 < wave_full || i0 + 32 * kB > sq.lq;
 #pragma unroll
       for (int b = 0; b < kB; ++b) {
         v16f s{}, dp;
@@ -518,14 +525,14 @@ attn_dkv_kernel(AttnArgs a) {
       buf ^= 1;
     } else if (n + step < n1) {
       wait_stream();
-      if constexpr (!SPLIT)
+      if constexpr (W > 1)
         __syncthreads();
       issue(n + step, 0);
     }
   }
 
   // rows behind the keys in use get zeros (no tile was added to them)
-  if constexpr (!SPLIT) {
+  if constexpr (W == 4) {
     bool bad = false;
     if (a.causal && key_ok) {
 #pragma unroll
@@ -551,21 +558,22 @@ attn_dkv_kernel(AttnArgs a) {
     // add the waves' sums, dk then dv through the same LDS; a wave ends with
     // rows w, w + 4, .. of both
     float *join = reinterpret_cast<float *>(lds);
-    float rk[32 / kBwdWaves][2], rv[32 / kBwdWaves][2];
+    constexpr int kMine = Shape::kRows / kBwdWaves;
+    float rk[kMine][2], rv[kMine][2];
     __syncthreads();
     spill_columns(join + w * 32 * Shape::kJoinRow, Shape::kJoinRow, dk);
     __syncthreads();
 #pragma unroll
-    for (int u = 0; u < 32 / kBwdWaves; ++u)
-      join_row<DP>(join, Shape::kJoinRow, w + u * kBwdWaves, rk[u][0], rk[u][1]);
+    for (int u = 0; u < kMine; ++u)
+      join_row<DP, Shape::kParts>(join, Shape::kJoinRow, w + u * kBwdWaves, rk[u][0], rk[u][1]);
     __syncthreads();
     spill_columns(join + w * 32 * Shape::kJoinRow, Shape::kJoinRow, dv);
     __syncthreads();
 #pragma unroll
-    for (int u = 0; u < 32 / kBwdWaves; ++u)
-      join_row<DP>(join, Shape::kJoinRow, w + u * kBwdWaves, rv[u][0], rv[u][1]);
+    for (int u = 0; u < kMine; ++u)
+      join_row<DP, Shape::kParts>(join, Shape::kJoinRow, w + u * kBwdWaves, rv[u][0], rv[u][1]);
 #pragma unroll
-    for (int u = 0; u < 32 / kBwdWaves; ++u) {
+    for (int u = 0; u < kMine; ++u) {
       const int32_t j = key0 + w + u * kBwdWaves;
       if (j >= room)
         break;
@@ -605,26 +613,24 @@ __global__ __launch_bounds__(kBwdThreads) void attn_dkv_join_kernel(AttnArgs a) 
 }
 
 struct BwdPlan {
-  bool split;
+  int32_t waves; // W
   int64_t tiles;
   int32_t splits;
 };
 // Over n rows (packed query rows or keys) for each key head; `others`: rows of
 // the other side, all sequences and heads of a group counted.
 BwdPlan plan_backward(int64_t n, int32_t n_seq, int32_t kv_heads, int64_t others, bool splits) {
-  BwdPlan p{false, n / kSharedRows + n_seq + 1, 1};
-  if (n / kSharedRows * kv_heads >= kFewWorkgroups)
+  BwdPlan p{4, 0, 1};
+  while (p.waves > 1 && n / (32 * p.waves) * kv_heads < kFewWorkgroups)
+    p.waves /= 2;
+  p.tiles = n / (32 * p.waves) + n_seq + 1;
+  if (p.waves > 1 || !splits)
     return p;
-  p.split = true;
-  p.tiles = n / kSplitRows + n_seq + 1;
-  if (!splits)
-    return p;
-  const int64_t busy =
-      std::max<int64_t>(1, (n / kSplitRows + std::min<int64_t>(n_seq, n)) * kv_heads);
+  const int64_t busy = std::max<int64_t>(1, (n / 32 + std::min<int64_t>(n_seq, n)) * kv_heads);
   // a split gets four 32-row tiles for each wave, at least
   const int64_t rows = n_seq > 0 ? others / n_seq : 0;
   p.splits = static_cast<int32_t>(std::max<int64_t>(
-      1, std::min<int64_t>({kSplitTarget / busy, rows / (16 * kSplitRows), kMaxSplits})));
+      1, std::min<int64_t>({kSplitTarget / busy, rows / 512, kMaxSplits})));
   return p;
 }
 
@@ -661,18 +667,18 @@ void attn_backward_run(const AttnArgs &args, int32_t dtype, bool vec, hipStream_
     constexpr bool VEC = decltype(v)::value;
     const dim3 b(kBwdThreads);
     if (args.n_q > 0) {
-      if (pq.split)
-        hipLaunchKernelGGL((attn_dq_kernel<T, DP, VEC, true>), dim3(gq), b, 0, stream, aq);
-      else
-        hipLaunchKernelGGL((attn_dq_kernel<T, DP, VEC, false>), dim3(gq), b, 0, stream, aq);
+      with_waves(pq.waves, [&](auto w) {
+        hipLaunchKernelGGL((attn_dq_kernel<T, DP, VEC, decltype(w)::value>), dim3(gq), b, 0,
+                           stream, aq);
+      });
       RHIP_LAUNCH_CHECK();
     }
     if (!args.gk || args.n_k == 0)
       return;
-    if (pk.split)
-      hipLaunchKernelGGL((attn_dkv_kernel<T, DP, VEC, true>), dim3(gk), b, 0, stream, ak);
-    else
-      hipLaunchKernelGGL((attn_dkv_kernel<T, DP, VEC, false>), dim3(gk), b, 0, stream, ak);
+    with_waves(pk.waves, [&](auto w) {
+      hipLaunchKernelGGL((attn_dkv_kernel<T, DP, VEC, decltype(w)::value>), dim3(gk), b, 0,
+                         stream, ak);
+    });
     RHIP_LAUNCH_CHECK();
     if (pk.splits > 1) {
       const int64_t rows = static_cast<int64_t>(args.n_k) * args.kv_heads;

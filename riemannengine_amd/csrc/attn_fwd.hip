@@ -4,14 +4,14 @@
 //
 // The heads of a group are packed: row r of a key head's sequence is query
 // row r / group, head r % group, so all rows that read the same keys stand in
-// the same tiles. Two launch shapes share one kernel:
-//   shared  128 rows per workgroup, 32 per wave; the four waves read the same
-//           LDS tiles of keys;
-//   split   32 rows per workgroup; each wave takes every fourth 32-key tile
-//           through LDS tiles of its own (no barrier until the end) and the
-//           waves' results are joined in LDS. The keys may further be split
-//           over workgroups, joined by a second kernel. For single tokens and
-//           wherever 128-row tiles leave the chip empty.
+// the same tiles. A workgroup's four waves hold W blocks of 32 rows:
+//   W = 4  each wave has a block; all read the same LDS tiles of keys;
+//   W = 2  two waves share a block, each with half of every tile's keys;
+//   W = 1  all share one, each with every fourth tile of 32 keys, through LDS
+//          tiles of its own (no barrier until the end).
+// Waves that share rows join their sums in LDS at the end. With W = 1 the
+// keys may further be split over workgroups, joined by a second kernel: for
+// single tokens, and wherever larger tiles leave the chip empty.
 #include "attn.hpp"
 
 namespace rhip {
@@ -19,22 +19,22 @@ namespace {
 
 constexpr int kFwdThreads = 256;
 constexpr int kFwdWaves = kFwdThreads / kWave;
-constexpr int kSharedRows = 128, kSplitRows = 32;
-// Workgroups below which the split shape is taken, and how many it aims for.
+// Workgroups below which W is halved, and how many the splits aim for.
 constexpr int64_t kFewWorkgroups = 256, kSplitTarget = 1024;
 constexpr int kMaxSplits = 64, kMinSplitKeys = 256;
 
-template <typename T, int DP, bool SPLIT> struct FwdShape {
-  static constexpr int kRows = SPLIT ? kSplitRows : kSharedRows;
+template <typename T, int DP, int W> struct FwdShape {
+  static constexpr int kRows = 32 * W;
+  static constexpr int kParts = kFwdWaves / W; // waves that share a block of rows
   // keys per LDS tile: two 32-key blocks where they fit
-  static constexpr int kBN = SPLIT || (sizeof(T) == 4 && DP == 128) ? 32 : 64;
-  static constexpr int kStreams = SPLIT ? kFwdWaves : 1;
+  static constexpr int kBN = W == 1 || (W == 4 && sizeof(T) == 4 && DP == 128) ? 32 : 64;
+  static constexpr int kStreams = W == 1 ? kFwdWaves : 1;
   static constexpr int kTileBytes = kBN * DP * sizeof(T);
   // two buffers, but for fp32 at full width where four waves' would not fit
   static constexpr int kBuffers = kStreams * 4 * kTileBytes <= 160 * 1024 ? 2 : 1;
   static constexpr int kJoinRow = DP + 4; // floats per row of the joined results
   static constexpr int kJoinBytes =
-      SPLIT ? kFwdWaves * 32 * (kJoinRow + 2) * static_cast<int>(sizeof(float)) : 0;
+      W < 4 ? kFwdWaves * 32 * (kJoinRow + 2) * static_cast<int>(sizeof(float)) : 0;
   static constexpr int kStageBytes = kStreams * kBuffers * 2 * kTileBytes;
   static constexpr int kLds = kStageBytes > kJoinBytes ? kStageBytes : kJoinBytes;
 };
@@ -133,14 +133,15 @@ __device__ void finish_row(const AttnArgs &a, const AttnSeq &sq, int32_t i, int3
 // in-lane but for one exchange, and P^T is the right operand of O^T = V^T P^T
 // as it lies. The next tile's loads are in flight while this one is
 // multiplied.
-template <typename T, int DP, bool VEC, bool SPLIT>
+template <typename T, int DP, bool VEC, int W>
 __global__ __launch_bounds__(kFwdThreads, sizeof(T) == 4 && DP == 128 ? 1 : 2) void
 attn_fwd_kernel(AttnArgs a) {
-  using Shape = FwdShape<T, DP, SPLIT>;
+  using Shape = FwdShape<T, DP, W>;
   using Tile = AttnTile<T, DP>;
   using Frag = typename Tile::Frag;
-  constexpr int kBN = Shape::kBN, kB = kBN / 32;
-  using Stream = TileStream<T, DP, kBN, SPLIT ? kWave : kFwdThreads, VEC>;
+  constexpr int kBN = Shape::kBN;
+  constexpr int kB = W == 2 ? 1 : kBN / 32; // blocks of a tile that are a wave's
+  using Stream = TileStream<T, DP, kBN, W == 1 ? kWave : kFwdThreads, VEC>;
   __shared__ alignas(16) char lds[Shape::kLds];
 
   int32_t t, kv, split;
@@ -152,7 +153,8 @@ attn_fwd_kernel(AttnArgs a) {
     return;
   const int lane = lane_id(), half = lane >> 5;
   const int w = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
-  const int32_t wave0 = row0 + (SPLIT ? 0 : w * 32);
+  const int32_t wave0 = row0 + w / Shape::kParts * 32;
+  const int b0 = W == 2 ? w % 2 : 0; // the wave's first block of a tile
   const int32_t row = wave0 + (lane & 31); // this lane's packed row
   const bool row_ok = row < n_rows;
   const int32_t rc = min(row, n_rows - 1);
@@ -170,19 +172,19 @@ attn_fwd_kernel(AttnArgs a) {
   const int32_t wave_full = wave0 < n_rows ? sees(wave0) : 0; // seen by all its rows
   // this workgroup's tiles [kt0, kt1) of keys; a wave's first and step
   int32_t kt0 = 0, kt1 = (wg_lim + kBN - 1) / kBN;
-  if (SPLIT && a.splits > 1) {
+  if (W == 1 && a.splits > 1) {
     const int32_t per = (kt1 + a.splits - 1) / a.splits;
     kt0 = min(split * per, kt1);
     kt1 = min(kt0 + per, kt1);
   }
-  const int32_t first = kt0 + (SPLIT ? w : 0), step = SPLIT ? kFwdWaves : 1;
+  const int32_t first = kt0 + (W == 1 ? w : 0), step = W == 1 ? kFwdWaves : 1;
 
   const T *kp = static_cast<const T *>(a.k) + sq.k0 * a.k_row + kv * a.k_head;
   const T *vp = static_cast<const T *>(a.v) + sq.k0 * a.v_row + kv * a.v_head;
   Stream ks, vs;
   ks.init(a.k_row, a.dim);
   vs.init(a.v_row, a.dim);
-  char *stage = lds + (SPLIT ? w : 0) * Shape::kBuffers * 2 * Shape::kTileBytes;
+  char *stage = lds + (W == 1 ? w : 0) * Shape::kBuffers * 2 * Shape::kTileBytes;
   auto issue = [&](int32_t kt, int buf) {
     char *to = stage + buf * 2 * Shape::kTileBytes;
     ks.issue(to, kp + static_cast<int64_t>(kt) * kBN * a.k_row, a.k_row, sq.lk - kt * kBN,
@@ -213,20 +215,20 @@ attn_fwd_kernel(AttnArgs a) {
     // this tile has landed; then every wave is past its reads of the other
     // buffer, which the next tile's loads overwrite
     wait_stream();
-    if constexpr (!SPLIT)
+    if constexpr (W > 1)
       __syncthreads();
-    const typename Tile::Lane at = lane_at.in(stage_at + buf * 2 * Shape::kTileBytes);
+    const typename Tile::Lane at = lane_at.in(stage_at + buf * 2 * Shape::kTileBytes + b0 * (32 / 4) * Tile::kGroup);
     if (Shape::kBuffers == 2 && kt + step < kt1)
       issue(kt + step, buf ^ 1);
-    const int32_t j0 = kt * kBN;
-    if (SPLIT || j0 < wave_lim) {
+    const int32_t j0 = kt * kBN + 32 * b0;
+    if (W == 1 || j0 < wave_lim) {
       v16f s[kB];
 #pragma unroll
       for (int b = 0; b < kB; ++b) {
         s[b] = v16f{};
         Tile::row_product(at, 0, 32 * b, qf, s[b]);
       }
-      if (j0 + kBN > wave_full) {
+      if (j0 + 32 * kB > wave_full) {
         rare_path();
 #pragma unroll
         for (int b = 0; b < kB; ++b)
@@ -266,14 +268,14 @@ attn_fwd_kernel(AttnArgs a) {
       buf ^= 1;
     } else if (kt + step < kt1) {
       wait_stream();
-      if constexpr (!SPLIT)
+      if constexpr (W > 1)
         __syncthreads();
       issue(kt + step, 0);
     }
   }
   sum = pair_sum(sum);
 
-  if constexpr (!SPLIT) {
+  if constexpr (W == 4) {
     const float inv = sum == 0.f ? 0.f : 1.f / sum;
     bool bad = false;
     if (a.causal) {
@@ -317,18 +319,20 @@ attn_fwd_kernel(AttnArgs a) {
       jm[(w * 32 + lane) * 2 + 1] = sum;
     }
     __syncthreads();
-    for (int r = w; r < 32 && row0 + r < n_rows; r += kFwdWaves) {
+    for (int r = w; r < Shape::kRows && row0 + r < n_rows; r += kFwdWaves) {
+      // the row in the first of its waves' results
+      const int first_at = r / 32 * Shape::kParts * 32 + r % 32;
       float mr = -INFINITY;
 #pragma unroll
-      for (int i = 0; i < kFwdWaves; ++i)
-        mr = fmaxf(mr, jm[(i * 32 + r) * 2]);
+      for (int i = 0; i < Shape::kParts; ++i)
+        mr = fmaxf(mr, jm[(i * 32 + first_at) * 2]);
       const float base = (mr == -INFINITY ? 0.f : mr) * a.c;
       float o0 = 0.f, o1 = 0.f, sr = 0.f;
 #pragma unroll
-      for (int i = 0; i < kFwdWaves; ++i) {
-        const float f = exp2_fast(jm[(i * 32 + r) * 2] * a.c - base);
-        sr = fmaf(jm[(i * 32 + r) * 2 + 1], f, sr);
-        const float *src = jo + (i * 32 + r) * Shape::kJoinRow;
+      for (int i = 0; i < Shape::kParts; ++i) {
+        const float f = exp2_fast(jm[(i * 32 + first_at) * 2] * a.c - base);
+        sr = fmaf(jm[(i * 32 + first_at) * 2 + 1], f, sr);
+        const float *src = jo + (i * 32 + first_at) * Shape::kJoinRow;
         if (lane < DP)
           o0 = fmaf(src[lane], f, o0);
         if (DP > kWave)
@@ -383,20 +387,21 @@ __global__ __launch_bounds__(kFwdThreads) void attn_join_kernel(AttnArgs a) {
 }
 
 struct FwdPlan {
-  bool split;
+  int32_t waves; // W
   int64_t tiles;
   int32_t splits;
 };
 FwdPlan plan_forward(int64_t n_q, int64_t n_k, int32_t n_seq, int32_t heads, int32_t kv_heads) {
   const int64_t rows = n_q * (heads / kv_heads);
-  FwdPlan p{false, rows / kSharedRows + n_seq + 1, 1};
-  if (rows / kSharedRows * kv_heads >= kFewWorkgroups)
+  FwdPlan p{4, 0, 1};
+  while (p.waves > 1 && rows / (32 * p.waves) * kv_heads < kFewWorkgroups)
+    p.waves /= 2;
+  p.tiles = rows / (32 * p.waves) + n_seq + 1;
+  if (p.waves > 1)
     return p;
-  p.split = true;
-  p.tiles = rows / kSplitRows + n_seq + 1;
   // workgroups with rows: a tile of every 32 rows, and one per sequence
-  const int64_t busy = std::max<int64_t>(1, (rows / kSplitRows + std::min<int64_t>(n_seq, rows)) *
-                                                kv_heads);
+  const int64_t busy =
+      std::max<int64_t>(1, (rows / 32 + std::min<int64_t>(n_seq, rows)) * kv_heads);
   const int64_t keys = n_seq > 0 ? n_k / n_seq : 0;
   p.splits = static_cast<int32_t>(std::max<int64_t>(
       1, std::min<int64_t>({kSplitTarget / busy, keys / kMinSplitKeys, kMaxSplits})));
@@ -422,10 +427,9 @@ void attn_forward_run(const AttnArgs &args, int32_t dtype, bool vec, hipStream_t
     constexpr int DP = decltype(dp)::value;
     constexpr bool VEC = decltype(v)::value;
     const dim3 g(static_cast<unsigned>(grid)), b(kFwdThreads);
-    if (plan.split)
-      hipLaunchKernelGGL((attn_fwd_kernel<T, DP, VEC, true>), g, b, 0, stream, a);
-    else
-      hipLaunchKernelGGL((attn_fwd_kernel<T, DP, VEC, false>), g, b, 0, stream, a);
+    with_waves(plan.waves, [&](auto w) {
+      hipLaunchKernelGGL((attn_fwd_kernel<T, DP, VEC, decltype(w)::value>), g, b, 0, stream, a);
+    });
     RHIP_LAUNCH_CHECK();
     if (a.splits > 1) {
       const int64_t rows = static_cast<int64_t>(a.n_q) * a.heads;

@@ -239,9 +239,10 @@ def test_rounding_error_of_out():
 
 @pytest.mark.parametrize("dtype", [F32, BF16])
 @pytest.mark.parametrize("heads,kv_heads,dim", [(8, 8, 32), (4, 4, 64), (8, 4, 128), (9, 3, 40)])
-def test_shared_tiles(dtype, heads, kv_heads, dim):
-    """Enough rows for whole 128-row tiles on every CU (both sides)."""
-    lens = [40000 // kv_heads // 3 + 77, 1, 0, 130, 3000]
+@pytest.mark.parametrize("total", [12000, 24000, 40000])
+def test_shared_tiles(dtype, heads, kv_heads, dim, total):
+    """Enough rows for tiles of 32, 64 and 128 rows on every CU (both sides)."""
+    lens = [total // kv_heads // 3 + 77, 1, 0, 130, total // 14]
     n = sum(lens)
     if heads == 9 and dtype == BF16:
         lens = [n, 0, 63]
