@@ -63,8 +63,7 @@ struct FwdWs {
 };
 FwdWs carve_forward(Carve &cv, const rhip_attn *a) {
   FwdWs w{};
-  const int32_t splits =
-      attn_forward_splits(a->n_q, a->n_k, a->n_seq, a->heads, a->kv_heads);
+  const int32_t splits = attn_forward_splits(*a);
   if (splits > 1) {
     const size_t rows = static_cast<size_t>(splits) * a->n_q * a->heads;
     w.part_o = cv.take<float>(rows * a->dim);
@@ -80,8 +79,7 @@ struct BwdWs {
 BwdWs carve_backward(Carve &cv, const rhip_attn *a) {
   BwdWs w{};
   w.stat = cv.take<float2>(static_cast<size_t>(std::max<int64_t>(1, a->n_q)) * a->heads);
-  const int32_t splits =
-      attn_backward_splits(a->n_q, a->n_k, a->n_seq, a->heads, a->kv_heads);
+  const int32_t splits = attn_backward_splits(*a);
   if (splits > 1) {
     const size_t n = static_cast<size_t>(splits) * a->n_k * a->kv_heads * a->dim;
     w.part_k = cv.take<float>(n);

@@ -12,10 +12,20 @@ void attn_forward_run(const AttnArgs &a, int32_t dtype, bool vec, hipStream_t st
 void attn_backward_run(const AttnArgs &a, int32_t dtype, bool vec, hipStream_t stream);
 // Workgroups that share one tile of query rows (forward) or of keys
 // (backward): their partial sums are the workspace.
-int32_t attn_forward_splits(int64_t n_q, int64_t n_k, int32_t n_seq, int32_t heads,
-                            int32_t kv_heads);
-int32_t attn_backward_splits(int64_t n_q, int64_t n_k, int32_t n_seq, int32_t heads,
-                             int32_t kv_heads);
+int32_t attn_forward_splits(const rhip_attn &d);
+int32_t attn_backward_splits(const rhip_attn &d);
+
+// 32-row blocks per workgroup of the kernels over query rows: as many as leave
+// two workgroups for each CU, or one with two blocks (bf16: a workgroup's own
+// tiles for each wave, W = 1, take twice the time of W = 2 at full width; fp32
+// is bound by its products, and W = 1 spreads them best). 8 heads of 6000
+// rows, 32 wide, dq: W = 4 110 us, W = 2 93; 8 of 3000, 128 wide, forward: W =
+// 2 46 us, W = 1 76; fp32, 2 key heads of 9903 rows: W = 2 77 us, W = 1 66.
+inline int32_t attn_waves(int64_t rows, int32_t kv_heads, int32_t dtype) {
+  if (rows / 128 * kv_heads >= 512)
+    return 4;
+  return rows / 64 * kv_heads >= (dtype == RHIP_F32 ? 512 : 256) ? 2 : 1;
+}
 
 // f(T{}, head width of the variant, whether rows load in 16-byte chunks).
 // Rows that do not (a width or a stride that is no multiple of 16 bytes, an

@@ -19,10 +19,6 @@ namespace {
 
 constexpr int kBwdThreads = 256;
 constexpr int kBwdWaves = kBwdThreads / kWave;
-// Workgroups below which W is halved, and how many the splits aim for.
-constexpr int64_t kFewWorkgroups = 256, kSplitTarget = 1024;
-constexpr int kMaxSplits = 32;
-
 template <typename T, int DP, int W> struct BwdShape {
   static constexpr int kRows = 32 * W;
   static constexpr int kParts = kBwdWaves / W; // waves that share a block of rows
@@ -38,24 +34,6 @@ template <typename T, int DP, int W> struct BwdShape {
   static constexpr int kStageBytes = kStreams * kBuffers * kBufBytes;
   static constexpr int kLds = kStageBytes > kJoinBytes ? kStageBytes : kJoinBytes;
 };
-
-// Workgroup -> (tile, head, split) as in the forward: head-major runs per XCD.
-// `last_first`: the tiles with the most work come first under a causal mask.
-__device__ __forceinline__ bool bwd_item(const AttnArgs &a, bool last_first, int32_t &tile,
-                                         int32_t &kv, int32_t &split) {
-  const uint32_t total = static_cast<uint32_t>(a.tiles) * a.kv_heads * a.splits;
-  const uint32_t per = (total + kXcds - 1) / kXcds;
-  const uint32_t i = (blockIdx.x % kXcds) * per + blockIdx.x / kXcds;
-  if (i >= total)
-    return false;
-  split = i % a.splits;
-  const uint32_t j = i / a.splits;
-  kv = j / a.tiles;
-  tile = j % a.tiles;
-  if (last_first)
-    tile = a.tiles - 1 - tile;
-  return true;
-}
 
 // The first query row that sees key j, and the keys that row i sees.
 __device__ __forceinline__ int32_t first_row(const AttnArgs &a, const AttnSeq &sq, int64_t j) {
@@ -226,8 +204,9 @@ attn_dq_kernel(AttnArgs a) {
   __shared__ alignas(16) char lds[Shape::kLds];
 
   int32_t t, kv, split;
-  if (!bwd_item(a, true, t, kv, split))
+  if (!attn_item(a, t, kv, split))
     return;
+  t = a.tiles - 1 - t; // as in the forward; the first keys have the most rows below
   const AttnSeq sq = query_tile(a, Shape::kRows, a.group, t);
   const int32_t n_rows = sq.lq * a.group, row0 = sq.tile * Shape::kRows;
   if (row0 >= n_rows)
@@ -397,7 +376,7 @@ attn_dkv_kernel(AttnArgs a) {
   __shared__ alignas(16) char lds[Shape::kLds];
 
   int32_t t, kv, split;
-  if (!bwd_item(a, false, t, kv, split))
+  if (!attn_item(a, t, kv, split))
     return;
   int32_t room;
   const AttnSeq sq = key_tile(a, Shape::kRows, t, room);
@@ -418,7 +397,7 @@ attn_dkv_kernel(AttnArgs a) {
   // workgroup's part of them
   const int32_t per_head = key0 < sq.lk ? max((sq.lq + kBM - 1) / kBM - it0, 0) : 0;
   int32_t n0 = 0, n1 = per_head * a.group;
-  if (W == 1 && a.splits > 1) {
+  if (a.splits > 1) {
     const int32_t per = (n1 + a.splits - 1) / a.splits;
     n0 = min(split * per, n1);
     n1 = min(n0 + per, n1);
@@ -441,8 +420,8 @@ attn_dkv_kernel(AttnArgs a) {
              sq.lq - i0, a.dim);
     // (lse2, -delta) of the tile's rows, parted: for every 32 rows 32 of each
     const __amdgpu_buffer_rsrc_t rsrc =
-        buf_rsrc(a.stat + static_cast<int64_t>(head) * a.n_q + r0,
-                 static_cast<int64_t>(min(sq.lq - i0, kBM)) * 8);
+        wave_rsrc(a.stat + static_cast<int64_t>(head) * a.n_q + r0,
+                  static_cast<int64_t>(min(sq.lq - i0, kBM)) * 8);
     const int block = W == 1 ? 0 : w;
     if (block * 32 < kBM)
       dma4(rsrc, lds_address(to + 2 * Shape::kTileBytes + block * 256),
@@ -533,6 +512,20 @@ attn_dkv_kernel(AttnArgs a) {
 
   // rows behind the keys in use get zeros (no tile was added to them)
   if constexpr (W == 4) {
+    if (a.splits > 1) {
+      if (key < room) {
+        const int64_t place = ((split * static_cast<int64_t>(a.n_k) + gk) * a.kv_heads + kv) * a.dim;
+        using Sum = AttnTile<float, DP>;
+        if (a.dim % 4 == 0) {
+          Sum::template store_column<true>(a.part_k + place, a.dim, 1.f, dk);
+          Sum::template store_column<true>(a.part_v + place, a.dim, 1.f, dv);
+        } else {
+          Sum::template store_column<false>(a.part_k + place, a.dim, 1.f, dk);
+          Sum::template store_column<false>(a.part_v + place, a.dim, 1.f, dv);
+        }
+      }
+      return;
+    }
     bool bad = false;
     if (a.causal && key_ok) {
 #pragma unroll
@@ -617,47 +610,73 @@ struct BwdPlan {
   int64_t tiles;
   int32_t splits;
 };
-// Over n rows (packed query rows or keys) for each key head; `others`: rows of
-// the other side, all sequences and heads of a group counted.
-BwdPlan plan_backward(int64_t n, int32_t n_seq, int32_t kv_heads, int64_t others, bool splits) {
-  BwdPlan p{4, 0, 1};
-  while (p.waves > 1 && n / (32 * p.waves) * kv_heads < kFewWorkgroups)
-    p.waves /= 2;
-  p.tiles = n / (32 * p.waves) + n_seq + 1;
-  if (p.waves > 1 || !splits)
-    return p;
-  const int64_t busy = std::max<int64_t>(1, (n / 32 + std::min<int64_t>(n_seq, n)) * kv_heads);
-  // a split gets four 32-row tiles for each wave, at least
-  const int64_t rows = n_seq > 0 ? others / n_seq : 0;
-  p.splits = static_cast<int32_t>(std::max<int64_t>(
-      1, std::min<int64_t>({kSplitTarget / busy, rows / 512, kMaxSplits})));
+BwdPlan plan_queries(int64_t rows, int32_t n_seq, int32_t kv_heads, int32_t dtype) {
+  BwdPlan p{attn_waves(rows, kv_heads, dtype), 0, 1};
+  p.tiles = rows / (32 * p.waves) + n_seq + 1;
   return p;
 }
 
-unsigned bwd_grid(int64_t items) {
-  const int64_t grid = ceil_div(items, kXcds) * kXcds;
+// The keys' kernel: W and the splits by estimated time, in microseconds. A
+// 32x32 block takes a SIMD `block` when two waves keep it busy (measured over
+// whole launches: 128-wide bf16 at 940 TFLOP/s 1.14 us, 64 and 32 in
+// proportion; fp32 at 125 TFLOP/s) and a wave on its own 1.5 times that. The
+// launch takes the larger of all blocks over 1024 SIMDs and the longest
+// workgroup's blocks one after another (under a causal mask the first keys'
+// have twice the mean; sequences of unlike lengths a quarter more). W = 2 and
+// 1 cost 1.3 and 1.7 times the blocks (less shared per tile); every round of
+// workgroups 10 us to start and finish; splits write and read fp32 partial
+// sums at 4.5 TB/s. (16 over 4 heads, 128 wide, four causal texts of 4096: 912
+// us with one split, 686 with three, joining included; 8 heads, eight of
+// 1024: 70 us with one, 113 with two.)
+BwdPlan plan_keys(int64_t n_q, int64_t n_k, int32_t n_seq, int32_t heads, int32_t kv_heads,
+                  int32_t dim, int32_t causal, int32_t dtype) {
+  const int64_t seqs = std::max<int64_t>(1, std::min<int64_t>(n_seq, n_k));
+  const double rows = static_cast<double>(n_q) * (heads / kv_heads) / seqs; // per key
+  const double block =
+      1.14 * (dim <= 32 ? 0.25 : dim <= 64 ? 0.5 : 1.0) * (dtype == RHIP_F32 ? 7.5 : 1.0);
+  const double all = static_cast<double>(n_k) * kv_heads * rows * (causal ? 0.5 : 1.0) / 1024.0;
+  const double traffic = static_cast<double>(n_k) * kv_heads * dim * 16 / 4.5e6;
+  BwdPlan best{};
+  double least = 0.0;
+  for (int32_t w = 4; w >= 1; w /= 2) {
+    const double wgs = static_cast<double>(n_k / (32 * w) + seqs) * kv_heads;
+    for (int32_t s : {1, 2, 3, 4, 6, 8, 12, 16, 24, 32}) {
+      // a split gets four 32-row tiles for each wave, at least
+      if (s > 1 && rows < 512.0 * s)
+        break;
+      const double spread = all / 1024.0 * block * (w == 4 ? 1.0 : w == 2 ? 1.3 : 1.7);
+      const double longest = 1.25 * rows / 32.0 * w / 4.0 / s * block * 1.5;
+      const double t = std::max(spread, longest) + (wgs * s / 512.0 + 1.0) * 10.0 +
+                       (s > 1 ? 4.0 + s * traffic : 0.0);
+      if (best.waves == 0 || t < least) {
+        least = t;
+        best = {w, n_k / (32 * w) + n_seq + 1, s};
+      }
+    }
+  }
+  return best;
+}
+
+unsigned bwd_grid(int64_t tiles, int64_t heads, int64_t splits) {
+  const int64_t grid = attn_grid(tiles, heads, splits);
   if (grid > INT32_MAX)
     throw Error(RHIP_ERR_UNSUPPORTED, "too many tiles for one launch");
   return static_cast<unsigned>(grid);
 }
 
-BwdPlan plan_keys(int64_t n_q, int64_t n_k, int32_t n_seq, int32_t heads, int32_t kv_heads) {
-  return plan_backward(n_k, n_seq, kv_heads, n_q * (heads / kv_heads), true);
-}
-
 } // namespace
 
-int32_t attn_backward_splits(int64_t n_q, int64_t n_k, int32_t n_seq, int32_t heads,
-                             int32_t kv_heads) {
-  return plan_keys(n_q, n_k, n_seq, heads, kv_heads).splits;
+int32_t attn_backward_splits(const rhip_attn &d) {
+  return plan_keys(d.n_q, d.n_k, d.n_seq, d.heads, d.kv_heads, d.dim, d.causal, d.dtype).splits;
 }
 
 void attn_backward_run(const AttnArgs &args, int32_t dtype, bool vec, hipStream_t stream) {
-  const BwdPlan pq = plan_backward(static_cast<int64_t>(args.n_q) * args.group, args.n_seq,
-                                   args.kv_heads, args.n_k, false);
-  const BwdPlan pk = plan_keys(args.n_q, args.n_k, args.n_seq, args.heads, args.kv_heads);
-  const unsigned gq = bwd_grid(pq.tiles * args.kv_heads);
-  const unsigned gk = bwd_grid(pk.tiles * args.kv_heads * pk.splits);
+  const BwdPlan pq =
+      plan_queries(static_cast<int64_t>(args.n_q) * args.group, args.n_seq, args.kv_heads, dtype);
+  const BwdPlan pk = plan_keys(args.n_q, args.n_k, args.n_seq, args.heads, args.kv_heads,
+                               args.dim, args.causal, dtype);
+  const unsigned gq = bwd_grid(pq.tiles, args.kv_heads, 1);
+  const unsigned gk = bwd_grid(pk.tiles, args.kv_heads, pk.splits);
   AttnArgs aq = args, ak = args;
   aq.tiles = static_cast<int32_t>(pq.tiles), aq.splits = 1;
   ak.tiles = static_cast<int32_t>(pk.tiles), ak.splits = pk.splits;

@@ -148,6 +148,41 @@ __device__ __forceinline__ AttnSeq key_row(const AttnArgs &a, int32_t row) {
   return q;
 }
 
+// Workgroup -> (tile, key head, split) of a launch over tiles x key heads x
+// splits. Workgroups are dealt to the 8 XCDs round-robin, and what reads the
+// same keys should share an L2: each XCD gets whole heads where there are
+// enough, or every second (fourth, eighth) tile of one head where 8 is a
+// multiple of the heads, else all of everything. Tiles come in order on every
+// XCD, so with the heaviest first (under a causal mask) their work evens out.
+__device__ __forceinline__ bool attn_item(const AttnArgs &a, int32_t &tile, int32_t &kv,
+                                          int32_t &split) {
+  const uint32_t x = blockIdx.x % kXcds, i = blockIdx.x / kXcds;
+  const uint32_t heads = a.kv_heads, units = static_cast<uint32_t>(a.tiles) * a.splits;
+  uint32_t unit;
+  if (heads % kXcds == 0) {
+    const uint32_t mine = heads / kXcds;
+    unit = i / mine;
+    kv = x * mine + i % mine;
+  } else if (kXcds % heads == 0) {
+    const uint32_t share = kXcds / heads;
+    unit = i * share + x % share;
+    kv = x / share;
+  } else {
+    unit = blockIdx.x / heads;
+    kv = blockIdx.x % heads;
+  }
+  tile = unit / a.splits;
+  split = unit % a.splits;
+  return unit < units;
+}
+// Workgroups of such a launch.
+inline int64_t attn_grid(int64_t tiles, int64_t heads, int64_t splits) {
+  const int64_t units = tiles * splits;
+  if (kXcds % heads == 0)
+    return ceil_div(units, kXcds / heads) * kXcds;
+  return units * heads;
+}
+
 // LDS reads by byte address (wave instructions' immediate offsets hold what is
 // constant, so a kernel keeps a handful of addresses per lane).
 template <typename V> __device__ __forceinline__ V lds_read(uint32_t addr) {
@@ -377,6 +412,16 @@ __device__ __forceinline__ uint32_t lds_address(const void *p) { // wave-uniform
   return __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(reinterpret_cast<uintptr_t>(p)));
 }
 
+// A buffer whose pointer and size are the same in every lane, in scalar
+// registers whatever the compiler can prove.
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t wave_rsrc(const void *p, int64_t bytes) {
+  const uint64_t a = reinterpret_cast<uint64_t>(p);
+  const uint32_t lo = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(a));
+  const uint32_t hi = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(a >> 32));
+  return buf_rsrc(reinterpret_cast<const void *>(static_cast<uint64_t>(hi) << 32 | lo),
+                  __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(bytes)));
+}
+
 // Tiles of ROWS rows streamed from global memory into swizzled LDS tiles by
 // THREADS threads (a workgroup, or a wave on its own). With VEC the loads go
 // straight to LDS and stay in flight until wait_stream: no registers, no LDS
@@ -406,7 +451,7 @@ template <typename T, int DP, int ROWS, int THREADS, bool VEC> struct TileStream
     if constexpr (VEC) {
       const int64_t bytes =
           rows > 0 ? ((rows - 1) * row_stride + dim) * static_cast<int64_t>(sizeof(T)) : 0;
-      const __amdgpu_buffer_rsrc_t rsrc = buf_rsrc(base, bytes);
+      const __amdgpu_buffer_rsrc_t rsrc = wave_rsrc(base, bytes);
       const uint32_t to = lds_address(lds) + lds_address_of_wave(t);
 #pragma unroll
       for (int i = 0; i < kPer; ++i)

@@ -19,8 +19,7 @@ namespace {
 
 constexpr int kFwdThreads = 256;
 constexpr int kFwdWaves = kFwdThreads / kWave;
-// Workgroups below which W is halved, and how many the splits aim for.
-constexpr int64_t kFewWorkgroups = 256, kSplitTarget = 1024;
+constexpr int64_t kSplitTarget = 1024; // workgroups that splits aim for
 constexpr int kMaxSplits = 64, kMinSplitKeys = 256;
 
 template <typename T, int DP, int W> struct FwdShape {
@@ -38,24 +37,6 @@ template <typename T, int DP, int W> struct FwdShape {
   static constexpr int kStageBytes = kStreams * kBuffers * 2 * kTileBytes;
   static constexpr int kLds = kStageBytes > kJoinBytes ? kStageBytes : kJoinBytes;
 };
-
-// Workgroup -> (tile, key head, split). Workgroups go to the XCDs round-robin;
-// each XCD takes a contiguous run of the head-major list, so the tiles that
-// read one head's keys share an L2. Within a head the last tiles come first:
-// under a causal mask those have the most keys.
-__device__ __forceinline__ bool fwd_item(const AttnArgs &a, int32_t &tile, int32_t &kv,
-                                         int32_t &split) {
-  const uint32_t total = static_cast<uint32_t>(a.tiles) * a.kv_heads * a.splits;
-  const uint32_t per = (total + kXcds - 1) / kXcds;
-  const uint32_t i = (blockIdx.x % kXcds) * per + blockIdx.x / kXcds;
-  if (i >= total)
-    return false;
-  split = i % a.splits;
-  const uint32_t j = i / a.splits;
-  kv = j / a.tiles;
-  tile = a.tiles - 1 - j % a.tiles;
-  return true;
-}
 
 // One row by its definition, for rows whose sums came out not finite under a
 // causal mask: there a product with a masked key's probability 0 and a value
@@ -145,8 +126,9 @@ attn_fwd_kernel(AttnArgs a) {
   __shared__ alignas(16) char lds[Shape::kLds];
 
   int32_t t, kv, split;
-  if (!fwd_item(a, t, kv, split))
+  if (!attn_item(a, t, kv, split))
     return;
+  t = a.tiles - 1 - t; // the last tiles first: under a causal mask they see the most keys
   const AttnSeq sq = query_tile(a, Shape::kRows, a.group, t);
   const int32_t n_rows = sq.lq * a.group, row0 = sq.tile * Shape::kRows;
   if (row0 >= n_rows)
@@ -391,11 +373,10 @@ struct FwdPlan {
   int64_t tiles;
   int32_t splits;
 };
-FwdPlan plan_forward(int64_t n_q, int64_t n_k, int32_t n_seq, int32_t heads, int32_t kv_heads) {
+FwdPlan plan_forward(int64_t n_q, int64_t n_k, int32_t n_seq, int32_t heads, int32_t kv_heads,
+                     int32_t dtype) {
   const int64_t rows = n_q * (heads / kv_heads);
-  FwdPlan p{4, 0, 1};
-  while (p.waves > 1 && rows / (32 * p.waves) * kv_heads < kFewWorkgroups)
-    p.waves /= 2;
+  FwdPlan p{attn_waves(rows, kv_heads, dtype), 0, 1};
   p.tiles = rows / (32 * p.waves) + n_seq + 1;
   if (p.waves > 1)
     return p;
@@ -410,15 +391,14 @@ FwdPlan plan_forward(int64_t n_q, int64_t n_k, int32_t n_seq, int32_t heads, int
 
 } // namespace
 
-int32_t attn_forward_splits(int64_t n_q, int64_t n_k, int32_t n_seq, int32_t heads,
-                            int32_t kv_heads) {
-  return plan_forward(n_q, n_k, n_seq, heads, kv_heads).splits;
+int32_t attn_forward_splits(const rhip_attn &d) {
+  return plan_forward(d.n_q, d.n_k, d.n_seq, d.heads, d.kv_heads, d.dtype).splits;
 }
 
 void attn_forward_run(const AttnArgs &args, int32_t dtype, bool vec, hipStream_t stream) {
   AttnArgs a = args;
-  const FwdPlan plan = plan_forward(a.n_q, a.n_k, a.n_seq, a.heads, a.kv_heads);
-  const int64_t grid = ceil_div(plan.tiles * a.kv_heads * plan.splits, kXcds) * kXcds;
+  const FwdPlan plan = plan_forward(a.n_q, a.n_k, a.n_seq, a.heads, a.kv_heads, dtype);
+  const int64_t grid = attn_grid(plan.tiles, a.kv_heads, plan.splits);
   if (grid > INT32_MAX)
     throw Error(RHIP_ERR_UNSUPPORTED, "too many query tiles for one launch");
   a.tiles = static_cast<int32_t>(plan.tiles), a.splits = plan.splits;
