@@ -15,8 +15,9 @@ namespace rhip {
 namespace {
 
 constexpr int kEmbThreads = 256;
-constexpr int kSegment = 64; // positions a group of lanes sums by itself, at most
-constexpr int kJoinLanes = 16; // partial sums added side by side by embed_join_kernel
+constexpr int kSegment = kWave; // positions a wave sums by itself, at most
+constexpr int kRowsPerWave = 4; // table rows a wave takes one after another
+constexpr int kJoinCols = 16, kJoinLanes = 64; // embed_join_kernel: columns by partial sums
 
 // Lanes per row: the row's chunks rounded up to a power of two, at most a wave.
 // Wider rows take several column tiles of 64 chunks.
@@ -72,13 +73,20 @@ __global__ __launch_bounds__(kEmbThreads) void embed_keys_kernel(const void *__r
 // fills the gaps between its keys together, so a few tokens in a large table
 // cost no more than many.
 __global__ __launch_bounds__(kEmbThreads) void embed_starts_kernel(
-    const uint32_t *__restrict__ keys, int64_t n, uint32_t vocab, int32_t *__restrict__ start) {
+    const uint32_t *__restrict__ keys, int64_t n, uint32_t vocab, int32_t *__restrict__ start,
+    int32_t *__restrict__ runs) {
+  if (blockIdx.x == 0 && threadIdx.x == 0)
+    *runs = 0;
+  constexpr int kShort = 8; // rows a lane fills by itself
   const int64_t i = static_cast<int64_t>(blockIdx.x) * kEmbThreads + threadIdx.x;
   int64_t lo = 0, hi = -1; // rows lo .. hi start at i
   if (i <= n) {
     lo = i == 0 ? 0 : static_cast<int64_t>(keys[i - 1]) + 1;
     hi = i == n ? vocab : keys[i];
   }
+  if (hi - lo < kShort)
+    for (; lo <= hi; ++lo)
+      start[lo] = static_cast<int32_t>(i);
   uint64_t gaps = __ballot(lo <= hi);
   while (gaps) {
     const int l = __ffsll(static_cast<unsigned long long>(gaps)) - 1;
@@ -90,74 +98,100 @@ __global__ __launch_bounds__(kEmbThreads) void embed_starts_kernel(
   }
 }
 
-// Sum of grad_y's rows at sorted positions [p0, p1) over one chunk column:
-// the wave's 64 / G position lanes take every (64 / G)-th position.
-template <typename T>
+// Sum of grad_y's rows at the sorted positions [p0, p1), at most 64 of them,
+// over a lane's NC chunks: the wave's 64 / G position lanes take every (64 /
+// G)-th position.
+template <typename T, int NC>
 __device__ __forceinline__ void sum_rows(const T *__restrict__ gy, int64_t gy_row,
                                          const int32_t *__restrict__ pos, int32_t p0, int32_t p1,
-                                         int c, int C, int log_g,
-                                         float (&acc)[RowChunk<T>::V]) {
+                                         const int (&c)[NC], int C, int log_g,
+                                         float (&acc)[NC][RowChunk<T>::V]) {
   using R = RowChunk<T>;
-  constexpr int kUnroll = 4;
-  const int plane = lane_id() >> log_g, planes = kWave >> log_g;
+  constexpr int kUnroll = NC == 1 ? 8 : NC == 2 ? 4 : 2; // rows in flight
+  const int plane = lane_id() >> log_g, planes = kWave >> log_g, count = p1 - p0;
 #pragma unroll
-  for (int e = 0; e < R::V; ++e)
-    acc[e] = 0.f;
-  for (int32_t p = p0 + plane; p < p1; p += kUnroll * planes) {
-    float v[kUnroll][R::V];
+  for (int i = 0; i < NC; ++i)
+#pragma unroll
+    for (int e = 0; e < R::V; ++e)
+      acc[i][e] = 0.f;
+  const int32_t mine = lane_id() < count ? pos[p0 + lane_id()] : 0;
+  for (int p = plane; p < count; p += kUnroll * planes) {
+    float v[kUnroll][NC][R::V];
 #pragma unroll
     for (int u = 0; u < kUnroll; ++u) {
-      const int32_t q = p + u * planes;
-      R::load(gy + static_cast<int64_t>(pos[min(q, p1 - 1)]) * gy_row + c, q < p1 ? C - c : 0,
-              v[u]);
+      const int q = p + u * planes;
+      const T *row = gy + static_cast<int64_t>(__shfl(mine, q, kWave)) * gy_row;
+#pragma unroll
+      for (int i = 0; i < NC; ++i)
+        R::load(row + c[i], q < count ? C - c[i] : 0, v[u][i]);
     }
 #pragma unroll
     for (int u = 0; u < kUnroll; ++u)
 #pragma unroll
-      for (int e = 0; e < R::V; ++e)
-        acc[e] += v[u][e];
+      for (int i = 0; i < NC; ++i)
+#pragma unroll
+        for (int e = 0; e < R::V; ++e)
+          acc[i][e] += v[u][i][e];
   }
   for (int off = 1 << log_g; off < kWave; off <<= 1)
 #pragma unroll
-    for (int e = 0; e < R::V; ++e)
-      acc[e] += __shfl_xor(acc[e], off, kWave);
+    for (int i = 0; i < NC; ++i)
+#pragma unroll
+      for (int e = 0; e < R::V; ++e)
+        acc[i][e] += __shfl_xor(acc[i][e], off, kWave);
 }
 
-// One wave per work item and column tile. Items [0, vocab): a table row with
-// at most kSegment positions, summed (or zeroed) and written. Items vocab + j:
-// chunk j of the sorted positions, for the parts of longer runs in it. A chunk
-// meets at most two of those: one from before it (partial sum 2 j) and one
-// that starts in it (2 j + 1).
-template <typename T>
+// One wave per work item and column tile of 64 NC chunks. The first items, the
+// longest: chunk j of the sorted positions, for the parts of long runs in it.
+// A chunk meets at most two of those: one from before it (partial sum 2 j) and
+// one that starts in it (2 j + 1), which then goes on the list of runs to join
+// (in any order: each is joined by itself). The others: four table rows, each
+// with at most kSegment positions, summed (or zeroed) and written; most rows
+// of a large table are in no batch, so a wave takes several.
+template <typename T, int NC>
 __global__ __launch_bounds__(kEmbThreads) void embed_backward_kernel(
     const T *__restrict__ gy, int64_t gy_row, const uint32_t *__restrict__ keys,
     const int32_t *__restrict__ pos, const int32_t *__restrict__ start, int64_t n, int64_t vocab,
-    int C, int log_g, float scale, T *__restrict__ gw, float *__restrict__ part) {
+    int C, int log_g, float scale, T *__restrict__ gw, float *__restrict__ part,
+    int32_t *__restrict__ runs) {
   using R = RowChunk<T>;
   const int64_t item = static_cast<int64_t>(blockIdx.x) * (kEmbThreads / kWave) +
-                       threadIdx.x / kWave;
+                       __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
   const int lane = lane_id() & ((1 << log_g) - 1);
-  const int c = (blockIdx.y * kWave + lane) * R::V;
-  const bool writer = (lane_id() >> log_g) == 0 && c < C;
-  const int cc = min(c, C - 1), left = c < C ? C : cc; // lanes past the row load nothing
-  float acc[R::V];
-  if (item < vocab) {
-    const int32_t p0 = start[item], p1 = start[item + 1];
-    if (p1 - p0 > kSegment)
-      return;
-    sum_rows(gy, gy_row, pos, p0, p1, cc, left, log_g, acc);
-    if (writer) {
+  const bool writer = (lane_id() >> log_g) == 0;
+  int c[NC];
 #pragma unroll
-      for (int e = 0; e < R::V; ++e)
-        acc[e] *= scale;
-      R::store(gw + item * C + c, C - c, acc);
+  for (int i = 0; i < NC; ++i) // chunks past the row: nothing to load or write
+    c[i] = min(((blockIdx.y * NC + i) * kWave + lane) * R::V, C);
+  float acc[NC][R::V];
+  const int64_t segments = (n + kSegment - 1) / kSegment;
+  if (item >= segments) {
+    const int64_t first = (item - segments) * kRowsPerWave;
+    if (first >= vocab)
+      return;
+    int32_t at[kRowsPerWave + 1];
+#pragma unroll
+    for (int r = 0; r <= kRowsPerWave; ++r)
+      at[r] = start[min(first + r, vocab)];
+#pragma unroll
+    for (int r = 0; r < kRowsPerWave; ++r) {
+      const int64_t v = first + r;
+      if (v >= vocab || at[r + 1] - at[r] > kSegment)
+        continue;
+      sum_rows<T, NC>(gy, gy_row, pos, at[r], at[r + 1], c, C, log_g, acc);
+      if (writer) {
+#pragma unroll
+        for (int i = 0; i < NC; ++i) {
+#pragma unroll
+          for (int e = 0; e < R::V; ++e)
+            acc[i][e] *= scale;
+          R::store(gw + v * C + c[i], C - c[i], acc[i]);
+        }
+      }
     }
     return;
   }
-  const int64_t j = item - vocab;
-  const int64_t s0 = j * kSegment, s1 = min(n, s0 + kSegment);
-  if (s0 >= n)
-    return;
+  const int64_t j = item, s0 = j * kSegment, s1 = min(n, s0 + kSegment);
   for (int k = 0; k < 2; ++k) {
     // the run at the chunk's first position, if it began before it, and the
     // run at the last position, if it began inside
@@ -168,50 +202,53 @@ __global__ __launch_bounds__(kEmbThreads) void embed_backward_kernel(
     const bool before = p0 < s0;
     if (p1 - p0 <= kSegment || before != (k == 0))
       continue;
-    sum_rows(gy, gy_row, pos, max(p0, static_cast<int32_t>(s0)),
-             min(p1, static_cast<int32_t>(s1)), cc, left, log_g, acc);
+    if (!before && blockIdx.y == 0 && lane_id() == 0)
+      runs[1 + atomicAdd(runs, 1)] = static_cast<int32_t>(j);
+    sum_rows<T, NC>(gy, gy_row, pos, max(p0, static_cast<int32_t>(s0)),
+                    min(p1, static_cast<int32_t>(s1)), c, C, log_g, acc);
     if (writer) {
-      float *dst = part + (2 * j + k) * C + c;
+      float *dst = part + (2 * j + k) * C;
 #pragma unroll
-      for (int e = 0; e < R::V; ++e)
-        if (c + e < C)
-          dst[e] = acc[e];
+      for (int i = 0; i < NC; ++i)
+#pragma unroll
+        for (int e = 0; e < R::V; ++e)
+          if (c[i] + e < C)
+            dst[c[i] + e] = acc[i][e];
     }
   }
 }
 
-// The table row of the run that starts in chunk j, if it is a long one: its
-// chunks' partial sums, 16 lanes over the chunks by 16 columns, then in lane
-// order.
+// The table rows of the long runs: for each on the list the partial sums of
+// its chunks, 64 lanes over the chunks by 16 columns, then a tree. The order of
+// the sums depends on the chunks alone.
 template <typename T>
-__global__ __launch_bounds__(kEmbThreads) void embed_join_kernel(
-    const uint32_t *__restrict__ keys, const int32_t *__restrict__ start, int64_t n,
-    int64_t vocab, int C, float scale, const float *__restrict__ part, T *__restrict__ gw) {
-  constexpr int kCols = kEmbThreads / kJoinLanes;
-  __shared__ float lds[kJoinLanes][kCols];
-  const int64_t j = blockIdx.x, s0 = j * kSegment, s1 = min(n, s0 + kSegment);
-  const uint32_t v = keys[s1 - 1];
-  if (v >= vocab)
-    return;
-  const int32_t p0 = start[v], p1 = start[v + 1];
-  if (p1 - p0 <= kSegment || p0 < s0)
-    return;
-  const int64_t last = (p1 - 1) / kSegment;
-  const int col = threadIdx.x % kCols, r = threadIdx.x / kCols;
-  for (int c0 = blockIdx.y * kCols; c0 < C; c0 += gridDim.y * kCols) {
-    const int c = c0 + col;
-    float s = 0.f;
-    if (c < C)
+__global__ __launch_bounds__(kJoinCols *kJoinLanes) void embed_join_kernel(
+    const uint32_t *__restrict__ keys, const int32_t *__restrict__ start, int64_t n, int C,
+    float scale, const float *__restrict__ part, const int32_t *__restrict__ runs,
+    T *__restrict__ gw) {
+  __shared__ float lds[kJoinLanes][kJoinCols];
+  const int col = threadIdx.x % kJoinCols, r = threadIdx.x / kJoinCols;
+  const int32_t count = runs[0];
+  for (int32_t k = blockIdx.x; k < count; k += gridDim.x) {
+    const int64_t j = runs[1 + k];
+    const uint32_t v = keys[min(n, (j + 1) * kSegment) - 1];
+    const int64_t last = (start[v + 1] - 1) / kSegment;
+    for (int c0 = blockIdx.y * kJoinCols; c0 < C; c0 += gridDim.y * kJoinCols) {
+      const int c = min(c0 + col, C - 1);
+      float s = 0.f;
+#pragma unroll 4
       for (int64_t q = j + r; q <= last; q += kJoinLanes)
         s += part[(2 * q + (q == j)) * C + c];
-    __syncthreads(); // the previous tile's sums have been read
-    lds[r][col] = s;
-    __syncthreads();
-    if (r == 0 && c < C) {
+      __syncthreads(); // the previous columns' sums have been read
+      lds[r][col] = s;
 #pragma unroll
-      for (int k = 1; k < kJoinLanes; ++k)
-        s += lds[k][col];
-      gw[static_cast<int64_t>(v) * C + c] = from_f32<T>(s * scale);
+      for (int off = kJoinLanes / 2; off; off >>= 1) {
+        __syncthreads();
+        if (r < off)
+          lds[r][col] += lds[r + off][col];
+      }
+      if (r == 0 && c0 + col < C)
+        gw[static_cast<int64_t>(v) * C + c] = from_f32<T>(lds[0][col] * scale);
     }
   }
 }
@@ -231,6 +268,7 @@ void check_embed_type(int32_t dtype) {
 struct EmbedWs {
   uint32_t *keys, *sorted;
   int32_t *pos, *order, *start;
+  int32_t *runs; // how many long runs there are, then the chunk each starts in
   float *part;
   void *sort;
   size_t sort_bytes;
@@ -243,6 +281,7 @@ EmbedWs carve_embed(Carve &cv, int64_t n, int64_t vocab, int32_t C) {
   w.pos = cv.take<int32_t>(m);
   w.order = cv.take<int32_t>(m);
   w.start = cv.take<int32_t>(vocab + 2);
+  w.runs = cv.take<int32_t>(1 + ceil_div(m, kSegment));
   w.part = cv.take<float>(2 * static_cast<size_t>(ceil_div(m, kSegment)) * C);
   w.sort_bytes = sort_pairs_u32_bytes(m);
   w.sort = cv.take<char>(w.sort_bytes);
@@ -325,27 +364,39 @@ extern "C" int rhip_embed_backward(const void *grad_y, int64_t grad_y_row, const
     hipLaunchKernelGGL(embed_starts_kernel,
                        dim3(static_cast<unsigned>(ceil_div(n + 1, kEmbThreads))),
                        dim3(kEmbThreads), 0, stream, w.sorted, n,
-                       static_cast<uint32_t>(vocabulary), w.start);
+                       static_cast<uint32_t>(vocabulary), w.start, w.runs);
     RHIP_LAUNCH_CHECK();
     with_embed_type(dtype, [&](auto t) {
       using T = decltype(t);
       const int chunks = static_cast<int>(ceil_div(C, RowChunk<T>::V));
       const int64_t segments = ceil_div(n, kSegment);
-      hipLaunchKernelGGL((embed_backward_kernel<T>),
-                         dim3(static_cast<unsigned>(
-                                  ceil_div(vocabulary + segments, kEmbThreads / kWave)),
-                              static_cast<unsigned>(ceil_div(chunks, kWave))),
-                         dim3(kEmbThreads), 0, stream, static_cast<const T *>(grad_y),
-                         grad_y_row, w.sorted, w.order, w.start, n, vocabulary, C,
-                         log2_of(lanes_per_row(chunks)), scale, static_cast<T *>(grad_weight),
-                         w.part);
-      RHIP_LAUNCH_CHECK();
+      // chunks per lane: whole rows in one wave as far as registers go
+      auto launch = [&](auto nc) {
+        constexpr int NC = decltype(nc)::value;
+        hipLaunchKernelGGL((embed_backward_kernel<T, NC>),
+                           dim3(static_cast<unsigned>(
+                                    ceil_div(ceil_div(vocabulary, kRowsPerWave) + segments,
+                                             kEmbThreads / kWave)),
+                                static_cast<unsigned>(ceil_div(chunks, kWave * NC))),
+                           dim3(kEmbThreads), 0, stream, static_cast<const T *>(grad_y),
+                           grad_y_row, w.sorted, w.order, w.start, n, vocabulary, C,
+                           log2_of(lanes_per_row(chunks)), scale,
+                           static_cast<T *>(grad_weight), w.part, w.runs);
+        RHIP_LAUNCH_CHECK();
+      };
+      if (chunks <= kWave)
+        launch(std::integral_constant<int, 1>{});
+      else if (chunks <= 2 * kWave)
+        launch(std::integral_constant<int, 2>{});
+      else
+        launch(std::integral_constant<int, 4>{});
       if (segments > 0) {
-        const unsigned tiles = static_cast<unsigned>(
-            std::min<int64_t>(ceil_div(C, kEmbThreads / kJoinLanes), 64));
-        hipLaunchKernelGGL((embed_join_kernel<T>), dim3(static_cast<unsigned>(segments), tiles),
-                           dim3(kEmbThreads), 0, stream, w.sorted, w.start, n, vocabulary, C,
-                           scale, w.part, static_cast<T *>(grad_weight));
+        const unsigned tiles =
+            static_cast<unsigned>(std::min<int64_t>(ceil_div(C, kJoinCols), 8));
+        hipLaunchKernelGGL((embed_join_kernel<T>),
+                           dim3(static_cast<unsigned>(std::min<int64_t>(segments, 64)), tiles),
+                           dim3(kJoinCols * kJoinLanes), 0, stream, w.sorted, w.start, n, C,
+                           scale, w.part, w.runs, static_cast<T *>(grad_weight));
         RHIP_LAUNCH_CHECK();
       }
     });

@@ -20,79 +20,112 @@ namespace rhip {
 namespace {
 
 constexpr int kLnThreads = 256;
-// Backward workgroups to aim for: each writes 2 C fp32 sums.
-constexpr int kLnBlocks = 1024;
+// Backward workgroups, two per CU: each writes 2 C fp32 sums, so more of them
+// move more bytes (1024 of them on 16384 rows of 4096: 66 MB beside 402).
+constexpr int kLnBlocks = 512;
 constexpr int kSumCols = 16, kSumRows = 64; // ln_sums_kernel's columns and row lanes
 
-// Sum over a row's G lanes, in every lane; G = 256: the workgroup, through
-// LDS (buf holds 4 floats and is free again after the next barrier).
-template <int G> __device__ __forceinline__ float row_sum(float v, float *buf) {
+// N sums over a row's G lanes, in every lane; G = 256: the workgroup, through
+// LDS (buf is free again after the next barrier but one).
+template <int G, int N>
+__device__ __forceinline__ void row_sums(float (&v)[N], float (*buf)[4]) {
 #pragma unroll
   for (int off = 1; off < (G < kWave ? G : kWave); off <<= 1)
-    v += __shfl_xor(v, off, kWave);
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+      v[i] += __shfl_xor(v[i], off, kWave);
   if constexpr (G > kWave) {
     if (lane_id() == 0)
-      buf[threadIdx.x / kWave] = v;
+#pragma unroll
+      for (int i = 0; i < N; ++i)
+        buf[i][threadIdx.x / kWave] = v[i];
     __syncthreads();
-    v = (buf[0] + buf[1]) + (buf[2] + buf[3]);
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+      v[i] = (buf[i][0] + buf[i][1]) + (buf[i][2] + buf[i][3]);
   }
-  return v;
 }
 
-// y = (x - mean) rstd w + b, NC chunks of a row per lane.
-template <typename T, int G, int NC>
+// y = (x - mean) rstd w + b: R rows at a time per group of G lanes, NC chunks
+// of each per lane.
+template <typename T, int G, int NC, int R>
 __global__ __launch_bounds__(kLnThreads) void ln_forward_kernel(
     const T *__restrict__ x, int64_t x_row, int64_t n, int C, const float *__restrict__ weight,
     const float *__restrict__ bias, float eps, T *__restrict__ y, float *__restrict__ mean_out,
     float *__restrict__ rstd_out) {
-  using R = RowChunk<T>;
-  __shared__ float buf[2][4];
+  using K = RowChunk<T>;
+  __shared__ float buf[2][R][4];
   const int lane = threadIdx.x % G;
-  const int64_t row = static_cast<int64_t>(blockIdx.x) * (kLnThreads / G) + threadIdx.x / G;
-  if (row >= n) // whole groups of lanes: the row sums stay within them
-    return;
-  float v[NC][R::V];
-  float s = 0.f;
+  // rows row0 + r * groups: neighbouring groups stay neighbours in memory
+  constexpr int kGroups = kLnThreads / G;
+  const int64_t row0 = static_cast<int64_t>(blockIdx.x) * kGroups * R + threadIdx.x / G;
+  float v[R][NC][K::V], mean[R], rstd[R];
 #pragma unroll
-  for (int i = 0; i < NC; ++i) {
-    const int c = (lane + i * G) * R::V;
-    R::load(x + row * x_row + c, C - c, v[i]);
-  }
+  for (int r = 0; r < R; ++r) {
+    const int64_t row = row0 + r * kGroups;
 #pragma unroll
-  for (int i = 0; i < NC; ++i)
-#pragma unroll
-    for (int e = 0; e < R::V; ++e)
-      s += v[i][e];
-  const float mean = row_sum<G>(s, buf[0]) / static_cast<float>(C);
-  s = 0.f;
-#pragma unroll
-  for (int i = 0; i < NC; ++i) {
-    const int c = (lane + i * G) * R::V;
-#pragma unroll
-    for (int e = 0; e < R::V; ++e) {
-      v[i][e] = c + e < C ? v[i][e] - mean : 0.f;
-      s = fmaf(v[i][e], v[i][e], s);
+    for (int i = 0; i < NC; ++i) {
+      const int c = (lane + i * G) * K::V;
+      K::load(x + row * x_row + c, row < n ? C - c : 0, v[r][i]);
     }
   }
-  const float var = row_sum<G>(s, buf[1]) / static_cast<float>(C);
-  const float rstd = 1.f / sqrtf(var + eps);
+  const float inv_c = 1.f / static_cast<float>(C);
 #pragma unroll
-  for (int i = 0; i < NC; ++i) {
-    const int c = (lane + i * G) * R::V;
-    if (c < C) {
-      float w[R::V], b[R::V];
-      load_params<R::V>(weight, c, C, 1.f, w);
-      load_params<R::V>(bias, c, C, 0.f, b);
+  for (int r = 0; r < R; ++r) {
+    mean[r] = 0.f;
 #pragma unroll
-      for (int e = 0; e < R::V; ++e)
-        v[i][e] = fmaf(v[i][e] * rstd, w[e], b[e]);
-      R::store(y + row * C + c, C - c, v[i]);
+    for (int i = 0; i < NC; ++i)
+#pragma unroll
+      for (int e = 0; e < K::V; ++e)
+        mean[r] += v[r][i][e];
+  }
+  row_sums<G>(mean, buf[0]);
+#pragma unroll
+  for (int r = 0; r < R; ++r) {
+    mean[r] *= inv_c;
+    rstd[r] = 0.f;
+#pragma unroll
+    for (int i = 0; i < NC; ++i) {
+      const int c = (lane + i * G) * K::V;
+#pragma unroll
+      for (int e = 0; e < K::V; ++e) {
+        v[r][i][e] = c + e < C ? v[r][i][e] - mean[r] : 0.f;
+        rstd[r] = fmaf(v[r][i][e], v[r][i][e], rstd[r]);
+      }
     }
   }
-  if (mean_out && lane == 0) {
-    mean_out[row] = mean;
-    rstd_out[row] = rstd;
+  row_sums<G>(rstd, buf[1]);
+#pragma unroll
+  for (int r = 0; r < R; ++r)
+    rstd[r] = 1.f / sqrtf(rstd[r] * inv_c + eps);
+#pragma unroll
+  for (int i = 0; i < NC; ++i) {
+    const int c = (lane + i * G) * K::V;
+    if (c >= C)
+      continue;
+    float w[K::V], b[K::V];
+    load_params<K::V>(weight, c, C, 1.f, w);
+    load_params<K::V>(bias, c, C, 0.f, b);
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      const int64_t row = row0 + r * kGroups;
+      if (row < n) {
+#pragma unroll
+        for (int e = 0; e < K::V; ++e)
+          v[r][i][e] = fmaf(v[r][i][e] * rstd[r], w[e], b[e]);
+        K::store(y + row * C + c, C - c, v[r][i]);
+      }
+    }
   }
+  if (mean_out && lane == 0)
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      const int64_t row = row0 + r * kGroups;
+      if (row < n) {
+        mean_out[row] = mean[r];
+        rstd_out[row] = rstd[r];
+      }
+    }
 }
 
 // Rows wider than the registers: three passes over the row, the later two
@@ -114,7 +147,9 @@ __global__ __launch_bounds__(kLnThreads) void ln_forward_wide_kernel(
     for (int e = 0; e < R::V; ++e)
       s += v[e];
   }
-  const float mean = row_sum<kLnThreads>(s, buf[0]) / static_cast<float>(C);
+  float one[1] = {s};
+  row_sums<kLnThreads>(one, &buf[0]);
+  const float mean = one[0] / static_cast<float>(C);
   s = 0.f;
   for (int c = c0; c < C; c += step) {
     R::load(xr + c, C - c, v);
@@ -124,8 +159,9 @@ __global__ __launch_bounds__(kLnThreads) void ln_forward_wide_kernel(
       s = fmaf(d, d, s);
     }
   }
-  const float var = row_sum<kLnThreads>(s, buf[1]) / static_cast<float>(C);
-  const float rstd = 1.f / sqrtf(var + eps);
+  one[0] = s;
+  row_sums<kLnThreads>(one, &buf[1]);
+  const float rstd = 1.f / sqrtf(one[0] / static_cast<float>(C) + eps);
   for (int c = c0; c < C; c += step) {
     float w[R::V], b[R::V];
     R::load(xr + c, C - c, v);
@@ -142,68 +178,93 @@ __global__ __launch_bounds__(kLnThreads) void ln_forward_wide_kernel(
   }
 }
 
-// grad_x of the rows b, b + blocks, .. (in groups of 256 / G rows) and the
-// workgroup's sums of grad_y and grad_y xhat into part[b] = [2][C].
-template <typename T, int G, int NC>
-__global__ __launch_bounds__(kLnThreads) void ln_backward_kernel(
+// grad_x of the workgroup's rows, R at a time per group of G lanes, and its
+// sums of grad_y and grad_y xhat over them into part[b] = [2][C]. The next
+// rows' loads are in flight while these are worked on.
+template <typename T, int G, int NC, int R>
+__global__ __launch_bounds__(kLnThreads, 2) void ln_backward_kernel(
     const T *__restrict__ gy, int64_t gy_row, const T *__restrict__ x, int64_t x_row, int64_t n,
     int C, const float *__restrict__ mean, const float *__restrict__ rstd,
     const float *__restrict__ weight, T *__restrict__ gx, float *__restrict__ part) {
-  using R = RowChunk<T>;
+  using K = RowChunk<T>;
   constexpr int kGroups = kLnThreads / G;
-  __shared__ float buf[2][2][4];
+  __shared__ float buf[2][2 * R][4];
   const int lane = threadIdx.x % G, group = threadIdx.x / G;
-  float w[NC][R::V], sb[NC][R::V], sw[NC][R::V];
+  const bool whole = C % K::V == 0; // no partial chunk: rows load as they lie
+  float w[NC][K::V], sb[NC][K::V], sw[NC][K::V];
 #pragma unroll
   for (int i = 0; i < NC; ++i) {
-    load_params<R::V>(weight, (lane + i * G) * R::V, C, 1.f, w[i]);
+    load_params<K::V>(weight, (lane + i * G) * K::V, C, 1.f, w[i]);
 #pragma unroll
-    for (int e = 0; e < R::V; ++e)
+    for (int e = 0; e < K::V; ++e)
       sb[i][e] = sw[i][e] = 0.f;
   }
   const float inv_c = 1.f / static_cast<float>(C);
-  int turn = 0;
-  // the workgroup's groups go through the loop together (its barriers)
-  for (int64_t r0 = static_cast<int64_t>(blockIdx.x) * kGroups; r0 < n;
-       r0 += static_cast<int64_t>(gridDim.x) * kGroups) {
-    const int64_t row = r0 + group;
-    const bool ok = row < n;
-    const float mu = ok ? mean[row] : 0.f, rs = ok ? rstd[row] : 0.f;
-    float g[NC][R::V], h[NC][R::V]; // grad_y, xhat
-    float s1 = 0.f, s2 = 0.f;
+  v4u ng[R][NC], nx[R][NC]; // the next rows
+  float nm[R], nr[R];
+  auto fetch = [&](int64_t r0) {
 #pragma unroll
-    for (int i = 0; i < NC; ++i) {
-      const int c = (lane + i * G) * R::V;
-      R::load(gy + row * gy_row + c, ok ? C - c : 0, g[i]);
-      R::load(x + row * x_row + c, ok ? C - c : 0, h[i]);
-    }
+    for (int r = 0; r < R; ++r) {
+      const int64_t row = r0 + r * kGroups + group;
+      const bool ok = row < n;
+      nm[r] = ok ? mean[row] : 0.f;
+      nr[r] = ok ? rstd[row] : 0.f;
 #pragma unroll
-    for (int i = 0; i < NC; ++i) {
-      const int c = (lane + i * G) * R::V;
-#pragma unroll
-      for (int e = 0; e < R::V; ++e) {
-        h[i][e] = c + e < C ? (h[i][e] - mu) * rs : 0.f;
-        const float gw = g[i][e] * w[i][e];
-        s1 += gw;
-        s2 = fmaf(gw, h[i][e], s2);
-        sb[i][e] += g[i][e];
-        sw[i][e] = fmaf(g[i][e], h[i][e], sw[i][e]);
+      for (int i = 0; i < NC; ++i) {
+        const int c = (lane + i * G) * K::V;
+        ng[r][i] = K::fetch(gy + row * gy_row + c, ok ? C - c : 0, whole);
+        nx[r][i] = K::fetch(x + row * x_row + c, ok ? C - c : 0, whole);
       }
     }
+  };
+  const int64_t step = static_cast<int64_t>(gridDim.x) * kGroups * R;
+  int64_t r0 = static_cast<int64_t>(blockIdx.x) * kGroups * R;
+  if (r0 < n)
+    fetch(r0);
+  int turn = 0;
+  // the workgroup's groups go through the loop together (its barriers)
+  for (; r0 < n; r0 += step) {
+    float g[R][NC][K::V], h[R][NC][K::V], rs[R], s[2 * R]; // grad_y, xhat
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      rs[r] = nr[r];
+      s[2 * r] = s[2 * r + 1] = 0.f;
+#pragma unroll
+      for (int i = 0; i < NC; ++i) {
+        const int c = (lane + i * G) * K::V;
+        K::unpack(ng[r][i], g[r][i]);
+        K::unpack(nx[r][i], h[r][i]);
+#pragma unroll
+        for (int e = 0; e < K::V; ++e) {
+          h[r][i][e] = (whole ? c : c + e) < C ? (h[r][i][e] - nm[r]) * rs[r] : 0.f;
+          const float gw = g[r][i][e] * w[i][e];
+          s[2 * r] += gw;
+          s[2 * r + 1] = fmaf(gw, h[r][i][e], s[2 * r + 1]);
+          sb[i][e] += g[r][i][e];
+          sw[i][e] = fmaf(g[r][i][e], h[r][i][e], sw[i][e]);
+        }
+      }
+    }
+    if (r0 + step < n)
+      fetch(r0 + step);
     if (gx) {
-      s1 = row_sum<G>(s1, buf[turn][0]) * inv_c;
-      s2 = row_sum<G>(s2, buf[turn][1]) * inv_c;
+      row_sums<G>(s, buf[turn]);
       turn ^= 1;
-      if (ok) {
 #pragma unroll
-        for (int i = 0; i < NC; ++i) {
-          const int c = (lane + i * G) * R::V;
-          if (c < C) {
-            float o[R::V];
+      for (int r = 0; r < R; ++r) {
+        const int64_t row = r0 + r * kGroups + group;
+        const float s1 = s[2 * r] * inv_c, s2 = s[2 * r + 1] * inv_c;
+        if (row < n) {
 #pragma unroll
-            for (int e = 0; e < R::V; ++e)
-              o[e] = rs * (g[i][e] * w[i][e] - s1 - h[i][e] * s2);
-            R::store(gx + row * C + c, C - c, o);
+          for (int i = 0; i < NC; ++i) {
+            const int c = (lane + i * G) * K::V;
+            if (c < C) {
+              float o[K::V];
+#pragma unroll
+              for (int e = 0; e < K::V; ++e)
+                o[e] = rs[r] * (g[r][i][e] * w[i][e] - s1 - h[r][i][e] * s2);
+              K::store(gx + row * C + c, C - c, o);
+            }
           }
         }
       }
@@ -212,10 +273,10 @@ __global__ __launch_bounds__(kLnThreads) void ln_backward_kernel(
   if (!part)
     return;
   float *dst = part + static_cast<int64_t>(blockIdx.x) * 2 * C;
-  auto put = [&](int i, const float (&b)[R::V], const float (&s)[R::V]) {
-    const int c = (lane + i * G) * R::V;
+  auto put = [&](int i, const float (&b)[K::V], const float (&s)[K::V]) {
+    const int c = (lane + i * G) * K::V;
 #pragma unroll
-    for (int e = 0; e < R::V; ++e)
+    for (int e = 0; e < K::V; ++e)
       if (c + e < C) {
         dst[c + e] = b[e];
         dst[C + c + e] = s[e];
@@ -227,23 +288,23 @@ __global__ __launch_bounds__(kLnThreads) void ln_backward_kernel(
       put(i, sb[i], sw[i]);
   } else {
     // the groups' sums, added in group order
-    __shared__ float lds[kLnThreads][2 * R::V + 1];
+    __shared__ float lds[kLnThreads][2 * K::V + 1];
 #pragma unroll
     for (int i = 0; i < NC; ++i) {
       __syncthreads();
 #pragma unroll
-      for (int e = 0; e < R::V; ++e) {
+      for (int e = 0; e < K::V; ++e) {
         lds[threadIdx.x][e] = sb[i][e];
-        lds[threadIdx.x][R::V + e] = sw[i][e];
+        lds[threadIdx.x][K::V + e] = sw[i][e];
       }
       __syncthreads();
       if (group == 0) {
 #pragma unroll 1
         for (int k = 1; k < kGroups; ++k)
 #pragma unroll
-          for (int e = 0; e < R::V; ++e) {
+          for (int e = 0; e < K::V; ++e) {
             sb[i][e] += lds[k * G + lane][e];
-            sw[i][e] += lds[k * G + lane][R::V + e];
+            sw[i][e] += lds[k * G + lane][K::V + e];
           }
         put(i, sb[i], sw[i]);
       }
@@ -282,8 +343,9 @@ __global__ __launch_bounds__(kLnThreads) void ln_backward_wide_kernel(
       s2 = fmaf(g[e], h[e], s2);
     }
   }
-  s1 = row_sum<kLnThreads>(s1, buf[0]) * inv_c;
-  s2 = row_sum<kLnThreads>(s2, buf[1]) * inv_c;
+  float both[2] = {s1, s2};
+  row_sums<kLnThreads>(both, buf);
+  s1 = both[0] * inv_c, s2 = both[1] * inv_c;
   for (int c = c0; c < C; c += step) {
     load(c);
 #pragma unroll
@@ -356,30 +418,31 @@ __global__ __launch_bounds__(kSumCols *kSumRows) void ln_sums_kernel(
 
 // ------------------------------------------------------------------ host
 
-// f(T{}, lanes per row, chunks per lane); lanes 0: wider than the registers.
-// Two chunks per lane until a wave is full, then up to four, then the
-// workgroup shares the row.
+// f(T{}, lanes per row, chunks per lane, rows at a time); lanes 0: wider than
+// the registers. Two chunks per lane until a wave is full, then up to four,
+// then the workgroup shares the row; several narrow rows at a time, so that
+// enough loads are in flight.
 template <typename F> void with_row(int32_t dtype, int C, F &&f) {
   auto typed = [&](auto t) {
     const int chunks = static_cast<int>(ceil_div(C, RowChunk<decltype(t)>::V));
-    auto go = [&](auto g, auto nc) { f(t, g, nc); };
+    auto go = [&](auto g, auto nc, auto r) { f(t, g, nc, r); };
     using std::integral_constant;
     if (chunks <= 16)
-      go(integral_constant<int, 8>{}, integral_constant<int, 2>{});
+      go(integral_constant<int, 8>{}, integral_constant<int, 2>{}, integral_constant<int, 2>{});
     else if (chunks <= 32)
-      go(integral_constant<int, 16>{}, integral_constant<int, 2>{});
+      go(integral_constant<int, 16>{}, integral_constant<int, 2>{}, integral_constant<int, 2>{});
     else if (chunks <= 64)
-      go(integral_constant<int, 32>{}, integral_constant<int, 2>{});
+      go(integral_constant<int, 32>{}, integral_constant<int, 2>{}, integral_constant<int, 2>{});
     else if (chunks <= 128)
-      go(integral_constant<int, 64>{}, integral_constant<int, 2>{});
+      go(integral_constant<int, 64>{}, integral_constant<int, 2>{}, integral_constant<int, 2>{});
     else if (chunks <= 256)
-      go(integral_constant<int, 64>{}, integral_constant<int, 4>{});
+      go(integral_constant<int, 64>{}, integral_constant<int, 4>{}, integral_constant<int, 1>{});
     else if (chunks <= 512)
-      go(integral_constant<int, 256>{}, integral_constant<int, 2>{});
+      go(integral_constant<int, 256>{}, integral_constant<int, 2>{}, integral_constant<int, 2>{});
     else if (chunks <= 1024)
-      go(integral_constant<int, 256>{}, integral_constant<int, 4>{});
+      go(integral_constant<int, 256>{}, integral_constant<int, 4>{}, integral_constant<int, 1>{});
     else
-      go(integral_constant<int, 0>{}, integral_constant<int, 0>{});
+      go(integral_constant<int, 0>{}, integral_constant<int, 0>{}, integral_constant<int, 0>{});
   };
   if (dtype == RHIP_F32)
     typed(float{});
@@ -423,9 +486,9 @@ extern "C" int rhip_ln_forward(const void *x, int64_t x_row, int64_t n, int32_t 
     if (n == 0)
       return;
     RHIP_CHECK_ARG(x && y, "x and y are required");
-    with_row(dtype, C, [&](auto t, auto g, auto nc) {
+    with_row(dtype, C, [&](auto t, auto g, auto nc, auto r) {
       using T = decltype(t);
-      constexpr int G = decltype(g)::value, NC = decltype(nc)::value;
+      constexpr int G = decltype(g)::value, NC = decltype(nc)::value, R = decltype(r)::value;
       const T *xp = static_cast<const T *>(x);
       T *yp = static_cast<T *>(y);
       const float e = static_cast<float>(eps);
@@ -434,8 +497,8 @@ extern "C" int rhip_ln_forward(const void *x, int64_t x_row, int64_t n, int32_t 
                            dim3(kLnThreads), 0, stream, xp, x_row, n, C, weight, bias, e, yp,
                            mean, rstd);
       else
-        hipLaunchKernelGGL((ln_forward_kernel<T, G, NC>),
-                           dim3(static_cast<unsigned>(ceil_div(n, kLnThreads / G))),
+        hipLaunchKernelGGL((ln_forward_kernel<T, G, NC, R>),
+                           dim3(static_cast<unsigned>(ceil_div(n, kLnThreads / G * R))),
                            dim3(kLnThreads), 0, stream, xp, x_row, n, C, weight, bias, e, yp,
                            mean, rstd);
       RHIP_LAUNCH_CHECK();
@@ -462,9 +525,9 @@ extern "C" int rhip_ln_backward(const void *grad_y, int64_t grad_y_row, const vo
     }
     if (!params && (!grad_x || n == 0))
       return;
-    with_row(dtype, C, [&](auto t, auto g, auto nc) {
+    with_row(dtype, C, [&](auto t, auto g, auto nc, auto r) {
       using T = decltype(t);
-      constexpr int G = decltype(g)::value, NC = decltype(nc)::value;
+      constexpr int G = decltype(g)::value, NC = decltype(nc)::value, R = decltype(r)::value;
       const T *gp = static_cast<const T *>(grad_y), *xp = static_cast<const T *>(x);
       T *gxp = static_cast<T *>(grad_x);
       if constexpr (G == 0) {
@@ -483,8 +546,8 @@ extern "C" int rhip_ln_backward(const void *grad_y, int64_t grad_y_row, const vo
           RHIP_LAUNCH_CHECK();
         }
       } else {
-        blocks = std::max<int64_t>(1, std::min(blocks, ceil_div(n, kLnThreads / G)));
-        hipLaunchKernelGGL((ln_backward_kernel<T, G, NC>), dim3(static_cast<unsigned>(blocks)),
+        blocks = std::max<int64_t>(1, std::min(blocks, ceil_div(n, kLnThreads / G * R)));
+        hipLaunchKernelGGL((ln_backward_kernel<T, G, NC, R>), dim3(static_cast<unsigned>(blocks)),
                            dim3(kLnThreads), 0, stream, gp, grad_y_row, xp, x_row, n, C, mean,
                            rstd, weight, n > 0 ? gxp : nullptr, part);
         RHIP_LAUNCH_CHECK();

@@ -9,6 +9,8 @@
 
 namespace rhip {
 
+typedef v4u v4u_any __attribute__((aligned(2)));
+
 template <typename T> struct RowChunk {
   static constexpr int V = 16 / sizeof(T); // elements per chunk
 
@@ -22,13 +24,16 @@ template <typename T> struct RowChunk {
         v[e] = e < left ? to_f32(p[e]) : 0.f;
     }
   }
+  // Stores bypass the caches' write allocation: the rows are written once and
+  // not read again here (16384 rows of 4096 bf16, layer norm forward: 75 us
+  // with ordinary stores, 46 with these).
   __device__ static __forceinline__ void store(T *p, int left, const float (&v)[V]) {
     T t[V];
 #pragma unroll
     for (int e = 0; e < V; ++e)
       t[e] = from_f32<T>(v[e]);
     if (left >= V) {
-      __builtin_memcpy(p, t, 16);
+      __builtin_nontemporal_store(__builtin_bit_cast(v4u, t), reinterpret_cast<v4u_any *>(p));
     } else {
 #pragma unroll
       for (int e = 0; e < V; ++e)
@@ -36,11 +41,24 @@ template <typename T> struct RowChunk {
           p[e] = t[e];
     }
   }
+  // The chunk as it lies, zeros from element `left` on; `whole`: rows hold
+  // whole chunks, so left is a multiple of V (or negative) in every lane.
+  __device__ static __forceinline__ v4u fetch(const T *p, int left, bool whole) {
+    if (left >= V)
+      return raw(p);
+    v4u u{0u, 0u, 0u, 0u};
+    if (!whole && left > 0) {
+      T t[V];
+#pragma unroll
+      for (int e = 0; e < V; ++e)
+        t[e] = e < left ? p[e] : static_cast<T>(0.f);
+      __builtin_memcpy(&u, t, 16);
+    }
+    return u;
+  }
   // the 16 bytes at p (all of them inside the row)
   __device__ static __forceinline__ v4u raw(const T *p) {
-    v4u u;
-    __builtin_memcpy(&u, p, 16);
-    return u;
+    return *reinterpret_cast<const v4u_any *>(p);
   }
   __device__ static __forceinline__ void unpack(const v4u &u, float (&v)[V]) {
     if constexpr (sizeof(T) == 4) {
