@@ -19,10 +19,15 @@ namespace {
 
 constexpr int kBwdThreads = 256;
 constexpr int kBwdWaves = kBwdThreads / kWave;
-template <typename T, int DP, int W> struct BwdShape {
+template <typename T, int DP, int W, bool KEYS> struct BwdShape {
   static constexpr int kRows = 32 * W;
   static constexpr int kParts = kBwdWaves / W; // waves that share a block of rows
-  static constexpr int kBN = W == 1 || (W == 4 && sizeof(T) == 4 && DP == 128) ? 32 : 64;
+  // The keys' kernel in bf16 at full width holds 192 registers of keys, values
+  // and sums, which leaves none to read ahead with: its values stay in LDS,
+  // where they fit beside 32-row tiles.
+  static constexpr bool kOwnInLds = KEYS && W == 4 && sizeof(T) == 2 && DP == 128;
+  static constexpr int kBN =
+      W == 1 || (W == 4 && sizeof(T) == 4 && DP == 128) || kOwnInLds ? 32 : 64;
   static constexpr int kStreams = W == 1 ? kBwdWaves : 1;
   static constexpr int kTileBytes = kBN * DP * sizeof(T);
   static constexpr int kStatBytes = kBN * 8; // (lse2, -delta) of a tile's rows
@@ -31,7 +36,8 @@ template <typename T, int DP, int W> struct BwdShape {
   static constexpr int kJoinRow = DP + 4; // floats per row of the joined sums
   static constexpr int kJoinBytes =
       W < 4 ? kBwdWaves * 32 * kJoinRow * static_cast<int>(sizeof(float)) : 0;
-  static constexpr int kStageBytes = kStreams * kBuffers * kBufBytes;
+  static constexpr int kOwnBytes = kOwnInLds ? kRows * DP * static_cast<int>(sizeof(T)) : 0;
+  static constexpr int kStageBytes = kStreams * kBuffers * kBufBytes + kOwnBytes;
   static constexpr int kLds = kStageBytes > kJoinBytes ? kStageBytes : kJoinBytes;
 };
 
@@ -195,10 +201,11 @@ __device__ __forceinline__ void join_row(const float *rows, int row_floats, int 
 template <typename T, int DP, bool VEC, int W>
 __global__ __launch_bounds__(kBwdThreads, sizeof(T) == 4 && DP == 128 ? 1 : 2) void
 attn_dq_kernel(AttnArgs a) {
-  using Shape = BwdShape<T, DP, W>;
+  using Shape = BwdShape<T, DP, W, false>;
   using Tile = AttnTile<T, DP>;
   using Frag = typename Tile::Frag;
   constexpr int kBN = Shape::kBN;
+  constexpr int kAhead = sizeof(T) == 2 ? 4 : 0; // LDS operands on their way to the products
   constexpr int kB = W == 2 ? 1 : kBN / 32; // blocks of a tile that are a wave's
   using Stream = TileStream<T, DP, kBN, W == 1 ? kWave : kBwdThreads, VEC>;
   __shared__ alignas(16) char lds[Shape::kLds];
@@ -301,20 +308,32 @@ attn_dq_kernel(AttnArgs a) {
 #pragma unroll
       for (int b = 0; b < kB; ++b) {
         v16f s{}, dp = dp0;
-        Tile::row_product(at, 0, 32 * b, qf, s);
-        Tile::row_product(at, Shape::kTileBytes, 32 * b, gf, dp);
-#pragma unroll
-        for (int r = 0; r < 16; ++r)
-          s[r] = exp2_fast(fmaf(s[r], a.c, -lse2)) * dp[r];
-        if (masked) {
-          rare_path();
-#pragma unroll
-          for (int r = 0; r < 16; ++r)
-            s[r] = j0 + 32 * b + block_row(r) < lim ? s[r] : 0.f;
-        }
+        ahead<2 * Tile::kSteps, kAhead>(
+            [&](int i) {
+              return Tile::row_operand(at, i % 2 * Shape::kTileBytes, 32 * b, i / 2);
+            },
+            [&](int i, const Frag &x) {
+              if (i % 2)
+                Tile::mma(x, gf[i / 2], dp);
+              else
+                Tile::mma(x, qf[i / 2], s);
+            });
         typename Tile::Block ds;
-        Tile::pack(s, ds);
-        Tile::col_product(at, 0, 32 * b, ds, dq);
+        ahead<Tile::kColSteps, kAhead>(
+            [&](int i) { return Tile::col_operand(at, 0, 32 * b, i); },
+            [&](int i, const typename Tile::ColOperand &x) { Tile::col_step(x, i, ds, dq); },
+            [&] {
+#pragma unroll
+              for (int r = 0; r < 16; ++r)
+                s[r] = exp2_fast(fmaf(s[r], a.c, -lse2)) * dp[r];
+              if (masked) {
+                rare_path();
+#pragma unroll
+                for (int r = 0; r < 16; ++r)
+                  s[r] = j0 + 32 * b + block_row(r) < lim ? s[r] : 0.f;
+              }
+              Tile::pack(s, ds);
+            });
       }
     }
     if (Shape::kBuffers == 2) {
@@ -367,10 +386,12 @@ attn_dq_kernel(AttnArgs a) {
 template <typename T, int DP, bool VEC, int W>
 __global__ __launch_bounds__(kBwdThreads, sizeof(T) == 4 && DP >= 64 ? 1 : 2) void
 attn_dkv_kernel(AttnArgs a) {
-  using Shape = BwdShape<T, DP, W>;
+  using Shape = BwdShape<T, DP, W, true>;
   using Tile = AttnTile<T, DP>;
   using Frag = typename Tile::Frag;
   constexpr int kBM = Shape::kBN;
+  constexpr bool kVLds = Shape::kOwnBytes > 0;
+  constexpr int kAhead = kVLds ? 3 : 0; // LDS operands on their way to the products
   constexpr int kB = W == 2 ? 1 : kBM / 32;
   using Stream = TileStream<T, DP, kBM, W == 1 ? kWave : kBwdThreads, VEC>;
   __shared__ alignas(16) char lds[Shape::kLds];
@@ -429,16 +450,26 @@ attn_dkv_kernel(AttnArgs a) {
   };
   if (first < n1)
     issue(first, 0);
+  char *own = lds + Shape::kStreams * Shape::kBuffers * Shape::kBufBytes;
+  if constexpr (kVLds) {
+    TileStream<T, DP, Shape::kRows, kBwdThreads, VEC> os;
+    os.init(a.v_row, a.dim);
+    os.issue(own,
+             static_cast<const T *>(a.v) + (sq.k0 + static_cast<int64_t>(key0)) * a.v_row +
+                 kv * a.v_head,
+             a.v_row, sq.lk - key0, a.dim);
+  }
 
   const int64_t gk = sq.k0 + static_cast<int64_t>(key);
   const T *kp = static_cast<const T *>(a.k) + gk * a.k_row + kv * a.k_head;
   const T *vp = static_cast<const T *>(a.v) + gk * a.v_row + kv * a.v_head;
-  Frag kf[Tile::kSteps], vf[Tile::kSteps];
+  Frag kf[Tile::kSteps], vf[kVLds ? 1 : Tile::kSteps];
 #pragma unroll
   for (int s = 0; s < Tile::kSteps; ++s) {
     const int c = 2 * s + half;
     kf[s] = __builtin_bit_cast(Frag, Tile::template chunk<VEC>(kp, c, a.dim, key_ok));
-    vf[s] = __builtin_bit_cast(Frag, Tile::template chunk<VEC>(vp, c, a.dim, key_ok));
+    if constexpr (!kVLds)
+      vf[s] = __builtin_bit_cast(Frag, Tile::template chunk<VEC>(vp, c, a.dim, key_ok));
   }
   v16f dk[Tile::kDBlocks], dv[Tile::kDBlocks];
 #pragma unroll
@@ -447,6 +478,9 @@ attn_dkv_kernel(AttnArgs a) {
 
   const typename Tile::Lane lane_at = Tile::lane_addresses();
   const uint32_t stage_at = lds_address(stage);
+  typename Tile::Lane own_at{}; // this wave's keys in `own`
+  if constexpr (kVLds)
+    own_at = lane_at.in(lds_address(own) + w * (32 / 4) * Tile::kGroup);
   int buf = 0;
   for (int32_t n = first; n < n1; n += step) {
     wait_stream();
@@ -472,8 +506,26 @@ attn_dkv_kernel(AttnArgs a) {
           for (int e = 0; e < 4; ++e)
             dp[4 * g + e] = d[e];
         }
-        Tile::row_product(at, Shape::kTileBytes, 32 * b, vf, dp);
-        Tile::row_product(at, 0, 32 * b, kf, s);
+        // dP, then S
+        struct Pair {
+          Frag x, v;
+        };
+        ahead<2 * Tile::kSteps, kAhead>(
+            [&](int i) {
+              Pair f{};
+              f.x = Tile::row_operand(at, i < Tile::kSteps ? Shape::kTileBytes : 0, 32 * b,
+                                      i % Tile::kSteps);
+              if (kVLds && i < Tile::kSteps)
+                f.v = Tile::row_operand(own_at, 0, 0, i);
+              return f;
+            },
+            [&](int i, const Pair &f) {
+              if (i >= Tile::kSteps)
+                Tile::mma(f.x, kf[i - Tile::kSteps], s);
+              else
+                Tile::mma(f.x, kVLds ? f.v : vf[kVLds ? 0 : i], dp);
+            });
+        typename Tile::Block p, ds;
 #pragma unroll
         for (int g = 0; g < 4; ++g) {
           const v4f l = lds_read<v4f>(stat + b * 256 + g * 32);
@@ -493,7 +545,6 @@ attn_dkv_kernel(AttnArgs a) {
             dp[r] = sees ? dp[r] : 0.f;
           }
         }
-        typename Tile::Block p, ds;
         Tile::pack(s, p);
         Tile::col_product(at, Shape::kTileBytes, 32 * b, p, dv);
         Tile::pack(dp, ds);

@@ -11,6 +11,8 @@
 // lanes, no trip through LDS).
 #pragma once
 
+#include <type_traits>
+
 #include "conv_device.hpp"
 
 namespace rhip {
@@ -273,15 +275,12 @@ template <typename T, int DP> struct AttnTile {
     }
   }
 
-  // acc += A[32 rows x dim] B[dim x 32 columns]: A's rows row0 .. row0 + 31
-  // of the LDS tile (plus `bytes`: of one a constant further on), B the chunks
-  // a lane holds of its column.
-  __device__ static __forceinline__ void row_product(const Lane &at, int bytes, int row0,
-                                                     const Frag (&b)[kSteps], v16f &acc) {
-#pragma unroll
-    for (int s = 0; s < kSteps; ++s)
-      mma(lds_read<Frag>(at.row[s & 1] + (bytes + row0 / 4 * kGroup + (s >> 1) * 256)), b[s],
-          acc);
+  // acc += A[32 rows x dim] B[dim x 32 columns], kSteps steps: A's rows row0 ..
+  // row0 + 31 of the LDS tile (plus `bytes`: of one a constant further on), B
+  // the chunks a lane holds of its column. A step's left operand:
+  __device__ static __forceinline__ Frag row_operand(const Lane &at, int bytes, int row0,
+                                                     int step) {
+    return lds_read<Frag>(at.row[step & 1] + (bytes + row0 / 4 * kGroup + (step >> 1) * 256));
   }
 
   // The product of one chunk pair: lane half h holds elements (2 s + h) E ..
@@ -313,34 +312,42 @@ template <typename T, int DP> struct AttnTile {
     }
   }
 
-  // acc[db] += X^T[dim x 32 rows] B[32 rows x 32 columns]: X's rows row0 ..
-  // row0 + 31 of the LDS tile, B the block the lanes hold. Slot j of half h
-  // in step s stands for row 16 s + 8 (j / 4) + 4 h + j % 4, B's own order;
-  // a transpose read gives four consecutive rows of a lane's element column.
+  // acc[db] += X^T[dim x 32 rows] B[32 rows x 32 columns], kColSteps steps: X's
+  // rows row0 .. row0 + 31 of the LDS tile, B the block the lanes hold. bf16:
+  // slot j of half h in step (s, db) stands for row 16 s + 8 (j / 4) + 4 h + j %
+  // 4, B's own order; a transpose read gives four consecutive rows of a lane's
+  // element column. fp32: two rows a step.
+  static constexpr int kColSteps = sizeof(T) == 2 ? 2 * kDBlocks : 16 * kDBlocks;
+  using ColOperand = std::conditional_t<sizeof(T) == 2, v8bf, float>;
+  __device__ static __forceinline__ ColOperand col_operand(const Lane &at, int bytes, int row0,
+                                                           int step) {
+    if constexpr (sizeof(T) == 2) {
+      const int s = step / kDBlocks, db = step % kDBlocks;
+      const int off = bytes + (row0 + 16 * s) / 4 * kGroup + db * 256;
+      const v4s lo = lds_read_tr16(at.col[0] + off), hi = lds_read_tr16(at.col[1] + off);
+      return __builtin_bit_cast(v8bf,
+                                __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+    } else {
+      const int e = step / kDBlocks, db = step % kDBlocks;
+      return lds_read<float>(at.col[(e >> 2) & 1] +
+                             (bytes + (row0 + 8 * (e >> 2)) / 4 * kGroup + db * 512 +
+                              (e & 3) * 64));
+    }
+  }
+  __device__ static __forceinline__ void col_step(const ColOperand &x, int step, const Block &b,
+                                                  v16f (&acc)[kDBlocks]) {
+    const int db = step % kDBlocks;
+    if constexpr (sizeof(T) == 2)
+      acc[db] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(x, step / kDBlocks ? b.hi : b.lo, acc[db],
+                                                        0, 0, 0);
+    else
+      acc[db] = __builtin_amdgcn_mfma_f32_32x32x2f32(x, b.f[step / kDBlocks], acc[db], 0, 0, 0);
+  }
   __device__ static __forceinline__ void col_product(const Lane &at, int bytes, int row0,
                                                      const Block &b, v16f (&acc)[kDBlocks]) {
-    if constexpr (sizeof(T) == 2) {
 #pragma unroll
-      for (int s = 0; s < 2; ++s)
-#pragma unroll
-        for (int db = 0; db < kDBlocks; ++db) {
-          const int off = bytes + (row0 + 16 * s) / 4 * kGroup + db * 256;
-          const v4s lo = lds_read_tr16(at.col[0] + off), hi = lds_read_tr16(at.col[1] + off);
-          const v8bf a = __builtin_bit_cast(
-              v8bf, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
-          acc[db] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, s ? b.hi : b.lo, acc[db], 0, 0, 0);
-        }
-    } else {
-#pragma unroll
-      for (int e = 0; e < 16; ++e)
-#pragma unroll
-        for (int db = 0; db < kDBlocks; ++db) {
-          const int off =
-              bytes + (row0 + 8 * (e >> 2)) / 4 * kGroup + db * 512 + (e & 3) * 64;
-          acc[db] = __builtin_amdgcn_mfma_f32_32x32x2f32(
-              lds_read<float>(at.col[(e >> 2) & 1] + off), b.f[e], acc[db], 0, 0, 0);
-        }
-    }
+    for (int i = 0; i < kColSteps; ++i)
+      col_step(col_operand(at, bytes, row0, i), i, b, acc);
   }
 
   // One lane's column of a [32 DB x 32] result, scaled, as a row of dim
@@ -431,12 +438,16 @@ template <typename T, int DP, int ROWS, int THREADS, bool VEC> struct TileStream
   using Tile = AttnTile<T, DP>;
   static constexpr int kBytes = ROWS * Tile::C * 16;
   static constexpr int kPer = ROWS * Tile::C / THREADS;
-  uint32_t off[kPer];
+  // Where a thread's loads step by whole swizzle periods (16 rows) they have
+  // one chunk column, and rows a constant apart: one offset and a step for all.
+  static constexpr bool kStep = THREADS / Tile::C % 16 == 0;
+  static constexpr int kOffs = kStep ? 1 : kPer;
+  uint32_t off[kOffs];
 
   __device__ __forceinline__ void init(int64_t row_stride, int dim) {
     const int t = threadIdx.x % THREADS;
 #pragma unroll
-    for (int i = 0; i < kPer; ++i) {
+    for (int i = 0; i < kOffs; ++i) {
       int r, c;
       Tile::place(t + i * THREADS, r, c);
       off[i] = c * Tile::E < dim ? static_cast<uint32_t>(r * row_stride * sizeof(T) + c * 16)
@@ -453,9 +464,11 @@ template <typename T, int DP, int ROWS, int THREADS, bool VEC> struct TileStream
           rows > 0 ? ((rows - 1) * row_stride + dim) * static_cast<int64_t>(sizeof(T)) : 0;
       const __amdgpu_buffer_rsrc_t rsrc = wave_rsrc(base, bytes);
       const uint32_t to = lds_address(lds) + lds_address_of_wave(t);
+      const uint32_t step = static_cast<uint32_t>(row_stride * sizeof(T)); // a row's bytes
 #pragma unroll
       for (int i = 0; i < kPer; ++i)
-        dma16(rsrc, to + i * THREADS * 16, off[i]);
+        dma16(rsrc, to + i * THREADS * 16,
+              kStep ? off[0] + i * (THREADS / Tile::C) * step : off[i % kOffs]);
     } else {
 #pragma unroll
       for (int i = 0; i < kPer; ++i) {
@@ -472,6 +485,40 @@ private:
     return __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(t / kWave * kWave * 16));
   }
 };
+
+// N matrix steps whose operands come from LDS: load(i) fetches step i's, A
+// steps before use(i, operand) needs it. Left to itself the compiler, short of
+// registers, reads each operand right before its product and waits out the
+// read's latency there (the keys' kernel, 128 wide: 940 TFLOP/s so).
+// `before`: what to do once the first operands are on their way.
+// A = 0 leaves the order to it.
+template <int N, int A, typename L, typename U, typename B>
+__device__ __forceinline__ void ahead(L &&load, U &&use, B &&before) {
+  if constexpr (A == 0) {
+    before();
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+      use(i, load(i));
+  } else {
+    decltype(load(0)) f[A];
+#pragma unroll
+    for (int i = 0; i < A && i < N; ++i)
+      f[i] = load(i);
+    __builtin_amdgcn_sched_barrier(0);
+    before();
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      use(i, f[i % A]);
+      if (i + A < N)
+        f[i % A] = load(i + A);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+  }
+}
+template <int N, int A, typename L, typename U>
+__device__ __forceinline__ void ahead(L &&load, U &&use) {
+  ahead<N, A>(load, use, [] {});
+}
 
 // Row r of a lane's 16 entries of a 32x32 block.
 __device__ __forceinline__ int block_row(int r) {

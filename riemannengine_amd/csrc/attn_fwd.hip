@@ -121,6 +121,7 @@ attn_fwd_kernel(AttnArgs a) {
   using Tile = AttnTile<T, DP>;
   using Frag = typename Tile::Frag;
   constexpr int kBN = Shape::kBN;
+  constexpr int kAhead = sizeof(T) == 2 ? 4 : 0; // LDS operands on their way to the products
   constexpr int kB = W == 2 ? 1 : kBN / 32; // blocks of a tile that are a wave's
   using Stream = TileStream<T, DP, kBN, W == 1 ? kWave : kFwdThreads, VEC>;
   __shared__ alignas(16) char lds[Shape::kLds];
@@ -206,10 +207,12 @@ attn_fwd_kernel(AttnArgs a) {
     if (W == 1 || j0 < wave_lim) {
       v16f s[kB];
 #pragma unroll
-      for (int b = 0; b < kB; ++b) {
+      for (int b = 0; b < kB; ++b)
         s[b] = v16f{};
-        Tile::row_product(at, 0, 32 * b, qf, s[b]);
-      }
+      // the blocks take turns: two sums to add to
+      ahead<kB * Tile::kSteps, kAhead>(
+          [&](int i) { return Tile::row_operand(at, 0, 32 * (i % kB), i / kB); },
+          [&](int i, const Frag &x) { Tile::mma(x, qf[i / kB], s[i % kB]); });
       if (j0 + 32 * kB > wave_full) {
         rare_path();
 #pragma unroll
