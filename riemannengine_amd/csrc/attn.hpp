@@ -38,6 +38,8 @@ template <typename F> void with_attn(int32_t dtype, int32_t dim, bool vec, F &&f
       f(t, std::integral_constant<int, 32>{}, std::true_type{});
     else if (dim <= 64)
       f(t, std::integral_constant<int, 64>{}, std::true_type{});
+    else if (dim <= 96)
+      f(t, std::integral_constant<int, 96>{}, std::true_type{});
     else
       f(t, std::integral_constant<int, 128>{}, std::true_type{});
   };

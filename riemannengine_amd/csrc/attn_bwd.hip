@@ -189,7 +189,7 @@ __device__ __forceinline__ void join_row(const float *rows, int row_floats, int 
     const float *src = rows + ((r / 32 * PARTS + i) * 32 + r % 32) * row_floats;
     if (lane < DP)
       v0 += src[lane];
-    if (DP > kWave)
+    if (lane + kWave < DP)
       v1 += src[lane + kWave];
   }
 }
@@ -199,7 +199,7 @@ __device__ __forceinline__ void join_row(const float *rows, int row_floats, int 
 // Q^T, dP^T = V dO^T), so dS^T is the right operand of dQ^T = K^T dS^T as it
 // lies. dP's sums start at -delta.
 template <typename T, int DP, bool VEC, int W>
-__global__ __launch_bounds__(kBwdThreads, sizeof(T) == 4 && DP == 128 ? 1 : 2) void
+__global__ __launch_bounds__(kBwdThreads, sizeof(T) == 4 && DP >= 96 ? 1 : 2) void
 attn_dq_kernel(AttnArgs a) {
   using Shape = BwdShape<T, DP, W, false>;
   using Tile = AttnTile<T, DP>;
@@ -669,7 +669,7 @@ BwdPlan plan_queries(int64_t rows, int32_t n_seq, int32_t kv_heads, int32_t dtyp
 
 // The keys' kernel: W and the splits by estimated time, in microseconds. A
 // 32x32 block takes a SIMD `block` when two waves keep it busy (measured over
-// whole launches: 128-wide bf16 at 940 TFLOP/s 1.14 us, 64 and 32 in
+// whole launches: 128-wide bf16 1.14 us, narrower ones in
 // proportion; fp32 at 125 TFLOP/s) and a wave on its own 1.5 times that. The
 // launch takes the larger of all blocks over 1024 SIMDs and the longest
 // workgroup's blocks one after another (under a causal mask the first keys'
@@ -684,7 +684,7 @@ BwdPlan plan_keys(int64_t n_q, int64_t n_k, int32_t n_seq, int32_t heads, int32_
   const int64_t seqs = std::max<int64_t>(1, std::min<int64_t>(n_seq, n_k));
   const double rows = static_cast<double>(n_q) * (heads / kv_heads) / seqs; // per key
   const double block =
-      1.14 * (dim <= 32 ? 0.25 : dim <= 64 ? 0.5 : 1.0) * (dtype == RHIP_F32 ? 7.5 : 1.0);
+      1.14 * (dim <= 32 ? 0.25 : dim <= 64 ? 0.5 : dim <= 96 ? 0.8 : 1.0) * (dtype == RHIP_F32 ? 7.5 : 1.0);
   const double all = static_cast<double>(n_k) * kv_heads * rows * (causal ? 0.5 : 1.0) / 1024.0;
   const double traffic = static_cast<double>(n_k) * kv_heads * dim * 16 / 4.5e6;
   BwdPlan best{};

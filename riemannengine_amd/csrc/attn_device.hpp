@@ -198,7 +198,7 @@ __device__ __forceinline__ v4s lds_read_tr16(uint32_t addr) {
 // cost every pass.
 __device__ __forceinline__ void rare_path() { asm volatile(""); }
 
-// Rows of `DP` elements (the head width padded to 32, 64 or 128) as 16-byte
+// Rows of `DP` elements (the head width padded to 32, 64, 96 or 128) as 16-byte
 // chunks in LDS, in groups of four rows: chunk c of row r lies at
 //   (r / 4) * 64 C + (c / 4) * 256 + (r % 4) * 64 + ((c % 4) ^ (r / 4 % 4)) * 16.
 // Then 16 consecutive rows hold one chunk column in 16 different bank groups

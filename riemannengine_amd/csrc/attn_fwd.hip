@@ -115,7 +115,7 @@ __device__ void finish_row(const AttnArgs &a, const AttnSeq &sq, int32_t i, int3
 // as it lies. The next tile's loads are in flight while this one is
 // multiplied.
 template <typename T, int DP, bool VEC, int W>
-__global__ __launch_bounds__(kFwdThreads, sizeof(T) == 4 && DP == 128 ? 1 : 2) void
+__global__ __launch_bounds__(kFwdThreads, sizeof(T) == 4 && DP >= 96 ? 1 : 2) void
 attn_fwd_kernel(AttnArgs a) {
   using Shape = FwdShape<T, DP, W>;
   using Tile = AttnTile<T, DP>;
@@ -320,7 +320,7 @@ attn_fwd_kernel(AttnArgs a) {
         const float *src = jo + (i * 32 + first_at) * Shape::kJoinRow;
         if (lane < DP)
           o0 = fmaf(src[lane], f, o0);
-        if (DP > kWave)
+        if (lane + kWave < DP)
           o1 = fmaf(src[lane + kWave], f, o1);
       }
       const int32_t i = (row0 + r) / a.group;

@@ -238,7 +238,8 @@ def test_rounding_error_of_out():
 
 
 @pytest.mark.parametrize("dtype", [F32, BF16])
-@pytest.mark.parametrize("heads,kv_heads,dim", [(8, 8, 32), (4, 4, 64), (8, 4, 128), (9, 3, 40)])
+@pytest.mark.parametrize("heads,kv_heads,dim", [(8, 8, 32), (4, 4, 64), (8, 4, 128), (9, 3, 40),
+                                                (4, 2, 80), (8, 8, 96)])
 @pytest.mark.parametrize("total", [12000, 24000, 40000])
 def test_shared_tiles(dtype, heads, kv_heads, dim, total):
     """Enough rows for tiles of 32, 64 and 128 rows on every CU (both sides)."""
