@@ -68,6 +68,53 @@ __global__ __launch_bounds__(kEmbThreads) void embed_keys_kernel(const void *__r
   pos[i] = static_cast<int32_t>(i);
 }
 
+// Keys and sort in one workgroup for up to kSmall ids: bitonic in LDS over (key,
+// position) words, which are all different, so the order is the stable one.
+// (100 ids 7 us, 2000 19 us, against 25 in the keys kernel and the six of a
+// radix sort, and six launches less for the host; 4096 would take 33.)
+constexpr int kSmall = 2048, kSmallThreads = 1024, kPosBits = 11;
+static_assert(kSmall == 1 << kPosBits, "a position fits its bits");
+__global__ __launch_bounds__(kSmallThreads) void embed_sort_small_kernel(
+    const void *__restrict__ ids, int is32, int n, uint32_t vocab, uint32_t *__restrict__ sorted,
+    int32_t *__restrict__ order) {
+  __shared__ uint64_t w[kSmall];
+  int m = 2; // n rounded up to a power of two; the words behind n sort last
+  while (m < n)
+    m *= 2;
+  for (int i = threadIdx.x; i < m; i += kSmallThreads) {
+    uint64_t word = ~0ull;
+    if (i < n) {
+      const int64_t id = id_at(ids, is32, i);
+      word = (id >= 0 && id < vocab ? static_cast<uint64_t>(id) : vocab) << kPosBits | i;
+    }
+    w[i] = word;
+  }
+  // A wave's pairs at distances up to 64 lie in 128 words of its own: there no
+  // step needs the other waves.
+  bool apart = true; // the step before may have crossed waves
+  for (int k = 2; k <= m; k *= 2)
+    for (int j = k / 2; j > 0; j /= 2) {
+      if (apart || j > kWave)
+        __syncthreads();
+      else
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+      apart = j > kWave;
+      for (int t = threadIdx.x; t < m / 2; t += kSmallThreads) {
+        const int i = 2 * t - (t & (j - 1)); // pairs (i, i + j)
+        const uint64_t a = w[i], b = w[i + j];
+        if ((a > b) == ((i & k) == 0)) {
+          w[i] = b;
+          w[i + j] = a;
+        }
+      }
+    }
+  __syncthreads();
+  for (int i = threadIdx.x; i < n; i += kSmallThreads) {
+    sorted[i] = static_cast<uint32_t>(w[i] >> kPosBits);
+    order[i] = static_cast<int32_t>(w[i] & (kSmall - 1));
+  }
+}
+
 // start[v] = first sorted position whose key is >= v, v = 0 .. vocab: the rows
 // after the key before position i, up to the key at i, start at i. The wave
 // fills the gaps between its keys together, so a few tokens in a large table
@@ -353,7 +400,12 @@ extern "C" int rhip_embed_backward(const void *grad_y, int64_t grad_y_row, const
     RHIP_CHECK_ARG(n == 0 || (grad_y && ids), "grad_y and ids are required");
     Carve cv(workspace, ws_bytes);
     const EmbedWs w = carve_embed(cv, n, vocabulary, C);
-    if (n > 0) {
+    if (n > 0 && n <= kSmall) {
+      hipLaunchKernelGGL(embed_sort_small_kernel, dim3(1), dim3(kSmallThreads), 0, stream, ids,
+                         ids_int32, static_cast<int>(n), static_cast<uint32_t>(vocabulary),
+                         w.sorted, w.order);
+      RHIP_LAUNCH_CHECK();
+    } else if (n > 0) {
       hipLaunchKernelGGL(embed_keys_kernel, dim3(static_cast<unsigned>(ceil_div(n, kEmbThreads))),
                          dim3(kEmbThreads), 0, stream, ids, ids_int32, n,
                          static_cast<uint32_t>(vocabulary), w.keys, w.pos);

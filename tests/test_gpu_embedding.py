@@ -54,7 +54,8 @@ def make(seed, n, V, C, dtype, ids=None, is32=False):
 @pytest.mark.parametrize("n,V,C", [(1, 1, 1), (1, 5000, 64), (5, 3, 7), (64, 1, 32), (65, 1, 33),
                                    (1000, 20, 64), (20000, 7, 129), (3000, 2000, 255),
                                    (4097, 511, 512), (500, 70000, 40), (300, 100, 1100),
-                                   (2048, 65536, 16), (40, 10, 4099)])
+                                   (2048, 65536, 16), (40, 10, 4099), (2, 9, 8),
+                                   (2047, 300, 24), (2049, 300, 24), (9000, 300000, 8)])
 def test_sizes(dtype, n, V, C):
     check(*make(n, n, V, C, dtype, is32=n % 2 == 0), 3.5, f"n {n} V {V} C {C}")
 
