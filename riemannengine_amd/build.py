@@ -36,6 +36,8 @@ HIP_SOURCES = ["abi.hip", "sort.hip", "hash.hip", "kmap.hip", "conv.hip", "conv_
 HIP_FLAGS = [
     "--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC",
     "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops",
+    # the loads into LDS name m0 as clobbered, a reserved register: a warning each
+    "-Wno-inline-asm",
     "-I" + INCLUDE, "-I" + CSRC,
 ]
 

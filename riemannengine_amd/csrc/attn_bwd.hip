@@ -39,6 +39,9 @@ template <typename T, int DP, int W, bool KEYS> struct BwdShape {
   static constexpr int kOwnBytes = kOwnInLds ? kRows * DP * static_cast<int>(sizeof(T)) : 0;
   static constexpr int kStageBytes = kStreams * kBuffers * kBufBytes + kOwnBytes;
   static constexpr int kLds = kStageBytes > kJoinBytes ? kStageBytes : kJoinBytes;
+  // waves per SIMD: two workgroups' where their LDS and registers fit
+  static constexpr int kOccupancy =
+      kLds > 80 * 1024 || (sizeof(T) == 4 && DP >= (KEYS ? 64 : 96)) ? 1 : 2;
 };
 
 // The first query row that sees key j, and the keys that row i sees.
@@ -199,7 +202,7 @@ __device__ __forceinline__ void join_row(const float *rows, int row_floats, int 
 // Q^T, dP^T = V dO^T), so dS^T is the right operand of dQ^T = K^T dS^T as it
 // lies. dP's sums start at -delta.
 template <typename T, int DP, bool VEC, int W>
-__global__ __launch_bounds__(kBwdThreads, sizeof(T) == 4 && DP >= 96 ? 1 : 2) void
+__global__ __launch_bounds__(kBwdThreads, (BwdShape<T, DP, W, false>::kOccupancy)) void
 attn_dq_kernel(AttnArgs a) {
   using Shape = BwdShape<T, DP, W, false>;
   using Tile = AttnTile<T, DP>;
@@ -384,7 +387,7 @@ attn_dq_kernel(AttnArgs a) {
 // so P and dS are the right operands of dV^T = dO^T P and dK^T = Q^T dS as
 // they lie.
 template <typename T, int DP, bool VEC, int W>
-__global__ __launch_bounds__(kBwdThreads, sizeof(T) == 4 && DP >= 64 ? 1 : 2) void
+__global__ __launch_bounds__(kBwdThreads, (BwdShape<T, DP, W, true>::kOccupancy)) void
 attn_dkv_kernel(AttnArgs a) {
   using Shape = BwdShape<T, DP, W, true>;
   using Tile = AttnTile<T, DP>;
@@ -448,10 +451,10 @@ attn_dkv_kernel(AttnArgs a) {
       dma4(rsrc, lds_address(to + 2 * Shape::kTileBytes + block * 256),
            (block * 32 + (lane & 31)) * 8 + half * 4);
   };
+  char *own = lds + Shape::kStreams * Shape::kBuffers * Shape::kBufBytes;
   if (first < n1)
     issue(first, 0);
-  char *own = lds + Shape::kStreams * Shape::kBuffers * Shape::kBufBytes;
-  if constexpr (kVLds) {
+  if (kVLds && first < n1) { // the first turn waits for it; without one it may not start
     TileStream<T, DP, Shape::kRows, kBwdThreads, VEC> os;
     os.init(a.v_row, a.dim);
     os.issue(own,
@@ -643,6 +646,7 @@ __global__ __launch_bounds__(kBwdThreads) void attn_dkv_join_kernel(AttnArgs a) 
   const int lane = lane_id();
   const int32_t key = static_cast<int32_t>(at / a.kv_heads);
   float gk[2] = {0.f, 0.f}, gv[2] = {0.f, 0.f};
+#pragma unroll 4
   for (int s = 0; s < a.splits; ++s) {
     const int64_t p = (s * rows + at) * a.dim;
 #pragma unroll

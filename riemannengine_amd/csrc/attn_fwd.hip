@@ -12,6 +12,8 @@
 // Waves that share rows join their sums in LDS at the end. With W = 1 the
 // keys may further be split over workgroups, joined by a second kernel: for
 // single tokens, and wherever larger tiles leave the chip empty.
+#include <cmath>
+
 #include "attn.hpp"
 
 namespace rhip {
@@ -19,8 +21,7 @@ namespace {
 
 constexpr int kFwdThreads = 256;
 constexpr int kFwdWaves = kFwdThreads / kWave;
-constexpr int64_t kSplitTarget = 1024; // workgroups that splits aim for
-constexpr int kMaxSplits = 64, kMinSplitKeys = 256;
+constexpr int kMinSplitKeys = 128; // a tile for each wave of every split
 
 template <typename T, int DP, int W> struct FwdShape {
   static constexpr int kRows = 32 * W;
@@ -36,6 +37,9 @@ template <typename T, int DP, int W> struct FwdShape {
       W < 4 ? kFwdWaves * 32 * (kJoinRow + 2) * static_cast<int>(sizeof(float)) : 0;
   static constexpr int kStageBytes = kStreams * kBuffers * 2 * kTileBytes;
   static constexpr int kLds = kStageBytes > kJoinBytes ? kStageBytes : kJoinBytes;
+  // waves per SIMD: two workgroups' where their LDS and registers fit
+  static constexpr int kOccupancy =
+      kLds > 80 * 1024 || (sizeof(T) == 4 && DP >= 96) ? 1 : 2;
 };
 
 // One row by its definition, for rows whose sums came out not finite under a
@@ -115,7 +119,7 @@ __device__ void finish_row(const AttnArgs &a, const AttnSeq &sq, int32_t i, int3
 // as it lies. The next tile's loads are in flight while this one is
 // multiplied.
 template <typename T, int DP, bool VEC, int W>
-__global__ __launch_bounds__(kFwdThreads, sizeof(T) == 4 && DP >= 96 ? 1 : 2) void
+__global__ __launch_bounds__(kFwdThreads, (FwdShape<T, DP, W>::kOccupancy)) void
 attn_fwd_kernel(AttnArgs a) {
   using Shape = FwdShape<T, DP, W>;
   using Tile = AttnTile<T, DP>;
@@ -343,31 +347,49 @@ attn_fwd_kernel(AttnArgs a) {
   }
 }
 
-// Joins the splits' partial sums: one wave per row and head, in split order.
+// Joins the splits' partial sums, a workgroup per row and head: each wave
+// weighs every fourth split (its loads all independent), the sums are added in
+// wave order.
 template <typename T>
 __global__ __launch_bounds__(kFwdThreads) void attn_join_kernel(AttnArgs a) {
-  const int64_t rows = static_cast<int64_t>(a.n_q) * a.heads;
-  const int64_t at = static_cast<int64_t>(blockIdx.x) * kFwdWaves + threadIdx.x / kWave;
-  if (at >= rows)
-    return;
-  const int lane = lane_id();
+  __shared__ float2 sums[kFwdWaves][kWave];
+  __shared__ float totals[kFwdWaves];
+  const int64_t rows = static_cast<int64_t>(a.n_q) * a.heads, at = blockIdx.x;
+  const int lane = lane_id(), w = threadIdx.x / kWave;
   const int32_t row = static_cast<int32_t>(at / a.heads), head = static_cast<int32_t>(at % a.heads);
-  float mr = -INFINITY;
-  for (int s = 0; s < a.splits; ++s)
-    mr = fmaxf(mr, a.part_ml[2 * (s * rows + at)]);
+  // lane s: split s (at most 64 of them)
+  const bool mine = lane < a.splits;
+  const float m = mine ? a.part_ml[2 * (lane * rows + at)] : -INFINITY;
+  const float l = mine ? a.part_ml[2 * (lane * rows + at) + 1] : 0.f;
+  float mr = m;
+#pragma unroll
+  for (int off = 32; off; off >>= 1)
+    mr = fmaxf(mr, __shfl_xor(mr, off, kWave));
   const float base = (mr == -INFINITY ? 0.f : mr) * a.c;
+  const float f = mine ? exp2_fast(m * a.c - base) : 0.f;
   float o0 = 0.f, o1 = 0.f, sr = 0.f;
-  for (int s = 0; s < a.splits; ++s) {
-    const float f = exp2_fast(a.part_ml[2 * (s * rows + at)] * a.c - base);
-    sr = fmaf(a.part_ml[2 * (s * rows + at) + 1], f, sr);
+#pragma unroll 4
+  for (int s = w; s < a.splits; s += kFwdWaves) {
+    const float fs = __shfl(f, s, kWave);
     const float *src = a.part_o + (s * rows + at) * a.dim;
-    if (lane < a.dim)
-      o0 = fmaf(src[lane], f, o0);
-    if (lane + kWave < a.dim)
-      o1 = fmaf(src[lane + kWave], f, o1);
+    sr = fmaf(__shfl(l, s, kWave), fs, sr);
+    o0 = fmaf(lane < a.dim ? src[lane] : 0.f, fs, o0);
+    o1 = fmaf(lane + kWave < a.dim ? src[lane + kWave] : 0.f, fs, o1);
+  }
+  sums[w][lane] = make_float2(o0, o1);
+  if (lane == 0)
+    totals[w] = sr;
+  __syncthreads();
+  if (w > 0)
+    return;
+#pragma unroll
+  for (int i = 1; i < kFwdWaves; ++i) {
+    o0 += sums[i][lane].x;
+    o1 += sums[i][lane].y;
+    sr += totals[i];
   }
   // the row's sequence, for rows that have to be computed again
-  AttnSeq sq = query_row(a, row);
+  const AttnSeq sq = query_row(a, row);
   finish_row<T>(a, sq, row - sq.q0, head, o0, o1, mr, sr);
 }
 
@@ -376,34 +398,62 @@ struct FwdPlan {
   int64_t tiles;
   int32_t splits;
 };
+// W by attn_waves; with W = 1 the splits by estimated time, in microseconds: a
+// round of workgroups (one or two per CU, as their LDS allows) takes 8 to start
+// and finish and `tile` for every four 32-key tiles (one to a wave) of the mean
+// sequence; no less than the longest sequence alone, taken as 1.5 times the
+// mean, or 3 times for single tokens, whose caches differ most; joining takes
+// another 8. (32 tokens over caches of 1 to 16384 keys, 8 key heads, 128 wide:
+// four splits 172 us, one 390. Three causal sequences of 1000, 2 heads of 96:
+// one split 26 us, three 32 and 7 to join.)
 FwdPlan plan_forward(int64_t n_q, int64_t n_k, int32_t n_seq, int32_t heads, int32_t kv_heads,
-                     int32_t dtype) {
+                     int32_t dim, int32_t causal, int32_t dtype) {
   const int64_t rows = n_q * (heads / kv_heads);
   FwdPlan p{attn_waves(rows, kv_heads, dtype), 0, 1};
   p.tiles = rows / (32 * p.waves) + n_seq + 1;
-  if (p.waves > 1)
+  if (p.waves > 1 || n_seq == 0)
     return p;
+  const bool f32 = dtype == RHIP_F32;
+  const double width = dim <= 32 ? 0.25 : dim <= 64 ? 0.5 : dim <= 96 ? 0.75 : 1.0;
+  const double slots = width * (f32 ? 2 : 1) <= 0.5 ? 512.0 : 256.0;
+  const double tile = std::max(1.2, (f32 ? 5.0 : 3.0) * width);
   // workgroups with rows: a tile of every 32 rows, and one per sequence
-  const int64_t busy =
-      std::max<int64_t>(1, (rows / 32 + std::min<int64_t>(n_seq, rows)) * kv_heads);
-  const int64_t keys = n_seq > 0 ? n_k / n_seq : 0;
-  p.splits = static_cast<int32_t>(std::max<int64_t>(
-      1, std::min<int64_t>({kSplitTarget / busy, keys / kMinSplitKeys, kMaxSplits})));
+  const double busy = static_cast<double>(rows / 32 + std::min<int64_t>(n_seq, rows)) * kv_heads;
+  const bool tokens = rows <= 32 * static_cast<int64_t>(n_seq);
+  const double tiles =
+      static_cast<double>(n_k) / n_seq / (32 * kFwdWaves) * (causal && !tokens ? 0.5 : 1.0);
+  double least = 0.0;
+  for (int32_t s : {1, 2, 3, 4, 6, 8, 12, 16, 24, 32, 48, 64}) {
+    if (s > 1 && n_k / n_seq < static_cast<int64_t>(kMinSplitKeys) * s)
+      break;
+    const double turn = std::ceil(tiles / s) * tile;
+    const double all = std::ceil(busy * s / slots) * (8.0 + turn);
+    const double longest = 8.0 + turn * (tokens ? 3.0 : 1.5);
+    const double t = std::max(all, longest) + (s > 1 ? 8.0 : 0.0);
+    if (s == 1 || t < least) {
+      least = t;
+      p.splits = s;
+    }
+  }
   return p;
 }
 
 } // namespace
 
 int32_t attn_forward_splits(const rhip_attn &d) {
-  return plan_forward(d.n_q, d.n_k, d.n_seq, d.heads, d.kv_heads, d.dtype).splits;
+  return plan_forward(d.n_q, d.n_k, d.n_seq, d.heads, d.kv_heads, d.dim, d.causal, d.dtype).splits;
 }
 
 void attn_forward_run(const AttnArgs &args, int32_t dtype, bool vec, hipStream_t stream) {
   AttnArgs a = args;
-  const FwdPlan plan = plan_forward(a.n_q, a.n_k, a.n_seq, a.heads, a.kv_heads, dtype);
+  const FwdPlan plan = plan_forward(a.n_q, a.n_k, a.n_seq, a.heads, a.kv_heads, a.dim,
+                                    a.causal, dtype);
   const int64_t grid = attn_grid(plan.tiles, a.kv_heads, plan.splits);
   if (grid > INT32_MAX)
     throw Error(RHIP_ERR_UNSUPPORTED, "too many query tiles for one launch");
+  const int64_t rows = static_cast<int64_t>(a.n_q) * a.heads;
+  if (plan.splits > 1 && rows > INT32_MAX)
+    throw Error(RHIP_ERR_UNSUPPORTED, "too many rows for one launch");
   a.tiles = static_cast<int32_t>(plan.tiles), a.splits = plan.splits;
   with_attn(dtype, a.dim, vec, [&](auto t, auto dp, auto v) {
     using T = decltype(t);
@@ -415,9 +465,8 @@ void attn_forward_run(const AttnArgs &args, int32_t dtype, bool vec, hipStream_t
     });
     RHIP_LAUNCH_CHECK();
     if (a.splits > 1) {
-      const int64_t rows = static_cast<int64_t>(a.n_q) * a.heads;
       hipLaunchKernelGGL((attn_join_kernel<T>),
-                         dim3(static_cast<unsigned>(ceil_div(rows, kFwdWaves))), b, 0, stream, a);
+                         dim3(static_cast<unsigned>(rows)), b, 0, stream, a);
       RHIP_LAUNCH_CHECK();
     }
   });
