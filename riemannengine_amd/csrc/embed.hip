@@ -162,11 +162,12 @@ __device__ __forceinline__ void sum_rows(const T *__restrict__ gy, int64_t gy_ro
     for (int e = 0; e < R::V; ++e)
       acc[i][e] = 0.f;
   const int32_t mine = lane_id() < count ? pos[p0 + lane_id()] : 0;
-  for (int p = plane; p < count; p += kUnroll * planes) {
+  // every lane goes every turn: lanes hand each other the positions
+  for (int p = 0; p < count; p += kUnroll * planes) {
     float v[kUnroll][NC][R::V];
 #pragma unroll
     for (int u = 0; u < kUnroll; ++u) {
-      const int q = p + u * planes;
+      const int q = p + plane + u * planes;
       const T *row = gy + static_cast<int64_t>(__shfl(mine, q, kWave)) * gy_row;
 #pragma unroll
       for (int i = 0; i < NC; ++i)

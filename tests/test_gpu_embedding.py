@@ -70,6 +70,18 @@ def test_runs_around_the_segments(dtype, runs):
     check(*make(1, len(ids), len(runs), 48, dtype, ids), 1.0, f"runs {runs}")
 
 
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("C", [4, 13, 32, 64, 100, 256, 520])
+def test_every_count(dtype, C):
+    """Rows used 0 to 66 times, and 67 to 200: every number of positions a
+    wave or a chunk's part can hold, for every number of lanes per row."""
+    for lo, hi in ((0, 67), (67, 201)):
+        runs = torch.arange(lo, hi)
+        ids = torch.repeat_interleave(torch.arange(len(runs)), runs)
+        ids = ids[torch.randperm(len(ids), generator=torch.Generator().manual_seed(C))]
+        check(*make(C, len(ids), len(runs), C, dtype, ids), 1.5, f"counts {lo}..{hi - 1} C {C}")
+
+
 @pytest.mark.parametrize("shift", [0, 1])
 @pytest.mark.parametrize("dtype", [F32, BF16])
 def test_strides(dtype, shift):
