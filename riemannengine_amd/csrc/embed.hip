@@ -423,13 +423,16 @@ extern "C" int rhip_embed_backward(const void *grad_y, int64_t grad_y_row, const
       using T = decltype(t);
       const int chunks = static_cast<int>(ceil_div(C, RowChunk<T>::V));
       const int64_t segments = ceil_div(n, kSegment);
-      // chunks per lane: whole rows in one wave as far as registers go
+      // chunks per lane: whole rows in one wave as far as registers go, unless
+      // that leaves too few waves (8340 labels of 3 classes, 986 wide: 53 us
+      // with two chunks per lane, 41 with one)
+      const int64_t items = ceil_div(vocabulary, kRowsPerWave) + segments;
+      const int64_t fill = 4096 / items; // column tiles that fill the chip
       auto launch = [&](auto nc) {
         constexpr int NC = decltype(nc)::value;
         hipLaunchKernelGGL((embed_backward_kernel<T, NC>),
                            dim3(static_cast<unsigned>(
-                                    ceil_div(ceil_div(vocabulary, kRowsPerWave) + segments,
-                                             kEmbThreads / kWave)),
+                                    ceil_div(items, kEmbThreads / kWave)),
                                 static_cast<unsigned>(ceil_div(chunks, kWave * NC))),
                            dim3(kEmbThreads), 0, stream, static_cast<const T *>(grad_y),
                            grad_y_row, w.sorted, w.order, w.start, n, vocabulary, C,
@@ -437,17 +440,19 @@ extern "C" int rhip_embed_backward(const void *grad_y, int64_t grad_y_row, const
                            static_cast<T *>(grad_weight), w.part, w.runs);
         RHIP_LAUNCH_CHECK();
       };
-      if (chunks <= kWave)
+      if (chunks <= kWave || fill >= ceil_div(chunks, kWave))
         launch(std::integral_constant<int, 1>{});
-      else if (chunks <= 2 * kWave)
+      else if (chunks <= 2 * kWave || fill >= ceil_div(chunks, 2 * kWave))
         launch(std::integral_constant<int, 2>{});
       else
         launch(std::integral_constant<int, 4>{});
       if (segments > 0) {
-        const unsigned tiles =
-            static_cast<unsigned>(std::min<int64_t>(ceil_div(C, kJoinCols), 8));
+        // about 512 workgroups over the runs (no more than table rows) and columns
+        const int64_t runs = std::min<int64_t>({segments, vocabulary, 64});
+        const int64_t tiles =
+            std::min<int64_t>(ceil_div(C, kJoinCols), std::max<int64_t>(1, 512 / runs));
         hipLaunchKernelGGL((embed_join_kernel<T>),
-                           dim3(static_cast<unsigned>(std::min<int64_t>(segments, 64)), tiles),
+                           dim3(static_cast<unsigned>(runs), static_cast<unsigned>(tiles)),
                            dim3(kJoinCols * kJoinLanes), 0, stream, w.sorted, w.start, n, C,
                            scale, w.part, w.runs, static_cast<T *>(grad_weight));
         RHIP_LAUNCH_CHECK();

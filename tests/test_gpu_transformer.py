@@ -136,3 +136,18 @@ def test_training_lowers_the_loss(dtype):
         losses.append(loss.item())
     print(dtype, losses[0], losses[-1], flush=True)
     assert losses[-1] < 0.7 * losses[0]
+
+
+def test_example_trains():
+    """The example's training loop, a few steps in each type."""
+    import importlib.util
+    import os
+    path = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "examples",
+                        "voxel_transformer.py")
+    spec = importlib.util.spec_from_file_location("voxel_transformer", path)
+    example = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(example)
+    for dtype in (torch.float32, torch.bfloat16):
+        losses = example.train(steps=25, n_scenes=2, voxels=600, channels=64, blocks=1,
+                               dtype=dtype, log=lambda text: print(text, flush=True))
+        assert losses[-1] < 0.9 * losses[0]
