@@ -2,6 +2,7 @@
 // each, and the choice of their kernel variants.
 #pragma once
 
+#include <algorithm>
 #include <type_traits>
 
 #include "attn_device.hpp"
@@ -47,6 +48,28 @@ template <typename F> void with_attn(int32_t dtype, int32_t dim, bool vec, F &&f
     typed(float{});
   else
     typed(__bf16{});
+}
+
+// Dynamic LDS, beside a kernel's own, that spreads 512 to 768 workgroups of
+// four blocks over the chip. Workgroups are packed into a CU as long as their
+// LDS fits, so these would fill some CUs and leave others idle; with an
+// allocation that lets no more of them into a CU than each has to take, they
+// spread. The count is the least that the rows can make: a tile of every 32 W.
+// Rows of ragged sequences make some more, which follow the first. Heads of 64,
+// four sequences of 2048: 8 heads (two a CU) forward 68 us packed, 55 spread, dq
+// 75 and 62; 12 heads (three) 81 and 70, dq 86 and 87; 16 heads (four) 89 and
+// 96, so no more than three. Twelve sequences of 650, 8 heads: 42 both ways,
+// but the keys' kernel, which holds its workgroups longer, 43 and 56: it is
+// left packed.
+template <int W> unsigned spread_lds(const AttnArgs &a, int own) {
+  constexpr int64_t kCus = 256;
+  constexpr int kLdsBytes = 160 * 1024;
+  const int64_t tiles = (a.n_q * (a.heads / a.kv_heads) + 32 * W - 1) / (32 * W);
+  const int64_t each = (tiles * a.kv_heads + kCus - 1) / kCus;
+  if (W < 4 || each < 2 || each > 3)
+    return 0;
+  const int fits = kLdsBytes / static_cast<int>(each + 1) + 1024; // each do, one more does not
+  return fits > own ? static_cast<unsigned>(fits - own) : 0u;
 }
 
 // f(W): 32-row blocks per workgroup, 4, 2 or 1.

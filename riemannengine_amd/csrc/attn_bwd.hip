@@ -26,8 +26,13 @@ template <typename T, int DP, int W, bool KEYS> struct BwdShape {
   // and sums, which leaves none to read ahead with: its values stay in LDS,
   // where they fit beside 32-row tiles.
   static constexpr bool kOwnInLds = KEYS && W == 4 && sizeof(T) == 2 && DP == 128;
+  // Rows of the other side per LDS tile: 64 where they fit, 128 of narrow heads
+  // in bf16 (32 wide, four sequences of 4096, 16 heads: 278 and 379 us in 64,
+  // 264 and 352 in 128).
   static constexpr int kBN =
-      W == 1 || (W == 4 && sizeof(T) == 4 && DP == 128) || kOwnInLds ? 32 : 64;
+      W == 1 || (W == 4 && sizeof(T) == 4 && DP == 128) || kOwnInLds ? 32
+      : sizeof(T) == 2 && DP == 32                                   ? 128
+                                                                     : 64;
   static constexpr int kStreams = W == 1 ? kBwdWaves : 1;
   static constexpr int kTileBytes = kBN * DP * sizeof(T);
   static constexpr int kStatBytes = kBN * 8; // (lse2, -delta) of a tile's rows
@@ -209,7 +214,7 @@ attn_dq_kernel(AttnArgs a) {
   using Frag = typename Tile::Frag;
   constexpr int kBN = Shape::kBN;
   constexpr int kAhead = sizeof(T) == 2 ? 4 : 0; // LDS operands on their way to the products
-  constexpr int kB = W == 2 ? 1 : kBN / 32; // blocks of a tile that are a wave's
+  constexpr int kB = kBN / 32 / (W == 2 ? 2 : 1); // blocks of a tile that are a wave's
   using Stream = TileStream<T, DP, kBN, W == 1 ? kWave : kBwdThreads, VEC>;
   __shared__ alignas(16) char lds[Shape::kLds];
 
@@ -224,7 +229,7 @@ attn_dq_kernel(AttnArgs a) {
   const int lane = lane_id(), half = lane >> 5;
   const int w = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
   const int32_t wave0 = row0 + w / Shape::kParts * 32;
-  const int b0 = W == 2 ? w % 2 : 0; // the wave's first block of a tile
+  const int b0 = W == 2 ? w % 2 * kB : 0; // the wave's first block of a tile
   const int32_t row = wave0 + (lane & 31);
   const bool row_ok = row < n_rows;
   const int32_t rc = min(row, n_rows - 1);
@@ -395,7 +400,7 @@ attn_dkv_kernel(AttnArgs a) {
   constexpr int kBM = Shape::kBN;
   constexpr bool kVLds = Shape::kOwnBytes > 0;
   constexpr int kAhead = kVLds ? 3 : 0; // LDS operands on their way to the products
-  constexpr int kB = W == 2 ? 1 : kBM / 32;
+  constexpr int kB = kBM / 32 / (W == 2 ? 2 : 1);
   using Stream = TileStream<T, DP, kBM, W == 1 ? kWave : kBwdThreads, VEC>;
   __shared__ alignas(16) char lds[Shape::kLds];
 
@@ -410,7 +415,7 @@ attn_dkv_kernel(AttnArgs a) {
   const int lane = lane_id(), half = lane >> 5;
   const int w = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
   const int32_t wave0 = key0 + w / Shape::kParts * 32;
-  const int b0 = W == 2 ? w % 2 : 0;
+  const int b0 = W == 2 ? w % 2 * kB : 0;
   const int32_t key = wave0 + (lane & 31);
   const bool key_ok = key < sq.lk;
   const int32_t lo = first_row(a, sq, key);
@@ -742,8 +747,9 @@ void attn_backward_run(const AttnArgs &args, int32_t dtype, bool vec, hipStream_
     const dim3 b(kBwdThreads);
     if (args.n_q > 0) {
       with_waves(pq.waves, [&](auto w) {
-        hipLaunchKernelGGL((attn_dq_kernel<T, DP, VEC, decltype(w)::value>), dim3(gq), b, 0,
-                           stream, aq);
+        constexpr int W = decltype(w)::value;
+        const unsigned spread = spread_lds<W>(aq, BwdShape<T, DP, W, false>::kLds);
+        hipLaunchKernelGGL((attn_dq_kernel<T, DP, VEC, W>), dim3(gq), b, spread, stream, aq);
       });
       RHIP_LAUNCH_CHECK();
     }
