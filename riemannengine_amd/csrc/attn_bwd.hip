@@ -24,8 +24,9 @@ template <typename T, int DP, int W, bool KEYS> struct BwdShape {
   static constexpr int kParts = kBwdWaves / W; // waves that share a block of rows
   // The keys' kernel in bf16 at full width holds 192 registers of keys, values
   // and sums, which leaves none to read ahead with: its values stay in LDS,
-  // where they fit beside 32-row tiles.
-  static constexpr bool kOwnInLds = KEYS && W == 4 && sizeof(T) == 2 && DP == 128;
+  // where they fit beside 32-row tiles. (W = 1, 4 heads, one causal sequence of
+  // 1000: 30 us from registers, which spill, 23 from LDS.)
+  static constexpr bool kOwnInLds = KEYS && W != 2 && sizeof(T) == 2 && DP == 128;
   // Rows of the other side per LDS tile: 64 where they fit, 128 of narrow heads
   // in bf16 (32 wide, four sequences of 4096, 16 heads: 278 and 379 us in 64,
   // 264 and 352 in 128).
@@ -33,11 +34,17 @@ template <typename T, int DP, int W, bool KEYS> struct BwdShape {
       W == 1 || (W == 4 && sizeof(T) == 4 && DP == 128) || kOwnInLds ? 32
       : sizeof(T) == 2 && DP == 32                                   ? 128
                                                                      : 64;
+  // Registers let two workgroups into a CU. Two buffers where they leave LDS for
+  // as many: two workgroups cover each other's waits better than a second
+  // buffer does. (W = 1, two buffers and one workgroup, then one buffer and two:
+  // fp32, 64 wide, 6 over 2 heads, three of 1100: dq 80 us, 71; bf16, 128 wide, 16
+  // over 2 heads, one of 1500: keys' kernel 71 us, 40.)
+  static constexpr bool kSlim = sizeof(T) == 2 || DP <= (KEYS && W == 4 ? 32 : 64);
   static constexpr int kStreams = W == 1 ? kBwdWaves : 1;
   static constexpr int kTileBytes = kBN * DP * sizeof(T);
   static constexpr int kStatBytes = kBN * 8; // (lse2, -delta) of a tile's rows
   static constexpr int kBufBytes = 2 * kTileBytes + kStatBytes;
-  static constexpr int kBuffers = kStreams * 2 * kBufBytes <= 160 * 1024 ? 2 : 1;
+  static constexpr int kBuffers = kStreams * 2 * kBufBytes <= (kSlim ? 80 : 160) * 1024 ? 2 : 1;
   static constexpr int kJoinRow = DP + 4; // floats per row of the joined sums
   static constexpr int kJoinBytes =
       W < 4 ? kBwdWaves * 32 * kJoinRow * static_cast<int>(sizeof(float)) : 0;
@@ -45,8 +52,7 @@ template <typename T, int DP, int W, bool KEYS> struct BwdShape {
   static constexpr int kStageBytes = kStreams * kBuffers * kBufBytes + kOwnBytes;
   static constexpr int kLds = kStageBytes > kJoinBytes ? kStageBytes : kJoinBytes;
   // waves per SIMD: two workgroups' where their LDS and registers fit
-  static constexpr int kOccupancy =
-      kLds > 80 * 1024 || (sizeof(T) == 4 && DP >= (KEYS ? 64 : 96)) ? 1 : 2;
+  static constexpr int kOccupancy = kSlim && kLds <= 80 * 1024 ? 2 : 1;
 };
 
 // The first query row that sees key j, and the keys that row i sees.
@@ -459,7 +465,7 @@ attn_dkv_kernel(AttnArgs a) {
   char *own = lds + Shape::kStreams * Shape::kBuffers * Shape::kBufBytes;
   if (first < n1)
     issue(first, 0);
-  if (kVLds && first < n1) { // the first turn waits for it; without one it may not start
+  if (kVLds && n0 < n1) { // waited for in the first turn; without one it may not start
     TileStream<T, DP, Shape::kRows, kBwdThreads, VEC> os;
     os.init(a.v_row, a.dim);
     os.issue(own,
@@ -488,7 +494,11 @@ attn_dkv_kernel(AttnArgs a) {
   const uint32_t stage_at = lds_address(stage);
   typename Tile::Lane own_at{}; // this wave's keys in `own`
   if constexpr (kVLds)
-    own_at = lane_at.in(lds_address(own) + w * (32 / 4) * Tile::kGroup);
+    own_at = lane_at.in(lds_address(own) + w / Shape::kParts * (32 / 4) * Tile::kGroup);
+  if constexpr (kVLds && W == 1) { // waves take turns of their own
+    wait_stream();
+    __syncthreads();
+  }
   int buf = 0;
   for (int32_t n = first; n < n1; n += step) {
     wait_stream();

@@ -33,16 +33,20 @@ template <typename T, int DP, int W> struct FwdShape {
                                                                                 : 64;
   static constexpr int kStreams = W == 1 ? kFwdWaves : 1;
   static constexpr int kTileBytes = kBN * DP * sizeof(T);
-  // two buffers, but for fp32 at full width where four waves' would not fit
-  static constexpr int kBuffers = kStreams * 4 * kTileBytes <= 160 * 1024 ? 2 : 1;
+  // Registers let two workgroups into a CU.
+  static constexpr bool kSlim = sizeof(T) == 2 || DP <= 64;
+  // Two buffers where they leave LDS for as many workgroups: two cover each
+  // other's waits better than a second buffer does. (fp32, 64 wide, 6 over 2
+  // heads, three causal sequences of 1100: two buffers and one workgroup 72 us,
+  // one buffer and two workgroups 57.)
+  static constexpr int kBuffers = kStreams * 4 * kTileBytes <= (kSlim ? 80 : 160) * 1024 ? 2 : 1;
   static constexpr int kJoinRow = DP + 4; // floats per row of the joined results
   static constexpr int kJoinBytes =
       W < 4 ? kFwdWaves * 32 * (kJoinRow + 2) * static_cast<int>(sizeof(float)) : 0;
   static constexpr int kStageBytes = kStreams * kBuffers * 2 * kTileBytes;
   static constexpr int kLds = kStageBytes > kJoinBytes ? kStageBytes : kJoinBytes;
   // waves per SIMD: two workgroups' where their LDS and registers fit
-  static constexpr int kOccupancy =
-      kLds > 80 * 1024 || (sizeof(T) == 4 && DP >= 96) ? 1 : 2;
+  static constexpr int kOccupancy = kSlim && kLds <= 80 * 1024 ? 2 : 1;
 };
 
 // One row by its definition, for rows whose sums came out not finite under a
