@@ -1,5 +1,7 @@
 /*
- * riemann_hip.h — C ABI of the MI355X (gfx950) sparse-convolution hot path.
+ * riemann_hip.h — C ABI of the MI355X (gfx950) sparse-convolution hot path,
+ * and of the operators of transformer stages over its packed rows (attention,
+ * layer norm, embedding: the last sections).
  *
  * The library is stateless: every buffer is owned by the caller (device
  * pointers unless stated otherwise), every call takes the HIP stream it runs

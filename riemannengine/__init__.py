@@ -12,7 +12,10 @@ layers call the gfx950 kernels through the C ABI:
     ConvolutionMode, PoolingMode, QuantizationMode, RegionType,
     RiemannAlgorithm, nn (RiemannConvolution, RiemannConvolutionTranspose,
     RiemannGenerativeConvolutionTranspose, the pooling layers,
-    RiemannBatchNorm, RiemannReLU, BasicBlock)
+    RiemannBatchNorm, RiemannReLU, BasicBlock; and, which the reference does
+    not have, transformer stages over packed rows: packed_attention,
+    layer_norm, embedding, RiemannAttention, RiemannLayerNorm,
+    RiemannEmbedding, AttentionBlock)
 
 The reference's names outside that path (``adaptive``, ``gaussian``,
 ``occupancy``, ``TensorField``, the collation helpers, ``RiemannLinear``, ...)

@@ -3,7 +3,8 @@
 Coordinate hashing, kernel-map generation, gather-GEMM-scatter sparse
 convolution (forward, dX, dW) and sparse pooling (stride maps, local and
 global sum / average / max) as hand-written gfx950 HIP kernels behind the C
-ABI in include/riemann_hip.h (libriemann_hip.so).
+ABI in include/riemann_hip.h (libriemann_hip.so), and with them the operators
+of a transformer stage over packed rows: attention, layer norm, embedding.
 
 * ``SparseTensor``, ``CoordinateManager``, ``CoordinateMapKey``, ``nn`` and
   the enums come from the C++ host layer (``_C``), which mirrors the

@@ -212,6 +212,9 @@ __device__ __forceinline__ void join_row(const float *rows, int row_floats, int 
 // also the rows' statistics. Blocks are transposed as in the forward (S^T = K
 // Q^T, dP^T = V dO^T), so dS^T is the right operand of dQ^T = K^T dS^T as it
 // lies. dP's sums start at -delta.
+//
+// Bound by the matrix cores (four causal prompts of 4096, 16 over 4 heads, 128
+// wide, bf16: 418 us, 987 TFLOP/s), by the vector instructions at 32 wide (840).
 template <typename T, int DP, bool VEC, int W>
 __global__ __launch_bounds__(kBwdThreads, (BwdShape<T, DP, W, false>::kOccupancy)) void
 attn_dq_kernel(AttnArgs a) {
@@ -397,6 +400,9 @@ attn_dq_kernel(AttnArgs a) {
 // head of its group. A lane holds one key's column (S = Q K^T, dP = dO V^T),
 // so P and dS are the right operands of dV^T = dO^T P and dK^T = Q^T dS as
 // they lie.
+//
+// Bound by the matrix cores and by the tiles' reads from LDS (same prompts: 613
+// us, 897 TFLOP/s, four products a block against the other kernel's three).
 template <typename T, int DP, bool VEC, int W>
 __global__ __launch_bounds__(kBwdThreads, (BwdShape<T, DP, W, true>::kOccupancy)) void
 attn_dkv_kernel(AttnArgs a) {

