@@ -130,7 +130,7 @@ __device__ void finish_row(const AttnArgs &a, const AttnSeq &sq, int32_t i, int3
 // multiplied.
 //
 // Bounds: the matrix cores at width 128 (four causal prompts of 4096, 16 over 4
-// heads, bf16: 327 us, 840 TFLOP/s; the cores busy for 61% of the launch, the
+// heads, bf16: 327 us, 840 TFLOP/s; the cores busy for 40% of the cycles, the
 // softmax's vector instructions beside them); the vector instructions at 32 and
 // 64 (600 and 870: a score costs one exponential whatever the width); memory
 // for single tokens (32 over caches of 1 to 16384, 8 key heads of 128: 4.7 TB/s).
