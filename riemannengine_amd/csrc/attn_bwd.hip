@@ -585,7 +585,14 @@ attn_dkv_kernel(AttnArgs a) {
     }
   }
 
-  // rows behind the keys in use get zeros (no tile was added to them)
+  // Rows of the region behind the keys in use get zeros: where their lanes
+  // share a wave with keys in use, those met them as a key of zeros, with a
+  // probability of exp(-lse).
+  if (!key_ok) {
+#pragma unroll
+    for (int db = 0; db < Tile::kDBlocks; ++db)
+      dk[db] = dv[db] = v16f{};
+  }
   if constexpr (W == 4) {
     if (a.splits > 1) {
       if (key < room) {
