@@ -985,10 +985,21 @@ def _dense_last(t: torch.Tensor) -> torch.Tensor:
     return t if t.shape[-1] <= 1 or t.stride(-1) == 1 else t.contiguous()
 
 
+def _require_dense(t: Optional[torch.Tensor], name: str, shape, dtype: torch.dtype,
+                   device: torch.device) -> None:
+    """t, which may be None, is what the library takes its pointer for: the
+    kernels read and write `shape` values of `dtype` from there on."""
+    if t is not None and (t.device != device or t.dtype != dtype or tuple(t.shape) != tuple(shape)
+                          or not t.is_contiguous()):
+        raise RuntimeError(f"{name} must be a dense {tuple(shape)} tensor of {dtype} on {device}")
+
+
 def _attn_desc(q, k, v, q_offsets, k_offsets, k_lengths, causal, scale) -> RhipAttn:
-    for t, name in ((q, "q"), (k, "k"), (v, "v"), (q_offsets, "q_offsets"),
-                    (k_offsets, "k_offsets")):
-        _require_cuda(t, name)
+    _require_cuda(q, "q")
+    for t, name in ((k, "k"), (v, "v"), (q_offsets, "q_offsets"), (k_offsets, "k_offsets"),
+                    (k_lengths, "k_lengths")):
+        if t is not None and t.device != q.device:
+            raise RuntimeError(f"{name} must be on the queries' device {q.device}")
     if q.dim() != 3 or k.dim() != 3 or v.shape != k.shape or q.shape[2] != k.shape[2]:
         raise RuntimeError("q must be [n_q, heads, dim], k and v [n_k, kv_heads, dim]")
     if k.dtype != q.dtype or v.dtype != q.dtype:
@@ -1022,6 +1033,7 @@ def attn_forward(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, q_offsets: t
     receives out's rounding error."""
     q, k, v = _dense_last(q), _dense_last(k), _dense_last(v)
     desc = _attn_desc(q, k, v, q_offsets, k_offsets, k_lengths, causal, scale)
+    _require_dense(rest, "rest", q.shape, torch.bfloat16, q.device)
     out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
     lse = torch.empty((q.shape[1], q.shape[0]), dtype=torch.float32, device=q.device)
     ws = _attn_ws(desc, False, q.device)
@@ -1040,6 +1052,11 @@ def attn_backward(grad_out: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: t
     q, k, v = _dense_last(q), _dense_last(k), _dense_last(v)
     grad_out = _dense_last(grad_out.to(q.dtype))
     desc = _attn_desc(q, k, v, q_offsets, k_offsets, k_lengths, causal, scale)
+    if grad_out.shape != q.shape or grad_out.device != q.device:
+        raise RuntimeError("grad_out does not match q")
+    _require_dense(out, "out", q.shape, q.dtype, q.device)
+    _require_dense(rest, "rest", q.shape, torch.bfloat16, q.device)
+    _require_dense(lse, "lse", (q.shape[1], q.shape[0]), torch.float32, q.device)
     gq = torch.empty(q.shape, dtype=q.dtype, device=q.device)
     gk = torch.empty(k.shape, dtype=q.dtype, device=q.device)
     gv = torch.empty(k.shape, dtype=q.dtype, device=q.device)
@@ -1057,8 +1074,12 @@ def ln_forward(x: torch.Tensor, weight: Optional[torch.Tensor] = None,
     """(y, mean, rstd) of the rows of x [n, C]; weight and bias fp32 [C]."""
     _require_cuda(x, "x")
     dt = _dtype_code(x.dtype)
+    if x.dim() != 2:
+        raise RuntimeError("x must be [n, C]")
     x = _dense_last(x)
     n, C = x.shape
+    _require_dense(weight, "weight", (C,), torch.float32, x.device)
+    _require_dense(bias, "bias", (C,), torch.float32, x.device)
     y = torch.empty((n, C), dtype=x.dtype, device=x.device)
     f32 = dict(dtype=torch.float32, device=x.device)
     mean, rstd = torch.empty(n, **f32), torch.empty(n, **f32)
@@ -1073,8 +1094,13 @@ def ln_backward(grad_y: torch.Tensor, x: torch.Tensor, mean: torch.Tensor, rstd:
     """(grad_x, grad_weight, grad_bias)."""
     _require_cuda(x, "x")
     dt = _dtype_code(x.dtype)
+    if x.dim() != 2 or grad_y.shape != x.shape or grad_y.device != x.device:
+        raise RuntimeError("x and grad_y must be [n, C] on one device")
     x, grad_y = _dense_last(x), _dense_last(grad_y.to(x.dtype))
     n, C = x.shape
+    _require_dense(mean, "mean", (n,), torch.float32, x.device)
+    _require_dense(rstd, "rstd", (n,), torch.float32, x.device)
+    _require_dense(weight, "weight", (C,), torch.float32, x.device)
     gx = torch.empty((n, C), dtype=x.dtype, device=x.device)
     f32 = dict(dtype=torch.float32, device=x.device)
     gw, gb = torch.empty(C, **f32), torch.empty(C, **f32)
@@ -1096,8 +1122,10 @@ def _ids(ids: torch.Tensor) -> torch.Tensor:
 
 def embed_forward(ids: torch.Tensor, weight: torch.Tensor, scale: float = 1.0) -> torch.Tensor:
     """scale * weight[ids], zero rows for ids outside the table."""
-    ids, weight = _ids(ids), _dense_last(weight)
-    _require_cuda(weight, "weight")
+    ids = _ids(ids)
+    if weight.dim() != 2 or weight.device != ids.device:
+        raise RuntimeError("weight must be [vocabulary, C] on the ids' device")
+    weight = _dense_last(weight)
     V, C = weight.shape
     y = torch.empty((ids.numel(), C), dtype=weight.dtype, device=weight.device)
     _check(lib().rhip_embed_forward(_ptr(ids), int(ids.dtype == torch.int32), ids.numel(),
@@ -1110,8 +1138,10 @@ def embed_forward(ids: torch.Tensor, weight: torch.Tensor, scale: float = 1.0) -
 def embed_backward(grad_y: torch.Tensor, ids: torch.Tensor, vocabulary: int,
                    scale: float = 1.0) -> torch.Tensor:
     """grad_weight [vocabulary, C] of embed_forward."""
-    ids, grad_y = _ids(ids), _dense_last(grad_y)
-    _require_cuda(grad_y, "grad_y")
+    ids = _ids(ids)
+    if grad_y.dim() != 2 or grad_y.shape[0] != ids.numel() or grad_y.device != ids.device:
+        raise RuntimeError("grad_y must hold one row for each id, on the ids' device")
+    grad_y = _dense_last(grad_y)
     n, C = grad_y.shape
     gw = torch.empty((vocabulary, C), dtype=grad_y.dtype, device=grad_y.device)
     ws = torch.empty(_sizeq(lib().rhip_embed_workspace_bytes, n, vocabulary, C),
