@@ -51,8 +51,11 @@ template <typename T, int DP, int W, bool KEYS> struct BwdShape {
   static constexpr int kOwnBytes = kOwnInLds ? kRows * DP * static_cast<int>(sizeof(T)) : 0;
   static constexpr int kStageBytes = kStreams * kBuffers * kBufBytes + kOwnBytes;
   static constexpr int kLds = kStageBytes > kJoinBytes ? kStageBytes : kJoinBytes;
-  // waves per SIMD: two workgroups' where their LDS and registers fit
-  static constexpr int kOccupancy = kSlim && kLds <= 80 * 1024 ? 2 : 1;
+  // Waves per SIMD: two workgroups' where their LDS and registers fit; 64 wide in
+  // bf16 three, within 168 registers, which the compiler would pass by two.
+  static constexpr int kOccupancy = !kSlim || kLds > 80 * 1024                      ? 1
+                                    : sizeof(T) == 2 && DP == 64 && kLds < 53 * 1024 ? 3
+                                                                                     : 2;
 };
 
 // The first query row that sees key j, and the keys that row i sees.
@@ -66,89 +69,6 @@ __device__ __forceinline__ int32_t keys_seen(const AttnArgs &a, const AttnSeq &s
   return static_cast<int32_t>(n < 0 ? 0 : n);
 }
 
-template <typename T> __device__ __forceinline__ float dot(const T *x, const T *y, int32_t dim) {
-  float s = 0.f;
-  for (int d = 0; d < dim; ++d)
-    s = fmaf(to_f32(x[d]), to_f32(y[d]), s);
-  return s;
-}
-
-// The places a gradient row is read and computed from.
-template <typename T> struct Rows {
-  const T *q, *go, *k, *v;
-};
-template <typename T>
-__device__ __forceinline__ Rows<T> rows_of(const AttnArgs &a, const AttnSeq &sq, int head) {
-  const int kv = head / a.group;
-  return {static_cast<const T *>(a.q) + sq.q0 * a.q_row + head * a.q_head,
-          static_cast<const T *>(a.go) + sq.q0 * a.go_row + head * a.go_head,
-          static_cast<const T *>(a.k) + sq.k0 * a.k_row + kv * a.k_head,
-          static_cast<const T *>(a.v) + sq.k0 * a.v_row + kv * a.v_head};
-}
-
-// A gradient row by its definition, reading only what it depends on, where
-// the tiles' sums came out not finite under a causal mask (a masked entry's
-// zero times a value that is not finite). One wave; lane l returns elements l
-// and l + 64 of dq (without scale).
-template <typename T>
-__device__ void exact_dq(const AttnArgs &a, const AttnSeq &sq, int32_t i, int head, float &g0,
-                         float &g1) {
-  const Rows<T> p = rows_of<T>(a, sq, head);
-  const int lane = lane_id();
-  const float2 st = a.stat[static_cast<int64_t>(head) * a.n_q + sq.q0 + i];
-  const int32_t lim = keys_seen(a, sq, i);
-  g0 = g1 = 0.f;
-  for (int32_t j0 = 0; j0 < lim; j0 += kWave) {
-    float ds = 0.f;
-    if (j0 + lane < lim) {
-      const T *kj = p.k + static_cast<int64_t>(j0 + lane) * a.k_row;
-      const T *vj = p.v + static_cast<int64_t>(j0 + lane) * a.v_row;
-      const float s = dot(p.q + i * a.q_row, kj, a.dim);
-      ds = exp2_fast(fmaf(s, a.c, -st.x)) * (dot(p.go + i * a.go_row, vj, a.dim) + st.y);
-    }
-    for (int e = 0; e < min(kWave, lim - j0); ++e) {
-      const float de = __shfl(ds, e, kWave);
-      const T *kj = p.k + static_cast<int64_t>(j0 + e) * a.k_row;
-      if (lane < a.dim)
-        g0 = fmaf(de, to_f32(kj[lane]), g0);
-      if (lane + kWave < a.dim)
-        g1 = fmaf(de, to_f32(kj[lane + kWave]), g1);
-    }
-  }
-}
-// The same for dk (without scale) and dv of key j.
-template <typename T>
-__device__ void exact_dkv(const AttnArgs &a, const AttnSeq &sq, int32_t j, int kv, float (&gk)[2],
-                          float (&gv)[2]) {
-  const int lane = lane_id();
-  gk[0] = gk[1] = gv[0] = gv[1] = 0.f;
-  for (int head = kv * a.group; head < (kv + 1) * a.group; ++head) {
-    const Rows<T> p = rows_of<T>(a, sq, head);
-    const T *kj = p.k + static_cast<int64_t>(j) * a.k_row;
-    const T *vj = p.v + static_cast<int64_t>(j) * a.v_row;
-    for (int32_t i0 = first_row(a, sq, j); i0 < sq.lq; i0 += kWave) {
-      float pe = 0.f, ds = 0.f;
-      const int64_t i = i0 + lane;
-      if (i < sq.lq) {
-        const float2 st = a.stat[static_cast<int64_t>(head) * a.n_q + sq.q0 + i];
-        pe = exp2_fast(fmaf(dot(p.q + i * a.q_row, kj, a.dim), a.c, -st.x));
-        ds = pe * (dot(p.go + i * a.go_row, vj, a.dim) + st.y);
-      }
-      for (int e = 0; e < min(kWave, sq.lq - i0); ++e) {
-        const float p1 = __shfl(pe, e, kWave), d1 = __shfl(ds, e, kWave);
-#pragma unroll
-        for (int u = 0; u < 2; ++u) {
-          const int d = lane + u * kWave;
-          if (d < a.dim) {
-            gv[u] = fmaf(p1, to_f32(p.go[static_cast<int64_t>(i0 + e) * a.go_row + d]), gv[u]);
-            gk[u] = fmaf(d1, to_f32(p.q[static_cast<int64_t>(i0 + e) * a.q_row + d]), gk[u]);
-          }
-        }
-      }
-    }
-  }
-}
-
 template <typename T>
 __device__ __forceinline__ void put2(T *p, int dim, float v0, float v1, float mul) {
   const int lane = lane_id();
@@ -158,23 +78,16 @@ __device__ __forceinline__ void put2(T *p, int dim, float v0, float v1, float mu
     p[lane + kWave] = from_f32<T>(v1 * mul);
 }
 
-// One wave writes a dq row; lane l holds elements l and l + 64 of its sum.
+// One wave writes a row of dq, or of dk and dv; lane l holds elements l and
+// l + 64 of its sum.
 template <typename T>
-__device__ void finish_dq(const AttnArgs &a, const AttnSeq &sq, int32_t i, int head, float g0,
-                          float g1) {
-  if (a.causal && __any(!isfinite(g0) || !isfinite(g1)))
-    exact_dq<T>(a, sq, i, head, g0, g1);
-  put2(static_cast<T *>(a.gq) +
-           ((sq.q0 + static_cast<int64_t>(i)) * a.heads + head) * a.dim,
-       a.dim, g0, g1, a.scale);
+__device__ void finish_dq(const AttnArgs &a, int64_t row, int head, float g0, float g1) {
+  put2(static_cast<T *>(a.gq) + (row * a.heads + head) * a.dim, a.dim, g0, g1, a.scale);
 }
 template <typename T>
-__device__ void finish_dkv(const AttnArgs &a, const AttnSeq &sq, int32_t j, int kv,
-                           float (&gk)[2], float (&gv)[2]) {
-  if (a.causal && j < sq.lk &&
-      __any(!isfinite(gk[0]) || !isfinite(gk[1]) || !isfinite(gv[0]) || !isfinite(gv[1])))
-    exact_dkv<T>(a, sq, j, kv, gk, gv);
-  const int64_t at = ((sq.k0 + static_cast<int64_t>(j)) * a.kv_heads + kv) * a.dim;
+__device__ void finish_dkv(const AttnArgs &a, int64_t key, int kv, const float (&gk)[2],
+                           const float (&gv)[2]) {
+  const int64_t at = (key * a.kv_heads + kv) * a.dim;
   put2(static_cast<T *>(a.gk) + at, a.dim, gk[0], gk[1], a.scale);
   put2(static_cast<T *>(a.gv) + at, a.dim, gv[0], gv[1], 1.f);
 }
@@ -226,6 +139,7 @@ attn_dq_kernel(AttnArgs a) {
   constexpr int kB = kBN / 32 / (W == 2 ? 2 : 1); // blocks of a tile that are a wave's
   using Stream = TileStream<T, DP, kBN, W == 1 ? kWave : kBwdThreads, VEC>;
   __shared__ alignas(16) char lds[Shape::kLds];
+  __shared__ int any_left_out;
 
   int32_t t, kv, split;
   if (!attn_item(a, t, kv, split))
@@ -246,9 +160,11 @@ attn_dq_kernel(AttnArgs a) {
   const int head = kv * a.group + rc % a.group;
   auto sees = [&](int32_t r) { return keys_seen(a, sq, r / a.group); };
   const int32_t lim = row_ok ? sees(row) : 0;
-  const int32_t wg_lim = sees(min(row0 + Shape::kRows, n_rows) - 1);
-  const int32_t wave_lim = wave0 < n_rows ? sees(min(wave0 + 32, n_rows) - 1) : 0;
-  const int32_t wave_full = wave0 < n_rows ? sees(wave0) : 0;
+  const int32_t wg_lim = wave_uniform(sees(min(row0 + Shape::kRows, n_rows) - 1));
+  const int32_t wg_full = wave_uniform(sees(row0));
+  const int32_t wave_lim =
+      wave_uniform(wave0 < n_rows ? sees(min(wave0 + 32, n_rows) - 1) : 0);
+  const int32_t wave_full = wave_uniform(wave0 < n_rows ? sees(wave0) : 0);
   const int32_t kt1 = a.gq ? (wg_lim + kBN - 1) / kBN : 0; // else statistics alone
   const int32_t first = W == 1 ? w : 0, step = W == 1 ? kBwdWaves : 1;
 
@@ -296,10 +212,18 @@ attn_dq_kernel(AttnArgs a) {
   if (row_ok) {
     const int64_t li = static_cast<int64_t>(head) * a.n_q + gr;
     lse2 = a.lse[li] * kLog2e;
+    if (lse2 == INFINITY) // an infinite score: the row's probabilities are NaN
+      lse2 = NAN;
     if (half == 0 && w % Shape::kParts == 0)
       a.stat[li] = make_float2(lse2, -delta);
   }
 
+  // As in the forward, but for whole keys: where the row's statistics are finite, a
+  // key that is not has probability zero and adds nothing but NaN at the places
+  // that are not finite. Where they are not, all of the row's sums are NaN.
+  bool left_out = false;
+  if (W > 1 && threadIdx.x == 0)
+    any_left_out = 0;
   v16f dq[Tile::kDBlocks], dp0;
 #pragma unroll
   for (int db = 0; db < Tile::kDBlocks; ++db)
@@ -315,6 +239,19 @@ attn_dq_kernel(AttnArgs a) {
     wait_stream(); // as in the forward
     if constexpr (W > 1)
       __syncthreads();
+    if (wg_full < wg_lim && (kt + 1) * kBN > wg_full) {
+      rare_path();
+      const bool found = Tile::template zero_not_finite<true, kBN, W == 1 ? 1 : kBwdWaves>(
+          stage_at + buf * Shape::kBufBytes, W == 1 ? 0 : w);
+      if constexpr (W > 1) {
+        if (found)
+          any_left_out = 1;
+        __syncthreads();
+        left_out = wave_uniform(any_left_out) != 0;
+      } else {
+        left_out |= found;
+      }
+    }
     const typename Tile::Lane at =
         lane_at.in(stage_at + buf * Shape::kBufBytes + b0 * (32 / 4) * Tile::kGroup);
     if (Shape::kBuffers == 2 && kt + step < kt1)
@@ -345,9 +282,10 @@ attn_dq_kernel(AttnArgs a) {
                 s[r] = exp2_fast(fmaf(s[r], a.c, -lse2)) * dp[r];
               if (masked) {
                 rare_path();
+                const int32_t seen = lim - j0 - 32 * b - 4 * half;
 #pragma unroll
                 for (int r = 0; r < 16; ++r)
-                  s[r] = j0 + 32 * b + block_row(r) < lim ? s[r] : 0.f;
+                  s[r] = block_row(r) < seen ? s[r] : 0.f;
               }
               Tile::pack(s, ds);
             });
@@ -364,24 +302,15 @@ attn_dq_kernel(AttnArgs a) {
   }
   if (!a.gq)
     return;
+  if (left_out)
+    Tile::template add_not_finite<true>(kp, a.k_row, a.dim, max(wg_full - kBN, 0), wave_lim,
+                                        [&](int32_t j) { return j < lim; }, dq);
   if constexpr (W == 4) {
-    bool bad = false;
-    if (a.causal && row_ok) {
-#pragma unroll
-      for (int db = 0; db < Tile::kDBlocks; ++db)
-#pragma unroll
-        for (int r = 0; r < 16; ++r)
-          bad |= !isfinite(dq[db][r]);
-    }
-    uint64_t redo = __ballot(bad);
-    redo = (redo | redo >> 32) & 0xffffffffull;
-    if (row_ok && !((redo >> (lane & 31)) & 1))
-      Tile::template store_column<VEC>(
-          static_cast<T *>(a.gq) + (gr * a.heads + head) * a.dim, a.dim, a.scale, dq);
-    while (redo) {
-      const int i = __ffsll(static_cast<unsigned long long>(redo)) - 1;
-      redo &= redo - 1;
-      finish_dq<T>(a, sq, __shfl(qi, i, kWave), __shfl(head, i, kWave), NAN, NAN);
+    const int32_t my_row = wave0 + (opaque(lane) & 31); // not kept through the loop
+    if (my_row < n_rows) {
+      const int64_t place = (sq.q0 + static_cast<int64_t>(my_row / a.group)) * a.heads +
+                            kv * a.group + my_row % a.group;
+      Tile::template store_column<VEC>(static_cast<T *>(a.gq) + place * a.dim, a.dim, a.scale, dq);
     }
   } else {
     __syncthreads(); // every wave is past its tiles
@@ -391,7 +320,8 @@ attn_dq_kernel(AttnArgs a) {
     for (int r = w; r < Shape::kRows && row0 + r < n_rows; r += kBwdWaves) {
       float g0, g1;
       join_row<DP, Shape::kParts>(join, Shape::kJoinRow, r, g0, g1);
-      finish_dq<T>(a, sq, (row0 + r) / a.group, kv * a.group + (row0 + r) % a.group, g0, g1);
+      finish_dq<T>(a, sq.q0 + static_cast<int64_t>((row0 + r) / a.group),
+                   kv * a.group + (row0 + r) % a.group, g0, g1);
     }
   }
 }
@@ -411,10 +341,13 @@ attn_dkv_kernel(AttnArgs a) {
   using Frag = typename Tile::Frag;
   constexpr int kBM = Shape::kBN;
   constexpr bool kVLds = Shape::kOwnBytes > 0;
-  constexpr int kAhead = kVLds ? 3 : 0; // LDS operands on their way to the products
+  // LDS operands on their way to the products (96 wide: 490 us for 558 left to the
+  // compiler, four causal texts of 4096, 16 over 4 heads)
+  constexpr int kAhead = kVLds || (sizeof(T) == 2 && DP == 96) ? 3 : 0;
   constexpr int kB = kBM / 32 / (W == 2 ? 2 : 1);
   using Stream = TileStream<T, DP, kBM, W == 1 ? kWave : kBwdThreads, VEC>;
   __shared__ alignas(16) char lds[Shape::kLds];
+  __shared__ int any_left_out;
 
   int32_t t, kv, split;
   if (!attn_item(a, t, kv, split))
@@ -431,9 +364,12 @@ attn_dkv_kernel(AttnArgs a) {
   const int32_t key = wave0 + (lane & 31);
   const bool key_ok = key < sq.lk;
   const int32_t lo = first_row(a, sq, key);
-  const int32_t wave_lo = first_row(a, sq, wave0);         // no earlier row sees any
-  const int32_t wave_full = first_row(a, sq, wave0 + 31);  // every later row sees all
-  const int32_t it0 = first_row(a, sq, key0) / kBM;
+  // no earlier row sees any key of the wave's; every later row sees all
+  const int32_t wave_lo = wave_uniform(first_row(a, sq, wave0));
+  const int32_t wave_full = wave_uniform(first_row(a, sq, wave0 + 31));
+  const int32_t wg_full =
+      wave_uniform(first_row(a, sq, min(key0 + Shape::kRows, sq.lk) - 1));
+  const int32_t it0 = wave_uniform(first_row(a, sq, key0)) / kBM;
   // tiles of query rows from the first that sees a key, for each head; this
   // workgroup's part of them
   const int32_t per_head = key0 < sq.lk ? max((sq.lq + kBM - 1) / kBM - it0, 0) : 0;
@@ -491,6 +427,12 @@ attn_dkv_kernel(AttnArgs a) {
     if constexpr (!kVLds)
       vf[s] = __builtin_bit_cast(Frag, Tile::template chunk<VEC>(vp, c, a.dim, key_ok));
   }
+  // As in the forward: values of grad_out that are not finite, and whole query
+  // rows that hold one, in tiles of which some keys are not seen. Such a query
+  // row's statistics are not finite, so what it adds is NaN without its values.
+  bool left_out = false;
+  if (W > 1 && threadIdx.x == 0)
+    any_left_out = 0;
   v16f dk[Tile::kDBlocks], dv[Tile::kDBlocks];
 #pragma unroll
   for (int db = 0; db < Tile::kDBlocks; ++db)
@@ -510,6 +452,22 @@ attn_dkv_kernel(AttnArgs a) {
     wait_stream();
     if constexpr (W > 1)
       __syncthreads();
+    if ((it0 + n % per_head) * kBM < wg_full) {
+      rare_path();
+      const uint32_t tile = stage_at + buf * Shape::kBufBytes;
+      constexpr int kShare = W == 1 ? 1 : kBwdWaves;
+      Tile::template zero_not_finite<true, kBM, kShare>(tile, W == 1 ? 0 : w);
+      const bool found = Tile::template zero_not_finite<false, kBM, kShare>(
+          tile + Shape::kTileBytes, W == 1 ? 0 : w);
+      if constexpr (W > 1) {
+        if (found)
+          any_left_out = 1;
+        __syncthreads();
+        left_out = wave_uniform(any_left_out) != 0;
+      } else {
+        left_out |= found;
+      }
+    }
     const typename Tile::Lane at =
         lane_at.in(stage_at + buf * Shape::kBufBytes + b0 * (32 / 4) * Tile::kGroup);
     const uint32_t stat = opaque(stage_at + buf * Shape::kBufBytes + 2 * Shape::kTileBytes +
@@ -561,10 +519,10 @@ attn_dkv_kernel(AttnArgs a) {
         }
         if (masked) {
           rare_path();
+          const int32_t at0 = i0 + 32 * b + 4 * half, from = lo - at0, to = sq.lq - at0;
 #pragma unroll
           for (int r = 0; r < 16; ++r) {
-            const int32_t i = i0 + 32 * b + block_row(r);
-            const bool sees = i >= lo && i < sq.lq;
+            const bool sees = block_row(r) >= from && block_row(r) < to;
             s[r] = sees ? s[r] : 0.f;
             dp[r] = sees ? dp[r] : 0.f;
           }
@@ -585,18 +543,25 @@ attn_dkv_kernel(AttnArgs a) {
     }
   }
 
+  if (left_out)
+    for (int head = kv * a.group; head < (kv + 1) * a.group; ++head)
+      Tile::template add_not_finite<false>(
+          static_cast<const T *>(a.go) + sq.q0 * a.go_row + head * a.go_head, a.go_row, a.dim,
+          wave_lo, min(wg_full + kBM, sq.lq), [&](int32_t i) { return i >= lo; }, dv);
   // Rows of the region behind the keys in use get zeros: where their lanes
   // share a wave with keys in use, those met them as a key of zeros, with a
   // probability of exp(-lse).
-  if (!key_ok) {
+  const int32_t my_key = wave0 + (opaque(lane_id()) & 31); // not kept through the loop
+  if (my_key >= sq.lk) {
 #pragma unroll
     for (int db = 0; db < Tile::kDBlocks; ++db)
       dk[db] = dv[db] = v16f{};
   }
   if constexpr (W == 4) {
     if (a.splits > 1) {
-      if (key < room) {
-        const int64_t place = ((split * static_cast<int64_t>(a.n_k) + gk) * a.kv_heads + kv) * a.dim;
+      if (my_key < room) {
+        const int64_t place =
+            ((split * static_cast<int64_t>(a.n_k) + sq.k0 + my_key) * a.kv_heads + kv) * a.dim;
         using Sum = AttnTile<float, DP>;
         if (a.dim % 4 == 0) {
           Sum::template store_column<true>(a.part_k + place, a.dim, 1.f, dk);
@@ -608,26 +573,11 @@ attn_dkv_kernel(AttnArgs a) {
       }
       return;
     }
-    bool bad = false;
-    if (a.causal && key_ok) {
-#pragma unroll
-      for (int db = 0; db < Tile::kDBlocks; ++db)
-#pragma unroll
-        for (int r = 0; r < 16; ++r)
-          bad |= !isfinite(dk[db][r]) || !isfinite(dv[db][r]);
-    }
-    uint64_t redo = __ballot(bad);
-    redo = (redo | redo >> 32) & 0xffffffffull;
-    if (key < room && !((redo >> (lane & 31)) & 1)) {
-      const int64_t place = (gk * a.kv_heads + kv) * a.dim;
+    if (my_key < room) {
+      const int64_t place =
+          ((sq.k0 + static_cast<int64_t>(my_key)) * a.kv_heads + kv) * a.dim;
       Tile::template store_column<VEC>(static_cast<T *>(a.gk) + place, a.dim, a.scale, dk);
       Tile::template store_column<VEC>(static_cast<T *>(a.gv) + place, a.dim, 1.f, dv);
-    }
-    while (redo) {
-      const int i = __ffsll(static_cast<unsigned long long>(redo)) - 1;
-      redo &= redo - 1;
-      float nk[2] = {NAN, NAN}, nv[2] = {NAN, NAN};
-      finish_dkv<T>(a, sq, wave0 + i, kv, nk, nv);
     }
   } else {
     // add the waves' sums, dk then dv through the same LDS; a wave ends with
@@ -653,7 +603,7 @@ attn_dkv_kernel(AttnArgs a) {
       if (j >= room)
         break;
       if (a.splits == 1) {
-        finish_dkv<T>(a, sq, j, kv, rk[u], rv[u]);
+        finish_dkv<T>(a, sq.k0 + static_cast<int64_t>(j), kv, rk[u], rv[u]);
       } else {
         const int64_t place =
             ((split * static_cast<int64_t>(a.n_k) + sq.k0 + j) * a.kv_heads + kv) * a.dim;
@@ -672,7 +622,6 @@ __global__ __launch_bounds__(kBwdThreads) void attn_dkv_join_kernel(AttnArgs a) 
   if (at >= rows)
     return;
   const int lane = lane_id();
-  const int32_t key = static_cast<int32_t>(at / a.kv_heads);
   float gk[2] = {0.f, 0.f}, gv[2] = {0.f, 0.f};
 #pragma unroll 4
   for (int s = 0; s < a.splits; ++s) {
@@ -684,8 +633,7 @@ __global__ __launch_bounds__(kBwdThreads) void attn_dkv_join_kernel(AttnArgs a) 
         gv[u] += a.part_v[p + lane + u * kWave];
       }
   }
-  const AttnSeq sq = key_row(a, key);
-  finish_dkv<T>(a, sq, key - sq.k0, static_cast<int>(at % a.kv_heads), gk, gv);
+  finish_dkv<T>(a, at / a.kv_heads, static_cast<int>(at % a.kv_heads), gk, gv);
 }
 
 struct BwdPlan {

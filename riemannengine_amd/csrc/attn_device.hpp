@@ -47,6 +47,18 @@ struct AttnSeq {
   int32_t q0, lq, k0, lk;
 };
 
+// A value that all lanes share, in a scalar register whatever the compiler can
+// prove: as vector registers the loops' bounds alone would cost a dozen.
+__device__ __forceinline__ int32_t wave_uniform(int32_t v) {
+  return __builtin_amdgcn_readfirstlane(v);
+}
+__device__ __forceinline__ AttnSeq wave_uniform(AttnSeq q) {
+  q.s = wave_uniform(q.s), q.tile = wave_uniform(q.tile);
+  q.q0 = wave_uniform(q.q0), q.lq = wave_uniform(q.lq);
+  q.k0 = wave_uniform(q.k0), q.lk = wave_uniform(q.lk);
+  return q;
+}
+
 __device__ __forceinline__ int32_t clamp_off(int32_t v, int32_t lo, int32_t hi) {
   return v < lo ? lo : (v > hi ? hi : v);
 }
@@ -92,25 +104,7 @@ __device__ __forceinline__ AttnSeq query_tile(const AttnArgs &a, int bm, int mul
   AttnSeq q;
   find_tile(a.q_off, a.n_seq, a.n_q, bm, mul, t, q.s, q.tile, q.q0, q.lq);
   key_range(a, q);
-  return q;
-}
-
-// The sequence of one query row.
-__device__ __forceinline__ AttnSeq query_row(const AttnArgs &a, int32_t row) {
-  AttnSeq q;
-  int lo = 0, hi = a.n_seq; // largest s with off[s] <= row (empty ones before it)
-  while (lo < hi) {
-    const int mid = (lo + hi + 1) >> 1;
-    if (clamp_off(a.q_off[mid], 0, a.n_q) <= row)
-      lo = mid;
-    else
-      hi = mid - 1;
-  }
-  q.s = lo, q.tile = 0;
-  q.q0 = lo == 0 ? 0 : clamp_off(a.q_off[lo], 0, a.n_q);
-  q.lq = (lo == a.n_seq ? a.n_q : clamp_off(a.q_off[lo + 1], q.q0, a.n_q)) - q.q0;
-  key_range(a, q);
-  return q;
+  return wave_uniform(q);
 }
 
 // The keys in use and the query rows of q.s, whose region holds `room` keys.
@@ -129,25 +123,8 @@ __device__ __forceinline__ AttnSeq key_tile(const AttnArgs &a, int bm, int32_t t
   AttnSeq q;
   find_tile(a.k_off, a.n_seq, a.n_k, bm, 1, t, q.s, q.tile, q.k0, room);
   query_range(a, q, room);
-  return q;
-}
-
-// The sequence of one key row; lk as in key_tile.
-__device__ __forceinline__ AttnSeq key_row(const AttnArgs &a, int32_t row) {
-  int lo = 0, hi = a.n_seq;
-  while (lo < hi) {
-    const int mid = (lo + hi + 1) >> 1;
-    if (clamp_off(a.k_off[mid], 0, a.n_k) <= row)
-      lo = mid;
-    else
-      hi = mid - 1;
-  }
-  AttnSeq q;
-  q.s = lo, q.tile = 0;
-  q.k0 = lo == 0 ? 0 : clamp_off(a.k_off[lo], 0, a.n_k);
-  const int32_t room = (lo == a.n_seq ? a.n_k : clamp_off(a.k_off[lo + 1], q.k0, a.n_k)) - q.k0;
-  query_range(a, q, room);
-  return q;
+  room = wave_uniform(room);
+  return wave_uniform(q);
 }
 
 // Workgroup -> (tile, key head, split) of a launch over tiles x key heads x
@@ -350,6 +327,113 @@ template <typename T, int DP> struct AttnTile {
       col_step(col_operand(at, bytes, row0, i), i, b, acc);
   }
 
+  // Zeroes what is not finite in the ROWS rows of the LDS tile at `tile`: the
+  // values, or with WHOLE the rows that hold one. WAVES waves share the rows;
+  // returns whether this one (`wave`) found any.
+  template <bool WHOLE, int ROWS, int WAVES>
+  __device__ static __forceinline__ bool zero_not_finite(uint32_t tile, int wave) {
+    constexpr int P = C <= 4 ? 4 : C <= 8 ? 8 : C <= 16 ? 16 : 32; // lanes to a row
+    constexpr int kTurn = kWave / P;                              // rows of a turn
+    static_assert(ROWS % (kTurn * WAVES) == 0, "every lane takes part in every turn");
+    const int lane = opaque(lane_id()); // nothing of this is kept in registers meanwhile
+    const int c = lane % P, r0 = wave * kTurn + lane / P;
+    auto address = [&](int r) {
+      return tile + (r >> 2) * kGroup + (c >> 2) * 256 + (r & 3) * 64 +
+             ((c & 3) ^ ((r >> 2) & 3)) * 16;
+    };
+    if (!__any(c < C && holds_not_finite<ROWS / (kTurn * WAVES), WAVES * kTurn>(r0, address)))
+      return false;
+    rare_path();
+    constexpr uint32_t kLow = sizeof(T) == 2 ? 0x7f80u : 0x7f800000u, kHigh = 0x7f800000u;
+    constexpr uint32_t kKeepHigh = sizeof(T) == 2 ? 0xffff0000u : 0u;
+    constexpr uint32_t kKeepLow = sizeof(T) == 2 ? 0x0000ffffu : 0u;
+#pragma unroll 1
+    for (int r = r0; r < ROWS; r += WAVES * kTurn) {
+      v4u u{0u, 0u, 0u, 0u}, clean;
+      if (c < C)
+        u = lds_read<v4u>(address(r));
+      bool bad = false;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) { // an exponent of ones
+        clean[e] = (u[e] & kLow) == kLow ? u[e] & kKeepHigh : u[e];
+        clean[e] = (u[e] & kHigh) == kHigh ? clean[e] & kKeepLow : clean[e];
+        bad |= clean[e] != u[e];
+      }
+      if constexpr (WHOLE) {
+        const uint64_t row = __ballot(bad) >> (lane / P * P);
+        bad = (row & ((uint64_t(1) << P) - 1)) != 0u;
+        clean = v4u{0u, 0u, 0u, 0u};
+      }
+      if (bad && c < C)
+        *reinterpret_cast<__attribute__((address_space(3))) v4u *>(address(r)) = clean;
+    }
+    return true;
+  }
+  // Whether the chunks at address(r), r = r0, r0 + STEP .. (N of them), hold a
+  // value that is not finite.
+  template <int N, int STEP, typename A>
+  __device__ static __forceinline__ bool holds_not_finite(int r0, A &&address) {
+    if constexpr (sizeof(T) == 2) {
+      typedef uint16_t v2us __attribute__((ext_vector_type(2)));
+      v2us top{};
+#pragma unroll 4
+      for (int i = 0; i < N; ++i) {
+        const v4u u = lds_read<v4u>(address(r0 + i * STEP));
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          top = __builtin_elementwise_max(top, __builtin_bit_cast(v2us, u[e] & 0x7fff7fffu));
+      }
+      return top[0] >= 0x7f80 || top[1] >= 0x7f80;
+    } else {
+      uint32_t top = 0;
+#pragma unroll 4
+      for (int i = 0; i < N; ++i) {
+        const v4u u = lds_read<v4u>(address(r0 + i * STEP));
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          top = max(top, u[e] & 0x7fffffffu);
+      }
+      return top >= 0x7f800000u;
+    }
+  }
+
+  // Adds what zero_not_finite took off rows r0 .. r1 - 1 at p to the columns
+  // whose lanes say sees(row): infinities and NaN as they are (an entry that a
+  // column sees has a weight above zero in out and grad_v), or NaN.
+  template <bool AS_NAN, typename S>
+  __device__ static void add_not_finite(const T *p, int64_t stride, int dim, int32_t r0,
+                                        int32_t r1, S &&sees, v16f (&acc)[kDBlocks]) {
+    const int lane = lane_id(), half = lane >> 5;
+#pragma unroll 1
+    for (int32_t r = r0; r < r1; ++r) {
+      const T *row = p + r * stride;
+      const float x[2] = {lane < dim ? to_f32(row[lane]) : 0.f,
+                          lane + kWave < dim ? to_f32(row[lane + kWave]) : 0.f};
+      const uint64_t bad[2] = {__ballot(!isfinite(x[0])), __ballot(!isfinite(x[1]))};
+      if (!(bad[0] | bad[1]))
+        continue;
+      const uint64_t none[2] = {__ballot(isnan(x[0])), __ballot(isnan(x[1]))};
+      const uint64_t negative[2] = {__ballot(x[0] < 0.f), __ballot(x[1] < 0.f)};
+      if (!sees(r))
+        continue;
+#pragma unroll
+      for (int db = 0; db < kDBlocks; ++db) {
+        // the row's elements 32 db + 4 half .. as bits from 0 on
+        auto bits = [&](const uint64_t (&m)[2]) {
+          return static_cast<uint32_t>(m[db / 2] >> (32 * (db % 2))) >> (4 * half);
+        };
+        const uint32_t b = bits(bad), n = AS_NAN ? b : bits(none), s = bits(negative);
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+          const uint32_t d = 1u << (8 * (e >> 2) + (e & 3));
+          const float v = n & d ? NAN : s & d ? -INFINITY : INFINITY;
+          acc[db][e] += b & d ? v : 0.f;
+          __builtin_amdgcn_sched_barrier(0); // registers, not speed
+        }
+      }
+    }
+  }
+
   // One lane's column of a [32 DB x 32] result, scaled, as a row of dim
   // elements at p; store_rest: what its rounding left over.
   template <bool VEC>
@@ -465,10 +549,11 @@ template <typename T, int DP, int ROWS, int THREADS, bool VEC> struct TileStream
       const __amdgpu_buffer_rsrc_t rsrc = wave_rsrc(base, bytes);
       const uint32_t to = lds_address(lds) + lds_address_of_wave(t);
       const uint32_t step = static_cast<uint32_t>(row_stride * sizeof(T)); // a row's bytes
+      const uint32_t first = opaque(off[0]); // one register, not one for each step
 #pragma unroll
       for (int i = 0; i < kPer; ++i)
         dma16(rsrc, to + i * THREADS * 16,
-              kStep ? off[0] + i * (THREADS / Tile::C) * step : off[i % kOffs]);
+              kStep ? first + i * (THREADS / Tile::C) * step : off[i % kOffs]);
     } else {
 #pragma unroll
       for (int i = 0; i < kPer; ++i) {
@@ -520,10 +605,8 @@ __device__ __forceinline__ void ahead(L &&load, U &&use) {
   ahead<N, A>(load, use, [] {});
 }
 
-// Row r of a lane's 16 entries of a 32x32 block.
-__device__ __forceinline__ int block_row(int r) {
-  return 8 * (r >> 2) + 4 * (lane_id() >> 5) + (r & 3);
-}
+// Entry r of a lane's 16 of a 32x32 block is row block_row(r) + 4 (lane / 32).
+constexpr int block_row(int r) { return 8 * (r >> 2) + (r & 3); }
 
 // Maximum and sum over the lane pair l, l ^ 32 (a column's two halves).
 __device__ __forceinline__ float pair_max(float v) {

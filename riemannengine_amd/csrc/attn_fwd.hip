@@ -52,60 +52,12 @@ template <typename T, int DP, int W> struct FwdShape {
   static constexpr int kOccupancy = kSlim && kLds <= 80 * 1024 ? 2 : 1;
 };
 
-// One row by its definition, for rows whose sums came out not finite under a
-// causal mask: there a product with a masked key's probability 0 and a value
-// that is not finite is not 0. Only keys the row sees are read. All 64 lanes
-// of the wave work on the row; lane l returns elements l and l + 64.
-template <typename T>
-__device__ void exact_row(const T *q, const T *k, int64_t k_row, const T *v, int64_t v_row,
-                          int32_t lim, int32_t dim, float c, float &o0, float &o1, float &m,
-                          float &sum) {
-  const int lane = lane_id();
-  auto score = [&](int32_t j) {
-    float s = 0.f;
-    for (int d = 0; d < dim; ++d)
-      s += to_f32(q[d]) * to_f32(k[j * k_row + d]);
-    return s;
-  };
-  m = -INFINITY;
-  for (int32_t j = lane; j < lim; j += kWave)
-    m = fmaxf(m, score(j));
-  for (int off = 32; off; off >>= 1)
-    m = fmaxf(m, __shfl_xor(m, off, kWave));
-  const float base = (m == -INFINITY ? 0.f : m) * c;
-  o0 = o1 = sum = 0.f;
-  for (int32_t j0 = 0; j0 < lim; j0 += kWave) {
-    const float p = j0 + lane < lim ? exp2_fast(score(j0 + lane) * c - base) : 0.f;
-    sum += p;
-    const int cnt = min(kWave, lim - j0);
-    for (int e = 0; e < cnt; ++e) {
-      const float pe = __shfl(p, e, kWave);
-      const T *row = v + (j0 + e) * v_row;
-      if (lane < dim)
-        o0 += pe * to_f32(row[lane]);
-      if (lane + kWave < dim)
-        o1 += pe * to_f32(row[lane + kWave]);
-    }
-  }
-  for (int off = 32; off; off >>= 1)
-    sum += __shfl_xor(sum, off, kWave);
-}
-
 // A row's result from one wave: lane l holds elements l and l + 64 of the
-// unnormalised sum. `at`: the row's place in out, [n_q, heads].
+// unnormalised sum.
 template <typename T>
-__device__ void finish_row(const AttnArgs &a, const AttnSeq &sq, int32_t i, int32_t head,
-                           float o0, float o1, float m, float sum) {
+__device__ void finish_row(const AttnArgs &a, int64_t row, int32_t head, float o0, float o1,
+                           float m, float sum) {
   const int lane = lane_id();
-  const int64_t row = sq.q0 + static_cast<int64_t>(i);
-  if (a.causal && __any(!isfinite(o0) || !isfinite(o1) || !isfinite(sum))) {
-    const int kv = head / a.group;
-    const int64_t lim = min<int64_t>(sq.lk, i + static_cast<int64_t>(sq.lk) - sq.lq + 1);
-    exact_row<T>(static_cast<const T *>(a.q) + row * a.q_row + head * a.q_head,
-                 static_cast<const T *>(a.k) + sq.k0 * a.k_row + kv * a.k_head, a.k_row,
-                 static_cast<const T *>(a.v) + sq.k0 * a.v_row + kv * a.v_head, a.v_row,
-                 static_cast<int32_t>(max<int64_t>(lim, 0)), a.dim, a.c, o0, o1, m, sum);
-  }
   const float inv = sum == 0.f ? 0.f : 1.f / sum;
   const int64_t at = (row * a.heads + head) * a.dim;
   auto put = [&](int d, float v) {
@@ -147,6 +99,7 @@ attn_fwd_kernel(AttnArgs a) {
   constexpr int kB = kBN / 32 / (W == 2 ? 2 : 1); // blocks of a tile that are a wave's
   using Stream = TileStream<T, DP, kBN, W == 1 ? kWave : kFwdThreads, VEC>;
   __shared__ alignas(16) char lds[Shape::kLds];
+  __shared__ int any_left_out; // of the workgroup
 
   int32_t t, kv, split;
   if (!attn_item(a, t, kv, split))
@@ -172,9 +125,11 @@ attn_fwd_kernel(AttnArgs a) {
     return static_cast<int32_t>(n < 0 ? 0 : n);
   };
   const int32_t lim = row_ok ? sees(row) : 0;
-  const int32_t wg_lim = sees(min(row0 + Shape::kRows, n_rows) - 1);
-  const int32_t wave_lim = wave0 < n_rows ? sees(min(wave0 + 32, n_rows) - 1) : 0;
-  const int32_t wave_full = wave0 < n_rows ? sees(wave0) : 0; // seen by all its rows
+  const int32_t wg_lim = wave_uniform(sees(min(row0 + Shape::kRows, n_rows) - 1));
+  const int32_t wg_full = wave_uniform(sees(row0)); // seen by all its rows
+  const int32_t wave_lim =
+      wave_uniform(wave0 < n_rows ? sees(min(wave0 + 32, n_rows) - 1) : 0);
+  const int32_t wave_full = wave_uniform(wave0 < n_rows ? sees(wave0) : 0);
   // this workgroup's tiles [kt0, kt1) of keys; a wave's first and step
   int32_t kt0 = 0, kt1 = (wg_lim + kBN - 1) / kBN;
   if (W == 1 && a.splits > 1) {
@@ -212,6 +167,12 @@ attn_fwd_kernel(AttnArgs a) {
   for (int db = 0; db < Tile::kDBlocks; ++db)
     o[db] = v16f{};
   float m = -INFINITY, sum = 0.f; // of this lane's row; sum over its half of the keys
+  // Values that are not finite, in tiles of which some rows see a part: a masked
+  // entry's zero times one would be NaN, so they are zeroed in LDS, and the rows
+  // that see them get them at the end.
+  bool left_out = false;
+  if (W > 1 && threadIdx.x == 0)
+    any_left_out = 0; // behind the barrier of the first turn
 
   const typename Tile::Lane lane_at = Tile::lane_addresses();
   const uint32_t stage_at = lds_address(stage);
@@ -222,7 +183,21 @@ attn_fwd_kernel(AttnArgs a) {
     wait_stream();
     if constexpr (W > 1)
       __syncthreads();
-    const typename Tile::Lane at = lane_at.in(stage_at + buf * 2 * Shape::kTileBytes + b0 * (32 / 4) * Tile::kGroup);
+    if (wg_full < wg_lim && (kt + 1) * kBN > wg_full) {
+      rare_path();
+      const bool found = Tile::template zero_not_finite<false, kBN, W == 1 ? 1 : kFwdWaves>(
+          stage_at + buf * 2 * Shape::kTileBytes + Shape::kTileBytes, W == 1 ? 0 : w);
+      if constexpr (W > 1) {
+        if (found)
+          any_left_out = 1;
+        __syncthreads();
+        left_out = wave_uniform(any_left_out) != 0;
+      } else {
+        left_out |= found;
+      }
+    }
+    const typename Tile::Lane at =
+        lane_at.in(stage_at + buf * 2 * Shape::kTileBytes + b0 * (32 / 4) * Tile::kGroup);
     if (Shape::kBuffers == 2 && kt + step < kt1)
       issue(kt + step, buf ^ 1);
     const int32_t j0 = kt * kBN + 32 * b0;
@@ -238,10 +213,12 @@ attn_fwd_kernel(AttnArgs a) {
       if (j0 + 32 * kB > wave_full) {
         rare_path();
 #pragma unroll
-        for (int b = 0; b < kB; ++b)
+        for (int b = 0; b < kB; ++b) {
+          const int32_t seen = lim - j0 - 32 * b - 4 * half; // of the lane's rows of the block
 #pragma unroll
           for (int r = 0; r < 16; ++r)
-            s[b][r] = j0 + 32 * b + block_row(r) < lim ? s[b][r] : -INFINITY;
+            s[b][r] = block_row(r) < seen ? s[b][r] : -INFINITY;
+        }
       }
       float top = m;
 #pragma unroll
@@ -281,33 +258,20 @@ attn_fwd_kernel(AttnArgs a) {
     }
   }
   sum = pair_sum(sum);
+  if (left_out)
+    Tile::template add_not_finite<false>(vp, a.v_row, a.dim, max(wg_full - kBN, 0), wave_lim,
+                                         [&](int32_t j) { return j < lim; }, o);
 
   if constexpr (W == 4) {
     const float inv = sum == 0.f ? 0.f : 1.f / sum;
-    bool bad = false;
-    if (a.causal) {
-#pragma unroll
-      for (int db = 0; db < Tile::kDBlocks; ++db)
-#pragma unroll
-        for (int r = 0; r < 16; ++r)
-          bad |= !isfinite(o[db][r]);
-      bad = (bad || !isfinite(sum)) && row_ok;
-    }
-    uint64_t redo = __ballot(bad);
-    redo = (redo | redo >> 32) & 0xffffffffull;
     const int64_t place = (sq.q0 + static_cast<int64_t>(qi)) * a.heads + head;
-    if (row_ok && !((redo >> (lane & 31)) & 1)) {
+    if (row_ok) {
       Tile::template store_column<VEC>(static_cast<T *>(a.o) + place * a.dim, a.dim, inv, o);
       if (sizeof(T) == 2 && a.rest)
         Tile::template store_rest<VEC>(static_cast<T *>(a.rest) + place * a.dim, a.dim, inv, o);
       if (a.lse && half == 0)
         a.lse[static_cast<int64_t>(head) * a.n_q + sq.q0 + qi] =
             sum == 0.f ? -INFINITY : m * a.scale + logf(sum);
-    }
-    while (redo) {
-      const int i = __ffsll(static_cast<unsigned long long>(redo)) - 1;
-      redo &= redo - 1;
-      finish_row<T>(a, sq, __shfl(qi, i, kWave), __shfl(head, i, kWave), NAN, NAN, 0.f, 0.f);
     }
   } else {
     // join the waves: [wave][row][DP] sums, then each row's maximum and sum
@@ -348,7 +312,7 @@ attn_fwd_kernel(AttnArgs a) {
       const int32_t i = (row0 + r) / a.group;
       const int h = kv * a.group + (row0 + r) % a.group;
       if (a.splits == 1) {
-        finish_row<T>(a, sq, i, h, o0, o1, mr, sr);
+        finish_row<T>(a, sq.q0 + static_cast<int64_t>(i), h, o0, o1, mr, sr);
       } else {
         const int64_t place = split * static_cast<int64_t>(a.n_q) * a.heads +
                            (sq.q0 + static_cast<int64_t>(i)) * a.heads + h;
@@ -406,9 +370,7 @@ __global__ __launch_bounds__(kFwdThreads) void attn_join_kernel(AttnArgs a) {
     o1 += sums[i][lane].y;
     sr += totals[i];
   }
-  // the row's sequence, for rows that have to be computed again
-  const AttnSeq sq = query_row(a, row);
-  finish_row<T>(a, sq, row - sq.q0, head, o0, o1, mr, sr);
+  finish_row<T>(a, row, head, o0, o1, mr, sr);
 }
 
 struct FwdPlan {
