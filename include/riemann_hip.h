@@ -739,6 +739,23 @@ typedef struct rhip_attn {
   float scale;
 } rhip_attn;
 
+/* The kernels of the two passes: rhip_attn_forward's, and the backward's over
+ * query rows (grad_q) and over keys (grad_k, grad_v). */
+typedef enum rhip_attn_pass {
+  RHIP_ATTN_FORWARD = 0,
+  RHIP_ATTN_QUERIES = 1,
+  RHIP_ATTN_KEYS = 2
+} rhip_attn_pass;
+
+/*
+ * The launch that a call with this descriptor's sizes makes: 32-row blocks of
+ * query rows (keys) per workgroup, 1, 2 or 4, and into how many parts the
+ * other side is split over workgroups (1: no split; parts keep fp32 partial
+ * sums in the workspace). Offsets, lengths and strides are not looked at. Host
+ * only, for tests and tools.
+ */
+int rhip_attn_plan(const rhip_attn *attn, int32_t pass, int32_t *blocks, int32_t *splits);
+
 /* Workspace bytes of rhip_attn_forward (backward = 0) or rhip_attn_backward. */
 int rhip_attn_workspace_bytes(const rhip_attn *attn, int32_t backward,
                               size_t *bytes);

@@ -49,7 +49,7 @@ EXPORTS = (
     "rhip_global_pool_forward", "rhip_global_pool_backward",
     "rhip_bn_workspace_bytes", "rhip_bn_stats", "rhip_bn_invstd", "rhip_bn_forward",
     "rhip_bn_backward",
-    "rhip_attn_workspace_bytes", "rhip_attn_forward", "rhip_attn_backward",
+    "rhip_attn_plan", "rhip_attn_workspace_bytes", "rhip_attn_forward", "rhip_attn_backward",
     "rhip_ln_workspace_bytes", "rhip_ln_forward", "rhip_ln_backward",
     "rhip_embed_forward", "rhip_embed_workspace_bytes", "rhip_embed_backward",
 )
@@ -168,6 +168,7 @@ def _declare(lib):
                                            _i32, _vp]),
         "rhip_bn_backward": (ctypes.c_int, [_vp, _vp, _vp, _i64, _i32, _vp, _vp, _vp, _i32,
                                             _i32, _vp, _vp, _vp, _vp, _i32, _vp, _sz, _vp]),
+        "rhip_attn_plan": (ctypes.c_int, [_P(RhipAttn), _i32, _P(_i32), _P(_i32)]),
         "rhip_attn_workspace_bytes": (ctypes.c_int, [_P(RhipAttn), _i32, _P(_sz)]),
         "rhip_attn_forward": (ctypes.c_int, [_P(RhipAttn), _vp, _vp, _vp, _vp, _vp, _vp, _vp,
                                              _sz, _vp]),
@@ -1017,6 +1018,21 @@ def _attn_desc(q, k, v, q_offsets, k_offsets, k_lengths, causal, scale) -> RhipA
                     None if k_lengths is None else k_lengths.data_ptr(), n_seq, q.shape[1],
                     k.shape[1], q.shape[2], int(causal), _dtype_code(q.dtype),
                     q.shape[2] ** -0.5 if scale is None else scale)
+
+
+ATTN_PASSES = ("forward", "queries", "keys")
+
+
+def attn_plan(which: str, dtype: torch.dtype, n_q: int, n_k: int, n_seq: int, heads: int,
+              kv_heads: int, dim: int, causal: bool):
+    """(32-row blocks per workgroup, splits) of an attention pass ("forward",
+    "queries": grad_q, "keys": grad_k and grad_v), from rhip_attn_plan."""
+    desc = RhipAttn(n_q=n_q, n_k=n_k, n_seq=n_seq, heads=heads, kv_heads=kv_heads, dim=dim,
+                    causal=int(causal), dtype=_dtype_code(dtype), scale=dim ** -0.5)
+    blocks, splits = _i32(0), _i32(0)
+    _check(lib().rhip_attn_plan(ctypes.byref(desc), ATTN_PASSES.index(which),
+                                ctypes.byref(blocks), ctypes.byref(splits)), "rhip_attn_plan")
+    return blocks.value, splits.value
 
 
 def _attn_ws(desc: RhipAttn, backward: bool, device) -> torch.Tensor:

@@ -10,7 +10,7 @@ using namespace rhip;
 
 namespace {
 
-void check_attn(const rhip_attn *a) {
+void check_attn_sizes(const rhip_attn *a) {
   RHIP_CHECK_ARG(a != nullptr, "descriptor is null");
   if (a->dtype != RHIP_F32 && a->dtype != RHIP_BF16)
     throw Error(RHIP_ERR_UNSUPPORTED, "dtype must be RHIP_F32 or RHIP_BF16");
@@ -25,6 +25,9 @@ void check_attn(const rhip_attn *a) {
   if (a->dim > kAttnMaxDim)
     throw Error(RHIP_ERR_UNSUPPORTED, "head width must not exceed 128");
   RHIP_CHECK_ARG(std::isfinite(a->scale) && a->scale > 0.f, "scale must be positive and finite");
+}
+void check_attn(const rhip_attn *a) {
+  check_attn_sizes(a);
   RHIP_CHECK_ARG(a->n_seq == 0 || (a->q_offsets && a->k_offsets),
                  "sequence offsets are required");
 }
@@ -63,7 +66,7 @@ struct FwdWs {
 };
 FwdWs carve_forward(Carve &cv, const rhip_attn *a) {
   FwdWs w{};
-  const int32_t splits = attn_forward_splits(*a);
+  const int32_t splits = attn_forward_plan(*a).splits;
   if (splits > 1) {
     const size_t rows = static_cast<size_t>(splits) * a->n_q * a->heads;
     w.part_o = cv.take<float>(rows * a->dim);
@@ -79,7 +82,7 @@ struct BwdWs {
 BwdWs carve_backward(Carve &cv, const rhip_attn *a) {
   BwdWs w{};
   w.stat = cv.take<float2>(static_cast<size_t>(std::max<int64_t>(1, a->n_q)) * a->heads);
-  const int32_t splits = attn_backward_splits(*a);
+  const int32_t splits = attn_keys_plan(*a).splits;
   if (splits > 1) {
     const size_t n = static_cast<size_t>(splits) * a->n_k * a->kv_heads * a->dim;
     w.part_k = cv.take<float>(n);
@@ -101,6 +104,21 @@ extern "C" int rhip_attn_workspace_bytes(const rhip_attn *attn, int32_t backward
     else
       carve_forward(cv, attn);
     *bytes = cv.used + 256;
+  });
+}
+
+extern "C" int rhip_attn_plan(const rhip_attn *attn, int32_t pass, int32_t *blocks,
+                              int32_t *splits) {
+  return guarded([&] {
+    check_attn_sizes(attn);
+    RHIP_CHECK_ARG(blocks && splits, "blocks and splits are required");
+    RHIP_CHECK_ARG(pass >= RHIP_ATTN_FORWARD && pass <= RHIP_ATTN_KEYS,
+                   "pass must be one of RHIP_ATTN_");
+    const AttnPlan p = pass == RHIP_ATTN_FORWARD   ? attn_forward_plan(*attn)
+                       : pass == RHIP_ATTN_QUERIES ? attn_queries_plan(*attn)
+                                                   : attn_keys_plan(*attn);
+    *blocks = p.waves;
+    *splits = p.splits;
   });
 }
 

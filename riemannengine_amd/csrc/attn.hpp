@@ -11,10 +11,17 @@ namespace rhip {
 
 void attn_forward_run(const AttnArgs &a, int32_t dtype, bool vec, hipStream_t stream);
 void attn_backward_run(const AttnArgs &a, int32_t dtype, bool vec, hipStream_t stream);
-// Workgroups that share one tile of query rows (forward) or of keys
-// (backward): their partial sums are the workspace.
-int32_t attn_forward_splits(const rhip_attn &d);
-int32_t attn_backward_splits(const rhip_attn &d);
+// The shape of a pass's launch: 32-row blocks per workgroup (W), tiles of 32 W
+// rows, and the workgroups that share one tile of query rows (forward) or of
+// keys (backward), whose partial sums are the workspace.
+struct AttnPlan {
+  int32_t waves; // W
+  int64_t tiles;
+  int32_t splits;
+};
+AttnPlan attn_forward_plan(const rhip_attn &d);
+AttnPlan attn_queries_plan(const rhip_attn &d);
+AttnPlan attn_keys_plan(const rhip_attn &d);
 
 // 32-row blocks per workgroup of the kernels over query rows: as many as leave
 // two workgroups for each CU, or one with two blocks (bf16: a workgroup's own

@@ -636,13 +636,8 @@ __global__ __launch_bounds__(kBwdThreads) void attn_dkv_join_kernel(AttnArgs a) 
   finish_dkv<T>(a, at / a.kv_heads, static_cast<int>(at % a.kv_heads), gk, gv);
 }
 
-struct BwdPlan {
-  int32_t waves; // W
-  int64_t tiles;
-  int32_t splits;
-};
-BwdPlan plan_queries(int64_t rows, int32_t n_seq, int32_t kv_heads, int32_t dtype) {
-  BwdPlan p{attn_waves(rows, kv_heads, dtype), 0, 1};
+AttnPlan plan_queries(int64_t rows, int32_t n_seq, int32_t kv_heads, int32_t dtype) {
+  AttnPlan p{attn_waves(rows, kv_heads, dtype), 0, 1};
   p.tiles = rows / (32 * p.waves) + n_seq + 1;
   return p;
 }
@@ -659,15 +654,15 @@ BwdPlan plan_queries(int64_t rows, int32_t n_seq, int32_t kv_heads, int32_t dtyp
 // sums at 4.5 TB/s. (16 over 4 heads, 128 wide, four causal texts of 4096: 912
 // us with one split, 686 with three, joining included; 8 heads, eight of
 // 1024: 70 us with one, 113 with two.)
-BwdPlan plan_keys(int64_t n_q, int64_t n_k, int32_t n_seq, int32_t heads, int32_t kv_heads,
-                  int32_t dim, int32_t causal, int32_t dtype) {
+AttnPlan plan_keys(int64_t n_q, int64_t n_k, int32_t n_seq, int32_t heads, int32_t kv_heads,
+                   int32_t dim, int32_t causal, int32_t dtype) {
   const int64_t seqs = std::max<int64_t>(1, std::min<int64_t>(n_seq, n_k));
   const double rows = static_cast<double>(n_q) * (heads / kv_heads) / seqs; // per key
   const double block =
       1.14 * (dim <= 32 ? 0.25 : dim <= 64 ? 0.5 : dim <= 96 ? 0.8 : 1.0) * (dtype == RHIP_F32 ? 7.5 : 1.0);
   const double all = static_cast<double>(n_k) * kv_heads * rows * (causal ? 0.5 : 1.0) / 1024.0;
   const double traffic = static_cast<double>(n_k) * kv_heads * dim * 16 / 4.5e6;
-  BwdPlan best{};
+  AttnPlan best{};
   double least = 0.0;
   for (int32_t w = 4; w >= 1; w /= 2) {
     const double wgs = static_cast<double>(n_k / (32 * w) + seqs) * kv_heads;
@@ -697,15 +692,18 @@ unsigned bwd_grid(int64_t tiles, int64_t heads, int64_t splits) {
 
 } // namespace
 
-int32_t attn_backward_splits(const rhip_attn &d) {
-  return plan_keys(d.n_q, d.n_k, d.n_seq, d.heads, d.kv_heads, d.dim, d.causal, d.dtype).splits;
+AttnPlan attn_queries_plan(const rhip_attn &d) {
+  return plan_queries(d.n_q * (d.heads / d.kv_heads), d.n_seq, d.kv_heads, d.dtype);
+}
+AttnPlan attn_keys_plan(const rhip_attn &d) {
+  return plan_keys(d.n_q, d.n_k, d.n_seq, d.heads, d.kv_heads, d.dim, d.causal, d.dtype);
 }
 
 void attn_backward_run(const AttnArgs &args, int32_t dtype, bool vec, hipStream_t stream) {
-  const BwdPlan pq =
+  const AttnPlan pq =
       plan_queries(static_cast<int64_t>(args.n_q) * args.group, args.n_seq, args.kv_heads, dtype);
-  const BwdPlan pk = plan_keys(args.n_q, args.n_k, args.n_seq, args.heads, args.kv_heads,
-                               args.dim, args.causal, dtype);
+  const AttnPlan pk = plan_keys(args.n_q, args.n_k, args.n_seq, args.heads, args.kv_heads,
+                                args.dim, args.causal, dtype);
   const unsigned gq = bwd_grid(pq.tiles, args.kv_heads, 1);
   const unsigned gk = bwd_grid(pk.tiles, args.kv_heads, pk.splits);
   AttnArgs aq = args, ak = args;

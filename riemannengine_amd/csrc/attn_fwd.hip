@@ -373,11 +373,6 @@ __global__ __launch_bounds__(kFwdThreads) void attn_join_kernel(AttnArgs a) {
   finish_row<T>(a, row, head, o0, o1, mr, sr);
 }
 
-struct FwdPlan {
-  int32_t waves; // W
-  int64_t tiles;
-  int32_t splits;
-};
 // W by attn_waves; with W = 1 the splits by estimated time, in microseconds: a
 // round of workgroups (two per CU with narrow rows, one with wide) takes 8 to start
 // and finish and `tile` for every four 32-key tiles (one to a wave) of the mean
@@ -386,10 +381,10 @@ struct FwdPlan {
 // another 8. (32 tokens over caches of 1 to 16384 keys, 8 key heads, 128 wide:
 // four splits 172 us, one 390. Three causal sequences of 1000, 2 heads of 96:
 // one split 26 us, three 32 and 7 to join.)
-FwdPlan plan_forward(int64_t n_q, int64_t n_k, int32_t n_seq, int32_t heads, int32_t kv_heads,
-                     int32_t dim, int32_t causal, int32_t dtype) {
+AttnPlan plan_forward(int64_t n_q, int64_t n_k, int32_t n_seq, int32_t heads, int32_t kv_heads,
+                      int32_t dim, int32_t causal, int32_t dtype) {
   const int64_t rows = n_q * (heads / kv_heads);
-  FwdPlan p{attn_waves(rows, kv_heads, dtype), 0, 1};
+  AttnPlan p{attn_waves(rows, kv_heads, dtype), 0, 1};
   p.tiles = rows / (32 * p.waves) + n_seq + 1;
   if (p.waves > 1 || n_seq == 0)
     return p;
@@ -420,14 +415,14 @@ FwdPlan plan_forward(int64_t n_q, int64_t n_k, int32_t n_seq, int32_t heads, int
 
 } // namespace
 
-int32_t attn_forward_splits(const rhip_attn &d) {
-  return plan_forward(d.n_q, d.n_k, d.n_seq, d.heads, d.kv_heads, d.dim, d.causal, d.dtype).splits;
+AttnPlan attn_forward_plan(const rhip_attn &d) {
+  return plan_forward(d.n_q, d.n_k, d.n_seq, d.heads, d.kv_heads, d.dim, d.causal, d.dtype);
 }
 
 void attn_forward_run(const AttnArgs &args, int32_t dtype, bool vec, hipStream_t stream) {
   AttnArgs a = args;
-  const FwdPlan plan = plan_forward(a.n_q, a.n_k, a.n_seq, a.heads, a.kv_heads, a.dim,
-                                    a.causal, dtype);
+  const AttnPlan plan = plan_forward(a.n_q, a.n_k, a.n_seq, a.heads, a.kv_heads, a.dim,
+                                     a.causal, dtype);
   const int64_t grid = attn_grid(plan.tiles, a.kv_heads, plan.splits);
   if (grid > INT32_MAX)
     throw Error(RHIP_ERR_UNSUPPORTED, "too many query tiles for one launch");
