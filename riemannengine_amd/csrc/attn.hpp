@@ -3,6 +3,7 @@
 #pragma once
 
 #include <algorithm>
+#include <climits>
 #include <type_traits>
 
 #include "attn_device.hpp"
@@ -79,6 +80,27 @@ template <int W> unsigned spread_lds(const AttnArgs &a, int own) {
     return 0;
   const int fits = kLdsBytes / static_cast<int>(each + 1) + 1024; // each do, one more does not
   return fits > own ? static_cast<unsigned>(fits - own) : 0u;
+}
+
+// launch(args, workgroups) for a pass's tiles, in as many launches as their
+// workgroups need (a great many short sequences on several heads).
+template <typename F>
+void attn_launches(const AttnArgs &args, const AttnPlan &plan, int threads, F &&launch) {
+  AttnArgs a = args;
+  if (plan.tiles > INT32_MAX)
+    throw Error(RHIP_ERR_UNSUPPORTED, "too many tiles");
+  a.tiles = static_cast<int32_t>(plan.tiles), a.splits = plan.splits;
+  // attn_grid rounds up to whole rounds of the XCDs
+  const int64_t units = max_groups(threads) / a.kv_heads - kXcds;
+  if (units < a.splits)
+    throw Error(RHIP_ERR_UNSUPPORTED, "too many heads");
+  const int64_t step = units / a.splits;
+  for (int64_t t = 0; t < plan.tiles; t += step) {
+    a.tile0 = static_cast<int32_t>(t);
+    a.launched = static_cast<int32_t>(std::min(step, plan.tiles - t));
+    launch(a, static_cast<unsigned>(attn_grid(a.launched, a.kv_heads, a.splits)));
+    RHIP_LAUNCH_CHECK();
+  }
 }
 
 // f(W): 32-row blocks per workgroup, 4, 2 or 1.

@@ -618,22 +618,22 @@ attn_dkv_kernel(AttnArgs a) {
 template <typename T>
 __global__ __launch_bounds__(kBwdThreads) void attn_dkv_join_kernel(AttnArgs a) {
   const int64_t rows = static_cast<int64_t>(a.n_k) * a.kv_heads;
-  const int64_t at = static_cast<int64_t>(blockIdx.x) * kBwdWaves + threadIdx.x / kWave;
-  if (at >= rows)
-    return;
   const int lane = lane_id();
-  float gk[2] = {0.f, 0.f}, gv[2] = {0.f, 0.f};
+  for (int64_t at = static_cast<int64_t>(blockIdx.x) * kBwdWaves + threadIdx.x / kWave; at < rows;
+       at += static_cast<int64_t>(gridDim.x) * kBwdWaves) {
+    float gk[2] = {0.f, 0.f}, gv[2] = {0.f, 0.f};
 #pragma unroll 4
-  for (int s = 0; s < a.splits; ++s) {
-    const int64_t p = (s * rows + at) * a.dim;
+    for (int s = 0; s < a.splits; ++s) {
+      const int64_t p = (s * rows + at) * a.dim;
 #pragma unroll
-    for (int u = 0; u < 2; ++u)
-      if (lane + u * kWave < a.dim) {
-        gk[u] += a.part_k[p + lane + u * kWave];
-        gv[u] += a.part_v[p + lane + u * kWave];
-      }
+      for (int u = 0; u < 2; ++u)
+        if (lane + u * kWave < a.dim) {
+          gk[u] += a.part_k[p + lane + u * kWave];
+          gv[u] += a.part_v[p + lane + u * kWave];
+        }
+    }
+    finish_dkv<T>(a, at / a.kv_heads, static_cast<int>(at % a.kv_heads), gk, gv);
   }
-  finish_dkv<T>(a, at / a.kv_heads, static_cast<int>(at % a.kv_heads), gk, gv);
 }
 
 AttnPlan plan_queries(int64_t rows, int32_t n_seq, int32_t kv_heads, int32_t dtype) {
@@ -683,13 +683,6 @@ AttnPlan plan_keys(int64_t n_q, int64_t n_k, int32_t n_seq, int32_t heads, int32
   return best;
 }
 
-unsigned bwd_grid(int64_t tiles, int64_t heads, int64_t splits) {
-  const int64_t grid = attn_grid(tiles, heads, splits);
-  if (grid > INT32_MAX)
-    throw Error(RHIP_ERR_UNSUPPORTED, "too many tiles for one launch");
-  return static_cast<unsigned>(grid);
-}
-
 } // namespace
 
 AttnPlan attn_queries_plan(const rhip_attn &d) {
@@ -704,11 +697,6 @@ void attn_backward_run(const AttnArgs &args, int32_t dtype, bool vec, hipStream_
       plan_queries(static_cast<int64_t>(args.n_q) * args.group, args.n_seq, args.kv_heads, dtype);
   const AttnPlan pk = plan_keys(args.n_q, args.n_k, args.n_seq, args.heads, args.kv_heads,
                                 args.dim, args.causal, dtype);
-  const unsigned gq = bwd_grid(pq.tiles, args.kv_heads, 1);
-  const unsigned gk = bwd_grid(pk.tiles, args.kv_heads, pk.splits);
-  AttnArgs aq = args, ak = args;
-  aq.tiles = static_cast<int32_t>(pq.tiles), aq.splits = 1;
-  ak.tiles = static_cast<int32_t>(pk.tiles), ak.splits = pk.splits;
   with_attn(dtype, args.dim, vec, [&](auto t, auto dp, auto v) {
     using T = decltype(t);
     constexpr int DP = decltype(dp)::value;
@@ -717,22 +705,29 @@ void attn_backward_run(const AttnArgs &args, int32_t dtype, bool vec, hipStream_
     if (args.n_q > 0) {
       with_waves(pq.waves, [&](auto w) {
         constexpr int W = decltype(w)::value;
-        const unsigned spread = spread_lds<W>(aq, BwdShape<T, DP, W, false>::kLds);
-        hipLaunchKernelGGL((attn_dq_kernel<T, DP, VEC, W>), dim3(gq), b, spread, stream, aq);
+        const unsigned spread = spread_lds<W>(args, BwdShape<T, DP, W, false>::kLds);
+        attn_launches(args, pq, kBwdThreads, [&](const AttnArgs &part, unsigned groups) {
+          hipLaunchKernelGGL((attn_dq_kernel<T, DP, VEC, W>), dim3(groups), b, spread, stream,
+                             part);
+        });
       });
-      RHIP_LAUNCH_CHECK();
     }
     if (!args.gk || args.n_k == 0)
       return;
     with_waves(pk.waves, [&](auto w) {
-      hipLaunchKernelGGL((attn_dkv_kernel<T, DP, VEC, decltype(w)::value>), dim3(gk), b, 0,
-                         stream, ak);
+      attn_launches(args, pk, kBwdThreads, [&](const AttnArgs &part, unsigned groups) {
+        hipLaunchKernelGGL((attn_dkv_kernel<T, DP, VEC, decltype(w)::value>), dim3(groups), b, 0,
+                           stream, part);
+      });
     });
-    RHIP_LAUNCH_CHECK();
     if (pk.splits > 1) {
       const int64_t rows = static_cast<int64_t>(args.n_k) * args.kv_heads;
+      AttnArgs a = args;
+      a.splits = pk.splits;
       hipLaunchKernelGGL((attn_dkv_join_kernel<T>),
-                         dim3(static_cast<unsigned>(ceil_div(rows, kBwdWaves))), b, 0, stream, ak);
+                         dim3(static_cast<unsigned>(
+                             std::min(ceil_div(rows, kBwdWaves), max_groups(kBwdThreads)))),
+                         b, 0, stream, a);
       RHIP_LAUNCH_CHECK();
     }
   });

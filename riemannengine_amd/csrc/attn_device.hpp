@@ -30,7 +30,8 @@ struct AttnArgs {
   const int32_t *q_off, *k_off, *k_len;
   int64_t q_row, q_head, k_row, k_head, v_row, v_head, go_row, go_head;
   int32_t n_q, n_k, n_seq, heads, kv_heads, group, dim, causal;
-  int32_t tiles, splits; // of the launch
+  int32_t tiles, splits; // of the pass
+  int32_t tile0, launched; // the tiles of this launch: launched of them from tile0 on
   float scale, c;        // c = scale * log2(e)
   void *o, *rest;        // out, and bf16 out's rounding error (training)
   float *lse;            // [heads, n_q], natural logarithm
@@ -136,7 +137,7 @@ __device__ __forceinline__ AttnSeq key_tile(const AttnArgs &a, int bm, int32_t t
 __device__ __forceinline__ bool attn_item(const AttnArgs &a, int32_t &tile, int32_t &kv,
                                           int32_t &split) {
   const uint32_t x = blockIdx.x % kXcds, i = blockIdx.x / kXcds;
-  const uint32_t heads = a.kv_heads, units = static_cast<uint32_t>(a.tiles) * a.splits;
+  const uint32_t heads = a.kv_heads, units = static_cast<uint32_t>(a.launched) * a.splits;
   uint32_t unit;
   if (heads % kXcds == 0) {
     const uint32_t mine = heads / kXcds;
@@ -150,7 +151,7 @@ __device__ __forceinline__ bool attn_item(const AttnArgs &a, int32_t &tile, int3
     unit = blockIdx.x / heads;
     kv = blockIdx.x % heads;
   }
-  tile = unit / a.splits;
+  tile = a.tile0 + unit / a.splits;
   split = unit % a.splits;
   return unit < units;
 }

@@ -423,25 +423,22 @@ void attn_forward_run(const AttnArgs &args, int32_t dtype, bool vec, hipStream_t
   AttnArgs a = args;
   const AttnPlan plan = plan_forward(a.n_q, a.n_k, a.n_seq, a.heads, a.kv_heads, a.dim,
                                      a.causal, dtype);
-  const int64_t grid = attn_grid(plan.tiles, a.kv_heads, plan.splits);
-  if (grid > INT32_MAX)
-    throw Error(RHIP_ERR_UNSUPPORTED, "too many query tiles for one launch");
   const int64_t rows = static_cast<int64_t>(a.n_q) * a.heads;
-  if (plan.splits > 1 && rows > INT32_MAX)
-    throw Error(RHIP_ERR_UNSUPPORTED, "too many rows for one launch");
-  a.tiles = static_cast<int32_t>(plan.tiles), a.splits = plan.splits;
+  a.splits = plan.splits;
   with_attn(dtype, a.dim, vec, [&](auto t, auto dp, auto v) {
     using T = decltype(t);
     constexpr int DP = decltype(dp)::value;
     constexpr bool VEC = decltype(v)::value;
-    const dim3 g(static_cast<unsigned>(grid)), b(kFwdThreads);
+    const dim3 b(kFwdThreads);
     with_waves(plan.waves, [&](auto w) {
       constexpr int W = decltype(w)::value;
       const unsigned spread = spread_lds<W>(a, FwdShape<T, DP, W>::kLds);
-      hipLaunchKernelGGL((attn_fwd_kernel<T, DP, VEC, W>), g, b, spread, stream, a);
+      attn_launches(a, plan, kFwdThreads, [&](const AttnArgs &part, unsigned groups) {
+        hipLaunchKernelGGL((attn_fwd_kernel<T, DP, VEC, W>), dim3(groups), b, spread, stream,
+                           part);
+      });
     });
-    RHIP_LAUNCH_CHECK();
-    if (a.splits > 1) {
+    if (a.splits > 1) { // with W = 1, so rows for a few hundred workgroups at most
       hipLaunchKernelGGL((attn_join_kernel<T>),
                          dim3(static_cast<unsigned>(rows)), b, 0, stream, a);
       RHIP_LAUNCH_CHECK();

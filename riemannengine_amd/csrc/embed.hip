@@ -201,9 +201,9 @@ __global__ __launch_bounds__(kEmbThreads) void embed_backward_kernel(
     const T *__restrict__ gy, int64_t gy_row, const uint32_t *__restrict__ keys,
     const int32_t *__restrict__ pos, const int32_t *__restrict__ start, int64_t n, int64_t vocab,
     int C, int log_g, float scale, T *__restrict__ gw, float *__restrict__ part,
-    int32_t *__restrict__ runs) {
+    int32_t *__restrict__ runs, int64_t item0) {
   using R = RowChunk<T>;
-  const int64_t item = static_cast<int64_t>(blockIdx.x) * (kEmbThreads / kWave) +
+  const int64_t item = item0 + static_cast<int64_t>(blockIdx.x) * (kEmbThreads / kWave) +
                        __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
   const int lane = lane_id() & ((1 << log_g) - 1);
   const bool writer = (lane_id() >> log_g) == 0;
@@ -366,13 +366,18 @@ extern "C" int rhip_embed_forward(const void *ids, int32_t ids_int32, int64_t n,
       using T = decltype(t);
       const int chunks = static_cast<int>(ceil_div(C, RowChunk<T>::V));
       const int g = lanes_per_row(chunks);
-      hipLaunchKernelGGL((embed_forward_kernel<T>),
-                         dim3(static_cast<unsigned>(ceil_div(n, kEmbThreads / g)),
-                              static_cast<unsigned>(ceil_div(chunks, kWave))),
-                         dim3(kEmbThreads), 0, stream, ids, ids_int32, n,
-                         static_cast<const T *>(weight), weight_row, vocabulary, C, log2_of(g),
-                         scale, static_cast<T *>(y));
-      RHIP_LAUNCH_CHECK();
+      const int64_t most = max_groups(kEmbThreads) * (kEmbThreads / g);
+      for (int64_t i = 0; i < n; i += most) { // more rows than one launch takes
+        const int64_t rows = std::min(n - i, most);
+        hipLaunchKernelGGL((embed_forward_kernel<T>),
+                           dim3(static_cast<unsigned>(ceil_div(rows, kEmbThreads / g)),
+                                static_cast<unsigned>(ceil_div(chunks, kWave))),
+                           dim3(kEmbThreads), 0, stream,
+                           static_cast<const char *>(ids) + i * (ids_int32 ? 4 : 8), ids_int32,
+                           rows, static_cast<const T *>(weight), weight_row, vocabulary, C,
+                           log2_of(g), scale, static_cast<T *>(y) + i * C);
+        RHIP_LAUNCH_CHECK();
+      }
     });
   });
 }
@@ -430,15 +435,18 @@ extern "C" int rhip_embed_backward(const void *grad_y, int64_t grad_y_row, const
       const int64_t fill = 4096 / items; // column tiles that fill the chip
       auto launch = [&](auto nc) {
         constexpr int NC = decltype(nc)::value;
-        hipLaunchKernelGGL((embed_backward_kernel<T, NC>),
-                           dim3(static_cast<unsigned>(
-                                    ceil_div(items, kEmbThreads / kWave)),
-                                static_cast<unsigned>(ceil_div(chunks, kWave * NC))),
-                           dim3(kEmbThreads), 0, stream, static_cast<const T *>(grad_y),
-                           grad_y_row, w.sorted, w.order, w.start, n, vocabulary, C,
-                           log2_of(lanes_per_row(chunks)), scale,
-                           static_cast<T *>(grad_weight), w.part, w.runs);
-        RHIP_LAUNCH_CHECK();
+        const int64_t most = max_groups(kEmbThreads) * (kEmbThreads / kWave);
+        for (int64_t i = 0; i < items; i += most) {
+          hipLaunchKernelGGL((embed_backward_kernel<T, NC>),
+                             dim3(static_cast<unsigned>(ceil_div(std::min(items - i, most),
+                                                                 kEmbThreads / kWave)),
+                                  static_cast<unsigned>(ceil_div(chunks, kWave * NC))),
+                             dim3(kEmbThreads), 0, stream, static_cast<const T *>(grad_y),
+                             grad_y_row, w.sorted, w.order, w.start, n, vocabulary, C,
+                             log2_of(lanes_per_row(chunks)), scale,
+                             static_cast<T *>(grad_weight), w.part, w.runs, i);
+          RHIP_LAUNCH_CHECK();
+        }
       };
       if (chunks <= kWave || fill >= ceil_div(chunks, kWave))
         launch(std::integral_constant<int, 1>{});

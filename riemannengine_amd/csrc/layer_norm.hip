@@ -496,16 +496,22 @@ extern "C" int rhip_ln_forward(const void *x, int64_t x_row, int64_t n, int32_t 
       const T *xp = static_cast<const T *>(x);
       T *yp = static_cast<T *>(y);
       const float e = static_cast<float>(eps);
-      if constexpr (G == 0)
-        hipLaunchKernelGGL((ln_forward_wide_kernel<T>), dim3(static_cast<unsigned>(n)),
-                           dim3(kLnThreads), 0, stream, xp, x_row, n, C, weight, bias, e, yp,
-                           mean, rstd);
-      else
-        hipLaunchKernelGGL((ln_forward_kernel<T, G, NC, R>),
-                           dim3(static_cast<unsigned>(ceil_div(n, kLnThreads / G * R))),
-                           dim3(kLnThreads), 0, stream, xp, x_row, n, C, weight, bias, e, yp,
-                           mean, rstd);
-      RHIP_LAUNCH_CHECK();
+      constexpr int64_t kRows = G == 0 ? 1 : kLnThreads / (G == 0 ? 1 : G) * R; // of a workgroup
+      const int64_t most = max_groups(kLnThreads) * kRows;
+      for (int64_t r = 0; r < n; r += most) { // more rows than one launch takes: some narrow ones
+        const int64_t rows = std::min(n - r, most);
+        const dim3 g(static_cast<unsigned>(ceil_div(rows, kRows)));
+        const T *xr = xp + r * x_row;
+        T *yr = yp + r * C;
+        float *mr = mean ? mean + r : nullptr, *sr = rstd ? rstd + r : nullptr;
+        if constexpr (G == 0)
+          hipLaunchKernelGGL((ln_forward_wide_kernel<T>), g, dim3(kLnThreads), 0, stream, xr, x_row,
+                             rows, C, weight, bias, e, yr, mr, sr);
+        else
+          hipLaunchKernelGGL((ln_forward_kernel<T, G, NC, R>), g, dim3(kLnThreads), 0, stream, xr,
+                             x_row, rows, C, weight, bias, e, yr, mr, sr);
+        RHIP_LAUNCH_CHECK();
+      }
     });
   });
 }
@@ -535,10 +541,12 @@ extern "C" int rhip_ln_backward(const void *grad_y, int64_t grad_y_row, const vo
       const T *gp = static_cast<const T *>(grad_y), *xp = static_cast<const T *>(x);
       T *gxp = static_cast<T *>(grad_x);
       if constexpr (G == 0) {
-        if (gxp && n > 0) {
-          hipLaunchKernelGGL((ln_backward_wide_kernel<T>), dim3(static_cast<unsigned>(n)),
-                             dim3(kLnThreads), 0, stream, gp, grad_y_row, xp, x_row, C, mean,
-                             rstd, weight, gxp);
+        const int64_t most = max_groups(kLnThreads);
+        for (int64_t r = 0; gxp && r < n; r += most) {
+          hipLaunchKernelGGL((ln_backward_wide_kernel<T>),
+                             dim3(static_cast<unsigned>(std::min(n - r, most))), dim3(kLnThreads),
+                             0, stream, gp + r * grad_y_row, grad_y_row, xp + r * x_row, x_row, C,
+                             mean + r, rstd + r, weight, gxp + r * C);
           RHIP_LAUNCH_CHECK();
         }
         if (part) {

@@ -77,6 +77,9 @@ template <typename F> int guarded(F &&body) {
 }
 
 inline int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
+// Workgroups of `threads` threads that one launch takes along an axis: HIP keeps
+// the threads along it below 2^32.
+constexpr int64_t max_groups(int threads) { return ((int64_t(1) << 32) - 1) / threads; }
 inline size_t align_up(size_t v, size_t a) { return (v + a - 1) / a * a; }
 
 // Bump allocator over a caller workspace (256-byte aligned pieces).
