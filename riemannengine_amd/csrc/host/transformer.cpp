@@ -53,11 +53,13 @@ at::Tensor int_vector(const at::Tensor &t, const at::Device &dev, const char *wh
   return t.to(torch::kInt).contiguous();
 }
 
-bool wants_grad(std::initializer_list<at::Tensor> ts) {
-  if (!torch::GradMode::is_enabled())
-    return false;
+// Whether a call goes through its autograd function: an input is recorded, or
+// carries a forward-mode tangent (which the function refuses; without it the
+// result would lose the tangent).
+bool through_autograd(std::initializer_list<at::Tensor> ts) {
   for (const auto &t : ts)
-    if (t.defined() && t.requires_grad())
+    if (t.defined() && ((torch::GradMode::is_enabled() && t.requires_grad()) ||
+                        t._fw_grad(0).defined()))
       return true;
   return false;
 }
@@ -332,7 +334,7 @@ at::Tensor hip_packed_attention(const at::Tensor &query, const at::Tensor &key,
   }
   const double s = scale.value_or(1.0 / std::sqrt(static_cast<double>(query.size(2))));
   auto q = dense_last(query), k = dense_last(key), v = dense_last(value);
-  if (wants_grad({query, key, value}))
+  if (through_autograd({query, key, value}))
     return HipAttentionFunction::apply(q, k, v, qo, ko, or_empty(kl, qo), causal, s);
   return Attention{q, k, v, qo, ko, kl, causal, s}.forward(nullptr, nullptr);
 }
@@ -352,7 +354,7 @@ at::Tensor hip_layer_norm(const at::Tensor &input, const at::Tensor &weight,
   auto x = dense_last(input.dim() == 2 ? input : input.reshape({-1, C}));
   auto w = weight.defined() ? weight.contiguous() : weight;
   auto b = bias.defined() ? bias.contiguous() : bias;
-  auto y = wants_grad({input, weight, bias})
+  auto y = through_autograd({input, weight, bias})
                ? HipLayerNormFunction::apply(x, or_empty(w, x), or_empty(b, x), eps)
                : run_layer_norm(x, w, b, eps, nullptr, nullptr);
   return input.dim() == 2 ? y : y.reshape(input.sizes());
@@ -368,7 +370,7 @@ at::Tensor hip_embedding(const at::Tensor &ids, const at::Tensor &weight, double
   hip_dtype(weight, "embedding weight");
   auto flat = ids.reshape({-1}).contiguous();
   auto w = dense_last(weight);
-  auto y = wants_grad({weight}) ? HipEmbeddingFunction::apply(flat, w, scale)
+  auto y = through_autograd({weight}) ? HipEmbeddingFunction::apply(flat, w, scale)
                                 : run_embedding(flat, w, scale);
   if (ids.dim() == 1)
     return y;

@@ -1,0 +1,36 @@
+"""Inputs that the transformer functions cannot serve are refused, never
+answered in part."""
+import pytest
+import torch
+import torch.autograd.forward_ad as forward_ad
+
+import riemannengine as rie
+from helpers import DEV
+
+pytestmark = pytest.mark.gpu
+
+
+def test_forward_mode_tangents_are_refused():
+    """As by the convolutions: a result without its tangent would be wrong."""
+    nn = rie.nn
+    x = torch.randn(12, 4, 16, device=DEV)
+    rows = x.view(12, 64)
+    w, b = torch.ones(64, device=DEV), torch.zeros(64, device=DEV)
+    o = torch.tensor([0, 5, 12], dtype=torch.int32, device=DEV)
+    ids = torch.zeros(3, dtype=torch.int64, device=DEV)
+    with forward_ad.dual_level():
+        for leaf, call in [
+            (x, lambda t: nn.packed_attention(t, x, x, o)),
+            (x, lambda t: nn.packed_attention(x, t, x, o)),
+            (x, lambda t: nn.packed_attention(x, x, t, o, causal=True)),
+            (rows, lambda t: nn.layer_norm(t, w, b)),
+            (w, lambda t: nn.layer_norm(rows, t, b)),
+            (b, lambda t: nn.layer_norm(rows, w, t)),
+            (rows, lambda t: nn.embedding(ids, t)),
+        ]:
+            dual = forward_ad.make_dual(leaf, torch.ones_like(leaf))
+            for grad in (True, False):
+                with torch.set_grad_enabled(grad), pytest.raises(RuntimeError, match="jvp"):
+                    call(dual)
+        # without tangents nothing changes
+        assert nn.packed_attention(x, x, x, o).shape == x.shape
