@@ -793,7 +793,8 @@ int rhip_attn_backward(const rhip_attn *attn, const void *grad_out,
  * Layer normalisation of the rows of x [n, C] (row stride x_row elements):
  * y = (x - mean) * rstd * weight + bias over each row's C channels, rstd =
  * 1 / sqrt(biased variance + eps); weight and bias fp32 [C] or null. The
- * variance is summed around the mean, in fp32.
+ * variance is summed around the mean, in fp32. C is
+ * at most 2^30, and below 2^25 - 15 for the parameters' gradients.
  */
 
 /* Workspace bytes for rhip_ln_backward. */
@@ -823,7 +824,7 @@ int rhip_ln_backward(const void *grad_y, int64_t grad_y_row, const void *x,
  * y[i] = scale * weight[ids[i]] for a table weight [vocabulary, C] (row stride
  * weight_row elements); ids outside [0, vocabulary) (voxels without a class)
  * give a zero row and take no part in the gradient. ids are int64, or int32
- * with ids_int32 != 0.
+ * with ids_int32 != 0. Rows hold at most 64 x 65535 chunks of 16 bytes.
  */
 int rhip_embed_forward(const void *ids, int32_t ids_int32, int64_t n,
                        const void *weight, int64_t weight_row,

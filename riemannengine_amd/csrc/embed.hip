@@ -308,9 +308,12 @@ void check_embed(int64_t n, int64_t vocab, int32_t C) {
   if (n > INT32_MAX - kSegment || vocab > INT32_MAX - 1)
     throw Error(RHIP_ERR_UNSUPPORTED, "ids and table rows must stay below 2^31 - 64");
 }
-void check_embed_type(int32_t dtype) {
+void check_embed_type(int32_t dtype, int32_t C) {
   if (dtype != RHIP_F32 && dtype != RHIP_BF16)
     throw Error(RHIP_ERR_UNSUPPORTED, "dtype must be RHIP_F32 or RHIP_BF16");
+  // column tiles of 64 chunks along the grid's second axis
+  if (ceil_div(C, kWave * (dtype == RHIP_F32 ? RowChunk<float>::V : RowChunk<__bf16>::V)) > 65535)
+    throw Error(RHIP_ERR_UNSUPPORTED, "an embedding takes at most 65535 x 64 chunks of 16 bytes");
 }
 
 struct EmbedWs {
@@ -356,7 +359,7 @@ extern "C" int rhip_embed_forward(const void *ids, int32_t ids_int32, int64_t n,
                                   int32_t C, float scale, void *y, int32_t dtype,
                                   hipStream_t stream) {
   return guarded([&] {
-    check_embed_type(dtype);
+    check_embed_type(dtype, C);
     check_embed(n, vocabulary, C);
     if (n == 0)
       return;
@@ -398,7 +401,7 @@ extern "C" int rhip_embed_backward(const void *grad_y, int64_t grad_y_row, const
                                    float scale, void *grad_weight, int32_t dtype,
                                    void *workspace, size_t ws_bytes, hipStream_t stream) {
   return guarded([&] {
-    check_embed_type(dtype);
+    check_embed_type(dtype, C);
     check_embed(n, vocabulary, C);
     if (vocabulary == 0)
       return;

@@ -345,6 +345,7 @@ at::Tensor hip_layer_norm(const at::Tensor &input, const at::Tensor &weight,
   TORCH_CHECK(input.dim() >= 1 && input.size(-1) > 0, "layer norm needs at least one channel");
   hip_dtype(input, "layer norm input");
   const int64_t C = input.size(-1);
+  TORCH_CHECK(C < INT32_MAX, "layer norm takes fewer than 2^31 - 1 channels, got ", C);
   for (const auto *p : {&weight, &bias})
     TORCH_CHECK(!p->defined() || (p->device() == input.device() &&
                                   p->scalar_type() == torch::kFloat && p->dim() == 1 &&
@@ -366,6 +367,8 @@ at::Tensor hip_embedding(const at::Tensor &ids, const at::Tensor &weight, double
   TORCH_CHECK(ids.scalar_type() == torch::kInt || ids.scalar_type() == torch::kLong,
               "ids must be int32 or int64");
   TORCH_CHECK(weight.dim() == 2 && weight.size(1) > 0, "embedding weight must be [rows, channels]");
+  TORCH_CHECK(weight.size(1) < INT32_MAX, "embedding takes fewer than 2^31 - 1 channels, got ",
+              weight.size(1));
   TORCH_CHECK(std::isfinite(scale), "scale must be finite");
   hip_dtype(weight, "embedding weight");
   auto flat = ids.reshape({-1}).contiguous();

@@ -28,6 +28,9 @@ constexpr int kLnThreads = 256;
 // move more bytes (1024 of them on 16384 rows of 4096: 66 MB beside 402).
 constexpr int kLnBlocks = 512;
 constexpr int kSumCols = 16, kSumRows = 64; // ln_sums_kernel's columns and row lanes
+constexpr int32_t kLnMaxC = 1 << 30; // a workgroup's steps along a row stay below 2^31
+// ln_sums_kernel's launch: 2 C columns, 64 threads each
+constexpr int32_t kLnMaxParams = (1 << 25) - kSumCols;
 
 // N sums over a row's G lanes, in every lane; G = 256: the workgroup, through
 // LDS (buf is free again after the next barrier but one).
@@ -460,6 +463,8 @@ void check_rows(int32_t dtype, int64_t n, int32_t C) {
   RHIP_CHECK_ARG(n >= 0 && C >= 1, "bad sizes");
   if (n > INT32_MAX)
     throw Error(RHIP_ERR_UNSUPPORTED, "too many rows");
+  if (C > kLnMaxC)
+    throw Error(RHIP_ERR_UNSUPPORTED, "layer norm takes at most 2^30 channels");
 }
 
 // Workgroups of the backward: no more than row groups, at most kLnBlocks.
@@ -527,6 +532,8 @@ extern "C" int rhip_ln_backward(const void *grad_y, int64_t grad_y_row, const vo
                    "grad_y, x, mean and rstd are required");
     const bool params = grad_weight || grad_bias;
     RHIP_CHECK_ARG(!params || workspace, "workspace is required");
+    if (params && C > kLnMaxParams)
+      throw Error(RHIP_ERR_UNSUPPORTED, "the parameters' gradients take fewer than 2^25 channels");
     int64_t blocks = ln_blocks(n);
     float *part = nullptr;
     if (params) {

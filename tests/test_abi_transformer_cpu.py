@@ -99,3 +99,21 @@ def test_embedding_operands(no_library):
     ]:
         with pytest.raises(RuntimeError, match=name):
             call()
+
+
+@pytest.mark.parametrize("call,msg", [
+    (lambda L: L.rhip_ln_forward(1, 8, 1, 2 ** 30 + 1, None, None, 1e-5, 1, None, None, abi.F32,
+                                 None), "2\\^30"),
+    (lambda L: L.rhip_ln_backward(1, 8, 1, 8, 1, 2 ** 25, 1, 1, None, None, 1, 1, abi.F32, 1,
+                                  2 ** 40, None), "2\\^25"),
+    (lambda L: L.rhip_embed_forward(1, 0, 1, 1, 8, 1, 65535 * 256 + 1, 1.0, 1, abi.F32, None),
+     "chunks"),
+    (lambda L: L.rhip_embed_backward(1, 8, 1, 0, 1, 1, 65535 * 512 + 1, 1.0, 1, abi.BF16, 1,
+                                     2 ** 40, None), "chunks"),
+])
+def test_widths_that_no_launch_takes(call, msg):
+    """Refused on the host: no pointer is looked at."""
+    import re
+    lib = abi.lib()
+    assert call(lib) != 0
+    assert re.search(msg, lib.rhip_last_error().decode())

@@ -34,3 +34,14 @@ def test_forward_mode_tangents_are_refused():
                     call(dual)
         # without tangents nothing changes
         assert nn.packed_attention(x, x, x, o).shape == x.shape
+
+
+def test_channels_past_32_bits():
+    """2^32 + 8 channels are 8 in 32 bits."""
+    one = torch.zeros(1, device=DEV, dtype=torch.bfloat16)
+    wide = one.expand(2 ** 32 + 8)
+    ids = torch.zeros(1, dtype=torch.int64, device=DEV)
+    with pytest.raises(RuntimeError, match="channels"):
+        rie.nn.layer_norm(torch.zeros(2 ** 32 + 8, device=DEV, dtype=torch.bfloat16))
+    with pytest.raises(RuntimeError, match="channels"):
+        rie.nn.embedding(ids, wide[None])
