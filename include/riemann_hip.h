@@ -793,8 +793,8 @@ int rhip_attn_backward(const rhip_attn *attn, const void *grad_out,
  * Layer normalisation of the rows of x [n, C] (row stride x_row elements):
  * y = (x - mean) * rstd * weight + bias over each row's C channels, rstd =
  * 1 / sqrt(biased variance + eps); weight and bias fp32 [C] or null. The
- * variance is summed around the mean, in fp32. C is
- * at most 2^30, and below 2^25 - 15 for the parameters' gradients.
+ * variance is summed around the mean, in fp32. eps must be above zero in fp32;
+ * C at most 2^30, and below 2^25 - 15 for the parameters' gradients.
  */
 
 /* Workspace bytes for rhip_ln_backward. */

@@ -490,7 +490,7 @@ extern "C" int rhip_ln_forward(const void *x, int64_t x_row, int64_t n, int32_t 
                                float *mean, float *rstd, int32_t dtype, hipStream_t stream) {
   return guarded([&] {
     check_rows(dtype, n, C);
-    RHIP_CHECK_ARG(eps > 0, "eps must be positive");
+    RHIP_CHECK_ARG(static_cast<float>(eps) > 0.f, "eps must be positive in fp32");
     RHIP_CHECK_ARG((mean == nullptr) == (rstd == nullptr), "mean and rstd go together");
     if (n == 0)
       return;

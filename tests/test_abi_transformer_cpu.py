@@ -104,6 +104,8 @@ def test_embedding_operands(no_library):
 @pytest.mark.parametrize("call,msg", [
     (lambda L: L.rhip_ln_forward(1, 8, 1, 2 ** 30 + 1, None, None, 1e-5, 1, None, None, abi.F32,
                                  None), "2\\^30"),
+    (lambda L: L.rhip_ln_forward(1, 8, 1, 8, None, None, 1e-46, 1, None, None, abi.F32, None),
+     "eps"),
     (lambda L: L.rhip_ln_backward(1, 8, 1, 8, 1, 2 ** 25, 1, 1, None, None, 1, 1, abi.F32, 1,
                                   2 ** 40, None), "2\\^25"),
     (lambda L: L.rhip_embed_forward(1, 0, 1, 1, 8, 1, 65535 * 256 + 1, 1.0, 1, abi.F32, None),

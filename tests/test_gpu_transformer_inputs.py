@@ -45,3 +45,10 @@ def test_channels_past_32_bits():
         rie.nn.layer_norm(torch.zeros(2 ** 32 + 8, device=DEV, dtype=torch.bfloat16))
     with pytest.raises(RuntimeError, match="channels"):
         rie.nn.embedding(ids, wide[None])
+
+
+@pytest.mark.parametrize("eps", [0.0, 1e-60, -1e-5, float("nan")])
+def test_eps_that_fp32_takes_for_zero(eps):
+    """A constant row would come out as 0 / 0."""
+    with pytest.raises(RuntimeError, match="eps"):
+        rie.nn.layer_norm(torch.ones(3, 8, device=DEV), eps=eps)
