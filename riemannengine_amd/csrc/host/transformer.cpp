@@ -3,6 +3,9 @@
 // (rhip_attn_*, rhip_ln_*, rhip_embed_*), and the layers that put them on
 // sparse tensors (a sequence = the rows of one batch). These layers have no
 // counterpart in the reference; they follow its layers' conventions.
+#include <cmath>
+#include <limits>
+
 #include <ATen/DeviceGuard.h>
 #include <c10/hip/HIPStream.h>
 
@@ -369,7 +372,7 @@ at::Tensor hip_embedding(const at::Tensor &ids, const at::Tensor &weight, double
   TORCH_CHECK(weight.dim() == 2 && weight.size(1) > 0, "embedding weight must be [rows, channels]");
   TORCH_CHECK(weight.size(1) < INT32_MAX, "embedding takes fewer than 2^31 - 1 channels, got ",
               weight.size(1));
-  TORCH_CHECK(std::isfinite(scale), "scale must be finite");
+  TORCH_CHECK(std::abs(scale) <= std::numeric_limits<float>::max(), "scale must be finite in fp32");
   hip_dtype(weight, "embedding weight");
   auto flat = ids.reshape({-1}).contiguous();
   auto w = dense_last(weight);

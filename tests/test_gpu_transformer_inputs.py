@@ -52,3 +52,10 @@ def test_eps_that_fp32_takes_for_zero(eps):
     """A constant row would come out as 0 / 0."""
     with pytest.raises(RuntimeError, match="eps"):
         rie.nn.layer_norm(torch.ones(3, 8, device=DEV), eps=eps)
+
+
+@pytest.mark.parametrize("scale", [1e39, -1e300, float("nan"), float("inf")])
+def test_scales_that_fp32_takes_for_infinity(scale):
+    ids = torch.zeros(4, dtype=torch.int64, device=DEV)
+    with pytest.raises(RuntimeError, match="finite"):
+        rie.nn.embedding(ids, torch.ones(3, 8, device=DEV), scale)
