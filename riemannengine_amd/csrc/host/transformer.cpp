@@ -438,11 +438,11 @@ SparseTensor RiemannEmbeddingImpl::forward(const at::Tensor &ids, const SparseTe
 
 RiemannAttentionImpl::RiemannAttentionImpl(int64_t channels, int64_t heads, int64_t kv_heads,
                                            bool causal, bool bias)
-    : channels_(channels), heads_(heads), kv_heads_(kv_heads > 0 ? kv_heads : heads),
+    : channels_(channels), heads_(heads), kv_heads_(kv_heads == 0 ? heads : kv_heads),
       causal_(causal), has_bias_(bias) {
   TORCH_CHECK(channels > 0 && heads > 0 && channels % heads == 0,
               "RiemannAttention needs a multiple of ", heads, " channels, got ", channels);
-  TORCH_CHECK(heads % kv_heads_ == 0, "heads ", heads, " must be a multiple of key heads ",
+  TORCH_CHECK(kv_heads_ > 0 && heads % kv_heads_ == 0, "heads ", heads, " must be a multiple of key heads ",
               kv_heads_);
   reset();
 }

@@ -59,3 +59,11 @@ def test_scales_that_fp32_takes_for_infinity(scale):
     ids = torch.zeros(4, dtype=torch.int64, device=DEV)
     with pytest.raises(RuntimeError, match="finite"):
         rie.nn.embedding(ids, torch.ones(3, 8, device=DEV), scale)
+
+
+def test_negative_key_heads():
+    with pytest.raises(RuntimeError, match="multiple"):
+        rie.nn.RiemannAttention(64, 4, -2)
+    with pytest.raises(RuntimeError, match="multiple"):
+        rie.nn.AttentionBlock(64, 4, kv_heads=-1)
+    assert list(rie.nn.RiemannAttention(64, 4, 0).parameters())
