@@ -17,6 +17,9 @@ namespace {
 constexpr int kEmbThreads = 256;
 constexpr int kSegment = kWave; // positions a wave sums by itself, at most
 constexpr int kRowsPerWave = 4; // table rows a wave takes one after another
+// Table rows per id past which the table is cleared as a whole, its rows search
+// their first positions and the sums go by positions.
+constexpr int64_t kSparse = 8;
 constexpr int kJoinCols = 16, kJoinLanes = 64; // embed_join_kernel: columns by partial sums
 
 // Lanes per row: the row's chunks rounded up to a power of two, at most a wave.
@@ -117,8 +120,8 @@ __global__ __launch_bounds__(kSmallThreads) void embed_sort_small_kernel(
 
 // start[v] = first sorted position whose key is >= v, v = 0 .. vocab: the rows
 // after the key before position i, up to the key at i, start at i. The wave
-// fills the gaps between its keys together, so a few tokens in a large table
-// cost no more than many.
+// fills the gaps between its keys together. For a few ids in a large table that
+// would be one wave's work (52 ids, 88325 rows: 50 us): embed_starts_search_kernel.
 __global__ __launch_bounds__(kEmbThreads) void embed_starts_kernel(
     const uint32_t *__restrict__ keys, int64_t n, uint32_t vocab, int32_t *__restrict__ start,
     int32_t *__restrict__ runs) {
@@ -143,6 +146,27 @@ __global__ __launch_bounds__(kEmbThreads) void embed_starts_kernel(
     for (int64_t v = first + lane_id(); v <= last; v += kWave)
       start[v] = at;
   }
+}
+
+// The same, each table row by a search of its own over the keys, all rows at
+// once.
+__global__ __launch_bounds__(kEmbThreads) void embed_starts_search_kernel(
+    const uint32_t *__restrict__ keys, int64_t n, uint32_t vocab, int32_t *__restrict__ start,
+    int32_t *__restrict__ runs) {
+  const int64_t v = static_cast<int64_t>(blockIdx.x) * kEmbThreads + threadIdx.x;
+  if (v == 0)
+    *runs = 0;
+  if (v > vocab)
+    return;
+  int32_t lo = 0, hi = static_cast<int32_t>(n);
+  while (lo < hi) {
+    const int32_t mid = (lo + hi) >> 1;
+    if (keys[mid] < v)
+      lo = mid + 1;
+    else
+      hi = mid;
+  }
+  start[v] = lo;
 }
 
 // Sum of grad_y's rows at the sorted positions [p0, p1), at most 64 of them,
@@ -189,14 +213,30 @@ __device__ __forceinline__ void sum_rows(const T *__restrict__ gy, int64_t gy_ro
         acc[i][e] += __shfl_xor(acc[i][e], off, kWave);
 }
 
+// Zeros, for a table most of whose rows no id names.
+__global__ __launch_bounds__(kEmbThreads) void embed_clear_kernel(char *__restrict__ p,
+                                                                  int64_t bytes) {
+  const int64_t step = static_cast<int64_t>(gridDim.x) * kEmbThreads * 16;
+  for (int64_t i = (static_cast<int64_t>(blockIdx.x) * kEmbThreads + threadIdx.x) * 16; i < bytes;
+       i += step) {
+    if (i + 16 <= bytes) {
+      __builtin_nontemporal_store(v4u{0u, 0u, 0u, 0u}, reinterpret_cast<v4u_any *>(p + i));
+    } else {
+      for (int64_t e = i; e < bytes; e += 2) // elements of two bytes at least
+        *reinterpret_cast<uint16_t *>(p + e) = 0;
+    }
+  }
+}
+
 // One wave per work item and column tile of 64 NC chunks. The first items, the
 // longest: chunk j of the sorted positions, for the parts of long runs in it.
 // A chunk meets at most two of those: one from before it (partial sum 2 j) and
 // one that starts in it (2 j + 1), which then goes on the list of runs to join
 // (in any order: each is joined by itself). The others: four table rows, each
 // with at most kSegment positions, summed (or zeroed) and written; most rows
-// of a large table are in no batch, so a wave takes several.
-template <typename T, int NC>
+// of a large table are in no batch, so a wave takes several. SPARSE: the table
+// has been cleared, and a wave takes the rows that begin at four positions.
+template <typename T, int NC, bool SPARSE>
 __global__ __launch_bounds__(kEmbThreads) void embed_backward_kernel(
     const T *__restrict__ gy, int64_t gy_row, const uint32_t *__restrict__ keys,
     const int32_t *__restrict__ pos, const int32_t *__restrict__ start, int64_t n, int64_t vocab,
@@ -215,18 +255,26 @@ __global__ __launch_bounds__(kEmbThreads) void embed_backward_kernel(
   const int64_t segments = (n + kSegment - 1) / kSegment;
   if (item >= segments) {
     const int64_t first = (item - segments) * kRowsPerWave;
-    if (first >= vocab)
+    if (first >= (SPARSE ? n : vocab))
       return;
-    int32_t at[kRowsPerWave + 1];
+    int32_t at[kRowsPerWave + 1], end[kRowsPerWave];
+    int64_t row[kRowsPerWave];
 #pragma unroll
-    for (int r = 0; r <= kRowsPerWave; ++r)
-      at[r] = start[min(first + r, vocab)];
+    for (int r = 0; r < kRowsPerWave; ++r)
+      row[r] = SPARSE ? keys[min(first + r, n - 1)] : min(first + r, vocab);
+#pragma unroll
+    for (int r = 0; r < kRowsPerWave; ++r)
+      at[r] = start[row[r]];
+    at[kRowsPerWave] = SPARSE ? 0 : start[min(first + kRowsPerWave, vocab)];
+#pragma unroll
+    for (int r = 0; r < kRowsPerWave; ++r)
+      end[r] = SPARSE ? start[min(row[r] + 1, vocab)] : at[r + 1];
 #pragma unroll
     for (int r = 0; r < kRowsPerWave; ++r) {
-      const int64_t v = first + r;
-      if (v >= vocab || at[r + 1] - at[r] > kSegment)
+      const int64_t v = row[r];
+      if (v >= vocab || end[r] - at[r] > kSegment || (SPARSE && at[r] != first + r))
         continue;
-      sum_rows<T, NC>(gy, gy_row, pos, at[r], at[r + 1], c, C, log_g, acc);
+      sum_rows<T, NC>(gy, gy_row, pos, at[r], end[r], c, C, log_g, acc);
       if (writer) {
 #pragma unroll
         for (int i = 0; i < NC; ++i) {
@@ -422,10 +470,17 @@ extern "C" int rhip_embed_backward(const void *grad_y, int64_t grad_y_row, const
       sort_pairs_u32(w.sort, w.sort_bytes, w.keys, w.sorted, w.pos, w.order, n,
                      bits_of(static_cast<uint64_t>(vocabulary)), stream);
     }
-    hipLaunchKernelGGL(embed_starts_kernel,
-                       dim3(static_cast<unsigned>(ceil_div(n + 1, kEmbThreads))),
-                       dim3(kEmbThreads), 0, stream, w.sorted, n,
-                       static_cast<uint32_t>(vocabulary), w.start, w.runs);
+    const bool sparse = vocabulary > kSparse * n;
+    if (sparse)
+      hipLaunchKernelGGL(embed_starts_search_kernel,
+                         dim3(static_cast<unsigned>(ceil_div(vocabulary + 1, kEmbThreads))),
+                         dim3(kEmbThreads), 0, stream, w.sorted, n,
+                         static_cast<uint32_t>(vocabulary), w.start, w.runs);
+    else
+      hipLaunchKernelGGL(embed_starts_kernel,
+                         dim3(static_cast<unsigned>(ceil_div(n + 1, kEmbThreads))),
+                         dim3(kEmbThreads), 0, stream, w.sorted, n,
+                         static_cast<uint32_t>(vocabulary), w.start, w.runs);
     RHIP_LAUNCH_CHECK();
     with_embed_type(dtype, [&](auto t) {
       using T = decltype(t);
@@ -434,13 +489,24 @@ extern "C" int rhip_embed_backward(const void *grad_y, int64_t grad_y_row, const
       // chunks per lane: whole rows in one wave as far as registers go, unless
       // that leaves too few waves (8340 labels of 3 classes, 986 wide: 53 us
       // with two chunks per lane, 41 with one)
-      const int64_t items = ceil_div(vocabulary, kRowsPerWave) + segments;
+      const int64_t items = ceil_div(sparse ? n : vocabulary, kRowsPerWave) + segments;
+      if (sparse) {
+        const int64_t bytes = vocabulary * C * static_cast<int64_t>(sizeof(T));
+        hipLaunchKernelGGL(embed_clear_kernel,
+                           dim3(static_cast<unsigned>(
+                               std::min<int64_t>(ceil_div(bytes, kEmbThreads * 16), 8192))),
+                           dim3(kEmbThreads), 0, stream, static_cast<char *>(grad_weight), bytes);
+        RHIP_LAUNCH_CHECK();
+        if (n == 0)
+          return;
+      }
       const int64_t fill = 4096 / items; // column tiles that fill the chip
-      auto launch = [&](auto nc) {
+      auto launch_rows = [&](auto nc, auto s) {
         constexpr int NC = decltype(nc)::value;
+        constexpr bool SPARSE = decltype(s)::value;
         const int64_t most = max_groups(kEmbThreads) * (kEmbThreads / kWave);
         for (int64_t i = 0; i < items; i += most) {
-          hipLaunchKernelGGL((embed_backward_kernel<T, NC>),
+          hipLaunchKernelGGL((embed_backward_kernel<T, NC, SPARSE>),
                              dim3(static_cast<unsigned>(ceil_div(std::min(items - i, most),
                                                                  kEmbThreads / kWave)),
                                   static_cast<unsigned>(ceil_div(chunks, kWave * NC))),
@@ -450,6 +516,12 @@ extern "C" int rhip_embed_backward(const void *grad_y, int64_t grad_y_row, const
                              static_cast<T *>(grad_weight), w.part, w.runs, i);
           RHIP_LAUNCH_CHECK();
         }
+      };
+      auto launch = [&](auto nc) {
+        if (sparse)
+          launch_rows(nc, std::true_type{});
+        else
+          launch_rows(nc, std::false_type{});
       };
       if (chunks <= kWave || fill >= ceil_div(chunks, kWave))
         launch(std::integral_constant<int, 1>{});
