@@ -16,9 +16,12 @@ namespace {
 
 constexpr int kEmbThreads = 256;
 constexpr int kSegment = kWave; // positions a wave sums by itself, at most
-constexpr int kRowsPerWave = 4; // table rows a wave takes one after another
+constexpr int kRowsPerWave = 4; // table rows a wave takes one after another, at most
+constexpr int64_t kManyRows = 16384; // rows by column tiles of 64 chunks from which on it does
 // Table rows per id past which the table is cleared as a whole, its rows search
-// their first positions and the sums go by positions.
+// their first positions and the sums go by positions. (fp32, 5000 ids in 100000
+// rows of 32: 54 us so, 66 the other way; in 60000 of 512: 83 and 75; bf16,
+// 40000 in 400000 of 256: 129 and 138, in 200000: 97 and 100.)
 constexpr int64_t kSparse = 8;
 constexpr int kJoinCols = 16, kJoinLanes = 64; // embed_join_kernel: columns by partial sums
 
@@ -232,16 +235,16 @@ __global__ __launch_bounds__(kEmbThreads) void embed_clear_kernel(char *__restri
 // longest: chunk j of the sorted positions, for the parts of long runs in it.
 // A chunk meets at most two of those: one from before it (partial sum 2 j) and
 // one that starts in it (2 j + 1), which then goes on the list of runs to join
-// (in any order: each is joined by itself). The others: four table rows, each
+// (in any order: each is joined by itself). The others: some table rows, each
 // with at most kSegment positions, summed (or zeroed) and written; most rows
-// of a large table are in no batch, so a wave takes several. SPARSE: the table
-// has been cleared, and a wave takes the rows that begin at four positions.
+// of a large table are in no batch, so a wave takes up to four. SPARSE: the table
+// has been cleared, and a wave takes the rows that begin at some positions.
 template <typename T, int NC, bool SPARSE>
 __global__ __launch_bounds__(kEmbThreads) void embed_backward_kernel(
     const T *__restrict__ gy, int64_t gy_row, const uint32_t *__restrict__ keys,
     const int32_t *__restrict__ pos, const int32_t *__restrict__ start, int64_t n, int64_t vocab,
     int C, int log_g, float scale, T *__restrict__ gw, float *__restrict__ part,
-    int32_t *__restrict__ runs, int64_t item0) {
+    int32_t *__restrict__ runs, int64_t item0, int rows_per_wave) {
   using R = RowChunk<T>;
   const int64_t item = item0 + static_cast<int64_t>(blockIdx.x) * (kEmbThreads / kWave) +
                        __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
@@ -254,7 +257,7 @@ __global__ __launch_bounds__(kEmbThreads) void embed_backward_kernel(
   float acc[NC][R::V];
   const int64_t segments = (n + kSegment - 1) / kSegment;
   if (item >= segments) {
-    const int64_t first = (item - segments) * kRowsPerWave;
+    const int64_t first = (item - segments) * rows_per_wave;
     if (first >= (SPARSE ? n : vocab))
       return;
     int32_t at[kRowsPerWave + 1], end[kRowsPerWave];
@@ -272,6 +275,8 @@ __global__ __launch_bounds__(kEmbThreads) void embed_backward_kernel(
 #pragma unroll
     for (int r = 0; r < kRowsPerWave; ++r) {
       const int64_t v = row[r];
+      if (r >= rows_per_wave)
+        break;
       if (v >= vocab || end[r] - at[r] > kSegment || (SPARSE && at[r] != first + r))
         continue;
       sum_rows<T, NC>(gy, gy_row, pos, at[r], end[r], c, C, log_g, acc);
@@ -489,7 +494,13 @@ extern "C" int rhip_embed_backward(const void *grad_y, int64_t grad_y_row, const
       // chunks per lane: whole rows in one wave as far as registers go, unless
       // that leaves too few waves (8340 labels of 3 classes, 986 wide: 53 us
       // with two chunks per lane, 41 with one)
-      const int64_t items = ceil_div(sparse ? n : vocabulary, kRowsPerWave) + segments;
+      // rows one after another only where waves are many: few rows with 64
+      // positions each would leave the chip to some waves. (1047 ids of 16 classes,
+      // 1973 wide in bf16, this kernel: 103 us four to a wave, 45 one; 40000 ids of
+      // 200000 rows, 256 wide, the whole gradient: 100 us and 127.)
+      const int64_t units = sparse ? n : vocabulary;
+      const int rows = units * ceil_div(chunks, kWave) >= kManyRows ? kRowsPerWave : 1;
+      const int64_t items = ceil_div(units, rows) + segments;
       if (sparse) {
         const int64_t bytes = vocabulary * C * static_cast<int64_t>(sizeof(T));
         hipLaunchKernelGGL(embed_clear_kernel,
@@ -513,7 +524,7 @@ extern "C" int rhip_embed_backward(const void *grad_y, int64_t grad_y_row, const
                              dim3(kEmbThreads), 0, stream, static_cast<const T *>(grad_y),
                              grad_y_row, w.sorted, w.order, w.start, n, vocabulary, C,
                              log2_of(lanes_per_row(chunks)), scale,
-                             static_cast<T *>(grad_weight), w.part, w.runs, i);
+                             static_cast<T *>(grad_weight), w.part, w.runs, i, rows);
           RHIP_LAUNCH_CHECK();
         }
       };

@@ -1,5 +1,5 @@
 """Embedding gradients whose time must follow their work, not a few waves': a
-few ids in a large table, and widths that end inside a 16-byte chunk."""
+few ids in a large table, a few classes."""
 import pytest
 import torch
 
@@ -38,3 +38,30 @@ def test_a_few_ids_in_a_large_table(n):
     assert got <= clear + 100
     want = torch.zeros(V, C, dtype=torch.float64, device=DEV).index_add_(0, ids, dy.double())
     assert (abi.embed_backward(dy, ids, V).double() - want).abs().max() <= 1e-5
+
+
+def replayed(call):
+    """Time of a call without the host's, microseconds: ten in a graph."""
+    stream = torch.cuda.Stream()
+    stream.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(stream):
+        call()
+    torch.cuda.current_stream().wait_stream(stream)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        for _ in range(10):
+            call()
+    return best(graph.replay) / 10
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("n,V", [(1000, 16), (3500, 56)])
+def test_classes_of_62_ids_each(dtype, n, V):
+    """Rows just short of being cut into parts: at most 1.5 times all ids in one
+    class, which are, and 5 us."""
+    dy = torch.randn(n, 512, device=DEV).to(dtype)
+    ids = torch.arange(n, device=DEV) % V
+    one = replayed(lambda: abi.embed_backward(dy, torch.zeros_like(ids), 1))
+    got = replayed(lambda: abi.embed_backward(dy, ids, V))
+    print("classes", n, V, dtype, one, got, flush=True)
+    assert got <= 1.5 * one + 5
