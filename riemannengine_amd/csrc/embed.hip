@@ -34,6 +34,16 @@ __host__ __device__ inline int lanes_per_row(int chunks) {
   return g;
 }
 
+// First column of chunk `chunk` of a row of C; C: past the row. The last chunk of
+// a row that ends inside one begins earlier, so that it is whole: its first
+// columns are also the chunk's before it, whose lane comes to the same values. (By
+// elements, the sums of 3780 ids of 51 classes, 383 wide in bf16, took 55 us; 384
+// wide 31.)
+template <int V> __device__ __forceinline__ int chunk_column(int chunk, int C) {
+  const int c = chunk * V;
+  return c >= C ? C : C < V ? c : min(c, C - V);
+}
+
 __device__ __forceinline__ int64_t id_at(const void *ids, int is32, int64_t i) {
   return is32 ? static_cast<const int32_t *>(ids)[i] : static_cast<const int64_t *>(ids)[i];
 }
@@ -47,7 +57,7 @@ __global__ __launch_bounds__(kEmbThreads) void embed_forward_kernel(
   const int lane = threadIdx.x & ((1 << log_g) - 1);
   const int64_t i =
       static_cast<int64_t>(blockIdx.x) * (kEmbThreads >> log_g) + (threadIdx.x >> log_g);
-  const int c = (blockIdx.y * kWave + lane) * R::V;
+  const int c = chunk_column<R::V>(blockIdx.y * kWave + lane, C);
   if (i >= n || c >= C)
     return;
   const int64_t id = id_at(ids, is32, i);
@@ -253,7 +263,7 @@ __global__ __launch_bounds__(kEmbThreads) void embed_backward_kernel(
   int c[NC];
 #pragma unroll
   for (int i = 0; i < NC; ++i) // chunks past the row: nothing to load or write
-    c[i] = min(((blockIdx.y * NC + i) * kWave + lane) * R::V, C);
+    c[i] = chunk_column<R::V>((blockIdx.y * NC + i) * kWave + lane, C);
   float acc[NC][R::V];
   const int64_t segments = (n + kSegment - 1) / kSegment;
   if (item >= segments) {

@@ -1,8 +1,8 @@
 // Rows in 16-byte chunks at any alignment, for the kernels that stream whole
 // rows (layer norm, embedding). Global loads and stores of 16 bytes need only
 // the element's own alignment on gfx950, so rows of odd widths, strides and
-// offsets move as fast as aligned ones; only a row's last, partial chunk goes
-// element by element.
+// offsets move as fast as aligned ones. A row's last, partial chunk goes element
+// by element here; the embedding moves it back to be whole.
 #pragma once
 
 #include "conv_device.hpp"

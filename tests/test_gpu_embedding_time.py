@@ -1,5 +1,6 @@
 """Embedding gradients whose time must follow their work, not a few waves': a
-few ids in a large table, a few classes."""
+few ids in a large table, a few classes, widths that end inside a 16-byte
+chunk."""
 import pytest
 import torch
 
@@ -65,3 +66,16 @@ def test_classes_of_62_ids_each(dtype, n, V):
     got = replayed(lambda: abi.embed_backward(dy, ids, V))
     print("classes", n, V, dtype, one, got, flush=True)
     assert got <= 1.5 * one + 5
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("n,V,C", [(3780, 51, 383), (900, 21, 1677), (20000, 30, 63)])
+def test_widths_that_end_inside_a_chunk(dtype, n, V, C):
+    """At most 1.1 times the next width of whole chunks, and 5 us."""
+    ids = torch.arange(n, device=DEV) % V
+    times = []
+    for width in (C, (C + 7) // 8 * 8):
+        dy = torch.randn(n, width, device=DEV).to(dtype)
+        times.append(replayed(lambda: abi.embed_backward(dy, ids, V)))
+    print("widths", n, V, C, dtype, times, flush=True)
+    assert times[0] <= 1.1 * times[1] + 5
