@@ -127,7 +127,7 @@ __device__ __forceinline__ void join_row(const float *rows, int row_floats, int 
 // lies. dP's sums start at -delta.
 //
 // Bound by the matrix cores (four causal prompts of 4096, 16 over 4 heads, 128
-// wide, bf16: 418 us, 987 TFLOP/s), by the vector instructions at 32 wide (840).
+// wide, bf16: 398 us, 1035 TFLOP/s), by the vector instructions at 32 wide (890).
 template <typename T, int DP, bool VEC, int W>
 __global__ __launch_bounds__(kBwdThreads, (BwdShape<T, DP, W, false>::kOccupancy)) void
 attn_dq_kernel(AttnArgs a) {

@@ -40,7 +40,8 @@ template <typename T, int DP, int W> struct FwdShape {
   // heads, three causal sequences of 1100: two buffers and one workgroup 72 us, one
   // buffer and two workgroups 57). bf16's W = 1 serves single tokens too, whose
   // stream of keys is better held by two buffers (32 over caches of 1 to 16384, 8
-  // key heads, 128 wide: 156 us, and 172 with two workgroups).
+  // key heads, 128 wide: 156 us, and 172 with two workgroups); other launches of
+  // few rows pay for that (16 rows a sequence over 3000 keys: 50 us, and 37).
   static constexpr int kBuffers =
       kStreams * 4 * kTileBytes <= (sizeof(T) == 4 && DP <= 64 ? 80 : 160) * 1024 ? 2 : 1;
   static constexpr int kJoinRow = DP + 4; // floats per row of the joined results
@@ -82,9 +83,9 @@ __device__ void finish_row(const AttnArgs &a, int64_t row, int32_t head, float o
 // multiplied.
 //
 // Bounds: the matrix cores at width 128 (four causal prompts of 4096, 16 over 4
-// heads, bf16: 327 us, 840 TFLOP/s; the cores busy for 40% of the cycles, the
+// heads, bf16: 327 us, 840 TFLOP/s; the cores busy for 38% of the cycles, the
 // softmax's vector instructions beside them); the vector instructions at 32 and
-// 64 (600 and 870: a score costs one exponential whatever the width); memory
+// 64 (630 and 900: a score costs one exponential whatever the width); memory
 // for single tokens (32 over caches of 1 to 16384, 8 key heads of 128: 4.7 TB/s).
 // Taken back as no faster: the next tile's scores computed beside this one's
 // softmax, row sums as a product with ones, priorities of waves.
