@@ -220,7 +220,9 @@ attn_dq_kernel(AttnArgs a) {
 
   // As in the forward, but for whole keys: where the row's statistics are finite, a
   // key that is not has probability zero and adds nothing but NaN at the places
-  // that are not finite. Where they are not, all of the row's sums are NaN.
+  // that are not finite (its score counts as 0, so a row of scores all below -88,
+  // where that weight overflows, gets NaN throughout). Where the statistics are
+  // not finite, all of the row's sums are NaN.
   bool left_out = false;
   if (W > 1 && threadIdx.x == 0)
     any_left_out = 0;
