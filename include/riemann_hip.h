@@ -788,6 +788,128 @@ int rhip_attn_backward(const rhip_attn *attn, const void *grad_out,
                        void *workspace, size_t workspace_bytes,
                        hipStream_t stream);
 
+/* -------------------------------------------------------------- rotation
+ *
+ * Rotation of the heads of queries and keys by positions of one or several
+ * axes (voxel coordinates; time, height and width; a text's places), with the
+ * heads' RMS norm before it. Rows x [n, heads, dim] with strides of their own
+ * for rows and heads; y dense. A head has P = sum of sections pairs, elements
+ * (p, P + p), or with interleaved != 0 (2 p, 2 p + 1); the first sections[0]
+ * pairs turn with the first axis, and so on:
+ *
+ *   t = positions[row][axis of p] * frequencies[p]   (fp64)
+ *   (a, b) -> (a cos t - b sin t, a sin t + b cos t)
+ *
+ * Elements 2 P .. dim - 1 stay as they are. With norm != 0 the heads are
+ * normed first: x / sqrt(mean(x^2) + eps) * weight, fp32 weight [dim] or null
+ * for ones. dim at most 256, up to 8 axes.
+ */
+#define RHIP_ROTARY_MAX_AXES 8
+
+typedef enum rhip_position_type {
+  RHIP_POSITION_I32 = 0,
+  RHIP_POSITION_I64 = 1,
+  RHIP_POSITION_F32 = 2
+} rhip_position_type;
+
+typedef struct rhip_rotary {
+  int64_t n;                              /* rows */
+  const void *positions;                  /* device [n, axes], the last axis dense */
+  int64_t position_row;                   /* row stride in elements */
+  const double *frequencies;              /* device [P], radians per step */
+  int32_t position_type;                  /* rhip_position_type */
+  int32_t axes;
+  int32_t sections[RHIP_ROTARY_MAX_AXES]; /* pairs of each axis */
+  int32_t dim;
+  int32_t interleaved;
+  int32_t norm;
+  int32_t dtype; /* of x, y and their gradients */
+  double eps;
+} rhip_rotary;
+
+/* One tensor of a call: x, weight and y for the forward; grad_y, x and weight
+ * (with norm), and grad_x and grad_weight (either may be null) for the
+ * backward. grad_x [n, heads, dim] and grad_weight [dim] are dense and
+ * overwritten. Strides in elements. */
+typedef struct rhip_rotary_heads {
+  const void *x;
+  int64_t x_row, x_head;
+  const void *grad_y;
+  int64_t grad_y_row, grad_y_head;
+  const float *weight;
+  void *y;
+  void *grad_x;
+  float *grad_weight;
+  int32_t heads;
+} rhip_rotary_heads;
+
+/* y of q and, unless k is null, of k, which has the same positions. */
+int rhip_rotary_forward(const rhip_rotary *rotary, const rhip_rotary_heads *q,
+                        const rhip_rotary_heads *k, hipStream_t stream);
+
+/* Workspace bytes of rhip_rotary_backward. */
+int rhip_rotary_workspace_bytes(const rhip_rotary *rotary, size_t *bytes);
+
+/*
+ * With d = grad_y turned back: without norm grad_x = d; with it, r = 1 /
+ * sqrt(mean(x^2) + eps): grad_x = r (d w - x r^2 mean(d w x)), grad_weight =
+ * sum over rows and heads of d x r, in an order that depends on the sizes
+ * alone. The workspace may be null without norm.
+ */
+int rhip_rotary_backward(const rhip_rotary *rotary, const rhip_rotary_heads *q,
+                         const rhip_rotary_heads *k, void *workspace,
+                         size_t workspace_bytes, hipStream_t stream);
+
+/* -------------------------------------------------- gated feed-forward
+ *
+ * y = (act(x gate^T) * (x up^T)) down^T for rows x [n, channels], weights gate
+ * and up [hidden, channels] and down [outputs, hidden], as linear layers hold
+ * them; row strides in elements, the last axes dense. act: g sigmoid(g), or g
+ * times the normal distribution's integral up to g. Sums are fp32; bf16: the
+ * product h in front of down, and in the backward the gradients of x gate^T
+ * and x up^T, are rounded to bf16 as operands of the matrix cores. Results do
+ * not change from run to run. channels, hidden and outputs at most 2^20.
+ */
+typedef enum rhip_activation { RHIP_ACT_SILU = 0, RHIP_ACT_GELU = 1 } rhip_activation;
+
+typedef enum rhip_gated_pass {
+  RHIP_GATED_INFERENCE = 0, /* the forward without a saved buffer */
+  RHIP_GATED_FORWARD = 1,   /* the forward with one */
+  RHIP_GATED_BACKWARD = 2
+} rhip_gated_pass;
+
+typedef struct rhip_gated {
+  int64_t n; /* rows */
+  const void *x, *gate, *up, *down;
+  const void *grad_y; /* backward: [n, outputs] */
+  int64_t x_row, gate_row, up_row, down_row, grad_y_row;
+  int32_t channels, hidden, outputs;
+  int32_t activation; /* rhip_activation */
+  int32_t dtype;      /* of all matrices */
+} rhip_gated;
+
+/* Bytes of what the forward keeps for the backward (256-byte aligned memory). */
+int rhip_gated_saved_bytes(const rhip_gated *gated, size_t *bytes);
+
+/* Workspace bytes of a pass with this descriptor's sizes, strides and pointers
+ * (what is not aligned to 16 bytes is laid out anew in the workspace). */
+int rhip_gated_workspace_bytes(const rhip_gated *gated, int32_t pass, size_t *bytes);
+
+/* y [n, outputs], dense; saved may be null where no backward follows. */
+int rhip_gated_forward(const rhip_gated *gated, void *y, void *saved,
+                       size_t saved_bytes, void *workspace,
+                       size_t workspace_bytes, hipStream_t stream);
+
+/*
+ * grad_x [n, channels], grad_gate and grad_up [hidden, channels], grad_down
+ * [outputs, hidden], dense and overwritten (the weights' are zeros without
+ * rows); any may be null, grad_gate and grad_up both.
+ */
+int rhip_gated_backward(const rhip_gated *gated, const void *saved,
+                        size_t saved_bytes, void *grad_x, void *grad_gate,
+                        void *grad_up, void *grad_down, void *workspace,
+                        size_t workspace_bytes, hipStream_t stream);
+
 /* ------------------------------------------------------------ layer norm
  *
  * Layer normalisation of the rows of x [n, C] (row stride x_row elements):

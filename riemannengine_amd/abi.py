@@ -52,6 +52,9 @@ EXPORTS = (
     "rhip_attn_plan", "rhip_attn_workspace_bytes", "rhip_attn_forward", "rhip_attn_backward",
     "rhip_ln_workspace_bytes", "rhip_ln_forward", "rhip_ln_backward",
     "rhip_embed_forward", "rhip_embed_workspace_bytes", "rhip_embed_backward",
+    "rhip_rotary_forward", "rhip_rotary_workspace_bytes", "rhip_rotary_backward",
+    "rhip_gated_saved_bytes", "rhip_gated_workspace_bytes", "rhip_gated_forward",
+    "rhip_gated_backward",
 )
 
 
@@ -85,6 +88,44 @@ class RhipAttn(ctypes.Structure):
 
 _vp, _i64, _i32, _sz = ctypes.c_void_p, ctypes.c_int64, ctypes.c_int32, ctypes.c_size_t
 _P = ctypes.POINTER
+
+
+ROTARY_MAX_AXES = 8
+POSITION_TYPES = {torch.int32: 0, torch.int64: 1, torch.float32: 2}
+
+
+class RhipRotary(ctypes.Structure):
+    _fields_ = [
+        ("n", ctypes.c_int64), ("positions", ctypes.c_void_p), ("position_row", ctypes.c_int64),
+        ("frequencies", ctypes.c_void_p), ("position_type", ctypes.c_int32),
+        ("axes", ctypes.c_int32), ("sections", ctypes.c_int32 * ROTARY_MAX_AXES),
+        ("dim", ctypes.c_int32), ("interleaved", ctypes.c_int32), ("norm", ctypes.c_int32),
+        ("dtype", ctypes.c_int32), ("eps", ctypes.c_double),
+    ]
+
+
+class RhipRotaryHeads(ctypes.Structure):
+    _fields_ = [
+        ("x", ctypes.c_void_p), ("x_row", ctypes.c_int64), ("x_head", ctypes.c_int64),
+        ("grad_y", ctypes.c_void_p), ("grad_y_row", ctypes.c_int64),
+        ("grad_y_head", ctypes.c_int64), ("weight", ctypes.c_void_p), ("y", ctypes.c_void_p),
+        ("grad_x", ctypes.c_void_p), ("grad_weight", ctypes.c_void_p), ("heads", ctypes.c_int32),
+    ]
+
+
+ACTIVATIONS = {"silu": 0, "gelu": 1}
+GATED_INFERENCE, GATED_FORWARD, GATED_BACKWARD = 0, 1, 2
+
+
+class RhipGated(ctypes.Structure):
+    _fields_ = [
+        ("n", ctypes.c_int64), ("x", ctypes.c_void_p), ("gate", ctypes.c_void_p),
+        ("up", ctypes.c_void_p), ("down", ctypes.c_void_p), ("grad_y", ctypes.c_void_p),
+        ("x_row", ctypes.c_int64), ("gate_row", ctypes.c_int64), ("up_row", ctypes.c_int64),
+        ("down_row", ctypes.c_int64), ("grad_y_row", ctypes.c_int64),
+        ("channels", ctypes.c_int32), ("hidden", ctypes.c_int32), ("outputs", ctypes.c_int32),
+        ("activation", ctypes.c_int32), ("dtype", ctypes.c_int32),
+    ]
 
 
 def _declare(lib):
@@ -184,6 +225,16 @@ def _declare(lib):
         "rhip_embed_workspace_bytes": (ctypes.c_int, [_i64, _i64, _i32, _P(_sz)]),
         "rhip_embed_backward": (ctypes.c_int, [_vp, _i64, _vp, _i32, _i64, _i64, _i32,
                                                ctypes.c_float, _vp, _i32, _vp, _sz, _vp]),
+        "rhip_rotary_forward": (ctypes.c_int, [_P(RhipRotary), _P(RhipRotaryHeads),
+                                               _P(RhipRotaryHeads), _vp]),
+        "rhip_rotary_workspace_bytes": (ctypes.c_int, [_P(RhipRotary), _P(_sz)]),
+        "rhip_rotary_backward": (ctypes.c_int, [_P(RhipRotary), _P(RhipRotaryHeads),
+                                                _P(RhipRotaryHeads), _vp, _sz, _vp]),
+        "rhip_gated_saved_bytes": (ctypes.c_int, [_P(RhipGated), _P(_sz)]),
+        "rhip_gated_workspace_bytes": (ctypes.c_int, [_P(RhipGated), _i32, _P(_sz)]),
+        "rhip_gated_forward": (ctypes.c_int, [_P(RhipGated), _vp, _vp, _sz, _vp, _sz, _vp]),
+        "rhip_gated_backward": (ctypes.c_int, [_P(RhipGated), _vp, _sz, _vp, _vp, _vp, _vp, _vp,
+                                               _sz, _vp]),
     }
     for name, (res, args) in sig.items():
         fn = getattr(lib, name)
@@ -1167,3 +1218,145 @@ def embed_backward(grad_y: torch.Tensor, ids: torch.Tensor, vocabulary: int,
                                      _ptr(gw), _dtype_code(grad_y.dtype), _ptr(ws), ws.numel(),
                                      _stream(grad_y.device)), "rhip_embed_backward")
     return gw
+
+
+def _rotary_desc(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Tensor,
+                 frequencies: torch.Tensor, sections, interleaved: bool, norm: bool,
+                 eps: float) -> RhipRotary:
+    _require_cuda(q, "q")
+    if q.dim() != 3 or (k is not None and (k.dim() != 3 or k.shape[0] != q.shape[0]
+                                           or k.shape[2] != q.shape[2] or k.dtype != q.dtype
+                                           or k.device != q.device)):
+        raise RuntimeError("q and k must be [n, heads, dim] of one dtype on one device")
+    sections = [int(v) for v in sections]
+    if not 1 <= len(sections) <= ROTARY_MAX_AXES:
+        raise RuntimeError("sections must hold 1 to 8 axes")
+    if (positions.dim() != 2 or tuple(positions.shape) != (q.shape[0], len(sections))
+            or positions.dtype not in POSITION_TYPES or positions.device != q.device
+            or (positions.shape[1] > 1 and positions.stride(1) != 1)):
+        raise RuntimeError(f"positions must be int32, int64 or fp32 [{q.shape[0]}, "
+                           f"{len(sections)}] with a dense last axis on the heads' device")
+    _require_dense(frequencies, "frequencies", (sum(sections),), torch.float64, q.device)
+    return RhipRotary(q.shape[0], positions.data_ptr(), positions.stride(0),
+                      frequencies.data_ptr(), POSITION_TYPES[positions.dtype], len(sections),
+                      (ctypes.c_int32 * ROTARY_MAX_AXES)(*sections), q.shape[2],
+                      int(interleaved), int(norm), _dtype_code(q.dtype), eps)
+
+
+def _rotary_weights(q, k, weights, norm):
+    for t, w in zip((q, k), weights):
+        if w is not None and (t is None or not norm):
+            raise RuntimeError("weights belong to normed tensors")
+        if w is not None:
+            _require_dense(w, "weight", (t.shape[2],), torch.float32, t.device)
+
+
+def rotary_forward(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Tensor,
+                   frequencies: torch.Tensor, sections, interleaved: bool = False,
+                   norm: bool = False, weights=(None, None), eps: float = 1e-6):
+    """y of q and of k (None without k): heads [n, heads, dim] turned by
+    positions [n, axes]; with norm, normed first (fp32 weights [dim] or None)."""
+    q, k = _dense_last(q), None if k is None else _dense_last(k)
+    desc = _rotary_desc(q, k, positions, frequencies, sections, interleaved, norm, eps)
+    _rotary_weights(q, k, weights, norm)
+    ys, heads = [], []
+    for t, w in zip((q, k), weights):
+        if t is None:
+            ys.append(None)
+            continue
+        ys.append(torch.empty(t.shape, dtype=t.dtype, device=t.device))
+        heads.append(RhipRotaryHeads(x=t.data_ptr(), x_row=t.stride(0), x_head=t.stride(1),
+                                     weight=None if w is None else w.data_ptr(),
+                                     y=ys[-1].data_ptr(), heads=t.shape[1]))
+    _check(lib().rhip_rotary_forward(ctypes.byref(desc), ctypes.byref(heads[0]),
+                                     ctypes.byref(heads[1]) if len(heads) > 1 else None,
+                                     _stream(q.device)), "rhip_rotary_forward")
+    return tuple(ys)
+
+
+def rotary_backward(grads, q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Tensor,
+                    frequencies: torch.Tensor, sections, interleaved: bool = False,
+                    norm: bool = False, weights=(None, None), eps: float = 1e-6):
+    """(grad_q, grad_k, grad of q's weight, of k's) from the gradients of both
+    results; None where there is no tensor or no weight."""
+    q, k = _dense_last(q), None if k is None else _dense_last(k)
+    desc = _rotary_desc(q, k, positions, frequencies, sections, interleaved, norm, eps)
+    _rotary_weights(q, k, weights, norm)
+    gx, gw, heads, keep = [None, None], [None, None], [], []
+    for i, (t, w) in enumerate(zip((q, k), weights)):
+        if t is None:
+            continue
+        g = _dense_last(grads[i].to(t.dtype))
+        if g.shape != t.shape or g.device != t.device:
+            raise RuntimeError("a gradient does not match its tensor")
+        keep.append(g)
+        gx[i] = torch.empty(t.shape, dtype=t.dtype, device=t.device)
+        gw[i] = None if w is None else torch.empty_like(w)
+        heads.append(RhipRotaryHeads(
+            x=t.data_ptr(), x_row=t.stride(0), x_head=t.stride(1), grad_y=g.data_ptr(),
+            grad_y_row=g.stride(0), grad_y_head=g.stride(1),
+            weight=None if w is None else w.data_ptr(), grad_x=gx[i].data_ptr(),
+            grad_weight=None if w is None else gw[i].data_ptr(), heads=t.shape[1]))
+    ws = torch.empty(_sizeq(lib().rhip_rotary_workspace_bytes, ctypes.byref(desc)),
+                     dtype=torch.uint8, device=q.device)
+    _check(lib().rhip_rotary_backward(ctypes.byref(desc), ctypes.byref(heads[0]),
+                                      ctypes.byref(heads[1]) if len(heads) > 1 else None,
+                                      _ptr(ws), ws.numel(), _stream(q.device)),
+           "rhip_rotary_backward")
+    return (*gx, *gw)
+
+
+def _gated_desc(x, gate, up, down, activation, grad_y=None) -> RhipGated:
+    _require_cuda(x, "x")
+    if activation not in ACTIVATIONS:
+        raise RuntimeError('activation must be "silu" or "gelu"')
+    if (x.dim() != 2 or gate.dim() != 2 or down.dim() != 2 or gate.shape[1] != x.shape[1]
+            or up.shape != gate.shape or down.shape[1] != gate.shape[0]):
+        raise RuntimeError("x must be [n, channels], gate and up [hidden, channels], down "
+                           "[outputs, hidden]")
+    for t, name in ((gate, "gate"), (up, "up"), (down, "down"), (grad_y, "grad_y")):
+        if t is not None and (t.device != x.device or t.dtype != x.dtype):
+            raise RuntimeError(f"{name} must be of the rows' dtype and device")
+    if grad_y is not None and tuple(grad_y.shape) != (x.shape[0], down.shape[0]):
+        raise RuntimeError("grad_y must be [n, outputs]")
+    return RhipGated(x.shape[0], x.data_ptr(), gate.data_ptr(), up.data_ptr(), down.data_ptr(),
+                     None if grad_y is None else grad_y.data_ptr(), x.stride(0), gate.stride(0),
+                     up.stride(0), down.stride(0), 0 if grad_y is None else grad_y.stride(0),
+                     x.shape[1], gate.shape[0], down.shape[0], ACTIVATIONS[activation],
+                     _dtype_code(x.dtype))
+
+
+def gated_forward(x: torch.Tensor, gate: torch.Tensor, up: torch.Tensor, down: torch.Tensor,
+                  activation: str = "silu", keep: bool = False):
+    """(y [n, outputs], what the backward needs or None)."""
+    x, gate, up, down = (_dense_last(t) for t in (x, gate, up, down))
+    desc = _gated_desc(x, gate, up, down, activation)
+    y = torch.empty((x.shape[0], down.shape[0]), dtype=x.dtype, device=x.device)
+    saved = None
+    if keep:
+        saved = torch.empty(_sizeq(lib().rhip_gated_saved_bytes, ctypes.byref(desc)),
+                            dtype=torch.uint8, device=x.device)
+    ws = torch.empty(_sizeq(lib().rhip_gated_workspace_bytes, ctypes.byref(desc),
+                            GATED_FORWARD if keep else GATED_INFERENCE),
+                     dtype=torch.uint8, device=x.device)
+    _check(lib().rhip_gated_forward(ctypes.byref(desc), _ptr(y), _ptr(saved),
+                                    0 if saved is None else saved.numel(), _ptr(ws), ws.numel(),
+                                    _stream(x.device)), "rhip_gated_forward")
+    return y, saved
+
+
+def gated_backward(grad_y: torch.Tensor, x: torch.Tensor, gate: torch.Tensor, up: torch.Tensor,
+                   down: torch.Tensor, saved: torch.Tensor, activation: str = "silu"):
+    """(grad_x, grad_gate, grad_up, grad_down) from the forward's saved buffer."""
+    x, gate, up, down = (_dense_last(t) for t in (x, gate, up, down))
+    grad_y = _dense_last(grad_y.to(x.dtype))
+    desc = _gated_desc(x, gate, up, down, activation, grad_y)
+    if saved.device != x.device or saved.dtype != torch.uint8 or not saved.is_contiguous():
+        raise RuntimeError("saved must be the forward's buffer on the rows' device")
+    grads = [torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (x, gate, up, down)]
+    ws = torch.empty(_sizeq(lib().rhip_gated_workspace_bytes, ctypes.byref(desc),
+                            GATED_BACKWARD), dtype=torch.uint8, device=x.device)
+    _check(lib().rhip_gated_backward(ctypes.byref(desc), _ptr(saved), saved.numel(),
+                                     *(_ptr(g) for g in grads), _ptr(ws), ws.numel(),
+                                     _stream(x.device)), "rhip_gated_backward")
+    return tuple(grads)

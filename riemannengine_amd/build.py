@@ -30,6 +30,7 @@ HIPCC = os.path.join(ROCM, "bin", "hipcc")
 HIP_SOURCES = ["abi.hip", "sort.hip", "hash.hip", "kmap.hip", "conv.hip", "conv_thin.hip",
                "conv_x3.hip", "conv_pad.hip", "conv_small.hip",
                "pool.hip", "norm.hip", "layer_norm.hip", "embed.hip",
+               "rotary.hip", "gated.hip",
                "attn.hip", "attn_fwd.hip", "attn_bwd.hip"]
 # gfx950 only. Packed-FP32 instructions are disabled: the compiler would
 # otherwise form v_pk_* FP32 ops from plain float code.
@@ -41,7 +42,8 @@ HIP_FLAGS = [
 
 # Of single sources: the attention kernels' loads into LDS name m0 as clobbered,
 # a reserved register, which would be a warning each.
-SOURCE_FLAGS = {src: ["-Wno-inline-asm"] for src in ("attn.hip", "attn_fwd.hip", "attn_bwd.hip")}
+SOURCE_FLAGS = {src: ["-Wno-inline-asm"] for src in ("attn.hip", "attn_fwd.hip", "attn_bwd.hip",
+                                                      "gated.hip")}
 
 
 def _run(cmd: list[str]) -> None:
@@ -53,7 +55,7 @@ def _run(cmd: list[str]) -> None:
         print(out)
 
 
-def build_hip(jobs: int = 4) -> str:
+def build_hip(jobs: int = 8) -> str:
     """Compile the HIP kernels and link libriemann_hip.so; returns its path."""
     if not os.path.exists(HIPCC):
         raise RuntimeError(f"hipcc not found at {HIPCC}")

@@ -1,0 +1,864 @@
+// Gated feed-forward block on gfx950, forward and backward:
+//   g = x gate^T, u = x up^T, h = act(g) u, y = h down^T.
+// One kernel makes both projections of a tile, the activation and the product:
+// its workgroups' tiles hold the same columns of g and u, so h (and for the
+// backward g and u) leave from registers. Backward, with dh = dy down:
+//   dg = dh u act'(g), du = dh act(g)      in the epilogue of that product,
+//   dx = dg gate + du up                   one product over 2 H,
+//   dgate = dg^T x, dup = du^T x           one launch,
+//   ddown = dy^T h.
+//
+// All are tiles of gemm_device.hpp's product; sums over a long k with few tiles
+// are split over workgroups, whose fp32 sums a second kernel adds in order and
+// finishes. Up to 64 rows (single tokens) a kernel that streams the weights
+// through registers takes the forward: it is bound by their bytes.
+//
+// Operands that do not hold aligned, whole 16-byte chunks (odd widths,
+// unaligned views) are laid out once per call in the workspace, zeros behind
+// their rows' ends.
+//
+// bf16: h, dg and du are rounded to bf16, as operands of the matrix cores. g and
+// u are kept for the backward to 16 significant bits (a bf16 plane each, the
+// next eight bits of both in a third), so that they add nothing to that.
+#include <climits>
+#include <type_traits>
+
+#include "gemm_device.hpp"
+
+namespace rhip {
+namespace {
+
+constexpr int kGatedMaxRows = 64; // of the kernel for few rows
+
+// ------------------------------------------------------------- activation
+
+__device__ __forceinline__ float act_exp(float v, __bf16) { return exp2_fast(v * kLog2e); }
+__device__ __forceinline__ float act_exp(float v, float) { return expf(v); }
+__device__ __forceinline__ float act_inv(float v, __bf16) { return __builtin_amdgcn_rcpf(v); }
+__device__ __forceinline__ float act_inv(float v, float) { return 1.f / v; }
+
+// The activation and its derivative at g, as exact as T's results need.
+template <typename T>
+__device__ __forceinline__ float activation(int32_t kind, float g, float &derivative) {
+  if (kind == RHIP_ACT_SILU) {
+    const float s = act_inv(1.f + act_exp(-g, T{}), T{});
+    derivative = s * fmaf(g, 1.f - s, 1.f);
+    return g * s;
+  }
+  const float half = 0.5f * erfcf(g * -0.70710678118654752f);
+  derivative = fmaf(g * 0.39894228040143268f, act_exp(-0.5f * g * g, T{}), half);
+  return g * half;
+}
+
+// g and u for the backward: fp32 as they are; bf16 the upper 24 bits, rounded.
+__device__ __forceinline__ uint32_t upper24(float v) {
+  const uint32_t b = __float_as_uint(v);
+  return (v != v ? b : b + 0x80u) >> 8;
+}
+
+struct GatedSaved { // planes [n, pitch]
+  void *h, *g, *u;
+  uint16_t *low; // bf16: the eight bits behind g's and u's planes
+};
+
+template <typename T>
+__device__ __forceinline__ void load_saved(const GatedSaved &s, int64_t at, float (&g)[4],
+                                           float (&u)[4]) {
+  if constexpr (sizeof(T) == 4) {
+    const v4f a = *reinterpret_cast<const v4f *>(static_cast<const float *>(s.g) + at);
+    const v4f b = *reinterpret_cast<const v4f *>(static_cast<const float *>(s.u) + at);
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      g[i] = a[i], u[i] = b[i];
+  } else {
+    uint16_t a[4], b[4], c[4];
+    __builtin_memcpy(a, __builtin_assume_aligned(static_cast<const uint16_t *>(s.g) + at, 8), 8);
+    __builtin_memcpy(b, __builtin_assume_aligned(static_cast<const uint16_t *>(s.u) + at, 8), 8);
+    __builtin_memcpy(c, __builtin_assume_aligned(s.low + at, 8), 8);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      g[i] = __uint_as_float(static_cast<uint32_t>(a[i]) << 16 | (c[i] & 0xff) << 8);
+      u[i] = __uint_as_float(static_cast<uint32_t>(b[i]) << 16 | (c[i] & 0xff00));
+    }
+  }
+}
+
+// ---------------------------------------------------------------- products
+
+enum GatedStage {
+  kProject,  // h (and the saved planes) from x, gate, up
+  kPlain,    // one matrix of results
+  kHidden,   // dg, du from dy, down and the saved planes
+  kPartial   // fp32 sums of a part of k
+};
+
+struct GatedArgs {
+  GemmSide y, x;
+  int32_t tiles_i, tiles_j, layers, splits, k_tiles; // layers: splits times `outs`
+  int32_t outs;                                      // results, each with its own y matrix
+  int32_t rows, cols;                                // of the results
+  void *out[2];
+  int64_t out_row;
+  float *part; // [splits * outs][halves][rows, part_row]
+  int64_t part_row;
+  GatedSaved saved;
+  int64_t pitch; // of h's, dg's, du's and the saved planes' rows
+  void *dg, *du;
+  int32_t keep; // kProject: whether to write the saved planes
+  int32_t kind; // activation
+};
+
+template <typename T, int NI, int NJ, bool YACROSS, bool XACROSS, GemmPair PAIR, GatedStage STAGE>
+__global__ __launch_bounds__(kGemmThreads, (NI * NJ > 4 ? 1 : 2)) void
+gated_product_kernel(GatedArgs a) {
+  using P = Gemm<T, NI, NJ, YACROSS, XACROSS, PAIR>;
+  __shared__ alignas(16) char lds[P::kLds];
+  int32_t ti, tj, layer;
+  if (!gemm_tile(a.tiles_i, a.tiles_j, a.layers, ti, tj, layer))
+    return;
+  const int32_t split = layer / a.outs, which = layer - split * a.outs;
+  constexpr int kHalf = PAIR == kGemmHalves ? 2 : 1;
+  const int32_t i0 = ti * P::BI, j0 = tj * (P::BJ / kHalf);
+  const int32_t per = (a.k_tiles + a.splits - 1) / a.splits;
+  const int32_t kt0 = min(split * per, a.k_tiles), kt1 = min(kt0 + per, a.k_tiles);
+  v16f acc[NJ][NI];
+  P::run(lds, a.y, static_cast<const T *>(a.y.p[which]), a.x, i0, j0, kt0, kt1, acc);
+
+  const int w = wave_uniform(threadIdx.x / kWave), half = lane_id() >> 5;
+  constexpr int NB = NJ / kHalf; // blocks of columns of a wave
+  const int32_t col0 = j0 + (w % 2) * NB * 32;
+  char *strip = lds + w * (P::kLds / 4);
+  // the columns behind the last, which fill h's rows to whole chunks, are zeros
+  if ((STAGE == kProject || STAGE == kHidden) && col0 + NB * 32 > a.cols) {
+    rare_path();
+#pragma unroll
+    for (int c = 0; c < NJ; ++c)
+#pragma unroll
+      for (int r = 0; r < 16; ++r)
+        if (col0 + c % NB * 32 + block_row(r) + 4 * half >= a.cols) {
+#pragma unroll
+          for (int b = 0; b < NI; ++b)
+            acc[c][b][r] = 0.f;
+        }
+  }
+#pragma unroll
+  for (int b = 0; b < NI; ++b) {
+    const int32_t row0 = i0 + ((w / 2) * NI + b) * 32;
+    const int32_t rows = a.rows - row0, mine = row0 + (lane_id() & 31);
+    const int64_t at = row0 * a.pitch + col0;
+    if constexpr (STAGE == kProject) {
+      const int32_t cols = static_cast<int32_t>(a.pitch) - col0;
+      using S = GemmStrip<T, NB>;
+      auto g = [&](int c, int r) { return acc[c][b][r]; };
+      auto u = [&](int c, int r) { return acc[c + NB][b][r]; };
+      S::store(strip, static_cast<T *>(a.saved.h) + at, a.pitch, rows, cols, [&](int c, int r) {
+        float d;
+        return from_f32<T>(activation<T>(a.kind, g(c, r), d) * u(c, r));
+      });
+      if (a.keep) {
+        if constexpr (sizeof(T) == 4) {
+          S::store(strip, static_cast<float *>(a.saved.g) + at, a.pitch, rows, cols, g);
+          S::store(strip, static_cast<float *>(a.saved.u) + at, a.pitch, rows, cols, u);
+        } else {
+          using B = GemmStrip<uint16_t, NB>;
+          B::store(strip, static_cast<uint16_t *>(a.saved.g) + at, a.pitch, rows, cols,
+                   [&](int c, int r) { return static_cast<uint16_t>(upper24(g(c, r)) >> 8); });
+          B::store(strip, static_cast<uint16_t *>(a.saved.u) + at, a.pitch, rows, cols,
+                   [&](int c, int r) { return static_cast<uint16_t>(upper24(u(c, r)) >> 8); });
+          B::store(strip, a.saved.low + at, a.pitch, rows, cols, [&](int c, int r) {
+            return static_cast<uint16_t>((upper24(g(c, r)) & 0xff) |
+                                         (upper24(u(c, r)) & 0xff) << 8);
+          });
+        }
+      }
+    } else if constexpr (STAGE == kPlain) {
+      GemmStrip<T, NB>::store(
+          strip, static_cast<T *>(a.out[which]) + row0 * a.out_row + col0, a.out_row, rows,
+          a.cols - col0, [&](int c, int r) { return from_f32<T>(acc[c][b][r]); });
+    } else if constexpr (STAGE == kHidden) {
+      const int32_t cols = static_cast<int32_t>(a.pitch) - col0;
+#pragma unroll
+      for (int c = 0; c < NB; ++c)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          const int32_t col = 32 * c + 8 * q + 4 * half;
+          float g[4] = {0.f, 0.f, 0.f, 0.f}, u[4] = {0.f, 0.f, 0.f, 0.f};
+          if (mine < a.rows && col < cols)
+            load_saved<T>(a.saved, mine * a.pitch + col0 + col, g, u);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            float d;
+            const float dh = acc[c][b][4 * q + e], v = activation<T>(a.kind, g[e], d);
+            acc[c][b][4 * q + e] = dh * v;
+            g[e] = dh * u[e] * d;
+          }
+          T e4[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            e4[e] = from_f32<T>(g[e]);
+          __builtin_memcpy(__builtin_assume_aligned(strip + (lane_id() & 31) *
+                                                                GemmStrip<T, NB>::kPitch +
+                                                        col * sizeof(T),
+                                                    4 * sizeof(T)),
+                           e4, sizeof(e4));
+        }
+      GemmStrip<T, NB>::flush(strip, static_cast<T *>(a.dg) + at, a.pitch, rows, cols);
+      GemmStrip<T, NB>::store(strip, static_cast<T *>(a.du) + at, a.pitch, rows, cols,
+                              [&](int c, int r) { return from_f32<T>(acc[c][b][r]); });
+    } else {
+      float *to = a.part + static_cast<int64_t>(layer) * kHalf * a.rows * a.part_row +
+                  row0 * a.part_row + col0;
+#pragma unroll
+      for (int h = 0; h < kHalf; ++h)
+        GemmStrip<float, NB>::store(
+            strip, to + h * a.rows * a.part_row, a.part_row, rows,
+            static_cast<int32_t>(a.part_row) - col0,
+            [&](int c, int r) { return acc[c + h * NB][b][r]; });
+    }
+  }
+}
+
+// Adds the splits' sums and finishes them as the products' own epilogues do:
+// four columns a thread (part_row is a multiple of four).
+template <typename T, GatedStage STAGE>
+__global__ __launch_bounds__(kGemmThreads) void gated_join_kernel(GatedArgs a) {
+  const int64_t quads = a.part_row / 4, total = quads * a.rows;
+  const int64_t q = static_cast<int64_t>(blockIdx.x) * kGemmThreads + threadIdx.x;
+  const int which = blockIdx.y;
+  if (q >= total)
+    return;
+  const int64_t row = q / quads, col = (q - row * quads) * 4;
+  constexpr int kHalf = STAGE == kProject ? 2 : 1;
+  const int64_t plane = static_cast<int64_t>(a.rows) * a.part_row;
+  v4f s[kHalf];
+#pragma unroll
+  for (int h = 0; h < kHalf; ++h)
+    s[h] = v4f{0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+  for (int p = 0; p < a.splits; ++p)
+#pragma unroll
+    for (int h = 0; h < kHalf; ++h)
+      s[h] += *reinterpret_cast<const v4f *>(
+          a.part + ((static_cast<int64_t>(p) * a.outs + which) * kHalf + h) * plane +
+          row * a.part_row + col);
+  auto put = [&](T *to, const float (&v)[4], int64_t cols) {
+    T e[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      e[i] = from_f32<T>(v[i]);
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (col + i < cols)
+        to[i] = e[i];
+  };
+  if constexpr (STAGE == kPlain) {
+    const float v[4] = {s[0][0], s[0][1], s[0][2], s[0][3]};
+    put(static_cast<T *>(a.out[which]) + row * a.out_row + col, v, a.cols);
+    return;
+  }
+  const int64_t at = row * a.pitch + col;
+  float v[4], w[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    if (col + i >= a.cols)
+      s[0][i] = s[kHalf - 1][i] = 0.f;
+  if constexpr (STAGE == kProject) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      float d;
+      v[i] = activation<T>(a.kind, s[0][i], d) * s[kHalf - 1][i];
+    }
+    put(static_cast<T *>(a.saved.h) + at, v, a.pitch);
+    if (a.keep) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float g = s[0][i], u = s[kHalf - 1][i];
+        if constexpr (sizeof(T) == 4) {
+          static_cast<float *>(a.saved.g)[at + i] = g;
+          static_cast<float *>(a.saved.u)[at + i] = u;
+        } else {
+          static_cast<uint16_t *>(a.saved.g)[at + i] = upper24(g) >> 8;
+          static_cast<uint16_t *>(a.saved.u)[at + i] = upper24(u) >> 8;
+          a.saved.low[at + i] = (upper24(g) & 0xff) | (upper24(u) & 0xff) << 8;
+        }
+      }
+    }
+  } else {
+    float g[4], u[4];
+    load_saved<T>(a.saved, at, g, u);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      float d;
+      const float act = activation<T>(a.kind, g[i], d);
+      v[i] = s[0][i] * u[i] * d;
+      w[i] = s[0][i] * act;
+    }
+    put(static_cast<T *>(a.dg) + at, v, a.pitch);
+    put(static_cast<T *>(a.du) + at, w, a.pitch);
+  }
+}
+
+// rows of `cols` elements at p, row stride `row`, as rows of `pitch` elements
+// (whole 16-byte chunks), zeros behind `cols`.
+template <typename T>
+__global__ __launch_bounds__(kGemmThreads) void gated_pack_kernel(const T *p, int64_t row,
+                                                                  int32_t rows, int32_t cols,
+                                                                  T *out, int32_t pitch) {
+  using K = RowChunk<T>;
+  const int32_t chunks = pitch / K::V;
+  for (int64_t q = static_cast<int64_t>(blockIdx.x) * kGemmThreads + threadIdx.x;
+       q < static_cast<int64_t>(rows) * chunks;
+       q += static_cast<int64_t>(gridDim.x) * kGemmThreads) {
+    const int64_t r = q / chunks;
+    const int32_t c = static_cast<int32_t>(q - r * chunks) * K::V;
+    *reinterpret_cast<v4u *>(out + r * pitch + c) = K::fetch(p + r * row + c, cols - c, false);
+  }
+}
+
+// ---------------------------------------------------------------- few rows
+
+// Up to 16 TB rows: a workgroup's eight waves share 16 columns (of g and u, or of
+// y) and part k among them; weights go from memory to registers and the matrix
+// cores as they come, 64 bytes of 16 rows to a load. The waves' sums are added
+// in LDS in order.
+constexpr int kFewThreads = 512;
+constexpr int kFewWaves = kFewThreads / kWave;
+struct FewArgs {
+  const void *y, *x[2]; // rows [n, k] and weights [cols, k]
+  int64_t y_row, x_row[2];
+  int32_t n, k, cols;
+  void *out; // kPlain: [n, cols]
+  int64_t out_row;
+  GatedSaved saved;
+  int64_t pitch;
+  int32_t keep, kind;
+};
+
+template <typename T, int TB, bool GATE>
+__global__ __launch_bounds__(kFewThreads) void gated_few_kernel(FewArgs a) {
+  using M = Mfma<T>;
+  using K = RowChunk<T>;
+  constexpr int N = GATE ? 2 : 1, E = K::V;
+  constexpr int kOuts = 256 * TB * N; // results of a workgroup
+  __shared__ float sums[kFewWaves][kOuts];
+  const int lane = lane_id(), w = wave_uniform(threadIdx.x / kWave);
+  const int32_t col0 = blockIdx.x * 16;
+  const int32_t steps = (a.k + M::kCh - 1) / M::kCh;
+  const int32_t per = (steps + kFewWaves - 1) / kFewWaves;
+  const int32_t s0 = min(w * per, steps), s1 = min(s0 + per, steps);
+  const int r = lane & 15, at = (lane >> 4) * E;
+  const T *xp[N], *yp[TB];
+#pragma unroll
+  for (int i = 0; i < N; ++i)
+    xp[i] = static_cast<const T *>(a.x[i]) + min(col0 + r, a.cols - 1) * a.x_row[i] + at;
+#pragma unroll
+  for (int b = 0; b < TB; ++b)
+    yp[b] = static_cast<const T *>(a.y) + min(16 * b + r, a.n - 1) * a.y_row + at;
+  v4f acc[N][TB];
+#pragma unroll
+  for (int i = 0; i < N; ++i)
+#pragma unroll
+    for (int b = 0; b < TB; ++b)
+      acc[i][b] = v4f{0.f, 0.f, 0.f, 0.f};
+  auto step = [&](int32_t k, auto turns, auto whole) {
+    constexpr int U = decltype(turns)::value;
+    v4u x[U][N], y[U][TB];
+    auto load = [&](const T *p, int32_t at_k) {
+      return decltype(whole)::value ? K::raw(p + at_k) : K::fetch(p + at_k, a.k - at_k - at, false);
+    };
+#pragma unroll
+    for (int t = 0; t < U; ++t) {
+#pragma unroll
+      for (int i = 0; i < N; ++i)
+        x[t][i] = load(xp[i], k + t * M::kCh);
+#pragma unroll
+      for (int b = 0; b < TB; ++b)
+        y[t][b] = load(yp[b], k + t * M::kCh);
+    }
+#pragma unroll
+    for (int t = 0; t < U; ++t)
+#pragma unroll
+      for (int i = 0; i < N; ++i)
+#pragma unroll
+        for (int b = 0; b < TB; ++b)
+          M::mma(__builtin_bit_cast(typename M::Frag, x[t][i]),
+                 __builtin_bit_cast(typename M::Frag, y[t][b]), acc[i][b]);
+  };
+  constexpr int kTurns = 4; // steps whose loads are in flight together
+  using One = std::integral_constant<int, 1>;
+  const int32_t full = min(s1, a.k / M::kCh); // steps with whole chunks
+  int32_t s = s0;
+  for (; s + kTurns <= full; s += kTurns)
+    step(s * M::kCh, std::integral_constant<int, kTurns>{}, std::true_type{});
+  for (; s < full; ++s)
+    step(s * M::kCh, One{}, std::true_type{});
+  for (; s < s1; ++s)
+    step(s * M::kCh, One{}, std::false_type{});
+  // entry e: column 4 (lane / 16) + e, row lane % 16 of block b
+#pragma unroll
+  for (int i = 0; i < N; ++i)
+#pragma unroll
+    for (int b = 0; b < TB; ++b)
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        sums[w][((b * 16 + r) * N + i) * 16 + 4 * (lane >> 4) + e] = acc[i][b][e];
+  __syncthreads();
+  for (int o = threadIdx.x; o < 256 * TB; o += kFewThreads) {
+    const int32_t row = o / 16, c = o % 16, col = col0 + c;
+    if (row >= a.n)
+      break;
+    float v[N];
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      v[i] = 0.f;
+#pragma unroll
+      for (int p = 0; p < kFewWaves; ++p)
+        v[i] += sums[p][(row * N + i) * 16 + c];
+    }
+    if constexpr (GATE) {
+      if (col >= a.pitch)
+        continue;
+      if (col >= a.cols) // the columns behind the last are zeros
+        v[0] = v[N - 1] = 0.f;
+      const int64_t to = row * a.pitch + col;
+      float d;
+      static_cast<T *>(a.saved.h)[to] = from_f32<T>(activation<T>(a.kind, v[0], d) * v[N - 1]);
+      if (a.keep) {
+        if constexpr (sizeof(T) == 4) {
+          static_cast<float *>(a.saved.g)[to] = v[0];
+          static_cast<float *>(a.saved.u)[to] = v[N - 1];
+        } else {
+          const uint32_t g = upper24(v[0]), u = upper24(v[N - 1]);
+          static_cast<uint16_t *>(a.saved.g)[to] = g >> 8;
+          static_cast<uint16_t *>(a.saved.u)[to] = u >> 8;
+          a.saved.low[to] = (g & 0xff) | (u & 0xff) << 8;
+        }
+      }
+    } else if (col < a.cols) {
+      static_cast<T *>(a.out)[row * a.out_row + col] = from_f32<T>(v[0]);
+    }
+  }
+}
+
+// ------------------------------------------------------------------ host
+
+void check_gated(const rhip_gated *d) {
+  RHIP_CHECK_ARG(d != nullptr, "descriptor is null");
+  if (d->dtype != RHIP_F32 && d->dtype != RHIP_BF16)
+    throw Error(RHIP_ERR_UNSUPPORTED, "dtype must be RHIP_F32 or RHIP_BF16");
+  RHIP_CHECK_ARG(d->n >= 0 && d->channels >= 1 && d->hidden >= 1 && d->outputs >= 1, "bad sizes");
+  if (d->n > INT32_MAX - 256 || d->channels > kGemmMaxRow || d->hidden > kGemmMaxRow ||
+      d->outputs > kGemmMaxRow)
+    throw Error(RHIP_ERR_UNSUPPORTED,
+                "at most 2^31 - 257 rows and 2^20 channels, hidden channels and outputs");
+  RHIP_CHECK_ARG(d->activation == RHIP_ACT_SILU || d->activation == RHIP_ACT_GELU,
+                 "activation must be one of RHIP_ACT_");
+  RHIP_CHECK_ARG((d->n == 0 || d->x) && d->gate && d->up && d->down,
+                 "x, gate, up and down are required");
+}
+
+int64_t chunk_elements(int32_t dtype) { return dtype == RHIP_F32 ? 4 : 8; }
+int64_t whole_chunks(int64_t n, int32_t dtype) {
+  return static_cast<int64_t>(align_up(static_cast<size_t>(n), chunk_elements(dtype)));
+}
+size_t element_bytes(int32_t dtype) { return dtype == RHIP_F32 ? 4 : 2; }
+
+// A matrix as the products take it: itself, or a copy in the workspace.
+struct Packed {
+  const void *src;
+  int64_t src_row;
+  int32_t rows, cols;
+  bool copied;
+  void *copy;
+  const void *p;
+  int64_t row; // of p
+};
+Packed plan_pack(Carve &cv, const void *p, int64_t row, int64_t rows, int64_t cols,
+                 int32_t dtype) {
+  const int64_t e = chunk_elements(dtype);
+  Packed m{p, row, static_cast<int32_t>(rows), static_cast<int32_t>(cols), false, nullptr, p, row};
+  // (a single row's stride does not matter, and may be anything)
+  if (!aligned16(p) || cols % e != 0 || (rows > 1 && (row % e != 0 || row < cols || row > kGemmMaxRow))) {
+    m.copied = true;
+    m.row = whole_chunks(cols, dtype);
+    m.copy = cv.take<char>(static_cast<size_t>(std::max<int64_t>(rows, 1)) * m.row *
+                           element_bytes(dtype));
+    m.p = m.copy;
+  } else if (rows <= 1) {
+    m.row = cols;
+  }
+  return m;
+}
+template <typename T> void run_pack(const Packed &m, hipStream_t stream) {
+  if (!m.copied || m.rows == 0)
+    return;
+  const int64_t chunks = m.rows * (m.row / RowChunk<T>::V);
+  hipLaunchKernelGGL((gated_pack_kernel<T>),
+                     dim3(static_cast<unsigned>(
+                         std::min<int64_t>(ceil_div(chunks, kGemmThreads), 1 << 20))),
+                     dim3(kGemmThreads), 0, stream, static_cast<const T *>(m.src), m.src_row,
+                     m.rows, m.cols, static_cast<T *>(m.copy), static_cast<int32_t>(m.row));
+  RHIP_LAUNCH_CHECK();
+}
+
+// The tiles and splits of a product by estimated time: 256x256 tiles, one
+// workgroup to a CU, or 128x128 ones, two, in rounds over the 256 CUs.
+struct ProductPlan {
+  bool large;
+  int32_t splits;
+  size_t part; // floats of the splits' sums
+};
+constexpr int64_t kMostParts = int64_t(64) << 20; // floats, of all splits
+ProductPlan plan_product(int64_t rows, int64_t cols, int64_t k_tiles, int64_t outs, bool halves,
+                         int32_t dtype) {
+  const int64_t part_row = static_cast<int64_t>(align_up(static_cast<size_t>(cols), 4));
+  const int64_t plane = rows * part_row * outs * (halves ? 2 : 1);
+  ProductPlan best{};
+  double least = 0.0;
+  for (const bool large : {true, false}) {
+    const int64_t bi = large ? 256 : 128, bj = bi / (halves ? 2 : 1);
+    const int64_t tiles = ceil_div(rows, bi) * ceil_div(cols, bj) * outs;
+    const double slots = large ? 256.0 : 512.0;
+    const double turn = (large ? 2.0 : 1.35) * (dtype == RHIP_F32 ? 4.2 : 1.0); // us a tile of k
+    for (int64_t s = 1; s <= 64; s *= 2) {
+      if (s > 1 && (k_tiles < 4 * s || plane * s > kMostParts))
+        break;
+      const double rounds = std::ceil(static_cast<double>(tiles * s) / slots);
+      // a round that does not fill the chip runs faster: less to share
+      const double fill = std::min(1.0, static_cast<double>(tiles * s) / slots);
+      double t = rounds * (3.0 + static_cast<double>(ceil_div(k_tiles, s)) * turn *
+                                     (0.75 + 0.25 * fill));
+      if (s > 1)
+        t += 4.0 + static_cast<double>(plane) * (s + 1) * 4.0 / 4.0e6;
+      if (least == 0.0 || t < least) {
+        least = t;
+        best = {large, static_cast<int32_t>(s), s > 1 ? static_cast<size_t>(plane * s) : 0};
+      }
+    }
+  }
+  return best;
+}
+
+// Launches a product of the given stage, and what joins its splits.
+template <typename T, bool YACROSS, bool XACROSS, GemmPair PAIR, GatedStage STAGE>
+void run_product(GatedArgs a, const ProductPlan &plan, float *part, hipStream_t stream) {
+  if (a.rows == 0)
+    return;
+  constexpr int kHalf = PAIR == kGemmHalves ? 2 : 1;
+  a.splits = plan.splits;
+  a.layers = plan.splits * a.outs;
+  a.part = part;
+  // h, dg and du have zeros behind the last column, up to their pitch
+  a.part_row = STAGE == kPlain ? static_cast<int64_t>(align_up(static_cast<size_t>(a.cols), 4))
+                               : a.pitch;
+  auto launch = [&](auto n, auto stage) {
+    constexpr int N = decltype(n)::value;
+    constexpr GatedStage S = static_cast<GatedStage>(decltype(stage)::value);
+    a.tiles_i = static_cast<int32_t>(ceil_div(a.rows, 64 * N));
+    a.tiles_j = static_cast<int32_t>(ceil_div(a.cols, 64 * N / kHalf));
+    const int64_t tiles = static_cast<int64_t>(a.tiles_i) * a.tiles_j * a.layers;
+    if (gemm_grid(tiles) > max_groups(kGemmThreads))
+      throw Error(RHIP_ERR_UNSUPPORTED, "too many tiles");
+    hipLaunchKernelGGL((gated_product_kernel<T, N, N, YACROSS, XACROSS, PAIR, S>),
+                       dim3(static_cast<unsigned>(gemm_grid(tiles))), dim3(kGemmThreads), 0,
+                       stream, a);
+    RHIP_LAUNCH_CHECK();
+  };
+  auto sized = [&](auto stage) {
+    if (plan.large)
+      launch(std::integral_constant<int, 4>{}, stage);
+    else
+      launch(std::integral_constant<int, 2>{}, stage);
+  };
+  if (plan.splits == 1) {
+    sized(std::integral_constant<int, STAGE>{});
+    return;
+  }
+  sized(std::integral_constant<int, kPartial>{});
+  const int64_t quads = a.part_row / 4 * a.rows; // of at most kMostParts / 4
+  hipLaunchKernelGGL((gated_join_kernel<T, STAGE>),
+                     dim3(static_cast<unsigned>(ceil_div(quads, kGemmThreads)), a.outs),
+                     dim3(kGemmThreads), 0, stream, a);
+  RHIP_LAUNCH_CHECK();
+}
+
+GemmSide side(const Packed &m, bool across, const Packed *second = nullptr) {
+  GemmSide s{};
+  s.p[0] = m.p, s.p[1] = second ? second->p : m.p;
+  s.row = m.row;
+  // along its rows a matrix is whole chunks
+  const int32_t wide = m.copied ? static_cast<int32_t>(m.row) : m.cols;
+  s.idx = across ? wide : m.rows;
+  s.k = across ? m.rows : wide;
+  return s;
+}
+GemmSide side(const void *p, const void *second, int32_t rows, int64_t pitch, bool across) {
+  GemmSide s{};
+  s.p[0] = p, s.p[1] = second;
+  s.row = pitch;
+  s.idx = across ? static_cast<int32_t>(pitch) : rows;
+  s.k = across ? rows : static_cast<int32_t>(pitch);
+  return s;
+}
+
+// gate and up as one pair of matrices with one row stride
+void pack_pair(Carve &cv, const rhip_gated *d, Packed &gate, Packed &up) {
+  Carve dry(nullptr, 0);
+  gate = plan_pack(dry, d->gate, d->gate_row, d->hidden, d->channels, d->dtype);
+  up = plan_pack(dry, d->up, d->up_row, d->hidden, d->channels, d->dtype);
+  const bool copy = gate.copied || up.copied || gate.row != up.row;
+  for (auto *m : {&gate, &up}) {
+    if (copy) {
+      m->copied = true;
+      m->row = whole_chunks(d->channels, d->dtype);
+      m->copy = cv.take<char>(static_cast<size_t>(d->hidden) * m->row * element_bytes(d->dtype));
+      m->p = m->copy;
+    }
+  }
+}
+
+GatedSaved carve_saved(Carve &cv, const rhip_gated *d, int64_t pitch, bool keep) {
+  GatedSaved s{};
+  const size_t n = static_cast<size_t>(std::max<int64_t>(d->n, 1)) * pitch;
+  s.h = cv.take<char>(n * element_bytes(d->dtype));
+  if (keep) {
+    s.g = cv.take<char>(n * element_bytes(d->dtype));
+    s.u = cv.take<char>(n * element_bytes(d->dtype));
+    if (d->dtype == RHIP_BF16)
+      s.low = cv.take<uint16_t>(n);
+  }
+  return s;
+}
+
+struct GatedForward {
+  Packed x, gate, up, down;
+  GatedSaved saved; // without a saved buffer: h alone
+  ProductPlan project, out;
+  float *part;
+};
+GatedForward plan_forward(Carve &cv, const rhip_gated *d, bool keep) {
+  GatedForward f{};
+  const int64_t pitch = whole_chunks(d->hidden, d->dtype);
+  if (!keep)
+    f.saved = carve_saved(cv, d, pitch, false);
+  if (d->n <= kGatedMaxRows)
+    return f;
+  f.x = plan_pack(cv, d->x, d->x_row, d->n, d->channels, d->dtype);
+  pack_pair(cv, d, f.gate, f.up);
+  f.down = plan_pack(cv, d->down, d->down_row, d->outputs, d->hidden, d->dtype);
+  const int64_t bk = kGemmTileBytes / static_cast<int64_t>(element_bytes(d->dtype));
+  f.project = plan_product(d->n, pitch, ceil_div(d->channels, bk), 1, true, d->dtype);
+  f.out = plan_product(d->n, d->outputs, ceil_div(pitch, bk), 1, false, d->dtype);
+  f.part = cv.take<float>(std::max(f.project.part, f.out.part));
+  return f;
+}
+
+struct GatedBackward {
+  Packed x, gate, up, down, gy;
+  void *dg, *du;
+  ProductPlan hidden, gx, gw, gd;
+  float *part;
+};
+GatedBackward plan_backward(Carve &cv, const rhip_gated *d) {
+  GatedBackward b{};
+  const int64_t pitch = whole_chunks(d->hidden, d->dtype);
+  b.x = plan_pack(cv, d->x, d->x_row, d->n, d->channels, d->dtype);
+  pack_pair(cv, d, b.gate, b.up);
+  b.down = plan_pack(cv, d->down, d->down_row, d->outputs, d->hidden, d->dtype);
+  b.gy = plan_pack(cv, d->grad_y, d->grad_y_row, d->n, d->outputs, d->dtype);
+  const size_t n = static_cast<size_t>(std::max<int64_t>(d->n, 1)) * pitch;
+  b.dg = cv.take<char>(n * element_bytes(d->dtype));
+  b.du = cv.take<char>(n * element_bytes(d->dtype));
+  const int64_t bk = kGemmTileBytes / static_cast<int64_t>(element_bytes(d->dtype));
+  const int64_t kn = ceil_div(d->n, bk);
+  b.hidden = plan_product(d->n, pitch, ceil_div(d->outputs, bk), 1, false, d->dtype);
+  b.gx = plan_product(d->n, d->channels, 2 * ceil_div(d->hidden, bk), 1, false, d->dtype);
+  b.gw = plan_product(d->hidden, d->channels, kn, 2, false, d->dtype);
+  b.gd = plan_product(d->outputs, d->hidden, kn, 1, false, d->dtype);
+  b.part = cv.take<float>(std::max({b.hidden.part, b.gx.part, b.gw.part, b.gd.part}));
+  return b;
+}
+
+template <typename F> void with_type(int32_t dtype, F &&f) {
+  if (dtype == RHIP_F32)
+    f(float{});
+  else
+    f(__bf16{});
+}
+
+GatedArgs gated_args(const rhip_gated *d, const GatedSaved &saved) {
+  GatedArgs a{};
+  a.outs = 1;
+  a.saved = saved;
+  a.pitch = whole_chunks(d->hidden, d->dtype);
+  a.kind = d->activation;
+  return a;
+}
+
+template <typename T, bool GATE> void run_few(const FewArgs &f, hipStream_t stream) {
+  const int64_t cols = GATE ? f.pitch : f.cols;
+  auto launch = [&](auto tb) {
+    hipLaunchKernelGGL((gated_few_kernel<T, decltype(tb)::value, GATE>),
+                       dim3(static_cast<unsigned>(ceil_div(cols, 16))), dim3(kFewThreads), 0,
+                       stream, f);
+    RHIP_LAUNCH_CHECK();
+  };
+  if (f.n <= 16)
+    launch(std::integral_constant<int, 1>{});
+  else if (f.n <= 32)
+    launch(std::integral_constant<int, 2>{});
+  else
+    launch(std::integral_constant<int, 4>{});
+}
+
+} // namespace
+} // namespace rhip
+
+using namespace rhip;
+
+extern "C" int rhip_gated_saved_bytes(const rhip_gated *gated, size_t *bytes) {
+  return guarded([&] {
+    check_gated(gated);
+    RHIP_CHECK_ARG(bytes != nullptr, "bytes is null");
+    Carve cv(nullptr, 0);
+    carve_saved(cv, gated, whole_chunks(gated->hidden, gated->dtype), true);
+    *bytes = cv.used + 256;
+  });
+}
+
+extern "C" int rhip_gated_workspace_bytes(const rhip_gated *gated, int32_t pass, size_t *bytes) {
+  return guarded([&] {
+    check_gated(gated);
+    RHIP_CHECK_ARG(bytes != nullptr, "bytes is null");
+    RHIP_CHECK_ARG(pass >= RHIP_GATED_INFERENCE && pass <= RHIP_GATED_BACKWARD,
+                   "pass must be one of RHIP_GATED_");
+    Carve cv(nullptr, 0);
+    if (pass == RHIP_GATED_BACKWARD)
+      plan_backward(cv, gated);
+    else
+      plan_forward(cv, gated, pass == RHIP_GATED_FORWARD);
+    *bytes = cv.used + 256;
+  });
+}
+
+extern "C" int rhip_gated_forward(const rhip_gated *gated, void *y, void *saved,
+                                  size_t saved_bytes, void *workspace, size_t ws_bytes,
+                                  hipStream_t stream) {
+  return guarded([&] {
+    const rhip_gated *d = gated;
+    check_gated(d);
+    if (d->n == 0)
+      return;
+    RHIP_CHECK_ARG(y != nullptr, "y is required");
+    RHIP_CHECK_ARG(workspace != nullptr, "workspace is required");
+    Carve cv(workspace, ws_bytes);
+    GatedForward f = plan_forward(cv, d, saved != nullptr);
+    if (saved) {
+      Carve keep(saved, saved_bytes);
+      f.saved = carve_saved(keep, d, whole_chunks(d->hidden, d->dtype), true);
+    }
+    with_type(d->dtype, [&](auto t) {
+      using T = decltype(t);
+      GatedArgs a = gated_args(d, f.saved);
+      if (d->n <= kGatedMaxRows) {
+        FewArgs w{};
+        w.y = d->x, w.y_row = d->x_row;
+        w.x[0] = d->gate, w.x[1] = d->up;
+        w.x_row[0] = d->gate_row, w.x_row[1] = d->up_row;
+        w.n = static_cast<int32_t>(d->n), w.k = d->channels, w.cols = d->hidden;
+        w.saved = f.saved, w.pitch = a.pitch, w.keep = saved != nullptr, w.kind = d->activation;
+        run_few<T, true>(w, stream);
+        w.y = f.saved.h, w.y_row = a.pitch;
+        w.x[0] = d->down, w.x_row[0] = d->down_row;
+        w.k = d->hidden, w.cols = d->outputs;
+        w.out = y, w.out_row = d->outputs;
+        run_few<T, false>(w, stream);
+        return;
+      }
+      for (const Packed *m : {&f.x, &f.gate, &f.up, &f.down})
+        run_pack<T>(*m, stream);
+      a.y = side(f.x, false);
+      a.x = side(f.gate, false, &f.up);
+      a.k_tiles = static_cast<int32_t>(ceil_div(a.x.k, gemm_bk<T>()));
+      a.rows = static_cast<int32_t>(d->n), a.cols = d->hidden;
+      a.keep = saved != nullptr;
+      run_product<T, false, false, kGemmHalves, kProject>(a, f.project, f.part, stream);
+      a.y = side(f.saved.h, f.saved.h, a.rows, a.pitch, false);
+      a.x = side(f.down, false);
+      a.k_tiles = static_cast<int32_t>(ceil_div(a.x.k, gemm_bk<T>()));
+      a.cols = d->outputs;
+      a.out[0] = y, a.out_row = d->outputs;
+      run_product<T, false, false, kGemmOne, kPlain>(a, f.out, f.part, stream);
+    });
+  });
+}
+
+extern "C" int rhip_gated_backward(const rhip_gated *gated, const void *saved,
+                                   size_t saved_bytes, void *grad_x, void *grad_gate,
+                                   void *grad_up, void *grad_down, void *workspace,
+                                   size_t ws_bytes, hipStream_t stream) {
+  return guarded([&] {
+    const rhip_gated *d = gated;
+    check_gated(d);
+    RHIP_CHECK_ARG((grad_gate == nullptr) == (grad_up == nullptr),
+                   "grad_gate and grad_up go together");
+    if (!(grad_x && d->n > 0) && !grad_gate && !grad_down)
+      return;
+    RHIP_CHECK_ARG(d->n == 0 || (d->grad_y && saved), "grad_y and saved are required");
+    RHIP_CHECK_ARG(workspace != nullptr, "workspace is required");
+    Carve cv(workspace, ws_bytes);
+    const GatedBackward b = plan_backward(cv, d);
+    GatedSaved s{};
+    if (saved) {
+      Carve keep(const_cast<void *>(saved), saved_bytes);
+      s = carve_saved(keep, d, whole_chunks(d->hidden, d->dtype), true);
+    }
+    with_type(d->dtype, [&](auto t) {
+      using T = decltype(t);
+      const GatedArgs base = gated_args(d, s);
+      const int32_t n = static_cast<int32_t>(d->n);
+      run_pack<T>(b.gy, stream);
+      if (grad_x || grad_gate) {
+        run_pack<T>(b.down, stream);
+        GatedArgs a = base;
+        a.y = side(b.gy, false);
+        a.x = side(b.down, true);
+        a.k_tiles = static_cast<int32_t>(ceil_div(a.x.k, gemm_bk<T>()));
+        a.rows = n, a.cols = d->hidden;
+        a.dg = b.dg, a.du = b.du;
+        run_product<T, false, true, kGemmOne, kHidden>(a, b.hidden, b.part, stream);
+      }
+      if (grad_x) {
+        run_pack<T>(b.gate, stream);
+        run_pack<T>(b.up, stream);
+        GatedArgs a = base;
+        a.y = side(b.dg, b.du, n, a.pitch, false);
+        a.x = side(b.gate, true, &b.up);
+        a.k_tiles = 2 * static_cast<int32_t>(ceil_div(a.x.k, gemm_bk<T>()));
+        a.rows = n, a.cols = d->channels;
+        a.out[0] = grad_x, a.out_row = d->channels;
+        run_product<T, false, true, kGemmBehind, kPlain>(a, b.gx, b.part, stream);
+      }
+      if (grad_gate) {
+        run_pack<T>(b.x, stream);
+        GatedArgs a = base;
+        a.y = side(b.dg, b.du, n, a.pitch, true);
+        a.x = side(b.x, true);
+        a.outs = 2;
+        a.k_tiles = static_cast<int32_t>(ceil_div(n, gemm_bk<T>()));
+        a.rows = d->hidden, a.cols = d->channels;
+        a.out[0] = grad_gate, a.out[1] = grad_up, a.out_row = d->channels;
+        run_product<T, true, true, kGemmOne, kPlain>(a, b.gw, b.part, stream);
+      }
+      if (grad_down) {
+        GatedArgs a = base;
+        a.y = side(b.gy, true);
+        a.x = side(s.h, s.h, n, a.pitch, true);
+        a.k_tiles = static_cast<int32_t>(ceil_div(n, gemm_bk<T>()));
+        a.rows = d->outputs, a.cols = d->hidden;
+        a.out[0] = grad_down, a.out_row = d->hidden;
+        run_product<T, true, true, kGemmOne, kPlain>(a, b.gd, b.part, stream);
+      }
+    });
+  });
+}

@@ -442,6 +442,52 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
       py::arg("key_offsets") = py::none(), py::arg("key_lengths") = py::none(),
       py::arg("causal") = false, py::arg("scale") = py::none());
   nn.def(
+      "rotate_heads",
+      [](const at::Tensor &input, const at::Tensor &positions, const at::Tensor &frequencies,
+         const std::vector<int64_t> &sections, bool interleaved) {
+        py::gil_scoped_release release;
+        return hip_rotate_heads(input, positions, frequencies, sections, interleaved);
+      },
+      "Heads [rows, heads, width] turned by positions [rows, axes]: pair p, elements (p, pairs + "
+      "p) or interleaved (2 p, 2 p + 1), by position * frequencies[p] of its axis (sections: pairs "
+      "of each axis; frequencies fp64).",
+      py::arg("input"), py::arg("positions"), py::arg("frequencies"), py::arg("sections"),
+      py::arg("interleaved") = false);
+  nn.def(
+      "norm_rotate_heads",
+      [](const at::Tensor &query, const at::Tensor &key, const at::Tensor &positions,
+         const at::Tensor &frequencies, const std::vector<int64_t> &sections,
+         OptTensor query_weight, OptTensor key_weight, double eps, bool interleaved) {
+        py::gil_scoped_release release;
+        return hip_norm_rotate_heads(query, key, positions, frequencies, sections,
+                                     query_weight.value_or(at::Tensor()),
+                                     key_weight.value_or(at::Tensor()), eps, interleaved);
+      },
+      "Queries and keys [rows, heads, width], each head normed (x / sqrt(mean(x^2) + eps) * "
+      "weight, fp32 weights) and then turned as by rotate_heads.",
+      py::arg("query"), py::arg("key"), py::arg("positions"), py::arg("frequencies"),
+      py::arg("sections"), py::arg("query_weight") = py::none(),
+      py::arg("key_weight") = py::none(), py::arg("eps") = 1e-6,
+      py::arg("interleaved") = false);
+  nn.def(
+      "rotary_frequencies",
+      [](const std::vector<int64_t> &sections, double base, const py::object &device) {
+        return rotary_frequencies(sections, base, at::Device(std::string(py::str(device))));
+      },
+      "base^(-i / s) for pair i of every section of s pairs, fp64.", py::arg("sections"),
+      py::arg("base") = 10000.0, py::arg("device") = "cuda");
+  nn.def(
+      "gated_feed_forward",
+      [](const at::Tensor &input, const at::Tensor &gate, const at::Tensor &up,
+         const at::Tensor &down, const std::string &activation) {
+        py::gil_scoped_release release;
+        return hip_gated_feed_forward(input, gate, up, down, activation);
+      },
+      "(act(input gate^T) * (input up^T)) down^T; gate and up [hidden, channels], down [outputs, "
+      "hidden]; activation \"silu\" or \"gelu\".",
+      py::arg("input"), py::arg("gate"), py::arg("up"), py::arg("down"),
+      py::arg("activation") = "silu");
+  nn.def(
       "layer_norm",
       [](const at::Tensor &input, OptTensor weight, OptTensor bias, double eps) {
         py::gil_scoped_release release;

@@ -635,6 +635,35 @@ at::Tensor hip_packed_attention(const at::Tensor &query, const at::Tensor &key,
                                 const at::Tensor &key_lengths = at::Tensor(),
                                 bool causal = false, c10::optional<double> scale = c10::nullopt);
 
+// Heads [rows, heads, width] turned by positions [rows, axes] (int32, int64 or
+// fp32; [rows] for one axis), autograd-aware: pair p of a head, elements (p,
+// pairs + p) or interleaved (2 p, 2 p + 1), by position * frequencies[p] of its
+// axis; sections: pairs of each axis, frequencies fp64 [pairs]. Elements behind
+// the pairs stay. fp32 or bf16, width <= 256.
+at::Tensor hip_rotate_heads(const at::Tensor &input, const at::Tensor &positions,
+                            const at::Tensor &frequencies, const std::vector<int64_t> &sections,
+                            bool interleaved = false);
+
+// The same for queries and keys in one pass, each head normed before it: x /
+// sqrt(mean(x^2) + eps) * weight, weights fp32 [width] or undefined.
+std::tuple<at::Tensor, at::Tensor>
+hip_norm_rotate_heads(const at::Tensor &query, const at::Tensor &key, const at::Tensor &positions,
+                      const at::Tensor &frequencies, const std::vector<int64_t> &sections,
+                      const at::Tensor &query_weight = at::Tensor(),
+                      const at::Tensor &key_weight = at::Tensor(), double eps = 1e-6,
+                      bool interleaved = false);
+
+// base^(-i / s) for pair i of every section of s pairs, fp64.
+at::Tensor rotary_frequencies(const std::vector<int64_t> &sections, double base,
+                              const at::Device &device);
+
+// (act(input gate^T) * (input up^T)) down^T over the last axis (autograd-aware):
+// gate and up [hidden, channels], down [outputs, hidden], all of the input's
+// dtype; activation "silu" or "gelu".
+at::Tensor hip_gated_feed_forward(const at::Tensor &input, const at::Tensor &gate,
+                                  const at::Tensor &up, const at::Tensor &down,
+                                  const std::string &activation = "silu");
+
 // Layer norm over the last axis (autograd-aware); weight and bias fp32 or
 // undefined.
 at::Tensor hip_layer_norm(const at::Tensor &input, const at::Tensor &weight = at::Tensor(),
