@@ -744,7 +744,8 @@ typedef struct rhip_attn {
 typedef enum rhip_attn_pass {
   RHIP_ATTN_FORWARD = 0,
   RHIP_ATTN_QUERIES = 1,
-  RHIP_ATTN_KEYS = 2
+  RHIP_ATTN_KEYS = 2,
+  RHIP_ATTN_APART = 3 /* with a window: over the blocks of keys that hold sinks */
 } rhip_attn_pass;
 
 /*
@@ -787,6 +788,36 @@ int rhip_attn_backward(const rhip_attn *attn, const void *grad_out,
                        void *grad_q, void *grad_k, void *grad_v,
                        void *workspace, size_t workspace_bytes,
                        hipStream_t stream);
+
+/* The same inside a window: with p = i + (Lk - Lq) the place of query row i among
+ * the keys in use, the row sees key j when |p - j| < window or j < sinks, and
+ * with causal != 0 only when j <= p as well. window at least 1 (the row's own
+ * place), sinks 0 or more. */
+typedef struct rhip_attn_window {
+  int32_t window, sinks;
+} rhip_attn_window;
+
+/* rhip_attn_plan, rhip_attn_workspace_bytes, rhip_attn_forward and
+ * rhip_attn_backward with a window. Work goes by the windows, not by the
+ * sequences' lengths. (The plan of a pass that makes no launch is 0 blocks.) */
+int rhip_attn_window_plan(const rhip_attn *attn, const rhip_attn_window *window,
+                          int32_t pass, int32_t *blocks, int32_t *splits);
+int rhip_attn_window_workspace_bytes(const rhip_attn *attn,
+                                     const rhip_attn_window *window,
+                                     int32_t backward, size_t *bytes);
+int rhip_attn_window_forward(const rhip_attn *attn, const rhip_attn_window *window,
+                             const void *q, const void *k, const void *v,
+                             void *out, void *out_rest, float *lse,
+                             void *workspace, size_t workspace_bytes,
+                             hipStream_t stream);
+int rhip_attn_window_backward(const rhip_attn *attn, const rhip_attn_window *window,
+                              const void *grad_out, int64_t grad_out_row,
+                              int64_t grad_out_head, const void *q,
+                              const void *k, const void *v, const void *out,
+                              const void *out_rest, const float *lse,
+                              void *grad_q, void *grad_k, void *grad_v,
+                              void *workspace, size_t workspace_bytes,
+                              hipStream_t stream);
 
 /* -------------------------------------------------------------- rotation
  *

@@ -50,6 +50,8 @@ EXPORTS = (
     "rhip_bn_workspace_bytes", "rhip_bn_stats", "rhip_bn_invstd", "rhip_bn_forward",
     "rhip_bn_backward",
     "rhip_attn_plan", "rhip_attn_workspace_bytes", "rhip_attn_forward", "rhip_attn_backward",
+    "rhip_attn_window_plan", "rhip_attn_window_workspace_bytes", "rhip_attn_window_forward",
+    "rhip_attn_window_backward",
     "rhip_ln_workspace_bytes", "rhip_ln_forward", "rhip_ln_backward",
     "rhip_embed_forward", "rhip_embed_workspace_bytes", "rhip_embed_backward",
     "rhip_rotary_forward", "rhip_rotary_workspace_bytes", "rhip_rotary_backward",
@@ -88,6 +90,10 @@ class RhipAttn(ctypes.Structure):
 
 _vp, _i64, _i32, _sz = ctypes.c_void_p, ctypes.c_int64, ctypes.c_int32, ctypes.c_size_t
 _P = ctypes.POINTER
+
+
+class RhipAttnWindow(ctypes.Structure):
+    _fields_ = [("window", ctypes.c_int32), ("sinks", ctypes.c_int32)]
 
 
 ROTARY_MAX_AXES = 8
@@ -215,6 +221,15 @@ def _declare(lib):
                                              _sz, _vp]),
         "rhip_attn_backward": (ctypes.c_int, [_P(RhipAttn), _vp, _i64, _i64, _vp, _vp, _vp, _vp,
                                               _vp, _vp, _vp, _vp, _vp, _vp, _sz, _vp]),
+        "rhip_attn_window_plan": (ctypes.c_int, [_P(RhipAttn), _P(RhipAttnWindow), _i32,
+                                                 _P(_i32), _P(_i32)]),
+        "rhip_attn_window_workspace_bytes": (ctypes.c_int, [_P(RhipAttn), _P(RhipAttnWindow),
+                                                            _i32, _P(_sz)]),
+        "rhip_attn_window_forward": (ctypes.c_int, [_P(RhipAttn), _P(RhipAttnWindow), _vp, _vp,
+                                                    _vp, _vp, _vp, _vp, _vp, _sz, _vp]),
+        "rhip_attn_window_backward": (ctypes.c_int, [_P(RhipAttn), _P(RhipAttnWindow), _vp, _i64,
+                                                     _i64, _vp, _vp, _vp, _vp, _vp, _vp, _vp,
+                                                     _vp, _vp, _vp, _sz, _vp]),
         "rhip_ln_workspace_bytes": (ctypes.c_int, [_i64, _i32, _P(_sz)]),
         "rhip_ln_forward": (ctypes.c_int, [_vp, _i64, _i64, _i32, _vp, _vp, ctypes.c_double, _vp,
                                            _vp, _vp, _i32, _vp]),
@@ -1072,41 +1087,65 @@ def _attn_desc(q, k, v, q_offsets, k_offsets, k_lengths, causal, scale) -> RhipA
 
 
 ATTN_PASSES = ("forward", "queries", "keys")
+ATTN_WINDOW_PASSES = (*ATTN_PASSES, "apart")
 
 
 def attn_plan(which: str, dtype: torch.dtype, n_q: int, n_k: int, n_seq: int, heads: int,
-              kv_heads: int, dim: int, causal: bool):
+              kv_heads: int, dim: int, causal: bool, window: Optional[int] = None,
+              sinks: int = 0):
     """(32-row blocks per workgroup, splits) of an attention pass ("forward",
-    "queries": grad_q, "keys": grad_k and grad_v), from rhip_attn_plan."""
+    "queries": grad_q, "keys": grad_k and grad_v; with a window "apart": those
+    of the sinks' blocks), from rhip_attn_plan or rhip_attn_window_plan."""
     desc = RhipAttn(n_q=n_q, n_k=n_k, n_seq=n_seq, heads=heads, kv_heads=kv_heads, dim=dim,
                     causal=int(causal), dtype=_dtype_code(dtype), scale=dim ** -0.5)
     blocks, splits = _i32(0), _i32(0)
-    _check(lib().rhip_attn_plan(ctypes.byref(desc), ATTN_PASSES.index(which),
+    if window is not None:
+        _check(lib().rhip_attn_window_plan(
+            ctypes.byref(desc), ctypes.byref(RhipAttnWindow(window, sinks)),
+            ATTN_WINDOW_PASSES.index(which), ctypes.byref(blocks), ctypes.byref(splits)),
+            "rhip_attn_window_plan")
+        return blocks.value, splits.value
+    _check(lib().rhip_attn_plan(ctypes.byref(desc), ATTN_WINDOW_PASSES.index(which),
                                 ctypes.byref(blocks), ctypes.byref(splits)), "rhip_attn_plan")
     return blocks.value, splits.value
 
 
-def _attn_ws(desc: RhipAttn, backward: bool, device) -> torch.Tensor:
-    return torch.empty(_sizeq(lib().rhip_attn_workspace_bytes, ctypes.byref(desc),
-                              int(backward)), dtype=torch.uint8, device=device)
+def _attn_call(name: str, desc: RhipAttn, window: Optional[int], sinks: int, *args) -> None:
+    """rhip_attn_<name>, or with a window rhip_attn_window_<name>."""
+    if window is None:
+        if sinks:
+            raise RuntimeError("sinks stand beside a window")
+        _check(getattr(lib(), f"rhip_attn_{name}")(ctypes.byref(desc), *args),
+               f"rhip_attn_{name}")
+    else:
+        _check(getattr(lib(), f"rhip_attn_window_{name}")(
+            ctypes.byref(desc), ctypes.byref(RhipAttnWindow(window, sinks)), *args),
+            f"rhip_attn_window_{name}")
+
+
+def _attn_ws(desc: RhipAttn, window: Optional[int], sinks: int, backward: bool,
+             device) -> torch.Tensor:
+    out = _sz(0)
+    _attn_call("workspace_bytes", desc, window, sinks, int(backward), ctypes.byref(out))
+    return torch.empty(int(out.value), dtype=torch.uint8, device=device)
 
 
 def attn_forward(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, q_offsets: torch.Tensor,
                  k_offsets: torch.Tensor, k_lengths: Optional[torch.Tensor] = None,
                  causal: bool = False, scale: Optional[float] = None,
-                 rest: Optional[torch.Tensor] = None):
+                 rest: Optional[torch.Tensor] = None, window: Optional[int] = None,
+                 sinks: int = 0):
     """(out [n_q, heads, dim], lse [heads, n_q]) of attention over packed
     sequences; offsets and lengths int32 on the device; rest (bf16, like out)
-    receives out's rounding error."""
+    receives out's rounding error; window and sinks as rhip_attn_window's."""
     q, k, v = _dense_last(q), _dense_last(k), _dense_last(v)
     desc = _attn_desc(q, k, v, q_offsets, k_offsets, k_lengths, causal, scale)
     _require_dense(rest, "rest", q.shape, torch.bfloat16, q.device)
     out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
     lse = torch.empty((q.shape[1], q.shape[0]), dtype=torch.float32, device=q.device)
-    ws = _attn_ws(desc, False, q.device)
-    _check(lib().rhip_attn_forward(ctypes.byref(desc), _ptr(q), _ptr(k), _ptr(v), _ptr(out),
-                                   _ptr(rest), _ptr(lse), _ptr(ws), ws.numel(),
-                                   _stream(q.device)), "rhip_attn_forward")
+    ws = _attn_ws(desc, window, sinks, False, q.device)
+    _attn_call("forward", desc, window, sinks, _ptr(q), _ptr(k), _ptr(v), _ptr(out), _ptr(rest),
+               _ptr(lse), _ptr(ws), ws.numel(), _stream(q.device))
     return out, lse
 
 
@@ -1114,7 +1153,8 @@ def attn_backward(grad_out: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: t
                   out: torch.Tensor, lse: torch.Tensor, q_offsets: torch.Tensor,
                   k_offsets: torch.Tensor, k_lengths: Optional[torch.Tensor] = None,
                   causal: bool = False, scale: Optional[float] = None,
-                  rest: Optional[torch.Tensor] = None):
+                  rest: Optional[torch.Tensor] = None, window: Optional[int] = None,
+                  sinks: int = 0):
     """(grad_q, grad_k, grad_v) from the forward's out, lse and rest."""
     q, k, v = _dense_last(q), _dense_last(k), _dense_last(v)
     grad_out = _dense_last(grad_out.to(q.dtype))
@@ -1127,12 +1167,10 @@ def attn_backward(grad_out: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: t
     gq = torch.empty(q.shape, dtype=q.dtype, device=q.device)
     gk = torch.empty(k.shape, dtype=q.dtype, device=q.device)
     gv = torch.empty(k.shape, dtype=q.dtype, device=q.device)
-    ws = _attn_ws(desc, True, q.device)
-    _check(lib().rhip_attn_backward(ctypes.byref(desc), _ptr(grad_out), grad_out.stride(0),
-                                    grad_out.stride(1), _ptr(q), _ptr(k), _ptr(v), _ptr(out),
-                                    _ptr(rest), _ptr(lse), _ptr(gq), _ptr(gk), _ptr(gv),
-                                    _ptr(ws), ws.numel(), _stream(q.device)),
-           "rhip_attn_backward")
+    ws = _attn_ws(desc, window, sinks, True, q.device)
+    _attn_call("backward", desc, window, sinks, _ptr(grad_out), grad_out.stride(0),
+               grad_out.stride(1), _ptr(q), _ptr(k), _ptr(v), _ptr(out), _ptr(rest), _ptr(lse),
+               _ptr(gq), _ptr(gk), _ptr(gv), _ptr(ws), ws.numel(), _stream(q.device))
     return gq, gk, gv
 
 

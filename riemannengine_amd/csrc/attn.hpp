@@ -11,7 +11,9 @@
 namespace rhip {
 
 void attn_forward_run(const AttnArgs &a, int32_t dtype, bool vec, hipStream_t stream);
-void attn_backward_run(const AttnArgs &a, int32_t dtype, bool vec, hipStream_t stream);
+struct AttnApart;
+void attn_backward_run(const AttnArgs &a, const AttnApart &apart, int32_t dtype, bool vec,
+                       hipStream_t stream);
 // The shape of a pass's launch: 32-row blocks per workgroup (W), tiles of 32 W
 // rows, and the workgroups that share one tile of query rows (forward) or of
 // keys (backward), whose partial sums are the workspace.
@@ -20,9 +22,20 @@ struct AttnPlan {
   int64_t tiles;
   int32_t splits;
 };
-AttnPlan attn_forward_plan(const rhip_attn &d);
+// A window and the sinks beside it; window 0: none, every key counts.
+struct AttnWindow {
+  int32_t window, sinks;
+};
+AttnPlan attn_forward_plan(const rhip_attn &d, const AttnWindow &window);
 AttnPlan attn_queries_plan(const rhip_attn &d);
-AttnPlan attn_keys_plan(const rhip_attn &d);
+AttnPlan attn_keys_plan(const rhip_attn &d, const AttnWindow &window);
+// The launch over the first keys of every sequence, the blocks of 32 that hold
+// sinks, which rows of the whole sequence see: `keys` of each.
+struct AttnApart {
+  int32_t keys;
+  AttnPlan plan;
+};
+AttnApart attn_apart_plan(const rhip_attn &d, const AttnWindow &window);
 
 // 32-row blocks per workgroup of the kernels over query rows: as many as leave
 // two workgroups for each CU, or one with two blocks (bf16: a workgroup's own

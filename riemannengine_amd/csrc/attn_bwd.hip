@@ -128,7 +128,9 @@ __device__ __forceinline__ void join_row(const float *rows, int row_floats, int 
 //
 // Bound by the matrix cores (four causal prompts of 4096, 16 over 4 heads, 128
 // wide, bf16: 398 us, 1035 TFLOP/s), by the vector instructions at 32 wide (890).
-template <typename T, int DP, bool VEC, int W>
+//
+// LOCAL: inside a window, as in the forward.
+template <typename T, int DP, bool VEC, int W, bool LOCAL>
 __global__ __launch_bounds__(kBwdThreads, (BwdShape<T, DP, W, false>::kOccupancy)) void
 attn_dq_kernel(AttnArgs a) {
   using Shape = BwdShape<T, DP, W, false>;
@@ -165,7 +167,19 @@ attn_dq_kernel(AttnArgs a) {
   const int32_t wave_lim =
       wave_uniform(wave0 < n_rows ? sees(min(wave0 + 32, n_rows) - 1) : 0);
   const int32_t wave_full = wave_uniform(wave0 < n_rows ? sees(wave0) : 0);
-  const int32_t kt1 = a.gq ? (wg_lim + kBN - 1) / kBN : 0; // else statistics alone
+  using Tiles = LocalTiles<kBN>;
+  auto local = [&](int32_t r) {
+    return LOCAL && r >= 0 ? local_keys(a, sq, r / a.group) : LocalKeys{0, 0, 0};
+  };
+  const LocalKeys mine = local(row_ok ? row : -1);
+  const Tiles wg(local(row0), local(min(row0 + Shape::kRows, n_rows) - 1));
+  const bool any_row = wave0 < n_rows;
+  const Tiles wave(local(any_row ? wave0 : -1), local(any_row ? min(wave0 + 32, n_rows) - 1 : -1));
+  auto cut = [&](int32_t kt) { // a tile of which some rows see a part
+    return LOCAL ? !wg.all(kt * kBN, min((kt + 1) * kBN, sq.lk))
+                 : wg_full < wg_lim && (kt + 1) * kBN > wg_full;
+  };
+  const int32_t kt1 = !a.gq ? 0 : LOCAL ? wg.count : (wg_lim + kBN - 1) / kBN; // 0: statistics alone
   const int32_t first = W == 1 ? w : 0, step = W == 1 ? kBwdWaves : 1;
 
   const T *kp = static_cast<const T *>(a.k) + sq.k0 * a.k_row + kv * a.k_head;
@@ -174,7 +188,8 @@ attn_dq_kernel(AttnArgs a) {
   ks.init(a.k_row, a.dim);
   vs.init(a.v_row, a.dim);
   char *stage = lds + (W == 1 ? w : 0) * Shape::kBuffers * Shape::kBufBytes;
-  auto issue = [&](int32_t kt, int buf) {
+  auto issue = [&](int32_t n, int buf) {
+    const int32_t kt = LOCAL ? wg.tile(n) : n;
     char *to = stage + buf * Shape::kBufBytes;
     ks.issue(to, kp + static_cast<int64_t>(kt) * kBN * a.k_row, a.k_row, sq.lk - kt * kBN,
              a.dim);
@@ -237,11 +252,12 @@ attn_dq_kernel(AttnArgs a) {
   const typename Tile::Lane lane_at = Tile::lane_addresses();
   const uint32_t stage_at = lds_address(stage);
   int buf = 0;
-  for (int32_t kt = first; kt < kt1; kt += step) {
+  for (int32_t n = first; n < kt1; n += step) {
+    const int32_t kt = LOCAL ? wg.tile(n) : n;
     wait_stream(); // as in the forward
     if constexpr (W > 1)
       __syncthreads();
-    if (wg_full < wg_lim && (kt + 1) * kBN > wg_full) {
+    if (cut(kt)) {
       rare_path();
       const bool found = Tile::template zero_not_finite<true, kBN, W == 1 ? 1 : kBwdWaves>(
           stage_at + buf * Shape::kBufBytes, W == 1 ? 0 : w);
@@ -256,11 +272,11 @@ attn_dq_kernel(AttnArgs a) {
     }
     const typename Tile::Lane at =
         lane_at.in(stage_at + buf * Shape::kBufBytes + b0 * (32 / 4) * Tile::kGroup);
-    if (Shape::kBuffers == 2 && kt + step < kt1)
-      issue(kt + step, buf ^ 1);
+    if (Shape::kBuffers == 2 && n + step < kt1)
+      issue(n + step, buf ^ 1);
     const int32_t j0 = kt * kBN + 32 * b0;
-    if (W == 1 || j0 < wave_lim) {
-      const bool masked = j0 + 32 * kB > wave_full;
+    if (W == 1 || (LOCAL ? wave.some(j0, j0 + 32 * kB) : j0 < wave_lim)) {
+      const bool masked = LOCAL ? !wave.all(j0, j0 + 32 * kB) : j0 + 32 * kB > wave_full;
 #pragma unroll
       for (int b = 0; b < kB; ++b) {
         v16f s{}, dp = dp0;
@@ -284,10 +300,14 @@ attn_dq_kernel(AttnArgs a) {
                 s[r] = exp2_fast(fmaf(s[r], a.c, -lse2)) * dp[r];
               if (masked) {
                 rare_path();
-                const int32_t seen = lim - j0 - 32 * b - 4 * half;
+                const int32_t at0 = j0 + 32 * b + 4 * half;
+                const int32_t seen = lim - at0;
+                const int32_t lo = mine.lo - at0, hi = mine.hi - at0, sinks = mine.first - at0;
 #pragma unroll
-                for (int r = 0; r < 16; ++r)
-                  s[r] = block_row(r) < seen ? s[r] : 0.f;
+                for (int r = 0; r < 16; ++r) {
+                  const int j = block_row(r);
+                  s[r] = (LOCAL ? (j >= lo && j < hi) || j < sinks : j < seen) ? s[r] : 0.f;
+                }
               }
               Tile::pack(s, ds);
             });
@@ -295,16 +315,26 @@ attn_dq_kernel(AttnArgs a) {
     }
     if (Shape::kBuffers == 2) {
       buf ^= 1;
-    } else if (kt + step < kt1) {
+    } else if (n + step < kt1) {
       wait_stream();
       if constexpr (W > 1)
         __syncthreads();
-      issue(kt + step, 0);
+      issue(n + step, 0);
     }
   }
   if (!a.gq)
     return;
-  if (left_out)
+  if (LOCAL) {
+    if (left_out)
+#pragma unroll 1
+      for (int32_t n = 0; n < kt1; ++n) {
+        const int32_t kt = wg.tile(n);
+        if (cut(kt))
+          Tile::template add_not_finite<true>(
+              kp, a.k_row, a.dim, kt * kBN, min((kt + 1) * kBN, sq.lk),
+              [&](int32_t j) { return (j >= mine.lo && j < mine.hi) || j < mine.first; }, dq);
+      }
+  } else if (left_out)
     Tile::template add_not_finite<true>(kp, a.k_row, a.dim, max(wg_full - kBN, 0), wave_lim,
                                         [&](int32_t j) { return j < lim; }, dq);
   if constexpr (W == 4) {
@@ -328,6 +358,30 @@ attn_dq_kernel(AttnArgs a) {
   }
 }
 
+// The launch over the keys apart: tile t of their sequences, `apart` keys each.
+__device__ __forceinline__ AttnSeq apart_tile(const AttnArgs &a, int bm, int32_t t,
+                                              int32_t &room) {
+  const int32_t per = a.apart / bm;
+  AttnSeq q;
+  q.s = t / per, q.tile = t - q.s * per;
+  room = 0, q.k0 = 0;
+  if (q.s < a.n_seq) {
+    q.k0 = q.s == 0 ? 0 : clamp_off(a.k_off[q.s], 0, a.n_k);
+    room = clamp_off(a.k_off[q.s + 1], q.k0, a.n_k) - q.k0;
+  }
+  query_range(a, q, room);
+  room = wave_uniform(room);
+  return wave_uniform(q);
+}
+// Rows of a split's partial sums, and where key j of a sequence stands there.
+__device__ __forceinline__ int64_t partial_rows(const AttnArgs &a, bool apart) {
+  return apart ? static_cast<int64_t>(a.n_seq) * a.apart : a.n_k;
+}
+__device__ __forceinline__ int64_t partial_row(const AttnArgs &a, const AttnSeq &sq, bool apart,
+                                               int32_t j) {
+  return (apart ? static_cast<int64_t>(sq.s) * a.apart : sq.k0) + j;
+}
+
 // dk and dv of 128 (32) keys of one key head over the query rows of every
 // head of its group. A lane holds one key's column (S = Q K^T, dP = dO V^T),
 // so P and dS are the right operands of dV^T = dO^T P and dK^T = Q^T dS as
@@ -335,7 +389,11 @@ attn_dq_kernel(AttnArgs a) {
 //
 // Bound by the matrix cores and by the tiles' reads from LDS (same prompts: 613
 // us, 897 TFLOP/s, four products a block against the other kernel's three).
-template <typename T, int DP, bool VEC, int W>
+//
+// LOCAL: inside a window (LocalRows). The keys of the tiles that hold sinks, which
+// rows of the whole sequence see, are a launch of their own (apart_pass), whose
+// workgroups split those rows; partial sums then lie by sequence.
+template <typename T, int DP, bool VEC, int W, bool LOCAL>
 __global__ __launch_bounds__(kBwdThreads, (BwdShape<T, DP, W, true>::kOccupancy)) void
 attn_dkv_kernel(AttnArgs a) {
   using Shape = BwdShape<T, DP, W, true>;
@@ -355,9 +413,14 @@ attn_dkv_kernel(AttnArgs a) {
   if (!attn_item(a, t, kv, split))
     return;
   int32_t room;
-  const AttnSeq sq = key_tile(a, Shape::kRows, t, room);
+  const bool apart = LOCAL && a.apart_pass;
+  const AttnSeq sq = apart ? apart_tile(a, Shape::kRows, t, room)
+                           : key_tile(a, Shape::kRows, t, room);
   const int32_t key0 = sq.tile * Shape::kRows;
-  if (key0 >= room)
+  // keys below `other` are the other launch's (whole waves; those behind the last
+  // sequence are in none)
+  const int32_t other = LOCAL && !apart && sq.s < a.n_seq ? a.apart : 0;
+  if (key0 >= room || key0 + Shape::kRows <= other)
     return;
   const int lane = lane_id(), half = lane >> 5;
   const int w = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
@@ -371,10 +434,32 @@ attn_dkv_kernel(AttnArgs a) {
   const int32_t wave_full = wave_uniform(first_row(a, sq, wave0 + 31));
   const int32_t wg_full =
       wave_uniform(first_row(a, sq, min(key0 + Shape::kRows, sq.lk) - 1));
-  const int32_t it0 = wave_uniform(first_row(a, sq, key0)) / kBM;
+  // LOCAL: the rows that see some key of the workgroup's (wave's), and those
+  // that see all of them; the lane's
+  auto rows_of = [&](int32_t from, int32_t to, LocalRows &some, LocalRows &all) {
+    const int32_t last = max(min(to, sq.lk) - 1, from);
+    const LocalRows x = local_rows(a, sq, from), y = local_rows(a, sq, last);
+    some = {wave_uniform(x.lo), wave_uniform(from < a.sinks ? sq.lq : y.hi)};
+    all = {wave_uniform(y.lo), wave_uniform(last < a.sinks
+                                                ? sq.lq
+                                                : local_rows(a, sq, max(from, a.sinks)).hi)};
+  };
+  LocalRows wg_some{}, wg_all{}, wave_some{}, wave_all{}, mine{};
+  if constexpr (LOCAL) {
+    rows_of(max(key0, other), key0 + Shape::kRows, wg_some, wg_all);
+    if (wave0 >= other) {
+      rows_of(wave0, wave0 + 32, wave_some, wave_all);
+      mine = local_rows(a, sq, key);
+    }
+  }
+  const int32_t it0 = (LOCAL ? wg_some.lo : wave_uniform(first_row(a, sq, key0))) / kBM;
+  const int32_t rows_end = LOCAL ? wg_some.hi : sq.lq;
+  auto cut = [&](int32_t i) { // a tile of rows from i on, some of which do not see all keys
+    return LOCAL ? !(i >= wg_all.lo && min(i + kBM, sq.lq) <= wg_all.hi) : i < wg_full;
+  };
   // tiles of query rows from the first that sees a key, for each head; this
   // workgroup's part of them
-  const int32_t per_head = key0 < sq.lk ? max((sq.lq + kBM - 1) / kBM - it0, 0) : 0;
+  const int32_t per_head = key0 < sq.lk ? max((rows_end + kBM - 1) / kBM - it0, 0) : 0;
   int32_t n0 = 0, n1 = per_head * a.group;
   if (a.splits > 1) {
     const int32_t per = (n1 + a.splits - 1) / a.splits;
@@ -454,7 +539,7 @@ attn_dkv_kernel(AttnArgs a) {
     wait_stream();
     if constexpr (W > 1)
       __syncthreads();
-    if ((it0 + n % per_head) * kBM < wg_full) {
+    if (cut((it0 + n % per_head) * kBM)) {
       rare_path();
       const uint32_t tile = stage_at + buf * Shape::kBufBytes;
       constexpr int kShare = W == 1 ? 1 : kBwdWaves;
@@ -477,8 +562,9 @@ attn_dkv_kernel(AttnArgs a) {
     if (Shape::kBuffers == 2 && n + step < n1)
       issue(n + step, buf ^ 1);
     const int32_t i0 = (it0 + n % per_head) * kBM + 32 * b0;
-    if (i0 + 32 * kB > wave_lo) {
-      const bool masked = i0 < wave_full || i0 + 32 * kB > sq.lq;
+    if (LOCAL ? i0 + 32 * kB > wave_some.lo && i0 < wave_some.hi : i0 + 32 * kB > wave_lo) {
+      const bool masked = LOCAL ? i0 < wave_all.lo || i0 + 32 * kB > wave_all.hi
+                                : i0 < wave_full || i0 + 32 * kB > sq.lq;
 #pragma unroll
       for (int b = 0; b < kB; ++b) {
         v16f s{}, dp;
@@ -521,7 +607,8 @@ attn_dkv_kernel(AttnArgs a) {
         }
         if (masked) {
           rare_path();
-          const int32_t at0 = i0 + 32 * b + 4 * half, from = lo - at0, to = sq.lq - at0;
+          const int32_t at0 = i0 + 32 * b + 4 * half;
+          const int32_t from = (LOCAL ? mine.lo : lo) - at0, to = (LOCAL ? mine.hi : sq.lq) - at0;
 #pragma unroll
           for (int r = 0; r < 16; ++r) {
             const bool sees = block_row(r) >= from && block_row(r) < to;
@@ -546,10 +633,21 @@ attn_dkv_kernel(AttnArgs a) {
   }
 
   if (left_out)
-    for (int head = kv * a.group; head < (kv + 1) * a.group; ++head)
-      Tile::template add_not_finite<false>(
-          static_cast<const T *>(a.go) + sq.q0 * a.go_row + head * a.go_head, a.go_row, a.dim,
-          wave_lo, min(wg_full + kBM, sq.lq), [&](int32_t i) { return i >= lo; }, dv);
+    for (int head = kv * a.group; head < (kv + 1) * a.group; ++head) {
+      const T *gp = static_cast<const T *>(a.go) + sq.q0 * a.go_row + head * a.go_head;
+      if (LOCAL) {
+#pragma unroll 1
+        for (int32_t i = it0 * kBM; i < rows_end; i += kBM)
+          if (cut(i))
+            Tile::template add_not_finite<false>(
+                gp, a.go_row, a.dim, i, min(i + kBM, sq.lq),
+                [&](int32_t r) { return r >= mine.lo && r < mine.hi; }, dv);
+      } else {
+        Tile::template add_not_finite<false>(gp, a.go_row, a.dim, wave_lo,
+                                             min(wg_full + kBM, sq.lq),
+                                             [&](int32_t i) { return i >= lo; }, dv);
+      }
+    }
   // Rows of the region behind the keys in use get zeros: where their lanes
   // share a wave with keys in use, those met them as a key of zeros, with a
   // probability of exp(-lse).
@@ -561,9 +659,10 @@ attn_dkv_kernel(AttnArgs a) {
   }
   if constexpr (W == 4) {
     if (a.splits > 1) {
-      if (my_key < room) {
+      if (my_key < room && (!LOCAL || my_key >= other)) {
         const int64_t place =
-            ((split * static_cast<int64_t>(a.n_k) + sq.k0 + my_key) * a.kv_heads + kv) * a.dim;
+            ((split * partial_rows(a, apart) + partial_row(a, sq, apart, my_key)) * a.kv_heads +
+             kv) * a.dim;
         using Sum = AttnTile<float, DP>;
         if (a.dim % 4 == 0) {
           Sum::template store_column<true>(a.part_k + place, a.dim, 1.f, dk);
@@ -575,7 +674,7 @@ attn_dkv_kernel(AttnArgs a) {
       }
       return;
     }
-    if (my_key < room) {
+    if (my_key < room && (!LOCAL || my_key >= other)) {
       const int64_t place =
           ((sq.k0 + static_cast<int64_t>(my_key)) * a.kv_heads + kv) * a.dim;
       Tile::template store_column<VEC>(static_cast<T *>(a.gk) + place, a.dim, a.scale, dk);
@@ -604,11 +703,14 @@ attn_dkv_kernel(AttnArgs a) {
       const int32_t j = key0 + w + u * kBwdWaves;
       if (j >= room)
         break;
+      if (LOCAL && j < other)
+        continue;
       if (a.splits == 1) {
         finish_dkv<T>(a, sq.k0 + static_cast<int64_t>(j), kv, rk[u], rv[u]);
       } else {
         const int64_t place =
-            ((split * static_cast<int64_t>(a.n_k) + sq.k0 + j) * a.kv_heads + kv) * a.dim;
+            ((split * partial_rows(a, apart) + partial_row(a, sq, apart, j)) * a.kv_heads + kv) *
+            a.dim;
         put2(a.part_k + place, a.dim, rk[u][0], rk[u][1], 1.f);
         put2(a.part_v + place, a.dim, rv[u][0], rv[u][1], 1.f);
       }
@@ -619,10 +721,19 @@ attn_dkv_kernel(AttnArgs a) {
 // Adds the splits' partial sums of dk and dv: one wave per key and key head.
 template <typename T>
 __global__ __launch_bounds__(kBwdThreads) void attn_dkv_join_kernel(AttnArgs a) {
-  const int64_t rows = static_cast<int64_t>(a.n_k) * a.kv_heads;
+  const int64_t rows = partial_rows(a, a.apart_pass) * a.kv_heads;
   const int lane = lane_id();
   for (int64_t at = static_cast<int64_t>(blockIdx.x) * kBwdWaves + threadIdx.x / kWave; at < rows;
        at += static_cast<int64_t>(gridDim.x) * kBwdWaves) {
+    int64_t key = at / a.kv_heads;
+    if (a.apart_pass) { // key j of a sequence, if its region holds it
+      const int32_t seq = static_cast<int32_t>(key / a.apart);
+      const int32_t j = static_cast<int32_t>(key - static_cast<int64_t>(seq) * a.apart);
+      const int32_t k0 = seq == 0 ? 0 : clamp_off(a.k_off[seq], 0, a.n_k);
+      if (j >= clamp_off(a.k_off[seq + 1], k0, a.n_k) - k0)
+        continue;
+      key = k0 + static_cast<int64_t>(j);
+    }
     float gk[2] = {0.f, 0.f}, gv[2] = {0.f, 0.f};
 #pragma unroll 4
     for (int s = 0; s < a.splits; ++s) {
@@ -634,7 +745,7 @@ __global__ __launch_bounds__(kBwdThreads) void attn_dkv_join_kernel(AttnArgs a) 
           gv[u] += a.part_v[p + lane + u * kWave];
         }
     }
-    finish_dkv<T>(a, at / a.kv_heads, static_cast<int>(at % a.kv_heads), gk, gv);
+    finish_dkv<T>(a, key, static_cast<int>(at % a.kv_heads), gk, gv);
   }
 }
 
@@ -657,9 +768,15 @@ AttnPlan plan_queries(int64_t rows, int32_t n_seq, int32_t kv_heads, int32_t dty
 // us with one split, 686 with three, joining included; 8 heads, eight of
 // 1024: 70 us with one, 113 with two.)
 AttnPlan plan_keys(int64_t n_q, int64_t n_k, int32_t n_seq, int32_t heads, int32_t kv_heads,
-                   int32_t dim, int32_t causal, int32_t dtype) {
+                   int32_t dim, int32_t causal, int32_t dtype, const AttnWindow &window) {
   const int64_t seqs = std::max<int64_t>(1, std::min<int64_t>(n_seq, n_k));
-  const double rows = static_cast<double>(n_q) * (heads / kv_heads) / seqs; // per key
+  double rows = static_cast<double>(n_q) * (heads / kv_heads) / seqs; // per key
+  if (window.window > 0) { // a window's rows, and no mask's half of them
+    const double seen =
+        (static_cast<double>(window.window) * (causal ? 1 : 2) + 64) * (heads / kv_heads);
+    causal = causal && seen > rows;
+    rows = std::min(rows, seen);
+  }
   const double block =
       1.14 * (dim <= 32 ? 0.25 : dim <= 64 ? 0.5 : dim <= 96 ? 0.8 : 1.0) * (dtype == RHIP_F32 ? 7.5 : 1.0);
   const double all = static_cast<double>(n_k) * kv_heads * rows * (causal ? 0.5 : 1.0) / 1024.0;
@@ -690,15 +807,35 @@ AttnPlan plan_keys(int64_t n_q, int64_t n_k, int32_t n_seq, int32_t heads, int32
 AttnPlan attn_queries_plan(const rhip_attn &d) {
   return plan_queries(d.n_q * (d.heads / d.kv_heads), d.n_seq, d.kv_heads, d.dtype);
 }
-AttnPlan attn_keys_plan(const rhip_attn &d) {
-  return plan_keys(d.n_q, d.n_k, d.n_seq, d.heads, d.kv_heads, d.dim, d.causal, d.dtype);
+AttnPlan attn_keys_plan(const rhip_attn &d, const AttnWindow &window) {
+  return plan_keys(d.n_q, d.n_k, d.n_seq, d.heads, d.kv_heads, d.dim, d.causal, d.dtype, window);
 }
 
-void attn_backward_run(const AttnArgs &args, int32_t dtype, bool vec, hipStream_t stream) {
+// Tiles of 32 keys (W = 1), each over all rows of its sequence in as many parts
+// as fill the chip twice, each part of 512 rows (four tiles a wave) at least.
+AttnApart attn_apart_plan(const rhip_attn &d, const AttnWindow &window) {
+  if (window.window == 0 || window.sinks == 0 || d.n_seq == 0 || d.n_k == 0)
+    return {};
+  AttnApart p{};
+  // whole blocks; no more than any sequence has
+  const int64_t keys = std::min<int64_t>(align_up(window.sinks, 32), align_up(d.n_k, 32));
+  p.keys = static_cast<int32_t>(keys);
+  p.plan.waves = 1;
+  p.plan.tiles = d.n_seq * (keys / 32);
+  const int64_t rows = d.n_q / d.n_seq * (d.heads / d.kv_heads);
+  const int64_t busy = p.plan.tiles * d.kv_heads;
+  p.plan.splits = 1;
+  while (p.plan.splits < 32 && busy * p.plan.splits < 512 && rows >= 1024 * p.plan.splits)
+    p.plan.splits *= 2;
+  return p;
+}
+
+void attn_backward_run(const AttnArgs &args, const AttnApart &apart, int32_t dtype, bool vec,
+                       hipStream_t stream) {
   const AttnPlan pq =
       plan_queries(static_cast<int64_t>(args.n_q) * args.group, args.n_seq, args.kv_heads, dtype);
   const AttnPlan pk = plan_keys(args.n_q, args.n_k, args.n_seq, args.heads, args.kv_heads,
-                                args.dim, args.causal, dtype);
+                                args.dim, args.causal, dtype, {args.window, args.sinks});
   with_attn(dtype, args.dim, vec, [&](auto t, auto dp, auto v) {
     using T = decltype(t);
     constexpr int DP = decltype(dp)::value;
@@ -709,28 +846,49 @@ void attn_backward_run(const AttnArgs &args, int32_t dtype, bool vec, hipStream_
         constexpr int W = decltype(w)::value;
         const unsigned spread = spread_lds<W>(args, BwdShape<T, DP, W, false>::kLds);
         attn_launches(args, pq, kBwdThreads, [&](const AttnArgs &part, unsigned groups) {
-          hipLaunchKernelGGL((attn_dq_kernel<T, DP, VEC, W>), dim3(groups), b, spread, stream,
-                             part);
+          if (args.window > 0)
+            hipLaunchKernelGGL((attn_dq_kernel<T, DP, VEC, W, true>), dim3(groups), b, spread,
+                               stream, part);
+          else
+            hipLaunchKernelGGL((attn_dq_kernel<T, DP, VEC, W, false>), dim3(groups), b, spread,
+                               stream, part);
         });
       });
     }
     if (!args.gk || args.n_k == 0)
       return;
-    with_waves(pk.waves, [&](auto w) {
-      attn_launches(args, pk, kBwdThreads, [&](const AttnArgs &part, unsigned groups) {
-        hipLaunchKernelGGL((attn_dkv_kernel<T, DP, VEC, decltype(w)::value>), dim3(groups), b, 0,
-                           stream, part);
-      });
-    });
-    if (pk.splits > 1) {
-      const int64_t rows = static_cast<int64_t>(args.n_k) * args.kv_heads;
-      AttnArgs a = args;
-      a.splits = pk.splits;
+    auto join = [&](AttnArgs a, int64_t keys, int32_t splits) {
+      const int64_t rows = keys * args.kv_heads;
+      a.splits = splits;
       hipLaunchKernelGGL((attn_dkv_join_kernel<T>),
                          dim3(static_cast<unsigned>(
                              std::min(ceil_div(rows, kBwdWaves), max_groups(kBwdThreads)))),
                          b, 0, stream, a);
       RHIP_LAUNCH_CHECK();
+    };
+    with_waves(pk.waves, [&](auto w) {
+      constexpr int W = decltype(w)::value;
+      attn_launches(args, pk, kBwdThreads, [&](const AttnArgs &part, unsigned groups) {
+        if (args.window > 0)
+          hipLaunchKernelGGL((attn_dkv_kernel<T, DP, VEC, W, true>), dim3(groups), b, 0, stream,
+                             part);
+        else
+          hipLaunchKernelGGL((attn_dkv_kernel<T, DP, VEC, W, false>), dim3(groups), b, 0, stream,
+                             part);
+      });
+    });
+    if (pk.splits > 1)
+      join(args, args.n_k, pk.splits);
+    if (apart.keys > 0) {
+      AttnArgs a = args;
+      a.apart_pass = 1;
+      a.part_k = args.apart_k, a.part_v = args.apart_v;
+      attn_launches(a, apart.plan, kBwdThreads, [&](const AttnArgs &part, unsigned groups) {
+        hipLaunchKernelGGL((attn_dkv_kernel<T, DP, VEC, 1, true>), dim3(groups), b, 0, stream,
+                           part);
+      });
+      if (apart.plan.splits > 1)
+        join(a, static_cast<int64_t>(a.n_seq) * a.apart, apart.plan.splits);
     }
   });
 }

@@ -39,6 +39,10 @@ struct AttnArgs {
   float2 *stat;          // [heads, n_q]: log2 of the denominator, -rowsum(grad_out * out)
   float *part_k, *part_v; // [splits, n_k * kv_heads, dim]
   void *gq, *gk, *gv;
+  int32_t window, sinks; // of the windowed kernels (below)
+  int32_t apart;         // first keys of each sequence whose gradients a launch of their own takes
+  int32_t apart_pass;    // whether this is that launch
+  float *apart_k, *apart_v; // its partial sums: [splits, n_seq * apart * kv_heads, dim]
 };
 
 // One sequence of the packed rows, clamped to the buffers whatever the
@@ -127,6 +131,62 @@ __device__ __forceinline__ AttnSeq key_tile(const AttnArgs &a, int bm, int32_t t
   room = wave_uniform(room);
   return wave_uniform(q);
 }
+
+// Attention inside a window: query row i stands at key i + shift, shift = Lk -
+// Lq, and sees the keys less than `window` away, the sequence's first `sinks`
+// keys, and of both under a causal mask none behind its own place: keys [lo,
+// hi) and [0, first). All three grow with i.
+struct LocalKeys {
+  int32_t lo, hi, first;
+};
+__device__ __forceinline__ LocalKeys local_keys(const AttnArgs &a, const AttnSeq &sq, int32_t i) {
+  const int64_t at = i + static_cast<int64_t>(sq.lk) - sq.lq, lk = sq.lk;
+  auto within = [](int64_t v, int64_t to) { return v < 0 ? 0 : (v > to ? to : v); };
+  LocalKeys k;
+  k.hi = static_cast<int32_t>(within(a.causal ? at + 1 : at + a.window, lk));
+  k.lo = static_cast<int32_t>(within(at - a.window + 1, k.hi));
+  k.first = static_cast<int32_t>(min<int64_t>(a.sinks, a.causal ? k.hi : lk));
+  return k;
+}
+__device__ __forceinline__ LocalKeys wave_uniform(LocalKeys k) {
+  return {wave_uniform(k.lo), wave_uniform(k.hi), wave_uniform(k.first)};
+}
+
+// The query rows that see key j: [lo, hi). Both grow with j among the sinks and
+// among the others, and no sink's lo is above another key's.
+struct LocalRows {
+  int32_t lo, hi;
+};
+__device__ __forceinline__ LocalRows local_rows(const AttnArgs &a, const AttnSeq &sq, int32_t j) {
+  const int64_t at = j - (static_cast<int64_t>(sq.lk) - sq.lq), lq = sq.lq;
+  auto within = [&](int64_t v) { return static_cast<int32_t>(v < 0 ? 0 : (v > lq ? lq : v)); };
+  if (j < a.sinks)
+    return {a.causal ? within(at) : 0, sq.lq};
+  return {within(a.causal ? at : at - a.window + 1), within(at + a.window)};
+}
+
+// What a run of rows first .. last needs of the keys, in tiles of kBN: those of
+// the sinks, then those of the windows.
+template <int kBN> struct LocalTiles {
+  LocalKeys a, b; // of the first and the last row
+  int32_t sinks, from, count;
+  __device__ __forceinline__ LocalTiles(const LocalKeys &first, const LocalKeys &last)
+      : a(wave_uniform(first)), b(wave_uniform(last)) {
+    sinks = (b.first + kBN - 1) / kBN;
+    from = max(a.lo / kBN, sinks);
+    count = sinks + max((b.hi + kBN - 1) / kBN - from, 0);
+  }
+  __device__ __forceinline__ int32_t tile(int32_t n) const {
+    return n < sinks ? n : n - sinks + from;
+  }
+  // whether every row sees all keys j0 .. j1 - 1; whether some row sees some
+  __device__ __forceinline__ bool all(int32_t j0, int32_t j1) const {
+    return (j0 >= b.lo && j1 <= a.hi) || j1 <= a.first;
+  }
+  __device__ __forceinline__ bool some(int32_t j0, int32_t j1) const {
+    return (j0 < b.hi && j1 > a.lo) || j0 < b.first;
+  }
+};
 
 // Workgroup -> (tile, key head, split) of a launch over tiles x key heads x
 // splits. Workgroups are dealt to the 8 XCDs round-robin, and what reads the

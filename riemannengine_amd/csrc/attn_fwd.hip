@@ -89,7 +89,11 @@ __device__ void finish_row(const AttnArgs &a, int64_t row, int32_t head, float o
 // for single tokens (32 over caches of 1 to 16384, 8 key heads of 128: 4.7 TB/s).
 // Taken back as no faster: the next tile's scores computed beside this one's
 // softmax, row sums as a product with ones, priorities of waves.
-template <typename T, int DP, bool VEC, int W>
+//
+// LOCAL: inside a window (LocalKeys). A workgroup goes through the tiles of its
+// rows' sinks and windows alone; blocks that all of a wave's rows see whole are
+// not masked.
+template <typename T, int DP, bool VEC, int W, bool LOCAL>
 __global__ __launch_bounds__(kFwdThreads, (FwdShape<T, DP, W>::kOccupancy)) void
 attn_fwd_kernel(AttnArgs a) {
   using Shape = FwdShape<T, DP, W>;
@@ -131,8 +135,16 @@ attn_fwd_kernel(AttnArgs a) {
   const int32_t wave_lim =
       wave_uniform(wave0 < n_rows ? sees(min(wave0 + 32, n_rows) - 1) : 0);
   const int32_t wave_full = wave_uniform(wave0 < n_rows ? sees(wave0) : 0);
+  using Tiles = LocalTiles<kBN>;
+  auto local = [&](int32_t r) {
+    return LOCAL && r >= 0 ? local_keys(a, sq, r / a.group) : LocalKeys{0, 0, 0};
+  };
+  const LocalKeys mine = local(row_ok ? row : -1);
+  const Tiles wg(local(row0), local(min(row0 + Shape::kRows, n_rows) - 1));
+  const bool any_row = wave0 < n_rows;
+  const Tiles wave(local(any_row ? wave0 : -1), local(any_row ? min(wave0 + 32, n_rows) - 1 : -1));
   // this workgroup's tiles [kt0, kt1) of keys; a wave's first and step
-  int32_t kt0 = 0, kt1 = (wg_lim + kBN - 1) / kBN;
+  int32_t kt0 = 0, kt1 = LOCAL ? wg.count : (wg_lim + kBN - 1) / kBN;
   if (W == 1 && a.splits > 1) {
     const int32_t per = (kt1 + a.splits - 1) / a.splits;
     kt0 = min(split * per, kt1);
@@ -146,7 +158,8 @@ attn_fwd_kernel(AttnArgs a) {
   ks.init(a.k_row, a.dim);
   vs.init(a.v_row, a.dim);
   char *stage = lds + (W == 1 ? w : 0) * Shape::kBuffers * 2 * Shape::kTileBytes;
-  auto issue = [&](int32_t kt, int buf) {
+  auto issue = [&](int32_t n, int buf) {
+    const int32_t kt = LOCAL ? wg.tile(n) : n;
     char *to = stage + buf * 2 * Shape::kTileBytes;
     ks.issue(to, kp + static_cast<int64_t>(kt) * kBN * a.k_row, a.k_row, sq.lk - kt * kBN,
              a.dim);
@@ -172,19 +185,23 @@ attn_fwd_kernel(AttnArgs a) {
   // entry's zero times one would be NaN, so they are zeroed in LDS, and the rows
   // that see them get them at the end.
   bool left_out = false;
+  auto cut = [&](int32_t kt) { // LOCAL: tile kt is such a tile
+    return !wg.all(kt * kBN, min((kt + 1) * kBN, sq.lk));
+  };
   if (W > 1 && threadIdx.x == 0)
     any_left_out = 0; // behind the barrier of the first turn
 
   const typename Tile::Lane lane_at = Tile::lane_addresses();
   const uint32_t stage_at = lds_address(stage);
   int buf = 0;
-  for (int32_t kt = first; kt < kt1; kt += step) {
+  for (int32_t n = first; n < kt1; n += step) {
+    const int32_t kt = LOCAL ? wg.tile(n) : n;
     // this tile has landed; then every wave is past its reads of the other
     // buffer, which the next tile's loads overwrite
     wait_stream();
     if constexpr (W > 1)
       __syncthreads();
-    if (wg_full < wg_lim && (kt + 1) * kBN > wg_full) {
+    if (LOCAL ? cut(kt) : wg_full < wg_lim && (kt + 1) * kBN > wg_full) {
       rare_path();
       const bool found = Tile::template zero_not_finite<false, kBN, W == 1 ? 1 : kFwdWaves>(
           stage_at + buf * 2 * Shape::kTileBytes + Shape::kTileBytes, W == 1 ? 0 : w);
@@ -199,10 +216,10 @@ attn_fwd_kernel(AttnArgs a) {
     }
     const typename Tile::Lane at =
         lane_at.in(stage_at + buf * 2 * Shape::kTileBytes + b0 * (32 / 4) * Tile::kGroup);
-    if (Shape::kBuffers == 2 && kt + step < kt1)
-      issue(kt + step, buf ^ 1);
+    if (Shape::kBuffers == 2 && n + step < kt1)
+      issue(n + step, buf ^ 1);
     const int32_t j0 = kt * kBN + 32 * b0;
-    if (W == 1 || j0 < wave_lim) {
+    if (W == 1 || (LOCAL ? wave.some(j0, j0 + 32 * kB) : j0 < wave_lim)) {
       v16f s[kB];
 #pragma unroll
       for (int b = 0; b < kB; ++b)
@@ -211,7 +228,21 @@ attn_fwd_kernel(AttnArgs a) {
       ahead<kB * Tile::kSteps, kAhead>(
           [&](int i) { return Tile::row_operand(at, 0, 32 * (i % kB), i / kB); },
           [&](int i, const Frag &x) { Tile::mma(x, qf[i / kB], s[i % kB]); });
-      if (j0 + 32 * kB > wave_full) {
+      if (LOCAL) {
+        if (!wave.all(j0, j0 + 32 * kB)) {
+          rare_path();
+#pragma unroll
+          for (int b = 0; b < kB; ++b) {
+            const int32_t at0 = j0 + 32 * b + 4 * half; // the lane's first key of the block
+            const int32_t lo = mine.lo - at0, hi = mine.hi - at0, sinks = mine.first - at0;
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+              const int j = block_row(r);
+              s[b][r] = (j >= lo && j < hi) || j < sinks ? s[b][r] : -INFINITY;
+            }
+          }
+        }
+      } else if (j0 + 32 * kB > wave_full) {
         rare_path();
 #pragma unroll
         for (int b = 0; b < kB; ++b) {
@@ -251,15 +282,25 @@ attn_fwd_kernel(AttnArgs a) {
     }
     if (Shape::kBuffers == 2) {
       buf ^= 1;
-    } else if (kt + step < kt1) {
+    } else if (n + step < kt1) {
       wait_stream();
       if constexpr (W > 1)
         __syncthreads();
-      issue(kt + step, 0);
+      issue(n + step, 0);
     }
   }
   sum = pair_sum(sum);
-  if (left_out)
+  if (LOCAL) {
+    if (left_out)
+#pragma unroll 1
+      for (int32_t n = kt0; n < kt1; ++n) {
+        const int32_t kt = wg.tile(n);
+        if (cut(kt))
+          Tile::template add_not_finite<false>(
+              vp, a.v_row, a.dim, kt * kBN, min((kt + 1) * kBN, sq.lk),
+              [&](int32_t j) { return (j >= mine.lo && j < mine.hi) || j < mine.first; }, o);
+      }
+  } else if (left_out)
     Tile::template add_not_finite<false>(vp, a.v_row, a.dim, max(wg_full - kBN, 0), wave_lim,
                                          [&](int32_t j) { return j < lim; }, o);
 
@@ -382,8 +423,9 @@ __global__ __launch_bounds__(kFwdThreads) void attn_join_kernel(AttnArgs a) {
 // another 8. (32 tokens over caches of 1 to 16384 keys, 8 key heads, 128 wide:
 // four splits 172 us, one 390. Three causal sequences of 1000, 2 heads of 96:
 // one split 26 us, three 32 and 7 to join.)
+// Inside a window a row's keys are those of its window and the sinks, at most.
 AttnPlan plan_forward(int64_t n_q, int64_t n_k, int32_t n_seq, int32_t heads, int32_t kv_heads,
-                      int32_t dim, int32_t causal, int32_t dtype) {
+                      int32_t dim, int32_t causal, int32_t dtype, const AttnWindow &window) {
   const int64_t rows = n_q * (heads / kv_heads);
   AttnPlan p{attn_waves(rows, kv_heads, dtype), 0, 1};
   p.tiles = rows / (32 * p.waves) + n_seq + 1;
@@ -396,15 +438,21 @@ AttnPlan plan_forward(int64_t n_q, int64_t n_k, int32_t n_seq, int32_t heads, in
   const double busy = static_cast<double>(rows / 32 + std::min<int64_t>(n_seq, rows)) * kv_heads;
   const bool tokens = rows <= 32 * static_cast<int64_t>(n_seq);
   const double slots = width * (f32 ? 2 : 1) <= 0.5 ? 512.0 : 256.0;
-  const double tiles =
+  int64_t keys = n_k / n_seq;
+  double tiles =
       static_cast<double>(n_k) / n_seq / (32 * kFwdWaves) * (causal && !tokens ? 0.5 : 1.0);
+  if (window.window > 0) {
+    keys = std::min<int64_t>(keys, static_cast<int64_t>(window.window) * (causal ? 1 : 2) +
+                                       window.sinks + 32 / (heads / kv_heads));
+    tiles = std::min(tiles, static_cast<double>(keys) / (32 * kFwdWaves));
+  }
   double least = 0.0;
   for (int32_t s : {1, 2, 3, 4, 6, 8, 12, 16, 24, 32, 48, 64}) {
-    if (s > 1 && n_k / n_seq < static_cast<int64_t>(kMinSplitKeys) * s)
+    if (s > 1 && keys < static_cast<int64_t>(kMinSplitKeys) * s)
       break;
     const double turn = std::ceil(tiles / s) * tile;
     const double all = std::ceil(busy * s / slots) * (8.0 + turn);
-    const double longest = 8.0 + turn * (tokens ? 3.0 : 1.5);
+    const double longest = 8.0 + turn * (window.window > 0 ? 1.0 : tokens ? 3.0 : 1.5);
     const double t = std::max(all, longest) + (s > 1 ? 8.0 : 0.0);
     if (s == 1 || t < least) {
       least = t;
@@ -416,14 +464,15 @@ AttnPlan plan_forward(int64_t n_q, int64_t n_k, int32_t n_seq, int32_t heads, in
 
 } // namespace
 
-AttnPlan attn_forward_plan(const rhip_attn &d) {
-  return plan_forward(d.n_q, d.n_k, d.n_seq, d.heads, d.kv_heads, d.dim, d.causal, d.dtype);
+AttnPlan attn_forward_plan(const rhip_attn &d, const AttnWindow &window) {
+  return plan_forward(d.n_q, d.n_k, d.n_seq, d.heads, d.kv_heads, d.dim, d.causal, d.dtype,
+                      window);
 }
 
 void attn_forward_run(const AttnArgs &args, int32_t dtype, bool vec, hipStream_t stream) {
   AttnArgs a = args;
   const AttnPlan plan = plan_forward(a.n_q, a.n_k, a.n_seq, a.heads, a.kv_heads, a.dim,
-                                     a.causal, dtype);
+                                     a.causal, dtype, {a.window, a.sinks});
   const int64_t rows = static_cast<int64_t>(a.n_q) * a.heads;
   a.splits = plan.splits;
   with_attn(dtype, a.dim, vec, [&](auto t, auto dp, auto v) {
@@ -435,8 +484,12 @@ void attn_forward_run(const AttnArgs &args, int32_t dtype, bool vec, hipStream_t
       constexpr int W = decltype(w)::value;
       const unsigned spread = spread_lds<W>(a, FwdShape<T, DP, W>::kLds);
       attn_launches(a, plan, kFwdThreads, [&](const AttnArgs &part, unsigned groups) {
-        hipLaunchKernelGGL((attn_fwd_kernel<T, DP, VEC, W>), dim3(groups), b, spread, stream,
-                           part);
+        if (a.window > 0)
+          hipLaunchKernelGGL((attn_fwd_kernel<T, DP, VEC, W, true>), dim3(groups), b, spread,
+                             stream, part);
+        else
+          hipLaunchKernelGGL((attn_fwd_kernel<T, DP, VEC, W, false>), dim3(groups), b, spread,
+                             stream, part);
       });
     });
     if (a.splits > 1) { // with W = 1, so rows for a few hundred workgroups at most

@@ -430,17 +430,21 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
       "packed_attention",
       [](const at::Tensor &query, const at::Tensor &key, const at::Tensor &value,
          const at::Tensor &query_offsets, OptTensor key_offsets, OptTensor key_lengths,
-         bool causal, c10::optional<double> scale) {
+         bool causal, c10::optional<double> scale, c10::optional<int64_t> window, int64_t sinks) {
         py::gil_scoped_release release;
         return hip_packed_attention(query, key, value, query_offsets,
                                     key_offsets.value_or(at::Tensor()),
-                                    key_lengths.value_or(at::Tensor()), causal, scale);
+                                    key_lengths.value_or(at::Tensor()), causal, scale, window,
+                                    sinks);
       },
       "softmax(scale * query key^T) value inside every packed sequence; query [rows, heads, "
-      "width], key and value [rows, key heads, width], offsets [sequences + 1].",
+      "width], key and value [rows, key heads, width], offsets [sequences + 1]. With a window, row "
+      "i of a sequence, at key p = i + keys - rows, sees the keys j with |p - j| < window and the "
+      "first `sinks` keys.",
       py::arg("query"), py::arg("key"), py::arg("value"), py::arg("query_offsets"),
       py::arg("key_offsets") = py::none(), py::arg("key_lengths") = py::none(),
-      py::arg("causal") = false, py::arg("scale") = py::none());
+      py::arg("causal") = false, py::arg("scale") = py::none(), py::arg("window") = py::none(),
+      py::arg("sinks") = 0);
   nn.def(
       "rotate_heads",
       [](const at::Tensor &input, const at::Tensor &positions, const at::Tensor &frequencies,

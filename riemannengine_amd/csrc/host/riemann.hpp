@@ -628,12 +628,15 @@ TORCH_MODULE(BasicBlock);
 // int32 or int64 [sequences + 1] (key_offsets undefined: the query's),
 // key_lengths (keys in use per sequence) may be undefined. causal: the last
 // query row of a sequence sees every key, each earlier one a key less. scale
-// defaults to 1 / sqrt(width). fp32 or bf16, width <= 128.
+// defaults to 1 / sqrt(width). fp32 or bf16, width <= 128. window: a row sees the
+// keys less than so many away from its own place (that of the last row is the
+// last key) and the sequence's first `sinks` keys.
 at::Tensor hip_packed_attention(const at::Tensor &query, const at::Tensor &key,
                                 const at::Tensor &value, const at::Tensor &query_offsets,
                                 const at::Tensor &key_offsets = at::Tensor(),
                                 const at::Tensor &key_lengths = at::Tensor(),
-                                bool causal = false, c10::optional<double> scale = c10::nullopt);
+                                bool causal = false, c10::optional<double> scale = c10::nullopt,
+                                c10::optional<int64_t> window = c10::nullopt, int64_t sinks = 0);
 
 // Heads [rows, heads, width] turned by positions [rows, axes] (int32, int64 or
 // fp32; [rows] for one axis), autograd-aware: pair p of a head, elements (p,

@@ -18,6 +18,21 @@ struct Attention {
   at::Tensor q, k, v, q_offsets, k_offsets, k_lengths;
   bool causal;
   double scale;
+  int64_t window, sinks; // window 0: every key counts
+
+  rhip_attn_window local() const {
+    return {static_cast<int32_t>(window), static_cast<int32_t>(sinks)};
+  }
+  at::Tensor workspace(const rhip_attn &d, int32_t backward) const {
+    size_t bytes = 0;
+    const rhip_attn_window w = local();
+    if (window > 0)
+      check_rhip(rhip_attn_window_workspace_bytes(&d, &w, backward, &bytes),
+                 "rhip_attn_window_workspace_bytes");
+    else
+      check_rhip(rhip_attn_workspace_bytes(&d, backward, &bytes), "rhip_attn_workspace_bytes");
+    return byte_buffer(bytes, q.device());
+  }
 
   rhip_attn desc() const {
     rhip_attn d{};
@@ -52,14 +67,19 @@ struct Attention {
       else
         *rest = torch::empty({0}, q.options());
     }
-    size_t bytes = 0;
-    check_rhip(rhip_attn_workspace_bytes(&d, 0, &bytes), "rhip_attn_workspace_bytes");
-    auto ws = byte_buffer(bytes, dev);
-    check_rhip(rhip_attn_forward(&d, q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(),
-                                 lse && present(*rest) ? rest->data_ptr() : nullptr,
-                                 lse ? lse->data_ptr<float>() : nullptr, ws.data_ptr(),
-                                 ws.numel(), stream_of(dev)),
-               "rhip_attn_forward");
+    auto ws = workspace(d, 0);
+    void *rest_p = lse && present(*rest) ? rest->data_ptr() : nullptr;
+    float *lse_p = lse ? lse->data_ptr<float>() : nullptr;
+    const rhip_attn_window w = local();
+    if (window > 0)
+      check_rhip(rhip_attn_window_forward(&d, &w, q.data_ptr(), k.data_ptr(), v.data_ptr(),
+                                          out.data_ptr(), rest_p, lse_p, ws.data_ptr(),
+                                          ws.numel(), stream_of(dev)),
+                 "rhip_attn_window_forward");
+    else
+      check_rhip(rhip_attn_forward(&d, q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(),
+                                   rest_p, lse_p, ws.data_ptr(), ws.numel(), stream_of(dev)),
+                 "rhip_attn_forward");
     return out;
   }
 };
@@ -67,20 +87,23 @@ struct Attention {
 struct HipAttentionFunction : public torch::autograd::Function<HipAttentionFunction> {
   static at::Tensor forward(AutogradContext *ctx, at::Tensor q, at::Tensor k, at::Tensor v,
                             at::Tensor q_offsets, at::Tensor k_offsets, at::Tensor k_lengths,
-                            bool causal, double scale) {
-    const Attention a{q, k, v, q_offsets, k_offsets, k_lengths, causal, scale};
+                            bool causal, double scale, int64_t window, int64_t sinks) {
+    const Attention a{q, k, v, q_offsets, k_offsets, k_lengths, causal, scale, window, sinks};
     at::Tensor lse, rest;
     auto out = a.forward(&lse, &rest);
     ctx->save_for_backward({q, k, v, out, lse, q_offsets, k_offsets, k_lengths, rest});
     ctx->saved_data["causal"] = causal;
     ctx->saved_data["scale"] = scale;
+    ctx->saved_data["window"] = window;
+    ctx->saved_data["sinks"] = sinks;
     return out;
   }
 
   static tensor_list backward(AutogradContext *ctx, tensor_list grads) {
     auto s = ctx->get_saved_variables();
     const Attention a{s[0], s[1], s[2], s[5], s[6], s[7], ctx->saved_data["causal"].toBool(),
-                      ctx->saved_data["scale"].toDouble()};
+                      ctx->saved_data["scale"].toDouble(), ctx->saved_data["window"].toInt(),
+                      ctx->saved_data["sinks"].toInt()};
     const auto dev = a.q.device();
     at::DeviceGuard guard(dev);
     const rhip_attn d = a.desc();
@@ -92,16 +115,24 @@ struct HipAttentionFunction : public torch::autograd::Function<HipAttentionFunct
       gk = torch::empty(a.k.sizes(), a.k.options());
       gv = torch::empty(a.v.sizes(), a.v.options());
     }
-    size_t bytes = 0;
-    check_rhip(rhip_attn_workspace_bytes(&d, 1, &bytes), "rhip_attn_workspace_bytes");
-    auto ws = byte_buffer(bytes, dev);
-    check_rhip(rhip_attn_backward(&d, go.data_ptr(), go.stride(0), go.stride(1), a.q.data_ptr(),
-                                  a.k.data_ptr(), a.v.data_ptr(), s[3].data_ptr(),
-                                  present(s[8]) ? s[8].data_ptr() : nullptr,
-                                  s[4].data_ptr<float>(), vptr_mut(gq), vptr_mut(gk),
-                                  vptr_mut(gv), ws.data_ptr(), ws.numel(), stream_of(dev)),
-               "rhip_attn_backward");
-    return {gq, gk, gv, {}, {}, {}, {}, {}};
+    auto ws = a.workspace(d, 1);
+    const rhip_attn_window w = a.local();
+    void *rest = present(s[8]) ? s[8].data_ptr() : nullptr;
+    if (a.window > 0)
+      check_rhip(rhip_attn_window_backward(&d, &w, go.data_ptr(), go.stride(0), go.stride(1),
+                                           a.q.data_ptr(), a.k.data_ptr(), a.v.data_ptr(),
+                                           s[3].data_ptr(), rest, s[4].data_ptr<float>(),
+                                           vptr_mut(gq), vptr_mut(gk), vptr_mut(gv),
+                                           ws.data_ptr(), ws.numel(), stream_of(dev)),
+                 "rhip_attn_window_backward");
+    else
+      check_rhip(rhip_attn_backward(&d, go.data_ptr(), go.stride(0), go.stride(1),
+                                    a.q.data_ptr(), a.k.data_ptr(), a.v.data_ptr(),
+                                    s[3].data_ptr(), rest, s[4].data_ptr<float>(), vptr_mut(gq),
+                                    vptr_mut(gk), vptr_mut(gv), ws.data_ptr(), ws.numel(),
+                                    stream_of(dev)),
+                 "rhip_attn_backward");
+    return {gq, gk, gv, {}, {}, {}, {}, {}, {}, {}};
   }
 };
 
@@ -250,7 +281,8 @@ Scenes scenes_of(const SparseTensor &input) {
 at::Tensor hip_packed_attention(const at::Tensor &query, const at::Tensor &key,
                                 const at::Tensor &value, const at::Tensor &query_offsets,
                                 const at::Tensor &key_offsets, const at::Tensor &key_lengths,
-                                bool causal, c10::optional<double> scale) {
+                                bool causal, c10::optional<double> scale,
+                                c10::optional<int64_t> window, int64_t sinks) {
   TORCH_CHECK(query.is_cuda() && key.device() == query.device() &&
                   value.device() == query.device(),
               "query, key and value must be on one device (the HIP path has no CPU fallback)");
@@ -281,10 +313,17 @@ at::Tensor hip_packed_attention(const at::Tensor &query, const at::Tensor &key,
     TORCH_CHECK(kl.numel() == qo.numel() - 1, "key lengths must hold one value per sequence");
   }
   const double s = scale.value_or(1.0 / std::sqrt(static_cast<double>(query.size(2))));
+  TORCH_CHECK(window.value_or(1) >= 1, "the window must hold at least one key, got ",
+              window.value_or(1));
+  TORCH_CHECK(sinks >= 0 && sinks <= INT32_MAX, "sinks must be a number of keys, got ", sinks);
+  TORCH_CHECK(window.has_value() || sinks == 0, "sinks stand beside a window: without one every "
+                                                "key counts");
+  // no sequence has 2^31 keys
+  const int64_t w = std::min<int64_t>(window.value_or(0), INT32_MAX);
   auto q = dense_last(query), k = dense_last(key), v = dense_last(value);
   if (through_autograd({query, key, value}))
-    return HipAttentionFunction::apply(q, k, v, qo, ko, or_empty(kl, qo), causal, s);
-  return Attention{q, k, v, qo, ko, kl, causal, s}.forward(nullptr, nullptr);
+    return HipAttentionFunction::apply(q, k, v, qo, ko, or_empty(kl, qo), causal, s, w, sinks);
+  return Attention{q, k, v, qo, ko, kl, causal, s, w, sinks}.forward(nullptr, nullptr);
 }
 
 at::Tensor hip_layer_norm(const at::Tensor &input, const at::Tensor &weight,
