@@ -29,6 +29,9 @@ namespace rhip {
 namespace {
 
 constexpr int kGatedMaxRows = 64; // of the kernel for few rows
+constexpr int kGatedThreads = 256; // of the kernels that join and pack
+using LargeTiles = GemmShape<2, 4, 4, 2>; // 256 x 256, eight waves, one workgroup to a CU
+using SmallTiles = GemmShape<2, 2, 2, 2>; // 128 x 128, four waves, two workgroups
 
 // ------------------------------------------------------------- activation
 
@@ -61,26 +64,58 @@ struct GatedSaved { // planes [n, pitch]
   uint16_t *low; // bf16: the eight bits behind g's and u's planes
 };
 
-template <typename T>
-__device__ __forceinline__ void load_saved(const GatedSaved &s, int64_t at, float (&g)[4],
-                                           float (&u)[4]) {
-  if constexpr (sizeof(T) == 4) {
-    const v4f a = *reinterpret_cast<const v4f *>(static_cast<const float *>(s.g) + at);
-    const v4f b = *reinterpret_cast<const v4f *>(static_cast<const float *>(s.u) + at);
+// E values of 32 bits from one 16-byte chunk (fp32) or of 16 bits (bf16's planes).
+template <typename T> struct SavedChunk {
+  static constexpr int E = 16 / sizeof(T);
+  // whole 16-byte chunks of the planes at `at`
+  __device__ static __forceinline__ void load(const GatedSaved &s, int64_t at, float (&g)[E],
+                                              float (&u)[E]) {
+    if constexpr (sizeof(T) == 4) {
+      const v4f a = *reinterpret_cast<const v4f *>(static_cast<const float *>(s.g) + at);
+      const v4f b = *reinterpret_cast<const v4f *>(static_cast<const float *>(s.u) + at);
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
-      g[i] = a[i], u[i] = b[i];
-  } else {
-    uint16_t a[4], b[4], c[4];
-    __builtin_memcpy(a, __builtin_assume_aligned(static_cast<const uint16_t *>(s.g) + at, 8), 8);
-    __builtin_memcpy(b, __builtin_assume_aligned(static_cast<const uint16_t *>(s.u) + at, 8), 8);
-    __builtin_memcpy(c, __builtin_assume_aligned(s.low + at, 8), 8);
+      for (int i = 0; i < E; ++i)
+        g[i] = a[i], u[i] = b[i];
+    } else {
+      const v4u a = *reinterpret_cast<const v4u *>(static_cast<const uint16_t *>(s.g) + at);
+      const v4u b = *reinterpret_cast<const v4u *>(static_cast<const uint16_t *>(s.u) + at);
+      const v4u c = *reinterpret_cast<const v4u *>(s.low + at);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      g[i] = __uint_as_float(static_cast<uint32_t>(a[i]) << 16 | (c[i] & 0xff) << 8);
-      u[i] = __uint_as_float(static_cast<uint32_t>(b[i]) << 16 | (c[i] & 0xff00));
+      for (int i = 0; i < E; ++i) {
+        const int sh = 16 * (i % 2);
+        g[i] = __uint_as_float(a[i / 2] >> sh << 16 | ((c[i / 2] >> sh) & 0xffu) << 8);
+        u[i] = __uint_as_float(b[i / 2] >> sh << 16 | ((c[i / 2] >> sh) & 0xff00u));
+      }
     }
   }
+  __device__ static __forceinline__ void store(const GatedSaved &s, int64_t at,
+                                               const float (&g)[E], const float (&u)[E]) {
+    if constexpr (sizeof(T) == 4) {
+      *reinterpret_cast<v4f *>(static_cast<float *>(s.g) + at) = v4f{g[0], g[1], g[2], g[3]};
+      *reinterpret_cast<v4f *>(static_cast<float *>(s.u) + at) = v4f{u[0], u[1], u[2], u[3]};
+    } else {
+      v4u a, b, c;
+#pragma unroll
+      for (int i = 0; i < E; i += 2) {
+        const uint32_t g0 = upper24(g[i]), g1 = upper24(g[i + 1]);
+        const uint32_t u0 = upper24(u[i]), u1 = upper24(u[i + 1]);
+        a[i / 2] = g0 >> 8 | (g1 >> 8) << 16;
+        b[i / 2] = u0 >> 8 | (u1 >> 8) << 16;
+        c[i / 2] = (g0 & 0xffu) | (u0 & 0xffu) << 8 | (g1 & 0xffu) << 16 | (u1 & 0xffu) << 24;
+      }
+      *reinterpret_cast<v4u *>(static_cast<uint16_t *>(s.g) + at) = a;
+      *reinterpret_cast<v4u *>(static_cast<uint16_t *>(s.u) + at) = b;
+      *reinterpret_cast<v4u *>(s.low + at) = c;
+    }
+  }
+};
+
+template <typename T, int E> __device__ __forceinline__ void put_chunk(T *p, const float (&v)[E]) {
+  T e[E];
+#pragma unroll
+  for (int i = 0; i < E; ++i)
+    e[i] = from_f32<T>(v[i]);
+  *reinterpret_cast<v4u *>(p) = __builtin_bit_cast(v4u, e);
 }
 
 // ---------------------------------------------------------------- products
@@ -108,10 +143,56 @@ struct GatedArgs {
   int32_t kind; // activation
 };
 
-template <typename T, int NI, int NJ, bool YACROSS, bool XACROSS, GemmPair PAIR, GatedStage STAGE>
-__global__ __launch_bounds__(kGemmThreads, (NI * NJ > 4 ? 1 : 2)) void
-gated_product_kernel(GatedArgs a) {
-  using P = Gemm<T, NI, NJ, YACROSS, XACROSS, PAIR>;
+// One 16-byte chunk (of T) of the results' rows: h and the saved planes from g
+// and u (v[0], v[1]), or dg and du from dh (v[0]). The columns behind the last,
+// `left` away, which fill the rows to whole chunks, are zeros.
+template <typename T, GatedStage STAGE>
+__device__ __forceinline__ void finish_chunk(const GatedArgs &a, int64_t at, int32_t left,
+                                             float (&v)[2][16 / sizeof(T)]) {
+  constexpr int E = 16 / sizeof(T);
+  float g[E], u[E], o[E];
+  if constexpr (STAGE == kProject) {
+#pragma unroll
+    for (int i = 0; i < E; ++i) {
+      g[i] = i < left ? v[0][i] : 0.f;
+      u[i] = i < left ? v[1][i] : 0.f;
+      float d;
+      o[i] = activation<T>(a.kind, g[i], d) * u[i];
+    }
+    put_chunk(static_cast<T *>(a.saved.h) + at, o);
+    if (a.keep)
+      SavedChunk<T>::store(a.saved, at, g, u);
+  } else {
+    SavedChunk<T>::load(a.saved, at, g, u);
+#pragma unroll
+    for (int i = 0; i < E; ++i) {
+      const float dh = i < left ? v[0][i] : 0.f;
+      float d;
+      const float act = activation<T>(a.kind, g[i], d);
+      o[i] = dh * u[i] * d;
+      u[i] = dh * act;
+    }
+    put_chunk(static_cast<T *>(a.dg) + at, o);
+    put_chunk(static_cast<T *>(a.du) + at, u);
+  }
+}
+
+// E fp32 values of a strip's row.
+template <typename S, int E>
+__device__ __forceinline__ void strip_values(const char *strip, int r, int c, float (&v)[E]) {
+#pragma unroll
+  for (int i = 0; i < E; i += 4) {
+    const v4u u = S::chunk(strip, r, c + i);
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      v[i + e] = __uint_as_float(u[e]);
+  }
+}
+
+template <typename T, typename SHAPE, bool YACROSS, bool XACROSS, GemmPair PAIR, GatedStage STAGE>
+__global__ __launch_bounds__(SHAPE::kThreads, 2) void gated_product_kernel(GatedArgs a) {
+  using P = Gemm<T, SHAPE, YACROSS, XACROSS, PAIR>;
+  constexpr int NI = P::NI, NJ = P::NJ, E = 16 / sizeof(T);
   __shared__ alignas(16) char lds[P::kLds];
   int32_t ti, tj, layer;
   if (!gemm_tile(a.tiles_i, a.tiles_j, a.layers, ti, tj, layer))
@@ -124,191 +205,113 @@ gated_product_kernel(GatedArgs a) {
   v16f acc[NJ][NI];
   P::run(lds, a.y, static_cast<const T *>(a.y.p[which]), a.x, i0, j0, kt0, kt1, acc);
 
-  const int w = wave_uniform(threadIdx.x / kWave), half = lane_id() >> 5;
+  const int w = wave_uniform(threadIdx.x / kWave);
   constexpr int NB = NJ / kHalf; // blocks of columns of a wave
-  const int32_t col0 = j0 + (w % 2) * NB * 32;
-  char *strip = lds + w * (P::kLds / 4);
-  // the columns behind the last, which fill h's rows to whole chunks, are zeros
-  if ((STAGE == kProject || STAGE == kHidden) && col0 + NB * 32 > a.cols) {
-    rare_path();
-#pragma unroll
-    for (int c = 0; c < NJ; ++c)
-#pragma unroll
-      for (int r = 0; r < 16; ++r)
-        if (col0 + c % NB * 32 + block_row(r) + 4 * half >= a.cols) {
-#pragma unroll
-          for (int b = 0; b < NI; ++b)
-            acc[c][b][r] = 0.f;
-        }
-  }
+  const int32_t col0 = j0 + (w % P::WJ) * NB * 32;
+  char *strip = lds + w * (P::kLds / SHAPE::kWaves);
 #pragma unroll
   for (int b = 0; b < NI; ++b) {
-    const int32_t row0 = i0 + ((w / 2) * NI + b) * 32;
-    const int32_t rows = a.rows - row0, mine = row0 + (lane_id() & 31);
-    const int64_t at = row0 * a.pitch + col0;
-    if constexpr (STAGE == kProject) {
-      const int32_t cols = static_cast<int32_t>(a.pitch) - col0;
-      using S = GemmStrip<T, NB>;
-      auto g = [&](int c, int r) { return acc[c][b][r]; };
-      auto u = [&](int c, int r) { return acc[c + NB][b][r]; };
-      S::store(strip, static_cast<T *>(a.saved.h) + at, a.pitch, rows, cols, [&](int c, int r) {
-        float d;
-        return from_f32<T>(activation<T>(a.kind, g(c, r), d) * u(c, r));
+    const int32_t row0 = i0 + ((w / P::WJ) * NI + b) * 32;
+    const int32_t rows = a.rows - row0;
+    if constexpr (STAGE == kProject || STAGE == kHidden) {
+      using S = GemmStrip<float, NB>;
+      static_assert(kHalf * S::kBytes <= P::kLds / SHAPE::kWaves, "a wave's strips fit its LDS");
+      S::put(strip, [&](int c, int r) { return acc[c][b][r]; });
+      if constexpr (STAGE == kProject)
+        S::put(strip + S::kBytes, [&](int c, int r) { return acc[c + NB][b][r]; });
+      __builtin_amdgcn_wave_barrier();
+      S::template walk<E>([&](int r, int c) {
+        if (r < rows && col0 + c < a.pitch) {
+          float v[2][E];
+          strip_values<S, E>(strip, r, c, v[0]);
+          if constexpr (STAGE == kProject)
+            strip_values<S, E>(strip + S::kBytes, r, c, v[1]);
+          finish_chunk<T, STAGE>(a, (row0 + static_cast<int64_t>(r)) * a.pitch + col0 + c,
+                                 a.cols - col0 - c, v);
+        }
       });
-      if (a.keep) {
-        if constexpr (sizeof(T) == 4) {
-          S::store(strip, static_cast<float *>(a.saved.g) + at, a.pitch, rows, cols, g);
-          S::store(strip, static_cast<float *>(a.saved.u) + at, a.pitch, rows, cols, u);
-        } else {
-          using B = GemmStrip<uint16_t, NB>;
-          B::store(strip, static_cast<uint16_t *>(a.saved.g) + at, a.pitch, rows, cols,
-                   [&](int c, int r) { return static_cast<uint16_t>(upper24(g(c, r)) >> 8); });
-          B::store(strip, static_cast<uint16_t *>(a.saved.u) + at, a.pitch, rows, cols,
-                   [&](int c, int r) { return static_cast<uint16_t>(upper24(u(c, r)) >> 8); });
-          B::store(strip, a.saved.low + at, a.pitch, rows, cols, [&](int c, int r) {
-            return static_cast<uint16_t>((upper24(g(c, r)) & 0xff) |
-                                         (upper24(u(c, r)) & 0xff) << 8);
-          });
-        }
-      }
     } else if constexpr (STAGE == kPlain) {
-      GemmStrip<T, NB>::store(
-          strip, static_cast<T *>(a.out[which]) + row0 * a.out_row + col0, a.out_row, rows,
-          a.cols - col0, [&](int c, int r) { return from_f32<T>(acc[c][b][r]); });
-    } else if constexpr (STAGE == kHidden) {
-      const int32_t cols = static_cast<int32_t>(a.pitch) - col0;
-#pragma unroll
-      for (int c = 0; c < NB; ++c)
-#pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          const int32_t col = 32 * c + 8 * q + 4 * half;
-          float g[4] = {0.f, 0.f, 0.f, 0.f}, u[4] = {0.f, 0.f, 0.f, 0.f};
-          if (mine < a.rows && col < cols)
-            load_saved<T>(a.saved, mine * a.pitch + col0 + col, g, u);
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            float d;
-            const float dh = acc[c][b][4 * q + e], v = activation<T>(a.kind, g[e], d);
-            acc[c][b][4 * q + e] = dh * v;
-            g[e] = dh * u[e] * d;
-          }
-          T e4[4];
-#pragma unroll
-          for (int e = 0; e < 4; ++e)
-            e4[e] = from_f32<T>(g[e]);
-          __builtin_memcpy(__builtin_assume_aligned(strip + (lane_id() & 31) *
-                                                                GemmStrip<T, NB>::kPitch +
-                                                        col * sizeof(T),
-                                                    4 * sizeof(T)),
-                           e4, sizeof(e4));
-        }
-      GemmStrip<T, NB>::flush(strip, static_cast<T *>(a.dg) + at, a.pitch, rows, cols);
-      GemmStrip<T, NB>::store(strip, static_cast<T *>(a.du) + at, a.pitch, rows, cols,
-                              [&](int c, int r) { return from_f32<T>(acc[c][b][r]); });
+      using S = GemmStrip<T, NB>;
+      S::put(strip, [&](int c, int r) { return from_f32<T>(acc[c][b][r]); });
+      __builtin_amdgcn_wave_barrier();
+      T *to = static_cast<T *>(a.out[which]) + row0 * a.out_row + col0;
+      S::template walk<E>([&](int r, int c) {
+        if (r < rows)
+          store_chunk(to + r * a.out_row + c, S::chunk(strip, r, c), a.cols - col0 - c);
+      });
     } else {
+      using S = GemmStrip<float, NB>;
       float *to = a.part + static_cast<int64_t>(layer) * kHalf * a.rows * a.part_row +
                   row0 * a.part_row + col0;
 #pragma unroll
-      for (int h = 0; h < kHalf; ++h)
-        GemmStrip<float, NB>::store(
-            strip, to + h * a.rows * a.part_row, a.part_row, rows,
-            static_cast<int32_t>(a.part_row) - col0,
-            [&](int c, int r) { return acc[c + h * NB][b][r]; });
+      for (int h = 0; h < kHalf; ++h) {
+        S::put(strip, [&](int c, int r) { return acc[c + h * NB][b][r]; });
+        __builtin_amdgcn_wave_barrier();
+        S::template walk<4>([&](int r, int c) {
+          if (r < rows && col0 + c < a.part_row)
+            *reinterpret_cast<v4u *>(to + h * a.rows * a.part_row + r * a.part_row + c) =
+                S::chunk(strip, r, c);
+        });
+        __builtin_amdgcn_wave_barrier();
+      }
     }
+    __builtin_amdgcn_wave_barrier(); // the strip is free
   }
 }
 
-// Adds the splits' sums and finishes them as the products' own epilogues do:
-// four columns a thread (part_row is a multiple of four).
+// Adds the splits' sums and finishes them as the products' own epilogues do, a
+// 16-byte chunk (of T) a thread.
 template <typename T, GatedStage STAGE>
-__global__ __launch_bounds__(kGemmThreads) void gated_join_kernel(GatedArgs a) {
-  const int64_t quads = a.part_row / 4, total = quads * a.rows;
-  const int64_t q = static_cast<int64_t>(blockIdx.x) * kGemmThreads + threadIdx.x;
+__global__ __launch_bounds__(kGatedThreads) void gated_join_kernel(GatedArgs a) {
+  constexpr int E = STAGE == kPlain ? 4 : 16 / sizeof(T);
+  const int64_t chunks = a.part_row / E, total = chunks * a.rows;
+  const int64_t q = static_cast<int64_t>(blockIdx.x) * kGatedThreads + threadIdx.x;
   const int which = blockIdx.y;
   if (q >= total)
     return;
-  const int64_t row = q / quads, col = (q - row * quads) * 4;
+  const int64_t row = q / chunks, col = (q - row * chunks) * E;
   constexpr int kHalf = STAGE == kProject ? 2 : 1;
   const int64_t plane = static_cast<int64_t>(a.rows) * a.part_row;
-  v4f s[kHalf];
+  float v[2][E];
 #pragma unroll
-  for (int h = 0; h < kHalf; ++h)
-    s[h] = v4f{0.f, 0.f, 0.f, 0.f};
-#pragma unroll 4
-  for (int p = 0; p < a.splits; ++p)
+  for (int h = 0; h < 2; ++h)
+#pragma unroll
+    for (int i = 0; i < E; ++i)
+      v[h][i] = 0.f;
+  const float *from = a.part + static_cast<int64_t>(which) * kHalf * plane + row * a.part_row + col;
+  for (int p = 0; p < a.splits; ++p, from += a.outs * kHalf * plane)
 #pragma unroll
     for (int h = 0; h < kHalf; ++h)
-      s[h] += *reinterpret_cast<const v4f *>(
-          a.part + ((static_cast<int64_t>(p) * a.outs + which) * kHalf + h) * plane +
-          row * a.part_row + col);
-  auto put = [&](T *to, const float (&v)[4], int64_t cols) {
-    T e[4];
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
-      e[i] = from_f32<T>(v[i]);
+      for (int i = 0; i < E; i += 4) {
+        const v4f f = *reinterpret_cast<const v4f *>(from + h * plane + i);
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
-      if (col + i < cols)
-        to[i] = e[i];
-  };
-  if constexpr (STAGE == kPlain) {
-    const float v[4] = {s[0][0], s[0][1], s[0][2], s[0][3]};
-    put(static_cast<T *>(a.out[which]) + row * a.out_row + col, v, a.cols);
-    return;
-  }
-  const int64_t at = row * a.pitch + col;
-  float v[4], w[4];
-#pragma unroll
-  for (int i = 0; i < 4; ++i)
-    if (col + i >= a.cols)
-      s[0][i] = s[kHalf - 1][i] = 0.f;
-  if constexpr (STAGE == kProject) {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      float d;
-      v[i] = activation<T>(a.kind, s[0][i], d) * s[kHalf - 1][i];
-    }
-    put(static_cast<T *>(a.saved.h) + at, v, a.pitch);
-    if (a.keep) {
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const float g = s[0][i], u = s[kHalf - 1][i];
-        if constexpr (sizeof(T) == 4) {
-          static_cast<float *>(a.saved.g)[at + i] = g;
-          static_cast<float *>(a.saved.u)[at + i] = u;
-        } else {
-          static_cast<uint16_t *>(a.saved.g)[at + i] = upper24(g) >> 8;
-          static_cast<uint16_t *>(a.saved.u)[at + i] = upper24(u) >> 8;
-          a.saved.low[at + i] = (upper24(g) & 0xff) | (upper24(u) & 0xff) << 8;
-        }
+        for (int e = 0; e < 4; ++e)
+          v[h][i + e] += f[e];
       }
-    }
-  } else {
-    float g[4], u[4];
-    load_saved<T>(a.saved, at, g, u);
+  const int32_t left = static_cast<int32_t>(a.cols - col);
+  if constexpr (STAGE == kPlain) {
+    T *to = static_cast<T *>(a.out[which]) + row * a.out_row + col;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      float d;
-      const float act = activation<T>(a.kind, g[i], d);
-      v[i] = s[0][i] * u[i] * d;
-      w[i] = s[0][i] * act;
-    }
-    put(static_cast<T *>(a.dg) + at, v, a.pitch);
-    put(static_cast<T *>(a.du) + at, w, a.pitch);
+    for (int i = 0; i < E; ++i)
+      if (i < left)
+        to[i] = from_f32<T>(v[0][i]);
+  } else {
+    finish_chunk<T, STAGE>(a, row * a.pitch + col, left, v);
   }
 }
 
 // rows of `cols` elements at p, row stride `row`, as rows of `pitch` elements
 // (whole 16-byte chunks), zeros behind `cols`.
 template <typename T>
-__global__ __launch_bounds__(kGemmThreads) void gated_pack_kernel(const T *p, int64_t row,
+__global__ __launch_bounds__(kGatedThreads) void gated_pack_kernel(const T *p, int64_t row,
                                                                   int32_t rows, int32_t cols,
                                                                   T *out, int32_t pitch) {
   using K = RowChunk<T>;
   const int32_t chunks = pitch / K::V;
-  for (int64_t q = static_cast<int64_t>(blockIdx.x) * kGemmThreads + threadIdx.x;
+  for (int64_t q = static_cast<int64_t>(blockIdx.x) * kGatedThreads + threadIdx.x;
        q < static_cast<int64_t>(rows) * chunks;
-       q += static_cast<int64_t>(gridDim.x) * kGemmThreads) {
+       q += static_cast<int64_t>(gridDim.x) * kGatedThreads) {
     const int64_t r = q / chunks;
     const int32_t c = static_cast<int32_t>(q - r * chunks) * K::V;
     *reinterpret_cast<v4u *>(out + r * pitch + c) = K::fetch(p + r * row + c, cols - c, false);
@@ -495,8 +498,8 @@ template <typename T> void run_pack(const Packed &m, hipStream_t stream) {
   const int64_t chunks = m.rows * (m.row / RowChunk<T>::V);
   hipLaunchKernelGGL((gated_pack_kernel<T>),
                      dim3(static_cast<unsigned>(
-                         std::min<int64_t>(ceil_div(chunks, kGemmThreads), 1 << 20))),
-                     dim3(kGemmThreads), 0, stream, static_cast<const T *>(m.src), m.src_row,
+                         std::min<int64_t>(ceil_div(chunks, kGatedThreads), 1 << 20))),
+                     dim3(kGatedThreads), 0, stream, static_cast<const T *>(m.src), m.src_row,
                      m.rows, m.cols, static_cast<T *>(m.copy), static_cast<int32_t>(m.row));
   RHIP_LAUNCH_CHECK();
 }
@@ -551,34 +554,36 @@ void run_product(GatedArgs a, const ProductPlan &plan, float *part, hipStream_t 
   // h, dg and du have zeros behind the last column, up to their pitch
   a.part_row = STAGE == kPlain ? static_cast<int64_t>(align_up(static_cast<size_t>(a.cols), 4))
                                : a.pitch;
-  auto launch = [&](auto n, auto stage) {
-    constexpr int N = decltype(n)::value;
+  auto launch = [&](auto shape, auto stage) {
+    using SHAPE = decltype(shape);
     constexpr GatedStage S = static_cast<GatedStage>(decltype(stage)::value);
-    a.tiles_i = static_cast<int32_t>(ceil_div(a.rows, 64 * N));
-    a.tiles_j = static_cast<int32_t>(ceil_div(a.cols, 64 * N / kHalf));
+    a.tiles_i = static_cast<int32_t>(ceil_div(a.rows, SHAPE::BI));
+    a.tiles_j = static_cast<int32_t>(ceil_div(a.cols, SHAPE::BJ / kHalf));
     const int64_t tiles = static_cast<int64_t>(a.tiles_i) * a.tiles_j * a.layers;
-    if (gemm_grid(tiles) > max_groups(kGemmThreads))
+    if (gemm_grid(tiles) > max_groups(SHAPE::kThreads))
       throw Error(RHIP_ERR_UNSUPPORTED, "too many tiles");
-    hipLaunchKernelGGL((gated_product_kernel<T, N, N, YACROSS, XACROSS, PAIR, S>),
-                       dim3(static_cast<unsigned>(gemm_grid(tiles))), dim3(kGemmThreads), 0,
+    hipLaunchKernelGGL((gated_product_kernel<T, SHAPE, YACROSS, XACROSS, PAIR, S>),
+                       dim3(static_cast<unsigned>(gemm_grid(tiles))), dim3(SHAPE::kThreads), 0,
                        stream, a);
     RHIP_LAUNCH_CHECK();
   };
   auto sized = [&](auto stage) {
     if (plan.large)
-      launch(std::integral_constant<int, 4>{}, stage);
+      launch(LargeTiles{}, stage);
     else
-      launch(std::integral_constant<int, 2>{}, stage);
+      launch(SmallTiles{}, stage);
   };
   if (plan.splits == 1) {
     sized(std::integral_constant<int, STAGE>{});
     return;
   }
   sized(std::integral_constant<int, kPartial>{});
-  const int64_t quads = a.part_row / 4 * a.rows; // of at most kMostParts / 4
+  // of at most kMostParts values
+  const int64_t chunks =
+      a.part_row / (STAGE == kPlain ? 4 : 16 / static_cast<int64_t>(sizeof(T))) * a.rows;
   hipLaunchKernelGGL((gated_join_kernel<T, STAGE>),
-                     dim3(static_cast<unsigned>(ceil_div(quads, kGemmThreads)), a.outs),
-                     dim3(kGemmThreads), 0, stream, a);
+                     dim3(static_cast<unsigned>(ceil_div(chunks, kGatedThreads)), a.outs),
+                     dim3(kGatedThreads), 0, stream, a);
   RHIP_LAUNCH_CHECK();
 }
 

@@ -22,7 +22,6 @@
 
 namespace rhip {
 
-constexpr int kGemmThreads = 256;
 constexpr int kGemmTileBytes = 128; // of k in a tile
 constexpr int64_t kGemmMaxRow = int64_t(1) << 20; // row stride in elements
 
@@ -37,14 +36,14 @@ struct GemmSide {
   int32_t idx, k;
 };
 
-template <typename T, int B, bool ACROSS> struct GemmTile {
+template <typename T, int B, bool ACROSS, int THREADS> struct GemmTile {
   static constexpr int E = 16 / sizeof(T);
   static constexpr int kBytes = B * kGemmTileBytes;
   static constexpr int kSteps = 4; // of two chunks of k
   static constexpr int kRowBytes = ACROSS ? B * static_cast<int>(sizeof(T)) : kGemmTileBytes;
   static constexpr int kRowChunks = kRowBytes / 16;
-  static constexpr int kLoads = kBytes / 16 / kGemmThreads;
-  static constexpr int kRowsPerLoad = kGemmThreads / kRowChunks;
+  static constexpr int kLoads = kBytes / 16 / THREADS;
+  static constexpr int kRowsPerLoad = THREADS / kRowChunks;
   using Frag = typename Mfma<T>::Frag;
 
   // A lane's read addresses: k along, of the four steps; across, of up to four
@@ -129,7 +128,7 @@ template <typename T, int B, bool ACROSS> struct GemmTile {
       first[i] = opaque(!ACROSS && chunk * E >= k_left ? kBufOob : off[i]);
 #pragma unroll
     for (int i = FIRST; i < LAST; ++i)
-      dma16(rsrc, to + i * kGemmThreads * 16, first[i % kOffs] + (i - FIRST) * step);
+      dma16(rsrc, to + i * THREADS * 16, first[i % kOffs] + (i - FIRST) * step);
   }
 };
 
@@ -156,24 +155,32 @@ __device__ __forceinline__ bool gemm_tile(uint32_t tiles_i, uint32_t tiles_j, ui
 }
 inline int64_t gemm_grid(int64_t tiles) { return ceil_div(tiles, kXcds) * kXcds; }
 
+// A workgroup's waves and each wave's blocks.
+template <int WI_, int WJ_, int NI_, int NJ_> struct GemmShape {
+  static constexpr int WI = WI_, WJ = WJ_, NI = NI_, NJ = NJ_;
+  static constexpr int BI = 32 * WI * NI, BJ = 32 * WJ * NJ;
+  static constexpr int kWaves = WI * WJ, kThreads = kWaves * kWave;
+};
+
 // What the rows of X in a tile are: one matrix', the halves of two matrices'
 // tiles (the same indices of both), or the second matrix behind the first along
 // k (both sides).
 enum GemmPair { kGemmOne, kGemmHalves, kGemmBehind };
 
-// The sums of a workgroup's tile of 64 NI by 64 NJ results over its tiles of k:
-// four waves, two by two, each with NI x NJ blocks. acc[b][a]: X block b, Y
-// block a. With kGemmHalves a wave's first NJ / 2 blocks are the first
+// The sums of a workgroup's tile of results over its tiles of k: WI x WJ waves,
+// each with NI x NJ blocks of 32 by 32. acc[b][a]: X block b, Y block a. With
+// kGemmHalves a wave's first NJ / 2 blocks are the first
 // matrix', the others the second's.
 //
 // Two LDS buffers and one barrier a tile: at the last of its four steps every
 // wave has read the whole tile and the next one has landed; the loads of the
 // one after it then go where this one lay, and the last step's products run
 // while the next tile's first operands arrive.
-template <typename T, int NI, int NJ, bool YACROSS, bool XACROSS, GemmPair PAIR> struct Gemm {
-  static constexpr int BI = 64 * NI, BJ = 64 * NJ, BK = gemm_bk<T>();
-  using YTile = GemmTile<T, BI, YACROSS>;
-  using XTile = GemmTile<T, BJ, XACROSS>;
+template <typename T, typename SHAPE, bool YACROSS, bool XACROSS, GemmPair PAIR> struct Gemm {
+  static constexpr int NI = SHAPE::NI, NJ = SHAPE::NJ, WI = SHAPE::WI, WJ = SHAPE::WJ;
+  static constexpr int BI = SHAPE::BI, BJ = SHAPE::BJ, BK = gemm_bk<T>();
+  using YTile = GemmTile<T, BI, YACROSS, SHAPE::kThreads>;
+  using XTile = GemmTile<T, BJ, XACROSS, SHAPE::kThreads>;
   using Frag = typename Mfma<T>::Frag;
   static constexpr int kLds = 2 * (YTile::kBytes + XTile::kBytes);
   static_assert(PAIR != kGemmHalves || (!XACROSS && NJ % 2 == 0), "halves: k along the rows");
@@ -183,7 +190,7 @@ template <typename T, int NI, int NJ, bool YACROSS, bool XACROSS, GemmPair PAIR>
   __device__ static __forceinline__ void run(char *lds, const GemmSide &y, const T *yp,
                                              const GemmSide &x, int32_t i0, int32_t j0,
                                              int32_t kt0, int32_t kt1, v16f (&acc)[NJ][NI]) {
-    const int w = wave_uniform(threadIdx.x / kWave), wi = w / 2, wj = w % 2;
+    const int w = wave_uniform(threadIdx.x / kWave), wi = w / WJ, wj = w % WJ;
     const uint32_t base = lds_address(lds);
     constexpr int kXAt = 2 * YTile::kBytes;
     const typename YTile::Lane ya = YTile::lane(base, wi * NI);
@@ -227,7 +234,7 @@ template <typename T, int NI, int NJ, bool YACROSS, bool XACROSS, GemmPair PAIR>
 #pragma unroll
       for (int b = 0; b < NJ; ++b)
         fx[set][b] = XTile::read(xa, buf * XTile::kBytes,
-                                 b < kHalf ? b : b - kHalf + BJ / 64, step);
+                                 b < kHalf ? b : b - kHalf + WJ * kHalf, step);
     };
     auto multiply = [&](int set) {
 #pragma unroll
@@ -270,17 +277,14 @@ template <typename T, int NI, int NJ, bool YACROSS, bool XACROSS, GemmPair PAIR>
 };
 
 // A wave's 32 rows (one a lane's two halves share) of 32 N columns from blocks as
-// the products leave them, through LDS, to rows of `row` elements at p (the
-// wave's first row and column): 16 bytes a lane, neighbouring lanes
-// neighbouring bytes. f(block, r): the value of entry r. rows, cols: how many
-// of them there are. Nothing is kept past the caches: the next product reads them.
+// the products leave them, through LDS: 16 bytes a lane of the rows' values as
+// O, neighbouring lanes neighbouring bytes.
 template <typename O, int N> struct GemmStrip {
   static constexpr int E = 16 / sizeof(O);
   static constexpr int kPitch = 32 * N * static_cast<int>(sizeof(O)) + 16;
   static constexpr int kBytes = 32 * kPitch;
-  template <typename F>
-  __device__ static __forceinline__ void store(char *lds, O *p, int64_t row, int32_t rows,
-                                               int32_t cols, F &&f) {
+  // f(block, r): the value of entry r
+  template <typename F> __device__ static __forceinline__ void put(char *lds, F &&f) {
     const int l = lane_id(), half = l >> 5;
     char *mine = lds + (l & 31) * kPitch;
 #pragma unroll
@@ -295,34 +299,32 @@ template <typename O, int N> struct GemmStrip {
                                                   4 * sizeof(O)),
                          e, sizeof(e));
       }
-    flush(lds, p, row, rows, cols);
   }
-  // What lies in the strip (rows of kPitch bytes) to memory.
-  __device__ static __forceinline__ void flush(char *lds, O *p, int64_t row, int32_t rows,
-                                               int32_t cols) {
-    const int l = lane_id();
-    __builtin_amdgcn_wave_barrier();
-    constexpr int kChunks = 32 * N / E; // of a row
-#pragma unroll
-    for (int i = 0; i < 32 * kChunks / kWave; ++i) {
-      const int q = i * kWave + l, r = q / kChunks, c = q % kChunks * E;
-      const v4u u = *reinterpret_cast<const v4u *>(lds + r * kPitch + c * sizeof(O));
-      if (r < rows && c < cols) {
-        O *to = p + r * row + c;
-        if (c + E <= cols) {
-          *reinterpret_cast<v4u_any *>(to) = u;
-        } else {
-          O e[E];
-          __builtin_memcpy(e, &u, 16);
-#pragma unroll
-          for (int j = 0; j < E; ++j)
-            if (c + j < cols)
-              to[j] = e[j];
-        }
-      }
-    }
-    __builtin_amdgcn_wave_barrier();
+  // each(row, column) for the lanes' shares of LEN values of the rows at a time
+  template <int LEN, typename F> __device__ static __forceinline__ void walk(F &&each) {
+    constexpr int kChunks = 32 * N / LEN;
+#pragma unroll 1
+    for (int q = lane_id(); q < 32 * kChunks; q += kWave)
+      each(q / kChunks, q % kChunks * LEN);
+  }
+  __device__ static __forceinline__ v4u chunk(const char *lds, int r, int c) {
+    return *reinterpret_cast<const v4u *>(lds + r * kPitch + c * sizeof(O));
   }
 };
+
+// The first `left` of a 16-byte chunk's values to p, at any alignment.
+template <typename O> __device__ __forceinline__ void store_chunk(O *p, const v4u &u, int left) {
+  constexpr int E = 16 / sizeof(O);
+  if (left >= E) {
+    *reinterpret_cast<v4u_any *>(p) = u;
+  } else {
+    O e[E];
+    __builtin_memcpy(e, &u, 16);
+#pragma unroll
+    for (int i = 0; i < E; ++i)
+      if (i < left)
+        p[i] = e[i];
+  }
+}
 
 } // namespace rhip
