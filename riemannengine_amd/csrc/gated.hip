@@ -320,12 +320,14 @@ __global__ __launch_bounds__(kGatedThreads) void gated_pack_kernel(const T *p, i
 
 // ---------------------------------------------------------------- few rows
 
-// Up to 16 TB rows: a workgroup's eight waves share 16 columns (of g and u, or of
-// y) and part k among them; weights go from memory to registers and the matrix
-// cores as they come, 64 bytes of 16 rows to a load. The waves' sums are added
-// in LDS in order.
-constexpr int kFewThreads = 512;
-constexpr int kFewWaves = kFewThreads / kWave;
+// Up to 16 TB rows: a workgroup's waves share 16 columns (of g and u, or of y) and
+// part k among them; weights go from memory to registers and the matrix cores as
+// they come, 64 bytes of 16 rows to a load. The waves' sums are added in LDS in
+// order.
+//
+// Bound by memory: 32 rows, 4096 channels, 11008 hidden, bf16: g and u 40 us (4.5
+// TB/s), y 27. (In the operands' own order of lanes the loads alone took 55 and
+// 37; with each wave's k in one piece 44 and 29; without a turn ahead 52.)
 struct FewArgs {
   const void *y, *x[2]; // rows [n, k] and weights [cols, k]
   int64_t y_row, x_row[2];
@@ -337,66 +339,85 @@ struct FewArgs {
   int32_t keep, kind;
 };
 
-template <typename T, int TB, bool GATE>
-__global__ __launch_bounds__(kFewThreads) void gated_few_kernel(FewArgs a) {
+template <typename T, int TB, bool GATE, int WAVES>
+__global__ __launch_bounds__(WAVES *kWave) void gated_few_kernel(FewArgs a) {
   using M = Mfma<T>;
   using K = RowChunk<T>;
   constexpr int N = GATE ? 2 : 1, E = K::V;
   constexpr int kOuts = 256 * TB * N; // results of a workgroup
-  __shared__ float sums[kFewWaves][kOuts];
+  __shared__ float sums[WAVES][kOuts];
   const int lane = lane_id(), w = wave_uniform(threadIdx.x / kWave);
   const int32_t col0 = blockIdx.x * 16;
   const int32_t steps = (a.k + M::kCh - 1) / M::kCh;
-  const int32_t per = (steps + kFewWaves - 1) / kFewWaves;
-  const int32_t s0 = min(w * per, steps), s1 = min(s0 + per, steps);
-  const int r = lane & 15, at = (lane >> 4) * E;
+  // a quad of lanes loads 64 bytes of one row, which then go to the lanes that
+  // hold them as operands: in those lanes' own order each would cost an access
+  const int r = lane & 15, lr = lane >> 2, at = (lane & 3) * E, src = quad_src(lane);
   const T *xp[N], *yp[TB];
 #pragma unroll
   for (int i = 0; i < N; ++i)
-    xp[i] = static_cast<const T *>(a.x[i]) + min(col0 + r, a.cols - 1) * a.x_row[i] + at;
+    xp[i] = static_cast<const T *>(a.x[i]) + min(col0 + lr, a.cols - 1) * a.x_row[i] + at;
 #pragma unroll
   for (int b = 0; b < TB; ++b)
-    yp[b] = static_cast<const T *>(a.y) + min(16 * b + r, a.n - 1) * a.y_row + at;
+    yp[b] = static_cast<const T *>(a.y) + min(16 * b + lr, a.n - 1) * a.y_row + at;
   v4f acc[N][TB];
 #pragma unroll
   for (int i = 0; i < N; ++i)
 #pragma unroll
     for (int b = 0; b < TB; ++b)
       acc[i][b] = v4f{0.f, 0.f, 0.f, 0.f};
-  auto step = [&](int32_t k, auto turns, auto whole) {
-    constexpr int U = decltype(turns)::value;
-    v4u x[U][N], y[U][TB];
-    auto load = [&](const T *p, int32_t at_k) {
-      return decltype(whole)::value ? K::raw(p + at_k) : K::fetch(p + at_k, a.k - at_k - at, false);
-    };
+  // the waves take turns of two steps, so that the workgroup reads a row's bytes in
+  // order, and hold the next turn's while they multiply one's
+  constexpr int kTurn = 2;
+  struct Turn {
+    v4u x[kTurn][N], y[kTurn][TB];
+  };
+  const int32_t full = a.k / M::kCh, whole = full / kTurn * kTurn; // steps of whole chunks
+  auto load = [&](Turn &c, int32_t s) {
+    if (s >= whole)
+      return;
 #pragma unroll
-    for (int t = 0; t < U; ++t) {
+    for (int t = 0; t < kTurn; ++t) {
 #pragma unroll
       for (int i = 0; i < N; ++i)
-        x[t][i] = load(xp[i], k + t * M::kCh);
+        c.x[t][i] = K::raw(xp[i] + (s + t) * M::kCh);
 #pragma unroll
       for (int b = 0; b < TB; ++b)
-        y[t][b] = load(yp[b], k + t * M::kCh);
+        c.y[t][b] = K::raw(yp[b] + (s + t) * M::kCh);
     }
-#pragma unroll
-    for (int t = 0; t < U; ++t)
-#pragma unroll
-      for (int i = 0; i < N; ++i)
-#pragma unroll
-        for (int b = 0; b < TB; ++b)
-          M::mma(__builtin_bit_cast(typename M::Frag, x[t][i]),
-                 __builtin_bit_cast(typename M::Frag, y[t][b]), acc[i][b]);
   };
-  constexpr int kTurns = 4; // steps whose loads are in flight together
-  using One = std::integral_constant<int, 1>;
-  const int32_t full = min(s1, a.k / M::kCh); // steps with whole chunks
-  int32_t s = s0;
-  for (; s + kTurns <= full; s += kTurns)
-    step(s * M::kCh, std::integral_constant<int, kTurns>{}, std::true_type{});
-  for (; s < full; ++s)
-    step(s * M::kCh, One{}, std::true_type{});
-  for (; s < s1; ++s)
-    step(s * M::kCh, One{}, std::false_type{});
+  auto multiply = [&](const v4u (&x)[N], const v4u (&y)[TB]) {
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+#pragma unroll
+      for (int b = 0; b < TB; ++b)
+        M::mma(__builtin_bit_cast(typename M::Frag, quad_to_mfma(x[i], src)),
+               __builtin_bit_cast(typename M::Frag, quad_to_mfma(y[b], src)), acc[i][b]);
+  };
+  constexpr int32_t kStride = kTurn * WAVES;
+  Turn turns[2];
+  int32_t s = w * kTurn;
+  load(turns[0], s);
+  load(turns[1], s + kStride);
+  for (; s < whole; s += 2 * kStride)
+#pragma unroll
+    for (int d = 0; d < 2; ++d)
+      if (s + d * kStride < whole) {
+#pragma unroll
+        for (int t = 0; t < kTurn; ++t)
+          multiply(turns[d].x[t], turns[d].y[t]);
+        load(turns[d], s + (d + 2) * kStride);
+      }
+  for (s = whole + w; s < steps; s += WAVES) { // what no turn holds, and a partial chunk
+    v4u x[N], y[TB];
+    const int32_t k = s * M::kCh;
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+      x[i] = K::fetch(xp[i] + k, a.k - k - at, false);
+#pragma unroll
+    for (int b = 0; b < TB; ++b)
+      y[b] = K::fetch(yp[b] + k, a.k - k - at, false);
+    multiply(x, y);
+  }
   // entry e: column 4 (lane / 16) + e, row lane % 16 of block b
 #pragma unroll
   for (int i = 0; i < N; ++i)
@@ -406,7 +427,7 @@ __global__ __launch_bounds__(kFewThreads) void gated_few_kernel(FewArgs a) {
       for (int e = 0; e < 4; ++e)
         sums[w][((b * 16 + r) * N + i) * 16 + 4 * (lane >> 4) + e] = acc[i][b][e];
   __syncthreads();
-  for (int o = threadIdx.x; o < 256 * TB; o += kFewThreads) {
+  for (int o = threadIdx.x; o < 256 * TB; o += WAVES * kWave) {
     const int32_t row = o / 16, c = o % 16, col = col0 + c;
     if (row >= a.n)
       break;
@@ -415,7 +436,7 @@ __global__ __launch_bounds__(kFewThreads) void gated_few_kernel(FewArgs a) {
     for (int i = 0; i < N; ++i) {
       v[i] = 0.f;
 #pragma unroll
-      for (int p = 0; p < kFewWaves; ++p)
+      for (int p = 0; p < WAVES; ++p)
         v[i] += sums[p][(row * N + i) * 16 + c];
     }
     if constexpr (GATE) {
@@ -703,9 +724,18 @@ GatedArgs gated_args(const rhip_gated *d, const GatedSaved &saved) {
 template <typename T, bool GATE> void run_few(const FewArgs &f, hipStream_t stream) {
   const int64_t cols = GATE ? f.pitch : f.cols;
   auto launch = [&](auto tb) {
-    hipLaunchKernelGGL((gated_few_kernel<T, decltype(tb)::value, GATE>),
-                       dim3(static_cast<unsigned>(ceil_div(cols, 16))), dim3(kFewThreads), 0,
-                       stream, f);
+    const int64_t groups = ceil_div(cols, 16);
+    auto waves = [&](auto n) {
+      constexpr int kWaves = decltype(n)::value;
+      hipLaunchKernelGGL((gated_few_kernel<T, decltype(tb)::value, GATE, kWaves>),
+                         dim3(static_cast<unsigned>(groups)), dim3(kWaves * kWave), 0, stream, f);
+    };
+    // two workgroups for each CU: four waves are enough (11008 hidden: 40 us, with
+    // eight 42), else eight (4096 columns: 27 and 28)
+    if (groups >= 512)
+      waves(std::integral_constant<int, 4>{});
+    else
+      waves(std::integral_constant<int, 8>{});
     RHIP_LAUNCH_CHECK();
   };
   if (f.n <= 16)
