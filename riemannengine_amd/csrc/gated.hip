@@ -21,6 +21,8 @@
 // u are kept for the backward to 16 significant bits (a bf16 plane each, the
 // next eight bits of both in a third), so that they add nothing to that.
 #include <climits>
+#include <cmath>
+#include <initializer_list>
 #include <type_traits>
 
 #include "gemm_device.hpp"
@@ -32,6 +34,8 @@ constexpr int kGatedMaxRows = 64; // of the kernel for few rows
 constexpr int kGatedThreads = 256; // of the kernels that join and pack
 using LargeTiles = GemmShape<2, 4, 4, 2>; // 256 x 256, eight waves, one workgroup to a CU
 using SmallTiles = GemmShape<2, 2, 2, 2>; // 128 x 128, four waves, two workgroups
+using TinyTiles = GemmShape<2, 2, 1, 1>;  // 64 x 64, four
+using TinyPairs = GemmShape<2, 2, 1, 2>;  // 64 x 64 of both projections
 
 // ------------------------------------------------------------- activation
 
@@ -259,18 +263,19 @@ __global__ __launch_bounds__(SHAPE::kThreads, 2) void gated_product_kernel(Gated
   }
 }
 
-// Adds the splits' sums and finishes them as the products' own epilogues do, a
-// 16-byte chunk (of T) a thread.
-template <typename T, GatedStage STAGE>
+// Adds the splits' sums and finishes them as the products' own epilogues do: a
+// 16-byte chunk (of T) for PARTS threads, which take every PARTS-th split each
+// and add up in order in LDS (one thread for a few splits of many chunks).
+template <typename T, GatedStage STAGE, int PARTS>
 __global__ __launch_bounds__(kGatedThreads) void gated_join_kernel(GatedArgs a) {
   constexpr int E = STAGE == kPlain ? 4 : 16 / sizeof(T);
+  constexpr int kHalf = STAGE == kProject ? 2 : 1, kSums = kHalf * E;
+  constexpr int kOwn = kGatedThreads / PARTS; // chunks of a workgroup
   const int64_t chunks = a.part_row / E, total = chunks * a.rows;
-  const int64_t q = static_cast<int64_t>(blockIdx.x) * kGatedThreads + threadIdx.x;
+  const int own = threadIdx.x % kOwn, part = threadIdx.x / kOwn;
+  const int64_t q = static_cast<int64_t>(blockIdx.x) * kOwn + own;
   const int which = blockIdx.y;
-  if (q >= total)
-    return;
   const int64_t row = q / chunks, col = (q - row * chunks) * E;
-  constexpr int kHalf = STAGE == kProject ? 2 : 1;
   const int64_t plane = static_cast<int64_t>(a.rows) * a.part_row;
   float v[2][E];
 #pragma unroll
@@ -278,17 +283,38 @@ __global__ __launch_bounds__(kGatedThreads) void gated_join_kernel(GatedArgs a) 
 #pragma unroll
     for (int i = 0; i < E; ++i)
       v[h][i] = 0.f;
-  const float *from = a.part + static_cast<int64_t>(which) * kHalf * plane + row * a.part_row + col;
-  for (int p = 0; p < a.splits; ++p, from += a.outs * kHalf * plane)
+  if (q < total) {
+    const float *from =
+        a.part + static_cast<int64_t>(which) * kHalf * plane + row * a.part_row + col;
+    for (int p = part; p < a.splits; p += PARTS) {
+      const float *at = from + static_cast<int64_t>(p) * a.outs * kHalf * plane;
 #pragma unroll
-    for (int h = 0; h < kHalf; ++h)
+      for (int h = 0; h < kHalf; ++h)
 #pragma unroll
-      for (int i = 0; i < E; i += 4) {
-        const v4f f = *reinterpret_cast<const v4f *>(from + h * plane + i);
+        for (int i = 0; i < E; i += 4) {
+          const v4f f = *reinterpret_cast<const v4f *>(at + h * plane + i);
 #pragma unroll
-        for (int e = 0; e < 4; ++e)
-          v[h][i + e] += f[e];
-      }
+          for (int e = 0; e < 4; ++e)
+            v[h][i + e] += f[e];
+        }
+    }
+  }
+  if constexpr (PARTS > 1) {
+    __shared__ float sums[PARTS][kSums][kOwn];
+#pragma unroll
+    for (int i = 0; i < kSums; ++i)
+      sums[part][i][own] = v[i / E][i % E];
+    __syncthreads();
+    if (part > 0)
+      return;
+#pragma unroll
+    for (int i = 0; i < kSums; ++i)
+#pragma unroll
+      for (int p = 1; p < PARTS; ++p)
+        v[i / E][i % E] += sums[p][i][own];
+  }
+  if (q >= total)
+    return;
   const int32_t left = static_cast<int32_t>(a.cols - col);
   if constexpr (STAGE == kPlain) {
     T *to = static_cast<T *>(a.out[which]) + row * a.out_row + col;
@@ -301,20 +327,35 @@ __global__ __launch_bounds__(kGatedThreads) void gated_join_kernel(GatedArgs a) 
   }
 }
 
-// rows of `cols` elements at p, row stride `row`, as rows of `pitch` elements
-// (whole 16-byte chunks), zeros behind `cols`.
+// Matrices laid out anew, all of a pass in one launch: rows of `cols` elements at
+// p, row stride `row`, as rows of `chunks` whole 16-byte chunks, zeros behind
+// `cols`. first: the matrix' first chunk in the launch.
+constexpr int kPackMost = 5;
+struct PackJobs {
+  struct Job {
+    const void *p;
+    void *out;
+    int64_t row, first;
+    int32_t cols, chunks;
+  } job[kPackMost];
+  int32_t n;
+  int64_t total;
+};
 template <typename T>
-__global__ __launch_bounds__(kGatedThreads) void gated_pack_kernel(const T *p, int64_t row,
-                                                                  int32_t rows, int32_t cols,
-                                                                  T *out, int32_t pitch) {
+__global__ __launch_bounds__(kGatedThreads) void gated_pack_kernel(PackJobs jobs) {
   using K = RowChunk<T>;
-  const int32_t chunks = pitch / K::V;
-  for (int64_t q = static_cast<int64_t>(blockIdx.x) * kGatedThreads + threadIdx.x;
-       q < static_cast<int64_t>(rows) * chunks;
+  for (int64_t q = static_cast<int64_t>(blockIdx.x) * kGatedThreads + threadIdx.x; q < jobs.total;
        q += static_cast<int64_t>(gridDim.x) * kGatedThreads) {
-    const int64_t r = q / chunks;
-    const int32_t c = static_cast<int32_t>(q - r * chunks) * K::V;
-    *reinterpret_cast<v4u *>(out + r * pitch + c) = K::fetch(p + r * row + c, cols - c, false);
+    int k = 0;
+    while (k + 1 < jobs.n && q >= jobs.job[k + 1].first)
+      ++k;
+    const PackJobs::Job &job = jobs.job[k];
+    const int64_t at = q - job.first;
+    const int64_t r = at >> 32 ? at / job.chunks
+                               : static_cast<uint32_t>(at) / static_cast<uint32_t>(job.chunks);
+    const int32_t c = static_cast<int32_t>(at - r * job.chunks) * K::V;
+    static_cast<v4u *>(job.out)[at] =
+        K::fetch(static_cast<const T *>(job.p) + r * job.row + c, job.cols - c, false);
   }
 }
 
@@ -513,50 +554,73 @@ Packed plan_pack(Carve &cv, const void *p, int64_t row, int64_t rows, int64_t co
   }
   return m;
 }
-template <typename T> void run_pack(const Packed &m, hipStream_t stream) {
-  if (!m.copied || m.rows == 0)
+template <typename T>
+void run_packs(std::initializer_list<const Packed *> matrices, hipStream_t stream) {
+  PackJobs jobs{};
+  for (const Packed *m : matrices) {
+    if (!m->copied || m->rows == 0)
+      continue;
+    const int32_t chunks = static_cast<int32_t>(m->row / RowChunk<T>::V);
+    jobs.job[jobs.n++] = {m->src, m->copy, m->src_row, jobs.total, m->cols, chunks};
+    jobs.total += static_cast<int64_t>(m->rows) * chunks;
+  }
+  if (jobs.n == 0)
     return;
-  const int64_t chunks = m.rows * (m.row / RowChunk<T>::V);
   hipLaunchKernelGGL((gated_pack_kernel<T>),
                      dim3(static_cast<unsigned>(
-                         std::min<int64_t>(ceil_div(chunks, kGatedThreads), 1 << 20))),
-                     dim3(kGatedThreads), 0, stream, static_cast<const T *>(m.src), m.src_row,
-                     m.rows, m.cols, static_cast<T *>(m.copy), static_cast<int32_t>(m.row));
+                         std::min<int64_t>(ceil_div(jobs.total, kGatedThreads), 1 << 20))),
+                     dim3(kGatedThreads), 0, stream, jobs);
   RHIP_LAUNCH_CHECK();
 }
 
-// The tiles and splits of a product by estimated time: 256x256 tiles, one
-// workgroup to a CU, or 128x128 ones, two, in rounds over the 256 CUs.
+// The tiles and splits of a product by estimated time, in microseconds: rounds of
+// 256x256 tiles, one workgroup to a CU (bf16), 128x128 ones, two, or 64x64 ones,
+// four. A tile of k takes `alone` however few workgroups there are; the CU's
+// share of it grows with their number up to `full`. (bf16, 4000 rows, 1024
+// channels, 4096 hidden: the weights' gradients 97 us in 256x256 tiles, which
+// fill half the chip, 71 in 128x128; fp32, 500 x 500 x 500: 15 to 18 us a product
+// in 128x128 tiles.) Splits add their sums' way through memory and a launch.
+enum ProductTiles { kLargeTiles, kSmallTiles, kTinyTiles };
 struct ProductPlan {
-  bool large;
+  ProductTiles tiles;
   int32_t splits;
   size_t part; // floats of the splits' sums
 };
 constexpr int64_t kMostParts = int64_t(64) << 20; // floats, of all splits
 ProductPlan plan_product(int64_t rows, int64_t cols, int64_t k_tiles, int64_t outs, bool halves,
                          int32_t dtype) {
+  struct Cost {
+    int64_t side;
+    double slots, start, alone, full;
+  };
+  static constexpr Cost kCosts[2][3] = {
+      {{256, 256, 6.0, 7.0, 9.0}, {128, 512, 3.0, 1.8, 4.0}, {64, 1024, 2.0, 0.55, 2.2}},
+      {{256, 256, 6.0, 1.65, 1.9}, {128, 512, 3.0, 0.35, 1.15}, {64, 1024, 2.0, 0.3, 0.75}}};
+  const bool f32 = dtype == RHIP_F32;
   const int64_t part_row = static_cast<int64_t>(align_up(static_cast<size_t>(cols), 4));
   const int64_t plane = rows * part_row * outs * (halves ? 2 : 1);
   ProductPlan best{};
   double least = 0.0;
-  for (const bool large : {true, false}) {
-    const int64_t bi = large ? 256 : 128, bj = bi / (halves ? 2 : 1);
-    const int64_t tiles = ceil_div(rows, bi) * ceil_div(cols, bj) * outs;
-    const double slots = large ? 256.0 : 512.0;
-    const double turn = (large ? 2.0 : 1.35) * (dtype == RHIP_F32 ? 4.2 : 1.0); // us a tile of k
+  for (int shape = f32 ? kSmallTiles : kLargeTiles; shape <= kTinyTiles; ++shape) {
+    const Cost &c = kCosts[f32 ? 0 : 1][shape];
+    const int64_t wide = c.side / (halves && shape != kTinyTiles ? 2 : 1);
+    const int64_t tiles = ceil_div(rows, c.side) * ceil_div(cols, wide) * outs;
+    // the pair of a 64x64 tile is twice a tile's work
+    const double twice = halves && shape == kTinyTiles ? 2.0 : 1.0;
     for (int64_t s = 1; s <= 64; s *= 2) {
       if (s > 1 && (k_tiles < 4 * s || plane * s > kMostParts))
         break;
-      const double rounds = std::ceil(static_cast<double>(tiles * s) / slots);
-      // a round that does not fill the chip runs faster: less to share
-      const double fill = std::min(1.0, static_cast<double>(tiles * s) / slots);
-      double t = rounds * (3.0 + static_cast<double>(ceil_div(k_tiles, s)) * turn *
-                                     (0.75 + 0.25 * fill));
+      const double rounds = std::ceil(static_cast<double>(tiles * s) / c.slots);
+      const double fill = std::min(1.0, static_cast<double>(tiles * s) / c.slots);
+      // of bf16 the sums are waited for, of fp32 the matrix cores
+      const double turn = std::max(c.alone, c.full * (f32 ? fill : std::sqrt(fill))) * twice;
+      double t = rounds * (c.start + static_cast<double>(ceil_div(k_tiles, s)) * turn);
       if (s > 1)
         t += 4.0 + static_cast<double>(plane) * (s + 1) * 4.0 / 4.0e6;
       if (least == 0.0 || t < least) {
         least = t;
-        best = {large, static_cast<int32_t>(s), s > 1 ? static_cast<size_t>(plane * s) : 0};
+        best = {static_cast<ProductTiles>(shape), static_cast<int32_t>(s),
+                s > 1 ? static_cast<size_t>(plane * s) : 0};
       }
     }
   }
@@ -589,10 +653,12 @@ void run_product(GatedArgs a, const ProductPlan &plan, float *part, hipStream_t 
     RHIP_LAUNCH_CHECK();
   };
   auto sized = [&](auto stage) {
-    if (plan.large)
-      launch(LargeTiles{}, stage);
-    else
-      launch(SmallTiles{}, stage);
+    if constexpr (sizeof(T) == 2) // in fp32 no faster than 128x128 tiles
+      if (plan.tiles == kLargeTiles)
+        return launch(LargeTiles{}, stage);
+    if (plan.tiles == kSmallTiles)
+      return launch(SmallTiles{}, stage);
+    launch(std::conditional_t<PAIR == kGemmHalves, TinyPairs, TinyTiles>{}, stage);
   };
   if (plan.splits == 1) {
     sized(std::integral_constant<int, STAGE>{});
@@ -602,9 +668,18 @@ void run_product(GatedArgs a, const ProductPlan &plan, float *part, hipStream_t 
   // of at most kMostParts values
   const int64_t chunks =
       a.part_row / (STAGE == kPlain ? 4 : 16 / static_cast<int64_t>(sizeof(T))) * a.rows;
-  hipLaunchKernelGGL((gated_join_kernel<T, STAGE>),
-                     dim3(static_cast<unsigned>(ceil_div(chunks, kGatedThreads)), a.outs),
-                     dim3(kGatedThreads), 0, stream, a);
+  auto join = [&](auto parts) {
+    constexpr int PARTS = decltype(parts)::value;
+    hipLaunchKernelGGL((gated_join_kernel<T, STAGE, PARTS>),
+                       dim3(static_cast<unsigned>(ceil_div(chunks, kGatedThreads / PARTS)),
+                            a.outs),
+                       dim3(kGatedThreads), 0, stream, a);
+  };
+  // few chunks leave most of the chip idle unless several threads share one
+  if (a.splits >= 8 && chunks * a.outs < 256 * 1024)
+    join(std::integral_constant<int, 8>{});
+  else
+    join(std::integral_constant<int, 1>{});
   RHIP_LAUNCH_CHECK();
 }
 
@@ -810,8 +885,7 @@ extern "C" int rhip_gated_forward(const rhip_gated *gated, void *y, void *saved,
         run_few<T, false>(w, stream);
         return;
       }
-      for (const Packed *m : {&f.x, &f.gate, &f.up, &f.down})
-        run_pack<T>(*m, stream);
+      run_packs<T>({&f.x, &f.gate, &f.up, &f.down}, stream);
       a.y = side(f.x, false);
       a.x = side(f.gate, false, &f.up);
       a.k_tiles = static_cast<int32_t>(ceil_div(a.x.k, gemm_bk<T>()));
@@ -852,9 +926,11 @@ extern "C" int rhip_gated_backward(const rhip_gated *gated, const void *saved,
       using T = decltype(t);
       const GatedArgs base = gated_args(d, s);
       const int32_t n = static_cast<int32_t>(d->n);
-      run_pack<T>(b.gy, stream);
+      const Packed none{};
+      run_packs<T>({&b.gy, grad_x || grad_gate ? &b.down : &none, grad_x ? &b.gate : &none,
+                    grad_x ? &b.up : &none, grad_gate ? &b.x : &none},
+                   stream);
       if (grad_x || grad_gate) {
-        run_pack<T>(b.down, stream);
         GatedArgs a = base;
         a.y = side(b.gy, false);
         a.x = side(b.down, true);
@@ -864,8 +940,6 @@ extern "C" int rhip_gated_backward(const rhip_gated *gated, const void *saved,
         run_product<T, false, true, kGemmOne, kHidden>(a, b.hidden, b.part, stream);
       }
       if (grad_x) {
-        run_pack<T>(b.gate, stream);
-        run_pack<T>(b.up, stream);
         GatedArgs a = base;
         a.y = side(b.dg, b.du, n, a.pitch, false);
         a.x = side(b.gate, true, &b.up);
@@ -875,7 +949,6 @@ extern "C" int rhip_gated_backward(const rhip_gated *gated, const void *saved,
         run_product<T, false, true, kGemmBehind, kPlain>(a, b.gx, b.part, stream);
       }
       if (grad_gate) {
-        run_pack<T>(b.x, stream);
         GatedArgs a = base;
         a.y = side(b.dg, b.du, n, a.pitch, true);
         a.x = side(b.x, true);

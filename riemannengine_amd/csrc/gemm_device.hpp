@@ -7,9 +7,10 @@
 // by 128 bytes of k (64 bf16, 32 fp32):
 //   k along:  row r at 128 r, its 16-byte chunk c at (c ^ (r / 2 % 8)) * 16, so
 //             16 consecutive rows hold one chunk column in 16 bank groups;
-//   k across: row k at B * sizeof(T) * k; bf16: chunk c at c ^ (k % 4 * 4), so
-//             four rows' pieces of a transpose read lie in four bank groups;
-//             fp32: c ^ (k / 4 % 2 * 8), for the lanes' two halves.
+//   k across: row k at B * sizeof(T) * k; bf16: chunk c at c ^ (k % 4 * 4) (rows of
+//             128 bytes: c ^ (k / 2 % 2 * 4)), so four rows' pieces of a transpose
+//             read lie in four bank groups; fp32: c ^ (k / 4 % 2 * 8), for the
+//             lanes' two halves.
 // The first operand of a matrix instruction is X, the second Y: a lane then
 // holds, of one i, runs of four consecutive j, which is the order of the
 // results in memory.
@@ -44,6 +45,10 @@ template <typename T, int B, bool ACROSS, int THREADS> struct GemmTile {
   static constexpr int kRowChunks = kRowBytes / 16;
   static constexpr int kLoads = kBytes / 16 / THREADS;
   static constexpr int kRowsPerLoad = THREADS / kRowChunks;
+  // the 64-byte piece of a row across, in units of four chunks, that row k % 4 swaps
+  __device__ static __forceinline__ int turn(int k) {
+    return kRowChunks >= 16 ? k & 3 : (k >> 1) & 1;
+  }
   using Frag = typename Mfma<T>::Frag;
 
   // A lane's read addresses: k along, of the four steps; across, of up to four
@@ -61,7 +66,7 @@ template <typename T, int B, bool ACROSS, int THREADS> struct GemmTile {
                   (((2 * i + half) ^ ((l >> 1) & 7)) * 16);
       } else if constexpr (sizeof(T) == 2) {
         const int j = (l & 15) >> 2, q = 2 * ((l >> 4) & 1) + ((l & 3) >> 1);
-        a.at[i] = lds + (8 * half + j) * kRowBytes + (((block0 + i) ^ j) * 4 + q) * 16 +
+        a.at[i] = lds + (8 * half + j) * kRowBytes + (((block0 + i) ^ turn(j)) * 4 + q) * 16 +
                   (l & 1) * 8;
       } else {
         a.at[i] = lds + 4 * half * kRowBytes + ((block0 + i) ^ half) * 128 + (l & 31) * 4;
@@ -101,7 +106,7 @@ template <typename T, int B, bool ACROSS, int THREADS> struct GemmTile {
 #pragma unroll
       for (int i = 0; i < kOffs; ++i) {
         const int rr = r + i * kRowsPerLoad;
-        const int c = sizeof(T) == 2 ? slot ^ ((rr & 3) << 2) : slot ^ (((rr >> 2) & 1) << 3);
+        const int c = sizeof(T) == 2 ? slot ^ (turn(rr) << 2) : slot ^ (((rr >> 2) & 1) << 3);
         off[i] = c * E < idx_left ? static_cast<uint32_t>(r * row * sizeof(T)) + c * 16 : kBufOob;
       }
       chunk = 0;
@@ -184,6 +189,8 @@ template <typename T, typename SHAPE, bool YACROSS, bool XACROSS, GemmPair PAIR>
   using Frag = typename Mfma<T>::Frag;
   static constexpr int kLds = 2 * (YTile::kBytes + XTile::kBytes);
   static_assert(PAIR != kGemmHalves || (!XACROSS && NJ % 2 == 0), "halves: k along the rows");
+  static_assert(YTile::kRowsPerLoad % 4 == 0 && XTile::kRowsPerLoad % 4 == 0,
+                "a thread's loads share their chunk's turn");
 
   // y, x: the sides; i0, j0: the tile's first indices; tiles [kt0, kt1) of k
   // (with kGemmBehind those of both matrices one after another)
