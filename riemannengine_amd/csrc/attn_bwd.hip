@@ -812,7 +812,8 @@ AttnPlan attn_keys_plan(const rhip_attn &d, const AttnWindow &window) {
 }
 
 // Tiles of 32 keys (W = 1), each over all rows of its sequence in as many parts
-// as fill the chip twice, each part of 512 rows (four tiles a wave) at least.
+// as fill the chip twice, each part of 256 rows (two tiles a wave) of the mean
+// sequence at least.
 AttnApart attn_apart_plan(const rhip_attn &d, const AttnWindow &window) {
   if (window.window == 0 || window.sinks == 0 || d.n_seq == 0 || d.n_k == 0)
     return {};
@@ -825,7 +826,7 @@ AttnApart attn_apart_plan(const rhip_attn &d, const AttnWindow &window) {
   const int64_t rows = d.n_q / d.n_seq * (d.heads / d.kv_heads);
   const int64_t busy = p.plan.tiles * d.kv_heads;
   p.plan.splits = 1;
-  while (p.plan.splits < 32 && busy * p.plan.splits < 512 && rows >= 1024 * p.plan.splits)
+  while (p.plan.splits < 64 && busy * p.plan.splits < 512 && rows >= 512 * p.plan.splits)
     p.plan.splits *= 2;
   return p;
 }

@@ -15,6 +15,11 @@
 // rotation, so x (and grad_y) are read once and y (grad_x) is written once.
 // Angles are products of fp64, reduced to a part of a turn in fp64: far
 // positions keep the accuracy of near ones.
+//
+// Bound by memory: 16384 rows of 32 + 8 heads of 128, bf16, with the norm: 71 us
+// forward (4.7 TB/s), 96 backward (5.2) and 6 for the weights' sums; by the angles
+// beside it for narrow heads (100003 rows of 8 heads of 32: 28 and 30 us, 3.6
+// TB/s). 32 rows: one launch, 6 us.
 #include <climits>
 #include <type_traits>
 
@@ -25,10 +30,12 @@ namespace {
 
 constexpr int kRotThreads = 256;
 constexpr int kRotMaxDim = 256;
-constexpr int kRotTable = 4096;  // pairs of a tile's table (32 KB)
+constexpr int kRotTable = 512;   // pairs of a tile's table (4 KB)
 constexpr int kRotMaxRows = 256; // rows of a tile
-// Backward workgroups that sum the weights' gradients: each writes a row of sums.
-constexpr int kRotBlocks = 1024;
+// Backward workgroups that sum the weights' gradients, three to a CU; each writes a
+// row of sums (16384 rows of 40 heads of 128: 96 us, with 1024 or 512 of them
+// a sixth more).
+constexpr int kRotBlocks = 768;
 
 struct RotHeads {
   const void *x, *gy;
@@ -36,6 +43,7 @@ struct RotHeads {
   const float *weight;
   void *y; // forward: y, backward: grad_x; dense
   int32_t heads;
+  uint32_t inverse; // of heads, 2^32 / heads rounded up; 0: too many heads for it
 };
 
 struct RotArgs {
@@ -47,7 +55,6 @@ struct RotArgs {
   int32_t axes, ends[RHIP_ROTARY_MAX_AXES]; // pairs of the axes up to and with this one
   int32_t n, dim, pairs, turning, passing;   // lanes of a group with pairs that turn, that stay
   int32_t rows, tiles;                       // rows of a tile; tiles
-  int32_t heads, heads_each;                 // of both tensors; of a workgroup
   int32_t interleaved;
   float eps;
   float *part; // backward: [workgroups][2][dim] sums of the weights' gradients
@@ -171,52 +178,60 @@ __device__ __forceinline__ void rot_weight(const float *w, const RotLane &l, flo
   load_params<V>(w ? w + l.b : nullptr, 0, l.nb, 1.f, wb);
 }
 
+// The row (of the tile) of item i of a tensor, heads fastest.
+__device__ __forceinline__ int32_t rot_row(const RotHeads &t, int32_t i) {
+  return t.inverse ? static_cast<int32_t>(__umulhi(static_cast<uint32_t>(i), t.inverse))
+                   : i / t.heads;
+}
+
 template <typename T, int G, bool NORM>
 __global__ __launch_bounds__(kRotThreads) void rot_forward_kernel(RotArgs p) {
   using K = RowChunk<T>;
   constexpr int V = K::V, kGroups = kRotThreads / G;
   __shared__ alignas(16) float cosines[kRotTable], sines[kRotTable];
   const RotLane l = rot_lane<V>(p, threadIdx.x % G);
-  const int32_t head0 = static_cast<int32_t>(blockIdx.y) * p.heads_each;
-  const int32_t heads = min(p.heads_each, p.heads - head0);
   const float inv = 1.f / static_cast<float>(p.dim);
   for (int32_t tile = blockIdx.x; tile < p.tiles; tile += gridDim.x) {
     const int32_t row0 = tile * p.rows, rows = min(p.rows, p.n - row0);
     __syncthreads(); // the last tile's table is free
     rot_table<V>(p, row0, rows, cosines, sines);
     __syncthreads();
-    for (int32_t i = threadIdx.x / G; i < rows * heads; i += kGroups) {
-      const int32_t r = i / heads;
-      int32_t head = head0 + i - r * heads;
-      const int which = head >= p.t[0].heads ? 1 : 0;
+#pragma unroll
+    for (int which = 0; which < 2; ++which) {
       const RotHeads &t = p.t[which];
-      head -= which ? p.t[0].heads : 0;
-      const int64_t row = static_cast<int64_t>(row0) + r;
-      const T *x = static_cast<const T *>(t.x) + row * t.x_row + head * t.x_head;
-      float a[V], b[V];
-      K::load(x + l.a, l.na, a);
-      K::load(x + l.b, l.nb, b);
-      if constexpr (NORM) {
-        float sum = 0.f;
-#pragma unroll
-        for (int e = 0; e < V; ++e) {
-          sum = fmaf(e >= l.skip_a ? a[e] : 0.f, a[e], sum);
-          sum = fmaf(e >= l.skip_b ? b[e] : 0.f, b[e], sum);
-        }
-        const float rs = 1.f / sqrtf(group_sum<G>(sum) * inv + p.eps);
-        float wa[V], wb[V];
+      float wa[V], wb[V];
+      if constexpr (NORM)
         rot_weight<V>(t.weight, l, wa, wb);
+      const int32_t step = gridDim.y * kGroups;
+      for (int32_t i = blockIdx.y * kGroups + threadIdx.x / G; i < rows * t.heads; i += step) {
+        const int32_t r = rot_row(t, i), head = i - r * t.heads;
+        const int64_t row = static_cast<int64_t>(row0) + r;
+        const T *x = static_cast<const T *>(t.x) + row * t.x_row + head * t.x_head;
+        // both loads before the first use
+        const v4u ra = K::fetch(x + l.a, l.na, false), rb = K::fetch(x + l.b, l.nb, false);
+        float a[V], b[V];
+        K::unpack(ra, a);
+        K::unpack(rb, b);
+        if constexpr (NORM) {
+          float sum = 0.f;
 #pragma unroll
-        for (int e = 0; e < V; ++e) {
-          a[e] *= rs * wa[e];
-          b[e] *= rs * wb[e];
+          for (int e = 0; e < V; ++e) {
+            sum = fmaf(e >= l.skip_a ? a[e] : 0.f, a[e], sum);
+            sum = fmaf(e >= l.skip_b ? b[e] : 0.f, b[e], sum);
+          }
+          const float rs = 1.f / sqrtf(group_sum<G>(sum) * inv + p.eps);
+#pragma unroll
+          for (int e = 0; e < V; ++e) {
+            a[e] *= rs * wa[e];
+            b[e] *= rs * wb[e];
+          }
         }
+        if (l.pair >= 0)
+          rot_turn<V>(p, false, cosines, sines, r * p.turning * V + l.pair, a, b);
+        T *y = static_cast<T *>(t.y) + (row * t.heads + head) * p.dim;
+        K::store(y + l.a, l.na, a);
+        K::store(y + l.b, l.nb, b);
       }
-      if (l.pair >= 0)
-        rot_turn<V>(p, false, cosines, sines, r * p.turning * V + l.pair, a, b);
-      T *y = static_cast<T *>(t.y) + (row * t.heads + head) * p.dim;
-      K::store(y + l.a, l.na, a);
-      K::store(y + l.b, l.nb, b);
     }
   }
 }
@@ -247,22 +262,26 @@ __global__ __launch_bounds__(kRotThreads) void rot_backward_kernel(RotArgs p) {
       if constexpr (NORM)
         rot_weight<V>(t.weight, l, wa, wb);
       for (int32_t i = group; i < rows * t.heads; i += kGroups) {
-        const int32_t r = i / t.heads, head = i - r * t.heads;
+        const int32_t r = rot_row(t, i), head = i - r * t.heads;
         const int64_t row = static_cast<int64_t>(row0) + r;
         const T *gy = static_cast<const T *>(t.gy) + row * t.gy_row + head * t.gy_head;
-        float a[V], b[V];
-        K::load(gy + l.a, l.na, a);
-        K::load(gy + l.b, l.nb, b);
-        float xa[V], xb[V];
+        // all loads before the first use
+        const v4u ra = K::fetch(gy + l.a, l.na, false), rb = K::fetch(gy + l.b, l.nb, false);
+        v4u rxa{}, rxb{};
         if constexpr (NORM) {
           const T *x = static_cast<const T *>(t.x) + row * t.x_row + head * t.x_head;
-          K::load(x + l.a, l.na, xa);
-          K::load(x + l.b, l.nb, xb);
+          rxa = K::fetch(x + l.a, l.na, false);
+          rxb = K::fetch(x + l.b, l.nb, false);
         }
+        float a[V], b[V];
+        K::unpack(ra, a);
+        K::unpack(rb, b);
         if (l.pair >= 0)
           rot_turn<V>(p, true, cosines, sines, r * p.turning * V + l.pair, a, b);
         if constexpr (NORM) {
-          float sq = 0.f, dot = 0.f;
+          float xa[V], xb[V], sq = 0.f, dot = 0.f;
+          K::unpack(rxa, xa);
+          K::unpack(rxb, xb);
 #pragma unroll
           for (int e = 0; e < V; ++e) {
             const float ya = e >= l.skip_a ? xa[e] : 0.f, yb = e >= l.skip_b ? xb[e] : 0.f;
@@ -399,12 +418,16 @@ RotShape rot_shape(const rhip_rotary *r) {
   return s;
 }
 
-// Rows per tile: about four heads for each group of a workgroup, while that
-// leaves two workgroups for each CU and the table holds them.
+// Rows per tile: at most sixteen heads for each group of a workgroup, and two
+// pairs of the table for each thread with the norm, one without (more make a
+// start that the others wait for: rotation of 100003 rows of 8 heads of 32 27 us,
+// with four 37), while that leaves two workgroups for each CU.
 int32_t rot_rows(const rhip_rotary *r, const RotShape &s, int64_t heads) {
   const int64_t groups = kRotThreads / s.group;
   const int64_t slots = static_cast<int64_t>(s.turning) * rot_v(r->dtype);
-  int64_t rows = std::min<int64_t>({4 * groups / heads, kRotTable / slots, kRotMaxRows, r->n / 512});
+  const int64_t rows = std::min<int64_t>({16 * groups / heads,
+                                          kRotTable / (r->norm ? 1 : 2) / slots, kRotMaxRows,
+                                          r->n / 512});
   return static_cast<int32_t>(std::max<int64_t>(rows, 1));
 }
 
@@ -417,6 +440,10 @@ RotArgs rot_args(const rhip_rotary *r, const rhip_rotary_heads *q, const rhip_ro
       continue;
     t.x = h->x, t.x_row = h->x_row, t.x_head = h->x_head;
     t.weight = h->weight, t.heads = h->heads;
+    // exact for items below 2^32 / heads; a tile has at most kRotMaxRows * heads
+    t.inverse = h->heads <= 4096 && h->heads > 1
+                    ? static_cast<uint32_t>(((uint64_t(1) << 32) + h->heads - 1) / h->heads)
+                    : 0u;
   }
   p.positions = r->positions, p.position_row = r->position_row;
   p.position_type = r->position_type, p.frequencies = r->frequencies;
@@ -427,9 +454,7 @@ RotArgs rot_args(const rhip_rotary *r, const rhip_rotary_heads *q, const rhip_ro
   }
   p.n = static_cast<int32_t>(r->n), p.dim = r->dim;
   p.turning = s.turning, p.passing = s.passing;
-  p.heads = q->heads + (k ? k->heads : 0);
-  p.heads_each = p.heads;
-  p.rows = rot_rows(r, s, p.heads);
+  p.rows = rot_rows(r, s, q->heads + (k ? k->heads : 0));
   p.tiles = static_cast<int32_t>(ceil_div(r->n, p.rows));
   p.interleaved = r->interleaved ? 1 : 0;
   p.eps = static_cast<float>(r->eps);
@@ -488,12 +513,12 @@ extern "C" int rhip_rotary_forward(const rhip_rotary *rotary, const rhip_rotary_
       p.t[1].y = k->y;
     with_rotary(rotary, [&](auto t, auto g, auto norm) {
       constexpr int G = decltype(g)::value;
-      // few rows: their heads over several workgroups
-      const int64_t each = std::max<int64_t>(
-          kRotThreads / G, ceil_div(p.heads, std::max<int64_t>(1, 1024 / p.tiles)));
-      p.heads_each = static_cast<int32_t>(p.rows > 1 ? p.heads : std::min<int64_t>(each, p.heads));
+      // few rows: their heads over several workgroups, one for each group
+      const int64_t items = static_cast<int64_t>(p.rows) * std::max(p.t[0].heads, p.t[1].heads);
+      const int64_t share = std::min<int64_t>(ceil_div(items, kRotThreads / G),
+                                              std::max<int64_t>(1, 1024 / p.tiles));
       const dim3 grid(static_cast<unsigned>(std::min<int64_t>(p.tiles, kRotMaxGrid)),
-                      static_cast<unsigned>(ceil_div(p.heads, p.heads_each)));
+                      static_cast<unsigned>(share));
       hipLaunchKernelGGL((rot_forward_kernel<decltype(t), G, decltype(norm)::value>), grid,
                          dim3(kRotThreads), 0, stream, p);
       RHIP_LAUNCH_CHECK();
