@@ -532,20 +532,46 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
             py::arg("ids"), py::arg("rows"));
   embedding.def_property_readonly("weight",
                                   [](RiemannEmbeddingImpl &self) { return self.weight_; });
+  using OptInt = c10::optional<int64_t>;
+  using Ints = std::vector<int64_t>;
   bind_unary<RiemannAttentionImpl>(nn, "RiemannAttention")
-      .def(py::init([](int64_t channels, int64_t heads, int64_t kv_heads, bool causal,
-                       bool bias) {
-             return std::make_shared<RiemannAttentionImpl>(channels, heads, kv_heads, causal,
-                                                           bias);
+      .def(py::init([](int64_t channels, int64_t heads, int64_t kv_heads, bool causal, bool bias,
+                       OptInt window, int64_t sinks, const Ints &rotary, double rotary_base,
+                       bool head_norm) {
+             return std::make_shared<RiemannAttentionImpl>(
+                 channels, heads, kv_heads, causal, bias,
+                 AttentionOptions{window, sinks, rotary, rotary_base, head_norm});
            }),
            py::arg("channels"), py::arg("heads"), py::arg("kv_heads") = 0,
-           py::arg("causal") = false, py::arg("bias") = true);
+           py::arg("causal") = false, py::arg("bias") = true, py::arg("window") = py::none(),
+           py::arg("sinks") = 0, py::arg("rotary") = Ints{}, py::arg("rotary_base") = 10000.0,
+           py::arg("head_norm") = false);
+  auto gated = bind_unary<RiemannGatedFeedForwardImpl>(nn, "RiemannGatedFeedForward");
+  gated
+      .def(py::init([](int64_t channels, int64_t hidden, const std::string &activation) {
+             return std::make_shared<RiemannGatedFeedForwardImpl>(channels, hidden, activation);
+           }),
+           py::arg("channels"), py::arg("hidden"), py::arg("activation") = "silu")
+      .def_property_readonly("gate", [](RiemannGatedFeedForwardImpl &self) { return self.gate_; })
+      .def_property_readonly("up", [](RiemannGatedFeedForwardImpl &self) { return self.up_; })
+      .def_property_readonly("down", [](RiemannGatedFeedForwardImpl &self) { return self.down_; });
+  for (const char *name : {"forward", "__call__"})
+    gated.def(
+        name,
+        [](RiemannGatedFeedForwardImpl &self, const at::Tensor &input) {
+          return self.forward(input);
+        },
+        py::arg("input"));
   bind_unary<AttentionBlockImpl>(nn, "AttentionBlock")
       .def(py::init([](int64_t channels, int64_t heads, int64_t kv_heads, int64_t expansion,
-                       bool causal) {
-             return std::make_shared<AttentionBlockImpl>(channels, heads, kv_heads, expansion,
-                                                         causal);
+                       bool causal, OptInt window, int64_t sinks, const Ints &rotary,
+                       double rotary_base, bool head_norm, bool gated) {
+             return std::make_shared<AttentionBlockImpl>(
+                 channels, heads, kv_heads, expansion, causal,
+                 AttentionOptions{window, sinks, rotary, rotary_base, head_norm}, gated);
            }),
            py::arg("channels"), py::arg("heads"), py::arg("kv_heads") = 0,
-           py::arg("expansion") = 4, py::arg("causal") = false);
+           py::arg("expansion") = 4, py::arg("causal") = false, py::arg("window") = py::none(),
+           py::arg("sinks") = 0, py::arg("rotary") = Ints{}, py::arg("rotary_base") = 10000.0,
+           py::arg("head_norm") = false, py::arg("gated") = false);
 }

@@ -1,5 +1,7 @@
 // The gated feed-forward block as an autograd function over the HIP kernels
 // (rhip_gated_*), and its layer on sparse tensors.
+#include <cmath>
+
 #include "transformer.hpp"
 
 namespace riemann {
@@ -122,6 +124,36 @@ at::Tensor hip_gated_feed_forward(const at::Tensor &input, const at::Tensor &gat
   auto shape = input.sizes().vec();
   shape.back() = down.size(0);
   return y.reshape(shape);
+}
+
+RiemannGatedFeedForwardImpl::RiemannGatedFeedForwardImpl(int64_t channels, int64_t hidden,
+                                                         const std::string &activation)
+    : channels_(channels), hidden_(hidden), activation_(activation) {
+  TORCH_CHECK(channels > 0 && hidden > 0, "RiemannGatedFeedForward needs channels and hidden ones");
+  activation_of(activation);
+  reset();
+}
+
+void RiemannGatedFeedForwardImpl::reset() {
+  // as torch's linear layers begin
+  auto weight = [&](const char *name, int64_t out, int64_t in) {
+    const double bound = 1.0 / std::sqrt(static_cast<double>(in));
+    return register_parameter(name, torch::empty({out, in}).uniform_(-bound, bound));
+  };
+  gate_ = weight("gate", hidden_, channels_);
+  up_ = weight("up", hidden_, channels_);
+  down_ = weight("down", channels_, hidden_);
+}
+
+at::Tensor RiemannGatedFeedForwardImpl::forward(const at::Tensor &input) {
+  return hip_gated_feed_forward(input, gate_, up_, down_, activation_);
+}
+
+SparseTensor RiemannGatedFeedForwardImpl::forward(const SparseTensor &input) {
+  const auto &x = input.F();
+  TORCH_CHECK(x.dim() == 2 && x.size(1) == channels_, "RiemannGatedFeedForward expects [N, ",
+              channels_, "] features, got ", x.sizes());
+  return SparseTensor(forward(x), input.coordinate_map_key(), input.coordinate_manager());
 }
 
 } // namespace riemann

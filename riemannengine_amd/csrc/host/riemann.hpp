@@ -712,36 +712,92 @@ private:
 };
 TORCH_MODULE(RiemannEmbedding);
 
+// The weight of a norm of heads, fp32 under a dtype cast as RiemannLayerNorm's.
+class RiemannHeadNormImpl : public torch::nn::Cloneable<RiemannHeadNormImpl> {
+public:
+  explicit RiemannHeadNormImpl(int64_t width) : width_(width) { reset(); }
+  void reset() override { weight_ = register_parameter("weight", torch::ones({width_})); }
+  using torch::nn::Module::to;
+  void to(torch::Dtype, bool = false) override {}
+  void to(torch::Device device, torch::Dtype, bool non_blocking = false) override {
+    torch::nn::Module::to(device, non_blocking);
+  }
+
+  torch::Tensor weight_;
+
+private:
+  int64_t width_;
+};
+TORCH_MODULE(RiemannHeadNorm);
+
+// What RiemannAttention and AttentionBlock do beside plain attention. window: a
+// row sees the rows less than so many away in its batch's row order, and the
+// first `sinks`; rotary: pairs of a head that turn with each spatial axis'
+// coordinate (empty: none); head_norm: queries and keys are normed by head before
+// they turn.
+struct AttentionOptions {
+  c10::optional<int64_t> window;
+  int64_t sinks = 0;
+  std::vector<int64_t> rotary;
+  double rotary_base = 10000.0;
+  bool head_norm = false;
+};
+
 // Multi-head attention among the rows of each batch, in their row order;
 // kv_heads 0: as many as heads.
 class RiemannAttentionImpl : public torch::nn::Cloneable<RiemannAttentionImpl> {
 public:
   RiemannAttentionImpl(int64_t channels, int64_t heads, int64_t kv_heads = 0,
-                       bool causal = false, bool bias = true);
+                       bool causal = false, bool bias = true, AttentionOptions options = {});
   void reset() override;
   SparseTensor forward(const SparseTensor &input);
 
 private:
   int64_t channels_, heads_, kv_heads_;
   bool causal_, has_bias_;
+  AttentionOptions options_;
   torch::nn::Linear projection_{nullptr}, output_{nullptr};
+  RiemannHeadNorm query_norm_{nullptr}, key_norm_{nullptr};
+  at::Tensor frequencies_; // of the rotation, on the device of the last call
 };
 TORCH_MODULE(RiemannAttention);
 
-// x + attention(norm1(x)), then x + down(gelu(up(norm2(x)))).
+// (act(x gate^T) * (x up^T)) down^T on the rows' features.
+class RiemannGatedFeedForwardImpl : public torch::nn::Cloneable<RiemannGatedFeedForwardImpl> {
+public:
+  RiemannGatedFeedForwardImpl(int64_t channels, int64_t hidden,
+                              const std::string &activation = "silu");
+  void reset() override;
+  SparseTensor forward(const SparseTensor &input);
+  at::Tensor forward(const at::Tensor &input);
+
+  torch::Tensor gate_, up_, down_;
+
+private:
+  int64_t channels_, hidden_;
+  std::string activation_;
+};
+TORCH_MODULE(RiemannGatedFeedForward);
+
+// x + attention(norm1(x)), then x + down(gelu(up(norm2(x)))), or with `gated` x +
+// feed_forward(norm2(x)), a RiemannGatedFeedForward.
 class AttentionBlockImpl : public torch::nn::Cloneable<AttentionBlockImpl> {
 public:
   AttentionBlockImpl(int64_t channels, int64_t heads, int64_t kv_heads = 0,
-                     int64_t expansion = 4, bool causal = false);
+                     int64_t expansion = 4, bool causal = false, AttentionOptions options = {},
+                     bool gated = false);
   void reset() override;
   SparseTensor forward(const SparseTensor &input);
 
 private:
   int64_t channels_, heads_, kv_heads_, expansion_;
   bool causal_;
+  AttentionOptions options_;
+  bool gated_;
   RiemannLayerNorm norm1_{nullptr}, norm2_{nullptr};
   RiemannAttention attention_{nullptr};
   torch::nn::Linear up_{nullptr}, down_{nullptr};
+  RiemannGatedFeedForward feed_forward_{nullptr};
 };
 TORCH_MODULE(AttentionBlock);
 

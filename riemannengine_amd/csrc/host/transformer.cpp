@@ -421,13 +421,27 @@ SparseTensor RiemannEmbeddingImpl::forward(const at::Tensor &ids, const SparseTe
 }
 
 RiemannAttentionImpl::RiemannAttentionImpl(int64_t channels, int64_t heads, int64_t kv_heads,
-                                           bool causal, bool bias)
+                                           bool causal, bool bias, AttentionOptions options)
     : channels_(channels), heads_(heads), kv_heads_(kv_heads == 0 ? heads : kv_heads),
-      causal_(causal), has_bias_(bias) {
+      causal_(causal), has_bias_(bias), options_(std::move(options)) {
   TORCH_CHECK(channels > 0 && heads > 0 && channels % heads == 0,
               "RiemannAttention needs a multiple of ", heads, " channels, got ", channels);
   TORCH_CHECK(kv_heads_ > 0 && heads % kv_heads_ == 0, "heads ", heads, " must be a multiple of key heads ",
               kv_heads_);
+  TORCH_CHECK(options_.window.value_or(1) >= 1 && options_.sinks >= 0,
+              "RiemannAttention needs a window of at least one row, and no fewer than 0 sinks");
+  TORCH_CHECK(options_.window.has_value() || options_.sinks == 0,
+              "RiemannAttention takes sinks beside a window");
+  int64_t pairs = 0;
+  for (const int64_t s : options_.rotary) {
+    TORCH_CHECK(s >= 0, "rotary must hold each axis' number of pairs");
+    pairs += s;
+  }
+  TORCH_CHECK(options_.rotary.empty() || (pairs > 0 && 2 * pairs <= channels / heads),
+              "rotary holds ", pairs, " pairs; heads of width ", channels / heads, " have 1 to ",
+              channels / heads / 2);
+  TORCH_CHECK(!options_.head_norm || !options_.rotary.empty(),
+              "head_norm stands before a rotation: RiemannAttention needs rotary with it");
   reset();
 }
 
@@ -440,6 +454,10 @@ void RiemannAttentionImpl::reset() {
   output_ = register_module(
       "output",
       torch::nn::Linear(torch::nn::LinearOptions(channels_, channels_).bias(has_bias_)));
+  if (options_.head_norm) {
+    query_norm_ = register_module("query_norm", RiemannHeadNorm(dim));
+    key_norm_ = register_module("key_norm", RiemannHeadNorm(dim));
+  }
 }
 
 SparseTensor RiemannAttentionImpl::forward(const SparseTensor &input) {
@@ -451,10 +469,27 @@ SparseTensor RiemannAttentionImpl::forward(const SparseTensor &input) {
   const Scenes scenes = scenes_of(input);
   auto rows = projection_->forward(x.index_select(0, scenes.members))
                   .view({n, heads_ + 2 * kv_heads_, dim});
-  auto mixed = hip_packed_attention(rows.narrow(1, 0, heads_),
-                                    rows.narrow(1, heads_, kv_heads_),
-                                    rows.narrow(1, heads_ + kv_heads_, kv_heads_), scenes.seg,
-                                    scenes.seg, at::Tensor(), causal_, c10::nullopt);
+  auto q = rows.narrow(1, 0, heads_), k = rows.narrow(1, heads_, kv_heads_);
+  if (!options_.rotary.empty()) {
+    const auto coords = input.C();
+    const int64_t axes = coords.size(1) - 1;
+    TORCH_CHECK(axes == static_cast<int64_t>(options_.rotary.size()),
+                "rotary holds the pairs of ", options_.rotary.size(), " axes, the tensor has ",
+                axes);
+    auto places = coords.index_select(0, scenes.members).narrow(1, 1, axes);
+    if (!frequencies_.defined() || frequencies_.device() != x.device())
+      frequencies_ = rotary_frequencies(options_.rotary, options_.rotary_base, x.device());
+    if (options_.head_norm) {
+      std::tie(q, k) = hip_norm_rotate_heads(q, k, places, frequencies_, options_.rotary,
+                                             query_norm_->weight_, key_norm_->weight_);
+    } else {
+      q = hip_rotate_heads(q, places, frequencies_, options_.rotary);
+      k = hip_rotate_heads(k, places, frequencies_, options_.rotary);
+    }
+  }
+  auto mixed = hip_packed_attention(q, k, rows.narrow(1, heads_ + kv_heads_, kv_heads_),
+                                    scenes.seg, scenes.seg, at::Tensor(), causal_, c10::nullopt,
+                                    options_.window, options_.sinks);
   auto out = output_->forward(mixed.view({n, channels_}));
   // back to the tensor's own row order
   auto back = torch::empty_like(scenes.members)
@@ -464,26 +499,36 @@ SparseTensor RiemannAttentionImpl::forward(const SparseTensor &input) {
 }
 
 AttentionBlockImpl::AttentionBlockImpl(int64_t channels, int64_t heads, int64_t kv_heads,
-                                       int64_t expansion, bool causal)
+                                       int64_t expansion, bool causal, AttentionOptions options,
+                                       bool gated)
     : channels_(channels), heads_(heads), kv_heads_(kv_heads), expansion_(expansion),
-      causal_(causal) {
+      causal_(causal), options_(std::move(options)), gated_(gated) {
   TORCH_CHECK(expansion > 0, "AttentionBlock expansion must be positive");
   reset();
 }
 
 void AttentionBlockImpl::reset() {
   norm1_ = register_module("norm1", RiemannLayerNorm(channels_));
-  attention_ =
-      register_module("attention", RiemannAttention(channels_, heads_, kv_heads_, causal_));
+  attention_ = register_module("attention", RiemannAttention(channels_, heads_, kv_heads_,
+                                                             causal_, true, options_));
   norm2_ = register_module("norm2", RiemannLayerNorm(channels_));
-  up_ = register_module("up", torch::nn::Linear(channels_, channels_ * expansion_));
-  down_ = register_module("down", torch::nn::Linear(channels_ * expansion_, channels_));
+  if (gated_) {
+    feed_forward_ = register_module("feed_forward",
+                                    RiemannGatedFeedForward(channels_, channels_ * expansion_));
+  } else {
+    up_ = register_module("up", torch::nn::Linear(channels_, channels_ * expansion_));
+    down_ = register_module("down", torch::nn::Linear(channels_ * expansion_, channels_));
+  }
 }
 
 SparseTensor AttentionBlockImpl::forward(const SparseTensor &input) {
   auto x = input.F() + attention_->forward(norm1_->forward(input)).F();
   SparseTensor mid(x, input.coordinate_map_key(), input.coordinate_manager());
-  x = x + down_->forward(torch::gelu(up_->forward(norm2_->forward(mid).F())));
+  auto normed = norm2_->forward(mid).F();
+  if (gated_)
+    x = x + feed_forward_->forward(normed);
+  else
+    x = x + down_->forward(torch::gelu(up_->forward(normed)));
   return SparseTensor(std::move(x), input.coordinate_map_key(), input.coordinate_manager());
 }
 
