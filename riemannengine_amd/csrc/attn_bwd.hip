@@ -771,7 +771,8 @@ AttnPlan plan_keys(int64_t n_q, int64_t n_k, int32_t n_seq, int32_t heads, int32
                    int32_t dim, int32_t causal, int32_t dtype, const AttnWindow &window) {
   const int64_t seqs = std::max<int64_t>(1, std::min<int64_t>(n_seq, n_k));
   double rows = static_cast<double>(n_q) * (heads / kv_heads) / seqs; // per key
-  if (window.window > 0) { // a window's rows, and no mask's half of them
+  // a window's rows, and no mask's half of them (unless sinks are most of the keys)
+  if (window.window > 0 && window.sinks <= n_k / seqs + 128) {
     const double seen =
         (static_cast<double>(window.window) * (causal ? 1 : 2) + 64) * (heads / kv_heads);
     causal = causal && seen > rows;
@@ -819,8 +820,11 @@ AttnApart attn_apart_plan(const rhip_attn &d, const AttnWindow &window) {
   if (window.window == 0 || window.sinks == 0 || d.n_seq == 0 || d.n_k == 0)
     return {};
   AttnApart p{};
-  // whole blocks; no more than any sequence has
-  const int64_t keys = std::min<int64_t>(align_up(window.sinks, 32), align_up(d.n_k, 32));
+  // Whole blocks. Where they would be more than the keys there are, sinks are
+  // most of every sequence, and all keys stay in one launch.
+  const int64_t keys = align_up(window.sinks, 32);
+  if (keys > d.n_k / d.n_seq + 128)
+    return p;
   p.keys = static_cast<int32_t>(keys);
   p.plan.waves = 1;
   p.plan.tiles = d.n_seq * (keys / 32);

@@ -861,6 +861,8 @@ extern "C" int rhip_gated_forward(const rhip_gated *gated, void *y, void *saved,
       return;
     RHIP_CHECK_ARG(y != nullptr, "y is required");
     RHIP_CHECK_ARG(workspace != nullptr, "workspace is required");
+    RHIP_CHECK_ARG(aligned16(saved) && aligned16(workspace),
+                   "saved and workspace must be aligned to 16 bytes");
     Carve cv(workspace, ws_bytes);
     GatedForward f = plan_forward(cv, d, saved != nullptr);
     if (saved) {
@@ -915,6 +917,8 @@ extern "C" int rhip_gated_backward(const rhip_gated *gated, const void *saved,
       return;
     RHIP_CHECK_ARG(d->n == 0 || (d->grad_y && saved), "grad_y and saved are required");
     RHIP_CHECK_ARG(workspace != nullptr, "workspace is required");
+    RHIP_CHECK_ARG(aligned16(saved) && aligned16(workspace),
+                   "saved and workspace must be aligned to 16 bytes");
     Carve cv(workspace, ws_bytes);
     const GatedBackward b = plan_backward(cv, d);
     GatedSaved s{};

@@ -5,6 +5,7 @@
 // counterpart in the reference; they follow its layers' conventions.
 #include <cmath>
 #include <limits>
+#include <mutex>
 
 #include "transformer.hpp"
 
@@ -477,14 +478,20 @@ SparseTensor RiemannAttentionImpl::forward(const SparseTensor &input) {
                 "rotary holds the pairs of ", options_.rotary.size(), " axes, the tensor has ",
                 axes);
     auto places = coords.index_select(0, scenes.members).narrow(1, 1, axes);
-    if (!frequencies_.defined() || frequencies_.device() != x.device())
-      frequencies_ = rotary_frequencies(options_.rotary, options_.rotary_base, x.device());
+    at::Tensor freq;
+    { // the layer may be called from several threads
+      static std::mutex mutex;
+      const std::lock_guard<std::mutex> lock(mutex);
+      if (!frequencies_.defined() || frequencies_.device() != x.device())
+        frequencies_ = rotary_frequencies(options_.rotary, options_.rotary_base, x.device());
+      freq = frequencies_;
+    }
     if (options_.head_norm) {
-      std::tie(q, k) = hip_norm_rotate_heads(q, k, places, frequencies_, options_.rotary,
+      std::tie(q, k) = hip_norm_rotate_heads(q, k, places, freq, options_.rotary,
                                              query_norm_->weight_, key_norm_->weight_);
     } else {
-      q = hip_rotate_heads(q, places, frequencies_, options_.rotary);
-      k = hip_rotate_heads(k, places, frequencies_, options_.rotary);
+      q = hip_rotate_heads(q, places, freq, options_.rotary);
+      k = hip_rotate_heads(k, places, freq, options_.rotary);
     }
   }
   auto mixed = hip_packed_attention(q, k, rows.narrow(1, heads_ + kv_heads_, kv_heads_),
