@@ -8,10 +8,11 @@
 //   dgate = dg^T x, dup = du^T x           one launch,
 //   ddown = dy^T h.
 //
-// All are tiles of gemm_device.hpp's product; sums over a long k with few tiles
-// are split over workgroups, whose fp32 sums a second kernel adds in order and
-// finishes. Up to 64 rows (single tokens) a kernel that streams the weights
-// through registers takes the forward: it is bound by their bytes.
+// All are tiles of gemm_device.hpp's product, bound by the matrix cores. Where
+// tiles leave part of the chip idle their k is shared by workgroups, whose fp32
+// sums a second kernel adds in order and finishes. Up to 64 rows (single tokens) a
+// kernel that streams the weights through registers takes the forward: it is bound
+// by their bytes.
 //
 // Operands that do not hold aligned, whole 16-byte chunks (odd widths,
 // unaligned views) are laid out once per call in the workspace, zeros behind
@@ -125,21 +126,20 @@ template <typename T, int E> __device__ __forceinline__ void put_chunk(T *p, con
 // ---------------------------------------------------------------- products
 
 enum GatedStage {
-  kProject,  // h (and the saved planes) from x, gate, up
-  kPlain,    // one matrix of results
-  kHidden,   // dg, du from dy, down and the saved planes
-  kPartial   // fp32 sums of a part of k
+  kProject, // h (and the saved planes) from x, gate, up
+  kPlain,   // one matrix of results
+  kHidden   // dg, du from dy, down and the saved planes
 };
 
 struct GatedArgs {
   GemmSide y, x;
-  int32_t tiles_i, tiles_j, layers, splits, k_tiles; // layers: splits times `outs`
-  int32_t outs;                                      // results, each with its own y matrix
-  int32_t rows, cols;                                // of the results
+  int32_t tiles_i, tiles_j, k_tiles;
+  int32_t outs;       // results, each with its own y matrix
+  int32_t parts;      // workgroups that share the work
+  int32_t rows, cols; // of the results
   void *out[2];
   int64_t out_row;
-  float *part; // [splits * outs][halves][rows, part_row]
-  int64_t part_row;
+  float *part; // fp32 sums of tiles that several workgroups share, two for each
   GatedSaved saved;
   int64_t pitch; // of h's, dg's, du's and the saved planes' rows
   void *dg, *du;
@@ -193,33 +193,32 @@ __device__ __forceinline__ void strip_values(const char *strip, int r, int c, fl
   }
 }
 
-template <typename T, typename SHAPE, bool YACROSS, bool XACROSS, GemmPair PAIR, GatedStage STAGE>
-__global__ __launch_bounds__(SHAPE::kThreads, 2) void gated_product_kernel(GatedArgs a) {
-  using P = Gemm<T, SHAPE, YACROSS, XACROSS, PAIR>;
-  constexpr int NI = P::NI, NJ = P::NJ, E = 16 / sizeof(T);
-  __shared__ alignas(16) char lds[P::kLds];
-  int32_t ti, tj, layer;
-  if (!gemm_tile(a.tiles_i, a.tiles_j, a.layers, ti, tj, layer))
-    return;
-  const int32_t split = layer / a.outs, which = layer - split * a.outs;
-  constexpr int kHalf = PAIR == kGemmHalves ? 2 : 1;
-  const int32_t i0 = ti * P::BI, j0 = tj * (P::BJ / kHalf);
-  const int32_t per = (a.k_tiles + a.splits - 1) / a.splits;
-  const int32_t kt0 = min(split * per, a.k_tiles), kt1 = min(kt0 + per, a.k_tiles);
-  v16f acc[NJ][NI];
-  P::run(lds, a.y, static_cast<const T *>(a.y.p[which]), a.x, i0, j0, kt0, kt1, acc);
-
+// A tile's results from the waves' sums.
+template <typename T, typename P, GatedStage STAGE>
+__device__ __forceinline__ void finish_tile(const GatedArgs &a, char *lds, int32_t which,
+                                            int32_t i0, int32_t j0,
+                                            v16f (&acc)[P::NJ][P::NI]) {
+  constexpr int E = 16 / sizeof(T), kHalf = P::kHalves;
+  constexpr int NB = P::NJ / kHalf; // blocks of columns of a wave
   const int w = wave_uniform(threadIdx.x / kWave);
-  constexpr int NB = NJ / kHalf; // blocks of columns of a wave
   const int32_t col0 = j0 + (w % P::WJ) * NB * 32;
-  char *strip = lds + w * (P::kLds / SHAPE::kWaves);
+  char *strip = lds + w * P::kStrip;
 #pragma unroll
-  for (int b = 0; b < NI; ++b) {
-    const int32_t row0 = i0 + ((w / P::WJ) * NI + b) * 32;
+  for (int b = 0; b < P::NI; ++b) {
+    const int32_t row0 = i0 + ((w / P::WJ) * P::NI + b) * 32;
     const int32_t rows = a.rows - row0;
-    if constexpr (STAGE == kProject || STAGE == kHidden) {
+    if constexpr (STAGE == kPlain) {
+      using S = GemmStrip<T, NB>;
+      S::put(strip, [&](int c, int r) { return from_f32<T>(acc[c][b][r]); });
+      __builtin_amdgcn_wave_barrier();
+      T *to = static_cast<T *>(a.out[which]) + row0 * a.out_row + col0;
+      S::template walk<E>([&](int r, int c) {
+        if (r < rows)
+          store_chunk(to + r * a.out_row + c, S::chunk(strip, r, c), a.cols - col0 - c);
+      });
+    } else {
       using S = GemmStrip<float, NB>;
-      static_assert(kHalf * S::kBytes <= P::kLds / SHAPE::kWaves, "a wave's strips fit its LDS");
+      static_assert(kHalf * S::kBytes <= P::kStrip, "a wave's strips fit its LDS");
       S::put(strip, [&](int c, int r) { return acc[c][b][r]; });
       if constexpr (STAGE == kProject)
         S::put(strip + S::kBytes, [&](int c, int r) { return acc[c + NB][b][r]; });
@@ -234,70 +233,134 @@ __global__ __launch_bounds__(SHAPE::kThreads, 2) void gated_product_kernel(Gated
                                  a.cols - col0 - c, v);
         }
       });
-    } else if constexpr (STAGE == kPlain) {
-      using S = GemmStrip<T, NB>;
-      S::put(strip, [&](int c, int r) { return from_f32<T>(acc[c][b][r]); });
-      __builtin_amdgcn_wave_barrier();
-      T *to = static_cast<T *>(a.out[which]) + row0 * a.out_row + col0;
-      S::template walk<E>([&](int r, int c) {
-        if (r < rows)
-          store_chunk(to + r * a.out_row + c, S::chunk(strip, r, c), a.cols - col0 - c);
-      });
-    } else {
-      using S = GemmStrip<float, NB>;
-      float *to = a.part + static_cast<int64_t>(layer) * kHalf * a.rows * a.part_row +
-                  row0 * a.part_row + col0;
-#pragma unroll
-      for (int h = 0; h < kHalf; ++h) {
-        S::put(strip, [&](int c, int r) { return acc[c + h * NB][b][r]; });
-        __builtin_amdgcn_wave_barrier();
-        S::template walk<4>([&](int r, int c) {
-          if (r < rows && col0 + c < a.part_row)
-            *reinterpret_cast<v4u *>(to + h * a.rows * a.part_row + r * a.part_row + c) =
-                S::chunk(strip, r, c);
-        });
-        __builtin_amdgcn_wave_barrier();
-      }
     }
     __builtin_amdgcn_wave_barrier(); // the strip is free
   }
 }
 
-// Adds the splits' sums and finishes them as the products' own epilogues do: a
-// 16-byte chunk (of T) for PARTS threads, which take every PARTS-th split each
-// and add up in order in LDS (one thread for a few splits of many chunks).
-template <typename T, GatedStage STAGE, int PARTS>
+// The waves' sums as they are: [halves][BI, BJ / halves] at `to`.
+template <typename P>
+__device__ __forceinline__ void keep_tile(char *lds, float *to, v16f (&acc)[P::NJ][P::NI]) {
+  constexpr int kHalf = P::kHalves, NB = P::NJ / kHalf, kRow = P::BJ / kHalf;
+  using S = GemmStrip<float, NB>;
+  const int w = wave_uniform(threadIdx.x / kWave);
+  char *strip = lds + w * P::kStrip;
+#pragma unroll
+  for (int h = 0; h < kHalf; ++h)
+#pragma unroll
+    for (int b = 0; b < P::NI; ++b) {
+      S::put(strip, [&](int c, int r) { return acc[c + h * NB][b][r]; });
+      __builtin_amdgcn_wave_barrier();
+      float *at = to + (h * P::BI + ((w / P::WJ) * P::NI + b) * 32) * kRow + (w % P::WJ) * NB * 32;
+      S::template walk<4>([&](int r, int c) {
+        *reinterpret_cast<v4u *>(at + r * kRow + c) = S::chunk(strip, r, c);
+      });
+      __builtin_amdgcn_wave_barrier();
+    }
+}
+
+// SHARED: the work is one line of tiles of k, of which every workgroup has an
+// equal part: whole tiles, and at its ends parts of tiles, whose sums the join
+// adds. Otherwise a workgroup has a tile.
+//
+// 8192 rows, 2048 channels, 5504 hidden, bf16: g, u and h 434 us (850 TFLOP/s: the
+// activation and what it saves follow the sums), y 175 (1050), dg and du 281, dx
+// 338 (1090), dgate and dup 400, ddown 218; of torch's products alone the best
+// reach 1300. 8320 rows, 256 channels, 683 hidden, fp32: g, u and h 73 us (80
+// TFLOP/s), y 42, dg and du 47, dx 78, dgate and dup 73, ddown 43; a tile to every
+// workgroup, or one k in two or four, took 407 us in all where equal parts take
+// 366.
+template <typename T, typename SHAPE, bool YACROSS, bool XACROSS, GemmPair PAIR, GatedStage STAGE,
+          bool SHARED>
+__global__ __launch_bounds__(SHAPE::kThreads, 2) void gated_product_kernel(GatedArgs a) {
+  using P = Gemm<T, SHAPE, YACROSS, XACROSS, PAIR>;
+  __shared__ alignas(16) char lds[P::kLds];
+  uint32_t place;
+  if (!gemm_place(a.parts, place))
+    return;
+  int32_t ti, tj, which;
+  v16f acc[P::NJ][P::NI];
+  auto sum = [&](uint32_t t, int32_t kt0, int32_t kt1) {
+    gemm_tile(a.tiles_i, a.tiles_j, t, ti, tj, which);
+    P::run(lds, a.y, static_cast<const T *>(a.y.p[which]), a.x, ti * P::BI,
+           tj * (P::BJ / P::kHalves), kt0, kt1, acc);
+  };
+  auto finish = [&] {
+    finish_tile<T, P, STAGE>(a, lds, which, ti * P::BI, tj * (P::BJ / P::kHalves), acc);
+  };
+  if constexpr (!SHARED) {
+    sum(place, 0, a.k_tiles);
+    finish();
+  } else {
+    const uint32_t tiles = static_cast<uint32_t>(a.tiles_i) * a.tiles_j * a.outs;
+    const int64_t units = static_cast<int64_t>(tiles) * a.k_tiles;
+    // tiles cut evenly: those of one slice of k follow one another, as they
+    // share what they load
+    if (a.parts % tiles == 0)
+      place = place % tiles * (a.parts / tiles) + place / tiles;
+    const int64_t first = gemm_cut(units, a.parts, place);
+    const int64_t end = gemm_cut(units, a.parts, place + 1);
+    for (int64_t u = first; u < end;) {
+      const uint32_t t = static_cast<uint32_t>(u / a.k_tiles);
+      const int32_t kt0 = static_cast<int32_t>(u - static_cast<int64_t>(t) * a.k_tiles);
+      const int32_t kt1 =
+          static_cast<int32_t>(min<int64_t>(a.k_tiles, kt0 + (end - u)));
+      sum(t, kt0, kt1);
+      if (kt0 == 0 && kt1 == a.k_tiles)
+        finish();
+      else
+        keep_tile<P>(lds,
+                     a.part + (static_cast<int64_t>(place) * 2 + (u == first ? 0 : 1)) * P::BI *
+                                  P::BJ,
+                     acc);
+      u += kt1 - kt0;
+      __syncthreads(); // the strips are free for the next tile
+    }
+  }
+}
+
+// Adds the sums of tiles that several workgroups share, in their order, and
+// finishes them as the products' own epilogues do: a 16-byte chunk (of T) for
+// PARTS threads, which take every PARTS-th sum each and add up in LDS.
+template <typename T, typename SHAPE, GemmPair PAIR, GatedStage STAGE, int PARTS>
 __global__ __launch_bounds__(kGatedThreads) void gated_join_kernel(GatedArgs a) {
   constexpr int E = STAGE == kPlain ? 4 : 16 / sizeof(T);
-  constexpr int kHalf = STAGE == kProject ? 2 : 1, kSums = kHalf * E;
-  constexpr int kOwn = kGatedThreads / PARTS; // chunks of a workgroup
-  const int64_t chunks = a.part_row / E, total = chunks * a.rows;
+  constexpr int kHalf = PAIR == kGemmHalves ? 2 : 1, kSums = kHalf * E;
+  constexpr int BI = SHAPE::BI, kRow = SHAPE::BJ / kHalf, kChunks = kRow / E; // of a tile's row
+  constexpr int kOwn = kGatedThreads / PARTS;             // chunks of a workgroup
+  constexpr int kGroups = BI * kChunks / kOwn;            // workgroups of a tile
+  const uint32_t t = blockIdx.x / kGroups;
+  const int64_t units = static_cast<int64_t>(a.tiles_i) * a.tiles_j * a.outs * a.k_tiles;
+  const int64_t u0 = static_cast<int64_t>(t) * a.k_tiles;
+  const int32_t w0 = wave_uniform(gemm_part(units, a.parts, u0));
+  const int32_t w1 = wave_uniform(gemm_part(units, a.parts, u0 + a.k_tiles - 1));
+  if (w0 == w1)
+    return; // one workgroup had it whole
+  int32_t ti, tj, which;
+  gemm_tile(a.tiles_i, a.tiles_j, t, ti, tj, which);
   const int own = threadIdx.x % kOwn, part = threadIdx.x / kOwn;
-  const int64_t q = static_cast<int64_t>(blockIdx.x) * kOwn + own;
-  const int which = blockIdx.y;
-  const int64_t row = q / chunks, col = (q - row * chunks) * E;
-  const int64_t plane = static_cast<int64_t>(a.rows) * a.part_row;
+  const int q = static_cast<int>(blockIdx.x % kGroups) * kOwn + own;
+  const int r = q / kChunks, c = q % kChunks * E;
   float v[2][E];
 #pragma unroll
   for (int h = 0; h < 2; ++h)
 #pragma unroll
     for (int i = 0; i < E; ++i)
       v[h][i] = 0.f;
-  if (q < total) {
-    const float *from =
-        a.part + static_cast<int64_t>(which) * kHalf * plane + row * a.part_row + col;
-    for (int p = part; p < a.splits; p += PARTS) {
-      const float *at = from + static_cast<int64_t>(p) * a.outs * kHalf * plane;
+  for (int32_t w = w0 + part; w <= w1; w += PARTS) {
+    // a workgroup whose part begins in this tile has its sums in its first place
+    const int slot = gemm_begins(units, a.parts, w, u0 - 1) ? 1 : 0;
+    const float *at =
+        a.part + (static_cast<int64_t>(w) * 2 + slot) * BI * SHAPE::BJ + r * kRow + c;
 #pragma unroll
-      for (int h = 0; h < kHalf; ++h)
+    for (int h = 0; h < kHalf; ++h)
 #pragma unroll
-        for (int i = 0; i < E; i += 4) {
-          const v4f f = *reinterpret_cast<const v4f *>(at + h * plane + i);
+      for (int i = 0; i < E; i += 4) {
+        const v4f f = *reinterpret_cast<const v4f *>(at + h * BI * kRow + i);
 #pragma unroll
-          for (int e = 0; e < 4; ++e)
-            v[h][i + e] += f[e];
-        }
-    }
+        for (int e = 0; e < 4; ++e)
+          v[h][i + e] += f[e];
+      }
   }
   if constexpr (PARTS > 1) {
     __shared__ float sums[PARTS][kSums][kOwn];
@@ -313,16 +376,16 @@ __global__ __launch_bounds__(kGatedThreads) void gated_join_kernel(GatedArgs a) 
       for (int p = 1; p < PARTS; ++p)
         v[i / E][i % E] += sums[p][i][own];
   }
-  if (q >= total)
+  const int32_t row = ti * BI + r, col = tj * kRow + c, left = a.cols - col;
+  if (row >= a.rows)
     return;
-  const int32_t left = static_cast<int32_t>(a.cols - col);
   if constexpr (STAGE == kPlain) {
     T *to = static_cast<T *>(a.out[which]) + row * a.out_row + col;
 #pragma unroll
     for (int i = 0; i < E; ++i)
       if (i < left)
         to[i] = from_f32<T>(v[0][i]);
-  } else {
+  } else if (col < a.pitch) {
     finish_chunk<T, STAGE>(a, row * a.pitch + col, left, v);
   }
 }
@@ -573,20 +636,25 @@ void run_packs(std::initializer_list<const Packed *> matrices, hipStream_t strea
   RHIP_LAUNCH_CHECK();
 }
 
-// The tiles and splits of a product by estimated time, in microseconds: rounds of
-// 256x256 tiles, one workgroup to a CU (bf16), 128x128 ones, two, or 64x64 ones,
-// four. A tile of k takes `alone` however few workgroups there are; the CU's
-// share of it grows with their number up to `full`. (bf16, 4000 rows, 1024
-// channels, 4096 hidden: the weights' gradients 97 us in 256x256 tiles, which
-// fill half the chip, 71 in 128x128; fp32, 500 x 500 x 500: 15 to 18 us a product
-// in 128x128 tiles.) Splits add their sums' way through memory and a launch.
-enum ProductTiles { kLargeTiles, kSmallTiles, kTinyTiles };
+enum ProductTiles : int32_t { kLargeTiles, kSmallTiles, kTinyTiles };
 struct ProductPlan {
   ProductTiles tiles;
-  int32_t splits;
-  size_t part; // floats of the splits' sums
+  int32_t parts; // workgroups that share the tiles; 0: one has each
+  size_t part;   // fp32 values of the parts' sums
 };
-constexpr int64_t kMostParts = int64_t(64) << 20; // floats, of all splits
+
+// How a product's work is shared, by estimated time in microseconds: 256x256 tiles,
+// one workgroup to a CU (bf16), 128x128 ones, two, or 64x64 ones, four; a
+// workgroup to every tile, or k shared: in fp32 by as many workgroups as the chip
+// holds at once, or a half or a quarter of them, an equal part of all tiles of k
+// each; in bf16 every tile by 2, 4 .. of them (parts that begin inside a tile
+// load other slices of k than their neighbours, which share what an XCD's L2
+// holds: 12000 rows, 300 channels, 700 hidden 206 us, 166 even; 16000, 512, 1024
+// 298 and 255). A tile of k takes `alone` however few workgroups there are; more
+// of them on a CU share its matrix cores (fp32) or its way to memory (bf16, up to
+// `full`). (bf16, 4000 rows, 1024 channels, 4096 hidden: the weights' gradients 97
+// us in 256x256 tiles, which fill half the chip, 71 in 128x128. fp32, 2000 rows,
+// 300 channels, 4000 hidden, a pass: 565 us with tiles cut evenly, 488.)
 ProductPlan plan_product(int64_t rows, int64_t cols, int64_t k_tiles, int64_t outs, bool halves,
                          int32_t dtype) {
   struct Cost {
@@ -594,93 +662,110 @@ ProductPlan plan_product(int64_t rows, int64_t cols, int64_t k_tiles, int64_t ou
     double slots, start, alone, full;
   };
   static constexpr Cost kCosts[2][3] = {
-      {{256, 256, 6.0, 7.0, 9.0}, {128, 512, 3.0, 1.8, 4.0}, {64, 1024, 2.0, 0.55, 2.2}},
-      {{256, 256, 6.0, 1.65, 1.9}, {128, 512, 3.0, 0.35, 1.15}, {64, 1024, 2.0, 0.3, 0.75}}};
+      {{256, 256, 6.0, 9.0, 9.0}, {128, 512, 4.0, 2.2, 2.2}, {64, 1024, 3.0, 0.82, 0.64}},
+      {{256, 256, 12.0, 1.65, 1.9}, {128, 512, 6.0, 0.9, 1.15}, {64, 1024, 3.0, 0.5, 0.9}}};
   const bool f32 = dtype == RHIP_F32;
-  const int64_t part_row = static_cast<int64_t>(align_up(static_cast<size_t>(cols), 4));
-  const int64_t plane = rows * part_row * outs * (halves ? 2 : 1);
   ProductPlan best{};
   double least = 0.0;
   for (int shape = f32 ? kSmallTiles : kLargeTiles; shape <= kTinyTiles; ++shape) {
     const Cost &c = kCosts[f32 ? 0 : 1][shape];
-    const int64_t wide = c.side / (halves && shape != kTinyTiles ? 2 : 1);
-    const int64_t tiles = ceil_div(rows, c.side) * ceil_div(cols, wide) * outs;
     // the pair of a 64x64 tile is twice a tile's work
-    const double twice = halves && shape == kTinyTiles ? 2.0 : 1.0;
-    for (int64_t s = 1; s <= 64; s *= 2) {
-      if (s > 1 && (k_tiles < 4 * s || plane * s > kMostParts))
-        break;
-      const double rounds = std::ceil(static_cast<double>(tiles * s) / c.slots);
-      const double fill = std::min(1.0, static_cast<double>(tiles * s) / c.slots);
-      // of bf16 the sums are waited for, of fp32 the matrix cores
-      const double turn = std::max(c.alone, c.full * (f32 ? fill : std::sqrt(fill))) * twice;
-      double t = rounds * (c.start + static_cast<double>(ceil_div(k_tiles, s)) * turn);
-      if (s > 1)
-        t += 4.0 + static_cast<double>(plane) * (s + 1) * 4.0 / 4.0e6;
-      if (least == 0.0 || t < least) {
-        least = t;
-        best = {static_cast<ProductTiles>(shape), static_cast<int32_t>(s),
-                s > 1 ? static_cast<size_t>(plane * s) : 0};
+    const bool pair = halves && shape == kTinyTiles;
+    const double twice = pair ? 2.0 : 1.0;
+    const int64_t wide = c.side / (halves && !pair ? 2 : 1);
+    const int64_t tiles = ceil_div(rows, c.side) * ceil_div(cols, wide) * outs;
+    const double n = static_cast<double>(tiles), k = static_cast<double>(k_tiles);
+    // a tile of k, with so many workgroups there: in bf16 the loads are waited
+    // for, in fp32 the fullest CU's matrix cores
+    auto turn = [&](double groups) {
+      return twice * std::max(c.alone, f32 ? c.full * std::ceil(groups / 256.0)
+                                           : c.full * std::sqrt(std::min(1.0, groups / c.slots)));
+    };
+    auto consider = [&](double t, int64_t parts) {
+      if (least != 0.0 && t >= least)
+        return;
+      least = t;
+      best = {static_cast<ProductTiles>(shape), static_cast<int32_t>(parts),
+              static_cast<size_t>(parts * 2 * c.side * c.side) * (pair ? 2 : 1)};
+    };
+    // `each` of a tile's turns for a workgroup, `starts` of tiles
+    auto shared = [&](int64_t parts, double starts, double each) {
+      const double p = static_cast<double>(parts);
+      const double sums = (p + std::min(p, n)) * c.side * c.side * 4.0 * twice;
+      consider(starts * c.start + each * turn(p) + 5.0 + sums / 4.0e6, parts);
+    };
+    if (f32) {
+      consider((std::floor(n / c.slots) + 1.0) * c.start + k * turn(n), 0);
+      for (const double share : {1.0, 0.5, 0.25}) {
+        const int64_t parts =
+            std::min<int64_t>(static_cast<int64_t>(c.slots * share), tiles * k_tiles / 4);
+        if (parts >= 2 && parts != tiles)
+          shared(parts, std::ceil(n / parts) + 1.0, n * k / parts);
       }
+      continue;
+    }
+    for (int64_t s = 1; s == 1 || (s <= 64 && 4 * s <= k_tiles && tiles * s <= 2 * c.slots);
+         s *= 2) {
+      const double rounds = std::ceil(n * s / c.slots);
+      if (s == 1)
+        consider(rounds * (c.start + k * turn(n)), 0);
+      else
+        shared(tiles * s, rounds, rounds * std::ceil(k / s));
     }
   }
   return best;
 }
 
-// Launches a product of the given stage, and what joins its splits.
+// Launches a product of the given stage, and what joins its shared tiles.
 template <typename T, bool YACROSS, bool XACROSS, GemmPair PAIR, GatedStage STAGE>
 void run_product(GatedArgs a, const ProductPlan &plan, float *part, hipStream_t stream) {
   if (a.rows == 0)
     return;
   constexpr int kHalf = PAIR == kGemmHalves ? 2 : 1;
-  a.splits = plan.splits;
-  a.layers = plan.splits * a.outs;
   a.part = part;
-  // h, dg and du have zeros behind the last column, up to their pitch
-  a.part_row = STAGE == kPlain ? static_cast<int64_t>(align_up(static_cast<size_t>(a.cols), 4))
-                               : a.pitch;
-  auto launch = [&](auto shape, auto stage) {
+  auto launch = [&](auto shape) {
     using SHAPE = decltype(shape);
-    constexpr GatedStage S = static_cast<GatedStage>(decltype(stage)::value);
     a.tiles_i = static_cast<int32_t>(ceil_div(a.rows, SHAPE::BI));
     a.tiles_j = static_cast<int32_t>(ceil_div(a.cols, SHAPE::BJ / kHalf));
-    const int64_t tiles = static_cast<int64_t>(a.tiles_i) * a.tiles_j * a.layers;
+    const int64_t tiles = static_cast<int64_t>(a.tiles_i) * a.tiles_j * a.outs;
     if (gemm_grid(tiles) > max_groups(SHAPE::kThreads))
       throw Error(RHIP_ERR_UNSUPPORTED, "too many tiles");
-    hipLaunchKernelGGL((gated_product_kernel<T, SHAPE, YACROSS, XACROSS, PAIR, S>),
-                       dim3(static_cast<unsigned>(gemm_grid(tiles))), dim3(SHAPE::kThreads), 0,
-                       stream, a);
+    const dim3 threads(SHAPE::kThreads);
+    if (plan.parts == 0) {
+      a.parts = static_cast<int32_t>(tiles);
+      hipLaunchKernelGGL((gated_product_kernel<T, SHAPE, YACROSS, XACROSS, PAIR, STAGE, false>),
+                         dim3(static_cast<unsigned>(gemm_grid(tiles))), threads, 0, stream, a);
+      RHIP_LAUNCH_CHECK();
+      return;
+    }
+    a.parts = plan.parts;
+    hipLaunchKernelGGL((gated_product_kernel<T, SHAPE, YACROSS, XACROSS, PAIR, STAGE, true>),
+                       dim3(static_cast<unsigned>(gemm_grid(a.parts))), threads, 0, stream, a);
     RHIP_LAUNCH_CHECK();
+    constexpr int E = STAGE == kPlain ? 4 : 16 / static_cast<int>(sizeof(T));
+    auto join = [&](auto n) {
+      constexpr int PARTS = decltype(n)::value;
+      constexpr int64_t kGroups = int64_t(SHAPE::BI) * (SHAPE::BJ / kHalf) / E /
+                                  (kGatedThreads / PARTS);
+      if (tiles * kGroups > max_groups(kGatedThreads))
+        throw Error(RHIP_ERR_UNSUPPORTED, "too many tiles");
+      hipLaunchKernelGGL((gated_join_kernel<T, SHAPE, PAIR, STAGE, PARTS>),
+                         dim3(static_cast<unsigned>(tiles * kGroups)), dim3(kGatedThreads), 0,
+                         stream, a);
+      RHIP_LAUNCH_CHECK();
+    };
+    // few chunks leave most of the chip idle unless several threads share one
+    if (a.parts >= 8 * tiles && tiles * (SHAPE::BI * (SHAPE::BJ / kHalf) / E) < 256 * 1024)
+      join(std::integral_constant<int, 8>{});
+    else
+      join(std::integral_constant<int, 1>{});
   };
-  auto sized = [&](auto stage) {
-    if constexpr (sizeof(T) == 2) // in fp32 no faster than 128x128 tiles
-      if (plan.tiles == kLargeTiles)
-        return launch(LargeTiles{}, stage);
-    if (plan.tiles == kSmallTiles)
-      return launch(SmallTiles{}, stage);
-    launch(std::conditional_t<PAIR == kGemmHalves, TinyPairs, TinyTiles>{}, stage);
-  };
-  if (plan.splits == 1) {
-    sized(std::integral_constant<int, STAGE>{});
-    return;
-  }
-  sized(std::integral_constant<int, kPartial>{});
-  // of at most kMostParts values
-  const int64_t chunks =
-      a.part_row / (STAGE == kPlain ? 4 : 16 / static_cast<int64_t>(sizeof(T))) * a.rows;
-  auto join = [&](auto parts) {
-    constexpr int PARTS = decltype(parts)::value;
-    hipLaunchKernelGGL((gated_join_kernel<T, STAGE, PARTS>),
-                       dim3(static_cast<unsigned>(ceil_div(chunks, kGatedThreads / PARTS)),
-                            a.outs),
-                       dim3(kGatedThreads), 0, stream, a);
-  };
-  // few chunks leave most of the chip idle unless several threads share one
-  if (a.splits >= 8 && chunks * a.outs < 256 * 1024)
-    join(std::integral_constant<int, 8>{});
-  else
-    join(std::integral_constant<int, 1>{});
-  RHIP_LAUNCH_CHECK();
+  if constexpr (sizeof(T) == 2) // in fp32 no faster than 128x128 tiles
+    if (plan.tiles == kLargeTiles)
+      return launch(LargeTiles{});
+  if (plan.tiles == kSmallTiles)
+    return launch(SmallTiles{});
+  launch(std::conditional_t<PAIR == kGemmHalves, TinyPairs, TinyTiles>{});
 }
 
 GemmSide side(const Packed &m, bool across, const Packed *second = nullptr) {

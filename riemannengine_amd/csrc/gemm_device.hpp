@@ -137,28 +137,48 @@ template <typename T, int B, bool ACROSS, int THREADS> struct GemmTile {
   }
 };
 
-// Workgroup -> tile. Workgroups are dealt to the XCDs round-robin; each XCD gets
-// a run of consecutive tiles, and the tiles come in bands of eight rows of
-// tiles, column by column: what runs at once on an XCD shares an L2's worth of
+// Workgroup -> its place among `groups`, so that each XCD, to which they are dealt
+// round-robin, gets consecutive ones; false for those that fill the grid up.
+__device__ __forceinline__ bool gemm_place(uint32_t groups, uint32_t &place) {
+  const uint32_t per = (groups + kXcds - 1) / kXcds, m = blockIdx.x / kXcds;
+  place = blockIdx.x % kXcds * per + m;
+  return m < per && place < groups;
+}
+inline int64_t gemm_grid(int64_t groups) { return ceil_div(groups, kXcds) * kXcds; }
+
+// Tile t of `outs` results of tiles_i x tiles_j tiles: in bands of eight rows of
+// tiles, column by column, so what runs at once on an XCD shares an L2's worth of
 // both sides.
-__device__ __forceinline__ bool gemm_tile(uint32_t tiles_i, uint32_t tiles_j, uint32_t layers,
-                                          int32_t &ti, int32_t &tj, int32_t &layer) {
-  const uint32_t total = tiles_i * tiles_j * layers;
-  const uint32_t per = (total + kXcds - 1) / kXcds, x = blockIdx.x % kXcds, m = blockIdx.x / kXcds;
-  const uint32_t t = x * per + m;
-  if (m >= per || t >= total)
-    return false;
+__device__ __forceinline__ void gemm_tile(uint32_t tiles_i, uint32_t tiles_j, uint32_t t,
+                                          int32_t &ti, int32_t &tj, int32_t &out) {
   constexpr uint32_t kBand = 8;
   const uint32_t plane = tiles_i * tiles_j;
-  layer = t / plane;
-  const uint32_t rem = t - layer * plane, band = rem / (kBand * tiles_j);
+  out = t / plane;
+  const uint32_t rem = t - out * plane, band = rem / (kBand * tiles_j);
   const uint32_t in = rem - band * kBand * tiles_j;
   const uint32_t high = min(kBand, tiles_i - band * kBand);
   ti = band * kBand + in % high;
   tj = in / high;
-  return true;
 }
-inline int64_t gemm_grid(int64_t tiles) { return ceil_div(tiles, kXcds) * kXcds; }
+
+// The work of a product as one line of `units`, tiles of k tile by tile, in equal
+// parts of the line: part w's first unit.
+__device__ __forceinline__ int64_t gemm_cut(int64_t units, int32_t parts, int64_t w) {
+  return units * w / parts;
+}
+// Whether part w begins at unit u or before it: gemm_cut(w) <= u, with no division.
+__device__ __forceinline__ bool gemm_begins(int64_t units, int32_t parts, int64_t w, int64_t u) {
+  return units * w < (u + 1) * parts;
+}
+// The part that holds unit u.
+__device__ __forceinline__ int32_t gemm_part(int64_t units, int32_t parts, int64_t u) {
+  int32_t w = static_cast<int32_t>(static_cast<double>(u) * parts / static_cast<double>(units));
+  while (w + 1 < parts && gemm_begins(units, parts, w + 1, u))
+    ++w;
+  while (w > 0 && !gemm_begins(units, parts, w, u))
+    --w;
+  return w;
+}
 
 // A workgroup's waves and each wave's blocks.
 template <int WI_, int WJ_, int NI_, int NJ_> struct GemmShape {
@@ -174,8 +194,8 @@ enum GemmPair { kGemmOne, kGemmHalves, kGemmBehind };
 
 // The sums of a workgroup's tile of results over its tiles of k: WI x WJ waves,
 // each with NI x NJ blocks of 32 by 32. acc[b][a]: X block b, Y block a. With
-// kGemmHalves a wave's first NJ / 2 blocks are the first
-// matrix', the others the second's.
+// kGemmHalves a wave's first NJ / 2 blocks are the first matrix', the others the
+// second's.
 //
 // Two LDS buffers and one barrier a tile: at the last of its four steps every
 // wave has read the whole tile and the next one has landed; the loads of the
@@ -188,6 +208,8 @@ template <typename T, typename SHAPE, bool YACROSS, bool XACROSS, GemmPair PAIR>
   using XTile = GemmTile<T, BJ, XACROSS, SHAPE::kThreads>;
   using Frag = typename Mfma<T>::Frag;
   static constexpr int kLds = 2 * (YTile::kBytes + XTile::kBytes);
+  static constexpr int kStrip = kLds / SHAPE::kWaves; // a wave's share once the sums are done
+  static constexpr int kHalves = PAIR == kGemmHalves ? 2 : 1;
   static_assert(PAIR != kGemmHalves || (!XACROSS && NJ % 2 == 0), "halves: k along the rows");
   static_assert(YTile::kRowsPerLoad % 4 == 0 && XTile::kRowsPerLoad % 4 == 0,
                 "a thread's loads share their chunk's turn");
