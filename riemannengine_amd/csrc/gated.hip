@@ -329,13 +329,23 @@ __global__ __launch_bounds__(kGatedThreads) void gated_join_kernel(GatedArgs a) 
   constexpr int BI = SHAPE::BI, kRow = SHAPE::BJ / kHalf, kChunks = kRow / E; // of a tile's row
   constexpr int kOwn = kGatedThreads / PARTS;             // chunks of a workgroup
   constexpr int kGroups = BI * kChunks / kOwn;            // workgroups of a tile
-  const uint32_t t = blockIdx.x / kGroups;
-  const int64_t units = static_cast<int64_t>(a.tiles_i) * a.tiles_j * a.outs * a.k_tiles;
-  const int64_t u0 = static_cast<int64_t>(t) * a.k_tiles;
-  const int32_t w0 = wave_uniform(gemm_part(units, a.parts, u0));
-  const int32_t w1 = wave_uniform(gemm_part(units, a.parts, u0 + a.k_tiles - 1));
+  const uint32_t tiles = static_cast<uint32_t>(a.tiles_i) * a.tiles_j * a.outs;
+  const int64_t units = static_cast<int64_t>(tiles) * a.k_tiles;
+  uint32_t t = blockIdx.x / kGroups;
+  int32_t w0, w1; // the first and last workgroup with a part of it
+  if (tiles <= static_cast<uint32_t>(a.parts)) {
+    w0 = wave_uniform(gemm_part(units, a.parts, static_cast<int64_t>(t) * a.k_tiles));
+    w1 = wave_uniform(gemm_part(units, a.parts, static_cast<int64_t>(t + 1) * a.k_tiles - 1));
+  } else { // the tile that workgroup t and its neighbour share
+    w0 = t, w1 = w0 + 1;
+    const int64_t cut = gemm_cut(units, a.parts, w1);
+    t = static_cast<uint32_t>(cut / a.k_tiles);
+    if (cut == static_cast<int64_t>(t) * a.k_tiles)
+      return;
+  }
   if (w0 == w1)
     return; // one workgroup had it whole
+  const int64_t u0 = static_cast<int64_t>(t) * a.k_tiles;
   int32_t ti, tj, which;
   gemm_tile(a.tiles_i, a.tiles_j, t, ti, tj, which);
   const int own = threadIdx.x % kOwn, part = threadIdx.x / kOwn;
@@ -747,10 +757,9 @@ void run_product(GatedArgs a, const ProductPlan &plan, float *part, hipStream_t 
       constexpr int PARTS = decltype(n)::value;
       constexpr int64_t kGroups = int64_t(SHAPE::BI) * (SHAPE::BJ / kHalf) / E /
                                   (kGatedThreads / PARTS);
-      if (tiles * kGroups > max_groups(kGatedThreads))
-        throw Error(RHIP_ERR_UNSUPPORTED, "too many tiles");
+      const int64_t shared = tiles <= a.parts ? tiles : a.parts - 1; // at most
       hipLaunchKernelGGL((gated_join_kernel<T, SHAPE, PAIR, STAGE, PARTS>),
-                         dim3(static_cast<unsigned>(tiles * kGroups)), dim3(kGatedThreads), 0,
+                         dim3(static_cast<unsigned>(shared * kGroups)), dim3(kGatedThreads), 0,
                          stream, a);
       RHIP_LAUNCH_CHECK();
     };

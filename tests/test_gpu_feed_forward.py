@@ -53,6 +53,7 @@ def test_sizes(n, channels, hidden, outputs, kind, dtype):
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("n,channels,hidden", [
     (4096, 1024, 2048), (4000, 1000, 2100), (70, 2048, 4099), (8300, 64, 96), (513, 4096, 512),
+    (3200, 1024, 1536),  # fp32: parts that hold whole tiles and share their ends
 ])
 def test_large(n, channels, hidden, dtype):
     check(*make(n, channels, hidden, channels, dtype, seed=1), "silu")
