@@ -14,8 +14,9 @@ layers call the gfx950 kernels through the C ABI:
     RiemannGenerativeConvolutionTranspose, the pooling layers,
     RiemannBatchNorm, RiemannReLU, BasicBlock; and, which the reference does
     not have, transformer stages over packed rows: packed_attention,
-    layer_norm, embedding, RiemannAttention, RiemannLayerNorm,
-    RiemannEmbedding, AttentionBlock)
+    rotate_heads, norm_rotate_heads, rotary_frequencies, gated_feed_forward,
+    layer_norm, embedding, RiemannAttention, RiemannGatedFeedForward,
+    RiemannLayerNorm, RiemannEmbedding, AttentionBlock)
 
 The reference's names outside that path (``adaptive``, ``gaussian``,
 ``occupancy``, ``TensorField``, the collation helpers, ``RiemannLinear``, ...)

@@ -1090,6 +1090,12 @@ ATTN_PASSES = ("forward", "queries", "keys")
 ATTN_WINDOW_PASSES = (*ATTN_PASSES, "apart")
 
 
+def _window(window: int, sinks: int) -> RhipAttnWindow:
+    if not all(-2 ** 31 <= v < 2 ** 31 for v in (window, sinks)):
+        raise RuntimeError("a window and its sinks must fit 32 bits")  # ctypes would wrap them
+    return RhipAttnWindow(window, sinks)
+
+
 def attn_plan(which: str, dtype: torch.dtype, n_q: int, n_k: int, n_seq: int, heads: int,
               kv_heads: int, dim: int, causal: bool, window: Optional[int] = None,
               sinks: int = 0):
@@ -1101,7 +1107,7 @@ def attn_plan(which: str, dtype: torch.dtype, n_q: int, n_k: int, n_seq: int, he
     blocks, splits = _i32(0), _i32(0)
     if window is not None:
         _check(lib().rhip_attn_window_plan(
-            ctypes.byref(desc), ctypes.byref(RhipAttnWindow(window, sinks)),
+            ctypes.byref(desc), ctypes.byref(_window(window, sinks)),
             ATTN_WINDOW_PASSES.index(which), ctypes.byref(blocks), ctypes.byref(splits)),
             "rhip_attn_window_plan")
         return blocks.value, splits.value
@@ -1119,7 +1125,7 @@ def _attn_call(name: str, desc: RhipAttn, window: Optional[int], sinks: int, *ar
                f"rhip_attn_{name}")
     else:
         _check(getattr(lib(), f"rhip_attn_window_{name}")(
-            ctypes.byref(desc), ctypes.byref(RhipAttnWindow(window, sinks)), *args),
+            ctypes.byref(desc), ctypes.byref(_window(window, sinks)), *args),
             f"rhip_attn_window_{name}")
 
 
@@ -1269,6 +1275,8 @@ def _rotary_desc(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Te
     sections = [int(v) for v in sections]
     if not 1 <= len(sections) <= ROTARY_MAX_AXES:
         raise RuntimeError("sections must hold 1 to 8 axes")
+    if not all(-2 ** 31 <= v < 2 ** 31 for v in sections):
+        raise RuntimeError("sections must fit 32 bits")
     if (positions.dim() != 2 or tuple(positions.shape) != (q.shape[0], len(sections))
             or positions.dtype not in POSITION_TYPES or positions.device != q.device
             or (positions.shape[1] > 1 and positions.stride(1) != 1)):

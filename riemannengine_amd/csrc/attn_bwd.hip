@@ -129,7 +129,9 @@ __device__ __forceinline__ void join_row(const float *rows, int row_floats, int 
 // Bound by the matrix cores (four causal prompts of 4096, 16 over 4 heads, 128
 // wide, bf16: 398 us, 1035 TFLOP/s), by the vector instructions at 32 wide (890).
 //
-// LOCAL: inside a window, as in the forward.
+// LOCAL: inside a window, as in the forward (causal, 16 over 4 heads of 128, four
+// texts of up to 4096, window 1024: 132 us; both sides, 8 heads of 32, window 256:
+// 32).
 template <typename T, int DP, bool VEC, int W, bool LOCAL>
 __global__ __launch_bounds__(kBwdThreads, (BwdShape<T, DP, W, false>::kOccupancy)) void
 attn_dq_kernel(AttnArgs a) {
@@ -392,7 +394,10 @@ __device__ __forceinline__ int64_t partial_row(const AttnArgs &a, const AttnSeq 
 //
 // LOCAL: inside a window (LocalRows). The keys of the tiles that hold sinks, which
 // rows of the whole sequence see, are a launch of their own (apart_pass), whose
-// workgroups split those rows; partial sums then lie by sequence.
+// workgroups split those rows; partial sums then lie by sequence. (Four causal
+// texts of up to 4096, 16 over 4 heads of 128, window 1024, 4 sinks: 155 us and 29
+// for the keys apart, joins of 16 and 8; in one launch the sinks' workgroups alone
+// would go through every row.)
 template <typename T, int DP, bool VEC, int W, bool LOCAL>
 __global__ __launch_bounds__(kBwdThreads, (BwdShape<T, DP, W, true>::kOccupancy)) void
 attn_dkv_kernel(AttnArgs a) {
@@ -718,8 +723,12 @@ attn_dkv_kernel(AttnArgs a) {
   }
 }
 
-// Adds the splits' partial sums of dk and dv: one wave per key and key head.
-template <typename T>
+// Adds the splits' partial sums of dk and dv, TURN of them at a time: one wave per
+// key and key head. Few splits of many keys are bound by memory (two of 8191 keys, 4
+// heads of 128: 16 us), many of few keys by the loads' latency (32 of 128 keys: 8
+// us; with branches around the lanes' loads 22 and 21). Turns of 16 for six splits
+// of 3301 keys read the last one ten times more: 8.9 us, of 4 5.6.
+template <typename T, int TURN>
 __global__ __launch_bounds__(kBwdThreads) void attn_dkv_join_kernel(AttnArgs a) {
   const int64_t rows = partial_rows(a, a.apart_pass) * a.kv_heads;
   const int lane = lane_id();
@@ -735,14 +744,26 @@ __global__ __launch_bounds__(kBwdThreads) void attn_dkv_join_kernel(AttnArgs a) 
       key = k0 + static_cast<int64_t>(j);
     }
     float gk[2] = {0.f, 0.f}, gv[2] = {0.f, 0.f};
-#pragma unroll 8
-    for (int s = 0; s < a.splits; ++s) {
-      const int64_t p = (s * rows + at) * a.dim;
+    // lanes behind the head's width read its last element, places behind the last
+    // split that split's: with no branch around them all loads of a turn are under
+    // way at once
+    const int c[2] = {min(lane, a.dim - 1), min(lane + kWave, a.dim - 1)};
+    for (int s0 = 0; s0 < a.splits; s0 += TURN) {
+      float k[TURN][2], v[TURN][2];
 #pragma unroll
-      for (int u = 0; u < 2; ++u)
-        if (lane + u * kWave < a.dim) {
-          gk[u] += a.part_k[p + lane + u * kWave];
-          gv[u] += a.part_v[p + lane + u * kWave];
+      for (int i = 0; i < TURN; ++i) {
+        const int64_t p = (min(s0 + i, a.splits - 1) * rows + at) * a.dim;
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+          k[i][u] = a.part_k[p + c[u]], v[i][u] = a.part_v[p + c[u]];
+      }
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int i = 0; i < TURN; ++i)
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          gk[u] += s0 + i < a.splits ? k[i][u] : 0.f;
+          gv[u] += s0 + i < a.splits ? v[i][u] : 0.f;
         }
     }
     finish_dkv<T>(a, key, static_cast<int>(at % a.kv_heads), gk, gv);
@@ -866,10 +887,14 @@ void attn_backward_run(const AttnArgs &args, const AttnApart &apart, int32_t dty
     auto join = [&](AttnArgs a, int64_t keys, int32_t splits) {
       const int64_t rows = keys * args.kv_heads;
       a.splits = splits;
-      hipLaunchKernelGGL((attn_dkv_join_kernel<T>),
-                         dim3(static_cast<unsigned>(
-                             std::min(ceil_div(rows, kBwdWaves), max_groups(kBwdThreads)))),
-                         b, 0, stream, a);
+      const dim3 groups(
+          static_cast<unsigned>(std::min(ceil_div(rows, kBwdWaves), max_groups(kBwdThreads))));
+      if (splits > 8)
+        hipLaunchKernelGGL((attn_dkv_join_kernel<T, 16>), groups, b, 0, stream, a);
+      else if (splits > 3)
+        hipLaunchKernelGGL((attn_dkv_join_kernel<T, 4>), groups, b, 0, stream, a);
+      else
+        hipLaunchKernelGGL((attn_dkv_join_kernel<T, 2>), groups, b, 0, stream, a);
       RHIP_LAUNCH_CHECK();
     };
     with_waves(pk.waves, [&](auto w) {

@@ -232,3 +232,14 @@ def test_sinks_without_a_window(no_library):
     offs = torch.tensor([0, 10], dtype=torch.int32)
     with pytest.raises(RuntimeError, match="beside a window"):
         abi.attn_forward(q, q, q, offs, offs, sinks=2)
+
+
+@pytest.mark.parametrize("window,sinks", [(2 ** 32 + 5, 0), (5, 2 ** 32), (2 ** 31, 1)])
+def test_windows_past_32_bits(window, sinks):
+    with pytest.raises(RuntimeError, match="32 bits"):
+        abi.attn_plan("forward", F32, 10, 10, 1, 4, 4, 16, False, window, sinks)
+
+
+def test_sections_past_32_bits(no_library):
+    with pytest.raises(RuntimeError, match="32 bits"):
+        abi.rotary_forward(**{**ROTARY, "sections": [5, 2 ** 32 + 3]})
