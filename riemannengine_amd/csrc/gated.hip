@@ -263,13 +263,13 @@ __device__ __forceinline__ void keep_tile(char *lds, float *to, v16f (&acc)[P::N
 // equal part: whole tiles, and at its ends parts of tiles, whose sums the join
 // adds. Otherwise a workgroup has a tile.
 //
-// 8192 rows, 2048 channels, 5504 hidden, bf16: g, u and h 434 us (850 TFLOP/s: the
-// activation and what it saves follow the sums), y 175 (1050), dg and du 281, dx
-// 338 (1090), dgate and dup 400, ddown 218; of torch's products alone the best
-// reach 1300. 8320 rows, 256 channels, 683 hidden, fp32: g, u and h 73 us (80
-// TFLOP/s), y 42, dg and du 47, dx 78, dgate and dup 73, ddown 43; a tile to every
-// workgroup, or one k in two or four, took 407 us in all where equal parts take
-// 366.
+// 8192 rows, 2048 channels, 5504 hidden, bf16: g, u and h 400 us (920 TFLOP/s: the
+// activation and what it saves follow the sums), y 169 (1090), dg and du 270 (their
+// bytes alone 94), dx 310 (1190), dgate and dup 380, ddown 206; the library's
+// products alone reach 1300 to 1390. 8320 rows, 256 channels, 683 hidden, fp32: g,
+// u and h 70 us (84 TFLOP/s), y 36 and a join of 8, dg and du 45, dx 61 and 8,
+// dgate and dup 62 and 5, ddown 35 and 6; a tile to every workgroup, or each
+// tile's k in two or four, took 407 us in all where this takes 345.
 template <typename T, typename SHAPE, bool YACROSS, bool XACROSS, GemmPair PAIR, GatedStage STAGE,
           bool SHARED>
 __global__ __launch_bounds__(SHAPE::kThreads, 2) void gated_product_kernel(GatedArgs a) {
