@@ -10,9 +10,9 @@
 //
 // All are tiles of gemm_device.hpp's product, bound by the matrix cores. Where
 // tiles leave part of the chip idle their k is shared by workgroups, whose fp32
-// sums a second kernel adds in order and finishes. Up to 64 rows (single tokens) a
-// kernel that streams the weights through registers takes the forward: it is bound
-// by their bytes.
+// sums a second kernel adds in order and finishes. The forward of few rows (single
+// tokens) goes to a kernel that streams the weights through registers, bound by
+// their bytes.
 //
 // Operands that do not hold aligned, whole 16-byte chunks (odd widths,
 // unaligned views) are laid out once per call in the workspace, zeros behind
@@ -31,7 +31,6 @@
 namespace rhip {
 namespace {
 
-constexpr int kGatedMaxRows = 64; // of the kernel for few rows
 constexpr int kGatedThreads = 256; // of the kernels that join and pack
 using LargeTiles = GemmShape<2, 4, 4, 2>; // 256 x 256, eight waves, one workgroup to a CU
 using SmallTiles = GemmShape<2, 2, 2, 2>; // 128 x 128, four waves, two workgroups
@@ -434,7 +433,7 @@ __global__ __launch_bounds__(kGatedThreads) void gated_pack_kernel(PackJobs jobs
 
 // ---------------------------------------------------------------- few rows
 
-// Up to 16 TB rows: a workgroup's waves share 16 columns (of g and u, or of y) and
+// 16 TB rows each: a workgroup's waves share 16 columns (of g and u, or of y) and
 // part k among them; weights go from memory to registers and the matrix cores as
 // they come, 64 bytes of 16 rows to a load. The waves' sums are added in LDS in
 // order.
@@ -461,7 +460,7 @@ __global__ __launch_bounds__(WAVES *kWave) void gated_few_kernel(FewArgs a) {
   constexpr int kOuts = 256 * TB * N; // results of a workgroup
   __shared__ float sums[WAVES][kOuts];
   const int lane = lane_id(), w = wave_uniform(threadIdx.x / kWave);
-  const int32_t col0 = blockIdx.x * 16;
+  const int32_t col0 = blockIdx.x * 16, row0 = blockIdx.y * 16 * TB;
   const int32_t steps = (a.k + M::kCh - 1) / M::kCh;
   // a quad of lanes loads 64 bytes of one row, which then go to the lanes that
   // hold them as operands: in those lanes' own order each would cost an access
@@ -472,7 +471,7 @@ __global__ __launch_bounds__(WAVES *kWave) void gated_few_kernel(FewArgs a) {
     xp[i] = static_cast<const T *>(a.x[i]) + min(col0 + lr, a.cols - 1) * a.x_row[i] + at;
 #pragma unroll
   for (int b = 0; b < TB; ++b)
-    yp[b] = static_cast<const T *>(a.y) + min(16 * b + lr, a.n - 1) * a.y_row + at;
+    yp[b] = static_cast<const T *>(a.y) + min(row0 + 16 * b + lr, a.n - 1) * a.y_row + at;
   v4f acc[N][TB];
 #pragma unroll
   for (int i = 0; i < N; ++i)
@@ -542,7 +541,7 @@ __global__ __launch_bounds__(WAVES *kWave) void gated_few_kernel(FewArgs a) {
         sums[w][((b * 16 + r) * N + i) * 16 + 4 * (lane >> 4) + e] = acc[i][b][e];
   __syncthreads();
   for (int o = threadIdx.x; o < 256 * TB; o += WAVES * kWave) {
-    const int32_t row = o / 16, c = o % 16, col = col0 + c;
+    const int32_t r = o / 16, c = o % 16, row = row0 + r, col = col0 + c;
     if (row >= a.n)
       break;
     float v[N];
@@ -551,7 +550,7 @@ __global__ __launch_bounds__(WAVES *kWave) void gated_few_kernel(FewArgs a) {
       v[i] = 0.f;
 #pragma unroll
       for (int p = 0; p < WAVES; ++p)
-        v[i] += sums[p][(row * N + i) * 16 + c];
+        v[i] += sums[p][(r * N + i) * 16 + c];
     }
     if constexpr (GATE) {
       if (col >= a.pitch)
@@ -831,12 +830,25 @@ struct GatedForward {
   ProductPlan project, out;
   float *part;
 };
+// Whether the kernel for few rows takes the forward: up to 64 rows, which it takes
+// at once (4096 channels, 11008 hidden, bf16, 64 rows: 80 us, in tiles 86 at 65),
+// and up to 256 where reading the weights again for every 64 rows, mostly from the
+// caches, costs less than the tiles' few workgroups and further launches. 128 rows,
+// bf16: 1024 channels, 2816 hidden 22 us, in tiles 27; 2048, 5504 45 and 36; fp32:
+// 512, 1376 19 and 28; 1024, 2816 44 and 42.
+bool few_rows(const rhip_gated *d) {
+  if (d->n <= 64)
+    return true;
+  const int64_t products =
+      d->n * (2 * static_cast<int64_t>(d->channels) + d->outputs) / 3 * d->hidden;
+  return d->n <= 256 && products <= (d->dtype == RHIP_F32 ? 200'000'000 : 600'000'000);
+}
 GatedForward plan_forward(Carve &cv, const rhip_gated *d, bool keep) {
   GatedForward f{};
   const int64_t pitch = whole_chunks(d->hidden, d->dtype);
   if (!keep)
     f.saved = carve_saved(cv, d, pitch, false);
-  if (d->n <= kGatedMaxRows)
+  if (few_rows(d))
     return f;
   f.x = plan_pack(cv, d->x, d->x_row, d->n, d->channels, d->dtype);
   pack_pair(cv, d, f.gate, f.up);
@@ -897,7 +909,9 @@ template <typename T, bool GATE> void run_few(const FewArgs &f, hipStream_t stre
     auto waves = [&](auto n) {
       constexpr int kWaves = decltype(n)::value;
       hipLaunchKernelGGL((gated_few_kernel<T, decltype(tb)::value, GATE, kWaves>),
-                         dim3(static_cast<unsigned>(groups)), dim3(kWaves * kWave), 0, stream, f);
+                         dim3(static_cast<unsigned>(groups),
+                              static_cast<unsigned>(ceil_div(f.n, 16 * decltype(tb)::value))),
+                         dim3(kWaves * kWave), 0, stream, f);
     };
     // two workgroups for each CU: four waves are enough (11008 hidden: 40 us, with
     // eight 42), else eight (4096 columns: 27 and 28)
@@ -966,7 +980,7 @@ extern "C" int rhip_gated_forward(const rhip_gated *gated, void *y, void *saved,
     with_type(d->dtype, [&](auto t) {
       using T = decltype(t);
       GatedArgs a = gated_args(d, f.saved);
-      if (d->n <= kGatedMaxRows) {
+      if (few_rows(d)) {
         FewArgs w{};
         w.y = d->x, w.y_row = d->x_row;
         w.x[0] = d->gate, w.x[1] = d->up;

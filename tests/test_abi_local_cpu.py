@@ -124,12 +124,14 @@ def test_gated_workspace_holds_what_is_laid_out_anew():
     def size(which=abi.GATED_INFERENCE, **kw):
         return abi._sizeq(L.rhip_gated_workspace_bytes, ctypes.byref(gated(**kw)), which)
 
-    plain = size()
-    assert size(x=4100) >= plain + 100 * 16 * 4
-    assert size(x_row=18) >= plain + 100 * 16 * 4
-    assert size(gate_row=20) >= plain + 2 * 24 * 16 * 4  # unlike strides: both
-    assert size(n=64, x=4100) < plain  # a few rows are read as they lie
-    assert size(channels=15, x_row=16, gate_row=16, up_row=16) >= plain + 100 * 16 * 4
+    n = 300
+    plain = size(n=n)
+    assert size(n=n, x=4100) >= plain + n * 16 * 4
+    assert size(n=n, x_row=18) >= plain + n * 16 * 4
+    assert size(n=n, gate_row=20) >= plain + 2 * 24 * 16 * 4  # unlike strides: both
+    for few in (64, 100, 256):  # read as they lie
+        assert size(n=few, x=4100, gate_row=20) == size(n=few) < plain
+    assert size(n=n, channels=15, x_row=16, gate_row=16, up_row=16) >= plain + n * 16 * 4
 
 
 def test_window_descriptors():

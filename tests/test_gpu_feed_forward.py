@@ -44,6 +44,7 @@ def check(x, gate, up, down, grad_y, kind):
     (1, 1, 1, 1), (1, 64, 96, 64), (3, 7, 5, 9), (16, 33, 47, 12), (17, 128, 200, 64),
     (33, 256, 100, 256), (64, 40, 1000, 40), (65, 40, 1000, 41), (128, 128, 128, 128),
     (129, 63, 130, 65), (300, 96, 257, 96), (257, 520, 300, 136), (1000, 32, 17, 32),
+    (200, 33, 47, 12), (256, 96, 200, 96), (193, 600, 700, 600),  # few rows in several parts
 ])
 def test_sizes(n, channels, hidden, outputs, kind, dtype):
     check(*make(n, channels, hidden, outputs, dtype), kind)
@@ -52,7 +53,7 @@ def test_sizes(n, channels, hidden, outputs, kind, dtype):
 # tiles of 256 rows and columns, and sums over k split or not
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("n,channels,hidden", [
-    (4096, 1024, 2048), (4000, 1000, 2100), (70, 2048, 4099), (8300, 64, 96), (513, 4096, 512),
+    (4096, 1024, 2048), (4000, 1000, 2100), (70, 2048, 4099), (8300, 64, 96), (513, 4096, 512), (180, 2048, 4099),
     (3200, 1024, 1536),  # fp32: parts that hold whole tiles and share their ends
 ])
 def test_large(n, channels, hidden, dtype):
