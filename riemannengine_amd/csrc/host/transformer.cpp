@@ -482,8 +482,11 @@ SparseTensor RiemannAttentionImpl::forward(const SparseTensor &input) {
     { // the layer may be called from several threads
       static std::mutex mutex;
       const std::lock_guard<std::mutex> lock(mutex);
-      if (!frequencies_.defined() || frequencies_.device() != x.device())
+      if (!frequencies_.defined() || frequencies_.device() != x.device()) {
+        // an ordinary tensor whatever this call's mode: later ones save it for a backward
+        const c10::InferenceMode ordinary(false);
         frequencies_ = rotary_frequencies(options_.rotary, options_.rotary_base, x.device());
+      }
       freq = frequencies_;
     }
     if (options_.head_norm) {
