@@ -3,6 +3,8 @@
 // (rhip_attn_*, rhip_ln_*, rhip_embed_*), and the layers that put them on
 // sparse tensors (a sequence = the rows of one batch). These layers have no
 // counterpart in the reference; they follow its layers' conventions.
+#include <c10/core/impl/VirtualGuardImpl.h>
+
 #include <cmath>
 #include <limits>
 #include <mutex>
@@ -489,6 +491,8 @@ SparseTensor RiemannAttentionImpl::forward(const SparseTensor &input) {
       }
       freq = frequencies_;
     }
+    // made on another call's stream, perhaps: kept until this one's kernels are through
+    freq.record_stream(c10::impl::VirtualGuardImpl(x.device().type()).getStream(x.device()));
     if (options_.head_norm) {
       std::tie(q, k) = hip_norm_rotate_heads(q, k, places, freq, options_.rotary,
                                              query_norm_->weight_, key_norm_->weight_);

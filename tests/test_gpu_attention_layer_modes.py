@@ -46,3 +46,30 @@ def test_training_behind_an_evaluation(head_norm, mode):
         assert torch.equal(got, ref)
     with mode():
         assert torch.equal(attention(rie.SparseTensor(x, coords)).F, want[0])
+
+
+def test_frequencies_outlive_another_streams_kernels():
+    """The layer is dropped while a second stream, which called it, has work queued:
+    its frequencies, from the first stream's memory, are held until that is done."""
+    coords, x = rows()
+    attention = layer(False)
+    a = torch.randn(8192, 8192, device=DEV)
+    b = torch.empty_like(a)
+    side = torch.cuda.Stream()
+    with torch.no_grad():
+        attention(rie.SparseTensor(x, coords))
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            out = attention(rie.SparseTensor(x, coords)).F
+            for _ in range(10):  # some 70 ms
+                torch.mm(a, a, out=b)
+
+        def held():  # blocks that are free but for another stream
+            stats = torch.cuda.memory_stats()
+            return stats["active.all.current"] - stats["allocation.all.current"]
+
+        before = held()
+        del attention
+        assert held() == before + 1
+    torch.cuda.synchronize()
+    assert out.isfinite().all()
