@@ -135,7 +135,8 @@ struct HipAttentionFunction : public torch::autograd::Function<HipAttentionFunct
                                     vptr_mut(gk), vptr_mut(gv), ws.data_ptr(), ws.numel(),
                                     stream_of(dev)),
                  "rhip_attn_backward");
-    return {gq, gk, gv, {}, {}, {}, {}, {}, {}, {}};
+    return not_twice({gq, gk, gv, {}, {}, {}, {}, {}, {}, {}}, {s[0], s[1], s[2], grads[0]},
+                     "attention");
   }
 };
 
@@ -197,7 +198,7 @@ struct HipLayerNormFunction : public torch::autograd::Function<HipLayerNormFunct
                                 hip_dtype(x, "layer norm input"), vptr_mut(ws),
                                 ws.defined() ? ws.numel() : 0, stream_of(dev)),
                "rhip_ln_backward");
-    return {gx, gw, gb, {}};
+    return not_twice({gx, gw, gb, {}}, {x, weight, grads[0]}, "layer norm");
   }
 };
 
@@ -243,7 +244,7 @@ struct HipEmbeddingFunction : public torch::autograd::Function<HipEmbeddingFunct
                                    gw.data_ptr(), hip_dtype(gy, "embedding gradient"),
                                    ws.data_ptr(), ws.numel(), stream_of(dev)),
                "rhip_embed_backward");
-    return {{}, gw, {}};
+    return not_twice({{}, gw, {}}, {grads[0]}, "the embedding");
   }
 };
 

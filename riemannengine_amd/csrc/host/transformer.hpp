@@ -4,6 +4,7 @@
 
 #include <ATen/DeviceGuard.h>
 #include <c10/hip/HIPStream.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
 
 #include "riemann.hpp"
 
@@ -66,6 +67,19 @@ inline bool through_autograd(std::initializer_list<at::Tensor> ts) {
 inline void first_derivative_only(const char *what) {
   TORCH_CHECK(!torch::GradMode::is_enabled(), what,
               " has no second derivatives (backward with create_graph)");
+}
+// The same where a backward with create_graph may go through: its gradients, of
+// what `on` holds, refuse to be differentiated themselves.
+inline tensor_list not_twice(tensor_list grads, const tensor_list &on, const char *what) {
+  if (!torch::GradMode::is_enabled())
+    return grads;
+  const size_t n = grads.size();
+  grads.insert(grads.end(), on.begin(), on.end());
+  auto refusal = std::make_shared<torch::autograd::DelayedError>(
+      std::string(what) + " has no second derivatives", static_cast<int64_t>(grads.size()));
+  grads = (*refusal)(std::move(grads));
+  grads.resize(n);
+  return grads;
 }
 
 } // namespace riemann
