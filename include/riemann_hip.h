@@ -828,7 +828,8 @@ int rhip_attn_window_backward(const rhip_attn *attn, const rhip_attn_window *win
  * (p, P + p), or with interleaved != 0 (2 p, 2 p + 1); the first sections[0]
  * pairs turn with the first axis, and so on:
  *
- *   t = positions[row][axis of p] * frequencies[p]   (fp64)
+ *   t = positions[row][axis of p] * frequencies[p]   (fp64; int64 positions
+ *                                                     are exact up to 2^53)
  *   (a, b) -> (a cos t - b sin t, a sin t + b cos t)
  *
  * Elements 2 P .. dim - 1 stay as they are. With norm != 0 the heads are

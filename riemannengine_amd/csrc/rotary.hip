@@ -13,8 +13,9 @@
 // through the (row, head) pairs, each lane with two chunks of 16 bytes that
 // hold its pairs. A head's values stay in registers between its norm and its
 // rotation, so x (and grad_y) are read once and y (grad_x) is written once.
-// Angles are products of fp64, reduced to a part of a turn in fp64: far
-// positions keep the accuracy of near ones.
+// Angles are products of fp64, reduced to a part of a turn by 1 / (2 pi) in two
+// fp64 parts: up to 2^53 radians the reduction is off by less than 2^-50 turns, so
+// a far angle is as exact as its product (half an fp64 step of it).
 //
 // Bound by memory: 16384 rows of 32 + 8 heads of 128, bf16, with the norm: 71 us
 // forward (4.7 TB/s), 96 backward (5.2) and 6 for the weights' sums; by the angles
@@ -113,6 +114,17 @@ __device__ __forceinline__ double rot_position(const RotArgs &p, int64_t row, in
   return static_cast<double>(static_cast<const float *>(p.positions)[at]);
 }
 
+// Angle t as turns, without the whole ones. t times the first part of 1 / (2 pi) less
+// its nearest whole number is exact, at any size; what it leaves with the second part
+// has whole turns again from 2^53 on. (One product and its difference
+// to the nearest whole number: off by up to 2^-24 of a turn at t = 2^31, by any part
+// of one from 2^53 on; in the same time.)
+__device__ __forceinline__ float rot_part(double t) {
+  constexpr double kTurn = 0.15915494309189535, kRest = -9.839338337591243e-18;
+  const double part = fma(t, kRest, fma(t, kTurn, -rint(t * kTurn)));
+  return static_cast<float>(part - rint(part));
+}
+
 // Cosines and sines of the tile's rows: [row][slot], slots = turning * V.
 template <int V>
 __device__ __forceinline__ void rot_table(const RotArgs &p, int32_t row0, int32_t rows,
@@ -123,10 +135,9 @@ __device__ __forceinline__ void rot_table(const RotArgs &p, int32_t row0, int32_
     int axis = 0;
     while (axis < p.axes - 1 && pair >= p.ends[axis])
       ++axis;
-    const double turns = rot_position(p, static_cast<int64_t>(row0) + r, axis) *
-                         p.frequencies[pair] * 0.15915494309189533577; // 1 / (2 pi)
-    const float part = static_cast<float>(turns - rint(turns));
-    sincospif(2.f * part, &sines[i], &cosines[i]);
+    const double t =
+        rot_position(p, static_cast<int64_t>(row0) + r, axis) * p.frequencies[pair];
+    sincospif(2.f * rot_part(t), &sines[i], &cosines[i]);
   }
 }
 
