@@ -927,6 +927,29 @@ int rhip_gated_saved_bytes(const rhip_gated *gated, size_t *bytes);
  * (what is not aligned to 16 bytes is laid out anew in the workspace). */
 int rhip_gated_workspace_bytes(const rhip_gated *gated, int32_t pass, size_t *bytes);
 
+/* The launch of one of a call's products (sizes and dtype alone count): results
+ * in tiles of side x side (the projections': of both, side x side / 2 each, at 64
+ * whole ones), each over k_tiles tiles of k. parts: workgroups that share the
+ * tiles of k, in equal parts of all of them one after another, and join, threads
+ * of the kernel that adds up a 16-byte chunk of a shared tile; both 0 where a
+ * workgroup has each tile. side is 0 where no such launch is made: without rows,
+ * or for few rows, whose forward has kernels of its own. */
+typedef enum rhip_gated_product {
+  RHIP_GATED_HIDDEN = 0,      /* x gate^T, x up^T, h */
+  RHIP_GATED_OUTPUT = 1,      /* y */
+  RHIP_GATED_GRAD_HIDDEN = 2, /* grad_y down, gradients of x gate^T and x up^T */
+  RHIP_GATED_GRAD_X = 3,
+  RHIP_GATED_GRAD_GATES = 4,  /* grad_gate, grad_up */
+  RHIP_GATED_GRAD_DOWN = 5
+} rhip_gated_product;
+
+typedef struct rhip_gated_launch {
+  int64_t tiles;
+  int32_t side, k_tiles, parts, join;
+} rhip_gated_launch;
+
+int rhip_gated_plan(const rhip_gated *gated, int32_t product, rhip_gated_launch *launch);
+
 /* y [n, outputs], dense; saved may be null where no backward follows. */
 int rhip_gated_forward(const rhip_gated *gated, void *y, void *saved,
                        size_t saved_bytes, void *workspace,

@@ -55,8 +55,8 @@ EXPORTS = (
     "rhip_ln_workspace_bytes", "rhip_ln_forward", "rhip_ln_backward",
     "rhip_embed_forward", "rhip_embed_workspace_bytes", "rhip_embed_backward",
     "rhip_rotary_forward", "rhip_rotary_workspace_bytes", "rhip_rotary_backward",
-    "rhip_gated_saved_bytes", "rhip_gated_workspace_bytes", "rhip_gated_forward",
-    "rhip_gated_backward",
+    "rhip_gated_saved_bytes", "rhip_gated_workspace_bytes", "rhip_gated_plan",
+    "rhip_gated_forward", "rhip_gated_backward",
 )
 
 
@@ -121,6 +121,7 @@ class RhipRotaryHeads(ctypes.Structure):
 
 ACTIVATIONS = {"silu": 0, "gelu": 1}
 GATED_INFERENCE, GATED_FORWARD, GATED_BACKWARD = 0, 1, 2
+GATED_PRODUCTS = ("hidden", "output", "grad_hidden", "grad_x", "grad_gates", "grad_down")
 
 
 class RhipGated(ctypes.Structure):
@@ -131,6 +132,13 @@ class RhipGated(ctypes.Structure):
         ("down_row", ctypes.c_int64), ("grad_y_row", ctypes.c_int64),
         ("channels", ctypes.c_int32), ("hidden", ctypes.c_int32), ("outputs", ctypes.c_int32),
         ("activation", ctypes.c_int32), ("dtype", ctypes.c_int32),
+    ]
+
+
+class RhipGatedLaunch(ctypes.Structure):
+    _fields_ = [
+        ("tiles", ctypes.c_int64), ("side", ctypes.c_int32), ("k_tiles", ctypes.c_int32),
+        ("parts", ctypes.c_int32), ("join", ctypes.c_int32),
     ]
 
 
@@ -247,6 +255,7 @@ def _declare(lib):
                                                 _P(RhipRotaryHeads), _vp, _sz, _vp]),
         "rhip_gated_saved_bytes": (ctypes.c_int, [_P(RhipGated), _P(_sz)]),
         "rhip_gated_workspace_bytes": (ctypes.c_int, [_P(RhipGated), _i32, _P(_sz)]),
+        "rhip_gated_plan": (ctypes.c_int, [_P(RhipGated), _i32, _P(RhipGatedLaunch)]),
         "rhip_gated_forward": (ctypes.c_int, [_P(RhipGated), _vp, _vp, _sz, _vp, _sz, _vp]),
         "rhip_gated_backward": (ctypes.c_int, [_P(RhipGated), _vp, _sz, _vp, _vp, _vp, _vp, _vp,
                                                _sz, _vp]),
@@ -1370,6 +1379,17 @@ def _gated_desc(x, gate, up, down, activation, grad_y=None) -> RhipGated:
                      up.stride(0), down.stride(0), 0 if grad_y is None else grad_y.stride(0),
                      x.shape[1], gate.shape[0], down.shape[0], ACTIVATIONS[activation],
                      _dtype_code(x.dtype))
+
+
+def gated_plan(product: str, dtype: torch.dtype, n: int, channels: int, hidden: int,
+               outputs: int) -> RhipGatedLaunch:
+    """The launch of one of GATED_PRODUCTS, from rhip_gated_plan."""
+    desc = RhipGated(n=n, channels=channels, hidden=hidden, outputs=outputs,
+                     dtype=_dtype_code(dtype))
+    launch = RhipGatedLaunch()
+    _check(lib().rhip_gated_plan(ctypes.byref(desc), GATED_PRODUCTS.index(product),
+                                 ctypes.byref(launch)), "rhip_gated_plan")
+    return launch
 
 
 def gated_forward(x: torch.Tensor, gate: torch.Tensor, up: torch.Tensor, down: torch.Tensor,

@@ -579,7 +579,7 @@ __global__ __launch_bounds__(WAVES *kWave) void gated_few_kernel(FewArgs a) {
 
 // ------------------------------------------------------------------ host
 
-void check_gated(const rhip_gated *d) {
+void check_gated_sizes(const rhip_gated *d) {
   RHIP_CHECK_ARG(d != nullptr, "descriptor is null");
   if (d->dtype != RHIP_F32 && d->dtype != RHIP_BF16)
     throw Error(RHIP_ERR_UNSUPPORTED, "dtype must be RHIP_F32 or RHIP_BF16");
@@ -590,6 +590,9 @@ void check_gated(const rhip_gated *d) {
                 "at most 2^31 - 257 rows and 2^20 channels, hidden channels and outputs");
   RHIP_CHECK_ARG(d->activation == RHIP_ACT_SILU || d->activation == RHIP_ACT_GELU,
                  "activation must be one of RHIP_ACT_");
+}
+void check_gated(const rhip_gated *d) {
+  check_gated_sizes(d);
   RHIP_CHECK_ARG((d->n == 0 || d->x) && d->gate && d->up && d->down,
                  "x, gate, up and down are required");
 }
@@ -652,6 +655,24 @@ struct ProductPlan {
   size_t part;   // fp32 values of the parts' sums
 };
 
+// A product's results, their tiles of k, and whether a tile holds both projections.
+struct ProductSize {
+  int64_t rows, cols, k_tiles, outs;
+  bool halves;
+};
+ProductSize product_size(const rhip_gated &d, int32_t product) {
+  const int64_t bk = kGemmTileBytes / static_cast<int64_t>(element_bytes(d.dtype));
+  const int64_t pitch = whole_chunks(d.hidden, d.dtype), kn = ceil_div(d.n, bk);
+  switch (product) {
+  case RHIP_GATED_HIDDEN: return {d.n, pitch, ceil_div(d.channels, bk), 1, true};
+  case RHIP_GATED_OUTPUT: return {d.n, d.outputs, ceil_div(pitch, bk), 1, false};
+  case RHIP_GATED_GRAD_HIDDEN: return {d.n, pitch, ceil_div(d.outputs, bk), 1, false};
+  case RHIP_GATED_GRAD_X: return {d.n, d.channels, 2 * ceil_div(d.hidden, bk), 1, false};
+  case RHIP_GATED_GRAD_GATES: return {d.hidden, d.channels, kn, 2, false};
+  default: return {d.outputs, d.hidden, kn, 1, false};
+  }
+}
+
 // How a product's work is shared, by estimated time in microseconds: 256x256 tiles,
 // one workgroup to a CU (bf16), 128x128 ones, two, or 64x64 ones, four; a
 // workgroup to every tile, or k shared: in fp32 by as many workgroups as the chip
@@ -664,8 +685,9 @@ struct ProductPlan {
 // `full`). (bf16, 4000 rows, 1024 channels, 4096 hidden: the weights' gradients 97
 // us in 256x256 tiles, which fill half the chip, 71 in 128x128. fp32, 2000 rows,
 // 300 channels, 4000 hidden, a pass: 565 us with tiles cut evenly, 488.)
-ProductPlan plan_product(int64_t rows, int64_t cols, int64_t k_tiles, int64_t outs, bool halves,
-                         int32_t dtype) {
+ProductPlan plan_product(const ProductSize &size, int32_t dtype) {
+  const int64_t rows = size.rows, cols = size.cols, k_tiles = size.k_tiles, outs = size.outs;
+  const bool halves = size.halves;
   struct Cost {
     int64_t side;
     double slots, start, alone, full;
@@ -725,6 +747,12 @@ ProductPlan plan_product(int64_t rows, int64_t cols, int64_t k_tiles, int64_t ou
   return best;
 }
 
+// Threads of the join for each of a product's chunks: few chunks leave most of the
+// chip idle unless several threads share one.
+int32_t join_threads(int64_t parts, int64_t tiles, int64_t tile_chunks) {
+  return parts >= 8 * tiles && tiles * tile_chunks < 256 * 1024 ? 8 : 1;
+}
+
 // Launches a product of the given stage, and what joins its shared tiles.
 template <typename T, bool YACROSS, bool XACROSS, GemmPair PAIR, GatedStage STAGE>
 void run_product(GatedArgs a, const ProductPlan &plan, float *part, hipStream_t stream) {
@@ -762,8 +790,7 @@ void run_product(GatedArgs a, const ProductPlan &plan, float *part, hipStream_t 
                          stream, a);
       RHIP_LAUNCH_CHECK();
     };
-    // few chunks leave most of the chip idle unless several threads share one
-    if (a.parts >= 8 * tiles && tiles * (SHAPE::BI * (SHAPE::BJ / kHalf) / E) < 256 * 1024)
+    if (join_threads(a.parts, tiles, SHAPE::BI * (SHAPE::BJ / kHalf) / E) > 1)
       join(std::integral_constant<int, 8>{});
     else
       join(std::integral_constant<int, 1>{});
@@ -853,9 +880,8 @@ GatedForward plan_forward(Carve &cv, const rhip_gated *d, bool keep) {
   f.x = plan_pack(cv, d->x, d->x_row, d->n, d->channels, d->dtype);
   pack_pair(cv, d, f.gate, f.up);
   f.down = plan_pack(cv, d->down, d->down_row, d->outputs, d->hidden, d->dtype);
-  const int64_t bk = kGemmTileBytes / static_cast<int64_t>(element_bytes(d->dtype));
-  f.project = plan_product(d->n, pitch, ceil_div(d->channels, bk), 1, true, d->dtype);
-  f.out = plan_product(d->n, d->outputs, ceil_div(pitch, bk), 1, false, d->dtype);
+  f.project = plan_product(product_size(*d, RHIP_GATED_HIDDEN), d->dtype);
+  f.out = plan_product(product_size(*d, RHIP_GATED_OUTPUT), d->dtype);
   f.part = cv.take<float>(std::max(f.project.part, f.out.part));
   return f;
 }
@@ -876,12 +902,10 @@ GatedBackward plan_backward(Carve &cv, const rhip_gated *d) {
   const size_t n = static_cast<size_t>(std::max<int64_t>(d->n, 1)) * pitch;
   b.dg = cv.take<char>(n * element_bytes(d->dtype));
   b.du = cv.take<char>(n * element_bytes(d->dtype));
-  const int64_t bk = kGemmTileBytes / static_cast<int64_t>(element_bytes(d->dtype));
-  const int64_t kn = ceil_div(d->n, bk);
-  b.hidden = plan_product(d->n, pitch, ceil_div(d->outputs, bk), 1, false, d->dtype);
-  b.gx = plan_product(d->n, d->channels, 2 * ceil_div(d->hidden, bk), 1, false, d->dtype);
-  b.gw = plan_product(d->hidden, d->channels, kn, 2, false, d->dtype);
-  b.gd = plan_product(d->outputs, d->hidden, kn, 1, false, d->dtype);
+  b.hidden = plan_product(product_size(*d, RHIP_GATED_GRAD_HIDDEN), d->dtype);
+  b.gx = plan_product(product_size(*d, RHIP_GATED_GRAD_X), d->dtype);
+  b.gw = plan_product(product_size(*d, RHIP_GATED_GRAD_GATES), d->dtype);
+  b.gd = plan_product(product_size(*d, RHIP_GATED_GRAD_DOWN), d->dtype);
   b.part = cv.take<float>(std::max({b.hidden.part, b.gx.part, b.gw.part, b.gd.part}));
   return b;
 }
@@ -956,6 +980,34 @@ extern "C" int rhip_gated_workspace_bytes(const rhip_gated *gated, int32_t pass,
     else
       plan_forward(cv, gated, pass == RHIP_GATED_FORWARD);
     *bytes = cv.used + 256;
+  });
+}
+
+extern "C" int rhip_gated_plan(const rhip_gated *gated, int32_t product, rhip_gated_launch *launch) {
+  return guarded([&] {
+    check_gated_sizes(gated);
+    RHIP_CHECK_ARG(launch != nullptr, "launch is null");
+    RHIP_CHECK_ARG(product >= RHIP_GATED_HIDDEN && product <= RHIP_GATED_GRAD_DOWN,
+                   "product must be one of RHIP_GATED_");
+    *launch = rhip_gated_launch{};
+    const rhip_gated &d = *gated;
+    const bool forward = product <= RHIP_GATED_OUTPUT;
+    if (d.n == 0 && product <= RHIP_GATED_GRAD_X)
+      return;
+    if (forward && few_rows(gated))
+      return;
+    const ProductSize s = product_size(d, product);
+    const ProductPlan p = plan_product(s, d.dtype);
+    const bool halves = s.halves, tiny = p.tiles == kTinyTiles;
+    launch->side = p.tiles == kLargeTiles ? 256 : p.tiles == kSmallTiles ? 128 : 64;
+    const int64_t wide = launch->side / (halves && !tiny ? 2 : 1);
+    launch->tiles = ceil_div(s.rows, launch->side) * ceil_div(s.cols, wide) * s.outs;
+    launch->k_tiles = static_cast<int32_t>(s.k_tiles);
+    launch->parts = p.parts;
+    const bool chunks = product == RHIP_GATED_HIDDEN || product == RHIP_GATED_GRAD_HIDDEN;
+    if (p.parts > 0)
+      launch->join = join_threads(p.parts, launch->tiles,
+                                  launch->side * wide / (chunks ? chunk_elements(d.dtype) : 4));
   });
 }
 
