@@ -124,6 +124,11 @@ template <typename T, int E> __device__ __forceinline__ void put_chunk(T *p, con
 
 // ---------------------------------------------------------------- products
 
+// Tiles of whose sums a workgroup may have a part: in bf16 tiles are cut evenly, so
+// its own; fp32's parts begin and end anywhere, so a last one beside the first.
+constexpr int part_tiles(bool f32) { return f32 ? 2 : 1; }
+template <typename T> constexpr int kPartTiles = part_tiles(sizeof(T) == 4);
+
 enum GatedStage {
   kProject, // h (and the saved planes) from x, gate, up
   kPlain,   // one matrix of results
@@ -138,7 +143,7 @@ struct GatedArgs {
   int32_t rows, cols; // of the results
   void *out[2];
   int64_t out_row;
-  float *part; // fp32 sums of tiles that several workgroups share, two for each
+  float *part; // fp32 sums of tiles that several workgroups share: kPartTiles for each
   GatedSaved saved;
   int64_t pitch; // of h's, dg's, du's and the saved planes' rows
   void *dg, *du;
@@ -309,8 +314,9 @@ __global__ __launch_bounds__(SHAPE::kThreads, 2) void gated_product_kernel(Gated
         finish();
       else
         keep_tile<P>(lds,
-                     a.part + (static_cast<int64_t>(place) * 2 + (u == first ? 0 : 1)) * P::BI *
-                                  P::BJ,
+                     a.part + (static_cast<int64_t>(place) * kPartTiles<T> +
+                               (kPartTiles<T> == 1 || u == first ? 0 : 1)) *
+                                  P::BI * P::BJ,
                      acc);
       u += kt1 - kt0;
       __syncthreads(); // the strips are free for the next tile
@@ -358,9 +364,9 @@ __global__ __launch_bounds__(kGatedThreads) void gated_join_kernel(GatedArgs a) 
       v[h][i] = 0.f;
   for (int32_t w = w0 + part; w <= w1; w += PARTS) {
     // a workgroup whose part begins in this tile has its sums in its first place
-    const int slot = gemm_begins(units, a.parts, w, u0 - 1) ? 1 : 0;
-    const float *at =
-        a.part + (static_cast<int64_t>(w) * 2 + slot) * BI * SHAPE::BJ + r * kRow + c;
+    const int slot = kPartTiles<T> > 1 && gemm_begins(units, a.parts, w, u0 - 1) ? 1 : 0;
+    const float *at = a.part + (static_cast<int64_t>(w) * kPartTiles<T> + slot) * BI * SHAPE::BJ +
+                      r * kRow + c;
 #pragma unroll
     for (int h = 0; h < kHalf; ++h)
 #pragma unroll
@@ -717,7 +723,7 @@ ProductPlan plan_product(const ProductSize &size, int32_t dtype) {
         return;
       least = t;
       best = {static_cast<ProductTiles>(shape), static_cast<int32_t>(parts),
-              static_cast<size_t>(parts * 2 * c.side * c.side) * (pair ? 2 : 1)};
+              static_cast<size_t>(parts * part_tiles(f32) * c.side * c.side) * (pair ? 2 : 1)};
     };
     // `each` of a tile's turns for a workgroup, `starts` of tiles
     auto shared = [&](int64_t parts, double starts, double each) {

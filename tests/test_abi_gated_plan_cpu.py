@@ -74,3 +74,21 @@ def test_refusals(kw, product, match):
     good = abi.RhipGated(n=8, channels=4, hidden=4, outputs=4, dtype=abi.F32)
     assert abi.lib().rhip_gated_plan(ctypes.byref(good), 0, None) != 0
     assert "launch is null" in abi.lib().rhip_last_error().decode()
+
+
+@pytest.mark.parametrize("sizes", [(1000, 4096, 11008, 4096), *SIZES[torch.bfloat16][:6]])
+def test_bf16_parts_hold_one_tile_each(sizes):
+    """bf16 cuts tiles evenly, so a part never has parts of two."""
+    n, channels, hidden, outputs = (s // 8 * 8 for s in sizes)  # nothing is laid out anew
+    d = abi.RhipGated(n=n, x=4096, gate=4096, up=4096, down=4096, grad_y=4096, x_row=channels,
+                      gate_row=channels, up_row=channels, down_row=hidden, grad_y_row=outputs,
+                      channels=channels, hidden=hidden, outputs=outputs, dtype=abi.BF16)
+    for which, products, hiddens in ((abi.GATED_FORWARD, ("hidden", "output"), 0),
+                                     (abi.GATED_BACKWARD, abi.GATED_PRODUCTS[2:], 2)):
+        sums = 0
+        for product in products:
+            launch = abi.gated_plan(product, torch.bfloat16, n, channels, hidden, outputs)
+            both = 2 if product == "hidden" and launch.side == 64 else 1
+            sums = max(sums, launch.parts * launch.side ** 2 * both * 4)
+        got = abi._sizeq(abi.lib().rhip_gated_workspace_bytes, ctypes.byref(d), which)
+        assert sums + hiddens * n * hidden * 2 <= got <= sums + hiddens * n * hidden * 2 + 2048
