@@ -724,12 +724,14 @@ attn_dkv_kernel(AttnArgs a) {
 }
 
 // Adds the splits' partial sums of dk and dv, TURN of them at a time: one wave per
-// key and key head. Few splits of many keys are bound by memory (two of 8191 keys, 4
-// heads of 128: 16 us), many of few keys by the loads' latency (32 of 128 keys: 8
-// us; with branches around the lanes' loads 22 and 21). Turns of 16 for six splits
-// of 3301 keys read the last one ten times more: 8.9 us, of 4 5.6.
-template <typename T, int TURN>
+// key and key head, WIDE: of more than 64 elements. Few splits of many keys are
+// bound by memory (two of 8191 keys, 4 heads of 128: 17 us), many of few keys by the
+// loads' latency (32 of 128 keys: 8 us; with branches around the lanes' loads 22 and
+// 21). Six splits of 3301 keys, 2 heads of 40: 5.1 us; in turns of four, with the
+// second half of a wide head's loads, 5.5; in turns of 16 8.9.
+template <typename T, int TURN, bool WIDE>
 __global__ __launch_bounds__(kBwdThreads) void attn_dkv_join_kernel(AttnArgs a) {
+  constexpr int U = WIDE ? 2 : 1;
   const int64_t rows = partial_rows(a, a.apart_pass) * a.kv_heads;
   const int lane = lane_id();
   for (int64_t at = static_cast<int64_t>(blockIdx.x) * kBwdWaves + threadIdx.x / kWave; at < rows;
@@ -749,19 +751,19 @@ __global__ __launch_bounds__(kBwdThreads) void attn_dkv_join_kernel(AttnArgs a) 
     // way at once
     const int c[2] = {min(lane, a.dim - 1), min(lane + kWave, a.dim - 1)};
     for (int s0 = 0; s0 < a.splits; s0 += TURN) {
-      float k[TURN][2], v[TURN][2];
+      float k[TURN][U], v[TURN][U];
 #pragma unroll
       for (int i = 0; i < TURN; ++i) {
         const int64_t p = (min(s0 + i, a.splits - 1) * rows + at) * a.dim;
 #pragma unroll
-        for (int u = 0; u < 2; ++u)
+        for (int u = 0; u < U; ++u)
           k[i][u] = a.part_k[p + c[u]], v[i][u] = a.part_v[p + c[u]];
       }
       __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
       for (int i = 0; i < TURN; ++i)
 #pragma unroll
-        for (int u = 0; u < 2; ++u) {
+        for (int u = 0; u < U; ++u) {
           gk[u] += s0 + i < a.splits ? k[i][u] : 0.f;
           gv[u] += s0 + i < a.splits ? v[i][u] : 0.f;
         }
@@ -889,12 +891,21 @@ void attn_backward_run(const AttnArgs &args, const AttnApart &apart, int32_t dty
       a.splits = splits;
       const dim3 groups(
           static_cast<unsigned>(std::min(ceil_div(rows, kBwdWaves), max_groups(kBwdThreads))));
+      auto launch = [&](auto turn) {
+        constexpr int TURN = decltype(turn)::value;
+        if (args.dim > kWave)
+          hipLaunchKernelGGL((attn_dkv_join_kernel<T, TURN, true>), groups, b, 0, stream, a);
+        else
+          hipLaunchKernelGGL((attn_dkv_join_kernel<T, TURN, false>), groups, b, 0, stream, a);
+      };
       if (splits > 8)
-        hipLaunchKernelGGL((attn_dkv_join_kernel<T, 16>), groups, b, 0, stream, a);
+        launch(std::integral_constant<int, 16>{});
+      else if (splits == 6)
+        launch(std::integral_constant<int, 6>{});
       else if (splits > 3)
-        hipLaunchKernelGGL((attn_dkv_join_kernel<T, 4>), groups, b, 0, stream, a);
+        launch(std::integral_constant<int, 4>{});
       else
-        hipLaunchKernelGGL((attn_dkv_join_kernel<T, 2>), groups, b, 0, stream, a);
+        launch(std::integral_constant<int, 2>{});
       RHIP_LAUNCH_CHECK();
     };
     with_waves(pk.waves, [&](auto w) {
