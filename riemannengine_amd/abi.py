@@ -1070,6 +1070,12 @@ def _require_dense(t: Optional[torch.Tensor], name: str, shape, dtype: torch.dty
         raise RuntimeError(f"{name} must be a dense {tuple(shape)} tensor of {dtype} on {device}")
 
 
+def _fit_int32(what: str, *values: int) -> None:
+    """ctypes would wrap what does not fit, and the call work on other sizes."""
+    if not all(-2 ** 31 <= v < 2 ** 31 for v in values):
+        raise RuntimeError(f"{what} must fit 32 bits")
+
+
 def _attn_desc(q, k, v, q_offsets, k_offsets, k_lengths, causal, scale) -> RhipAttn:
     _require_cuda(q, "q")
     for t, name in ((k, "k"), (v, "v"), (q_offsets, "q_offsets"), (k_offsets, "k_offsets"),
@@ -1088,6 +1094,7 @@ def _attn_desc(q, k, v, q_offsets, k_offsets, k_lengths, causal, scale) -> RhipA
         raise RuntimeError("q_offsets and k_offsets must hold n_seq + 1 values each")
     if k_lengths is not None and k_lengths.numel() != n_seq:
         raise RuntimeError("k_lengths must hold one value per sequence")
+    _fit_int32("sequences, heads and widths", n_seq, q.shape[1], k.shape[1], q.shape[2])
     return RhipAttn(q.shape[0], k.shape[0], q.stride(0), q.stride(1), k.stride(0), k.stride(1),
                     v.stride(0), v.stride(1), q_offsets.data_ptr(), k_offsets.data_ptr(),
                     None if k_lengths is None else k_lengths.data_ptr(), n_seq, q.shape[1],
@@ -1100,8 +1107,7 @@ ATTN_WINDOW_PASSES = (*ATTN_PASSES, "apart")
 
 
 def _window(window: int, sinks: int) -> RhipAttnWindow:
-    if not all(-2 ** 31 <= v < 2 ** 31 for v in (window, sinks)):
-        raise RuntimeError("a window and its sinks must fit 32 bits")  # ctypes would wrap them
+    _fit_int32("a window and its sinks", window, sinks)
     return RhipAttnWindow(window, sinks)
 
 
@@ -1111,6 +1117,7 @@ def attn_plan(which: str, dtype: torch.dtype, n_q: int, n_k: int, n_seq: int, he
     """(32-row blocks per workgroup, splits) of an attention pass ("forward",
     "queries": grad_q, "keys": grad_k and grad_v; with a window "apart": those
     of the sinks' blocks), from rhip_attn_plan or rhip_attn_window_plan."""
+    _fit_int32("sequences, heads and widths", n_seq, heads, kv_heads, dim)
     desc = RhipAttn(n_q=n_q, n_k=n_k, n_seq=n_seq, heads=heads, kv_heads=kv_heads, dim=dim,
                     causal=int(causal), dtype=_dtype_code(dtype), scale=dim ** -0.5)
     blocks, splits = _i32(0), _i32(0)
@@ -1284,8 +1291,8 @@ def _rotary_desc(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Te
     sections = [int(v) for v in sections]
     if not 1 <= len(sections) <= ROTARY_MAX_AXES:
         raise RuntimeError("sections must hold 1 to 8 axes")
-    if not all(-2 ** 31 <= v < 2 ** 31 for v in sections):
-        raise RuntimeError("sections must fit 32 bits")
+    _fit_int32("sections, heads and widths", *sections, q.shape[1], q.shape[2],
+               0 if k is None else k.shape[1])
     if (positions.dim() != 2 or tuple(positions.shape) != (q.shape[0], len(sections))
             or positions.dtype not in POSITION_TYPES or positions.device != q.device
             or (positions.shape[1] > 1 and positions.stride(1) != 1)):
@@ -1374,6 +1381,7 @@ def _gated_desc(x, gate, up, down, activation, grad_y=None) -> RhipGated:
             raise RuntimeError(f"{name} must be of the rows' dtype and device")
     if grad_y is not None and tuple(grad_y.shape) != (x.shape[0], down.shape[0]):
         raise RuntimeError("grad_y must be [n, outputs]")
+    _fit_int32("widths", x.shape[1], gate.shape[0], down.shape[0])
     return RhipGated(x.shape[0], x.data_ptr(), gate.data_ptr(), up.data_ptr(), down.data_ptr(),
                      None if grad_y is None else grad_y.data_ptr(), x.stride(0), gate.stride(0),
                      up.stride(0), down.stride(0), 0 if grad_y is None else grad_y.stride(0),
@@ -1384,6 +1392,7 @@ def _gated_desc(x, gate, up, down, activation, grad_y=None) -> RhipGated:
 def gated_plan(product: str, dtype: torch.dtype, n: int, channels: int, hidden: int,
                outputs: int) -> RhipGatedLaunch:
     """The launch of one of GATED_PRODUCTS, from rhip_gated_plan."""
+    _fit_int32("widths", channels, hidden, outputs)
     desc = RhipGated(n=n, channels=channels, hidden=hidden, outputs=outputs,
                      dtype=_dtype_code(dtype))
     launch = RhipGatedLaunch()

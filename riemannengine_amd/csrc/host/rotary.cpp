@@ -9,6 +9,7 @@ namespace riemann {
 namespace {
 
 using Sections = std::vector<int64_t>;
+constexpr int64_t kMaxHeads = int64_t(1) << 20;
 
 struct Rotation {
   at::Tensor positions, frequencies;
@@ -144,6 +145,7 @@ Rotation checked_rotation(const at::Tensor &query, const at::Tensor &positions,
   TORCH_CHECK(query.dim() == 3 && query.size(1) > 0 && query.size(2) > 0,
               "heads must be [rows, heads, width], got ", query.sizes());
   TORCH_CHECK(query.size(2) <= 256, "rotation takes head widths up to 256, got ", query.size(2));
+  TORCH_CHECK(query.size(1) <= kMaxHeads, "rotation takes up to 2^20 heads, got ", query.size(1));
   hip_dtype(query, "rotated heads");
   TORCH_CHECK(!sections.empty() && sections.size() <= RHIP_ROTARY_MAX_AXES,
               "rotation takes 1 to ", RHIP_ROTARY_MAX_AXES, " sections, got ", sections.size());
@@ -193,9 +195,9 @@ hip_norm_rotate_heads(const at::Tensor &query, const at::Tensor &key, const at::
   const Rotation r =
       checked_rotation(query, positions, frequencies, sections, interleaved, true, eps);
   TORCH_CHECK(key.dim() == 3 && key.size(0) == query.size(0) && key.size(1) > 0 &&
-                  key.size(2) == query.size(2) && key.device() == query.device() &&
-                  key.scalar_type() == query.scalar_type(),
-              "keys must be [", query.size(0), " rows, heads, ", query.size(2),
+                  key.size(1) <= kMaxHeads && key.size(2) == query.size(2) &&
+                  key.device() == query.device() && key.scalar_type() == query.scalar_type(),
+              "keys must be [", query.size(0), " rows, up to 2^20 heads, ", query.size(2),
               "] of the queries' dtype and device, got ", key.sizes());
   for (const auto *w : {&query_weight, &key_weight})
     TORCH_CHECK(!w->defined() || (w->device() == query.device() &&

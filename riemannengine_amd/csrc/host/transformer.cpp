@@ -298,6 +298,10 @@ at::Tensor hip_packed_attention(const at::Tensor &query, const at::Tensor &key,
               key.size(2));
   TORCH_CHECK(key.size(1) > 0 && query.size(1) > 0 && query.size(1) % key.size(1) == 0,
               "query heads ", query.size(1), " must be a multiple of key heads ", key.size(1));
+  TORCH_CHECK(query.size(1) <= INT32_MAX && query.size(2) <= INT32_MAX &&
+                  query_offsets.numel() <= INT32_MAX,
+              "attention takes heads, widths and sequences that fit 32 bits, got ", query.sizes(),
+              " and ", query_offsets.numel(), " offsets");
   hip_dtype(query, "query");
   TORCH_CHECK(key.scalar_type() == query.scalar_type() &&
                   value.scalar_type() == query.scalar_type(),
