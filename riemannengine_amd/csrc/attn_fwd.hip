@@ -191,8 +191,9 @@ attn_fwd_kernel(AttnArgs a) {
   // entry's zero times one would be NaN, so they are zeroed in LDS, and the rows
   // that see them get them at the end.
   bool left_out = false;
-  auto cut = [&](int32_t kt) { // LOCAL: tile kt is such a tile
-    return !wg.all(kt * kBN, min((kt + 1) * kBN, sq.lk));
+  auto cut = [&](int32_t kt) { // tile kt is such a tile
+    return LOCAL ? !wg.all(kt * kBN, min((kt + 1) * kBN, sq.lk))
+                 : wg_full < wg_lim && (kt + 1) * kBN > wg_full;
   };
   if (W > 1 && threadIdx.x == 0)
     any_left_out = 0; // behind the barrier of the first turn
@@ -207,7 +208,7 @@ attn_fwd_kernel(AttnArgs a) {
     wait_stream();
     if constexpr (W > 1)
       __syncthreads();
-    if (LOCAL ? cut(kt) : wg_full < wg_lim && (kt + 1) * kBN > wg_full) {
+    if (cut(kt)) {
       rare_path();
       const bool found = Tile::template zero_not_finite<false, kBN, W == 1 ? 1 : kFwdWaves>(
           stage_at + buf * 2 * Shape::kTileBytes + Shape::kTileBytes, W == 1 ? 0 : w);
@@ -296,19 +297,20 @@ attn_fwd_kernel(AttnArgs a) {
     }
   }
   sum = pair_sum(sum);
-  if (LOCAL) {
-    if (left_out)
+  // each wave those of its own keys: another's, where this one sees none, would be
+  // an infinity times a weight of zero in the joins
+  if (left_out)
 #pragma unroll 1
-      for (int32_t n = kt0; n < kt1; ++n) {
-        const int32_t kt = wg.tile(n);
-        if (cut(kt))
-          Tile::template add_not_finite<false>(
-              vp, a.v_row, a.dim, kt * kBN, min((kt + 1) * kBN, sq.lk),
-              [&](int32_t j) { return (j >= mine.lo && j < mine.hi) || j < mine.first; }, o);
-      }
-  } else if (left_out)
-    Tile::template add_not_finite<false>(vp, a.v_row, a.dim, max(wg_full - kBN, 0), wave_lim,
-                                         [&](int32_t j) { return j < lim; }, o);
+    for (int32_t n = first; n < kt1; n += step) {
+      const int32_t kt = LOCAL ? wg.tile(n) : n, j0 = kt * kBN + 32 * b0;
+      if (cut(kt))
+        Tile::template add_not_finite<false>(
+            vp, a.v_row, a.dim, j0, min(j0 + 32 * kB, sq.lk),
+            [&](int32_t j) {
+              return LOCAL ? (j >= mine.lo && j < mine.hi) || j < mine.first : j < lim;
+            },
+            o);
+    }
 
   if constexpr (W == 4) {
     const float inv = sum == 0.f ? 0.f : 1.f / sum;
