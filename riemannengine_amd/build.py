@@ -56,7 +56,8 @@ def _run(cmd: list[str]) -> None:
 
 
 def build_hip(jobs: int = 8) -> str:
-    """Compile the HIP kernels and link libriemann_hip.so; returns its path."""
+    """Compile the HIP kernels, `jobs` sources at once, and link libriemann_hip.so;
+    returns its path."""
     if not os.path.exists(HIPCC):
         raise RuntimeError(f"hipcc not found at {HIPCC}")
     os.makedirs(BUILD, exist_ok=True)

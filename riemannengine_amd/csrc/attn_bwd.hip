@@ -395,7 +395,7 @@ __device__ __forceinline__ int64_t partial_row(const AttnArgs &a, const AttnSeq 
 // LOCAL: inside a window (LocalRows). The keys of the tiles that hold sinks, which
 // rows of the whole sequence see, are a launch of their own (apart_pass), whose
 // workgroups split those rows; partial sums then lie by sequence. (Four causal
-// texts of up to 4096, 16 over 4 heads of 128, window 1024, 4 sinks: 155 us and 29
+// texts of up to 4096, 16 over 4 heads of 128, window 1024, 4 sinks: 151 to 158 us, 29
 // for the keys apart, joins of 16 and 8; in one launch the sinks' workgroups alone
 // would go through every row.)
 template <typename T, int DP, bool VEC, int W, bool LOCAL>

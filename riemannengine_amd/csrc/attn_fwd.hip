@@ -91,12 +91,13 @@ __device__ void finish_row(const AttnArgs &a, int64_t row, int32_t head, float o
 // softmax, row sums as a product with ones, priorities of waves.
 //
 // LOCAL: inside a window (LocalKeys). A workgroup goes through the tiles of its
-// rows' sinks and windows alone; blocks that all of a wave's rows see whole are
-// not masked. A window of w keys costs the tiles that rows + 2 w (causal: w) keys
+// rows' sinks and windows alone; a wave skips its share of a tile, kB blocks, where
+// none of its rows sees a part of it, and does not mask it where all see all of it.
+// A window of w keys costs the tiles that rows + 2 w (causal: w) keys
 // touch, so narrow windows lose more to the edges: causal, 16 over 4 heads of 128,
-// window 1024: 101 us, 520 TFLOP/s of visible pairs; prompts of up to 16384, 32
-// over 8 heads, window 2048: 1030, 840; both sides, 8 heads of 32, window 256: 27
-// us, 150. The rule for W holds here too (those 27 us at W = 4 are 39 at 2 and 42
+// window 1024: 98 to 104 us, 520 TFLOP/s of visible pairs; prompts of up to 16384,
+// 32 over 8 heads, window 2048: 985 to 1060, 820 to 875; both sides, 8 heads of 32,
+// window 256: 27 us, 150. The rule for W holds here too (those 27 us at W = 4 are 39 at 2 and 42
 // at 1; fp32, 2 key heads of 9903 rows: 41 at each). 32 single tokens, window
 // 1024: 27 us, 4.1 TB/s.
 template <typename T, int DP, bool VEC, int W, bool LOCAL>

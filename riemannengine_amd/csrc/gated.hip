@@ -864,11 +864,16 @@ struct GatedForward {
   float *part;
 };
 // Whether the kernel for few rows takes the forward: up to 64 rows, which it takes
-// at once (4096 channels, 11008 hidden, bf16, 64 rows: 80 us, in tiles 86 at 65),
+// at once (4096 channels, 11008 hidden, bf16, 64 rows: 89 us, in tiles 91 at 65),
 // and up to 256 where reading the weights again for every 64 rows, mostly from the
-// caches, costs less than the tiles' few workgroups and further launches. 128 rows,
-// bf16: 1024 channels, 2816 hidden 22 us, in tiles 27; 2048, 5504 45 and 36; fp32:
-// 512, 1376 19 and 28; 1024, 2816 44 and 42.
+// caches, costs less than the tiles' few workgroups and further launches. 65, 128
+// and 256 rows of so many channels and hidden ones, few rows / tiles, us:
+//   bf16  512, 1376   12/18  13/18  18/18    fp32  20/28  20/28  28/34
+//         1024, 2816  21/27  22/27  29/27          42/42  43/43  56/63
+//         1536, 4096  28/30  29/30  51/35          62/62  64/62  114/103
+//         2048, 5504  47/42  50/43  86/59          99/95  102/96  186/163
+// Between 200 and 400 million products of fp32 the tiles, which then run, are up to
+// a quarter behind (768, 2048, 128 rows: 26/32) or level.
 bool few_rows(const rhip_gated *d) {
   if (d->n <= 64)
     return true;
